@@ -354,6 +354,82 @@ int r4c_ce_bwd(const void* logits, const int64_t* target, int64_t vox, int C, in
                const float* loss_count, const float* grad_loss, void* dlogits, r4c_stream_t stream);
 
 /*
+ * Rows of logits for the two operators below. A row is the class axis at one
+ * voxel of an (N, C, D, H, W) map or at one token of an (R, C) matrix. Row r
+ * starts at (r / inner) * outer_stride + (r % inner) * inner_stride, class c
+ * of it is class_stride elements apart from class c - 1 (all in elements; any
+ * strides, 0 included); grad_* is the same for the logits' gradient, where no
+ * two elements may share a place. Logits bf16, fp16 or fp32; arithmetic and
+ * sums in fp32 or wider. Per-row inputs and outputs are dense, in row order.
+ * No reference counterpart: the reference has no operator on logits.
+ */
+typedef struct r4c_rows_desc {
+  int64_t rows, inner;
+  int64_t outer_stride, inner_stride, class_stride;
+  int64_t grad_outer_stride, grad_inner_stride, grad_class_stride;
+  int32_t classes;
+  int32_t dtype;             /* R4C_BF16, R4C_F16 or R4C_F32 */
+  float temperature;         /* finite, > 0; logits are divided by it */
+} r4c_rows_desc;
+
+#define R4C_TOPK_MAX 128
+
+/*
+ * Log-probability of a given class, entropy, log-sum-exp and the top_k most
+ * probable classes of softmax(z / T), per row.
+ *   logp[r]      = z[r][t] / T - lse[r]; 0 where target[r] == ignore_index (logp and target both null: not wanted)
+ *   entropy[r]   = -sum p ln p,  lse[r] = ln sum exp(z / T)
+ *   top_logp, top_index [rows][top_k]: largest first, equal logits by lowest class (0 <= top_k <= R4C_TOPK_MAX, <= classes)
+ * Rows without a finite logit (all -inf): lse, logp and top_logp -inf, entropy
+ * 0, no gradient. Rows that hold a NaN or +inf have no distribution: every
+ * float is NaN and top_index -1. A class outside [0, C) that is not
+ * ignore_index counts as ignored and sets code 6 in the device error flag.
+ * `stats` (r4c_logp_stats_size(desc) bytes, null allowed when that is 0 or
+ * when no backward follows) carries the rows' maxima and sums to r4c_logp_bwd,
+ * which writes
+ *   dz_c = (1/T) [ p_c (g_lse - g_logp - g_entropy (ln p_c + H)) + g_logp [c = t] ]
+ * in the logits' type. Each upstream gradient may be null (none) and has an
+ * increment per row: 1, or 0 for one value that all rows share.
+ */
+size_t r4c_logp_stats_size(const r4c_rows_desc* desc);
+int r4c_logp_fwd(const r4c_rows_desc* desc, const void* logits, const int64_t* target, int64_t ignore_index,
+                 int top_k, float* logp, float* entropy, float* lse, float* top_logp, int32_t* top_index, void* stats,
+                 r4c_stream_t stream);
+int r4c_logp_bwd(const r4c_rows_desc* desc, const void* logits, const int64_t* target, int64_t ignore_index,
+                 const float* entropy, const void* stats, const float* g_logp, int g_logp_inc, const float* g_entropy,
+                 int g_entropy_inc, const float* g_lse, int g_lse_inc, void* dlogits, r4c_stream_t stream);
+
+/*
+ * Distillation from a teacher's top classes. The teacher of a row is k pairs
+ * (log-probability, class), [rows][k]; the student its logits, p = softmax(z / T).
+ *   rest = 0:  q = the k probabilities renormalised (a constant added to a row's log-probabilities drops out)
+ *   rest = 1:  q as given, and q_r = max(0, 1 - sum q) for all unlisted classes together, against their p_r
+ *   L[r] = T^2 [ sum_j q_j (ln q_j - ln p_j) + q_r (ln q_r - ln p_r) ]
+ * A pair with a negative class or log-probability -inf is void; a class >= C
+ * is void and sets code 6 in the device error flag; a class listed twice
+ * counts with both its q. q_r below 1e-6 is the rounding of the sum and counts
+ * as 0. A row takes no part (weight 0, gradient 0) when all its pairs are
+ * void, its weight is 0 or it has no finite logit. teacher_logp is bf16, fp16
+ * or fp32, teacher_index 32- or 64-bit integers (index_bits), weight (fp32,
+ * >= 0) may be null: 1 for every row.
+ * r4c_distill_fwd writes row_loss[r] = w[r] L[r] (may be null) and
+ * loss_weight[0] = sum(w L) / sum(w), loss_weight[1] = sum(w) (device memory,
+ * 2 floats, may be null; summed in a fixed order in double; NaN when no row
+ * takes part), and `stats` for the backward.
+ * r4c_distill_bwd writes dlogits = grad * w / sum(w) * dL/dz with loss_weight
+ * (of the forward) given, else grad[r * grad_inc] * w * dL/dz.
+ */
+size_t r4c_distill_stats_size(const r4c_rows_desc* desc);
+size_t r4c_distill_workspace_size(const r4c_rows_desc* desc);
+int r4c_distill_fwd(const r4c_rows_desc* desc, const void* logits, int k, const void* teacher_logp, int teacher_dtype,
+                    const void* teacher_index, int index_bits, int rest, const float* weight, float* row_loss,
+                    float* loss_weight, void* stats, void* ws, size_t ws_bytes, r4c_stream_t stream);
+int r4c_distill_bwd(const r4c_rows_desc* desc, const void* logits, int k, const void* teacher_logp, int teacher_dtype,
+                    const void* teacher_index, int index_bits, int rest, const float* weight,
+                    const float* loss_weight, const float* grad, int grad_inc, const void* stats, void* dlogits,
+                    r4c_stream_t stream);
+
+/*
  * Conv3d weight and bias gradient without any allocation. No counterpart in
  * the reference: it exists for callers that cannot allocate device memory,
  * e.g. a plugin or custom op running inside another framework that owns the

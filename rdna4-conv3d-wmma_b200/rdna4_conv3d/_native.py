@@ -47,6 +47,15 @@ class ConvexDesc(ctypes.Structure):
         "pd", "ph", "pw", "dd", "dh", "dw", "dtype")]
 
 
+class RowsDesc(ctypes.Structure):
+    """r4c_rows_desc: rows of logits (include/r4c_conv3d.h)."""
+    _fields_ = [("rows", ctypes.c_int64), ("inner", ctypes.c_int64),
+                ("outer_stride", ctypes.c_int64), ("inner_stride", ctypes.c_int64), ("class_stride", ctypes.c_int64),
+                ("grad_outer_stride", ctypes.c_int64), ("grad_inner_stride", ctypes.c_int64),
+                ("grad_class_stride", ctypes.c_int64),
+                ("classes", ctypes.c_int32), ("dtype", ctypes.c_int32), ("temperature", ctypes.c_float)]
+
+
 class NativeError(RuntimeError):
     """A C-ABI entry point returned a non-zero status."""
 
@@ -59,6 +68,7 @@ def _bind(lib) -> None:
     P = ctypes.c_void_p
     D = ctypes.POINTER(ConvDesc)
     X = ctypes.POINTER(ConvexDesc)
+    R = ctypes.POINTER(RowsDesc)
     sz = ctypes.c_size_t
     i = ctypes.c_int
     i64 = ctypes.c_int64
@@ -97,6 +107,13 @@ def _bind(lib) -> None:
         "r4c_ce_workspace_size": ([i64], sz),
         "r4c_ce_fwd": ([P, P, i64, i, i, i64, P, P, sz, P], i),
         "r4c_ce_bwd": ([P, P, i64, i, i, i64, P, P, P, P], i),
+        "r4c_logp_stats_size": ([R], sz),
+        "r4c_logp_fwd": ([R, P, P, i64, i, P, P, P, P, P, P, P], i),
+        "r4c_logp_bwd": ([R, P, P, i64, P, P, P, i, P, i, P, i, P, P], i),
+        "r4c_distill_stats_size": ([R], sz),
+        "r4c_distill_workspace_size": ([R], sz),
+        "r4c_distill_fwd": ([R, P, i, P, i, P, i, i, P, P, P, P, P, sz, P], i),
+        "r4c_distill_bwd": ([R, P, i, P, i, P, i, i, P, P, P, i, P, P, P], i),
         "r4c_convex_plan": ([X], i),
         "r4c_convex_workspace_size": ([X, i], sz),
         "r4c_convex_fwd": ([X, P, P, P, P, P, sz, P], i),
@@ -580,4 +597,149 @@ def ce_backward(logits_cl: torch.Tensor, target: torch.Tensor, ignore_index: int
         st = lib().r4c_ce_bwd(_ptr(logits_cl), _ptr(target), vox, C, dtype_code(logits_cl.dtype), int(ignore_index),
                               _ptr(loss_count), _ptr(g), _ptr(dz), _stream(dev))
     _check(st, "r4c_ce_bwd")
+    return dz
+
+
+# ---------------------------------------------------------------------------
+# Rows of logits: log-probabilities (r4c_logp_*), distillation (r4c_distill_*)
+# ---------------------------------------------------------------------------
+TOPK_MAX = 128
+_TILE_CLASSES = 32    # rows up to this many classes are read with any class stride
+
+
+def _row_strides(t: torch.Tensor):
+    """(inner, outer stride, inner stride, class stride) of (N, C, ...) logits
+    whose dims after the class walk one stride; None when they do not."""
+    n, c = int(t.shape[0]), int(t.shape[1])
+    st = t.stride()
+    inner, si = 1, 0
+    for size, stride in zip(reversed(t.shape[2:]), reversed(st[2:])):
+        if size == 1:
+            continue
+        if inner == 1:
+            si = stride
+        elif stride != si * inner:
+            return None
+        inner *= int(size)
+    sc = st[1] if c > 1 else 1
+    if inner == 1:                       # rows are the outer dim
+        return max(n, 1), 0, st[0] if n > 1 else c, sc
+    if n == 1 or st[0] == si * inner:    # one stride over everything
+        return n * inner, 0, si, sc
+    return inner, st[0], si, sc
+
+
+def class_last_empty(t: torch.Tensor) -> torch.Tensor:
+    """A new tensor of t's shape whose memory order puts the classes (dim 1) last."""
+    shape = t.shape
+    return torch.empty((shape[0], *shape[2:], shape[1]), dtype=t.dtype, device=t.device).movedim(-1, 1)
+
+
+class Rows:
+    """Logits as the row kernels read them: ``z`` (the logits themselves, or a
+    class-last copy where the kernels cannot walk their strides), their
+    descriptor, and the per-row shape (N, ...)."""
+    __slots__ = ("z", "desc", "shape", "stats")
+
+    def __init__(self, logits: torch.Tensor, temperature: float):
+        z = logits
+        st = _row_strides(z)
+        if st is None or (st[3] != 1 and z.shape[1] > _TILE_CLASSES):
+            z = class_last_empty(logits).copy_(logits)
+            st = _row_strides(z)
+        shape = logits.shape[:1] + logits.shape[2:]
+        inner, so, si, sc = st
+        self.z, self.shape = z, shape
+        self.desc = RowsDesc(shape.numel(), max(inner, 1), so, si, sc, so, si, sc, int(logits.shape[1]),
+                             dtype_code(logits.dtype), temperature)
+
+    def grad_like(self) -> torch.Tensor:
+        """A new tensor for the gradient; sets the descriptor's gradient strides."""
+        z = self.z
+        dz = torch.empty_like(z)
+        if dz.stride() != z.stride():                    # z overlaps or has gaps: a dense class-last gradient
+            dz = class_last_empty(z)
+            inner, so, si, sc = _row_strides(dz)
+            d = self.desc
+            if d.inner != inner:                         # the gradient's rows in the logits' (outer, inner) split
+                so = si * d.inner
+            d.grad_outer_stride, d.grad_inner_stride, d.grad_class_stride = so, si, sc
+        return dz
+
+
+def _grad_inc(g: Optional[torch.Tensor]):
+    """(fp32 tensor, increment per row) of an upstream gradient: one shared value has increment 0."""
+    if g is None:
+        return None, 0
+    if g.numel() > 1 and not any(g.stride()):
+        return g[(0,) * g.dim()].float(), 0
+    return g.float().contiguous(), 1
+
+
+def logp_forward(rows: Rows, target: Optional[torch.Tensor], ignore_index: int, top_k: int, want_stats: bool):
+    """(logp or None, entropy, lse, top_logp or None, top_index or None, stats or None)."""
+    dev = _require_cuda(rows.z, target)
+    L, d, shape = lib(), rows.desc, rows.shape
+    f32 = dict(dtype=torch.float32, device=dev)
+    logp = torch.empty(shape, **f32) if target is not None else None
+    entropy, lse = torch.empty(shape, **f32), torch.empty(shape, **f32)
+    top_logp = torch.empty((*shape, top_k), **f32) if top_k else None
+    top_index = torch.empty((*shape, top_k), dtype=torch.int32, device=dev) if top_k else None
+    stats = None
+    if want_stats:
+        nb = int(L.r4c_logp_stats_size(ctypes.byref(d)))
+        stats = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    with torch.cuda.device(dev):
+        st = L.r4c_logp_fwd(ctypes.byref(d), _ptr(rows.z), _ptr(target), ignore_index, top_k, _ptr(logp),
+                            _ptr(entropy), _ptr(lse), _ptr(top_logp), _ptr(top_index), _ptr(stats), _stream(dev))
+    _check(st, "r4c_logp_fwd")
+    return logp, entropy, lse, top_logp, top_index, stats
+
+
+def logp_backward(rows: Rows, target: Optional[torch.Tensor], ignore_index: int, entropy: torch.Tensor,
+                  stats: Optional[torch.Tensor], g_logp, g_entropy, g_lse) -> torch.Tensor:
+    dev = _require_cuda(rows.z)
+    dz = rows.grad_like()
+    (gl, il), (gh, ih), (gs, is_) = _grad_inc(g_logp), _grad_inc(g_entropy), _grad_inc(g_lse)
+    with torch.cuda.device(dev):
+        st = lib().r4c_logp_bwd(ctypes.byref(rows.desc), _ptr(rows.z), _ptr(target), ignore_index, _ptr(entropy),
+                                _ptr(stats), _ptr(gl), il, _ptr(gh), ih, _ptr(gs), is_, _ptr(dz), _stream(dev))
+    _check(st, "r4c_logp_bwd")
+    return dz
+
+
+def distill_forward(rows: Rows, teacher_logp: torch.Tensor, teacher_index: torch.Tensor, rest: bool,
+                    weight: Optional[torch.Tensor], mean: bool):
+    """(row losses or None, (mean, total weight) or None, stats)."""
+    dev = _require_cuda(rows.z, teacher_logp, teacher_index, weight)
+    L, d = lib(), rows.desc
+    row_loss = None if mean else torch.empty(rows.shape, dtype=torch.float32, device=dev)
+    loss_weight = torch.empty(2, dtype=torch.float32, device=dev) if mean else None
+    nb = int(L.r4c_distill_stats_size(ctypes.byref(d)))
+    stats = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    nb = int(L.r4c_distill_workspace_size(ctypes.byref(d)))
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    with torch.cuda.device(dev):
+        st = L.r4c_distill_fwd(ctypes.byref(d), _ptr(rows.z), int(teacher_logp.shape[-1]), _ptr(teacher_logp),
+                               dtype_code(teacher_logp.dtype), _ptr(teacher_index), 8 * teacher_index.element_size(),
+                               1 if rest else 0, _ptr(weight), _ptr(row_loss), _ptr(loss_weight), _ptr(stats),
+                               _ptr(ws), nb, _stream(dev))
+    _check(st, "r4c_distill_fwd")
+    return row_loss, loss_weight, stats
+
+
+def distill_backward(rows: Rows, teacher_logp: torch.Tensor, teacher_index: torch.Tensor, rest: bool,
+                     weight: Optional[torch.Tensor], loss_weight: Optional[torch.Tensor],
+                     stats: Optional[torch.Tensor], grad: torch.Tensor) -> torch.Tensor:
+    dev = _require_cuda(rows.z)
+    dz = rows.grad_like()
+    g, inc = _grad_inc(grad)
+    if loss_weight is not None:
+        inc = 0
+    with torch.cuda.device(dev):
+        st = lib().r4c_distill_bwd(ctypes.byref(rows.desc), _ptr(rows.z), int(teacher_logp.shape[-1]),
+                                   _ptr(teacher_logp), dtype_code(teacher_logp.dtype), _ptr(teacher_index),
+                                   8 * teacher_index.element_size(), 1 if rest else 0, _ptr(weight),
+                                   _ptr(loss_weight), _ptr(g), inc, _ptr(stats), _ptr(dz), _stream(dev))
+    _check(st, "r4c_distill_bwd")
     return dz

@@ -1,0 +1,144 @@
+"""Log-probabilities of given labels, with entropy and the most probable classes.
+
+``log_probs(logits, target)`` reads (N, C, ...) logits -- the per-voxel maps
+of the UNet, or (R, C) rows of tokens -- once and answers, for every voxel or
+row, how likely the given label is, how unsure the prediction is (entropy),
+the log-sum-exp, and with ``top_k`` the most probable classes with their
+log-probabilities: a confidence map, a scoring pass, or the export of a
+teacher for ``losses.distill_topk``. On a CUDA device it runs on the native
+kernels (r4c_logp_*), forward and backward, for bf16, fp16 and fp32 logits;
+CPU tensors take the same formulas in torch operations (any float type, so
+gradients can be checked in 64 bits). No reference counterpart: the
+reference's models end at their logits (benches/unet_e2e.py:35-38).
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _native
+
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+class LogProbs(NamedTuple):
+    """Per voxel or row, all fp32 (indices int32); shape (N, ...), top_* (N, ..., top_k)."""
+    logp: Optional[torch.Tensor]        # log-probability of the target, 0 where ignored; None without a target
+    entropy: torch.Tensor               # -sum p ln p
+    lse: torch.Tensor                   # ln sum exp(logits / temperature)
+    top_logp: Optional[torch.Tensor]    # largest first; None with top_k = 0
+    top_index: Optional[torch.Tensor]   # their classes, equal logits by lowest class
+
+
+def check_logits(logits: torch.Tensor, temperature: float) -> None:
+    if logits.dim() < 2:
+        raise ValueError(f"logits must be (N, C, ...), got shape {tuple(logits.shape)}")
+    if logits.shape[1] == 0:
+        raise ValueError("logits have no classes")
+    if not logits.is_floating_point() or (logits.is_cuda and logits.dtype not in _FLOATS):
+        raise TypeError(f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    if not (math.isfinite(temperature) and temperature > 0):
+        raise ValueError(f"temperature must be finite and positive, got {temperature}")
+
+
+class LogProbsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, target, top_k, temperature, ignore_index):
+        rows = _native.Rows(logits, temperature)
+        ctx.set_materialize_grads(False)
+        logp, entropy, lse, top_logp, top_index, stats = _native.logp_forward(
+            rows, target, ignore_index, top_k, logits.requires_grad)
+        ctx.save_for_backward(rows.z, target, entropy, stats)
+        ctx.temperature, ctx.ignore_index = temperature, ignore_index
+        ctx.mark_non_differentiable(*(t for t in (top_logp, top_index) if t is not None))
+        return logp, entropy, lse, top_logp, top_index
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_lse, _top_logp, _top_index):
+        z, target, entropy, stats = ctx.saved_tensors
+        dz = _native.logp_backward(_native.Rows(z, ctx.temperature), target, ctx.ignore_index, entropy, stats,
+                                   g_logp, g_entropy, g_lse)
+        return dz, None, None, None, None
+
+
+def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, *, top_k: int = 0,
+              temperature: float = 1.0, ignore_index: int = -100) -> LogProbs:
+    """Log-probabilities under softmax(logits / temperature) over dim 1.
+
+    logits: (N, C, ...); any strides (channels-last is read as it lies).
+    target: integer classes (N, ...), or None. ``ignore_index`` gives
+        log-probability 0 and no gradient; any other class outside [0, C) is
+        an error (on a CUDA device it counts as ignored and sets code 6 in
+        ``_native.device_error()``).
+    top_k: how many of the most probable classes to return, at most 128.
+
+    ``logp``, ``entropy`` and ``lse`` carry gradients to the logits;
+    ``top_logp`` does not. A row without a finite logit has lse, logp and
+    top_logp -inf, entropy 0 and no gradient; one that holds a NaN or +inf has
+    no distribution: its values are NaN and its top_index -1.
+    """
+    check_logits(logits, temperature)
+    shape = logits.shape[:1] + logits.shape[2:]
+    if not 0 <= top_k <= min(_native.TOPK_MAX, logits.shape[1]):
+        raise ValueError(f"top_k must be in [0, min({_native.TOPK_MAX}, C = {logits.shape[1]})], got {top_k}")
+    if target is not None:
+        if target.shape != shape:
+            raise ValueError(f"target must have shape {tuple(shape)}, got {tuple(target.shape)}")
+        if target.is_floating_point() or target.is_complex() or target.dtype == torch.bool:
+            raise TypeError(f"target must hold integers, got {target.dtype}")
+        if target.device != logits.device:
+            raise ValueError(f"target is on {target.device}, logits on {logits.device}")
+    if not logits.is_cuda:
+        return _log_probs_torch(logits, target, top_k, temperature, ignore_index)
+    if target is not None:
+        target = target.to(torch.int64).contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return LogProbs(*LogProbsFn.apply(logits, target, top_k, temperature, ignore_index))
+    return LogProbs(*_native.logp_forward(_native.Rows(logits, temperature), target, ignore_index, top_k, False)[:5])
+
+
+def _log_probs_torch(logits, target, top_k, temperature, ignore_index) -> LogProbs:
+    """The same values in torch operations, at least in fp32."""
+    acc = torch.promote_types(logits.dtype, torch.float32)
+    out = torch.float32 if acc == torch.float32 else acc
+    z = logits.movedim(1, -1).to(acc)
+    c = z.shape[-1]
+    s = z / temperature
+    inf = float("inf")
+    empty = (z == -inf).all(-1, keepdim=True)
+    bad = (z.isnan() | (z == inf)).any(-1, keepdim=True)
+    m = s.detach().amax(-1, keepdim=True)
+    m = torch.where(empty | bad, torch.zeros_like(m), m)
+    d = s - m
+    # masked classes leave the graph: their gradient is 0, not 0 * inf
+    dead = (d == -inf) | bad
+    e = torch.where(dead, torch.zeros_like(d), torch.exp(torch.where(dead, torch.zeros_like(d), d)))
+    total = e.sum(-1, keepdim=True)
+    ln_s = torch.log(torch.where(empty | bad, torch.ones_like(total), total))
+    ln_p = torch.where(d == -inf, torch.full_like(d, -inf), d - ln_s)
+    p = e / torch.where(empty | bad, torch.ones_like(total), total)
+    entropy = -(p * torch.where(dead, torch.zeros_like(d), ln_p)).sum(-1)
+    lse = (m + ln_s).squeeze(-1)
+    lse = torch.where(empty.squeeze(-1), torch.full_like(lse, -inf), lse)
+    nan = torch.full_like(lse, float("nan"))
+    b = bad.squeeze(-1)
+    entropy, lse = torch.where(b, nan, entropy), torch.where(b, nan, lse)
+    logp = None
+    if target is not None:
+        t = target.to(torch.int64)
+        counted = t != ignore_index
+        if bool((((t < 0) | (t >= c)) & counted).any()):
+            raise IndexError(f"target out of range [0, {c})")
+        at = torch.where(counted, t, torch.zeros_like(t)).unsqueeze(-1)
+        logp = torch.where(b, nan, ln_p.gather(-1, at).squeeze(-1))
+        logp = torch.where(counted, logp, torch.zeros_like(logp)).to(out)
+    top_logp = top_index = None
+    if top_k:
+        # a stable descending sort keeps equal logits in class order
+        order = torch.sort(z.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
+        top_logp = torch.where(bad, nan.unsqueeze(-1), ln_p.detach().gather(-1, order)).to(out)
+        top_index = torch.where(bad, torch.full_like(order, -1), order).to(torch.int32)
+    return LogProbs(logp, entropy.to(out), lse.to(out), top_logp, top_index)

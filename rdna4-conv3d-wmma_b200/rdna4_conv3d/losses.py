@@ -1,19 +1,28 @@
-"""Cross-entropy over NDHWC logits on the native kernels (r4c_ce_*).
+"""Losses over logits on the native kernels: cross-entropy (r4c_ce_*) and
+distillation from a teacher's top classes (r4c_distill_*).
 
 ``cross_entropy(logits, target)`` is ``F.cross_entropy(logits, target)``
 (reduction 'mean', no class weights, ``ignore_index``) for channels_last_3d
 bf16/fp16 logits on a CUDA device: one kernel pass forward (per-voxel
 log-sum-exp in fp32, deterministic mean) and one backward, with no fp32
 copy of the logits and no layout change. Other inputs take F.cross_entropy.
-No reference counterpart: the reference's training step computes its loss
+
+``distill_topk(logits, teacher_logp, teacher_index)`` trains a student on
+what ``logprobs.log_probs(teacher_logits, top_k=k)`` gave for a teacher: its
+k most probable classes per voxel or token, as they are stored.
+
+No reference counterparts: the reference's training step computes its loss
 with stock PyTorch (benches/unet_e2e.py:41-52).
 """
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 import torch.nn.functional as F
 
 from . import _native
+from .logprobs import check_logits
 
 
 class CrossEntropyNDHWCFn(torch.autograd.Function):
@@ -45,3 +54,113 @@ def cross_entropy(logits: torch.Tensor, target: torch.Tensor, ignore_index: int 
     if _native_ok(logits, target):
         return CrossEntropyNDHWCFn.apply(logits, target, int(ignore_index))
     return F.cross_entropy(logits, target, ignore_index=ignore_index)
+
+
+class DistillTopKFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_logp, teacher_index, temperature, rest, weight, mean):
+        rows = _native.Rows(logits, temperature)
+        row_loss, loss_weight, stats = _native.distill_forward(rows, teacher_logp, teacher_index, rest, weight, mean)
+        ctx.save_for_backward(rows.z, teacher_logp, teacher_index, weight, loss_weight, stats)
+        ctx.temperature, ctx.rest = temperature, rest
+        return loss_weight[0].clone() if mean else row_loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        z, teacher_logp, teacher_index, weight, loss_weight, stats = ctx.saved_tensors
+        dz = _native.distill_backward(_native.Rows(z, ctx.temperature), teacher_logp, teacher_index, ctx.rest, weight,
+                                      loss_weight, stats, grad)
+        return dz, None, None, None, None, None, None
+
+
+def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index: torch.Tensor, *,
+                 temperature: float = 1.0, rest: bool = False, weight: Optional[torch.Tensor] = None,
+                 reduction: str = "mean") -> torch.Tensor:
+    """T^2 KL(teacher || student) where the teacher is given by its top classes.
+
+    logits: (N, C, ...) of the student, p = softmax(logits / temperature) over dim 1; any strides.
+    teacher_logp, teacher_index: (N, ..., k), the teacher's k log-probabilities
+        (at the same temperature) and their classes, k at most 128. A negative
+        index or a log-probability of -inf marks an unused place. A class that
+        is listed twice counts with both its probabilities.
+    rest: False -- the k probabilities are renormalised (so the teacher's
+        logits / temperature serve as well); True -- they are taken as they
+        are, and what is missing to 1 stands for all other classes together.
+    weight: (N, ...), >= 0: the weight of each voxel or token (0: masked).
+    reduction: 'mean' -- sum(w L) / sum(w), NaN when no row takes part; 'none' -- w L, (N, ...).
+
+    Rows whose places are all unused, whose weight is 0 or whose logits are
+    all -inf take no part: loss 0, no share of the mean, no gradient. The
+    gradient reaches the logits only. An index beyond the classes is an error
+    (on a CUDA device it is unused and sets code 6 in ``_native.device_error()``).
+    """
+    check_logits(logits, temperature)
+    shape = logits.shape[:1] + logits.shape[2:]
+    if reduction not in ("mean", "none"):
+        raise ValueError(f"reduction must be 'mean' or 'none', got {reduction!r}")
+    if teacher_logp.shape != teacher_index.shape or teacher_logp.shape[:-1] != shape:
+        raise ValueError(f"teacher_logp and teacher_index must have shape {tuple(shape)} + (k,), got "
+                         f"{tuple(teacher_logp.shape)} and {tuple(teacher_index.shape)}")
+    k = teacher_logp.shape[-1]
+    if not 1 <= k <= _native.TOPK_MAX:
+        raise ValueError(f"the teacher's classes per row must be in [1, {_native.TOPK_MAX}], got {k}")
+    if not teacher_logp.is_floating_point():
+        raise TypeError(f"teacher_logp must be a floating type, got {teacher_logp.dtype}")
+    if teacher_index.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"teacher_index must be int32 or int64, got {teacher_index.dtype}")
+    if weight is not None and weight.shape != shape:
+        raise ValueError(f"weight must have shape {tuple(shape)}, got {tuple(weight.shape)}")
+    for name, t in (("teacher_logp", teacher_logp), ("teacher_index", teacher_index), ("weight", weight)):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"{name} is on {t.device}, logits on {logits.device}")
+    if not logits.is_cuda:
+        return _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weight, reduction)
+    if teacher_logp.dtype == torch.float64:
+        teacher_logp = teacher_logp.float()
+    if weight is not None:
+        weight = weight.detach().to(torch.float32).contiguous()
+    return DistillTopKFn.apply(logits, teacher_logp.detach().contiguous(), teacher_index.contiguous(), temperature,
+                               rest, weight, reduction == "mean")
+
+
+def _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weight, reduction):
+    """The same loss in torch operations, at least in fp32."""
+    acc = torch.promote_types(logits.dtype, torch.float32)
+    inf = float("inf")
+    z = logits.movedim(1, -1).to(acc)
+    v, i = teacher_logp.detach().to(acc), teacher_index.to(torch.int64)
+    c = z.shape[-1]
+    valid = (i >= 0) & (v != -inf)
+    if bool((valid & (i >= c)).any()):
+        raise IndexError(f"teacher_index out of range [0, {c})")
+    zero = torch.zeros((), dtype=acc, device=z.device)
+    i = torch.where(valid, i, torch.zeros_like(i))
+    w = torch.ones(z.shape[:-1], dtype=acc, device=z.device) if weight is None else weight.detach().to(acc)
+    part = valid.any(-1) & ~(z == -inf).all(-1) & (w != 0)
+    w = torch.where(part, w, zero)
+    z = torch.where(part.unsqueeze(-1), z, zero)
+    s = z / temperature
+    lse = torch.logsumexp(s, -1, keepdim=True)
+    v = torch.where(valid, v, zero - inf)
+    if not rest:
+        v = v - torch.where(part.unsqueeze(-1), torch.logsumexp(v, -1, keepdim=True), zero)
+    q = torch.where(valid, torch.exp(v), zero)
+    ln_p = s.gather(-1, i) - lse
+    some = valid & ~(q == 0)
+    row = torch.where(some, q * (torch.where(some, v, zero) - torch.where(some, ln_p, zero)), zero).sum(-1)
+    if rest:
+        qr = 1.0 - q.sum(-1)
+        qr = torch.where(qr >= 1e-6, qr, zero)
+        seen = torch.zeros(z.shape, dtype=torch.int64, device=z.device).scatter_add(-1, i, valid.long()) > 0
+        alive = ~seen & (s != -inf)
+        any_alive = alive.any(-1)
+        lse_r = torch.logsumexp(torch.where(alive | ~any_alive.unsqueeze(-1), s, zero - inf), -1)
+        lse_r = torch.where(any_alive, lse_r, zero - inf)
+        rest_term = qr * (torch.log(torch.where(qr > 0, qr, zero + 1.0)) - lse_r + lse.squeeze(-1))
+        row = row + torch.where(qr > 0, rest_term, zero)
+    out = torch.float32 if acc == torch.float32 else acc
+    row = torch.where(part, temperature * temperature * w * row, zero)
+    if reduction == "none":
+        return row.to(out)
+    return (row.sum() / w.sum()).to(out)
