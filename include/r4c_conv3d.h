@@ -384,6 +384,7 @@ typedef struct r4c_rows_desc {
  * 0, no gradient. Rows that hold a NaN or +inf have no distribution: every
  * float is NaN and top_index -1. A class outside [0, C) that is not
  * ignore_index counts as ignored and sets code 6 in the device error flag.
+ * Above 1024 classes the classes must be contiguous (class_stride 1).
  * `stats` (r4c_logp_stats_size(desc) bytes, null allowed when that is 0 or
  * when no backward follows) carries the rows' maxima and sums to r4c_logp_bwd,
  * which writes
@@ -412,21 +413,24 @@ int r4c_logp_bwd(const r4c_rows_desc* desc, const void* logits, const int64_t* t
  * void, its weight is 0 or it has no finite logit. teacher_logp is bf16, fp16
  * or fp32, teacher_index 32- or 64-bit integers (index_bits), weight (fp32,
  * >= 0) may be null: 1 for every row.
- * r4c_distill_fwd writes row_loss[r] = w[r] L[r] (may be null) and
- * loss_weight[0] = sum(w L) / sum(w), loss_weight[1] = sum(w) (device memory,
- * 2 floats, may be null; summed in a fixed order in double; NaN when no row
- * takes part), and `stats` for the backward.
- * r4c_distill_bwd writes dlogits = grad * w / sum(w) * dL/dz with loss_weight
- * (of the forward) given, else grad[r * grad_inc] * w * dL/dz.
+ * r4c_distill_fwd writes row_loss[r] = w[r] L[r] (may be null), and
+ * loss[0] = sum(w L) / sum(w) with total_weight[0] = sum(w) (device memory,
+ * both may be null; summed in a fixed order in double; NaN when no row takes
+ * part; `ws` of r4c_distill_workspace_size(desc) bytes is needed for these),
+ * and `stats` for the backward (r4c_distill_stats_size(desc) bytes, null when
+ * that is 0). Above 1024 classes the classes must be contiguous
+ * (class_stride 1), and rest = 1 takes about ten million classes at most.
+ * r4c_distill_bwd writes dlogits = grad[r * grad_inc] * w / sum(w) * dL/dz
+ * with total_weight (of the forward) given, else without the division.
  */
 size_t r4c_distill_stats_size(const r4c_rows_desc* desc);
 size_t r4c_distill_workspace_size(const r4c_rows_desc* desc);
 int r4c_distill_fwd(const r4c_rows_desc* desc, const void* logits, int k, const void* teacher_logp, int teacher_dtype,
                     const void* teacher_index, int index_bits, int rest, const float* weight, float* row_loss,
-                    float* loss_weight, void* stats, void* ws, size_t ws_bytes, r4c_stream_t stream);
+                    float* loss, float* total_weight, void* stats, void* ws, size_t ws_bytes, r4c_stream_t stream);
 int r4c_distill_bwd(const r4c_rows_desc* desc, const void* logits, int k, const void* teacher_logp, int teacher_dtype,
                     const void* teacher_index, int index_bits, int rest, const float* weight,
-                    const float* loss_weight, const float* grad, int grad_inc, const void* stats, void* dlogits,
+                    const float* total_weight, const float* grad, int grad_inc, const void* stats, void* dlogits,
                     r4c_stream_t stream);
 
 /*

@@ -19,9 +19,7 @@ namespace distill {
 
 using namespace rows;
 
-constexpr int kThreads = 256;
-
-struct Stats {           // per row, written by the forward for the backward
+struct Stats {           // per streamed row, written by the forward for the backward
   float m, ln_s;         // lse = m / T + ln_s (m a logit, not yet scaled)
   float mr, ln_sr;       // the same over the unlisted classes
   float q_norm;          // ln q_j = v_j - q_norm
@@ -29,20 +27,23 @@ struct Stats {           // per row, written by the forward for the backward
   float w;               // the row's weight, 0: takes no part
 };
 
+constexpr int kParts = kSMs * 16;   // most blocks of a forward: each leaves one partial sum
+
 struct Args {
   const void* z;
   View v, dv;
+  Tile tile;
   int64_t nrows;
-  int C, K, rest;
+  int C, K, rest, segs;
   float temp, inv_t;
   const void* t_logp;
   const void* t_index;
   int t_dtype, t_wide;
   const float* weight;
-  float* row_loss;       // forward: w L
-  float* row_w;          // forward: w of a row that takes part
+  float* row_loss;       // forward: w L per row, or null
+  double* part;          // forward: (sum w L, sum w) of each block, or null
   Stats* stats;
-  const float* loss_weight;
+  const float* total_weight;
   const float* grad;
   int grad_inc;
   void* dz;
@@ -50,13 +51,14 @@ struct Args {
 };
 
 __device__ __forceinline__ float teacher_logp(const Args& a, int64_t i) {
-  if (a.t_dtype == R4C_F32) return static_cast<const float*>(a.t_logp)[i];
+  if (a.t_dtype == R4C_F32) return __ldg(static_cast<const float*>(a.t_logp) + i);
   if (a.t_dtype == R4C_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(a.t_logp)[i]);
   return __half2float(static_cast<const __half*>(a.t_logp)[i]);
 }
 // The pair's class, -1 when the pair is void.
 __device__ __forceinline__ int teacher_class(const Args& a, int64_t i, float v) {
-  const int64_t c = a.t_wide ? static_cast<const int64_t*>(a.t_index)[i] : static_cast<const int32_t*>(a.t_index)[i];
+  const int64_t c = a.t_wide ? __ldg(static_cast<const long long*>(a.t_index) + i)
+                             : (int64_t)__ldg(static_cast<const int32_t*>(a.t_index) + i);
   if (c < 0 || v == -INFINITY) return -1;
   if (c >= a.C) {
     atomicExch(a.err, 6);
@@ -64,108 +66,416 @@ __device__ __forceinline__ int teacher_class(const Args& a, int64_t i, float v) 
   }
   return (int)c;
 }
-
-// One warp per row, any strides.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(Args a) {
-  __shared__ int sh_idx[kThreads / 32][R4C_TOPK_MAX];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + warp;
-  if (r >= a.nrows) return;
-  const T* z = static_cast<const T*>(a.z) + a.v.base(r);
-  const float k2 = a.inv_t * kLog2e;
-  float w = a.weight ? a.weight[r] : 1.f;
-  float qm = -INFINITY;
-  for (int j = lane; j < a.K; j += 32) {
-    const float v = teacher_logp(a, r * a.K + j);
-    const int c = teacher_class(a, r * a.K + j, v);
-    sh_idx[warp][j] = c;
-    if (c >= 0) qm = fmaxf(qm, v);
+__device__ __forceinline__ float grad_scale(const Args& a, int64_t r, float w) {
+  return a.temp * w * a.grad[r * a.grad_inc] / (a.total_weight ? a.total_weight[0] : 1.f);
+}
+// A block's (sum of losses, sum of weights), in a fixed order.
+template <int NT>
+__device__ __forceinline__ void leave_part(double loss, double w, double* part) {
+  __shared__ double sh[2][NT / 32];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    loss += __shfl_xor_sync(0xffffffffu, loss, o);
+    w += __shfl_xor_sync(0xffffffffu, w, o);
   }
-  __syncwarp();
-  const bool any = __any_sync(0xffffffffu, [&] {
-    bool x = false;
-    for (int j = lane; j < a.K; j += 32) x |= sh_idx[warp][j] >= 0;
-    return x;
-  }());
-  qm = warp_max(qm);
-  if (!any) w = 0.f;
-  Stats st{};
-  float loss = 0.f;
-  if (w != 0.f) {
-    auto listed = [&](int c) {
-      for (int j = 0; j < a.K; ++j)
-        if (sh_idx[warp][j] == c) return true;
-      return false;
-    };
-    float m = -INFINITY, mr = -INFINITY;
-    for (int c = lane; c < a.C; c += 32) {
-      const float x = Elem<T>::to_f(z[c * a.v.sc]);
-      m = fmaxf(m, x);
-      if (a.rest && x > mr && !listed(c)) mr = x;
-    }
-    m = warp_max(m);
-    mr = warp_max(mr);
-    const float mm = m == -INFINITY ? 0.f : m, mmr = mr == -INFINITY ? 0.f : mr;
-    float s = 0.f, sr = 0.f;
-    for (int c = lane; c < a.C; c += 32) {
-      const float x = Elem<T>::to_f(z[c * a.v.sc]);
-      s += ex2((x - mm) * k2);
-      if (a.rest && !listed(c)) sr += ex2((x - mmr) * k2);
-    }
-    s = warp_sum(s);
-    sr = warp_sum(sr);
-    if (s == 0.f) w = 0.f;   // no finite logit
-    st.m = mm;
-    st.ln_s = logf(s);
-    st.mr = mmr;
-    st.ln_sr = logf(sr);
-    st.q_norm = 0.f;
-    if (!a.rest) {
-      float qs = 0.f;
-      for (int j = lane; j < a.K; j += 32)
-        if (sh_idx[warp][j] >= 0) qs += expf(teacher_logp(a, r * a.K + j) - qm);
-      st.q_norm = qm + logf(warp_sum(qs));
-    }
-    float sum_q = 0.f;
-    for (int j = lane; j < a.K; j += 32) {
-      const int c = sh_idx[warp][j];
-      if (c < 0) continue;
-      const float ln_q = teacher_logp(a, r * a.K + j) - st.q_norm, q = expf(ln_q);
-      sum_q += q;
-      if (!(q == 0.f)) loss += q * (ln_q - ((Elem<T>::to_f(z[c * a.v.sc]) - mm) * a.inv_t - st.ln_s));
-    }
-    sum_q = warp_sum(sum_q);
-    loss = warp_sum(loss);
-    if (a.rest) {
-      const float qr = 1.f - sum_q;
-      st.q_rest = qr >= kRestNoise ? qr : 0.f;
-      if (st.q_rest > 0.f)
-        loss += st.q_rest * (logf(st.q_rest) - ((mmr - mm) * a.inv_t + (st.ln_sr - st.ln_s)));
-    }
-    st.mass = sum_q + st.q_rest;
-    loss *= a.temp * a.temp;
+  if ((threadIdx.x & 31) == 0) {
+    sh[0][threadIdx.x >> 5] = loss;
+    sh[1][threadIdx.x >> 5] = w;
   }
-  st.w = w;
-  if (lane == 0) {
-    a.row_loss[r] = w == 0.f ? 0.f : w * loss;
-    if (a.row_w) a.row_w[r] = w;
-    a.stats[r] = st;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < NT / 32; ++i) {
+      loss += sh[0][i];
+      w += sh[1][i];
+    }
+    part[2 * blockIdx.x] = loss;
+    part[2 * blockIdx.x + 1] = w;
   }
 }
 
-// loss_weight = (sum of row losses / sum of weights, sum of weights), summed in a fixed order in double.
-__global__ void __launch_bounds__(1024) mean_kernel(const float* loss, const float* w, int64_t n, float* loss_weight) {
-  __shared__ double sh[2][1024];
-  double s = 0.0, t = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    s += loss[i];
-    t += w[i];
+// The terms of a row that come from its sums: r over the unlisted classes
+// (rest) or all of them, l over the listed ones (rest).
+struct RowSums {
+  float m, ln_s, mr, ln_sr;
+  bool empty;
+  __device__ __forceinline__ RowSums(const Run& r, const Run& l, bool rest, float k) {
+    const Run all = rest ? run_merge(r, l, k) : r;
+    empty = all.s == 0.f;
+    m = anchor(all.m);
+    ln_s = logf(all.s);
+    mr = anchor(r.m);
+    ln_sr = logf(r.s);
+  }
+};
+// q_r from the sum of the listed q.
+__device__ __forceinline__ float rest_mass(float sum_q) {
+  const float qr = 1.f - sum_q;
+  return qr >= kRestNoise ? qr : 0.f;
+}
+__device__ __forceinline__ float rest_loss(float qr, const RowSums& s, float inv_t) {
+  return qr > 0.f ? qr * (logf(qr) - ((s.mr - s.m) * inv_t + (s.ln_sr - s.ln_s))) : 0.f;
+}
+// The factor of exp(s_c - lse_r) in an unlisted class's gradient.
+__device__ __forceinline__ float rest_coef(float mass, float qr, float mr, float ln_sr, float m, float ln_s, float inv_t) {
+  return mass * ex2(((mr - m) * inv_t + (ln_sr - ln_s)) * kLog2e) - qr;
+}
+
+// ---- rows in registers -------------------------------------------------------
+template <typename T, int G, int E, bool BWD>
+__global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
+  const float k = a.inv_t * kLog2e;
+  double sum_loss = 0.0, sum_w = 0.0;
+  tile_walk<T, G, BWD>(a.tile, a.z, a.v, a.dz, [&](int64_t r, T* row, bool in) {
+    const bool staged = a.tile.staged;
+    const int64_t sc = staged ? 1 : a.v.sc;
+    TileRow<T, G, E> x;
+    x.load(row, a.v.sc, a.C, staged);
+    float w = a.weight ? a.weight[r] : 1.f;
+    // which of this lane's values the teacher lists
+    uint32_t listed = 0;
+    float qm = -INFINITY;
+    bool any = false, twice = false;
+    for (int j = 0; j < a.K; ++j) {
+      const float v = teacher_logp(a, r * a.K + j);
+      const int c = teacher_class(a, r * a.K + j, v);
+      int e;
+      if (c < 0) continue;
+      any = true;
+      qm = fmaxf(qm, v);
+      if (x.owns(c, &e)) {
+        twice |= listed >> e & 1;
+        listed |= 1u << e;
+      }
+    }
+    if (!any) w = 0.f;
+    if (G > 1) twice = group_any<G>(twice);
+    // sums over the unlisted classes, with a maximum of their own, and over the listed ones
+    Run u = run_empty(), l = run_empty();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (a.rest && (listed >> e & 1)) l.m = fmaxf(l.m, x.v[e]);
+      else u.m = fmaxf(u.m, x.v[e]);
+    }
+    u.m = group_max<G>(u.m);
+    if (a.rest) l.m = group_max<G>(l.m);
+    const float um = anchor(u.m), lm = anchor(l.m);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool at = a.rest && (listed >> e & 1);
+      const float p = ex2((x.v[e] - (at ? lm : um)) * k);
+      if (at) l.s += p;
+      else u.s += p;
+    }
+    u.s = group_sum<G>(u.s);
+    if (a.rest) l.s = group_sum<G>(l.s);
+    const RowSums s(u, l, a.rest, k);
+    if (s.empty) w = 0.f;
+    float q_norm = 0.f;
+    if (!a.rest) {
+      float qs = 0.f;
+      for (int j = x.lane; j < a.K; j += G) {
+        const float v = teacher_logp(a, r * a.K + j);
+        if (teacher_class(a, r * a.K + j, v) >= 0) qs += expf(v - qm);
+      }
+      q_norm = qm + logf(group_sum<G>(qs));
+    }
+    // the pairs, one a lane
+    float sum_q = 0.f, loss = 0.f;
+    if (!BWD || a.rest) {
+      for (int j = x.lane; j < a.K; j += G) {
+        const float v = teacher_logp(a, r * a.K + j);
+        const int c = teacher_class(a, r * a.K + j, v);
+        if (c < 0) continue;
+        const float ln_q = v - q_norm, q = expf(ln_q);
+        sum_q += q;
+        if (!BWD && !(q == 0.f)) loss += q * (ln_q - ((Elem<T>::to_f(row[c * sc]) - s.m) * a.inv_t - s.ln_s));
+      }
+      sum_q = group_sum<G>(sum_q);
+    }
+    const float qr = a.rest ? rest_mass(sum_q) : 0.f;
+    if (!BWD) {
+      loss = group_sum<G>(loss) + rest_loss(qr, s, a.inv_t);
+      if (in && x.lane == 0) {
+        loss = w == 0.f ? 0.f : w * a.temp * a.temp * loss;
+        if (a.row_loss) a.row_loss[r] = loss;
+        sum_loss += loss;
+        sum_w += w;
+      }
+    } else {
+      const float scale = w == 0.f ? 0.f : grad_scale(a, r, w), mass = a.rest ? sum_q + qr : 1.f;
+      const float coef = a.rest ? rest_coef(mass, qr, s.mr, s.ln_sr, s.m, s.ln_s, a.inv_t) : mass;
+      T* out = staged ? row : static_cast<T*>(a.dz) + a.dv.base(r);
+      float g[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float p = coef * ex2(((x.v[e] - s.mr) * a.inv_t - s.ln_sr) * kLog2e);
+        // masked classes of a row whose unlisted classes are all masked: 0, not 0 * inf
+        g[e] = w == 0.f || x.v[e] == -INFINITY ? 0.f : scale * p;
+      }
+      // the listed classes keep their logits until the lanes of the pairs have read them
+      if (in) x.store(out, a.dv.sc, staged, g, w == 0.f ? x.live : x.live & ~listed);
+      if (in && w != 0.f) {
+        for (int j = x.lane; j < a.K; j += G) {
+          const float v = teacher_logp(a, r * a.K + j);
+          const int c = teacher_class(a, r * a.K + j, v);
+          if (c < 0) continue;
+          float q = expf(v - q_norm);
+          if (twice) {   // a class listed again: its first pair writes, with all its q
+            bool first = true;
+            q = 0.f;
+            for (int i = 0; i < a.K; ++i) {
+              const float vi = teacher_logp(a, r * a.K + i);
+              if (teacher_class(a, r * a.K + i, vi) != c) continue;
+              if (i < j) first = false;
+              q += expf(vi - q_norm);
+            }
+            if (!first) continue;
+          }
+          const float p = ex2(((Elem<T>::to_f(row[c * sc]) - s.m) * a.inv_t - s.ln_s) * kLog2e);
+          out[c * (staged ? 1 : a.dv.sc)] = Elem<T>::from_f(scale * (mass * p - q));
+        }
+      }
+    }
+  });
+  if (!BWD && a.part) leave_part<kTileThreads>(sum_loss, sum_w, a.part);
+}
+
+// ---- rows streamed -----------------------------------------------------------
+// One block (or cluster) per row. The listed classes are marked by a bit each
+// (a byte per vector) in shared memory, so that the streaming loop leaves
+// them out at the price of one byte load per vector; their own sum comes from
+// the K pairs.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
+  constexpr int VE = Vec<T>::kElems, U = 4;
+  extern __shared__ __align__(16) uint8_t marks[];
+  __shared__ Run runs[NT / 32];
+  __shared__ Run mine;
+  __shared__ int idx[R4C_TOPK_MAX];
+  __shared__ float lq[R4C_TOPK_MAX];
+  const int tid = threadIdx.x;
+  uint32_t cs = 1, cr = 0;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cs));
+  if (cs > 1) cr = cluster_rank();
+  const float k = a.inv_t * kLog2e;
+  double sum_loss = 0.0, sum_w = 0.0;
+  if (a.rest) {
+    const int bytes = ((a.C + 2 * VE) / VE + (int)cs) / (int)cs + 8;
+    for (int i = tid; i < bytes / 4 + 1; i += NT) reinterpret_cast<uint32_t*>(marks)[i] = 0;
+  }
+  __syncthreads();
+  for (int64_t r = blockIdx.x / cs; r < a.nrows; r += gridDim.x / cs) {
+    const VecRow<T> x(static_cast<const T*>(a.z) + a.v.base(r), a.C);
+    const int per = (x.nv + (int)cs - 1) / (int)cs;
+    const int v0 = min((int)cr * per, x.nv), v1 = min(v0 + per, x.nv);
+    const int f0 = max(v0, x.first_full()), f1 = min(v1, x.end_full());
+    float w = a.weight ? a.weight[r] : 1.f;
+    // the pairs; each class's first pair stands for it in the sums
+    int c = -1;
+    float v = 0.f;
+    if (tid < a.K) {
+      v = teacher_logp(a, r * a.K + tid);
+      c = teacher_class(a, r * a.K + tid, v);
+      idx[tid] = c;
+      lq[tid] = v;
+    }
+    const bool any = __syncthreads_or(c >= 0);
+    if (!any || w == 0.f) {   // the same for all blocks of the cluster
+      if (cr == 0 && tid == 0) {
+        if (a.row_loss) a.row_loss[r] = 0.f;
+        a.stats[r].w = 0.f;
+      }
+      __syncthreads();
+      continue;
+    }
+    float zc = -INFINITY;
+    bool first = c >= 0;
+    int mark = -1;
+    if (c >= 0) {
+      zc = Elem<T>::to_f(x.row[c]);
+      for (int i = 0; i < tid; ++i)
+        if (idx[i] == c) first = false;
+      if (a.rest) {
+        const int vec = (c + x.off) / VE;
+        if (vec >= v0 && vec < v1) {
+          mark = (vec - v0) * 8 + (c + x.off) % VE;
+          atomicOr(reinterpret_cast<uint32_t*>(marks) + (mark >> 5), 1u << (mark & 31));
+        }
+      }
+    }
+    __syncthreads();
+    Run run = run_empty();
+    for (int q = f0 + tid; q < f1; q += U * NT) {
+      uint4 y4[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (q + i * NT < f1) y4[i] = __ldg(x.p + q + i * NT);
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (q + i * NT < f1) {
+          float y[VE];
+          Vec<T>::split(y4[i], y);
+          if (a.rest) {
+            const uint32_t b = marks[q + i * NT - v0];
+            if (b) {
+#pragma unroll
+              for (int j = 0; j < VE; ++j)
+                if (b >> j & 1) y[j] = -INFINITY;
+            }
+          }
+          run_add<VE, false>(run, y, k);
+        }
+      }
+    }
+    auto edge = [&](int vec, int j) {   // one element of a partial vector
+      const int e = x.cls(vec) + j;
+      float y = e >= 0 && e < a.C ? Elem<T>::to_f(x.row[e]) : -INFINITY;
+      if (a.rest && (marks[vec - v0] >> j & 1)) y = -INFINITY;
+      run_add<1, false>(run, &y, k);
+    };
+    if (f0 > v0 && tid < VE) edge(v0, tid);
+    if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) edge(f1, tid - 32);
+    run = run_block<NT>(run, k, runs);
+    if (mark >= 0) reinterpret_cast<uint32_t*>(marks)[mark >> 5] = 0;
+    if (cs > 1) {
+      if (tid == 0) mine = run;
+      cluster_sync();
+      if (cr == 0)
+        for (uint32_t q = 1; q < cs; ++q) run = run_merge(run, cluster_ld_run(&mine, q), k);
+    }
+    if (cr == 0) {
+      __syncthreads();   // runs is free again
+      Run l{first ? zc : -INFINITY, first && zc != -INFINITY ? 1.f : 0.f, 0.f};
+      if (isnan(zc)) l = {0.f, zc, 0.f};
+      if (a.rest) l = run_block<NT>(l, k, runs);
+      const RowSums s(run, l, a.rest, k);
+      // renormalised: ln sum exp(v) of the pairs, by the same joining
+      float q_norm = 0.f;
+      if (!a.rest) {
+        const Run q = run_block<NT>(Run{c >= 0 ? v : -INFINITY, c >= 0 ? 1.f : 0.f, 0.f}, kLog2e, runs);
+        q_norm = q.m + logf(q.s);
+      }
+      float q = 0.f, loss = 0.f;
+      if (c >= 0) {
+        const float ln_q = v - q_norm;
+        q = expf(ln_q);
+        if (!(q == 0.f)) loss = q * (ln_q - ((zc - s.m) * a.inv_t - s.ln_s));
+      }
+      __syncthreads();
+      // (the sums of K <= 128 numbers: the first four warps hold them)
+      q = group_sum<32>(q);
+      loss = group_sum<32>(loss);
+      if ((tid & 31) == 0) runs[tid >> 5] = {q, loss, 0.f};
+      __syncthreads();
+      if (tid == 0) {
+        float sum_q = 0.f;
+        loss = 0.f;
+        for (int i = 0; i < 4; ++i) {
+          sum_q += runs[i].m;
+          loss += runs[i].s;
+        }
+        const float qr = a.rest ? rest_mass(sum_q) : 0.f;
+        if (s.empty) w = 0.f;
+        loss = w == 0.f ? 0.f : w * a.temp * a.temp * (loss + rest_loss(qr, s, a.inv_t));
+        if (a.row_loss) a.row_loss[r] = loss;
+        sum_loss += loss;
+        sum_w += w;
+        a.stats[r] = {s.m, s.ln_s, s.mr, s.ln_sr, q_norm, a.rest ? sum_q + qr : 1.f, qr, w};
+      }
+    }
+    if (cs > 1) cluster_sync();
+    else __syncthreads();
+  }
+  if (a.part) leave_part<NT>(sum_loss, sum_w, a.part);
+}
+
+// One block per piece of a row; the listed classes are written over at the end.
+constexpr int kBwdThreads = 256, kBwdVecs = 4;
+template <typename T>
+__global__ void __launch_bounds__(kBwdThreads) bwd_block_kernel(Args a) {
+  constexpr int VE = Vec<T>::kElems;
+  __shared__ int idx[R4C_TOPK_MAX];
+  __shared__ float lq[R4C_TOPK_MAX];
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x / a.segs;
+  const int seg = blockIdx.x % a.segs;
+  const VecRow<T> x(static_cast<const T*>(a.z) + a.v.base(r), a.C);
+  const VecRow<T> y(static_cast<T*>(a.dz) + a.dv.base(r), a.C);
+  uint4* out = const_cast<uint4*>(y.p);
+  T* out_row = const_cast<T*>(y.row);
+  const bool same = x.off == y.off;   // both rows break into vectors at the same classes
+  const int v0 = seg * kBwdThreads * kBwdVecs, v1 = min(v0 + kBwdThreads * kBwdVecs, x.nv);
+  uint4 z4[kBwdVecs];
+#pragma unroll
+  for (int i = 0; i < kBwdVecs; ++i) {
+    const int v = v0 + tid + i * kBwdThreads;
+    if (v < v1 && v >= x.first_full() && v < x.end_full()) z4[i] = __ldg(x.p + v);
+  }
+  const Stats st = a.stats[r];
+  const bool part = st.w != 0.f;
+  int c = -1;
+  if (part && tid < a.K) {
+    const float v = teacher_logp(a, r * a.K + tid);
+    c = teacher_class(a, r * a.K + tid, v);
+    idx[tid] = c;
+    lq[tid] = v - st.q_norm;
+  }
+  const float scale = part ? grad_scale(a, r, st.w) : 0.f;
+  const float base = a.rest ? st.mr : st.m, ln_b = a.rest ? st.ln_sr : st.ln_s;
+  const float coef = scale * (a.rest ? rest_coef(st.mass, st.q_rest, st.mr, st.ln_sr, st.m, st.ln_s, a.inv_t) : st.mass);
+  auto grad = [&](float z) {
+    const float g = coef * ex2(((z - base) * a.inv_t - ln_b) * kLog2e);
+    return !part || z == -INFINITY ? 0.f : g;
+  };
+#pragma unroll
+  for (int i = 0; i < kBwdVecs; ++i) {
+    const int v = v0 + tid + i * kBwdThreads;
+    if (v >= v1) continue;
+    const int c0 = x.cls(v);
+    if (v >= x.first_full() && v < x.end_full()) {
+      float g[VE];
+      Vec<T>::split(z4[i], g);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) g[j] = grad(g[j]);
+      if (same) out[v] = Vec<T>::join(g);
+      else
+        for (int j = 0; j < VE; ++j) out_row[c0 + j] = Elem<T>::from_f(g[j]);
+    } else {
+      for (int j = 0; j < VE; ++j)
+        if (c0 + j >= 0 && c0 + j < a.C) out_row[c0 + j] = Elem<T>::from_f(grad(Elem<T>::to_f(x.row[c0 + j])));
+    }
+  }
+  if (!part) return;
+  __syncthreads();   // the block's own stores come before these
+  if (c >= 0) {
+    const int vec = (c + x.off) / VE;
+    if (vec >= v0 && vec < v1) {
+      float q = 0.f;
+      bool first = true;
+      for (int i = 0; i < a.K; ++i) {
+        if (idx[i] != c) continue;
+        if (i < tid) first = false;
+        q += expf(lq[i]);
+      }
+      const float p = ex2(((Elem<T>::to_f(x.row[c]) - st.m) * a.inv_t - st.ln_s) * kLog2e);
+      if (first) out_row[c] = Elem<T>::from_f(scale * (st.mass * p - q));
+    }
+  }
+}
+
+// loss = sum w L / sum w, total_weight = sum w: the blocks' partial sums in a fixed order.
+constexpr int kMeanThreads = 256;
+__global__ void __launch_bounds__(kMeanThreads) mean_kernel(const double* part, int n, float* loss, float* total_weight) {
+  __shared__ double sh[2][kMeanThreads];
+  double s = 0.0, w = 0.0;
+  for (int i = threadIdx.x; i < n; i += kMeanThreads) {
+    s += part[2 * i];
+    w += part[2 * i + 1];
   }
   sh[0][threadIdx.x] = s;
-  sh[1][threadIdx.x] = t;
+  sh[1][threadIdx.x] = w;
   __syncthreads();
-  for (int off = 512; off > 0; off >>= 1) {
+  for (int off = kMeanThreads / 2; off > 0; off >>= 1) {
     if ((int)threadIdx.x < off) {
       sh[0][threadIdx.x] += sh[0][threadIdx.x + off];
       sh[1][threadIdx.x] += sh[1][threadIdx.x + off];
@@ -173,45 +483,61 @@ __global__ void __launch_bounds__(1024) mean_kernel(const float* loss, const flo
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    loss_weight[0] = (float)(sh[0][0] / sh[1][0]);   // no row takes part: NaN
-    loss_weight[1] = (float)sh[1][0];
+    loss[0] = (float)(sh[0][0] / sh[1][0]);   // no row takes part: NaN
+    total_weight[0] = (float)sh[1][0];
   }
 }
 
+// ---- launches ----------------------------------------------------------------
+template <typename T, bool BWD>
+cudaError_t launch_tiles(Args& a, int* blocks, cudaStream_t s) {
+  const TileKind kind = tile_kind(a.C);
+  r4c_rows_desc d{};
+  d.rows = a.nrows;
+  d.classes = a.C;
+  const bool dense = dense_rows(a.v, a.nrows, a.C, a.z) && (!BWD || dense_rows(a.dv, a.nrows, a.C, a.dz));
+  a.tile = make_tile(&d, sizeof(T), kind.g, dense);
+  *blocks = tile_grid(a.tile, kTileThreads / kind.g);
+#define R4C_TILE(G, E) \
+  if (kind.g == G && kind.e == E) return launch_tile(tile_kernel<T, G, E, BWD>, a.tile, kTileThreads / G, s, a);
+  R4C_TILE(1, 4) R4C_TILE(1, 8) R4C_TILE(1, 16) R4C_TILE(1, 32) R4C_TILE(4, 16) R4C_TILE(8, 16) R4C_TILE(16, 16)
+  R4C_TILE(32, 16) R4C_TILE(32, 32)
+#undef R4C_TILE
+  return cudaErrorInvalidValue;
+}
+
+// Shared memory for the marks of a block's share of the vectors.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) bwd_kernel(Args a) {
-  __shared__ int sh_idx[kThreads / 32][R4C_TOPK_MAX];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + warp;
-  if (r >= a.nrows) return;
-  const T* z = static_cast<const T*>(a.z) + a.v.base(r);
-  T* dz = static_cast<T*>(a.dz) + a.dv.base(r);
-  const Stats st = a.stats[r];
-  if (st.w == 0.f) {
-    for (int c = lane; c < a.C; c += 32) dz[c * a.dv.sc] = Elem<T>::from_f(0.f);
-    return;
-  }
-  for (int j = lane; j < a.K; j += 32)
-    sh_idx[warp][j] = teacher_class(a, r * a.K + j, teacher_logp(a, r * a.K + j));
-  __syncwarp();
-  const float scale = a.temp * st.w * a.grad[r * a.grad_inc] / (a.loss_weight ? a.loss_weight[1] : 1.f);
-  const float base = a.rest ? st.mr : st.m, ln_b = a.rest ? st.ln_sr : st.ln_s;
-  const float p_r = expf((st.mr - st.m) * a.inv_t + (st.ln_sr - st.ln_s));
-  const float coef = a.rest ? st.mass * p_r - st.q_rest : st.mass;
-  for (int c = lane; c < a.C; c += 32) {
-    const float x = Elem<T>::to_f(z[c * a.v.sc]);
-    float q = 0.f;
-    bool listed = false;
-    for (int j = 0; j < a.K; ++j)
-      if (sh_idx[warp][j] == c) {
-        listed = true;
-        q += expf(teacher_logp(a, r * a.K + j) - st.q_norm);
-      }
-    float g;
-    if (listed) g = st.mass * ex2(((x - st.m) * a.inv_t - st.ln_s) * kLog2e) - q;
-    else g = x == -INFINITY ? 0.f : coef * ex2(((x - base) * a.inv_t - ln_b) * kLog2e);
-    dz[c * a.dv.sc] = Elem<T>::from_f(scale * g);
-  }
+size_t mark_bytes(int C, int cs) {
+  return (size_t)((C + 2 * Vec<T>::kElems) / Vec<T>::kElems + cs) / cs + 16;
+}
+constexpr size_t kMostMarks = 160 << 10;
+
+template <typename T, int NT>
+cudaError_t launch_fwd_block(const Args& a, int* blocks, cudaStream_t s) {
+  int cs = cluster_size(a.nrows, a.C, sizeof(T), NT);
+  while (a.rest && cs < 16 && mark_bytes<T>(a.C, cs) > kMostMarks) cs *= 2;
+  const int64_t most = (int64_t)kSMs * (2048 / NT) / cs * cs;
+  int64_t grid = a.nrows * cs;
+  if (grid > most) grid = most;
+  *blocks = (int)grid;
+  return launch_cluster(fwd_block_kernel<T, NT>, grid, NT, cs, a.rest ? mark_bytes<T>(a.C, cs) : 0, s, a);
+}
+
+template <typename T>
+cudaError_t launch_fwd(Args& a, int* blocks, cudaStream_t s) {
+  if (a.C <= kTileClasses) return launch_tiles<T, false>(a, blocks, s);
+  if ((int64_t)a.C * sizeof(T) <= 16 << 10) return launch_fwd_block<T, 128>(a, blocks, s);
+  return launch_fwd_block<T, 512>(a, blocks, s);
+}
+template <typename T>
+cudaError_t launch_bwd(Args& a, cudaStream_t s) {
+  int blocks;
+  if (a.C <= kTileClasses) return launch_tiles<T, true>(a, &blocks, s);
+  a.segs = (a.C / Vec<T>::kElems + 2 + kBwdThreads * kBwdVecs - 1) / (kBwdThreads * kBwdVecs);
+  if (a.nrows * a.segs > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  bwd_block_kernel<T><<<(unsigned)(a.nrows * a.segs), kBwdThreads, 0, s>>>(a);
+  return cudaGetLastError();
 }
 
 }  // namespace distill
@@ -220,19 +546,22 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(Args a) {
 using namespace r4c;
 
 namespace {
-int check(const r4c_rows_desc* d, int k, const void* t_logp, int t_dtype, const void* t_index, int index_bits) {
+int check(const r4c_rows_desc* d, int k, const void* t_logp, int t_dtype, const void* t_index, int index_bits, int rest) {
   if (!rows::valid_desc(d) || k <= 0 || (index_bits != 32 && index_bits != 64)) return R4C_ERR_INVALID;
   if (d->rows > 0 && (!t_logp || !t_index)) return R4C_ERR_INVALID;
   if (!rows::valid_dtype(d->dtype) || !rows::valid_dtype(t_dtype)) return R4C_ERR_UNSUPPORTED;
-  if (k > R4C_TOPK_MAX || d->rows > (int64_t)0x7fffffff * 8) return R4C_ERR_TOO_LARGE;
+  if (d->classes > rows::kTileClasses && (d->class_stride != 1 || d->grad_class_stride != 1)) return R4C_ERR_UNSUPPORTED;
+  if (k > R4C_TOPK_MAX) return R4C_ERR_TOO_LARGE;
+  // the marks of the listed classes, spread over a cluster of 16 blocks
+  if (rest && distill::mark_bytes<float>(d->classes, 16) > distill::kMostMarks) return R4C_ERR_TOO_LARGE;
   return R4C_OK;
 }
 distill::Args make_args(const r4c_rows_desc* d, const void* logits, int k, const void* t_logp, int t_dtype,
                         const void* t_index, int index_bits, int rest, const float* weight, void* stats) {
   distill::Args a{};
   a.z = logits;
-  a.v = {d->inner, d->outer_stride, d->inner_stride, d->class_stride};
-  a.dv = {d->inner, d->grad_outer_stride, d->grad_inner_stride, d->grad_class_stride};
+  a.v = rows::make_view(d);
+  a.dv = rows::make_grad_view(d);
   a.nrows = d->rows;
   a.C = d->classes;
   a.K = k;
@@ -250,61 +579,65 @@ distill::Args make_args(const r4c_rows_desc* d, const void* logits, int k, const
 }  // namespace
 
 extern "C" size_t r4c_distill_stats_size(const r4c_rows_desc* d) {
-  return rows::valid_desc(d) ? (size_t)d->rows * sizeof(distill::Stats) : 0;
+  if (!rows::valid_desc(d) || d->classes <= rows::kTileClasses) return 0;
+  return (size_t)d->rows * sizeof(distill::Stats);
 }
 extern "C" size_t r4c_distill_workspace_size(const r4c_rows_desc* d) {
-  return rows::valid_desc(d) ? (size_t)d->rows * 2 * sizeof(float) : 0;
+  return rows::valid_desc(d) ? (size_t)distill::kParts * 2 * sizeof(double) : 0;
 }
 
 extern "C" int r4c_distill_fwd(const r4c_rows_desc* d, const void* logits, int k, const void* teacher_logp,
                                int teacher_dtype, const void* teacher_index, int index_bits, int rest,
-                               const float* weight, float* row_loss, float* loss_weight, void* stats, void* ws,
-                               size_t ws_bytes, r4c_stream_t stream) {
-  const int rc = check(d, k, teacher_logp, teacher_dtype, teacher_index, index_bits);
+                               const float* weight, float* row_loss, float* loss, float* total_weight, void* stats,
+                               void* ws, size_t ws_bytes, r4c_stream_t stream) {
+  const int rc = check(d, k, teacher_logp, teacher_dtype, teacher_index, index_bits, rest);
   if (rc != R4C_OK) return rc;
-  if ((!row_loss && !loss_weight) || (d->rows > 0 && (!logits || !stats))) return R4C_ERR_INVALID;
-  if (d->rows > 0 && (!ws || ws_bytes < r4c_distill_workspace_size(d))) return R4C_ERR_WORKSPACE;
+  if ((!row_loss && !loss) || (loss && !total_weight)) return R4C_ERR_INVALID;
+  if (d->rows > 0 && (!logits || (!stats && r4c_distill_stats_size(d)))) return R4C_ERR_INVALID;
+  if (loss && (!ws || ws_bytes < r4c_distill_workspace_size(d))) return R4C_ERR_WORKSPACE;
   distill::Args a = make_args(d, logits, k, teacher_logp, teacher_dtype, teacher_index, index_bits, rest, weight, stats);
   a.err = tc::device_error_flag();
   if (!a.err) return R4C_ERR_NO_DEVICE;
-  a.row_loss = row_loss ? row_loss : static_cast<float*>(ws);
-  a.row_w = loss_weight ? static_cast<float*>(ws) + d->rows : nullptr;
+  a.row_loss = row_loss;
+  a.part = loss ? static_cast<double*>(ws) : nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int grid = (int)((d->rows + 7) / 8);
+  cudaError_t e = cudaSuccess;
+  int blocks = 0;
   if (d->rows > 0) {
-    if (d->dtype == R4C_BF16) distill::fwd_kernel<__nv_bfloat16><<<grid, distill::kThreads, 0, s>>>(a);
-    else if (d->dtype == R4C_F16) distill::fwd_kernel<__half><<<grid, distill::kThreads, 0, s>>>(a);
-    else distill::fwd_kernel<float><<<grid, distill::kThreads, 0, s>>>(a);
+    if (d->dtype == R4C_BF16) e = distill::launch_fwd<__nv_bfloat16>(a, &blocks, s);
+    else if (d->dtype == R4C_F16) e = distill::launch_fwd<__half>(a, &blocks, s);
+    else e = distill::launch_fwd<float>(a, &blocks, s);
     note_launches(1);
   }
-  if (loss_weight) {
-    distill::mean_kernel<<<1, 1024, 0, s>>>(a.row_loss, a.row_w, d->rows, loss_weight);
+  if (e == cudaSuccess && loss) {
+    distill::mean_kernel<<<1, distill::kMeanThreads, 0, s>>>(a.part, blocks, loss, total_weight);
+    e = cudaGetLastError();
     note_launches(1);
   }
-  return cudaGetLastError() == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
+  return e == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
 }
 
 extern "C" int r4c_distill_bwd(const r4c_rows_desc* d, const void* logits, int k, const void* teacher_logp,
                                int teacher_dtype, const void* teacher_index, int index_bits, int rest,
-                               const float* weight, const float* loss_weight, const float* grad, int grad_inc,
+                               const float* weight, const float* total_weight, const float* grad, int grad_inc,
                                const void* stats, void* dlogits, r4c_stream_t stream) {
-  const int rc = check(d, k, teacher_logp, teacher_dtype, teacher_index, index_bits);
+  const int rc = check(d, k, teacher_logp, teacher_dtype, teacher_index, index_bits, rest);
   if (rc != R4C_OK) return rc;
   if (d->rows == 0) return R4C_OK;
-  if (!logits || !dlogits || !grad || !stats) return R4C_ERR_INVALID;
+  if (!logits || !dlogits || !grad || (!stats && r4c_distill_stats_size(d))) return R4C_ERR_INVALID;
   distill::Args a = make_args(d, logits, k, teacher_logp, teacher_dtype, teacher_index, index_bits, rest, weight,
                               const_cast<void*>(stats));
   a.err = tc::device_error_flag();
   if (!a.err) return R4C_ERR_NO_DEVICE;
-  a.loss_weight = loss_weight;
+  a.total_weight = total_weight;
   a.grad = grad;
   a.grad_inc = grad_inc;
   a.dz = dlogits;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int grid = (int)((d->rows + 7) / 8);
-  if (d->dtype == R4C_BF16) distill::bwd_kernel<__nv_bfloat16><<<grid, distill::kThreads, 0, s>>>(a);
-  else if (d->dtype == R4C_F16) distill::bwd_kernel<__half><<<grid, distill::kThreads, 0, s>>>(a);
-  else distill::bwd_kernel<float><<<grid, distill::kThreads, 0, s>>>(a);
+  cudaError_t e;
+  if (d->dtype == R4C_BF16) e = distill::launch_bwd<__nv_bfloat16>(a, s);
+  else if (d->dtype == R4C_F16) e = distill::launch_bwd<__half>(a, s);
+  else e = distill::launch_bwd<float>(a, s);
   note_launches(1);
-  return cudaGetLastError() == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
+  return e == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
 }

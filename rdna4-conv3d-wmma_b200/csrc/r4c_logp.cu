@@ -5,8 +5,10 @@
 //   logp = s_t - lse,   H = ln S - (1/S) sum exp(s_c - m) (s_c - m)
 //   dz_c = (1/T) [ p_c (g_lse - g_logp - g_H (ln p_c + H)) + g_logp [c = t] ],  p_c = exp(s_c - lse)
 //
-// The difference s_c - m is taken before it is scaled, so rows of the type's
-// lowest value stay a uniform distribution instead of overflowing.
+// The difference z_c - max z is taken before it is scaled, so rows of the
+// type's lowest value stay a uniform distribution instead of overflowing.
+// Both directions read each logit once and are bound by memory; the kernels
+// for short and long rows are described in r4c_rows.cuh.
 #include "r4c_rows.cuh"
 
 namespace r4c {
@@ -14,13 +16,12 @@ namespace logp {
 
 using namespace rows;
 
-constexpr int kThreads = 256;
-
 struct FwdArgs {
   const void* z;
   const int64_t* target;
   int64_t ignore, nrows;
   View v;
+  Tile tile;
   int C, K;
   float inv_t;
   float *logp, *entropy, *lse, *top_logp;
@@ -34,7 +35,8 @@ struct BwdArgs {
   const int64_t* target;
   int64_t ignore, nrows;
   View v, dv;
-  int C;
+  Tile tile;
+  int C, segs;
   float inv_t;
   const float* entropy;
   const float2* stats;
@@ -44,6 +46,7 @@ struct BwdArgs {
   int* err;
 };
 
+// The row's label, -1 when it has none or takes no part.
 __device__ __forceinline__ int label_of(const int64_t* target, int64_t r, int C, int64_t ignore, int* err) {
   if (!target) return -1;
   const int64_t t = target[r];
@@ -55,77 +58,477 @@ __device__ __forceinline__ int label_of(const int64_t* target, int64_t r, int C,
   return (int)t;
 }
 
-// One warp per row, any strides.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(FwdArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (r >= a.nrows) return;
-  const T* z = static_cast<const T*>(a.z) + a.v.base(r);
-  const float k2 = a.inv_t * kLog2e;
-  float m = -INFINITY;
-  for (int c = lane; c < a.C; c += 32) m = fmaxf(m, Elem<T>::to_f(z[c * a.v.sc]));
-  m = warp_max(m);
-  const float mm = m == -INFINITY ? 0.f : m;
-  float s = 0.f, u = 0.f;
-  for (int c = lane; c < a.C; c += 32) {
-    const float d = Elem<T>::to_f(z[c * a.v.sc]) - mm;
-    const float e = ex2(d * k2);
-    s += e;
-    u += e * fmaxf(d, -1e30f);
+struct RowOut {   // what a row's sums say; bad: NaN or +inf in the row
+  float mm, ln_s, inv_t;
+  bool bad, empty;
+  __device__ __forceinline__ RowOut(const Run& r, float it) : mm(anchor(r.m)), inv_t(it), bad(isnan(r.s)), empty(r.s == 0.f) {
+    ln_s = empty ? -INFINITY : logf(r.s);
   }
-  s = warp_sum(s);
-  u = warp_sum(u);
-  const bool bad = isnan(s), empty = s == 0.f;
-  const float ln_s = empty ? -INFINITY : logf(s);
-  if (lane == 0) {
-    const int t = label_of(a.target, r, a.C, a.ignore, a.err);
-    if (a.target) a.logp[r] = t < 0 ? 0.f : empty ? -INFINITY : (Elem<T>::to_f(z[t * a.v.sc]) - mm) * a.inv_t - ln_s;
-    a.entropy[r] = empty ? 0.f : ln_s - a.inv_t * (u / s);
-    a.lse[r] = mm * a.inv_t + ln_s;
-    if (a.stats) a.stats[r] = make_float2(mm, ln_s);
+  __device__ __forceinline__ float logp(float z) const { return empty ? -INFINITY : (z - mm) * inv_t - ln_s; }
+  __device__ __forceinline__ float entropy(const Run& r) const { return empty ? 0.f : ln_s - inv_t * (r.u / r.s); }
+  __device__ __forceinline__ float lse() const { return mm * inv_t + ln_s; }
+};
+
+// ---- rows in registers -------------------------------------------------------
+template <typename T, int G, int E>
+__device__ __forceinline__ Run row_run(const TileRow<T, G, E>& x, float k) {
+  Run r = run_empty();
+#pragma unroll
+  for (int e = 0; e < E; ++e) r.m = fmaxf(r.m, x.v[e]);
+  r.m = group_max<G>(r.m);
+  const float mm = anchor(r.m);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float d = x.v[e] - mm, p = ex2(d * k);   // a place outside the row holds -inf: adds nothing
+    r.s += p;
+    r.u = fmaf(p, fmaxf(d, -1e30f), r.u);
   }
-  uint64_t last = ~0ull;
-  for (int j = 0; j < a.K; ++j) {
-    uint64_t best = 0;
-    if (!bad) {
-      for (int c = lane; c < a.C; c += 32) {
-        const uint64_t key = rank_key(Elem<T>::to_f(z[c * a.v.sc]), c);
-        if (key < last && key > best) best = key;
+  r.s = group_sum<G>(r.s);
+  r.u = group_sum<G>(r.u);
+  return r;
+}
+
+template <typename T, int G, int E>
+__global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
+  const float k = a.inv_t * kLog2e;
+  tile_walk<T, G, false>(a.tile, a.z, a.v, nullptr, [&](int64_t r, T* row, bool in) {
+    TileRow<T, G, E> x;
+    const bool staged = a.tile.staged;
+    x.load(row, a.v.sc, a.C, staged);
+    const Run run = row_run(x, k);
+    const RowOut o(run, a.inv_t);
+    if (in && x.lane == 0) {
+      if (a.target) {
+        const int t = label_of(a.target, r, a.C, a.ignore, a.err);
+        a.logp[r] = t < 0 ? 0.f : o.logp(Elem<T>::to_f(row[staged ? t : t * a.v.sc]));
       }
-      last = best = warp_max64(best);
+      a.entropy[r] = o.entropy(run);
+      a.lse[r] = o.lse();
     }
-    if (lane == 0) {
-      a.top_logp[r * a.K + j] = bad ? NAN : empty ? -INFINITY : (key_value(best) - mm) * a.inv_t - ln_s;
-      a.top_index[r * a.K + j] = bad ? -1 : key_class(best);
+    // the most probable classes, one after the other: lanes offer their best
+    // value that is not taken (ties: lowest class)
+    uint32_t open = x.live;
+    for (int j = 0; j < a.K; ++j) {
+      float b = -INFINITY;
+      int bc = 0x7fffffff, be = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = x.cls(e);
+        if ((open >> e & 1) && (x.v[e] > b || (x.v[e] == b && c < bc))) {
+          b = x.v[e];
+          bc = c;
+          be = e;
+        }
+      }
+      const int mine = bc;
+#pragma unroll
+      for (int off = G / 2; off; off >>= 1) {
+        const float ob = __shfl_xor_sync(0xffffffffu, b, off);
+        const int oc = __shfl_xor_sync(0xffffffffu, bc, off);
+        if (ob > b || (ob == b && oc < bc)) {
+          b = ob;
+          bc = oc;
+        }
+      }
+      if (mine == bc) open &= ~(1u << be);
+      if (in && x.lane == 0) {
+        a.top_logp[r * a.K + j] = o.bad ? NAN : o.logp(b);
+        a.top_index[r * a.K + j] = o.bad ? -1 : bc;
+      }
     }
+  });
+}
+
+template <typename T, int G, int E>
+__global__ void __launch_bounds__(kTileThreads) bwd_tile_kernel(BwdArgs a) {
+  const float k = a.inv_t * kLog2e;
+  tile_walk<T, G, true>(a.tile, a.z, a.v, a.dz, [&](int64_t r, T* row, bool in) {
+    TileRow<T, G, E> x;
+    const bool staged = a.tile.staged;
+    x.load(row, a.v.sc, a.C, staged);
+    const int t = label_of(a.target, r, a.C, a.ignore, a.err);
+    const float gl = a.g_logp && t >= 0 ? a.g_logp[r * a.gl_inc] : 0.f;
+    const float gh = a.g_entropy ? a.g_entropy[r * a.gh_inc] : 0.f;
+    const float gs = a.g_lse ? a.g_lse[r * a.gs_inc] : 0.f;
+    const Run run = row_run(x, k);
+    const RowOut o(run, a.inv_t);
+    const bool none = (gl == 0.f && gh == 0.f && gs == 0.f) || o.empty;
+    const float ca = a.inv_t * (gs - gl - gh * o.entropy(run)), cb = a.inv_t * gh;
+    float g[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float ln_p = fmaxf((x.v[e] - o.mm) * a.inv_t, -1e30f) - o.ln_s;
+      g[e] = ex2(ln_p * kLog2e) * (ca - cb * ln_p);
+      if (x.cls(e) == t) g[e] += a.inv_t * gl;
+      if (none) g[e] = 0.f;
+      else if (o.bad) g[e] = NAN;
+    }
+    if (in) {
+      T* out = staged ? row : static_cast<T*>(a.dz) + a.dv.base(r);
+      x.store(out, a.dv.sc, staged, g, x.live);
+    }
+  });
+}
+
+// ---- rows streamed -----------------------------------------------------------
+constexpr int kCand = 2048;   // candidate keys a block keeps while it selects
+
+// The K largest keys of a block's part of a row, in order, into sh.top
+// (0 where the part has fewer). Each thread knows the largest value of its
+// own vectors and the vector it is in; the K-th largest of those is a bound
+// that at least K elements reach, and few more do, so only the vectors of
+// the threads that reach it are looked at again. Keys are unique (value,
+// then class), which makes the result exact whatever the ties; if elements
+// crowd above the bound (more than kCand) it is raised by bisection first.
+struct TopShared {
+  uint64_t* cand;     // kCand
+  uint64_t* top;      // R4C_TOPK_MAX
+  uint64_t* keys;     // a thread's best, as a lower bound
+  int* active;        // threads that reach the bound
+  uint64_t tau;
+  int n_active, n_cand;
+};
+
+template <typename T, int NT>
+__device__ void block_topk(const VecRow<T>& x, int v0, int v1, int f0, int f1, float tm, int tv, int K, bool skip,
+                           TopShared& sh) {
+  constexpr int VE = Vec<T>::kElems;
+  const int tid = threadIdx.x;
+  const bool have = tv >= 0;
+  const int nd = f1 - f0 < 0 ? 0 : f1 - f0 < NT ? f1 - f0 : NT;   // threads with a vector
+  sh.keys[tid] = have ? rank_key(tm, x.cls(tv) + VE - 1) : 0;
+  if (tid == 0) {
+    sh.n_active = 0;
+    sh.n_cand = 0;
+    sh.tau = 0;
+  }
+  for (int j = tid; j < K; j += NT) sh.top[j] = 0;
+  __syncthreads();
+  if (nd >= K && tid < 32) {
+    uint64_t kk[NT / 32], lo = ~0ull, hi = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) {
+      kk[i] = sh.keys[tid + 32 * i];
+      hi = kk[i] > hi ? kk[i] : hi;
+      if (kk[i] && kk[i] < lo) lo = kk[i];
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const uint64_t l = __shfl_xor_sync(0xffffffffu, lo, o), h = __shfl_xor_sync(0xffffffffu, hi, o);
+      lo = l < lo ? l : lo;
+      hi = h > hi ? h : hi;
+    }
+    hi += 1;   // none reach it; all nd >= K reach lo
+    const int enough = K + (K >> 1) + 4;
+    int reach = nd;
+    while (reach > enough && hi - lo > 1) {
+      const uint64_t mid = lo + ((hi - lo) >> 1);
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < NT / 32; ++i) c += kk[i] >= mid;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (c >= K) {
+        lo = mid;
+        reach = c;
+      } else {
+        hi = mid;
+      }
+    }
+    if (tid == 0) sh.tau = lo;
+  }
+  __syncthreads();
+  uint64_t tau = sh.tau;
+  if (have && rank_key(tm, x.cls(tv)) >= tau) sh.active[atomicAdd(&sh.n_active, 1)] = tid;
+  __syncthreads();
+  const int iters = (f1 - f0 + NT - 1) / NT;
+  const int items = skip ? 0 : sh.n_active * iters;
+  // every element that reaches `bound`: kept in cand (keep) or counted
+  auto scan = [&](uint64_t bound, bool keep) {
+    auto look = [&](float z, int c) {
+      const uint64_t key = rank_key(z, c);
+      if (key >= bound) {
+        const int at = atomicAdd(&sh.n_cand, 1);
+        if (keep && at < kCand) sh.cand[at] = key;
+      }
+    };
+    for (int q = tid; q < items; q += NT) {
+      const int v = f0 + sh.active[q / iters] + (q % iters) * NT;
+      if (v < f1) {
+        float y[VE];
+        Vec<T>::split(__ldg(x.p + v), y);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) look(y[i], x.cls(v) + i);
+      }
+    }
+    if (!skip) {   // the partial vectors at the row's ends
+      if (f0 > v0 && tid < VE) {
+        const int c = x.cls(v0) + tid;
+        if (c >= 0 && c < x.C) look(Elem<T>::to_f(x.row[c]), c);
+      }
+      if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) {
+        const int c = x.cls(f1) + tid - 32;
+        if (c >= 0 && c < x.C) look(Elem<T>::to_f(x.row[c]), c);
+      }
+    }
+    __syncthreads();
+    const int n = sh.n_cand;
+    __syncthreads();
+    if (tid == 0) sh.n_cand = 0;
+    __syncthreads();
+    return n;
+  };
+  int n = scan(tau, true);
+  if (n > kCand) {
+    uint64_t lo = tau, hi = ~0ull;
+    while (hi - lo > 1) {
+      const uint64_t mid = lo + ((hi - lo) >> 1);
+      const int c = scan(mid, false);
+      if (c >= K) {
+        lo = mid;
+        if (c <= kCand) break;
+      } else {
+        hi = mid;
+      }
+    }
+    n = scan(lo, true);
+    n = n < kCand ? n : kCand;
+  }
+  for (int i = tid; i < n; i += NT) {
+    const uint64_t key = sh.cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += sh.cand[j] > key;
+    if (rank < K) sh.top[rank] = key;
+  }
+  __syncthreads();
+}
+
+template <typename T, int NT, bool TOP>
+__global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
+  constexpr int VE = Vec<T>::kElems, U = 4;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ Run runs[NT / 32];
+  __shared__ Run mine;
+  __shared__ TopShared top;
+  const int tid = threadIdx.x;
+  uint32_t cs = 1, cr = 0;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cs));
+  if (cs > 1) cr = cluster_rank();
+  if (TOP && tid == 0) {
+    top.cand = reinterpret_cast<uint64_t*>(dyn);
+    top.top = top.cand + kCand;
+    top.keys = top.top + R4C_TOPK_MAX;
+    top.active = reinterpret_cast<int*>(top.keys + NT);
+  }
+  __syncthreads();
+  const float k = a.inv_t * kLog2e;
+  for (int64_t r = blockIdx.x / cs; r < a.nrows; r += gridDim.x / cs) {
+    const VecRow<T> x(static_cast<const T*>(a.z) + a.v.base(r), a.C);
+    const int per = (x.nv + (int)cs - 1) / (int)cs;
+    const int v0 = min((int)cr * per, x.nv), v1 = min(v0 + per, x.nv);
+    const int f0 = max(v0, x.first_full()), f1 = min(v1, x.end_full());
+    Run run = run_empty();
+    float tm = 0.f;   // the largest value of this thread's full vectors, and the first vector that has it
+    int tv = -1;
+    for (int v = f0 + tid; v < f1; v += U * NT) {
+      uint4 w[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (v + i * NT < f1) w[i] = __ldg(x.p + v + i * NT);
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (v + i * NT < f1) {
+          float y[VE];
+          Vec<T>::split(w[i], y);
+          run_add<VE, true>(run, y, k);
+          if (TOP) {
+            float vm = y[0];
+#pragma unroll
+            for (int j = 1; j < VE; ++j) vm = fmaxf(vm, y[j]);
+            if (tv < 0 || vm > tm) {
+              tm = vm;
+              tv = v + i * NT;
+            }
+          }
+        }
+      }
+    }
+    if (f0 > v0 && tid < VE) {   // partial vectors: one element a thread
+      const int c = x.cls(v0) + tid;
+      const float y = c >= 0 && c < a.C ? Elem<T>::to_f(x.row[c]) : -INFINITY;
+      run_add<1, true>(run, &y, k);
+    }
+    if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) {
+      const int c = x.cls(f1) + tid - 32;
+      const float y = c >= 0 && c < a.C ? Elem<T>::to_f(x.row[c]) : -INFINITY;
+      run_add<1, true>(run, &y, k);
+    }
+    run = run_block<NT>(run, k, runs);
+    if (TOP) block_topk<T, NT>(x, v0, v1, f0, f1, tm, tv, a.K, isnan(run.s), top);
+    if (cs > 1) {
+      if (tid == 0) mine = run;
+      cluster_sync();
+      if (cr == 0) {
+        for (uint32_t q = 1; q < cs; ++q) run = run_merge(run, cluster_ld_run(&mine, q), k);
+        if (TOP) {
+          // the blocks' ordered lists, side by side: a key's place is the number of larger keys in each
+          for (int i = tid; i < (int)cs * a.K; i += NT)
+            top.cand[i] = cluster_ld_u64(cluster_map(top.top + i % a.K, i / a.K));
+          __syncthreads();
+        }
+      }
+    }
+    if (cr == 0) {
+      const RowOut o(run, a.inv_t);
+      if (tid == 0) {
+        if (a.target) {
+          const int t = label_of(a.target, r, a.C, a.ignore, a.err);
+          a.logp[r] = t < 0 ? 0.f : o.logp(Elem<T>::to_f(x.row[t]));
+        }
+        a.entropy[r] = o.entropy(run);
+        a.lse[r] = o.lse();
+        if (a.stats) a.stats[r] = make_float2(o.mm, o.ln_s);
+      }
+      if (TOP) {
+        for (int i = tid; i < (int)cs * a.K; i += NT) {
+          uint64_t key = top.top[i % a.K];
+          int rank = i;
+          if (cs > 1) {
+            key = top.cand[i];
+            rank = 0;
+            for (uint32_t q = 0; key && q < cs; ++q) {
+              int lo = 0, hi = a.K;
+              while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (top.cand[q * a.K + mid] > key) lo = mid + 1;
+                else hi = mid;
+              }
+              rank += lo;
+            }
+          }
+          if (o.bad && i < a.K) {
+            a.top_logp[r * a.K + i] = NAN;
+            a.top_index[r * a.K + i] = -1;
+          } else if (!o.bad && key && rank < a.K) {
+            a.top_logp[r * a.K + rank] = o.logp(key_value(key));
+            a.top_index[r * a.K + rank] = key_class(key);
+          }
+        }
+      }
+    }
+    if (cs > 1) cluster_sync();   // the other blocks' sums and lists have been read
+    else __syncthreads();
   }
 }
 
+// One block per piece of a row.
+constexpr int kBwdThreads = 256, kBwdVecs = 4;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) bwd_kernel(BwdArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (r >= a.nrows) return;
-  const T* z = static_cast<const T*>(a.z) + a.v.base(r);
-  T* dz = static_cast<T*>(a.dz) + a.dv.base(r);
+__global__ void __launch_bounds__(kBwdThreads) bwd_block_kernel(BwdArgs a) {
+  constexpr int VE = Vec<T>::kElems;
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x / a.segs;
+  const int seg = blockIdx.x % a.segs;
+  const VecRow<T> x(static_cast<const T*>(a.z) + a.v.base(r), a.C);
+  const VecRow<T> y(static_cast<T*>(a.dz) + a.dv.base(r), a.C);
+  uint4* out = const_cast<uint4*>(y.p);
+  T* out_row = const_cast<T*>(y.row);
+  const bool same = x.off == y.off;   // both rows break into vectors at the same classes
+  const int v0 = seg * kBwdThreads * kBwdVecs, v1 = min(v0 + kBwdThreads * kBwdVecs, x.nv);
+  uint4 w[kBwdVecs];
+#pragma unroll
+  for (int i = 0; i < kBwdVecs; ++i) {
+    const int v = v0 + tid + i * kBwdThreads;
+    if (v < v1 && v >= x.first_full() && v < x.end_full()) w[i] = __ldg(x.p + v);
+  }
   const int t = label_of(a.target, r, a.C, a.ignore, a.err);
   const float gl = a.g_logp && t >= 0 ? a.g_logp[r * a.gl_inc] : 0.f;
   const float gh = a.g_entropy ? a.g_entropy[r * a.gh_inc] : 0.f;
   const float gs = a.g_lse ? a.g_lse[r * a.gs_inc] : 0.f;
   const float2 st = a.stats[r];
-  const float h = a.entropy[r];
-  const bool none = (gl == 0.f && gh == 0.f && gs == 0.f) || st.y == -INFINITY;
-  for (int c = lane; c < a.C; c += 32) {
-    float g = 0.f;
-    if (!none) {
-      const float ln_p = fmaxf((Elem<T>::to_f(z[c * a.v.sc]) - st.x) * a.inv_t, -1e30f) - st.y;
-      const float p = ex2(ln_p * kLog2e);
-      g = a.inv_t * (p * (gs - gl - gh * (ln_p + h)) + (c == t ? gl : 0.f));
-      if (isnan(Elem<T>::to_f(z[c * a.v.sc]))) g = NAN;
+  const bool none = (gl == 0.f && gh == 0.f && gs == 0.f) || st.y == -INFINITY, bad = isnan(st.y);
+  const float ca = a.inv_t * (gs - gl - gh * a.entropy[r]), cb = a.inv_t * gh;
+  auto grad = [&](float z, int c) {
+    const float ln_p = fmaxf((z - st.x) * a.inv_t, -1e30f) - st.y;
+    float g = ex2(ln_p * kLog2e) * (ca - cb * ln_p);
+    if (c == t) g += a.inv_t * gl;
+    return none ? 0.f : bad ? NAN : g;
+  };
+#pragma unroll
+  for (int i = 0; i < kBwdVecs; ++i) {
+    const int v = v0 + tid + i * kBwdThreads;
+    if (v >= v1) continue;
+    const int c0 = x.cls(v);
+    if (v >= x.first_full() && v < x.end_full()) {
+      float g[VE];
+      Vec<T>::split(w[i], g);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) g[j] = grad(g[j], c0 + j);
+      if (same) out[v] = Vec<T>::join(g);
+      else
+        for (int j = 0; j < VE; ++j) out_row[c0 + j] = Elem<T>::from_f(g[j]);
+    } else {
+      for (int j = 0; j < VE; ++j)
+        if (c0 + j >= 0 && c0 + j < a.C) out_row[c0 + j] = Elem<T>::from_f(grad(Elem<T>::to_f(x.row[c0 + j]), c0 + j));
     }
-    dz[c * a.dv.sc] = Elem<T>::from_f(g);
   }
+}
+
+// ---- launches ----------------------------------------------------------------
+template <typename T, bool BWD, typename A>
+cudaError_t launch_tiles(A& a, const TileKind& kind, cudaStream_t s) {
+#define R4C_TILE(G, E)                                                                             \
+  if (kind.g == G && kind.e == E) {                                                                \
+    if constexpr (BWD) return launch_tile(bwd_tile_kernel<T, G, E>, a.tile, kTileThreads / G, s, a); \
+    else return launch_tile(fwd_tile_kernel<T, G, E>, a.tile, kTileThreads / G, s, a);             \
+  }
+  R4C_TILE(1, 4) R4C_TILE(1, 8) R4C_TILE(1, 16) R4C_TILE(1, 32) R4C_TILE(4, 16) R4C_TILE(8, 16) R4C_TILE(16, 16)
+  R4C_TILE(32, 16) R4C_TILE(32, 32)
+#undef R4C_TILE
+  return cudaErrorInvalidValue;
+}
+
+template <typename T, int NT>
+cudaError_t launch_fwd_block(const FwdArgs& a, cudaStream_t s) {
+  const int cs = cluster_size(a.nrows, a.C, sizeof(T), NT);
+  const int64_t most = (int64_t)kSMs * (2048 / NT);
+  int64_t grid = a.nrows * cs;
+  if (cs == 1 && grid > most) grid = most;
+  if (a.K > 0) {
+    const size_t smem = (kCand + R4C_TOPK_MAX + NT) * sizeof(uint64_t) + NT * sizeof(int);
+    return launch_cluster(fwd_block_kernel<T, NT, true>, grid, NT, cs, smem, s, a);
+  }
+  return launch_cluster(fwd_block_kernel<T, NT, false>, grid, NT, cs, 0, s, a);
+}
+
+template <typename T>
+cudaError_t launch_fwd(FwdArgs& a, cudaStream_t s) {
+  if (a.C <= kTileClasses) {
+    const TileKind kind = tile_kind(a.C);
+    r4c_rows_desc d{};
+    d.rows = a.nrows;
+    d.classes = a.C;
+    a.tile = make_tile(&d, sizeof(T), kind.g, dense_rows(a.v, a.nrows, a.C, a.z));
+    return launch_tiles<T, false>(a, kind, s);
+  }
+  if ((int64_t)a.C * sizeof(T) <= 16 << 10) return launch_fwd_block<T, 128>(a, s);
+  return launch_fwd_block<T, 512>(a, s);
+}
+
+template <typename T>
+cudaError_t launch_bwd(BwdArgs& a, cudaStream_t s) {
+  if (a.C <= kTileClasses) {
+    const TileKind kind = tile_kind(a.C);
+    r4c_rows_desc d{};
+    d.rows = a.nrows;
+    d.classes = a.C;
+    a.tile = make_tile(&d, sizeof(T), kind.g,
+                       dense_rows(a.v, a.nrows, a.C, a.z) && dense_rows(a.dv, a.nrows, a.C, a.dz));
+    return launch_tiles<T, true>(a, kind, s);
+  }
+  a.segs = (a.C / Vec<T>::kElems + 2 + kBwdThreads * kBwdVecs - 1) / (kBwdThreads * kBwdVecs);
+  if (a.nrows * a.segs > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  bwd_block_kernel<T><<<(unsigned)(a.nrows * a.segs), kBwdThreads, 0, s>>>(a);
+  return cudaGetLastError();
 }
 
 }  // namespace logp
@@ -133,53 +536,60 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(BwdArgs a) {
 
 using namespace r4c;
 
+namespace {
+int check(const r4c_rows_desc* d) {
+  if (!rows::valid_desc(d)) return R4C_ERR_INVALID;
+  if (!rows::valid_dtype(d->dtype)) return R4C_ERR_UNSUPPORTED;
+  if (d->classes > rows::kTileClasses && (d->class_stride != 1 || d->grad_class_stride != 1)) return R4C_ERR_UNSUPPORTED;
+  return R4C_OK;
+}
+}  // namespace
+
 extern "C" size_t r4c_logp_stats_size(const r4c_rows_desc* d) {
-  return rows::valid_desc(d) ? (size_t)d->rows * sizeof(float2) : 0;
+  if (!rows::valid_desc(d) || d->classes <= rows::kTileClasses) return 0;
+  return (size_t)d->rows * sizeof(float2);
 }
 
 extern "C" int r4c_logp_fwd(const r4c_rows_desc* d, const void* logits, const int64_t* target, int64_t ignore_index,
                             int top_k, float* logp, float* entropy, float* lse, float* top_logp, int32_t* top_index,
                             void* stats, r4c_stream_t stream) {
-  if (!rows::valid_desc(d) || top_k < 0 || top_k > d->classes) return R4C_ERR_INVALID;
+  const int rc = check(d);
+  if (rc != R4C_OK) return rc;
+  if (top_k < 0 || top_k > d->classes) return R4C_ERR_INVALID;
+  if (top_k > R4C_TOPK_MAX) return R4C_ERR_TOO_LARGE;
   if (d->rows == 0) return R4C_OK;
   if (!logits || !entropy || !lse || (target && !logp) || (top_k > 0 && (!top_logp || !top_index))) return R4C_ERR_INVALID;
-  if (!rows::valid_dtype(d->dtype)) return R4C_ERR_UNSUPPORTED;
-  if (top_k > R4C_TOPK_MAX) return R4C_ERR_TOO_LARGE;
   int* err = tc::device_error_flag();
   if (!err) return R4C_ERR_NO_DEVICE;
-  logp::FwdArgs a{logits, target, ignore_index, d->rows, {d->inner, d->outer_stride, d->inner_stride, d->class_stride},
-                  d->classes, top_k, 1.f / d->temperature, logp, entropy, lse, top_logp, top_index,
-                  static_cast<float2*>(stats), err};
+  logp::FwdArgs a{logits, target, ignore_index, d->rows, rows::make_view(d), {}, d->classes, top_k,
+                  1.f / d->temperature, logp, entropy, lse, top_logp, top_index, static_cast<float2*>(stats), err};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int64_t grid = (d->rows + 7) / 8;
-  if (grid > 0x7fffffff) return R4C_ERR_TOO_LARGE;
-  if (d->dtype == R4C_BF16) logp::fwd_kernel<__nv_bfloat16><<<(int)grid, logp::kThreads, 0, s>>>(a);
-  else if (d->dtype == R4C_F16) logp::fwd_kernel<__half><<<(int)grid, logp::kThreads, 0, s>>>(a);
-  else logp::fwd_kernel<float><<<(int)grid, logp::kThreads, 0, s>>>(a);
+  cudaError_t e;
+  if (d->dtype == R4C_BF16) e = logp::launch_fwd<__nv_bfloat16>(a, s);
+  else if (d->dtype == R4C_F16) e = logp::launch_fwd<__half>(a, s);
+  else e = logp::launch_fwd<float>(a, s);
   note_launches(1);
-  return cudaGetLastError() == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
+  return e == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
 }
 
 extern "C" int r4c_logp_bwd(const r4c_rows_desc* d, const void* logits, const int64_t* target, int64_t ignore_index,
                             const float* entropy, const void* stats, const float* g_logp, int g_logp_inc,
                             const float* g_entropy, int g_entropy_inc, const float* g_lse, int g_lse_inc,
                             void* dlogits, r4c_stream_t stream) {
-  if (!rows::valid_desc(d)) return R4C_ERR_INVALID;
+  const int rc = check(d);
+  if (rc != R4C_OK) return rc;
   if (d->rows == 0) return R4C_OK;
-  if (!logits || !dlogits || !entropy || !stats || (g_logp && !target)) return R4C_ERR_INVALID;
-  if (!rows::valid_dtype(d->dtype)) return R4C_ERR_UNSUPPORTED;
+  if (!logits || !dlogits || !entropy || (!stats && r4c_logp_stats_size(d)) || (g_logp && !target)) return R4C_ERR_INVALID;
   int* err = tc::device_error_flag();
   if (!err) return R4C_ERR_NO_DEVICE;
-  logp::BwdArgs a{logits, target, ignore_index, d->rows, {d->inner, d->outer_stride, d->inner_stride, d->class_stride},
-                  {d->inner, d->grad_outer_stride, d->grad_inner_stride, d->grad_class_stride}, d->classes,
-                  1.f / d->temperature, entropy, static_cast<const float2*>(stats), g_logp, g_entropy, g_lse,
+  logp::BwdArgs a{logits, target, ignore_index, d->rows, rows::make_view(d), rows::make_grad_view(d), {}, d->classes,
+                  0, 1.f / d->temperature, entropy, static_cast<const float2*>(stats), g_logp, g_entropy, g_lse,
                   g_logp_inc, g_entropy_inc, g_lse_inc, dlogits, err};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int64_t grid = (d->rows + 7) / 8;
-  if (grid > 0x7fffffff) return R4C_ERR_TOO_LARGE;
-  if (d->dtype == R4C_BF16) logp::bwd_kernel<__nv_bfloat16><<<(int)grid, logp::kThreads, 0, s>>>(a);
-  else if (d->dtype == R4C_F16) logp::bwd_kernel<__half><<<(int)grid, logp::kThreads, 0, s>>>(a);
-  else logp::bwd_kernel<float><<<(int)grid, logp::kThreads, 0, s>>>(a);
+  cudaError_t e;
+  if (d->dtype == R4C_BF16) e = logp::launch_bwd<__nv_bfloat16>(a, s);
+  else if (d->dtype == R4C_F16) e = logp::launch_bwd<__half>(a, s);
+  else e = logp::launch_bwd<float>(a, s);
   note_launches(1);
-  return cudaGetLastError() == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
+  return e == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
 }

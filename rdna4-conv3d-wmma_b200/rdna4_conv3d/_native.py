@@ -112,7 +112,7 @@ def _bind(lib) -> None:
         "r4c_logp_bwd": ([R, P, P, i64, P, P, P, i, P, i, P, i, P, P], i),
         "r4c_distill_stats_size": ([R], sz),
         "r4c_distill_workspace_size": ([R], sz),
-        "r4c_distill_fwd": ([R, P, i, P, i, P, i, i, P, P, P, P, P, sz, P], i),
+        "r4c_distill_fwd": ([R, P, i, P, i, P, i, i, P, P, P, P, P, P, sz, P], i),
         "r4c_distill_bwd": ([R, P, i, P, i, P, i, i, P, P, P, i, P, P, P], i),
         "r4c_convex_plan": ([X], i),
         "r4c_convex_workspace_size": ([X, i], sz),
@@ -710,36 +710,36 @@ def logp_backward(rows: Rows, target: Optional[torch.Tensor], ignore_index: int,
 
 def distill_forward(rows: Rows, teacher_logp: torch.Tensor, teacher_index: torch.Tensor, rest: bool,
                     weight: Optional[torch.Tensor], mean: bool):
-    """(row losses or None, (mean, total weight) or None, stats)."""
+    """(loss, total weight or None, stats or None): the mean over rows, or the rows' own losses."""
     dev = _require_cuda(rows.z, teacher_logp, teacher_index, weight)
     L, d = lib(), rows.desc
-    row_loss = None if mean else torch.empty(rows.shape, dtype=torch.float32, device=dev)
-    loss_weight = torch.empty(2, dtype=torch.float32, device=dev) if mean else None
+    loss = torch.empty(() if mean else rows.shape, dtype=torch.float32, device=dev)
+    total = torch.empty((), dtype=torch.float32, device=dev) if mean else None
     nb = int(L.r4c_distill_stats_size(ctypes.byref(d)))
     stats = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-    nb = int(L.r4c_distill_workspace_size(ctypes.byref(d)))
+    nb = int(L.r4c_distill_workspace_size(ctypes.byref(d))) if mean else 0
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
     with torch.cuda.device(dev):
         st = L.r4c_distill_fwd(ctypes.byref(d), _ptr(rows.z), int(teacher_logp.shape[-1]), _ptr(teacher_logp),
                                dtype_code(teacher_logp.dtype), _ptr(teacher_index), 8 * teacher_index.element_size(),
-                               1 if rest else 0, _ptr(weight), _ptr(row_loss), _ptr(loss_weight), _ptr(stats),
-                               _ptr(ws), nb, _stream(dev))
+                               1 if rest else 0, _ptr(weight), _ptr(None if mean else loss),
+                               _ptr(loss if mean else None), _ptr(total), _ptr(stats), _ptr(ws), nb, _stream(dev))
     _check(st, "r4c_distill_fwd")
-    return row_loss, loss_weight, stats
+    return loss, total, stats
 
 
 def distill_backward(rows: Rows, teacher_logp: torch.Tensor, teacher_index: torch.Tensor, rest: bool,
-                     weight: Optional[torch.Tensor], loss_weight: Optional[torch.Tensor],
+                     weight: Optional[torch.Tensor], total_weight: Optional[torch.Tensor],
                      stats: Optional[torch.Tensor], grad: torch.Tensor) -> torch.Tensor:
     dev = _require_cuda(rows.z)
     dz = rows.grad_like()
     g, inc = _grad_inc(grad)
-    if loss_weight is not None:
+    if total_weight is not None:
         inc = 0
     with torch.cuda.device(dev):
         st = lib().r4c_distill_bwd(ctypes.byref(rows.desc), _ptr(rows.z), int(teacher_logp.shape[-1]),
                                    _ptr(teacher_logp), dtype_code(teacher_logp.dtype), _ptr(teacher_index),
                                    8 * teacher_index.element_size(), 1 if rest else 0, _ptr(weight),
-                                   _ptr(loss_weight), _ptr(g), inc, _ptr(stats), _ptr(dz), _stream(dev))
+                                   _ptr(total_weight), _ptr(g), inc, _ptr(stats), _ptr(dz), _stream(dev))
     _check(st, "r4c_distill_bwd")
     return dz

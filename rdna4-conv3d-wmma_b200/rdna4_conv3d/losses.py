@@ -60,17 +60,17 @@ class DistillTopKFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_logp, teacher_index, temperature, rest, weight, mean):
         rows = _native.Rows(logits, temperature)
-        row_loss, loss_weight, stats = _native.distill_forward(rows, teacher_logp, teacher_index, rest, weight, mean)
-        ctx.save_for_backward(rows.z, teacher_logp, teacher_index, weight, loss_weight, stats)
+        loss, total, stats = _native.distill_forward(rows, teacher_logp, teacher_index, rest, weight, mean)
+        ctx.save_for_backward(rows.z, teacher_logp, teacher_index, weight, total, stats)
         ctx.temperature, ctx.rest = temperature, rest
-        return loss_weight[0].clone() if mean else row_loss
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        z, teacher_logp, teacher_index, weight, loss_weight, stats = ctx.saved_tensors
+        z, teacher_logp, teacher_index, weight, total, stats = ctx.saved_tensors
         dz = _native.distill_backward(_native.Rows(z, ctx.temperature), teacher_logp, teacher_index, ctx.rest, weight,
-                                      loss_weight, stats, grad)
+                                      total, stats, grad)
         return dz, None, None, None, None, None, None
 
 

@@ -447,7 +447,9 @@ def test_steps_in_a_graph(cuda_ready):
 
 @pytest.mark.parametrize("c", [2, 70000])
 def test_many_rows_past_32_bits(cuda_ready, c):
-    """Rows whose element offsets pass 2^31: the last rows against those rows alone."""
+    """Rows whose element offsets pass 2^31: the last rows against those rows
+    alone (a few long rows are split over blocks, which sums in another order,
+    so values agree to the derived bounds and classes exactly)."""
     from rdna4_conv3d.logprobs import log_probs
     from rdna4_conv3d.losses import distill_topk
     n = (2 ** 31 + 2 ** 20) // c
@@ -461,9 +463,11 @@ def test_many_rows_past_32_bits(cuda_ready, c):
     dz, = torch.autograd.grad(loss, z)
     tail = z.detach()[-3:].clone().requires_grad_(True)
     p = log_probs(tail, t[-3:], top_k=1)
-    for a, b in zip(o, p):
-        assert torch.equal(a[-3:], b)
+    for name in ("logp", "entropy", "lse", "top_logp"):
+        assert_values(getattr(o, name)[-3:], getattr(p, name).detach().cpu().double(), name)
+    assert torch.equal(o.top_index[-3:], p.top_index)
     small = distill_topk(tail, v[-3:], p.top_index)
-    assert_values(loss.reshape(1), small.detach().cpu().double().reshape(1), "loss", 1e-6, 1e-6)
+    assert_values(loss.reshape(1), small.detach().cpu().double().reshape(1), "loss", 3e-5, 5e-6)
     ref, = torch.autograd.grad(small, tail)
-    assert torch.equal(dz[-3:], ref) and float(dz[:-3].abs().max()) == 0.0
+    assert_grad(rows_of(dz[-3:]), rows_of(ref), BF)
+    assert float(dz[:-3].abs().max()) == 0.0

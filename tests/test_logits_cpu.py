@@ -236,7 +236,7 @@ def test_c_entries_check_their_arguments():
     assert L.r4c_logp_fwd(d, *[None] * 2, -100, 0, *null, None) == -1
     assert L.r4c_logp_fwd(d, 1 << 20, None, -100, 9, *null, None) == -1          # more than the classes
     assert L.r4c_logp_bwd(d, None, None, -100, None, None, None, 1, None, 1, None, 1, None, None) == -1
-    assert L.r4c_distill_fwd(d, None, 0, None, 0, None, 32, 0, *[None] * 5, 0, None) == -1
+    assert L.r4c_distill_fwd(d, None, 0, None, 0, None, 32, 0, *[None] * 6, 0, None) == -1
     for field, value in (("temperature", 0.0), ("temperature", float("inf")), ("classes", 0), ("rows", -1), ("inner", 0)):
         e = _native.RowsDesc(4, 4, 0, 8, 1, 0, 8, 1, 8, _native.R4C_BF16, 1.0)
         setattr(e, field, value)
