@@ -413,25 +413,23 @@ int r4c_logp_bwd(const r4c_rows_desc* desc, const void* logits, const int64_t* t
  * void, its weight is 0 or it has no finite logit. teacher_logp is bf16, fp16
  * or fp32, teacher_index 32- or 64-bit integers (index_bits), weight (fp32,
  * >= 0) may be null: 1 for every row.
- * r4c_distill_fwd writes row_loss[r] = w[r] L[r] (may be null), and
- * loss[0] = sum(w L) / sum(w) with total_weight[0] = sum(w) (device memory,
- * both may be null; summed in a fixed order in double; NaN when no row takes
- * part; `ws` of r4c_distill_workspace_size(desc) bytes is needed for these),
- * and `stats` for the backward (r4c_distill_stats_size(desc) bytes, null when
- * that is 0). Above 1024 classes the classes must be contiguous
- * (class_stride 1), and rest = 1 takes about ten million classes at most.
- * r4c_distill_bwd writes dlogits = grad[r * grad_inc] * w / sum(w) * dL/dz
- * with total_weight (of the forward) given, else without the division.
+ * r4c_distill_fwd writes row_loss[r] = w[r] L[r] (may be null) or, with loss
+ * given, loss[0] = sum(w L) / sum(w) (device memory; summed in a fixed order
+ * in double; NaN when no row takes part). `state` of
+ * r4c_distill_state_size(desc) bytes, 16-byte aligned, is its workspace and
+ * carries the rows' sums and sum(w) to the backward.
+ * r4c_distill_bwd writes dlogits = grad[r * grad_inc] * w * dL/dz, divided by
+ * sum(w) with mean = 1 (the forward had loss given).
+ * Above 1024 classes the classes must be contiguous (class_stride 1), and
+ * rest = 1 takes about ten million classes at most.
  */
-size_t r4c_distill_stats_size(const r4c_rows_desc* desc);
-size_t r4c_distill_workspace_size(const r4c_rows_desc* desc);
+size_t r4c_distill_state_size(const r4c_rows_desc* desc);
 int r4c_distill_fwd(const r4c_rows_desc* desc, const void* logits, int k, const void* teacher_logp, int teacher_dtype,
                     const void* teacher_index, int index_bits, int rest, const float* weight, float* row_loss,
-                    float* loss, float* total_weight, void* stats, void* ws, size_t ws_bytes, r4c_stream_t stream);
+                    float* loss, void* state, size_t state_bytes, r4c_stream_t stream);
 int r4c_distill_bwd(const r4c_rows_desc* desc, const void* logits, int k, const void* teacher_logp, int teacher_dtype,
-                    const void* teacher_index, int index_bits, int rest, const float* weight,
-                    const float* total_weight, const float* grad, int grad_inc, const void* stats, void* dlogits,
-                    r4c_stream_t stream);
+                    const void* teacher_index, int index_bits, int rest, const float* weight, int mean,
+                    const float* grad, int grad_inc, const void* state, void* dlogits, r4c_stream_t stream);
 
 /*
  * Conv3d weight and bias gradient without any allocation. No counterpart in

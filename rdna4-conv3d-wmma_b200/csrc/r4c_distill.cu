@@ -556,8 +556,11 @@ int check(const r4c_rows_desc* d, int k, const void* t_logp, int t_dtype, const 
   if (rest && distill::mark_bytes<float>(d->classes, 16) > distill::kMostMarks) return R4C_ERR_TOO_LARGE;
   return R4C_OK;
 }
+// The state: the blocks' partial sums, the sum of weights, the rows' statistics.
+constexpr size_t kTotalAt = (size_t)distill::kParts * 2 * sizeof(double), kStatsAt = kTotalAt + 16;
+
 distill::Args make_args(const r4c_rows_desc* d, const void* logits, int k, const void* t_logp, int t_dtype,
-                        const void* t_index, int index_bits, int rest, const float* weight, void* stats) {
+                        const void* t_index, int index_bits, int rest, const float* weight, void* state) {
   distill::Args a{};
   a.z = logits;
   a.v = rows::make_view(d);
@@ -573,33 +576,30 @@ distill::Args make_args(const r4c_rows_desc* d, const void* logits, int k, const
   a.t_dtype = t_dtype;
   a.t_wide = index_bits == 64;
   a.weight = weight;
-  a.stats = static_cast<distill::Stats*>(stats);
+  a.stats = reinterpret_cast<distill::Stats*>(static_cast<char*>(state) + kStatsAt);
   return a;
 }
 }  // namespace
 
-extern "C" size_t r4c_distill_stats_size(const r4c_rows_desc* d) {
-  if (!rows::valid_desc(d) || d->classes <= rows::kTileClasses) return 0;
-  return (size_t)d->rows * sizeof(distill::Stats);
-}
-extern "C" size_t r4c_distill_workspace_size(const r4c_rows_desc* d) {
-  return rows::valid_desc(d) ? (size_t)distill::kParts * 2 * sizeof(double) : 0;
+extern "C" size_t r4c_distill_state_size(const r4c_rows_desc* d) {
+  if (!rows::valid_desc(d)) return 0;
+  return kStatsAt + (d->classes <= rows::kTileClasses ? 0 : (size_t)d->rows * sizeof(distill::Stats));
 }
 
 extern "C" int r4c_distill_fwd(const r4c_rows_desc* d, const void* logits, int k, const void* teacher_logp,
                                int teacher_dtype, const void* teacher_index, int index_bits, int rest,
-                               const float* weight, float* row_loss, float* loss, float* total_weight, void* stats,
-                               void* ws, size_t ws_bytes, r4c_stream_t stream) {
+                               const float* weight, float* row_loss, float* loss, void* state, size_t state_bytes,
+                               r4c_stream_t stream) {
   const int rc = check(d, k, teacher_logp, teacher_dtype, teacher_index, index_bits, rest);
   if (rc != R4C_OK) return rc;
-  if ((!row_loss && !loss) || (loss && !total_weight)) return R4C_ERR_INVALID;
-  if (d->rows > 0 && (!logits || (!stats && r4c_distill_stats_size(d)))) return R4C_ERR_INVALID;
-  if (loss && (!ws || ws_bytes < r4c_distill_workspace_size(d))) return R4C_ERR_WORKSPACE;
-  distill::Args a = make_args(d, logits, k, teacher_logp, teacher_dtype, teacher_index, index_bits, rest, weight, stats);
+  if ((!row_loss && !loss) || (d->rows > 0 && !logits)) return R4C_ERR_INVALID;
+  if (!state || state_bytes < r4c_distill_state_size(d)) return R4C_ERR_WORKSPACE;
+  if ((uintptr_t)state & 15) return R4C_ERR_ALIGN;
+  distill::Args a = make_args(d, logits, k, teacher_logp, teacher_dtype, teacher_index, index_bits, rest, weight, state);
   a.err = tc::device_error_flag();
   if (!a.err) return R4C_ERR_NO_DEVICE;
   a.row_loss = row_loss;
-  a.part = loss ? static_cast<double*>(ws) : nullptr;
+  a.part = loss ? static_cast<double*>(state) : nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   int blocks = 0;
@@ -610,7 +610,8 @@ extern "C" int r4c_distill_fwd(const r4c_rows_desc* d, const void* logits, int k
     note_launches(1);
   }
   if (e == cudaSuccess && loss) {
-    distill::mean_kernel<<<1, distill::kMeanThreads, 0, s>>>(a.part, blocks, loss, total_weight);
+    distill::mean_kernel<<<1, distill::kMeanThreads, 0, s>>>(
+        a.part, blocks, loss, reinterpret_cast<float*>(static_cast<char*>(state) + kTotalAt));
     e = cudaGetLastError();
     note_launches(1);
   }
@@ -619,17 +620,17 @@ extern "C" int r4c_distill_fwd(const r4c_rows_desc* d, const void* logits, int k
 
 extern "C" int r4c_distill_bwd(const r4c_rows_desc* d, const void* logits, int k, const void* teacher_logp,
                                int teacher_dtype, const void* teacher_index, int index_bits, int rest,
-                               const float* weight, const float* total_weight, const float* grad, int grad_inc,
-                               const void* stats, void* dlogits, r4c_stream_t stream) {
+                               const float* weight, int mean, const float* grad, int grad_inc, const void* state,
+                               void* dlogits, r4c_stream_t stream) {
   const int rc = check(d, k, teacher_logp, teacher_dtype, teacher_index, index_bits, rest);
   if (rc != R4C_OK) return rc;
   if (d->rows == 0) return R4C_OK;
-  if (!logits || !dlogits || !grad || (!stats && r4c_distill_stats_size(d))) return R4C_ERR_INVALID;
+  if (!logits || !dlogits || !grad || !state) return R4C_ERR_INVALID;
   distill::Args a = make_args(d, logits, k, teacher_logp, teacher_dtype, teacher_index, index_bits, rest, weight,
-                              const_cast<void*>(stats));
+                              const_cast<void*>(state));
   a.err = tc::device_error_flag();
   if (!a.err) return R4C_ERR_NO_DEVICE;
-  a.total_weight = total_weight;
+  a.total_weight = mean ? reinterpret_cast<const float*>(static_cast<const char*>(state) + kTotalAt) : nullptr;
   a.grad = grad;
   a.grad_inc = grad_inc;
   a.dz = dlogits;

@@ -110,10 +110,9 @@ def _bind(lib) -> None:
         "r4c_logp_stats_size": ([R], sz),
         "r4c_logp_fwd": ([R, P, P, i64, i, P, P, P, P, P, P, P], i),
         "r4c_logp_bwd": ([R, P, P, i64, P, P, P, i, P, i, P, i, P, P], i),
-        "r4c_distill_stats_size": ([R], sz),
-        "r4c_distill_workspace_size": ([R], sz),
-        "r4c_distill_fwd": ([R, P, i, P, i, P, i, i, P, P, P, P, P, P, sz, P], i),
-        "r4c_distill_bwd": ([R, P, i, P, i, P, i, i, P, P, P, i, P, P, P], i),
+        "r4c_distill_state_size": ([R], sz),
+        "r4c_distill_fwd": ([R, P, i, P, i, P, i, i, P, P, P, P, sz, P], i),
+        "r4c_distill_bwd": ([R, P, i, P, i, P, i, i, P, i, P, i, P, P, P], i),
         "r4c_convex_plan": ([X], i),
         "r4c_convex_workspace_size": ([X, i], sz),
         "r4c_convex_fwd": ([X, P, P, P, P, P, sz, P], i),
@@ -639,107 +638,121 @@ class Rows:
     """Logits as the row kernels read them: ``z`` (the logits themselves, or a
     class-last copy where the kernels cannot walk their strides), their
     descriptor, and the per-row shape (N, ...)."""
-    __slots__ = ("z", "desc", "shape", "stats")
+    __slots__ = ("z", "desc", "shape")
 
     def __init__(self, logits: torch.Tensor, temperature: float):
         z = logits
-        st = _row_strides(z)
-        if st is None or (st[3] != 1 and z.shape[1] > _TILE_CLASSES):
-            z = class_last_empty(logits).copy_(logits)
+        shape = z.shape
+        c = shape[1]
+        if len(shape) == 2 and z.is_contiguous():
+            n = shape[0]
+            inner, so, si, sc = n or 1, 0, c, 1
+            self.shape = shape[:1]
+        else:
             st = _row_strides(z)
-        shape = logits.shape[:1] + logits.shape[2:]
-        inner, so, si, sc = st
-        self.z, self.shape = z, shape
-        self.desc = RowsDesc(shape.numel(), max(inner, 1), so, si, sc, so, si, sc, int(logits.shape[1]),
-                             dtype_code(logits.dtype), temperature)
+            if st is None or (st[3] != 1 and c > _TILE_CLASSES):
+                z = class_last_empty(logits).copy_(logits)
+                st = _row_strides(z)
+            inner, so, si, sc = st
+            self.shape = shape[:1] + shape[2:]
+            n = self.shape.numel()
+        self.z = z
+        self.desc = RowsDesc(n, inner or 1, so, si, sc, so, si, sc, c, dtype_code(z.dtype), temperature)
 
-    def grad_like(self) -> torch.Tensor:
-        """A new tensor for the gradient; sets the descriptor's gradient strides."""
-        z = self.z
-        dz = torch.empty_like(z)
-        if dz.stride() != z.stride():                    # z overlaps or has gaps: a dense class-last gradient
-            dz = class_last_empty(z)
-            inner, so, si, sc = _row_strides(dz)
-            d = self.desc
-            if d.inner != inner:                         # the gradient's rows in the logits' (outer, inner) split
-                so = si * d.inner
-            d.grad_outer_stride, d.grad_inner_stride, d.grad_class_stride = so, si, sc
-        return dz
+
+def rows_grad(z: torch.Tensor, desc: RowsDesc) -> torch.Tensor:
+    """A new tensor for the gradient of rows that lie as ``z``; sets the descriptor's gradient strides."""
+    dz = torch.empty_like(z)
+    if dz.stride() != z.stride():                        # z overlaps or has gaps: a dense class-last gradient
+        dz = class_last_empty(z)
+        inner, so, si, sc = _row_strides(dz)
+        if desc.inner != inner:                          # the gradient's rows in the logits' (outer, inner) split
+            so = si * desc.inner
+        desc.grad_outer_stride, desc.grad_inner_stride, desc.grad_class_stride = so, si, sc
+    return dz
 
 
 def _grad_inc(g: Optional[torch.Tensor]):
     """(fp32 tensor, increment per row) of an upstream gradient: one shared value has increment 0."""
     if g is None:
         return None, 0
-    if g.numel() > 1 and not any(g.stride()):
-        return g[(0,) * g.dim()].float(), 0
-    return g.float().contiguous(), 1
+    if g.dtype != torch.float32:
+        g = g.float()
+    if g.is_contiguous():
+        return g, 1
+    if not any(g.stride()):
+        return g[(0,) * g.dim()], 0
+    return g.contiguous(), 1
+
+
+def _launch(what: str, fn, dev: torch.device, *args) -> None:
+    """Calls a row entry with the device current and its current stream last."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if st != R4C_OK:
+        _check(st, what)
 
 
 def logp_forward(rows: Rows, target: Optional[torch.Tensor], ignore_index: int, top_k: int, want_stats: bool):
     """(logp or None, entropy, lse, top_logp or None, top_index or None, stats or None)."""
-    dev = _require_cuda(rows.z, target)
-    L, d, shape = lib(), rows.desc, rows.shape
-    f32 = dict(dtype=torch.float32, device=dev)
-    logp = torch.empty(shape, **f32) if target is not None else None
-    entropy, lse = torch.empty(shape, **f32), torch.empty(shape, **f32)
-    top_logp = torch.empty((*shape, top_k), **f32) if top_k else None
-    top_index = torch.empty((*shape, top_k), dtype=torch.int32, device=dev) if top_k else None
-    stats = None
+    L, d, z = lib(), rows.desc, rows.z
+    shape = rows.shape
+    entropy = z.new_empty(shape, dtype=torch.float32)
+    lse = torch.empty_like(entropy)
+    logp = tl = ti = stats = None
+    if target is not None:
+        logp = torch.empty_like(entropy)
+    if top_k:
+        tl = z.new_empty((*shape, top_k), dtype=torch.float32)
+        ti = torch.empty_like(tl, dtype=torch.int32)
     if want_stats:
-        nb = int(L.r4c_logp_stats_size(ctypes.byref(d)))
-        stats = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-    with torch.cuda.device(dev):
-        st = L.r4c_logp_fwd(ctypes.byref(d), _ptr(rows.z), _ptr(target), ignore_index, top_k, _ptr(logp),
-                            _ptr(entropy), _ptr(lse), _ptr(top_logp), _ptr(top_index), _ptr(stats), _stream(dev))
-    _check(st, "r4c_logp_fwd")
-    return logp, entropy, lse, top_logp, top_index, stats
+        nb = L.r4c_logp_stats_size(d)
+        if nb:
+            stats = z.new_empty(nb, dtype=torch.uint8)
+    _launch("r4c_logp_fwd", L.r4c_logp_fwd, z.device, d, z.data_ptr(), None if target is None else target.data_ptr(),
+            ignore_index, top_k, None if logp is None else logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(),
+            None if tl is None else tl.data_ptr(), None if ti is None else ti.data_ptr(),
+            None if stats is None else stats.data_ptr())
+    return logp, entropy, lse, tl, ti, stats
 
 
-def logp_backward(rows: Rows, target: Optional[torch.Tensor], ignore_index: int, entropy: torch.Tensor,
-                  stats: Optional[torch.Tensor], g_logp, g_entropy, g_lse) -> torch.Tensor:
-    dev = _require_cuda(rows.z)
-    dz = rows.grad_like()
+def logp_backward(z: torch.Tensor, desc: RowsDesc, target: Optional[torch.Tensor], ignore_index: int,
+                  entropy: torch.Tensor, stats: Optional[torch.Tensor], g_logp, g_entropy, g_lse) -> torch.Tensor:
+    dz = rows_grad(z, desc)
     (gl, il), (gh, ih), (gs, is_) = _grad_inc(g_logp), _grad_inc(g_entropy), _grad_inc(g_lse)
-    with torch.cuda.device(dev):
-        st = lib().r4c_logp_bwd(ctypes.byref(rows.desc), _ptr(rows.z), _ptr(target), ignore_index, _ptr(entropy),
-                                _ptr(stats), _ptr(gl), il, _ptr(gh), ih, _ptr(gs), is_, _ptr(dz), _stream(dev))
-    _check(st, "r4c_logp_bwd")
+    _launch("r4c_logp_bwd", lib().r4c_logp_bwd, z.device, desc, z.data_ptr(),
+            None if target is None else target.data_ptr(), ignore_index, entropy.data_ptr(),
+            None if stats is None else stats.data_ptr(), None if gl is None else gl.data_ptr(), il,
+            None if gh is None else gh.data_ptr(), ih, None if gs is None else gs.data_ptr(), is_, dz.data_ptr())
     return dz
 
 
 def distill_forward(rows: Rows, teacher_logp: torch.Tensor, teacher_index: torch.Tensor, rest: bool,
                     weight: Optional[torch.Tensor], mean: bool):
-    """(loss, total weight or None, stats or None): the mean over rows, or the rows' own losses."""
-    dev = _require_cuda(rows.z, teacher_logp, teacher_index, weight)
-    L, d = lib(), rows.desc
-    loss = torch.empty(() if mean else rows.shape, dtype=torch.float32, device=dev)
-    total = torch.empty((), dtype=torch.float32, device=dev) if mean else None
-    nb = int(L.r4c_distill_stats_size(ctypes.byref(d)))
-    stats = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-    nb = int(L.r4c_distill_workspace_size(ctypes.byref(d))) if mean else 0
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-    with torch.cuda.device(dev):
-        st = L.r4c_distill_fwd(ctypes.byref(d), _ptr(rows.z), int(teacher_logp.shape[-1]), _ptr(teacher_logp),
-                               dtype_code(teacher_logp.dtype), _ptr(teacher_index), 8 * teacher_index.element_size(),
-                               1 if rest else 0, _ptr(weight), _ptr(None if mean else loss),
-                               _ptr(loss if mean else None), _ptr(total), _ptr(stats), _ptr(ws), nb, _stream(dev))
-    _check(st, "r4c_distill_fwd")
-    return loss, total, stats
+    """(loss, state): the mean over rows or the rows' own losses, and what the backward needs."""
+    L, d, z = lib(), rows.desc, rows.z
+    loss = z.new_empty(() if mean else rows.shape, dtype=torch.float32)
+    nb = L.r4c_distill_state_size(d)
+    state = z.new_empty(nb, dtype=torch.uint8)
+    at = loss.data_ptr()
+    _launch("r4c_distill_fwd", L.r4c_distill_fwd, z.device, d, z.data_ptr(), teacher_logp.shape[-1],
+            teacher_logp.data_ptr(), dtype_code(teacher_logp.dtype), teacher_index.data_ptr(),
+            8 * teacher_index.element_size(), rest, None if weight is None else weight.data_ptr(),
+            None if mean else at, at if mean else None, state.data_ptr(), nb)
+    return loss, state
 
 
-def distill_backward(rows: Rows, teacher_logp: torch.Tensor, teacher_index: torch.Tensor, rest: bool,
-                     weight: Optional[torch.Tensor], total_weight: Optional[torch.Tensor],
-                     stats: Optional[torch.Tensor], grad: torch.Tensor) -> torch.Tensor:
-    dev = _require_cuda(rows.z)
-    dz = rows.grad_like()
+def distill_backward(z: torch.Tensor, desc: RowsDesc, teacher_logp: torch.Tensor, teacher_index: torch.Tensor,
+                     rest: bool, weight: Optional[torch.Tensor], mean: bool, state: torch.Tensor,
+                     grad: torch.Tensor) -> torch.Tensor:
+    dz = rows_grad(z, desc)
     g, inc = _grad_inc(grad)
-    if total_weight is not None:
-        inc = 0
-    with torch.cuda.device(dev):
-        st = lib().r4c_distill_bwd(ctypes.byref(rows.desc), _ptr(rows.z), int(teacher_logp.shape[-1]),
-                                   _ptr(teacher_logp), dtype_code(teacher_logp.dtype), _ptr(teacher_index),
-                                   8 * teacher_index.element_size(), 1 if rest else 0, _ptr(weight),
-                                   _ptr(total_weight), _ptr(g), inc, _ptr(stats), _ptr(dz), _stream(dev))
-    _check(st, "r4c_distill_bwd")
+    _launch("r4c_distill_bwd", lib().r4c_distill_bwd, z.device, desc, z.data_ptr(), teacher_logp.shape[-1],
+            teacher_logp.data_ptr(), dtype_code(teacher_logp.dtype), teacher_index.data_ptr(),
+            8 * teacher_index.element_size(), rest, None if weight is None else weight.data_ptr(), mean,
+            g.data_ptr(), 0 if mean else inc, state.data_ptr(), dz.data_ptr())
     return dz

@@ -43,24 +43,29 @@ def check_logits(logits: torch.Tensor, temperature: float) -> None:
         raise ValueError(f"temperature must be finite and positive, got {temperature}")
 
 
+def refuse_twice() -> None:
+    """In a backward: the native gradients have no graph of their own."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the native gradient of this operator cannot be differentiated again (create_graph)")
+
+
 class LogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target, top_k, temperature, ignore_index):
         rows = _native.Rows(logits, temperature)
+        logp, entropy, lse, top_logp, top_index, stats = _native.logp_forward(rows, target, ignore_index, top_k, True)
         ctx.set_materialize_grads(False)
-        logp, entropy, lse, top_logp, top_index, stats = _native.logp_forward(
-            rows, target, ignore_index, top_k, logits.requires_grad)
         ctx.save_for_backward(rows.z, target, entropy, stats)
-        ctx.temperature, ctx.ignore_index = temperature, ignore_index
-        ctx.mark_non_differentiable(*(t for t in (top_logp, top_index) if t is not None))
+        ctx.desc, ctx.ignore_index = rows.desc, ignore_index
+        if top_k:
+            ctx.mark_non_differentiable(top_logp, top_index)
         return logp, entropy, lse, top_logp, top_index
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy, g_lse, _top_logp, _top_index):
+        refuse_twice()
         z, target, entropy, stats = ctx.saved_tensors
-        dz = _native.logp_backward(_native.Rows(z, ctx.temperature), target, ctx.ignore_index, entropy, stats,
-                                   g_logp, g_entropy, g_lse)
+        dz = _native.logp_backward(z, ctx.desc, target, ctx.ignore_index, entropy, stats, g_logp, g_entropy, g_lse)
         return dz, None, None, None, None
 
 
@@ -94,7 +99,9 @@ def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, *, to
     if not logits.is_cuda:
         return _log_probs_torch(logits, target, top_k, temperature, ignore_index)
     if target is not None:
-        target = target.to(torch.int64).contiguous()
+        if target.dtype != torch.int64:
+            target = target.to(torch.int64)
+        target = target.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
         return LogProbs(*LogProbsFn.apply(logits, target, top_k, temperature, ignore_index))
     return LogProbs(*_native.logp_forward(_native.Rows(logits, temperature), target, ignore_index, top_k, False)[:5])

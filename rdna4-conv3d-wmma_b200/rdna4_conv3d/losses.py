@@ -22,7 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _native
-from .logprobs import check_logits
+from .logprobs import check_logits, refuse_twice
 
 
 class CrossEntropyNDHWCFn(torch.autograd.Function):
@@ -60,17 +60,16 @@ class DistillTopKFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_logp, teacher_index, temperature, rest, weight, mean):
         rows = _native.Rows(logits, temperature)
-        loss, total, stats = _native.distill_forward(rows, teacher_logp, teacher_index, rest, weight, mean)
-        ctx.save_for_backward(rows.z, teacher_logp, teacher_index, weight, total, stats)
-        ctx.temperature, ctx.rest = temperature, rest
+        loss, state = _native.distill_forward(rows, teacher_logp, teacher_index, rest, weight, mean)
+        ctx.save_for_backward(rows.z, teacher_logp, teacher_index, weight, state)
+        ctx.desc, ctx.rest, ctx.mean = rows.desc, rest, mean
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        z, teacher_logp, teacher_index, weight, total, stats = ctx.saved_tensors
-        dz = _native.distill_backward(_native.Rows(z, ctx.temperature), teacher_logp, teacher_index, ctx.rest, weight,
-                                      total, stats, grad)
+        refuse_twice()
+        z, teacher_logp, teacher_index, weight, state = ctx.saved_tensors
+        dz = _native.distill_backward(z, ctx.desc, teacher_logp, teacher_index, ctx.rest, weight, ctx.mean, state, grad)
         return dz, None, None, None, None, None, None
 
 
@@ -116,12 +115,17 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
             raise ValueError(f"{name} is on {t.device}, logits on {logits.device}")
     if not logits.is_cuda:
         return _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weight, reduction)
+    if teacher_logp.requires_grad:
+        teacher_logp = teacher_logp.detach()
     if teacher_logp.dtype == torch.float64:
         teacher_logp = teacher_logp.float()
     if weight is not None:
         weight = weight.detach().to(torch.float32).contiguous()
-    return DistillTopKFn.apply(logits, teacher_logp.detach().contiguous(), teacher_index.contiguous(), temperature,
-                               rest, weight, reduction == "mean")
+    teacher_logp, teacher_index, mean = teacher_logp.contiguous(), teacher_index.contiguous(), reduction == "mean"
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return DistillTopKFn.apply(logits, teacher_logp, teacher_index, temperature, bool(rest), weight, mean)
+    rows = _native.Rows(logits, temperature)
+    return _native.distill_forward(rows, teacher_logp, teacher_index, bool(rest), weight, mean)[0]
 
 
 def _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weight, reduction):

@@ -187,6 +187,16 @@ def test_log_probs_differences(cuda_ready, c):
     assert abs(float(diff) - float((dz.double() * u.double()).sum())) <= 1.5e-3
 
 
+def test_second_derivatives_are_refused(cuda_ready):
+    from rdna4_conv3d.logprobs import log_probs
+    from rdna4_conv3d.losses import distill_topk
+    z = _logits((3, 5), FP).requires_grad_(True)
+    v, idx = _teacher(3, 5, 2)
+    for y in (log_probs(z).entropy.sum(), distill_topk(z, v, idx)):
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(y, z, create_graph=True)
+
+
 def test_log_probs_out_of_range_sets_the_flag(cuda_ready):
     from rdna4_conv3d import _native
     from rdna4_conv3d.logprobs import log_probs

@@ -208,9 +208,9 @@ def test_row_descriptors_walk_the_logits(c):
         flat = rows.z.as_strided((rows.z.untyped_storage().nbytes() // 4,), (1,), 0)
         got = flat[_places(rows.desc, n, c) + rows.z.storage_offset()]
         assert torch.equal(got, z.movedim(1, -1).reshape(-1, c)), z.stride()
-        dz = rows.grad_like()
-        assert dz.shape == z.shape
         d = rows.desc
+        dz = _native.rows_grad(rows.z, d)
+        assert dz.shape == z.shape
         seen = (torch.arange(n)[:, None] // d.inner) * d.grad_outer_stride + \
             (torch.arange(n)[:, None] % d.inner) * d.grad_inner_stride + torch.arange(c) * d.grad_class_stride
         assert sorted(seen.reshape(-1).tolist()) == list(range(n * c))
@@ -236,11 +236,11 @@ def test_c_entries_check_their_arguments():
     assert L.r4c_logp_fwd(d, *[None] * 2, -100, 0, *null, None) == -1
     assert L.r4c_logp_fwd(d, 1 << 20, None, -100, 9, *null, None) == -1          # more than the classes
     assert L.r4c_logp_bwd(d, None, None, -100, None, None, None, 1, None, 1, None, 1, None, None) == -1
-    assert L.r4c_distill_fwd(d, None, 0, None, 0, None, 32, 0, *[None] * 6, 0, None) == -1
+    assert L.r4c_distill_fwd(d, None, 0, None, 0, None, 32, 0, *[None] * 4, 0, None) == -1
     for field, value in (("temperature", 0.0), ("temperature", float("inf")), ("classes", 0), ("rows", -1), ("inner", 0)):
         e = _native.RowsDesc(4, 4, 0, 8, 1, 0, 8, 1, 8, _native.R4C_BF16, 1.0)
         setattr(e, field, value)
-        assert L.r4c_logp_stats_size(e) == 0 and L.r4c_distill_stats_size(e) == 0
+        assert L.r4c_logp_stats_size(e) == 0 and L.r4c_distill_state_size(e) == 0
         assert L.r4c_logp_fwd(e, *[None] * 2, -100, 0, *null, None) == -1
     e = _native.RowsDesc(0, 1, 0, 8, 1, 0, 8, 1, 8, _native.R4C_BF16, 1.0)
     assert L.r4c_logp_fwd(e, *[None] * 2, -100, 0, *null, None) == 0              # no rows: nothing to do
