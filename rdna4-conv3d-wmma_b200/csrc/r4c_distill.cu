@@ -20,9 +20,9 @@ namespace distill {
 using namespace rows;
 
 struct Stats {           // per streamed row, written by the forward for the backward
-  float m, ln_s;         // lse = m / T + ln_s (m a logit, not yet scaled)
-  float mr, ln_sr;       // the same over the unlisted classes
-  float q_norm;          // ln q_j = v_j - q_norm
+  float m, s;            // lse = m / T + ln s (m a logit, not yet scaled)
+  float mr, sr;          // the same over the unlisted classes
+  float qm, qs;          // q_j = exp(v_j - qm) / qs
   float mass, q_rest;    // Q, q_r
   float w;               // the row's weight, 0: takes no part
 };
@@ -94,17 +94,19 @@ __device__ __forceinline__ void leave_part(double loss, double w, double* part) 
 }
 
 // The terms of a row that come from its sums: r over the unlisted classes
-// (rest) or all of them, l over the listed ones (rest).
+// (rest) or all of them, l over the listed ones (rest). Probabilities are
+// exponentials divided by their sum, logarithms serve the loss alone: a
+// difference p - q then keeps the exponentials' own error.
 struct RowSums {
-  float m, ln_s, mr, ln_sr;
+  float m, s, mr, sr;
   bool empty;
   __device__ __forceinline__ RowSums(const Run& r, const Run& l, bool rest, float k) {
     const Run all = rest ? run_merge(r, l, k) : r;
     empty = all.s == 0.f;
     m = anchor(all.m);
-    ln_s = logf(all.s);
+    s = all.s;
     mr = anchor(r.m);
-    ln_sr = logf(r.s);
+    sr = r.s;
   }
 };
 // q_r from the sum of the listed q.
@@ -112,128 +114,176 @@ __device__ __forceinline__ float rest_mass(float sum_q) {
   const float qr = 1.f - sum_q;
   return qr >= kRestNoise ? qr : 0.f;
 }
+// q_r (ln q_r - ln p_r)
 __device__ __forceinline__ float rest_loss(float qr, const RowSums& s, float inv_t) {
-  return qr > 0.f ? qr * (logf(qr) - ((s.mr - s.m) * inv_t + (s.ln_sr - s.ln_s))) : 0.f;
+  return qr > 0.f ? qr * (kLn2 * (__log2f(qr) - __log2f(s.sr) + __log2f(s.s)) - (s.mr - s.m) * inv_t) : 0.f;
 }
-// The factor of exp(s_c - lse_r) in an unlisted class's gradient.
-__device__ __forceinline__ float rest_coef(float mass, float qr, float mr, float ln_sr, float m, float ln_s, float inv_t) {
-  return mass * ex2(((mr - m) * inv_t + (ln_sr - ln_s)) * kLog2e) - qr;
+// The factor of 2^t (t from mr) in the gradient of an unlisted class: (Q p_r - q_r) / sr, 0 without any.
+__device__ __forceinline__ float rest_coef(bool rest, float mass, float qr, float m, float s, float mr, float sr, float k) {
+  if (!rest) return __fdividef(mass, s);
+  return sr == 0.f ? 0.f : mass * ex2((mr - m) * k) / s - qr / sr;
 }
+// The pairs' exponentials: few, and their difference from the student's is the gradient.
+__device__ __forceinline__ float prob(float ln_q) { return expf(ln_q); }
 
 // ---- rows in registers -------------------------------------------------------
-template <typename T, int G, int E, bool BWD>
+// The teacher's pairs of a row, lane l of the group taking pairs l, l + G,
+// ...; the first kSlots of a lane stay in registers, more are read again.
+constexpr int kSlots = 2;
+struct Pair {
+  float v, z;   // the teacher's log-probability, the student's logit
+  int c;        // class, -1: void
+};
+
+template <typename T, int G, int E, bool VEC, bool BWD>
 __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
+  constexpr int ES = (int)sizeof(T);
   const float k = a.inv_t * kLog2e;
+  const bool rest = a.rest;
   double sum_loss = 0.0, sum_w = 0.0;
-  tile_walk<T, G, BWD>(a.tile, a.z, a.v, a.dz, [&](int64_t r, T* row, bool in) {
-    const bool staged = a.tile.staged;
-    const int64_t sc = staged ? 1 : a.v.sc;
-    TileRow<T, G, E> x;
-    x.load(row, a.v.sc, a.C, staged);
+  tile_walk<T, G, BWD>(a.tile, a.v, a.z, a.dv, a.dz, [&](int64_t r, uint32_t row, bool in) {
+    const int lane = threadIdx.x & (G - 1);
+    const int64_t p0 = r * a.K;
     float w = a.weight ? a.weight[r] : 1.f;
-    // which of this lane's values the teacher lists
-    uint32_t listed = 0;
+    auto read = [&](int j) {   // from memory: the row in shared memory changes below
+      Pair p;
+      p.v = teacher_logp(a, p0 + j);
+      p.c = teacher_class(a, p0 + j, p.v);
+      return p;
+    };
+    auto logit = [&](int c) { return Elem<T>::to_f(static_cast<const T*>(a.z)[a.v.base(r) + c * a.v.sc]); };
+    Pair held[kSlots];
     float qm = -INFINITY;
-    bool any = false, twice = false;
-    for (int j = 0; j < a.K; ++j) {
-      const float v = teacher_logp(a, r * a.K + j);
-      const int c = teacher_class(a, r * a.K + j, v);
-      int e;
-      if (c < 0) continue;
-      any = true;
-      qm = fmaxf(qm, v);
-      if (x.owns(c, &e)) {
-        twice |= listed >> e & 1;
-        listed |= 1u << e;
+    bool any = false;
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      held[s].c = -1;
+      if (s * G < a.K && lane + s * G < a.K) {
+        held[s] = read(lane + s * G);
+        if (held[s].c >= 0) {
+          held[s].z = sh_get<T>(row + held[s].c * ES);
+          qm = fmaxf(qm, held[s].v);
+          any = true;
+        }
       }
     }
+    for (int j = lane + kSlots * G; j < a.K; j += G) {
+      const Pair p = read(j);
+      if (p.c >= 0) {
+        qm = fmaxf(qm, p.v);
+        any = true;
+      }
+    }
+    if (G > 1) any = group_any<G>(any);
     if (!any) w = 0.f;
-    if (G > 1) twice = group_any<G>(twice);
-    // sums over the unlisted classes, with a maximum of their own, and over the listed ones
+    // f(pair, its number) for each valid pair of this lane
+    auto pairs = [&](auto&& f) {
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s)
+        if (s * G < a.K && held[s].c >= 0) f(held[s], lane + s * G);
+      for (int j = lane + kSlots * G; j < a.K; j += G) {
+        Pair p = read(j);
+        if (p.c < 0) continue;
+        p.z = logit(p.c);
+        f(p, j);
+      }
+    };
+    // Is a class listed twice? Each pair leaves its number at its class and
+    // looks whether it is still there; the logits are put back after that.
+    bool twice = false;
+    if ((rest || BWD) && a.K > 1) {
+      __syncwarp();
+      if (in) pairs([&](const Pair& p, int j) { sh_put<T>(row + p.c * ES, (float)(j + 1)); });
+      __syncwarp();
+      if (in) pairs([&](const Pair& p, int j) { twice |= sh_get<T>(row + p.c * ES) != (float)(j + 1); });
+      if (G > 1) twice = group_any<G>(twice);
+      __syncwarp();
+    }
+    // With a rest the listed classes leave the row; their own sum comes from the pairs.
+    if ((rest || BWD) && in && (rest || a.K > 1))
+      pairs([&](const Pair& p, int) { sh_put<T>(row + p.c * ES, rest ? -INFINITY : p.z); });
+    __syncwarp();
+    TileRow<T, G, E, VEC> x;
+    x.load(row, a.C);
+    if (G > 1) __syncwarp();   // read by all before any of it is written over
+    auto first = [&](const Pair& p, int j) {   // of the pairs with this class
+      if (!twice) return true;
+      for (int i = 0; i < j; ++i)
+        if (read(i).c == p.c) return false;
+      return true;
+    };
     Run u = run_empty(), l = run_empty();
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (a.rest && (listed >> e & 1)) l.m = fmaxf(l.m, x.v[e]);
-      else u.m = fmaxf(u.m, x.v[e]);
+    {
+      Run2 part = run2_empty();
+      part.m = x.max();
+      run2_add<E, false>(part, x.v, k);
+      u = part.join();
+      u.s = group_sum<G>(u.s);
     }
-    u.m = group_max<G>(u.m);
-    if (a.rest) l.m = group_max<G>(l.m);
-    const float um = anchor(u.m), lm = anchor(l.m);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const bool at = a.rest && (listed >> e & 1);
-      const float p = ex2((x.v[e] - (at ? lm : um)) * k);
-      if (at) l.s += p;
-      else u.s += p;
+    if (rest) {
+      pairs([&](const Pair& p, int) { l.m = fmaxf(l.m, p.z); });
+      l.m = group_max<G>(l.m);
+      const float lm = anchor(l.m);
+      pairs([&](const Pair& p, int j) { if (first(p, j)) l.s += ex2((p.z - lm) * k); });
+      l.s = group_sum<G>(l.s);
     }
-    u.s = group_sum<G>(u.s);
-    if (a.rest) l.s = group_sum<G>(l.s);
-    const RowSums s(u, l, a.rest, k);
+    const RowSums s(u, l, rest, k);
     if (s.empty) w = 0.f;
-    float q_norm = 0.f;
-    if (!a.rest) {
+    float q0 = 0.f, qi = 1.f;   // q_j = exp(v_j - q0) qi
+    if (!rest) {
       float qs = 0.f;
-      for (int j = x.lane; j < a.K; j += G) {
-        const float v = teacher_logp(a, r * a.K + j);
-        if (teacher_class(a, r * a.K + j, v) >= 0) qs += expf(v - qm);
-      }
-      q_norm = qm + logf(group_sum<G>(qs));
+      q0 = anchor(group_max<G>(qm));
+      pairs([&](const Pair& p, int) { qs += prob(p.v - q0); });
+      qi = 1.f / group_sum<G>(qs);
     }
-    // the pairs, one a lane
-    float sum_q = 0.f, loss = 0.f;
-    if (!BWD || a.rest) {
-      for (int j = x.lane; j < a.K; j += G) {
-        const float v = teacher_logp(a, r * a.K + j);
-        const int c = teacher_class(a, r * a.K + j, v);
-        if (c < 0) continue;
-        const float ln_q = v - q_norm, q = expf(ln_q);
-        sum_q += q;
-        if (!BWD && !(q == 0.f)) loss += q * (ln_q - ((Elem<T>::to_f(row[c * sc]) - s.m) * a.inv_t - s.ln_s));
-      }
+    float sum_q = 1.f, qr = 0.f;
+    if (rest) {
+      sum_q = 0.f;
+      pairs([&](const Pair& p, int) { sum_q += prob(p.v); });
       sum_q = group_sum<G>(sum_q);
+      qr = rest_mass(sum_q);
     }
-    const float qr = a.rest ? rest_mass(sum_q) : 0.f;
-    if (!BWD) {
+    if constexpr (!BWD) {
+      const float c0 = kLn2 * (__log2f(qi) + __log2f(s.s)) - q0;
+      float loss = 0.f;
+      pairs([&](const Pair& p, int) {
+        const float q = prob(p.v - q0) * qi;
+        if (!(q == 0.f)) loss += q * (p.v + c0 - (p.z - s.m) * a.inv_t);
+      });
       loss = group_sum<G>(loss) + rest_loss(qr, s, a.inv_t);
-      if (in && x.lane == 0) {
+      if (in && lane == 0) {
         loss = w == 0.f ? 0.f : w * a.temp * a.temp * loss;
         if (a.row_loss) a.row_loss[r] = loss;
         sum_loss += loss;
         sum_w += w;
       }
     } else {
-      const float scale = w == 0.f ? 0.f : grad_scale(a, r, w), mass = a.rest ? sum_q + qr : 1.f;
-      const float coef = a.rest ? rest_coef(mass, qr, s.mr, s.ln_sr, s.m, s.ln_s, a.inv_t) : mass;
-      T* out = staged ? row : static_cast<T*>(a.dz) + a.dv.base(r);
-      float g[E];
+      const float scale = w == 0.f ? 0.f : grad_scale(a, r, w), mass = rest ? sum_q + qr : 1.f;
+      const float coef = w == 0.f ? 0.f : scale * rest_coef(rest, mass, qr, s.m, s.s, s.mr, s.sr, k);
+      const float2 m2 = {-s.mr, -s.mr}, k2 = {k, k}, c2 = {coef, coef};
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float p = coef * ex2(((x.v[e] - s.mr) * a.inv_t - s.ln_sr) * kLog2e);
-        // masked classes of a row whose unlisted classes are all masked: 0, not 0 * inf
-        g[e] = w == 0.f || x.v[e] == -INFINITY ? 0.f : scale * p;
+      for (int e = 0; e < E; e += 2) {
+        const float2 t = __fmul2_rn(__fadd2_rn(make_float2(x.v[e], x.v[e + 1]), m2), k2);
+        const float2 g = __fmul2_rn(make_float2(ex2(t.x), ex2(t.y)), c2);
+        x.v[e] = w == 0.f ? 0.f : g.x;
+        x.v[e + 1] = w == 0.f ? 0.f : g.y;
       }
-      // the listed classes keep their logits until the lanes of the pairs have read them
-      if (in) x.store(out, a.dv.sc, staged, g, w == 0.f ? x.live : x.live & ~listed);
+      if (in) x.store(x.v);
+      __syncwarp();
       if (in && w != 0.f) {
-        for (int j = x.lane; j < a.K; j += G) {
-          const float v = teacher_logp(a, r * a.K + j);
-          const int c = teacher_class(a, r * a.K + j, v);
-          if (c < 0) continue;
-          float q = expf(v - q_norm);
-          if (twice) {   // a class listed again: its first pair writes, with all its q
-            bool first = true;
+        const float mass_s = mass / s.s;
+        pairs([&](const Pair& p, int j) {
+          float q = prob(p.v - q0) * qi;
+          if (twice) {   // the class's first pair writes, with all its q
+            if (!first(p, j)) return;
             q = 0.f;
             for (int i = 0; i < a.K; ++i) {
-              const float vi = teacher_logp(a, r * a.K + i);
-              if (teacher_class(a, r * a.K + i, vi) != c) continue;
-              if (i < j) first = false;
-              q += expf(vi - q_norm);
+              const Pair o = read(i);
+              if (o.c == p.c) q += prob(o.v - q0) * qi;
             }
-            if (!first) continue;
           }
-          const float p = ex2(((Elem<T>::to_f(row[c * sc]) - s.m) * a.inv_t - s.ln_s) * kLog2e);
-          out[c * (staged ? 1 : a.dv.sc)] = Elem<T>::from_f(scale * (mass * p - q));
-        }
+          sh_put<T>(row + p.c * ES, scale * (mass_s * prob((p.z - s.m) * a.inv_t) - q));
+        });
       }
     }
   });
@@ -241,6 +291,20 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
 }
 
 // ---- rows streamed -----------------------------------------------------------
+// -inf in the places of a vector whose bit is set.
+template <typename T>
+__device__ __forceinline__ uint4 mask_vec(uint4 w, uint32_t bits) {
+  constexpr int n = Word<T>::kElems;
+  uint32_t* p = &w.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = bits >> (i * n);
+    const uint32_t m = n == 1 ? (b & 1 ? ~0u : 0u) : (b & 1 ? 0xffffu : 0u) | (b & 2 ? 0xffff0000u : 0u);
+    p[i] = (p[i] & ~m) | (Word<T>::kNegInf & m);
+  }
+  return w;
+}
+
 // One block (or cluster) per row. The listed classes are marked by a bit each
 // (a byte per vector) in shared memory, so that the streaming loop leaves
 // them out at the price of one byte load per vector; their own sum comes from
@@ -252,7 +316,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
   __shared__ Run runs[NT / 32];
   __shared__ Run mine;
   __shared__ int idx[R4C_TOPK_MAX];
-  __shared__ float lq[R4C_TOPK_MAX];
   const int tid = threadIdx.x;
   uint32_t cs = 1, cr = 0;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cs));
@@ -277,7 +340,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
       v = teacher_logp(a, r * a.K + tid);
       c = teacher_class(a, r * a.K + tid, v);
       idx[tid] = c;
-      lq[tid] = v;
     }
     const bool any = __syncthreads_or(c >= 0);
     if (!any || w == 0.f) {   // the same for all blocks of the cluster
@@ -304,38 +366,47 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
       }
     }
     __syncthreads();
-    Run run = run_empty();
-    for (int q = f0 + tid; q < f1; q += U * NT) {
+    Run2 part = run2_empty();
+    int at = f0 + tid;
+    const uint4* p = x.p + at;
+    const uint8_t* mk = marks + (at - v0);
+    for (; at + (U - 1) * NT < f1; at += U * NT, p += U * NT, mk += U * NT) {
       uint4 y4[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (q + i * NT < f1) y4[i] = __ldg(x.p + q + i * NT);
+      for (int i = 0; i < U; ++i) y4[i] = __ldg(p + i * NT);
+      if (a.rest) {
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+          if (const uint32_t b = mk[i * NT]) y4[i] = mask_vec<T>(y4[i], b);
+      }
+      float vm = Vec<T>::top(y4[0]);
+#pragma unroll
+      for (int i = 1; i < U; ++i) vm = fmaxf(vm, Vec<T>::top(y4[i]));
+      run2_raise<false>(part, vm, k);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        if (q + i * NT < f1) {
-          float y[VE];
-          Vec<T>::split(y4[i], y);
-          if (a.rest) {
-            const uint32_t b = marks[q + i * NT - v0];
-            if (b) {
-#pragma unroll
-              for (int j = 0; j < VE; ++j)
-                if (b >> j & 1) y[j] = -INFINITY;
-            }
-          }
-          run_add<VE, false>(run, y, k);
-        }
+        float y[VE];
+        Vec<T>::split(y4[i], y);
+        run2_add<VE, false>(part, y, k);
       }
+    }
+    for (; at < f1; at += NT, p += NT, mk += NT) {
+      uint4 y4 = __ldg(p);
+      if (a.rest)
+        if (const uint32_t b = *mk) y4 = mask_vec<T>(y4, b);
+      run2_raise<false>(part, Vec<T>::top(y4), k);
+      float y[VE];
+      Vec<T>::split(y4, y);
+      run2_add<VE, false>(part, y, k);
     }
     auto edge = [&](int vec, int j) {   // one element of a partial vector
       const int e = x.cls(vec) + j;
-      float y = e >= 0 && e < a.C ? Elem<T>::to_f(x.row[e]) : -INFINITY;
-      if (a.rest && (marks[vec - v0] >> j & 1)) y = -INFINITY;
-      run_add<1, false>(run, &y, k);
+      if (e >= 0 && e < a.C && !(a.rest && (marks[vec - v0] >> j & 1)))
+        run2_one<false>(part, Elem<T>::to_f(x.row[e]), k);
     };
     if (f0 > v0 && tid < VE) edge(v0, tid);
     if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) edge(f1, tid - 32);
-    run = run_block<NT>(run, k, runs);
+    Run run = run_block<NT>(part.join(), k, runs);
     if (mark >= 0) reinterpret_cast<uint32_t*>(marks)[mark >> 5] = 0;
     if (cs > 1) {
       if (tid == 0) mine = run;
@@ -350,16 +421,16 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
       if (a.rest) l = run_block<NT>(l, k, runs);
       const RowSums s(run, l, a.rest, k);
       // renormalised: ln sum exp(v) of the pairs, by the same joining
-      float q_norm = 0.f;
+      float q0 = 0.f, qs = 1.f;
       if (!a.rest) {
         const Run q = run_block<NT>(Run{c >= 0 ? v : -INFINITY, c >= 0 ? 1.f : 0.f, 0.f}, kLog2e, runs);
-        q_norm = q.m + logf(q.s);
+        q0 = q.m;
+        qs = q.s;
       }
       float q = 0.f, loss = 0.f;
       if (c >= 0) {
-        const float ln_q = v - q_norm;
-        q = expf(ln_q);
-        if (!(q == 0.f)) loss = q * (ln_q - ((zc - s.m) * a.inv_t - s.ln_s));
+        q = prob(v - q0) / qs;
+        if (!(q == 0.f)) loss = q * ((v - q0) - kLn2 * log2f(qs) - (zc - s.m) * a.inv_t + kLn2 * log2f(s.s));
       }
       __syncthreads();
       // (the sums of K <= 128 numbers: the first four warps hold them)
@@ -380,7 +451,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
         if (a.row_loss) a.row_loss[r] = loss;
         sum_loss += loss;
         sum_w += w;
-        a.stats[r] = {s.m, s.ln_s, s.mr, s.ln_sr, q_norm, a.rest ? sum_q + qr : 1.f, qr, w};
+        a.stats[r] = {s.m, s.s, s.mr, s.sr, q0, qs, a.rest ? sum_q + qr : 1.f, qr, w};
       }
     }
     if (cs > 1) cluster_sync();
@@ -390,76 +461,44 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
 }
 
 // One block per piece of a row; the listed classes are written over at the end.
-constexpr int kBwdThreads = 256, kBwdVecs = 4;
 template <typename T>
-__global__ void __launch_bounds__(kBwdThreads) bwd_block_kernel(Args a) {
-  constexpr int VE = Vec<T>::kElems;
+__global__ void __launch_bounds__(kGradThreads) bwd_block_kernel(Args a) {
   __shared__ int idx[R4C_TOPK_MAX];
-  __shared__ float lq[R4C_TOPK_MAX];
+  __shared__ float qj[R4C_TOPK_MAX];
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x / a.segs;
-  const int seg = blockIdx.x % a.segs;
-  const VecRow<T> x(static_cast<const T*>(a.z) + a.v.base(r), a.C);
-  const VecRow<T> y(static_cast<T*>(a.dz) + a.dv.base(r), a.C);
-  uint4* out = const_cast<uint4*>(y.p);
-  T* out_row = const_cast<T*>(y.row);
-  const bool same = x.off == y.off;   // both rows break into vectors at the same classes
-  const int v0 = seg * kBwdThreads * kBwdVecs, v1 = min(v0 + kBwdThreads * kBwdVecs, x.nv);
-  uint4 z4[kBwdVecs];
-#pragma unroll
-  for (int i = 0; i < kBwdVecs; ++i) {
-    const int v = v0 + tid + i * kBwdThreads;
-    if (v < v1 && v >= x.first_full() && v < x.end_full()) z4[i] = __ldg(x.p + v);
-  }
+  T* dz = static_cast<T*>(a.dz) + a.dv.base(r);
+  GradPiece<T> piece(static_cast<const T*>(a.z) + a.v.base(r), dz, a.C, blockIdx.x % a.segs, a.segs);
   const Stats st = a.stats[r];
-  const bool part = st.w != 0.f;
+  if (st.w == 0.f) {
+    piece.write([](float2) { return make_float2(0.f, 0.f); });
+    return;
+  }
   int c = -1;
-  if (part && tid < a.K) {
+  if (tid < a.K) {
     const float v = teacher_logp(a, r * a.K + tid);
     c = teacher_class(a, r * a.K + tid, v);
     idx[tid] = c;
-    lq[tid] = v - st.q_norm;
+    qj[tid] = c < 0 ? 0.f : prob(v - st.qm) / st.qs;
   }
-  const float scale = part ? grad_scale(a, r, st.w) : 0.f;
-  const float base = a.rest ? st.mr : st.m, ln_b = a.rest ? st.ln_sr : st.ln_s;
-  const float coef = scale * (a.rest ? rest_coef(st.mass, st.q_rest, st.mr, st.ln_sr, st.m, st.ln_s, a.inv_t) : st.mass);
-  auto grad = [&](float z) {
-    const float g = coef * ex2(((z - base) * a.inv_t - ln_b) * kLog2e);
-    return !part || z == -INFINITY ? 0.f : g;
-  };
-#pragma unroll
-  for (int i = 0; i < kBwdVecs; ++i) {
-    const int v = v0 + tid + i * kBwdThreads;
-    if (v >= v1) continue;
-    const int c0 = x.cls(v);
-    if (v >= x.first_full() && v < x.end_full()) {
-      float g[VE];
-      Vec<T>::split(z4[i], g);
-#pragma unroll
-      for (int j = 0; j < VE; ++j) g[j] = grad(g[j]);
-      if (same) out[v] = Vec<T>::join(g);
-      else
-        for (int j = 0; j < VE; ++j) out_row[c0 + j] = Elem<T>::from_f(g[j]);
-    } else {
-      for (int j = 0; j < VE; ++j)
-        if (c0 + j >= 0 && c0 + j < a.C) out_row[c0 + j] = Elem<T>::from_f(grad(Elem<T>::to_f(x.row[c0 + j])));
-    }
-  }
-  if (!part) return;
+  const float k = a.inv_t * kLog2e, scale = grad_scale(a, r, st.w), mr = a.rest ? st.mr : st.m;
+  const float coef = scale * rest_coef(a.rest, st.mass, st.q_rest, st.m, st.s, st.mr, st.sr, k);
+  const float2 m2 = {-mr, -mr}, k2 = {k, k}, c2 = {coef, coef};
+  piece.write([&](float2 z) {
+    const float2 t = __fmul2_rn(__fadd2_rn(z, m2), k2);
+    return __fmul2_rn(make_float2(ex2(t.x), ex2(t.y)), c2);
+  });
   __syncthreads();   // the block's own stores come before these
-  if (c >= 0) {
-    const int vec = (c + x.off) / VE;
-    if (vec >= v0 && vec < v1) {
-      float q = 0.f;
-      bool first = true;
-      for (int i = 0; i < a.K; ++i) {
-        if (idx[i] != c) continue;
-        if (i < tid) first = false;
-        q += expf(lq[i]);
-      }
-      const float p = ex2(((Elem<T>::to_f(x.row[c]) - st.m) * a.inv_t - st.ln_s) * kLog2e);
-      if (first) out_row[c] = Elem<T>::from_f(scale * (st.mass * p - q));
+  if (c >= 0 && piece.has(c)) {
+    float q = 0.f;
+    bool first = true;
+    for (int i = 0; i < a.K; ++i) {
+      if (idx[i] != c) continue;
+      if (i < tid) first = false;
+      q += qj[i];
     }
+    const float p = prob((Elem<T>::to_f(piece.x.row[c]) - st.m) * a.inv_t) / st.s;
+    if (first) dz[c] = Elem<T>::from_f(scale * (st.mass * p - q));
   }
 }
 
@@ -491,19 +530,13 @@ __global__ void __launch_bounds__(kMeanThreads) mean_kernel(const double* part, 
 // ---- launches ----------------------------------------------------------------
 template <typename T, bool BWD>
 cudaError_t launch_tiles(Args& a, int* blocks, cudaStream_t s) {
-  const TileKind kind = tile_kind(a.C);
-  r4c_rows_desc d{};
-  d.rows = a.nrows;
-  d.classes = a.C;
-  const bool dense = dense_rows(a.v, a.nrows, a.C, a.z) && (!BWD || dense_rows(a.dv, a.nrows, a.C, a.dz));
-  a.tile = make_tile(&d, sizeof(T), kind.g, dense);
-  *blocks = tile_grid(a.tile, kTileThreads / kind.g);
-#define R4C_TILE(G, E) \
-  if (kind.g == G && kind.e == E) return launch_tile(tile_kernel<T, G, E, BWD>, a.tile, kTileThreads / G, s, a);
-  R4C_TILE(1, 4) R4C_TILE(1, 8) R4C_TILE(1, 16) R4C_TILE(1, 32) R4C_TILE(4, 16) R4C_TILE(8, 16) R4C_TILE(16, 16)
-  R4C_TILE(32, 16) R4C_TILE(32, 32)
-#undef R4C_TILE
-  return cudaErrorInvalidValue;
+  const TileKind kind = tile_kind(a.C, sizeof(T));
+  a.tile = make_tile(a.nrows, a.C, sizeof(T), kind.g,
+                     dense_rows(a.v, a.nrows, a.C, a.z) && (!BWD || dense_rows(a.dv, a.nrows, a.C, a.dz)));
+  *blocks = tile_grid(a.tile);
+  return for_tile_kind<T>(kind, [&](auto c) {
+    return launch_tile(tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::VEC, BWD>, a.tile, s, a);
+  });
 }
 
 // Shared memory for the marks of a block's share of the vectors.
@@ -517,7 +550,7 @@ template <typename T, int NT>
 cudaError_t launch_fwd_block(const Args& a, int* blocks, cudaStream_t s) {
   int cs = cluster_size(a.nrows, a.C, sizeof(T), NT);
   while (a.rest && cs < 16 && mark_bytes<T>(a.C, cs) > kMostMarks) cs *= 2;
-  const int64_t most = (int64_t)kSMs * (2048 / NT) / cs * cs;
+  const int64_t most = (int64_t)kSMs * (1024 / NT) / cs * cs;
   int64_t grid = a.nrows * cs;
   if (grid > most) grid = most;
   *blocks = (int)grid;
@@ -528,15 +561,15 @@ template <typename T>
 cudaError_t launch_fwd(Args& a, int* blocks, cudaStream_t s) {
   if (a.C <= kTileClasses) return launch_tiles<T, false>(a, blocks, s);
   if ((int64_t)a.C * sizeof(T) <= 16 << 10) return launch_fwd_block<T, 128>(a, blocks, s);
-  return launch_fwd_block<T, 512>(a, blocks, s);
+  return launch_fwd_block<T, 256>(a, blocks, s);
 }
 template <typename T>
 cudaError_t launch_bwd(Args& a, cudaStream_t s) {
   int blocks;
   if (a.C <= kTileClasses) return launch_tiles<T, true>(a, &blocks, s);
-  a.segs = (a.C / Vec<T>::kElems + 2 + kBwdThreads * kBwdVecs - 1) / (kBwdThreads * kBwdVecs);
+  a.segs = grad_pieces(a.C, sizeof(T));
   if (a.nrows * a.segs > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  bwd_block_kernel<T><<<(unsigned)(a.nrows * a.segs), kBwdThreads, 0, s>>>(a);
+  bwd_block_kernel<T><<<(unsigned)(a.nrows * a.segs), kGradThreads, 0, s>>>(a);
   return cudaGetLastError();
 }
 

@@ -22,11 +22,11 @@ struct FwdArgs {
   int64_t ignore, nrows;
   View v;
   Tile tile;
-  int C, K;
+  int C, K, pairs;   // pairs: K = 2 and the outputs 8-byte aligned
   float inv_t;
   float *logp, *entropy, *lse, *top_logp;
   int32_t* top_index;
-  float2* stats;
+  float2* stats;      // (max z, S) of streamed rows
   int* err;
 };
 
@@ -58,114 +58,153 @@ __device__ __forceinline__ int label_of(const int64_t* target, int64_t r, int C,
   return (int)t;
 }
 
-struct RowOut {   // what a row's sums say; bad: NaN or +inf in the row
-  float mm, ln_s, inv_t;
+// What a row's sums say; bad: NaN or +inf in the row, empty: no finite logit.
+struct RowOut {
+  float mm, l2s, inv_t;
   bool bad, empty;
-  __device__ __forceinline__ RowOut(const Run& r, float it) : mm(anchor(r.m)), inv_t(it), bad(isnan(r.s)), empty(r.s == 0.f) {
-    ln_s = empty ? -INFINITY : logf(r.s);
-  }
-  __device__ __forceinline__ float logp(float z) const { return empty ? -INFINITY : (z - mm) * inv_t - ln_s; }
-  __device__ __forceinline__ float entropy(const Run& r) const { return empty ? 0.f : ln_s - inv_t * (r.u / r.s); }
-  __device__ __forceinline__ float lse() const { return mm * inv_t + ln_s; }
+  __device__ __forceinline__ RowOut(const Run& r, float log2_s, float it)
+      : mm(anchor(r.m)), l2s(log2_s), inv_t(it), bad(isnan(r.s)), empty(r.s == 0.f) {}
+  __device__ __forceinline__ float logp(float z) const { return empty ? -INFINITY : fmaf(z - mm, inv_t, -kLn2 * l2s); }
+  __device__ __forceinline__ float entropy(const Run& r) const { return empty ? 0.f : kLn2 * (l2s - __fdividef(r.u, r.s)); }
+  __device__ __forceinline__ float lse() const { return fmaf(mm, inv_t, kLn2 * l2s); }
 };
 
 // ---- rows in registers -------------------------------------------------------
-template <typename T, int G, int E>
-__device__ __forceinline__ Run row_run(const TileRow<T, G, E>& x, float k) {
-  Run r = run_empty();
-#pragma unroll
-  for (int e = 0; e < E; ++e) r.m = fmaxf(r.m, x.v[e]);
-  r.m = group_max<G>(r.m);
-  const float mm = anchor(r.m);
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float d = x.v[e] - mm, p = ex2(d * k);   // a place outside the row holds -inf: adds nothing
-    r.s += p;
-    r.u = fmaf(p, fmaxf(d, -1e30f), r.u);
-  }
+template <typename Row>
+__device__ __forceinline__ Run row_run(const Row& x, float k) {
+  Run2 r = run2_empty();
+  r.m = x.max();
+  run2_add<sizeof(x.v) / sizeof(float), true>(r, x.v, k);   // places outside the row hold -inf and add nothing
+  return r.join();
+}
+template <int G>
+__device__ __forceinline__ void run_group(Run& r) {
   r.s = group_sum<G>(r.s);
   r.u = group_sum<G>(r.u);
-  return r;
 }
 
-template <typename T, int G, int E>
+// Keys that order a row's values, equal ones by lowest class; the least is no
+// class. 16-bit types: 19 bits of the value hold it exactly, 13 the class.
+template <typename T> struct TopKey {
+  using type = int;
+  static constexpr int kNone = (int)0x80000000;
+  static __device__ __forceinline__ int make(float v, int c) {
+    const int b = __float_as_int(v + 0.f);
+    return ((b ^ ((b >> 31) & 0x7fffffff)) & ~0x1fff) | (0x1fff - c);
+  }
+  static __device__ __forceinline__ int cls(int k) { return 0x1fff - (k & 0x1fff); }
+  static __device__ __forceinline__ float value(int k) {
+    const int o = (k & ~0x1fff) | (k < 0 ? 0x1fff : 0);
+    return __int_as_float(o ^ ((o >> 31) & 0x7fffffff));
+  }
+};
+template <> struct TopKey<float> {
+  using type = long long;
+  static constexpr long long kNone = (long long)0x8000000000000000ull;
+  static __device__ __forceinline__ long long make(float v, int c) { return (long long)(rank_key(v, c) ^ 0x8000000000000000ull); }
+  static __device__ __forceinline__ int cls(long long k) { return key_class((uint64_t)k); }
+  static __device__ __forceinline__ float value(long long k) { return key_value((uint64_t)k ^ 0x8000000000000000ull); }
+};
+
+template <typename T, int G, int E, bool VEC>
 __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
   const float k = a.inv_t * kLog2e;
-  tile_walk<T, G, false>(a.tile, a.z, a.v, nullptr, [&](int64_t r, T* row, bool in) {
-    TileRow<T, G, E> x;
-    const bool staged = a.tile.staged;
-    x.load(row, a.v.sc, a.C, staged);
-    const Run run = row_run(x, k);
-    const RowOut o(run, a.inv_t);
+  tile_walk<T, G, false>(a.tile, a.v, a.z, a.v, nullptr, [&](int64_t r, uint32_t row, bool in) {
+    TileRow<T, G, E, VEC> x;
+    x.load(row, a.C);
+    Run run = row_run(x, k);
+    run_group<G>(run);
+    const RowOut o(run, __log2f(run.s), a.inv_t);
     if (in && x.lane == 0) {
       if (a.target) {
         const int t = label_of(a.target, r, a.C, a.ignore, a.err);
-        a.logp[r] = t < 0 ? 0.f : o.logp(Elem<T>::to_f(row[staged ? t : t * a.v.sc]));
+        a.logp[r] = t < 0 ? 0.f : o.logp(sh_get<T>(row + t * (int)sizeof(T)));
       }
       a.entropy[r] = o.entropy(run);
       a.lse[r] = o.lse();
     }
-    // the most probable classes, one after the other: lanes offer their best
-    // value that is not taken (ties: lowest class)
-    uint32_t open = x.live;
+    if (a.K == 0) return;
+    // the most probable classes, one after the other
+    using Key = TopKey<T>;
+    typename Key::type key[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) key[e] = x.ok(e) ? Key::make(x.v[e], x.cls(e)) : Key::kNone;
+    float* tl = a.top_logp + r * a.K;
+    int32_t* ti = a.top_index + r * a.K;
+    auto next = [&](float* l, int* c) {
+      typename Key::type b = key[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) b = key[e] > b ? key[e] : b;
+#pragma unroll
+      for (int q = G / 2; q; q >>= 1) {
+        const typename Key::type w = __shfl_xor_sync(0xffffffffu, b, q);
+        b = w > b ? w : b;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) key[e] = key[e] == b ? Key::kNone : key[e];
+      *l = o.bad ? NAN : o.logp(Key::value(b));
+      *c = o.bad ? -1 : Key::cls(b);
+    };
+    if (G == 1 && a.pairs) {   // two alternatives are stored whole: half-written sectors cost twice
+      float2 l;
+      int2 c;
+      next(&l.x, &c.x);
+      next(&l.y, &c.y);
+      if (in) {
+        *reinterpret_cast<float2*>(tl) = l;
+        *reinterpret_cast<int2*>(ti) = c;
+      }
+      return;
+    }
     for (int j = 0; j < a.K; ++j) {
-      float b = -INFINITY;
-      int bc = 0x7fffffff, be = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int c = x.cls(e);
-        if ((open >> e & 1) && (x.v[e] > b || (x.v[e] == b && c < bc))) {
-          b = x.v[e];
-          bc = c;
-          be = e;
-        }
-      }
-      const int mine = bc;
-#pragma unroll
-      for (int off = G / 2; off; off >>= 1) {
-        const float ob = __shfl_xor_sync(0xffffffffu, b, off);
-        const int oc = __shfl_xor_sync(0xffffffffu, bc, off);
-        if (ob > b || (ob == b && oc < bc)) {
-          b = ob;
-          bc = oc;
-        }
-      }
-      if (mine == bc) open &= ~(1u << be);
+      float l;
+      int c;
+      next(&l, &c);
       if (in && x.lane == 0) {
-        a.top_logp[r * a.K + j] = o.bad ? NAN : o.logp(b);
-        a.top_index[r * a.K + j] = o.bad ? -1 : bc;
+        tl[j] = l;
+        ti[j] = c;
       }
     }
   });
 }
 
-template <typename T, int G, int E>
+template <typename T, int G, int E, bool VEC>
 __global__ void __launch_bounds__(kTileThreads) bwd_tile_kernel(BwdArgs a) {
   const float k = a.inv_t * kLog2e;
-  tile_walk<T, G, true>(a.tile, a.z, a.v, a.dz, [&](int64_t r, T* row, bool in) {
-    TileRow<T, G, E> x;
-    const bool staged = a.tile.staged;
-    x.load(row, a.v.sc, a.C, staged);
+  tile_walk<T, G, true>(a.tile, a.v, a.z, a.dv, a.dz, [&](int64_t r, uint32_t row, bool in) {
+    TileRow<T, G, E, VEC> x;
+    x.load(row, a.C);
     const int t = label_of(a.target, r, a.C, a.ignore, a.err);
     const float gl = a.g_logp && t >= 0 ? a.g_logp[r * a.gl_inc] : 0.f;
     const float gh = a.g_entropy ? a.g_entropy[r * a.gh_inc] : 0.f;
     const float gs = a.g_lse ? a.g_lse[r * a.gs_inc] : 0.f;
-    const Run run = row_run(x, k);
-    const RowOut o(run, a.inv_t);
-    const bool none = (gl == 0.f && gh == 0.f && gs == 0.f) || o.empty;
-    const float ca = a.inv_t * (gs - gl - gh * o.entropy(run)), cb = a.inv_t * gh;
-    float g[E];
+    Run run = row_run(x, k);
+    run_group<G>(run);
+    const float l2s = __log2f(run.s);
+    const bool none = (gl == 0.f && gh == 0.f && gs == 0.f) || run.s == 0.f;
+    const float h = kLn2 * (l2s - __fdividef(run.u, run.s));
+    const float f = none ? 0.f : __fdividef(a.inv_t, run.s), ca = f * (gs - gl - gh * h), cb = f * gh * kLn2;
+    const float mm = -anchor(run.m), lb = cb * l2s;
+    const float2 m2 = {mm, mm}, k2 = {k, k};
+    // 2^t (ca - cb (t - l2s))
+    const float c0 = none ? 0.f : ca + lb;
+    const float2 c2 = {c0, c0}, b2 = {none ? 0.f : -cb, none ? 0.f : -cb};
+    float zt = 0.f;
+    if (t >= 0) zt = sh_get<T>(row + t * (int)sizeof(T));
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float ln_p = fmaxf((x.v[e] - o.mm) * a.inv_t, -1e30f) - o.ln_s;
-      g[e] = ex2(ln_p * kLog2e) * (ca - cb * ln_p);
-      if (x.cls(e) == t) g[e] += a.inv_t * gl;
-      if (none) g[e] = 0.f;
-      else if (o.bad) g[e] = NAN;
+    for (int e = 0; e < E; e += 2) {
+      float2 q = __fmul2_rn(__fadd2_rn(make_float2(x.v[e], x.v[e + 1]), m2), k2);
+      q = make_float2(max_nan(q.x, kFloor), max_nan(q.y, kFloor));
+      q = __fmul2_rn(make_float2(ex2(q.x), ex2(q.y)), __ffma2_rn(b2, q, c2));
+      x.v[e] = q.x;
+      x.v[e + 1] = q.y;
     }
-    if (in) {
-      T* out = staged ? row : static_cast<T*>(a.dz) + a.dv.base(r);
-      x.store(out, a.dv.sc, staged, g, x.live);
+    if (G > 1) __syncwarp();   // every lane has read the row (and the label's logit)
+    if (in) x.store(x.v);
+    if (G > 1) __syncwarp();
+    if (in && t >= 0 && x.lane == 0 && !none) {
+      const float q = max_nan((zt + mm) * k, kFloor);
+      sh_put<T>(row + t * (int)sizeof(T), fmaf(a.inv_t, gl, ex2(q) * fmaf(-cb, q, c0)));
     }
   });
 }
@@ -326,43 +365,46 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
     const int per = (x.nv + (int)cs - 1) / (int)cs;
     const int v0 = min((int)cr * per, x.nv), v1 = min(v0 + per, x.nv);
     const int f0 = max(v0, x.first_full()), f1 = min(v1, x.end_full());
-    Run run = run_empty();
+    Run2 part = run2_empty();
     float tm = 0.f;   // the largest value of this thread's full vectors, and the first vector that has it
     int tv = -1;
-    for (int v = f0 + tid; v < f1; v += U * NT) {
+    auto track = [&](float vm, int v) {
+      if (TOP && (tv < 0 || vm > tm)) {
+        tm = vm;
+        tv = v;
+      }
+    };
+    int v = f0 + tid;
+    const uint4* p = x.p + v;
+    for (; v + (U - 1) * NT < f1; v += U * NT, p += U * NT) {
       uint4 w[U];
+      float vm[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (v + i * NT < f1) w[i] = __ldg(x.p + v + i * NT);
+      for (int i = 0; i < U; ++i) w[i] = __ldg(p + i * NT);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        if (v + i * NT < f1) {
-          float y[VE];
-          Vec<T>::split(w[i], y);
-          run_add<VE, true>(run, y, k);
-          if (TOP) {
-            float vm = y[0];
-#pragma unroll
-            for (int j = 1; j < VE; ++j) vm = fmaxf(vm, y[j]);
-            if (tv < 0 || vm > tm) {
-              tm = vm;
-              tv = v + i * NT;
-            }
-          }
-        }
+        vm[i] = Vec<T>::top(w[i]);
+        track(vm[i], v + i * NT);
       }
+      run2_raise<true>(part, fmaxf(fmaxf(vm[0], vm[1]), fmaxf(vm[2], vm[3])), k);
+      run2_batch<VE, U>(part, k, [&](int i, float* y) { Vec<T>::split(i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3], y); });
+    }
+    for (; v < f1; v += NT, p += NT) {
+      const uint4 w = __ldg(p);
+      const float vm = Vec<T>::top(w);
+      track(vm, v);
+      run2_raise<true>(part, vm, k);
+      run2_batch<VE, 1>(part, k, [&](int, float* y) { Vec<T>::split(w, y); });
     }
     if (f0 > v0 && tid < VE) {   // partial vectors: one element a thread
       const int c = x.cls(v0) + tid;
-      const float y = c >= 0 && c < a.C ? Elem<T>::to_f(x.row[c]) : -INFINITY;
-      run_add<1, true>(run, &y, k);
+      if (c >= 0 && c < a.C) run2_one<true>(part, Elem<T>::to_f(x.row[c]), k);
     }
     if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) {
       const int c = x.cls(f1) + tid - 32;
-      const float y = c >= 0 && c < a.C ? Elem<T>::to_f(x.row[c]) : -INFINITY;
-      run_add<1, true>(run, &y, k);
+      if (c >= 0 && c < a.C) run2_one<true>(part, Elem<T>::to_f(x.row[c]), k);
     }
-    run = run_block<NT>(run, k, runs);
+    Run run = run_block<NT>(part.join(), k, runs);
     if (TOP) block_topk<T, NT>(x, v0, v1, f0, f1, tm, tv, a.K, isnan(run.s), top);
     if (cs > 1) {
       if (tid == 0) mine = run;
@@ -378,7 +420,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
       }
     }
     if (cr == 0) {
-      const RowOut o(run, a.inv_t);
+      const RowOut o(run, log2f(run.s), a.inv_t);
       if (tid == 0) {
         if (a.target) {
           const int t = label_of(a.target, r, a.C, a.ignore, a.err);
@@ -386,7 +428,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
         }
         a.entropy[r] = o.entropy(run);
         a.lse[r] = o.lse();
-        if (a.stats) a.stats[r] = make_float2(o.mm, o.ln_s);
+        if (a.stats) a.stats[r] = make_float2(o.mm, run.s);
       }
       if (TOP) {
         for (int i = tid; i < (int)cs * a.K; i += NT) {
@@ -421,76 +463,50 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
 }
 
 // One block per piece of a row.
-constexpr int kBwdThreads = 256, kBwdVecs = 4;
 template <typename T>
-__global__ void __launch_bounds__(kBwdThreads) bwd_block_kernel(BwdArgs a) {
-  constexpr int VE = Vec<T>::kElems;
-  const int tid = threadIdx.x;
+__global__ void __launch_bounds__(kGradThreads) bwd_block_kernel(BwdArgs a) {
   const int64_t r = blockIdx.x / a.segs;
-  const int seg = blockIdx.x % a.segs;
-  const VecRow<T> x(static_cast<const T*>(a.z) + a.v.base(r), a.C);
-  const VecRow<T> y(static_cast<T*>(a.dz) + a.dv.base(r), a.C);
-  uint4* out = const_cast<uint4*>(y.p);
-  T* out_row = const_cast<T*>(y.row);
-  const bool same = x.off == y.off;   // both rows break into vectors at the same classes
-  const int v0 = seg * kBwdThreads * kBwdVecs, v1 = min(v0 + kBwdThreads * kBwdVecs, x.nv);
-  uint4 w[kBwdVecs];
-#pragma unroll
-  for (int i = 0; i < kBwdVecs; ++i) {
-    const int v = v0 + tid + i * kBwdThreads;
-    if (v < v1 && v >= x.first_full() && v < x.end_full()) w[i] = __ldg(x.p + v);
-  }
+  T* dz = static_cast<T*>(a.dz) + a.dv.base(r);
+  GradPiece<T> piece(static_cast<const T*>(a.z) + a.v.base(r), dz, a.C, blockIdx.x % a.segs, a.segs);
   const int t = label_of(a.target, r, a.C, a.ignore, a.err);
   const float gl = a.g_logp && t >= 0 ? a.g_logp[r * a.gl_inc] : 0.f;
   const float gh = a.g_entropy ? a.g_entropy[r * a.gh_inc] : 0.f;
   const float gs = a.g_lse ? a.g_lse[r * a.gs_inc] : 0.f;
   const float2 st = a.stats[r];
-  const bool none = (gl == 0.f && gh == 0.f && gs == 0.f) || st.y == -INFINITY, bad = isnan(st.y);
-  const float ca = a.inv_t * (gs - gl - gh * a.entropy[r]), cb = a.inv_t * gh;
-  auto grad = [&](float z, int c) {
-    const float ln_p = fmaxf((z - st.x) * a.inv_t, -1e30f) - st.y;
-    float g = ex2(ln_p * kLog2e) * (ca - cb * ln_p);
-    if (c == t) g += a.inv_t * gl;
-    return none ? 0.f : bad ? NAN : g;
+  // a row without a finite logit has no gradient; a bad row's is NaN, from its statistics
+  if ((gl == 0.f && gh == 0.f && gs == 0.f) || st.y == 0.f) {
+    piece.write([](float2) { return make_float2(0.f, 0.f); });
+    return;
+  }
+  const float k = a.inv_t * kLog2e, f = a.inv_t / st.y;
+  const float ca = f * (gs - gl - gh * a.entropy[r]), cb = f * gh * kLn2;
+  const float c0 = cb != 0.f ? fmaf(cb, log2f(st.y), ca) : ca;   // p (ca - cb log2 p) as 2^t (c0 - cb t) / S
+  const float2 m2 = {-st.x, -st.x}, k2 = {k, k}, c2 = {c0, c0}, b2 = {-cb, -cb};
+  auto with_entropy = [&](float2 z) {
+    float2 q = __fmul2_rn(__fadd2_rn(z, m2), k2);
+    q = make_float2(max_nan(q.x, kFloor), max_nan(q.y, kFloor));
+    return __fmul2_rn(make_float2(ex2(q.x), ex2(q.y)), __ffma2_rn(b2, q, c2));
   };
-#pragma unroll
-  for (int i = 0; i < kBwdVecs; ++i) {
-    const int v = v0 + tid + i * kBwdThreads;
-    if (v >= v1) continue;
-    const int c0 = x.cls(v);
-    if (v >= x.first_full() && v < x.end_full()) {
-      float g[VE];
-      Vec<T>::split(w[i], g);
-#pragma unroll
-      for (int j = 0; j < VE; ++j) g[j] = grad(g[j], c0 + j);
-      if (same) out[v] = Vec<T>::join(g);
-      else
-        for (int j = 0; j < VE; ++j) out_row[c0 + j] = Elem<T>::from_f(g[j]);
-    } else {
-      for (int j = 0; j < VE; ++j)
-        if (c0 + j >= 0 && c0 + j < a.C) out_row[c0 + j] = Elem<T>::from_f(grad(Elem<T>::to_f(x.row[c0 + j]), c0 + j));
-    }
+  if (cb != 0.f) {
+    piece.write(with_entropy);
+  } else {
+    piece.write([&](float2 z) {
+      const float2 q = __fmul2_rn(__fadd2_rn(z, m2), k2);
+      return __fmul2_rn(make_float2(ex2(q.x), ex2(q.y)), c2);
+    });
+  }
+  if (t >= 0 && piece.has(t)) {   // the label's own term, over what the block has stored
+    __syncthreads();
+    if (threadIdx.x == 0)
+      dz[t] = Elem<T>::from_f(with_entropy(make_float2(Elem<T>::to_f(piece.x.row[t]), 0.f)).x + a.inv_t * gl);
   }
 }
 
 // ---- launches ----------------------------------------------------------------
-template <typename T, bool BWD, typename A>
-cudaError_t launch_tiles(A& a, const TileKind& kind, cudaStream_t s) {
-#define R4C_TILE(G, E)                                                                             \
-  if (kind.g == G && kind.e == E) {                                                                \
-    if constexpr (BWD) return launch_tile(bwd_tile_kernel<T, G, E>, a.tile, kTileThreads / G, s, a); \
-    else return launch_tile(fwd_tile_kernel<T, G, E>, a.tile, kTileThreads / G, s, a);             \
-  }
-  R4C_TILE(1, 4) R4C_TILE(1, 8) R4C_TILE(1, 16) R4C_TILE(1, 32) R4C_TILE(4, 16) R4C_TILE(8, 16) R4C_TILE(16, 16)
-  R4C_TILE(32, 16) R4C_TILE(32, 32)
-#undef R4C_TILE
-  return cudaErrorInvalidValue;
-}
-
 template <typename T, int NT>
 cudaError_t launch_fwd_block(const FwdArgs& a, cudaStream_t s) {
   const int cs = cluster_size(a.nrows, a.C, sizeof(T), NT);
-  const int64_t most = (int64_t)kSMs * (2048 / NT);
+  const int64_t most = (int64_t)kSMs * (1024 / NT);
   int64_t grid = a.nrows * cs;
   if (cs == 1 && grid > most) grid = most;
   if (a.K > 0) {
@@ -503,31 +519,29 @@ cudaError_t launch_fwd_block(const FwdArgs& a, cudaStream_t s) {
 template <typename T>
 cudaError_t launch_fwd(FwdArgs& a, cudaStream_t s) {
   if (a.C <= kTileClasses) {
-    const TileKind kind = tile_kind(a.C);
-    r4c_rows_desc d{};
-    d.rows = a.nrows;
-    d.classes = a.C;
-    a.tile = make_tile(&d, sizeof(T), kind.g, dense_rows(a.v, a.nrows, a.C, a.z));
-    return launch_tiles<T, false>(a, kind, s);
+    const TileKind kind = tile_kind(a.C, sizeof(T));
+    a.tile = make_tile(a.nrows, a.C, sizeof(T), kind.g, dense_rows(a.v, a.nrows, a.C, a.z));
+    return for_tile_kind<T>(kind, [&](auto c) {
+      return launch_tile(fwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::VEC>, a.tile, s, a);
+    });
   }
   if ((int64_t)a.C * sizeof(T) <= 16 << 10) return launch_fwd_block<T, 128>(a, s);
-  return launch_fwd_block<T, 512>(a, s);
+  return launch_fwd_block<T, 256>(a, s);
 }
 
 template <typename T>
 cudaError_t launch_bwd(BwdArgs& a, cudaStream_t s) {
   if (a.C <= kTileClasses) {
-    const TileKind kind = tile_kind(a.C);
-    r4c_rows_desc d{};
-    d.rows = a.nrows;
-    d.classes = a.C;
-    a.tile = make_tile(&d, sizeof(T), kind.g,
+    const TileKind kind = tile_kind(a.C, sizeof(T));
+    a.tile = make_tile(a.nrows, a.C, sizeof(T), kind.g,
                        dense_rows(a.v, a.nrows, a.C, a.z) && dense_rows(a.dv, a.nrows, a.C, a.dz));
-    return launch_tiles<T, true>(a, kind, s);
+    return for_tile_kind<T>(kind, [&](auto c) {
+      return launch_tile(bwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::VEC>, a.tile, s, a);
+    });
   }
-  a.segs = (a.C / Vec<T>::kElems + 2 + kBwdThreads * kBwdVecs - 1) / (kBwdThreads * kBwdVecs);
+  a.segs = grad_pieces(a.C, sizeof(T));
   if (a.nrows * a.segs > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  bwd_block_kernel<T><<<(unsigned)(a.nrows * a.segs), kBwdThreads, 0, s>>>(a);
+  bwd_block_kernel<T><<<(unsigned)(a.nrows * a.segs), kGradThreads, 0, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -561,7 +575,8 @@ extern "C" int r4c_logp_fwd(const r4c_rows_desc* d, const void* logits, const in
   if (!logits || !entropy || !lse || (target && !logp) || (top_k > 0 && (!top_logp || !top_index))) return R4C_ERR_INVALID;
   int* err = tc::device_error_flag();
   if (!err) return R4C_ERR_NO_DEVICE;
-  logp::FwdArgs a{logits, target, ignore_index, d->rows, rows::make_view(d), {}, d->classes, top_k,
+  const int pairs = top_k == 2 && !(((uintptr_t)top_logp | (uintptr_t)top_index) & 7);
+  logp::FwdArgs a{logits, target, ignore_index, d->rows, rows::make_view(d), {}, d->classes, top_k, pairs,
                   1.f / d->temperature, logp, entropy, lse, top_logp, top_index, static_cast<float2*>(stats), err};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;

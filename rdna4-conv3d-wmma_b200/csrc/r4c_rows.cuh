@@ -5,14 +5,19 @@
 // A row is the class axis at one voxel of an (N, C, D, H, W) map or at one
 // token of an (R, C) matrix; r4c_rows_desc gives its place for any strides.
 //
-// * Up to kTileClasses classes ("tile"): G lanes hold a whole row in
-//   registers, so a kernel reads it once whatever it needs of it, and a
-//   backward recomputes the softmax instead of loading saved statistics.
-//   Dense rows come through shared memory: tiles of consecutive rows are one
-//   contiguous piece of memory, copied with 16-byte cp.async whatever the
-//   alignment of each row (105 classes of 2 bytes start on any even byte).
+// * Up to kTileClasses classes ("tile"): rows wait in shared memory and G lanes
+//   take one into registers, so a kernel reads it once whatever it needs of
+//   it, and a backward recomputes the softmax instead of loading saved
+//   statistics. Tiles of dense rows are one contiguous piece of memory, copied
+//   ahead with 16-byte cp.async whatever the alignment of each row (105
+//   classes of 2 bytes start on any even byte); other strides are gathered.
 // * Above ("block"): a block, or a cluster of blocks when there are few rows,
 //   streams over the row in 16-byte loads and keeps a running maximum and sum.
+//
+// These kernels are bound by instruction issue before they are bound by
+// memory: at 6.5 TB/s an SM has about 11 instructions for each 16-bit logit.
+// So the arithmetic is packed (two fp32 a instruction), maxima are taken on
+// packed words, and checks are made per vector or per row, not per element.
 #pragma once
 
 #include <cmath>
@@ -24,6 +29,7 @@ namespace r4c {
 namespace rows {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 // A rest mass 1 - sum(q) below this is the rounding of the teacher's own sum.
 constexpr float kRestNoise = 1e-6f;
 constexpr int kTileClasses = 1024;
@@ -53,6 +59,14 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The larger of two, NaN if either is (fmaxf would drop it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// Exponents below this give 0 whatever they are; bounding them keeps 0 * -inf out of the entropy.
+constexpr float kFloor = -200.f;
 // A maximum that may be -inf as the point that differences are taken from.
 __device__ __forceinline__ float anchor(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -88,15 +102,28 @@ __device__ __forceinline__ bool group_any(bool p) {
   return ((b >> ((threadIdx.x & 31) & ~(G - 1))) & ((1u << (G & 31)) - 1u)) != 0;
 }
 
-// ---- 32-bit words of logits -------------------------------------------------
+// ---- 32-bit words of logits, and their largest value without unpacking them all -------------------------------------------------
 template <typename T> struct Word;
 template <> struct Word<float> {
   static constexpr int kElems = 1;
+  static constexpr uint32_t kNegInf = 0xff800000u;
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float top(uint32_t w) { return __uint_as_float(w); }
   static __device__ __forceinline__ void split(uint32_t w, float* v) { v[0] = __uint_as_float(w); }
   static __device__ __forceinline__ uint32_t join(const float* v) { return __float_as_uint(v[0]); }
 };
 template <> struct Word<__nv_bfloat16> {
   static constexpr int kElems = 2;
+  static constexpr uint32_t kNegInf = 0xff80ff80u;
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+  static __device__ __forceinline__ float top(uint32_t w) {
+    return fmaxf(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
   static __device__ __forceinline__ void split(uint32_t w, float* v) {
     v[0] = __uint_as_float(w << 16);
     v[1] = __uint_as_float(w & 0xffff0000u);
@@ -108,6 +135,15 @@ template <> struct Word<__nv_bfloat16> {
 };
 template <> struct Word<__half> {
   static constexpr int kElems = 2;
+  static constexpr uint32_t kNegInf = 0xfc00fc00u;
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+  static __device__ __forceinline__ float top(uint32_t w) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return fmaxf(f.x, f.y);
+  }
   static __device__ __forceinline__ void split(uint32_t w, float* v) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
     v[0] = f.x;
@@ -120,207 +156,293 @@ template <> struct Word<__half> {
 };
 
 // ---- tile: rows held in registers --------------------------------------------
-// Geometry of a tile launch. `staged`: rows dense and 16-byte aligned as a
-// whole, read (and for a backward written) through shared memory.
+enum { kGather = 0, kCopy = 1, kCopyPadded = 2 };
 struct Tile {
   int64_t nrows, ntiles;
-  int C, rows_per_tile, staged, stage_bytes;
+  int C, stride;          // classes; elements between rows in shared memory
+  int rows, mode;         // rows of a tile; how they come to shared memory
+  int stage_bytes;
+  int chunks;             // kCopyPadded: 16-byte chunks of a row
+  uint32_t recip;         // ... and 2^32 / chunks, rounded up
 };
 constexpr int kTileStages = 3;
 
-// One lane's part of a row: E values, value e = i * kElems + h being class
-// cls(e). Lanes take words cyclically (lane l words l, l + G, ...), each row
-// starting at another one of them (`rot`), so that rows whose width is a
-// multiple of the banks do not meet in the same bank.
-template <typename T, int G, int E>
+// One lane's part of a row: E values in units of a 16-byte vector (VEC: rows
+// are 16-byte aligned) or a 32-bit word, taken cyclically by the lanes, so
+// value e is class c0 + off(e) and classes ascend with e. A row of 2-byte
+// elements may start in the middle of a word: c0 is then one lower (-1 in
+// lane 0: not a class).
+template <typename T, int G, int E, bool VEC>
 struct TileRow {
-  static constexpr int kW = Word<T>::kElems, kEW = E / kW;
+  static constexpr int kW = Word<T>::kElems;
+  static constexpr int kU = VEC ? 16 / (int)sizeof(T) : kW;   // elements of a unit
+  static constexpr int kN = E / kU;                           // units of a lane
   float v[E];
-  uint32_t live;        // bit e: v[e] is a class of the row
-  int lane, rot, odd;   // odd: the row starts at the second half of a word
+  int lane, c0, C;
+  uint32_t at;   // shared address of the lane's first unit
 
-  __device__ __forceinline__ int word(int i) const { return lane + G * ((i + rot) & (kEW - 1)); }
-  __device__ __forceinline__ int cls(int e) const { return kW * word(e / kW) + e % kW - odd; }
-  // Where class c sits: true and its e when this lane holds it.
-  __device__ __forceinline__ bool owns(int c, int* e) const {
-    const int p = c + odd, w = p / kW;
-    *e = (((w / G) - rot) & (kEW - 1)) * kW + p % kW;
-    return w % G == lane;
-  }
-  // row: the row's first element, in shared memory (staged) or global memory.
-  __device__ __forceinline__ void load(const T* row, int64_t sc, int C, bool staged) {
-    const int wl = threadIdx.x & 31;
-    lane = wl & (G - 1);
-    live = 0;
-    if (staged) {
-      const uint32_t a = sm100::smem_u32(row);
-      odd = kW == 2 ? (a >> 1) & 1 : 0;
-      const int nw = (odd + C + kW - 1) / kW;
-      rot = (nw & 1) ? 0 : G == 1 ? wl / (32 / (kEW < 32 ? kEW : 32)) : wl / G;
+  static __device__ __forceinline__ constexpr int off(int e) { return e / kU * (G * kU) + e % kU; }
+  __device__ __forceinline__ int cls(int e) const { return c0 + off(e); }
+  // Units whose elements are classes in every lane of every row (but for the half word before a row).
+  __device__ __forceinline__ bool inner(int i) const { return kU * G * (i + 1) <= C; }
+  __device__ __forceinline__ bool ok(int e) const { return (unsigned)cls(e) < (unsigned)C; }
+
+  __device__ __forceinline__ void load(uint32_t row, int classes) {
+    C = classes;
+    lane = (threadIdx.x & 31) & (G - 1);
+    c0 = kU * lane - (kU == 2 ? (row >> 1) & 1 : 0);
+    at = (kU == 2 ? row & ~3u : row) + lane * (kU * (int)sizeof(T));
 #pragma unroll
-      for (int i = 0; i < kEW; ++i) {
-        const int w = word(i);
-        uint32_t x = 0;
-        if (w < nw) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"((a & ~3u) + 4 * w) : "memory");
-        Word<T>::split(x, v + i * kW);
+    for (int i = 0; i < kN; ++i) {
+      float* x = v + i * kU;
+      const uint32_t a = at + i * (G * kU * (int)sizeof(T));
+      if (VEC) {
+        uint32_t w[4] = {Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf};
+        if (inner(i) || cls(i * kU) < C)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
 #pragma unroll
-        for (int h = 0; h < kW; ++h) {
-          const int c = kW * w + h - odd;
-          const bool ok = c >= 0 && c < C;
-          if (!ok) v[i * kW + h] = -INFINITY;
-          live |= (uint32_t)ok << (i * kW + h);
-        }
-      }
-    } else {
-      odd = rot = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int c = cls(e);
-        const bool ok = c < C;
-        v[e] = ok ? Elem<T>::to_f(row[c * sc]) : -INFINITY;
-        live |= (uint32_t)ok << e;
+        for (int h = 0; h < 4; ++h) Word<T>::split(w[h], x + h * kW);
+      } else {
+        uint32_t w = Word<T>::kNegInf;
+        if (inner(i) || cls(i * kU) < C) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(a) : "memory");
+        Word<T>::split(w, x);
+        if (kU == 2 && i == 0 && c0 < 0) x[0] = -INFINITY;
+        if (kU == 2 && !inner(i) && cls(i * kU + 1) >= C) x[1] = -INFINITY;
       }
     }
   }
-  // g[e] to the classes of `which` (a subset of live), in the row's own place or at `row`.
-  __device__ __forceinline__ void store(T* row, int64_t sc, bool staged, const float* g, uint32_t which) const {
-    if (staged) {
-      const uint32_t a = sm100::smem_u32(row) & ~3u;
+  // Writes g over the row in shared memory.
+  __device__ __forceinline__ void store(const float* g) const {
 #pragma unroll
-      for (int i = 0; i < kEW; ++i) {
-        const uint32_t at = a + 4 * word(i);
-        const uint32_t x = Word<T>::join(g + i * kW);
-        const uint32_t sel = (which >> (i * kW)) & ((1u << kW) - 1u);
-        if (sel == (1u << kW) - 1u) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(x) : "memory");
-        else if (kW == 2 && sel == 1u) asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"((uint16_t)x) : "memory");
-        else if (kW == 2 && sel == 2u)
-          asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + 2), "h"((uint16_t)(x >> 16)) : "memory");
+    for (int i = 0; i < kN; ++i) {
+      const float* x = g + i * kU;
+      const uint32_t a = at + i * (G * kU * (int)sizeof(T));
+      if (VEC) {
+        uint32_t w[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) w[h] = Word<T>::join(x + h * kW);
+        if (inner(i) || cls(i * kU) < C)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                       : "memory");
+      } else {
+        const uint32_t w = Word<T>::join(x);
+        const bool lo = !(kU == 2 && i == 0) || c0 >= 0;
+        const bool in = inner(i) || cls(i * kU) < C, hi = kU == 1 || inner(i) || cls(i * kU + 1) < C;
+        if (in && lo && hi) asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(w) : "memory");
+        else if (in && !lo && hi) asm volatile("st.shared.b16 [%0], %1;" ::"r"(a + 2), "h"((uint16_t)(w >> 16)) : "memory");
+        else if (in && lo) asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"((uint16_t)w) : "memory");
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (which >> e & 1) row[cls(e) * sc] = Elem<T>::from_f(g[e]);
     }
+  }
+  __device__ __forceinline__ float max() const {
+    float m = v[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) m = fmaxf(m, v[e]);
+    return group_max<G>(m);
   }
 };
+template <typename T>
+__device__ __forceinline__ float sh_get(uint32_t a) {
+  if (sizeof(T) == 4) {
+    float x;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(a) : "memory");
+    return x;
+  }
+  uint16_t h;
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(h) : "r"(a) : "memory");
+  return Elem<T>::to_f(*reinterpret_cast<const T*>(&h));
+}
+template <typename T>
+__device__ __forceinline__ void sh_put(uint32_t a, float x) {
+  if (sizeof(T) == 4) asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(x) : "memory");
+  else {
+    const T t = Elem<T>::from_f(x);
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"(*reinterpret_cast<const uint16_t*>(&t)) : "memory");
+  }
+}
 
-// Copies a tile's bytes into a stage (the last chunk of the last tile in part).
-__device__ __forceinline__ void tile_fetch(const Tile& t, const void* z, int64_t tile, int es, uint8_t* stage) {
-  const int64_t r0 = tile * t.rows_per_tile;
+// Starts the copy of a tile of dense rows (the last chunk of the last tile in part).
+__device__ __forceinline__ void tile_fetch(const Tile& t, const void* z, int64_t tile, int es, uint32_t dst) {
+  const int64_t r0 = tile * t.rows;
   if (tile < t.ntiles) {
-    const int64_t nr = t.nrows - r0 < t.rows_per_tile ? t.nrows - r0 : t.rows_per_tile;
-    const int bytes = (int)(nr * t.C * es);
+    const int nr = (int)(t.nrows - r0 < t.rows ? t.nrows - r0 : t.rows);
+    const int bytes = nr * t.C * es;
     const uint8_t* src = static_cast<const uint8_t*>(z) + r0 * t.C * es;
-    const uint32_t dst = sm100::smem_u32(stage);
-    for (int b = threadIdx.x * 16; b < bytes; b += kTileThreads * 16)
-      sm100::cp_async_16(dst + b, src + b, bytes - b < 16 ? bytes - b : 16);
+    const int pad = t.stride * es - t.chunks * 16;
+    for (int b = threadIdx.x; b * 16 < bytes; b += kTileThreads) {
+      const uint32_t d = dst + b * 16 + (t.mode == kCopyPadded ? (int)__umulhi(b, t.recip) * pad : 0);
+      sm100::cp_async_16(d, src + (int64_t)b * 16, bytes - b * 16 < 16 ? bytes - b * 16 : 16);
+    }
   }
   sm100::cp_async_commit();
 }
-// Writes a stage back to dense rows of dz (the block has synchronized).
+// Gathers a tile of rows that lie anyhow.
 template <typename T>
-__device__ __forceinline__ void tile_flush(const Tile& t, void* dz, int64_t tile, const uint8_t* stage) {
-  const int64_t r0 = tile * t.rows_per_tile;
-  const int64_t nr = t.nrows - r0 < t.rows_per_tile ? t.nrows - r0 : t.rows_per_tile;
-  const int bytes = (int)(nr * t.C * sizeof(T));
-  uint8_t* dst = static_cast<uint8_t*>(dz) + r0 * t.C * sizeof(T);
-  for (int b = threadIdx.x * 16; b < bytes; b += kTileThreads * 16) {
-    if (bytes - b >= 16) *reinterpret_cast<uint4*>(dst + b) = *reinterpret_cast<const uint4*>(stage + b);
-    else
-      for (int i = b; i < bytes; i += (int)sizeof(T)) *reinterpret_cast<T*>(dst + i) = *reinterpret_cast<const T*>(stage + i);
+__device__ __forceinline__ void tile_gather(const Tile& t, const View& v, const void* z, int64_t tile, T* stage) {
+  const int64_t r0 = tile * t.rows;
+  const int nr = (int)(t.nrows - r0 < t.rows ? t.nrows - r0 : t.rows);
+  const T* src = static_cast<const T*>(z);
+  if (v.sc == 1 && t.C >= 16) {   // lanes along the classes
+    for (int q = threadIdx.x / 32; q < nr; q += kTileThreads / 32) {
+      const int64_t at = v.base(r0 + q);
+      for (int c = threadIdx.x & 31; c < t.C; c += 32) stage[q * t.stride + c] = src[at + c];
+    }
+  } else {                        // lanes along the rows
+    for (int q = threadIdx.x; q < nr; q += kTileThreads) {
+      const int64_t at = v.base(r0 + q);
+#pragma unroll 8
+      for (int c = 0; c < t.C; ++c) stage[q * t.stride + c] = src[at + c * v.sc];
+    }
+  }
+}
+// Writes a stage back to the rows of dz (the block has synchronized). dz lies as the stage was filled.
+template <typename T>
+__device__ __forceinline__ void tile_flush(const Tile& t, const View& v, void* dz, int64_t tile, const T* stage) {
+  const int64_t r0 = tile * t.rows;
+  const int nr = (int)(t.nrows - r0 < t.rows ? t.nrows - r0 : t.rows);
+  if (t.mode != kGather) {
+    const int bytes = nr * t.C * (int)sizeof(T);
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(stage);
+    uint8_t* dst = static_cast<uint8_t*>(dz) + r0 * t.C * sizeof(T);
+    const int pad = t.stride * (int)sizeof(T) - t.chunks * 16;
+    for (int b = threadIdx.x; b * 16 < bytes; b += kTileThreads) {
+      const int s = b * 16 + (t.mode == kCopyPadded ? (int)__umulhi(b, t.recip) * pad : 0);
+      if (bytes - b * 16 >= 16) *reinterpret_cast<uint4*>(dst + (int64_t)b * 16) = *reinterpret_cast<const uint4*>(src + s);
+      else
+        for (int i = 0; i < bytes - b * 16; i += (int)sizeof(T))
+          *reinterpret_cast<T*>(dst + (int64_t)b * 16 + i) = *reinterpret_cast<const T*>(src + s + i);
+    }
+  } else if (v.sc == 1 && t.C >= 16) {
+    T* dst = static_cast<T*>(dz);
+    for (int q = threadIdx.x / 32; q < nr; q += kTileThreads / 32) {
+      const int64_t at = v.base(r0 + q);
+      for (int c = threadIdx.x & 31; c < t.C; c += 32) dst[at + c] = stage[q * t.stride + c];
+    }
+  } else {
+    T* dst = static_cast<T*>(dz);
+    for (int q = threadIdx.x; q < nr; q += kTileThreads) {
+      const int64_t at = v.base(r0 + q);
+#pragma unroll 4
+      for (int c = 0; c < t.C; ++c) dst[at + c * v.sc] = stage[q * t.stride + c];
+    }
   }
 }
 
-// Walks the tiles of a persistent block: body(row index, row pointer in
-// shared or global memory, in range) for each group of G lanes and row. All
-// lanes of a warp call body together; rows out of range repeat the last row.
+// Walks the tiles of a persistent block: body(row index, shared address of
+// the row, in range) for each group of G lanes and row. All lanes of a warp
+// call body together; a group without a row of its own repeats the last one
+// and writes nothing.
 template <typename T, int G, bool WRITES, typename Body>
-__device__ __forceinline__ void tile_walk(const Tile& t, const void* z, const View& v, void* dz, Body&& body) {
+__device__ __forceinline__ void tile_walk(const Tile& t, const View& v, const void* z, const View& dv, void* dz,
+                                          Body&& body) {
   extern __shared__ __align__(16) uint8_t stages[];
   constexpr int R = kTileThreads / G;
   const int sub = threadIdx.x / G;
-  if (t.staged) {
+  const uint32_t base = sm100::smem_u32(stages);
+  if (t.mode != kGather)
     for (int s = 0; s < kTileStages - 1; ++s)
-      tile_fetch(t, z, blockIdx.x + (int64_t)s * gridDim.x, sizeof(T), stages + s * t.stage_bytes);
-    int st = 0;
-    for (int64_t tile = blockIdx.x; tile < t.ntiles; tile += gridDim.x) {
+      tile_fetch(t, z, blockIdx.x + (int64_t)s * gridDim.x, sizeof(T), base + s * t.stage_bytes);
+  int st = 0;
+  for (int64_t tile = blockIdx.x; tile < t.ntiles; tile += gridDim.x) {
+    if (t.mode != kGather) {
       sm100::cp_async_wait<kTileStages - 2>();
       __syncthreads();   // this tile has landed for everyone, the last one is done with
-      tile_fetch(t, z, tile + (int64_t)(kTileStages - 1) * gridDim.x, sizeof(T),
-                 stages + ((st + kTileStages - 1) % kTileStages) * t.stage_bytes);
-      T* base = reinterpret_cast<T*>(stages + st * t.stage_bytes);
-      const int64_t r0 = tile * t.rows_per_tile;
-      const int nr = (int)(t.nrows - r0 < t.rows_per_tile ? t.nrows - r0 : t.rows_per_tile);
-      for (int i = 0; i < nr; i += R) {
-        const int q = i + sub, at = q < nr ? q : nr - 1;
-        body(r0 + at, base + (int64_t)at * t.C, q < nr);
-      }
-      if (WRITES) {
-        __syncthreads();
-        tile_flush<T>(t, dz, tile, stages + st * t.stage_bytes);
-      }
-      st = (st + 1) % kTileStages;
+      const int nx = st == 0 ? kTileStages - 1 : st - 1;
+      tile_fetch(t, z, tile + (int64_t)(kTileStages - 1) * gridDim.x, sizeof(T), base + nx * t.stage_bytes);
+    } else {
+      __syncthreads();
+      tile_gather<T>(t, v, z, tile, reinterpret_cast<T*>(stages));
+      __syncthreads();
     }
-  } else {
-    for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < t.nrows; r0 += (int64_t)gridDim.x * R) {
-      const int64_t q = r0 + sub, at = q < t.nrows ? q : t.nrows - 1;
-      body(at, const_cast<T*>(static_cast<const T*>(z)) + v.base(at), q < t.nrows);
+    const int64_t r0 = tile * t.rows;
+    const int nr = (int)(t.nrows - r0 < t.rows ? t.nrows - r0 : t.rows);
+    for (int i = 0; i < nr; i += R) {
+      const int q = i + sub, at = q < nr ? q : nr - 1;
+      body(r0 + at, base + st * t.stage_bytes + at * (t.stride * (int)sizeof(T)), q < nr);
     }
+    if (WRITES) {
+      __syncthreads();
+      tile_flush<T>(t, dv, dz, tile, reinterpret_cast<T*>(stages + st * t.stage_bytes));
+    }
+    if (t.mode != kGather) st = st == kTileStages - 1 ? 0 : st + 1;
   }
 }
 
-// Lanes per row and values per lane by the number of classes.
-struct TileKind { int g, e; };
-inline TileKind tile_kind(int C) {
-  if (C <= 4) return {1, 4};
-  if (C <= 8) return {1, 8};
-  if (C <= 16) return {1, 16};
-  if (C <= 32) return {1, 32};
-  if (C <= 64) return {4, 16};
-  if (C <= 128) return {8, 16};
-  if (C <= 256) return {16, 16};
-  if (C <= 512) return {32, 16};
-  return {32, 32};
-}
-// One tile of up to 16 KB (at least one row for each group of lanes): three
-// of them in flight in each of the blocks of an SM keep the memory busy.
-inline Tile make_tile(const r4c_rows_desc* d, int es, int g, bool dense) {
-  Tile t;
-  t.nrows = d->rows;
-  t.C = d->classes;
-  t.staged = dense;
-  const int r = kTileThreads / g;
-  int reps = (16 << 10) / (r * d->classes * es);
-  reps = reps < 1 ? 1 : reps > 16 ? 16 : reps;
-  // few rows: smaller tiles, so that every SM gets some
-  while (reps > 1 && d->rows < (int64_t)r * reps * 2 * kSMs) reps /= 2;
-  t.rows_per_tile = r * reps;
-  t.ntiles = (d->rows + t.rows_per_tile - 1) / t.rows_per_tile;
-  t.stage_bytes = (t.rows_per_tile * d->classes * es + 31) / 16 * 16;
-  return t;
-}
 inline bool dense_rows(const View& v, int64_t rows, int classes, const void* p) {
   return v.inner == 0 && (v.sc == 1 || classes == 1) && (v.si == classes || rows == 1) && ((uintptr_t)p & 15) == 0;
 }
-// Blocks of a persistent tile launch: what shared memory and threads let an SM hold.
-inline int tile_grid(const Tile& t, int threads_rows) {
-  if (!t.staged) {
-    const int64_t n = (t.nrows + threads_rows - 1) / threads_rows;
-    return (int)(n < kSMs * 8 ? n : kSMs * 8);
+// Lanes per row and values per lane by the number of classes: as few lanes as
+// 32 registers of values allow, since what a row costs beyond its elements is
+// paid once per group of lanes.
+struct TileKind {
+  int g, e;
+  bool vec;
+};
+inline TileKind tile_kind(int C, int es) {
+  const bool vec = C * es % 16 == 0;
+  if (C <= 32) return {1, C <= 4 ? 4 : C <= 8 ? 8 : C <= 16 ? 16 : 32, vec};
+  int g = 2;
+  while (C > g * 32) g *= 2;
+  return {g, 32, vec};
+}
+// Calls f(G, E, VEC as constants) for a kind; vectors need as many values as they hold.
+template <int G_, int E_, bool VEC_>
+struct TileConst {
+  static constexpr int G = G_, E = E_;
+  static constexpr bool VEC = VEC_;
+};
+template <typename T, typename F>
+inline cudaError_t for_tile_kind(const TileKind& k, F&& f) {
+#define R4C_TILE(G, E)                                                             \
+  if (k.g == G && k.e == E) {                                                      \
+    if constexpr (E * sizeof(T) >= 16) {                                           \
+      if (k.vec) return f(TileConst<G, E, true>{});                                \
+    }                                                                              \
+    return f(TileConst<G, E, false>{});                                            \
   }
-  int per_sm = (216 << 10) / (kTileStages * t.stage_bytes + 1024);
+  R4C_TILE(1, 4) R4C_TILE(1, 8) R4C_TILE(1, 16) R4C_TILE(1, 32) R4C_TILE(2, 32) R4C_TILE(4, 32) R4C_TILE(8, 32)
+  R4C_TILE(16, 32) R4C_TILE(32, 32)
+#undef R4C_TILE
+  return cudaErrorInvalidValue;
+}
+// Tiles of up to 16 KB (at least one row for each group of lanes): three of
+// them in flight in each of the blocks of an SM keep the memory busy.
+inline Tile make_tile(int64_t nrows, int C, int es, int g, bool dense) {
+  Tile t{};
+  t.nrows = nrows;
+  t.C = C;
+  t.mode = !dense ? kGather : C * es % 16 ? kCopy : kCopyPadded;
+  // rows that lie an even number of 16-byte chunks (or 4-byte words) apart would meet in the same banks
+  const int unit = C * es % 16 == 0 ? 16 : 4;
+  t.stride = t.mode == kCopy ? C : ((C * es + unit - 1) / unit | 1) * unit / es;
+  t.chunks = C * es / 16;
+  t.recip = t.chunks ? (uint32_t)(((1ull << 32) + t.chunks - 1) / t.chunks) : 0;
+  const int r = kTileThreads / g;
+  int reps = (16 << 10) / (r * t.stride * es);
+  reps = reps < 1 ? 1 : reps > 16 ? 16 : reps;
+  // few rows: smaller tiles, so that every SM gets some
+  while (reps > 1 && nrows < (int64_t)r * reps * 2 * kSMs) reps /= 2;
+  t.rows = r * reps;
+  t.ntiles = (nrows + t.rows - 1) / t.rows;
+  t.stage_bytes = (t.rows * t.stride * es + 31) / 16 * 16;
+  return t;
+}
+// Blocks of a persistent tile launch: what shared memory and threads let an SM hold.
+inline size_t tile_smem(const Tile& t) { return (size_t)(t.mode == kGather ? 1 : kTileStages) * t.stage_bytes; }
+inline int tile_grid(const Tile& t) {
+  int per_sm = (int)((216 << 10) / (tile_smem(t) + 1024));
   per_sm = per_sm < 1 ? 1 : per_sm > 8 ? 8 : per_sm;
   return (int)(t.ntiles < kSMs * per_sm ? t.ntiles : kSMs * per_sm);
 }
-
 template <typename K, typename A>
-inline cudaError_t launch_tile(K* kernel, const Tile& t, int threads_rows, cudaStream_t st, const A& a) {
-  const size_t smem = t.staged ? (size_t)kTileStages * t.stage_bytes : 0;
+inline cudaError_t launch_tile(K* kernel, const Tile& t, cudaStream_t st, const A& a) {
+  const size_t smem = tile_smem(t);
   if (smem > 48 << 10) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  kernel<<<tile_grid(t, threads_rows), kTileThreads, smem, st>>>(a);
+  kernel<<<tile_grid(t), kTileThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -333,6 +455,9 @@ template <typename T> struct Vec {
     Word<T>::split(x.y, v + w);
     Word<T>::split(x.z, v + 2 * w);
     Word<T>::split(x.w, v + 3 * w);
+  }
+  static __device__ __forceinline__ float top(const uint4& x) {
+    return Word<T>::top(Word<T>::max(Word<T>::max(x.x, x.y), Word<T>::max(x.z, x.w)));
   }
   static __device__ __forceinline__ uint4 join(const float* v) {
     constexpr int w = Word<T>::kElems;
@@ -357,37 +482,89 @@ struct VecRow {
   __device__ __forceinline__ int cls(int v) const { return v * Vec<T>::kElems - off; }
 };
 
-// Running maximum and sums of exponentials: s = sum exp2((z - m) k),
-// u = sum exp2((z - m) k) (z - m), k = log2(e) / T. m = -inf: nothing finite yet.
+// Running maximum and sums of exponentials, t_c = (z_c - m) k with
+// k = log2(e) / T: s = sum 2^t, u = sum 2^t t. m = -inf: nothing finite yet.
 struct Run {
   float m, s, u;
 };
 __device__ __forceinline__ Run run_empty() { return {-INFINITY, 0.f, 0.f}; }
 __device__ __forceinline__ Run run_merge(const Run& a, const Run& b, float k) {
   const float m = fmaxf(a.m, b.m), mm = anchor(m);
-  const float da = a.m - mm, db = b.m - mm;
-  const float fa = ex2(da * k), fb = ex2(db * k);
-  // an empty side has s = u = 0 and a difference of -inf: bounded, so that 0 * it stays 0
-  return {m, a.s * fa + b.s * fb, fa * (a.u + fmaxf(da, -1e30f) * a.s) + fb * (b.u + fmaxf(db, -1e30f) * b.s)};
+  const float ta = max_nan((a.m - mm) * k, kFloor), tb = max_nan((b.m - mm) * k, kFloor);
+  const float fa = ex2(ta), fb = ex2(tb);
+  return {m, a.s * fa + b.s * fb, fa * (a.u + ta * a.s) + fb * (b.u + tb * b.s)};
 }
+// A thread's part, in two interleaved chains (packed fp32 arithmetic).
+struct Run2 {
+  float m;
+  float2 s, u;
+  __device__ __forceinline__ Run join() const { return {m, s.x + s.y, u.x + u.y}; }
+};
+__device__ __forceinline__ Run2 run2_empty() { return {-INFINITY, {0.f, 0.f}, {0.f, 0.f}}; }
+template <bool ENT>
+__device__ __forceinline__ void run2_raise(Run2& r, float m, float k) {
+  if (m > r.m) {
+    const float t = max_nan((r.m - m) * k, kFloor), f = ex2(t);
+    const float2 f2 = {f, f}, t2 = {t, t};
+    if (ENT) r.u = __fmul2_rn(f2, __ffma2_rn(t2, r.s, r.u));
+    r.s = __fmul2_rn(f2, r.s);
+    r.m = m;
+  }
+}
+// x[0..N) with r.m at least their maximum; N even.
 template <int N, bool ENT>
-__device__ __forceinline__ void run_add(Run& r, const float* x, float k) {
-  float bm = x[0];
+__device__ __forceinline__ void run2_add(Run2& r, const float* x, float k) {
+  const float mm = -anchor(r.m);
+  const float2 m2 = {mm, mm}, k2 = {k, k};
 #pragma unroll
-  for (int i = 1; i < N; ++i) bm = fmaxf(bm, x[i]);
-  if (bm > r.m) {
-    const float d = r.m - bm, f = ex2(d * k);
-    if (ENT) r.u = f * (r.u + fmaxf(d, -1e30f) * r.s);
-    r.s *= f;
-    r.m = bm;
+  for (int i = 0; i < N; i += 2) {
+    float2 t = __fmul2_rn(__fadd2_rn(make_float2(x[i], x[i + 1]), m2), k2);
+    if (ENT) t = make_float2(max_nan(t.x, kFloor), max_nan(t.y, kFloor));
+    const float2 e = {ex2(t.x), ex2(t.y)};
+    r.s = __fadd2_rn(r.s, e);
+    if (ENT) r.u = __ffma2_rn(e, t, r.u);
   }
-  const float mm = anchor(r.m);
+}
+// As run2_add<N, true>, with the exponents bounded only in a batch that turns
+// u into NaN: 0 * -inf, from a masked class (the sum s then needs no repair).
+template <int N, int U, typename Split>
+__device__ __forceinline__ void run2_batch(Run2& r, float k, Split&& split) {
+  const float mm = -anchor(r.m);
+  const float2 m2 = {mm, mm}, k2 = {k, k};
+  float2 u = r.u;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = x[i] - mm, e = ex2(d * k);
-    r.s += e;
-    if (ENT) r.u = fmaf(e, fmaxf(d, -1e30f), r.u);
+  for (int i = 0; i < U; ++i) {
+    float x[N];
+    split(i, x);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const float2 t = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), m2), k2);
+      const float2 e = {ex2(t.x), ex2(t.y)};
+      r.s = __fadd2_rn(r.s, e);
+      u = __ffma2_rn(e, t, u);
+    }
   }
+  if (isnan(u.x + u.y)) {
+    u = r.u;
+#pragma unroll 1
+    for (int i = 0; i < U; ++i) {
+      float x[N];
+      split(i, x);
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        float2 t = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), m2), k2);
+        t = make_float2(max_nan(t.x, kFloor), max_nan(t.y, kFloor));
+        u = __ffma2_rn(make_float2(ex2(t.x), ex2(t.y)), t, u);
+      }
+    }
+  }
+  r.u = u;
+}
+template <bool ENT>
+__device__ __forceinline__ void run2_one(Run2& r, float x, float k) {
+  run2_raise<ENT>(r, x, k);
+  const float y[2] = {x, -INFINITY};
+  run2_add<2, ENT>(r, y, k);
 }
 // Joins the threads' runs of a block; every thread gets the result.
 template <int NT>
@@ -404,6 +581,64 @@ __device__ __forceinline__ Run run_block(Run r, float k, Run* sh) {
   for (int i = 1; i < NT / 32; ++i) r = run_merge(r, sh[i], k);
   return r;
 }
+
+// A block's piece of a row's gradient: dz = pair(z) for every class of the
+// piece, two at a time. The piece is one batch of up to kGradVecs vectors a
+// thread, loaded before `ready` (which may read what else the row needs).
+constexpr int kGradThreads = 256, kGradVecs = 4;
+inline int grad_pieces(int C, int es) {
+  const int nv = (int)(((int64_t)C * es + 15) / 16) + 1;
+  return (nv + kGradThreads * kGradVecs - 1) / (kGradThreads * kGradVecs);
+}
+template <typename T>
+struct GradPiece {
+  static constexpr int VE = Vec<T>::kElems;
+  VecRow<T> x, y;
+  int v0, v1, f0, f1;
+  uint4 w[kGradVecs];
+  __device__ __forceinline__ GradPiece(const T* z, T* dz, int C, int piece, int pieces) : x(z, C), y(dz, C) {
+    const int per = (x.nv + pieces - 1) / pieces;
+    v0 = min(piece * per, x.nv);
+    v1 = min(v0 + per, x.nv);
+    f0 = max(v0, x.first_full());
+    f1 = min(v1, x.end_full());
+#pragma unroll
+    for (int i = 0; i < kGradVecs; ++i)
+      if (f0 + (int)threadIdx.x + i * kGradThreads < f1) w[i] = __ldg(x.p + f0 + threadIdx.x + i * kGradThreads);
+  }
+  __device__ __forceinline__ bool has(int c) const {
+    const int v = (c + x.off) / VE;
+    return v >= v0 && v < v1;
+  }
+  template <typename Pair>
+  __device__ __forceinline__ void write(Pair&& pair) {
+    T* row = const_cast<T*>(y.row);
+    uint4* out = const_cast<uint4*>(y.p) + f0 + threadIdx.x;
+    const bool same = x.off == y.off;   // both rows break into vectors at the same classes
+#pragma unroll
+    for (int i = 0; i < kGradVecs; ++i) {
+      const int v = f0 + (int)threadIdx.x + i * kGradThreads;
+      if (v >= f1) break;
+      float g[VE];
+      Vec<T>::split(w[i], g);
+#pragma unroll
+      for (int j = 0; j < VE; j += 2) {
+        const float2 q = pair(make_float2(g[j], g[j + 1]));
+        g[j] = q.x;
+        g[j + 1] = q.y;
+      }
+      if (same) out[i * kGradThreads] = Vec<T>::join(g);
+      else
+        for (int j = 0; j < VE; ++j) row[x.cls(v) + j] = Elem<T>::from_f(g[j]);
+    }
+    // the partial vectors at the row's ends, one element a thread
+    auto edge = [&](int c) {
+      if (c >= 0 && c < x.C) row[c] = Elem<T>::from_f(pair(make_float2(Elem<T>::to_f(x.row[c]), 0.f)).x);
+    };
+    if (f0 > v0 && threadIdx.x < VE) edge(x.cls(v0) + threadIdx.x);
+    if (f1 < v1 && f1 >= f0 && threadIdx.x >= 32 && threadIdx.x < 32 + VE) edge(x.cls(f1) + threadIdx.x - 32);
+  }
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
