@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
     x.load(row, a.C);
     Run run = row_run(x, k);
     run_group<G>(run);
-    const RowOut o(run, __log2f(run.s), a.inv_t);
+    const RowOut o(run, lg2(run.s), a.inv_t);
     if (in && x.lane == 0) {
       if (a.target) {
         const int t = label_of(a.target, r, a.C, a.ignore, a.err);
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kTileThreads) bwd_tile_kernel(BwdArgs a) {
     const float gs = a.g_lse ? a.g_lse[r * a.gs_inc] : 0.f;
     Run run = row_run(x, k);
     run_group<G>(run);
-    const float l2s = __log2f(run.s);
+    const float l2s = lg2(run.s);
     const bool none = (gl == 0.f && gh == 0.f && gs == 0.f) || run.s == 0.f;
     const float h = kLn2 * (l2s - __fdividef(run.u, run.s));
     const float f = none ? 0.f : __fdividef(a.inv_t, run.s), ca = f * (gs - gl - gh * h), cb = f * gh * kLn2;
@@ -341,11 +341,15 @@ __device__ void block_topk(const VecRow<T>& x, int v0, int v1, int f0, int f1, f
   __syncthreads();
 }
 
+#ifndef KS
+#define KS 2
+#endif
+constexpr int kBatch = 4, kStages = KS;
 template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
-  constexpr int VE = Vec<T>::kElems, U = 4;
+  constexpr int VE = Vec<T>::kElems, U = kBatch;
   extern __shared__ __align__(16) uint8_t dyn[];
-  __shared__ Run runs[NT / 32];
+  __shared__ RunShared<NT> runs;
   __shared__ Run mine;
   __shared__ TopShared top;
   const int tid = threadIdx.x;
@@ -353,18 +357,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cs));
   if (cs > 1) cr = cluster_rank();
   if (TOP && tid == 0) {
-    top.cand = reinterpret_cast<uint64_t*>(dyn);
+    top.cand = reinterpret_cast<uint64_t*>(dyn + VecRing<NT, U, kStages>::kBytes);
     top.top = top.cand + kCand;
     top.keys = top.top + R4C_TOPK_MAX;
     top.active = reinterpret_cast<int*>(top.keys + NT);
   }
   __syncthreads();
   const float k = a.inv_t * kLog2e;
-  for (int64_t r = blockIdx.x / cs; r < a.nrows; r += gridDim.x / cs) {
+  auto none = [](int64_t) { return false; };
+  RowStream<T, NT, U, kStages, decltype(none)> stream(dyn, static_cast<const T*>(a.z), a.v, a.nrows, a.C, (int)cs, (int)cr,
+                                                      none);
+  for (int64_t r = blockIdx.x / cs; r < a.nrows; r += stream.step) {
     const VecRow<T> x(static_cast<const T*>(a.z) + a.v.base(r), a.C);
-    const int per = (x.nv + (int)cs - 1) / (int)cs;
-    const int v0 = min((int)cr * per, x.nv), v1 = min(v0 + per, x.nv);
-    const int f0 = max(v0, x.first_full()), f1 = min(v1, x.end_full());
+    int v0, v1, f0, f1;
+    stream.share(x, &v0, &v1, &f0, &f1);
     Run2 part = run2_empty();
     float tm = 0.f;   // the largest value of this thread's full vectors, and the first vector that has it
     int tv = -1;
@@ -375,26 +381,28 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
       }
     };
     int v = f0 + tid;
-    const uint4* p = x.p + v;
-    for (; v + (U - 1) * NT < f1; v += U * NT, p += U * NT) {
+    for (int left = f1 - f0; left > 0; left -= U * NT, v += U * NT) {
       uint4 w[U];
-      float vm[U];
+      stream.take(w);
+      if (left >= U * NT) {
+        float vm[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) w[i] = __ldg(p + i * NT);
+        for (int i = 0; i < U; ++i) {
+          vm[i] = Vec<T>::top(w[i]);
+          track(vm[i], v + i * NT);
+        }
+        run2_raise<true>(part, fmaxf(fmaxf(vm[0], vm[1]), fmaxf(vm[2], vm[3])), k);
+        run2_batch<VE, U>(part, k, [&](int i, float* y) { Vec<T>::split(i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3], y); });
+      } else {
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        vm[i] = Vec<T>::top(w[i]);
-        track(vm[i], v + i * NT);
+        for (int i = 0; i < U; ++i) {
+          if (v + i * NT >= f1) break;
+          const float vm = Vec<T>::top(w[i]);
+          track(vm, v + i * NT);
+          run2_raise<true>(part, vm, k);
+          run2_batch<VE, 1>(part, k, [&](int, float* y) { Vec<T>::split(w[i], y); });
+        }
       }
-      run2_raise<true>(part, fmaxf(fmaxf(vm[0], vm[1]), fmaxf(vm[2], vm[3])), k);
-      run2_batch<VE, U>(part, k, [&](int i, float* y) { Vec<T>::split(i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3], y); });
-    }
-    for (; v < f1; v += NT, p += NT) {
-      const uint4 w = __ldg(p);
-      const float vm = Vec<T>::top(w);
-      track(vm, v);
-      run2_raise<true>(part, vm, k);
-      run2_batch<VE, 1>(part, k, [&](int, float* y) { Vec<T>::split(w, y); });
     }
     if (f0 > v0 && tid < VE) {   // partial vectors: one element a thread
       const int c = x.cls(v0) + tid;
@@ -465,9 +473,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
 // One block per piece of a row.
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads) bwd_block_kernel(BwdArgs a) {
+  extern __shared__ __align__(16) uint8_t ring[];
   const int64_t r = blockIdx.x / a.segs;
   T* dz = static_cast<T*>(a.dz) + a.dv.base(r);
-  GradPiece<T> piece(static_cast<const T*>(a.z) + a.v.base(r), dz, a.C, blockIdx.x % a.segs, a.segs);
+  GradPiece<T> piece(static_cast<const T*>(a.z) + a.v.base(r), dz, a.C, blockIdx.x % a.segs, a.segs, ring);
   const int t = label_of(a.target, r, a.C, a.ignore, a.err);
   const float gl = a.g_logp && t >= 0 ? a.g_logp[r * a.gl_inc] : 0.f;
   const float gh = a.g_entropy ? a.g_entropy[r * a.gh_inc] : 0.f;
@@ -506,14 +515,13 @@ __global__ void __launch_bounds__(kGradThreads) bwd_block_kernel(BwdArgs a) {
 template <typename T, int NT>
 cudaError_t launch_fwd_block(const FwdArgs& a, cudaStream_t s) {
   const int cs = cluster_size(a.nrows, a.C, sizeof(T), NT);
-  const int64_t most = (int64_t)kSMs * (1024 / NT);
+  constexpr size_t ring = VecRing<NT, kBatch, kStages>::kBytes;
+  const size_t smem = ring + (a.K > 0 ? (kCand + R4C_TOPK_MAX + NT) * sizeof(uint64_t) + NT * sizeof(int) : 0);
+  const int64_t most = (int64_t)kSMs * blocks_per_sm(NT, smem);
   int64_t grid = a.nrows * cs;
   if (cs == 1 && grid > most) grid = most;
-  if (a.K > 0) {
-    const size_t smem = (kCand + R4C_TOPK_MAX + NT) * sizeof(uint64_t) + NT * sizeof(int);
-    return launch_cluster(fwd_block_kernel<T, NT, true>, grid, NT, cs, smem, s, a);
-  }
-  return launch_cluster(fwd_block_kernel<T, NT, false>, grid, NT, cs, 0, s, a);
+  if (a.K > 0) return launch_cluster(fwd_block_kernel<T, NT, true>, grid, NT, cs, smem, s, a);
+  return launch_cluster(fwd_block_kernel<T, NT, false>, grid, NT, cs, smem, s, a);
 }
 
 template <typename T>
@@ -539,10 +547,10 @@ cudaError_t launch_bwd(BwdArgs& a, cudaStream_t s) {
       return launch_tile(bwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::VEC>, a.tile, s, a);
     });
   }
-  a.segs = grad_pieces(a.C, sizeof(T));
+  a.segs = grad_pieces(a.nrows, a.C, sizeof(T));
   if (a.nrows * a.segs > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  bwd_block_kernel<T><<<(unsigned)(a.nrows * a.segs), kGradThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  return launch_cluster(bwd_block_kernel<T>, a.nrows * a.segs, kGradThreads, 1,
+                        VecRing<kGradThreads, kGradBatch, kGradStages>::kBytes, s, a);
 }
 
 }  // namespace logp

@@ -59,6 +59,12 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Of normal positive numbers (0 gives -inf).
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // The larger of two, NaN if either is (fmaxf would drop it).
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
@@ -419,7 +425,7 @@ inline Tile make_tile(int64_t nrows, int C, int es, int g, bool dense) {
   t.chunks = C * es / 16;
   t.recip = t.chunks ? (uint32_t)(((1ull << 32) + t.chunks - 1) / t.chunks) : 0;
   const int r = kTileThreads / g;
-  int reps = (16 << 10) / (r * t.stride * es);
+  int reps = (g == 1 ? 8 << 10 : 16 << 10) / (r * t.stride * es);
   reps = reps < 1 ? 1 : reps > 16 ? 16 : reps;
   // few rows: smaller tiles, so that every SM gets some
   while (reps > 1 && nrows < (int64_t)r * reps * 2 * kSMs) reps /= 2;
@@ -566,45 +572,101 @@ __device__ __forceinline__ void run2_one(Run2& r, float x, float k) {
   const float y[2] = {x, -INFINITY};
   run2_add<2, ENT>(r, y, k);
 }
-// Joins the threads' runs of a block; every thread gets the result.
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+// Joins the threads' runs of a block; every thread gets the result. The
+// maximum goes first, so that each thread rescales its sums once.
 template <int NT>
-__device__ __forceinline__ Run run_block(Run r, float k, Run* sh) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const Run b{__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o),
-                __shfl_xor_sync(0xffffffffu, r.u, o)};
-    r = run_merge(r, b, k);
-  }
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = r;
+struct RunShared {
+  float m[NT / 32];
+  float2 su[NT / 32];
+};
+template <int NT>
+__device__ __forceinline__ Run run_block(Run r, float k, RunShared<NT>& sh) {
+  constexpr int W = NT / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float wm = warp_max(r.m);
+  if (lane == 0) sh.m[warp] = wm;
   __syncthreads();
-  r = sh[0];
-  for (int i = 1; i < NT / 32; ++i) r = run_merge(r, sh[i], k);
-  return r;
+  float m = sh.m[0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) m = fmaxf(m, sh.m[i]);
+  const float t = max_nan((r.m - anchor(m)) * k, kFloor), f = ex2(t);
+  const float s = group_sum<32>(f * r.s), u = group_sum<32>(f * (r.u + t * r.s));
+  if (lane == 0) sh.su[warp] = make_float2(s, u);
+  __syncthreads();
+  Run out{m, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    out.s += sh.su[i].x;
+    out.u += sh.su[i].y;
+  }
+  return out;
 }
 
+// A thread's own ring of 16-byte vectors in shared memory: batches of U
+// vectors (a block's stride apart) are copied ahead with cp.async and read
+// back by the thread that asked for them, so the copies in flight cost
+// neither registers nor barriers.
+template <int NT, int U, int S>
+struct VecRing {
+  static constexpr int kBytes = NT * U * S * 16;
+  uint32_t base;
+  int in, out;
+  __device__ __forceinline__ explicit VecRing(void* smem)
+      : base(sm100::smem_u32(smem) + threadIdx.x * 16), in(0), out(0) {}
+  // Vectors p[i * NT] for i * NT < left (left counts from this thread's first); any left: the batch is counted.
+  __device__ __forceinline__ void issue(const uint4* p, int left) {
+    const uint32_t d = base + in * (U * NT * 16);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (i * NT < left) sm100::cp_async_16(d + i * (NT * 16), p + i * NT, 16);
+    sm100::cp_async_commit();
+    in = in == S - 1 ? 0 : in + 1;
+  }
+  // The oldest batch, with S - 1 issued since the start of it or later.
+  __device__ __forceinline__ void take(uint4* w) {
+    sm100::cp_async_wait<S - 2>();
+    const uint32_t d = base + out * (U * NT * 16);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w) : "r"(d + i * (NT * 16)) : "memory");
+    out = out == S - 1 ? 0 : out + 1;
+  }
+};
+
 // A block's piece of a row's gradient: dz = pair(z) for every class of the
-// piece, two at a time. The piece is one batch of up to kGradVecs vectors a
-// thread, loaded before `ready` (which may read what else the row needs).
-constexpr int kGradThreads = 256, kGradVecs = 4;
-inline int grad_pieces(int C, int es) {
-  const int nv = (int)(((int64_t)C * es + 15) / 16) + 1;
-  return (nv + kGradThreads * kGradVecs - 1) / (kGradThreads * kGradVecs);
+// piece, two at a time.
+constexpr int kGradThreads = 256, kGradBatch = 4, kGradStages = 3;
+// Pieces of a row: about sixteen vectors a thread, fewer where the rows alone leave SMs idle.
+inline int grad_pieces(int64_t nrows, int C, int es) {
+  const int64_t nv = ((int64_t)C * es + 15) / 16 + 1;
+  int64_t most = (nv + kGradThreads * 2 - 1) / (kGradThreads * 2), p = (nv + kGradThreads * 16 - 1) / (kGradThreads * 16);
+  while (p < most && nrows * p < 4 * kSMs) ++p;
+  return (int)p;
 }
 template <typename T>
 struct GradPiece {
-  static constexpr int VE = Vec<T>::kElems;
+  static constexpr int VE = Vec<T>::kElems, U = kGradBatch, NT = kGradThreads;
   VecRow<T> x, y;
   int v0, v1, f0, f1;
-  uint4 w[kGradVecs];
-  __device__ __forceinline__ GradPiece(const T* z, T* dz, int C, int piece, int pieces) : x(z, C), y(dz, C) {
+  VecRing<NT, U, kGradStages> ring;
+  __device__ __forceinline__ GradPiece(const T* z, T* dz, int C, int piece, int pieces, void* smem)
+      : x(z, C), y(dz, C), ring(smem) {
     const int per = (x.nv + pieces - 1) / pieces;
     v0 = min(piece * per, x.nv);
     v1 = min(v0 + per, x.nv);
     f0 = max(v0, x.first_full());
     f1 = min(v1, x.end_full());
-#pragma unroll
-    for (int i = 0; i < kGradVecs; ++i)
-      if (f0 + (int)threadIdx.x + i * kGradThreads < f1) w[i] = __ldg(x.p + f0 + threadIdx.x + i * kGradThreads);
+    for (int b = 0; b < kGradStages - 1; ++b) fetch(b);
+  }
+  __device__ __forceinline__ void fetch(int b) {
+    const int v = f0 + b * (U * NT) + (int)threadIdx.x;
+    ring.issue(x.p + v, f1 - v);
   }
   __device__ __forceinline__ bool has(int c) const {
     const int v = (c + x.off) / VE;
@@ -615,21 +677,27 @@ struct GradPiece {
     T* row = const_cast<T*>(y.row);
     uint4* out = const_cast<uint4*>(y.p) + f0 + threadIdx.x;
     const bool same = x.off == y.off;   // both rows break into vectors at the same classes
+    int b = 0;
+    for (int left = f1 - f0 - (int)threadIdx.x; left > -(int)threadIdx.x; left -= U * NT, ++b) {
+      uint4 w[U];
+      ring.take(w);
+      fetch(b + kGradStages - 1);
 #pragma unroll
-    for (int i = 0; i < kGradVecs; ++i) {
-      const int v = f0 + (int)threadIdx.x + i * kGradThreads;
-      if (v >= f1) break;
-      float g[VE];
-      Vec<T>::split(w[i], g);
+      for (int i = 0; i < U; ++i) {
+        if (i * NT >= left) break;
+        float g[VE];
+        Vec<T>::split(w[i], g);
 #pragma unroll
-      for (int j = 0; j < VE; j += 2) {
-        const float2 q = pair(make_float2(g[j], g[j + 1]));
-        g[j] = q.x;
-        g[j + 1] = q.y;
+        for (int j = 0; j < VE; j += 2) {
+          const float2 q = pair(make_float2(g[j], g[j + 1]));
+          g[j] = q.x;
+          g[j + 1] = q.y;
+        }
+        const int at = b * (U * NT) + i * NT;
+        if (same) out[at] = Vec<T>::join(g);
+        else
+          for (int j = 0; j < VE; ++j) row[x.cls(f0 + at + (int)threadIdx.x) + j] = Elem<T>::from_f(g[j]);
       }
-      if (same) out[i * kGradThreads] = Vec<T>::join(g);
-      else
-        for (int j = 0; j < VE; ++j) row[x.cls(v) + j] = Elem<T>::from_f(g[j]);
     }
     // the partial vectors at the row's ends, one element a thread
     auto edge = [&](int c) {
@@ -669,6 +737,67 @@ __device__ __forceinline__ Run cluster_ld_run(const Run* p, uint32_t rank) {
   return {cluster_ld_f32(a), cluster_ld_f32(a + 4), cluster_ld_f32(a + 8)};
 }
 
+// The vectors of the rows that a block (of a cluster) takes in turn, batch by
+// batch and ahead across the rows' ends, so that the memory stays busy while
+// a row is finished. skip(row): neither read nor taken.
+template <typename T, int NT, int U, int S, typename Skip>
+struct RowStream {
+  VecRing<NT, U, S> ring;
+  const T* z;
+  const View& v;
+  int64_t nrows, step, row;   // row: the one that is read ahead
+  int C, cs, cr;
+  const uint4* p;
+  int left;                   // full vectors of it not asked for yet
+  Skip skip;
+  bool skip_next;
+  __device__ __forceinline__ RowStream(void* smem, const T* z_, const View& v_, int64_t nrows_, int C_, int cs_, int cr_,
+                                       Skip skip_)
+      : ring(smem), z(z_), v(v_), nrows(nrows_), step(gridDim.x / cs_), row(blockIdx.x / cs_), C(C_), cs(cs_), cr(cr_),
+        left(0), skip(skip_), skip_next(false) {
+    skip_next = row < nrows && skip(row);
+    open();
+    for (int s = 0; s < S - 1; ++s) ahead();
+  }
+  // This block's share of a row: vectors [v0, v1), the whole ones [f0, f1).
+  __device__ __forceinline__ void share(const VecRow<T>& x, int* v0, int* v1, int* f0, int* f1) const {
+    const int per = cs == 1 ? x.nv : (x.nv + cs - 1) / cs;
+    *v0 = min(cr * per, x.nv);
+    *v1 = min(*v0 + per, x.nv);
+    *f0 = max(*v0, x.first_full());
+    *f1 = min(*v1, x.end_full());
+  }
+  __device__ __forceinline__ void open() {   // at `row`, or the first one after it that has something to read
+    while (row < nrows) {
+      const bool sk = skip_next;
+      skip_next = row + step < nrows && skip(row + step);   // loaded a row early
+      if (!sk) {
+        const VecRow<T> x(z + v.base(row), C);
+        int v0, v1, f0, f1;
+        share(x, &v0, &v1, &f0, &f1);
+        left = f1 - f0;
+        p = x.p + f0 + threadIdx.x;
+        if (left > 0) return;
+      }
+      row += step;
+    }
+    left = 0;
+  }
+  __device__ __forceinline__ void ahead() {
+    ring.issue(p, left - (int)threadIdx.x);
+    p += U * NT;
+    left -= U * NT;
+    if (left <= 0 && row < nrows) {
+      row += step;
+      open();
+    }
+  }
+  __device__ __forceinline__ void take(uint4* w) {
+    ring.take(w);
+    ahead();
+  }
+};
+
 // Blocks that share a row: as many as bring the rows to two blocks an SM, in
 // powers of two up to 16, while each keeps a few vectors a thread.
 inline int cluster_size(int64_t nrows, int C, int es, int threads) {
@@ -677,9 +806,17 @@ inline int cluster_size(int64_t nrows, int C, int es, int threads) {
   return cs;
 }
 
+// Blocks of `threads` that an SM holds with this much dynamic shared memory
+// (the kernels keep to 64 registers a thread): a persistent grid of more
+// would leave some of them to run alone after the others.
+inline int blocks_per_sm(int threads, size_t smem) {
+  const int by_smem = (int)((227 << 10) / (smem + 4096)), by_threads = 1024 / threads;
+  return by_smem < by_threads ? by_smem : by_threads;
+}
+
 template <typename K, typename A>
 inline cudaError_t launch_cluster(K* kernel, int64_t grid, int threads, int cs, size_t smem, cudaStream_t st, const A& a) {
-  if (smem > 48 << 10) {
+  if (smem > 44 << 10) {   // with the kernels' static shared memory, above the default
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
