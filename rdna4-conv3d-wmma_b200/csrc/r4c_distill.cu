@@ -25,10 +25,7 @@ __device__ __forceinline__ uint4 mask_vec(uint4 w, uint32_t bits) {
 // (a byte per vector) in shared memory, so that the streaming loop leaves
 // them out at the price of one byte load per vector; their own sum comes from
 // the K pairs.
-#ifndef KS
-#define KS 2
-#endif
-constexpr int kBatch = 4, kStages = KS;
+constexpr int kBatch = 4, kStages = 2;
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
   constexpr int VE = Vec<T>::kElems, U = kBatch;
@@ -61,8 +58,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
     int c = -1;
     float v = 0.f;
     if (tid < a.K) {
-      v = teacher_logp<false>(a, r * a.K + tid);
-      c = teacher_class<false>(a, r * a.K + tid, v);
+      v = teacher_logp<false>(a, r * a.K, tid);
+      c = teacher_class<false>(a, r * a.K, tid, v);
       idx[tid] = c;
     }
     const bool any = __syncthreads_or(c >= 0);
@@ -206,12 +203,12 @@ __global__ void __launch_bounds__(kGradThreads) bwd_block_kernel(Args a) {
   }
   int c = -1;
   if (tid < a.K) {
-    const float v = teacher_logp<false>(a, r * a.K + tid);
-    c = teacher_class<false>(a, r * a.K + tid, v);
+    const float v = teacher_logp<false>(a, r * a.K, tid);
+    c = teacher_class<false>(a, r * a.K, tid, v);
     idx[tid] = c;
     qj[tid] = c < 0 ? 0.f : prob(v - st.qm) / st.qs;
   }
-  const float k = a.inv_t * kLog2e, scale = grad_scale(a, r, st.w), mr = a.rest ? st.mr : st.m;
+  const float k = a.inv_t * kLog2e, scale = st.w * grad_scale(a, r), mr = a.rest ? st.mr : st.m;
   const float coef = scale * rest_coef(a.rest, st.mass, st.q_rest, st.m, st.s, st.mr, st.sr, k);
   const float2 m2 = {-mr, -mr}, k2 = {k, k}, c2 = {coef, coef};
   piece.write([&](float2 z) {

@@ -55,13 +55,14 @@ struct Args {
 
 // PLAIN: fp32 log-probabilities and 32-bit classes; else what the types say.
 template <bool PLAIN>
-__device__ __forceinline__ float teacher_logp(const Args& a, int64_t i) {
-  if (PLAIN || a.t_dtype == R4C_F32) return __ldg(static_cast<const float*>(a.t_logp) + i);
-  if (a.t_dtype == R4C_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(a.t_logp)[i]);
-  return __half2float(static_cast<const __half*>(a.t_logp)[i]);
+__device__ __forceinline__ float teacher_logp(const Args& a, int64_t first, int i) {
+  if (PLAIN || a.t_dtype == R4C_F32) return __ldg(static_cast<const float*>(a.t_logp) + first + i);
+  if (a.t_dtype == R4C_BF16) return __bfloat162float((static_cast<const __nv_bfloat16*>(a.t_logp) + first)[i]);
+  return __half2float((static_cast<const __half*>(a.t_logp) + first)[i]);
 }
 // The class of a pair as the kernels use it, -1 when the pair is void.
-__device__ __forceinline__ int valid_class(const Args& a, int64_t c, float v) {
+template <typename I>
+__device__ __forceinline__ int valid_class(const Args& a, I c, float v) {
   if (c < 0 || v == -INFINITY) return -1;
   if (c >= a.C) {
     atomicExch(a.err, 6);
@@ -70,12 +71,13 @@ __device__ __forceinline__ int valid_class(const Args& a, int64_t c, float v) {
   return (int)c;
 }
 template <bool PLAIN>
-__device__ __forceinline__ int teacher_class(const Args& a, int64_t i, float v) {
-  if (PLAIN || !a.t_wide) return valid_class(a, __ldg(static_cast<const int32_t*>(a.t_index) + i), v);
-  return valid_class(a, __ldg(static_cast<const long long*>(a.t_index) + i), v);
+__device__ __forceinline__ int teacher_class(const Args& a, int64_t first, int i, float v) {
+  if (PLAIN || !a.t_wide) return valid_class(a, __ldg(static_cast<const int32_t*>(a.t_index) + first + i), v);
+  return valid_class(a, __ldg(static_cast<const long long*>(a.t_index) + first + i), v);
 }
-__device__ __forceinline__ float grad_scale(const Args& a, int64_t r, float w) {
-  return a.temp * w * a.grad[r * a.grad_inc] / (a.total_weight ? a.total_weight[0] : 1.f);
+// T g / W of the row; its weight comes on top.
+__device__ __forceinline__ float grad_scale(const Args& a, int64_t r) {
+  return a.temp * a.grad[r * a.grad_inc] / (a.total_weight ? a.total_weight[0] : 1.f);
 }
 // A block's (sum of losses, sum of weights), in a fixed order.
 template <int NT>
@@ -109,12 +111,12 @@ struct RowSums {
   float m, s, mr, sr;
   bool empty;
   __device__ __forceinline__ RowSums(const Run& r, const Run& l, bool rest, float k) {
-    const Run all = rest ? run_merge(r, l, k) : r;
-    empty = all.s == 0.f;
-    m = anchor(all.m);
-    s = all.s;
+    const float top = rest ? fmaxf(r.m, l.m) : r.m;
+    m = anchor(top);
     mr = anchor(r.m);
-    sr = r.s;
+    sr = s = r.s;
+    if (rest) s = r.s * ex2((r.m - m) * k) + l.s * ex2((l.m - m) * k);   // an empty side: 0 * 2^-inf
+    empty = s == 0.f;
   }
 };
 // q_r from the sum of the listed q.

@@ -15,29 +15,33 @@
 namespace r4c {
 namespace distill {
 
-constexpr int kSlots = 4;   // pairs of a lane
+constexpr int kMostSlots = 4;   // pairs of a lane; kernels hold two or four
 
-template <typename T, int G, int E, bool VEC, bool BWD, bool PLAIN>
+template <typename T, int G, int E, bool VEC, bool BWD, int kSlots, bool PLAIN>
 __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
   constexpr int ES = (int)sizeof(T);
   const float k = a.inv_t * kLog2e;
   const bool rest = a.rest;
   const int K = a.K;
-  double sum_loss = 0.0, sum_w = 0.0;
-  tile_walk<T, G, BWD>(a.tile, a.v, a.z, a.dv, a.dz, [&](int64_t r, uint32_t row, bool in) {
+  auto has = [&](int s) { return s < 2 || s * G < K; };   // no test for the first two: an unused place is void
+  Sum2 sum_loss, sum_w;
+  const float scale1 = BWD && a.grad_inc == 0 ? grad_scale(a, 0) : 0.f;
+  tile_walk<T, G, BWD>(a.tile, a.v, a.z, a.dv, a.dz, [&](int64_t r0, int r, uint32_t row, bool in) {
     const int lane = threadIdx.x & (G - 1);
-    float w = a.weight ? a.weight[r] : 1.f;
+    float w = a.weight ? (a.weight + r0)[r] : 1.f;
     float pv[kSlots], pz[kSlots], pq[kSlots];
     int pc[kSlots];
-    const int64_t p0 = r * K + lane;
+    const int64_t pairs0 = r0 * K;   // the tile's first pair
+    const int p0 = r * K + lane;
     float qm = -INFINITY;
     bool any = false;
     if (PLAIN && G == 1 && a.even) {   // an even number of pairs, 8-byte aligned
-      const float2* v2 = reinterpret_cast<const float2*>(static_cast<const float*>(a.t_logp) + p0);
-      const int2* c2 = reinterpret_cast<const int2*>(static_cast<const int32_t*>(a.t_index) + p0);
+      const float2* v2 = reinterpret_cast<const float2*>(static_cast<const float*>(a.t_logp) + pairs0 + p0);
+      const int2* c2 = reinterpret_cast<const int2*>(static_cast<const int32_t*>(a.t_index) + pairs0 + p0);
 #pragma unroll
       for (int s = 0; s < kSlots; s += 2) {
         pc[s] = pc[s + 1] = -1;
+        pv[s] = pv[s + 1] = -INFINITY;
         if (s < K) {
           const float2 v = __ldg(v2 + s / 2);
           const int2 c = __ldg(c2 + s / 2);
@@ -51,16 +55,17 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
 #pragma unroll
       for (int s = 0; s < kSlots; ++s) {
         pc[s] = -1;
-        if (s * G < K && lane + s * G < K) {
-          pv[s] = teacher_logp<PLAIN>(a, p0 + s * G);
-          pc[s] = teacher_class<PLAIN>(a, p0 + s * G, pv[s]);
+        pv[s] = -INFINITY;
+        if (has(s) && lane + s * G < K) {
+          pv[s] = teacher_logp<PLAIN>(a, pairs0, p0 + s * G);
+          pc[s] = teacher_class<PLAIN>(a, pairs0, p0 + s * G, pv[s]);
         }
       }
     }
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
       pz[s] = -INFINITY;
-      if (s * G < K && pc[s] >= 0) {
+      if (has(s) && pc[s] >= 0) {
         pz[s] = sh_get<T>(row + pc[s] * ES);
         qm = fmaxf(qm, pv[s]);
         any = true;
@@ -79,23 +84,23 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
         for (int s = 1; s < kSlots; ++s)
 #pragma unroll
           for (int q = 0; q < s; ++q)
-            if (s < K && pc[s] >= 0 && pc[s] == pc[q]) other |= 1u << s;
+            if (pc[s] >= 0 && pc[s] == pc[q]) other |= 1u << s;
         twice = other != 0;
       } else {
         // each pair leaves its number at its class and looks whether it is still there
         __syncwarp();
 #pragma unroll
         for (int s = 0; s < kSlots; ++s)
-          if (s * G < K && in && pc[s] >= 0) sh_put<T>(row + pc[s] * ES, (float)(lane + s * G + 1));
+          if (has(s) && in && pc[s] >= 0) sh_put<T>(row + pc[s] * ES, (float)(lane + s * G + 1));
         __syncwarp();
 #pragma unroll
         for (int s = 0; s < kSlots; ++s)
-          if (s * G < K && in && pc[s] >= 0) twice |= sh_get<T>(row + pc[s] * ES) != (float)(lane + s * G + 1);
+          if (has(s) && in && pc[s] >= 0) twice |= sh_get<T>(row + pc[s] * ES) != (float)(lane + s * G + 1);
         twice = group_any<G>(twice);
         if (__any_sync(0xffffffffu, twice)) {
 #pragma unroll
           for (int s = 0; s < kSlots; ++s) {
-            if (s * G >= K) continue;
+            if (!has(s)) continue;
             for (int i = 0; i < G; ++i) {
               const int c = __shfl_sync(0xffffffffu, pc[s], i, G);
 #pragma unroll
@@ -111,7 +116,7 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
     if (rest || (BWD && G > 1 && K > 1)) {
 #pragma unroll
       for (int s = 0; s < kSlots; ++s)
-        if (s * G < K && in && pc[s] >= 0) sh_put<T>(row + pc[s] * ES, rest ? -INFINITY : pz[s]);
+        if (has(s) && in && pc[s] >= 0) sh_put<T>(row + pc[s] * ES, rest ? -INFINITY : pz[s]);
       if (G > 1) __syncwarp();
     }
     TileRow<T, G, E, VEC> x;
@@ -119,23 +124,17 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
     if (BWD && G > 1) __syncwarp();   // read by all before any of it is written over
 
     // The sums over the row as it stands and, with a rest, over the listed classes.
-    Run u, l = run_empty();
-    {
-      Run2 part = run2_empty();
-      part.m = x.max();
-      run2_add<E, false>(part, x.v, k);
-      u = part.join();
-      u.s = group_sum<G>(u.s);
-    }
+    const Run u = tile_exp(x, k);   // x: the exponentials from u.m
+    Run l = run_empty();
     if (rest) {
 #pragma unroll
       for (int s = 0; s < kSlots; ++s)
-        if (s * G < K) l.m = fmaxf(l.m, pz[s]);
+        if (has(s)) l.m = fmaxf(l.m, pz[s]);
       l.m = group_max<G>(l.m);
       const float lm = anchor(l.m);
 #pragma unroll
       for (int s = 0; s < kSlots; ++s)
-        if (s * G < K && pc[s] >= 0 && !(other >> s & 1)) l.s += ex2((pz[s] - lm) * k);
+        if (has(s) && pc[s] >= 0 && !(other >> s & 1)) l.s += ex2((pz[s] - lm) * k);
       l.s = group_sum<G>(l.s);
     }
     RowSums s(u, l, rest, k);
@@ -146,7 +145,7 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
     float sum_q = 0.f;
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-      pq[i] = i * G < K && pc[i] >= 0 ? prob(pv[i] - q0) : 0.f;
+      pq[i] = has(i) && pc[i] >= 0 ? prob(pv[i] - q0) : 0.f;
       sum_q += pq[i];
     }
     sum_q = group_sum<G>(sum_q);
@@ -160,25 +159,19 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
       float loss = 0.f;
 #pragma unroll
       for (int i = 0; i < kSlots; ++i)
-        if (i * G < K && pc[i] >= 0 && !(pq[i] == 0.f)) loss += pq[i] * (pv[i] + c0 - (pz[i] - s.m) * a.inv_t);
+        if (has(i) && pc[i] >= 0 && !(pq[i] == 0.f)) loss += pq[i] * (pv[i] + c0 - (pz[i] - s.m) * a.inv_t);
       loss = group_sum<G>(loss) + rest_loss(qr, s, a.inv_t);
       if (in && lane == 0) {
         loss = w == 0.f ? 0.f : w * a.temp * a.temp * loss;
-        if (a.row_loss) a.row_loss[r] = loss;
-        sum_loss += loss;
-        sum_w += w;
+        if (a.row_loss) (a.row_loss + r0)[r] = loss;
+        sum_loss.add(loss);
+        sum_w.add(w);
       }
     } else {
-      const float scale = w == 0.f ? 0.f : grad_scale(a, r, w), mass = rest ? sum_q + qr : 1.f;
+      const float scale = w == 0.f ? 0.f : w * (a.grad_inc == 0 ? scale1 : grad_scale(a, r0 + r)), mass = rest ? sum_q + qr : 1.f;
       const float coef = w == 0.f ? 0.f : scale * rest_coef(rest, mass, qr, s.m, s.s, s.mr, s.sr, k);
-      const float2 m2 = {-s.mr, -s.mr}, k2 = {k, k}, c2 = {coef, coef};
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 t = __fmul2_rn(__fadd2_rn(make_float2(x.v[e], x.v[e + 1]), m2), k2);
-        const float2 g = __fmul2_rn(make_float2(ex2(t.x), ex2(t.y)), c2);
-        x.v[e] = g.x;
-        x.v[e + 1] = g.y;
-      }
+      const float2 c2 = {coef, coef};
+      x.each2([&](float2 e) { return __fmul2_rn(e, c2); });
       if (w == 0.f) {   // not 0 * NaN
 #pragma unroll
         for (int e = 0; e < E; ++e) x.v[e] = 0.f;
@@ -194,13 +187,13 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
         for (int i = 1; i < kSlots; ++i)
 #pragma unroll
           for (int q = 0; q < i; ++q)
-            if (i < K && pc[i] >= 0 && pc[i] == pc[q]) q_of[q] += pq[i];
+            if (pc[i] >= 0 && pc[i] == pc[q]) q_of[q] += pq[i];
       } else if (__any_sync(0xffffffffu, twice)) {
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) q_of[i] = 0.f;
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
-          if (i * G >= K) continue;
+          if (!has(i)) continue;
           for (int j = 0; j < G; ++j) {
             const int c = __shfl_sync(0xffffffffu, pc[i], j, G);
             const float q = __shfl_sync(0xffffffffu, pq[i], j, G);
@@ -213,18 +206,18 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
       const float mass_s = mass / s.s;
 #pragma unroll
       for (int i = 0; i < kSlots; ++i)
-        if (i * G < K && in && w != 0.f && pc[i] >= 0 && !(other >> i & 1))
+        if (has(i) && in && w != 0.f && pc[i] >= 0 && !(other >> i & 1))
           sh_put<T>(row + pc[i] * ES, scale * (mass_s * prob((pz[i] - s.m) * a.inv_t) - q_of[i]));
     }
   });
-  if (!BWD && a.part) leave_part<kTileThreads>(sum_loss, sum_w, a.part);
+  if (!BWD && a.part) leave_part<kTileThreads>(sum_loss.value(), sum_w.value(), a.part);
 }
 
 // As for other tiles, with lanes enough for the pairs.
 inline TileKind pairs_kind(int C, int K, int es) {
   TileKind kind = tile_kind(C, es);
-  if (K <= kind.g * kSlots) return kind;
-  if (C <= 64 && K <= 8 * kSlots) return {8, 8, kind.vec};
+  if (K <= kind.g * kMostSlots) return kind;
+  if (C <= 64 && K <= 8 * kMostSlots) return {8, 8, kind.vec};
   if (C <= 256) return {32, 8, kind.vec};
   return {32, 32, kind.vec};
 }
@@ -240,10 +233,14 @@ cudaError_t launch_tiles(Args& a, bool bwd, int* blocks, cudaStream_t s) {
   auto launch = [&](auto c) {
     constexpr int G = decltype(c)::G, E = decltype(c)::E;
     constexpr bool VEC = decltype(c)::VEC;
-    if (plain && bwd) return launch_tile(tile_kernel<T, G, E, VEC, true, true>, a.tile, s, a);
-    if (plain) return launch_tile(tile_kernel<T, G, E, VEC, false, true>, a.tile, s, a);
-    if (bwd) return launch_tile(tile_kernel<T, G, E, VEC, true, false>, a.tile, s, a);
-    return launch_tile(tile_kernel<T, G, E, VEC, false, false>, a.tile, s, a);
+    if (plain && a.K <= 2 * G) {
+      if (bwd) return launch_tile(tile_kernel<T, G, E, VEC, true, 2, true>, a.tile, s, a);
+      return launch_tile(tile_kernel<T, G, E, VEC, false, 2, true>, a.tile, s, a);
+    }
+    if (plain && bwd) return launch_tile(tile_kernel<T, G, E, VEC, true, 4, true>, a.tile, s, a);
+    if (plain) return launch_tile(tile_kernel<T, G, E, VEC, false, 4, true>, a.tile, s, a);
+    if (bwd) return launch_tile(tile_kernel<T, G, E, VEC, true, 4, false>, a.tile, s, a);
+    return launch_tile(tile_kernel<T, G, E, VEC, false, 4, false>, a.tile, s, a);
   };
   if (kind.g == 8 && kind.e == 8) return kind.vec ? launch(TileConst<8, 8, true>{}) : launch(TileConst<8, 8, false>{});
   if (kind.g == 32 && kind.e == 8) return kind.vec ? launch(TileConst<32, 8, true>{}) : launch(TileConst<32, 8, false>{});

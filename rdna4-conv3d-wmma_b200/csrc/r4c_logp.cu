@@ -70,19 +70,6 @@ struct RowOut {
 };
 
 // ---- rows in registers -------------------------------------------------------
-template <typename Row>
-__device__ __forceinline__ Run row_run(const Row& x, float k) {
-  Run2 r = run2_empty();
-  r.m = x.max();
-  run2_add<sizeof(x.v) / sizeof(float), true>(r, x.v, k);   // places outside the row hold -inf and add nothing
-  return r.join();
-}
-template <int G>
-__device__ __forceinline__ void run_group(Run& r) {
-  r.s = group_sum<G>(r.s);
-  r.u = group_sum<G>(r.u);
-}
-
 // Keys that order a row's values, equal ones by lowest class; the least is no
 // class. 16-bit types: 19 bits of the value hold it exactly, 13 the class.
 template <typename T> struct TopKey {
@@ -109,28 +96,29 @@ template <> struct TopKey<float> {
 template <typename T, int G, int E, bool VEC>
 __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
   const float k = a.inv_t * kLog2e;
-  tile_walk<T, G, false>(a.tile, a.v, a.z, a.v, nullptr, [&](int64_t r, uint32_t row, bool in) {
+  tile_walk<T, G, false>(a.tile, a.v, a.z, a.v, nullptr, [&](int64_t r0, int r, uint32_t row, bool in) {
     TileRow<T, G, E, VEC> x;
     x.load(row, a.C);
-    Run run = row_run(x, k);
-    run_group<G>(run);
+    const Run run = tile_run(x, k);
     const RowOut o(run, lg2(run.s), a.inv_t);
     if (in && x.lane == 0) {
       if (a.target) {
-        const int t = label_of(a.target, r, a.C, a.ignore, a.err);
-        a.logp[r] = t < 0 ? 0.f : o.logp(sh_get<T>(row + t * (int)sizeof(T)));
+        const int t = label_of(a.target + r0, r, a.C, a.ignore, a.err);
+        (a.logp + r0)[r] = t < 0 ? 0.f : o.logp(sh_get<T>(row + t * (int)sizeof(T)));
       }
-      a.entropy[r] = o.entropy(run);
-      a.lse[r] = o.lse();
+      (a.entropy + r0)[r] = o.entropy(run);
+      (a.lse + r0)[r] = o.lse();
     }
     if (a.K == 0) return;
-    // the most probable classes, one after the other
+    // the most probable classes, one after the other, from the row as it was
+    x.load(row, a.C);
     using Key = TopKey<T>;
     typename Key::type key[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) key[e] = x.ok(e) ? Key::make(x.v[e], x.cls(e)) : Key::kNone;
-    float* tl = a.top_logp + r * a.K;
-    int32_t* ti = a.top_index + r * a.K;
+    for (int e = 0; e < E; ++e) key[e] = Key::make(x.v[e], x.cls(e));   // past the row: -inf, ranked after every class
+    if (x.c0 < 0) key[0] = Key::kNone;                                  // the half word before it is no class
+    float* tl = a.top_logp + r0 * a.K + r * a.K;
+    int32_t* ti = a.top_index + r0 * a.K + r * a.K;
     auto next = [&](float* l, int* c) {
       typename Key::type b = key[0];
 #pragma unroll
@@ -171,34 +159,25 @@ __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
 template <typename T, int G, int E, bool VEC>
 __global__ void __launch_bounds__(kTileThreads) bwd_tile_kernel(BwdArgs a) {
   const float k = a.inv_t * kLog2e;
-  tile_walk<T, G, true>(a.tile, a.v, a.z, a.dv, a.dz, [&](int64_t r, uint32_t row, bool in) {
+  tile_walk<T, G, true>(a.tile, a.v, a.z, a.dv, a.dz, [&](int64_t r0, int r, uint32_t row, bool in) {
     TileRow<T, G, E, VEC> x;
+    const int t = a.target ? label_of(a.target + r0, r, a.C, a.ignore, a.err) : -1;
+    const float gl = a.g_logp && t >= 0 ? (a.g_logp + r0 * a.gl_inc)[r * a.gl_inc] : 0.f;
+    const float gh = a.g_entropy ? (a.g_entropy + r0 * a.gh_inc)[r * a.gh_inc] : 0.f;
+    const float gs = a.g_lse ? (a.g_lse + r0 * a.gs_inc)[r * a.gs_inc] : 0.f;
     x.load(row, a.C);
-    const int t = label_of(a.target, r, a.C, a.ignore, a.err);
-    const float gl = a.g_logp && t >= 0 ? a.g_logp[r * a.gl_inc] : 0.f;
-    const float gh = a.g_entropy ? a.g_entropy[r * a.gh_inc] : 0.f;
-    const float gs = a.g_lse ? a.g_lse[r * a.gs_inc] : 0.f;
-    Run run = row_run(x, k);
-    run_group<G>(run);
+    const Run run = tile_run(x, k);   // x: the exponents
     const float l2s = lg2(run.s);
     const bool none = (gl == 0.f && gh == 0.f && gs == 0.f) || run.s == 0.f;
     const float h = kLn2 * (l2s - __fdividef(run.u, run.s));
     const float f = none ? 0.f : __fdividef(a.inv_t, run.s), ca = f * (gs - gl - gh * h), cb = f * gh * kLn2;
     const float mm = -anchor(run.m), lb = cb * l2s;
-    const float2 m2 = {mm, mm}, k2 = {k, k};
     // 2^t (ca - cb (t - l2s))
-    const float c0 = none ? 0.f : ca + lb;
-    const float2 c2 = {c0, c0}, b2 = {none ? 0.f : -cb, none ? 0.f : -cb};
+    const float c0 = none ? 0.f : ca + lb, b0 = none ? 0.f : -cb;
+    const float2 c2 = {c0, c0}, b2 = {b0, b0};
     float zt = 0.f;
     if (t >= 0) zt = sh_get<T>(row + t * (int)sizeof(T));
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      float2 q = __fmul2_rn(__fadd2_rn(make_float2(x.v[e], x.v[e + 1]), m2), k2);
-      q = make_float2(max_nan(q.x, kFloor), max_nan(q.y, kFloor));
-      q = __fmul2_rn(make_float2(ex2(q.x), ex2(q.y)), __ffma2_rn(b2, q, c2));
-      x.v[e] = q.x;
-      x.v[e + 1] = q.y;
-    }
+    x.each2([&](float2 q) { return __fmul2_rn(make_float2(ex2(q.x), ex2(q.y)), __ffma2_rn(b2, q, c2)); });
     if (G > 1) __syncwarp();   // every lane has read the row (and the label's logit)
     if (in) x.store(x.v);
     if (G > 1) __syncwarp();
@@ -210,141 +189,170 @@ __global__ void __launch_bounds__(kTileThreads) bwd_tile_kernel(BwdArgs a) {
 }
 
 // ---- rows streamed -----------------------------------------------------------
-constexpr int kCand = 2048;   // candidate keys a block keeps while it selects
-
-// The K largest keys of a block's part of a row, in order, into sh.top
-// (0 where the part has fewer). Each thread knows the largest value of its
-// own vectors and the vector it is in; the K-th largest of those is a bound
-// that at least K elements reach, and few more do, so only the vectors of
-// the threads that reach it are looked at again. Keys are unique (value,
-// then class), which makes the result exact whatever the ties; if elements
-// crowd above the bound (more than kCand) it is raised by bisection first.
+// The K largest keys of a block's part of a row (unique: value, then class,
+// so the result is exact whatever the ties). While it streams, each thread
+// notes the largest value of each quarter of its own vectors. The K-th
+// largest of these is a bound that at least K elements reach, and few more
+// do, so only the quarters that reach it are read again, from L2 as a rule.
+// If elements crowd above the bound (more than there are places: a row of
+// equal values, for one) it is raised by bisection over them first.
+constexpr int kQuarters = 4;
+// Candidate places; a cluster's first block also takes in the others' lists.
+__host__ __device__ inline int cand_places(int cs, int K) { return cs * K > 512 ? cs * K : 512; }
 struct TopShared {
-  uint64_t* cand;     // kCand
+  uint64_t* cand;     // `places` of them
   uint64_t* top;      // R4C_TOPK_MAX
-  uint64_t* keys;     // a thread's best, as a lower bound
-  int* active;        // threads that reach the bound
-  uint64_t tau;
-  int n_active, n_cand;
+  uint32_t* best;     // [kQuarters][threads]: the order of a quarter's largest value, 0: no vector
+  int* active;        // [kQuarters * threads]: quarters that reach the bound
+  uint32_t bound;
+  int places, n_active, n_cand;
 };
+inline size_t top_bytes(int cs, int K, int threads) {
+  return (cand_places(cs, K) + R4C_TOPK_MAX) * sizeof(uint64_t) + kQuarters * threads * 2 * sizeof(uint32_t);
+}
+__device__ __forceinline__ uint32_t order_of(float v) { return (uint32_t)(rank_key(v, 0) >> 32); }
 
+// Called by one warp: the largest value (up to the 13 bits that 16-bit types
+// do not have) that at least K of the n orders at p reach; a slightly smaller
+// one if that is quicker found, 0 with fewer than K of them.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t warp_bound(const uint32_t* p, int K) {
+  constexpr int SH = sizeof(T) == 4 ? 0 : 13;
+  const int lane = threadIdx.x & 31;
+  uint32_t kv[N], lo = ~0u, hi = 0;
+  int reach = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    kv[i] = p[lane + 32 * i] >> SH;
+    reach += kv[i] != 0;
+    hi = kv[i] > hi ? kv[i] : hi;
+    if (kv[i] && kv[i] < lo) lo = kv[i];
+  }
+  reach = __reduce_add_sync(0xffffffffu, reach);
+  if (reach < K) return 0;
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi) + 1;   // none reach it
+  const int enough = K + (K >> 1) + 2;
+  while (reach > enough && hi - lo > 1) {
+    const uint32_t mid = lo + ((hi - lo) >> 1);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) c += kv[i] >= mid;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= K) {
+      lo = mid;
+      reach = c;
+    } else {
+      hi = mid;
+    }
+  }
+  return lo << SH;
+}
+
+// (Called, not inlined: its registers would spill the streaming loop's.)
 template <typename T, int NT>
-__device__ void block_topk(const VecRow<T>& x, int v0, int v1, int f0, int f1, float tm, int tv, int K, bool skip,
-                           TopShared& sh) {
-  constexpr int VE = Vec<T>::kElems;
+__device__ __noinline__ void select_top(const uint4* p, const T* row, int off, int C, int v0, int v1, int f0, int f1,
+                                        int per, int K, TopShared* shp) {
+  constexpr int VE = Vec<T>::kElems, U = 4;
+  TopShared& sh = *shp;
   const int tid = threadIdx.x;
-  const bool have = tv >= 0;
-  const int nd = f1 - f0 < 0 ? 0 : f1 - f0 < NT ? f1 - f0 : NT;   // threads with a vector
-  sh.keys[tid] = have ? rank_key(tm, x.cls(tv) + VE - 1) : 0;
-  if (tid == 0) {
-    sh.n_active = 0;
-    sh.n_cand = 0;
-    sh.tau = 0;
-  }
   for (int j = tid; j < K; j += NT) sh.top[j] = 0;
-  __syncthreads();
-  if (nd >= K && tid < 32) {
-    uint64_t kk[NT / 32], lo = ~0ull, hi = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 32; ++i) {
-      kk[i] = sh.keys[tid + 32 * i];
-      hi = kk[i] > hi ? kk[i] : hi;
-      if (kk[i] && kk[i] < lo) lo = kk[i];
+  if (tid < 32) {
+    const uint32_t b = warp_bound<T, kQuarters * NT / 32>(sh.best, K);
+    if (tid == 0) {
+      sh.bound = b;
+      sh.n_active = sh.n_cand = 0;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const uint64_t l = __shfl_xor_sync(0xffffffffu, lo, o), h = __shfl_xor_sync(0xffffffffu, hi, o);
-      lo = l < lo ? l : lo;
-      hi = h > hi ? h : hi;
-    }
-    hi += 1;   // none reach it; all nd >= K reach lo
-    const int enough = K + (K >> 1) + 4;
-    int reach = nd;
-    while (reach > enough && hi - lo > 1) {
-      const uint64_t mid = lo + ((hi - lo) >> 1);
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < NT / 32; ++i) c += kk[i] >= mid;
-      c = __reduce_add_sync(0xffffffffu, c);
-      if (c >= K) {
-        lo = mid;
-        reach = c;
-      } else {
-        hi = mid;
-      }
-    }
-    if (tid == 0) sh.tau = lo;
   }
   __syncthreads();
-  uint64_t tau = sh.tau;
-  if (have && rank_key(tm, x.cls(tv)) >= tau) sh.active[atomicAdd(&sh.n_active, 1)] = tid;
+  uint64_t bound = (uint64_t)sh.bound << 32;
+#pragma unroll
+  for (int q = 0; q < kQuarters; ++q) {
+    const uint32_t o = sh.best[q * NT + tid];
+    if (o && o >= sh.bound) sh.active[atomicAdd(&sh.n_active, 1)] = q * NT + tid;
+  }
   __syncthreads();
-  const int iters = (f1 - f0 + NT - 1) / NT;
-  const int items = skip ? 0 : sh.n_active * iters;
-  // every element that reaches `bound`: kept in cand (keep) or counted
-  auto scan = [&](uint64_t bound, bool keep) {
+  const int items = sh.n_active * per, places = sh.places;
+  uint64_t lo = bound, hi = ~0ull;
+  bool keep = true;   // keep the elements that reach the bound, or count them
+  for (;;) {
+    const float low = bound >> 32 <= 0x007fffffu ? -INFINITY : key_value(bound | ((bound >> 63) || sizeof(T) == 4 ? 0ull : 0x1fffull << 32));
+    int count = 0;
     auto look = [&](float z, int c) {
       const uint64_t key = rank_key(z, c);
-      if (key >= bound) {
+      if (key < bound) return;
+      if (keep) {
         const int at = atomicAdd(&sh.n_cand, 1);
-        if (keep && at < kCand) sh.cand[at] = key;
+        if (at < places) sh.cand[at] = key;
+      } else {
+        ++count;
       }
     };
-    for (int q = tid; q < items; q += NT) {
-      const int v = f0 + sh.active[q / iters] + (q % iters) * NT;
-      if (v < f1) {
-        float y[VE];
-        Vec<T>::split(__ldg(x.p + v), y);
+    for (int i0 = tid; i0 < items; i0 += U * NT) {
+      uint4 w[U];
+      int v[U];
 #pragma unroll
-        for (int i = 0; i < VE; ++i) look(y[i], x.cls(v) + i);
+      for (int j = 0; j < U; ++j) {
+        const int i = i0 + j * NT;
+        v[j] = f1;
+        if (i < items) {
+          const int g = sh.active[i / per];
+          v[j] = f0 + g % NT + ((g / NT) * per + i % per) * NT;
+        }
+        w[j] = v[j] < f1 ? __ldg(p + v[j]) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        if (v[j] >= f1 || Vec<T>::top(w[j]) < low) continue;
+        float y[VE];
+        Vec<T>::split(w[j], y);
+        unsigned hits = 0;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) hits |= (unsigned)(y[e] >= low) << e;
+        const T* at = reinterpret_cast<const T*>(p + v[j]);
+        for (; hits; hits &= hits - 1) {
+          const int e = __ffs(hits) - 1;
+          look(Elem<T>::to_f(at[e]), v[j] * VE - off + e);
+        }
       }
     }
-    if (!skip) {   // the partial vectors at the row's ends
-      if (f0 > v0 && tid < VE) {
-        const int c = x.cls(v0) + tid;
-        if (c >= 0 && c < x.C) look(Elem<T>::to_f(x.row[c]), c);
-      }
-      if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) {
-        const int c = x.cls(f1) + tid - 32;
-        if (c >= 0 && c < x.C) look(Elem<T>::to_f(x.row[c]), c);
-      }
+    // the partial vectors at the row's ends
+    if (f0 > v0 && tid < VE) {
+      const int c = v0 * VE - off + tid;
+      if (c >= 0 && c < C) look(Elem<T>::to_f(row[c]), c);
     }
+    if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) {
+      const int c = f1 * VE - off + tid - 32;
+      if (c >= 0 && c < C) look(Elem<T>::to_f(row[c]), c);
+    }
+    if (!keep && count) atomicAdd(&sh.n_cand, count);
     __syncthreads();
     const int n = sh.n_cand;
+    if (keep && n <= places) break;
+    // raise the bound: at least K reach lo, fewer than K reach hi; at most 64 halvings
+    if (!keep) {
+      if (n < K) hi = bound;
+      else lo = bound;
+    }
+    keep = (!keep && n >= K && n <= places) || hi - lo <= 1;
+    bound = keep ? lo : lo + ((hi - lo) >> 1);
     __syncthreads();
     if (tid == 0) sh.n_cand = 0;
     __syncthreads();
-    return n;
-  };
-  int n = scan(tau, true);
-  if (n > kCand) {
-    uint64_t lo = tau, hi = ~0ull;
-    while (hi - lo > 1) {
-      const uint64_t mid = lo + ((hi - lo) >> 1);
-      const int c = scan(mid, false);
-      if (c >= K) {
-        lo = mid;
-        if (c <= kCand) break;
-      } else {
-        hi = mid;
-      }
-    }
-    n = scan(lo, true);
-    n = n < kCand ? n : kCand;
   }
+  // their order, by counting
+  const int n = sh.n_cand;
   for (int i = tid; i < n; i += NT) {
     const uint64_t key = sh.cand[i];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) rank += sh.cand[j] > key;
     if (rank < K) sh.top[rank] = key;
   }
   __syncthreads();
 }
 
-#ifndef KS
-#define KS 2
-#endif
-constexpr int kBatch = 4, kStages = KS;
+constexpr int kBatch = 4, kStages = 2;
 template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
   constexpr int VE = Vec<T>::kElems, U = kBatch;
@@ -358,9 +366,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
   if (cs > 1) cr = cluster_rank();
   if (TOP && tid == 0) {
     top.cand = reinterpret_cast<uint64_t*>(dyn + VecRing<NT, U, kStages>::kBytes);
-    top.top = top.cand + kCand;
-    top.keys = top.top + R4C_TOPK_MAX;
-    top.active = reinterpret_cast<int*>(top.keys + NT);
+    top.places = cand_places((int)cs, a.K);
+    top.top = top.cand + top.places;
+    top.best = reinterpret_cast<uint32_t*>(top.top + R4C_TOPK_MAX);
+    top.active = reinterpret_cast<int*>(top.best + kQuarters * NT);
   }
   __syncthreads();
   const float k = a.inv_t * kLog2e;
@@ -372,48 +381,46 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
     int v0, v1, f0, f1;
     stream.share(x, &v0, &v1, &f0, &f1);
     Run2 part = run2_empty();
-    float tm = 0.f;   // the largest value of this thread's full vectors, and the first vector that has it
-    int tv = -1;
-    auto track = [&](float vm, int v) {
-      if (TOP && (tv < 0 || vm > tm)) {
-        tm = vm;
-        tv = v;
-      }
-    };
-    int v = f0 + tid;
-    for (int left = f1 - f0; left > 0; left -= U * NT, v += U * NT) {
+    // batches of a quarter, and the vectors of a thread in it
+    const int quarter = (f1 - f0 + kQuarters * U * NT - 1) / (kQuarters * U * NT), per = quarter * U;
+    float tm = -INFINITY;
+    int b = 0, q = 0;
+    if (TOP) {
+#pragma unroll
+      for (int i = 0; i < kQuarters; ++i) top.best[i * NT + tid] = 0;
+    }
+    for (int left = f1 - f0; left > 0; left -= U * NT) {
       uint4 w[U];
+      float vm[U];
       stream.take(w);
-      if (left >= U * NT) {
-        float vm[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-          vm[i] = Vec<T>::top(w[i]);
-          track(vm[i], v + i * NT);
-        }
-        run2_raise<true>(part, fmaxf(fmaxf(vm[0], vm[1]), fmaxf(vm[2], vm[3])), k);
-        run2_batch<VE, U>(part, k, [&](int i, float* y) { Vec<T>::split(i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3], y); });
-      } else {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-          if (v + i * NT >= f1) break;
-          const float vm = Vec<T>::top(w[i]);
-          track(vm, v + i * NT);
-          run2_raise<true>(part, vm, k);
-          run2_batch<VE, 1>(part, k, [&](int, float* y) { Vec<T>::split(w[i], y); });
+      for (int i = 0; i < U; ++i) {
+        if (left < U * NT && tid + i * NT >= left)
+          w[i] = make_uint4(Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf);
+        vm[i] = Vec<T>::top(w[i]);
+      }
+      const float bm = fmaxf(fmaxf(vm[0], vm[1]), fmaxf(vm[2], vm[3]));
+      run2_raise<true>(part, bm, k);
+      run2_batch<VE, U>(part, k, [&](int i, float* y) { Vec<T>::split(i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3], y); });
+      if (TOP) {
+        tm = fmaxf(tm, bm);
+        if (++b == quarter || left <= U * NT) {
+          // (a quarter counts where this thread has a vector in it)
+          if (f0 + tid + q * per * NT < f1) top.best[q * NT + tid] = order_of(tm);
+          tm = -INFINITY;
+          b = 0;
+          ++q;
         }
       }
     }
-    if (f0 > v0 && tid < VE) {   // partial vectors: one element a thread
-      const int c = x.cls(v0) + tid;
+    // partial vectors: one element a thread
+    auto edge = [&](int c) {
       if (c >= 0 && c < a.C) run2_one<true>(part, Elem<T>::to_f(x.row[c]), k);
-    }
-    if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) {
-      const int c = x.cls(f1) + tid - 32;
-      if (c >= 0 && c < a.C) run2_one<true>(part, Elem<T>::to_f(x.row[c]), k);
-    }
-    Run run = run_block<NT>(part.join(), k, runs);
-    if (TOP) block_topk<T, NT>(x, v0, v1, f0, f1, tm, tv, a.K, isnan(run.s), top);
+    };
+    if (f0 > v0 && tid < VE) edge(x.cls(v0) + tid);
+    if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) edge(x.cls(f1) + tid - 32);
+    Run run = run_block<NT>(part.join(), k, runs);   // (and the quarters' values are in place)
+    if (TOP) select_top<T, NT>(x.p, x.row, x.off, a.C, v0, v1, f0, f1, per, a.K, &top);
     if (cs > 1) {
       if (tid == 0) mine = run;
       cluster_sync();
@@ -445,14 +452,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
           if (cs > 1) {
             key = top.cand[i];
             rank = 0;
-            for (uint32_t q = 0; key && q < cs; ++q) {
-              int lo = 0, hi = a.K;
-              while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (top.cand[q * a.K + mid] > key) lo = mid + 1;
-                else hi = mid;
+            for (uint32_t q0 = 0; key && q0 < cs; q0 += 4) {   // four searches at a time
+              int at[4] = {0, 0, 0, 0};
+              for (int step = 64; step; step >>= 1) {
+                if (step > a.K) continue;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (q0 + j < cs && at[j] + step <= a.K && top.cand[(q0 + j) * a.K + at[j] + step - 1] > key) at[j] += step;
               }
-              rank += lo;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (q0 + j < cs && at[j] < a.K && top.cand[(q0 + j) * a.K + at[j]] > key) ++at[j];   // all of 2^n
+                rank += at[j];
+              }
             }
           }
           if (o.bad && i < a.K) {
@@ -515,8 +527,8 @@ __global__ void __launch_bounds__(kGradThreads) bwd_block_kernel(BwdArgs a) {
 template <typename T, int NT>
 cudaError_t launch_fwd_block(const FwdArgs& a, cudaStream_t s) {
   const int cs = cluster_size(a.nrows, a.C, sizeof(T), NT);
-  constexpr size_t ring = VecRing<NT, kBatch, kStages>::kBytes;
-  const size_t smem = ring + (a.K > 0 ? (kCand + R4C_TOPK_MAX + NT) * sizeof(uint64_t) + NT * sizeof(int) : 0);
+  const size_t smem = VecRing<NT, kBatch, kStages>::kBytes +
+                      (a.K > 0 ? top_bytes(cs, a.K, NT) : 0);
   const int64_t most = (int64_t)kSMs * blocks_per_sm(NT, smem);
   int64_t grid = a.nrows * cs;
   if (cs == 1 && grid > most) grid = most;

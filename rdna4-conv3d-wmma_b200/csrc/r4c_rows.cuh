@@ -108,6 +108,17 @@ __device__ __forceinline__ bool group_any(bool p) {
   return ((b >> ((threadIdx.x & 31) & ~(G - 1))) & ((1u << (G & 31)) - 1u)) != 0;
 }
 
+// A sum of fp32 numbers that keeps what each addition rounds off.
+struct Sum2 {
+  float s = 0.f, r = 0.f;
+  __device__ __forceinline__ void add(float x) {
+    const float y = x - r, t = s + y;
+    r = fabsf(t) < INFINITY ? (t - s) - y : 0.f;
+    s = t;
+  }
+  __device__ __forceinline__ double value() const { return (double)s - (double)r; }
+};
+
 // ---- 32-bit words of logits, and their largest value without unpacking them all -------------------------------------------------
 template <typename T> struct Word;
 template <> struct Word<float> {
@@ -161,6 +172,12 @@ template <> struct Word<__half> {
   }
 };
 
+// Running maximum and sums of exponentials, t_c = (z_c - m) k with
+// k = log2(e) / T: s = sum 2^t, u = sum 2^t t. m = -inf: nothing finite yet.
+struct Run {
+  float m, s, u;
+};
+
 // ---- tile: rows held in registers --------------------------------------------
 enum { kGather = 0, kCopy = 1, kCopyPadded = 2 };
 struct Tile {
@@ -180,7 +197,7 @@ constexpr int kTileStages = 3;
 // lane 0: not a class).
 template <typename T, int G, int E, bool VEC>
 struct TileRow {
-  static constexpr int kW = Word<T>::kElems;
+  static constexpr int kG = G, kW = Word<T>::kElems;
   static constexpr int kU = VEC ? 16 / (int)sizeof(T) : kW;   // elements of a unit
   static constexpr int kN = E / kU;                           // units of a lane
   float v[E];
@@ -189,9 +206,11 @@ struct TileRow {
 
   static __device__ __forceinline__ constexpr int off(int e) { return e / kU * (G * kU) + e % kU; }
   __device__ __forceinline__ int cls(int e) const { return c0 + off(e); }
-  // Units whose elements are classes in every lane of every row (but for the half word before a row).
-  __device__ __forceinline__ bool inner(int i) const { return kU * G * (i + 1) <= C; }
-  __device__ __forceinline__ bool ok(int e) const { return (unsigned)cls(e) < (unsigned)C; }
+  // Units are checked in groups: one test for all lanes and elements of a
+  // group, and element by element only in the group where the row ends.
+  static constexpr int kGroup = VEC || kN < 4 ? (VEC ? 1 : kN) : 4;
+  __device__ __forceinline__ bool whole(int i) const { return kU * G * (i + kGroup) <= C; }
+  static __device__ __forceinline__ constexpr int step(int i) { return i * (G * kU * (int)sizeof(T)); }
 
   __device__ __forceinline__ void load(uint32_t row, int classes) {
     C = classes;
@@ -199,53 +218,86 @@ struct TileRow {
     c0 = kU * lane - (kU == 2 ? (row >> 1) & 1 : 0);
     at = (kU == 2 ? row & ~3u : row) + lane * (kU * (int)sizeof(T));
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      float* x = v + i * kU;
-      const uint32_t a = at + i * (G * kU * (int)sizeof(T));
+    for (int i0 = 0; i0 < kN; i0 += kGroup) {
       if (VEC) {
         uint32_t w[4] = {Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf};
-        if (inner(i) || cls(i * kU) < C)
+        if (cls(i0 * kU) < C)
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + step(i0)) : "memory");
 #pragma unroll
-        for (int h = 0; h < 4; ++h) Word<T>::split(w[h], x + h * kW);
+        for (int h = 0; h < 4; ++h) Word<T>::split(w[h], v + i0 * kU + h * kW);
       } else {
-        uint32_t w = Word<T>::kNegInf;
-        if (inner(i) || cls(i * kU) < C) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(a) : "memory");
-        Word<T>::split(w, x);
-        if (kU == 2 && i == 0 && c0 < 0) x[0] = -INFINITY;
-        if (kU == 2 && !inner(i) && cls(i * kU + 1) >= C) x[1] = -INFINITY;
+        uint32_t w[kGroup];
+        if (whole(i0)) {
+#pragma unroll
+          for (int j = 0; j < kGroup; ++j)
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[j]) : "r"(at + step(i0 + j)) : "memory");
+        } else {
+#pragma unroll
+          for (int j = 0; j < kGroup; ++j) {
+            const int c = cls((i0 + j) * kU);
+            w[j] = Word<T>::kNegInf;
+            if (c < C) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[j]) : "r"(at + step(i0 + j)) : "memory");
+            if (kU == 2 && c + 1 >= C) w[j] = (w[j] & 0xffffu) | (Word<T>::kNegInf & 0xffff0000u);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) Word<T>::split(w[j], v + (i0 + j) * kU);
       }
     }
+    if (kU == 2 && c0 < 0) v[0] = -INFINITY;
   }
   // Writes g over the row in shared memory.
   __device__ __forceinline__ void store(const float* g) const {
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const float* x = g + i * kU;
-      const uint32_t a = at + i * (G * kU * (int)sizeof(T));
+    for (int i0 = 0; i0 < kN; i0 += kGroup) {
       if (VEC) {
         uint32_t w[4];
 #pragma unroll
-        for (int h = 0; h < 4; ++h) w[h] = Word<T>::join(x + h * kW);
-        if (inner(i) || cls(i * kU) < C)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                       : "memory");
-      } else {
-        const uint32_t w = Word<T>::join(x);
-        const bool lo = !(kU == 2 && i == 0) || c0 >= 0;
-        const bool in = inner(i) || cls(i * kU) < C, hi = kU == 1 || inner(i) || cls(i * kU + 1) < C;
-        if (in && lo && hi) asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(w) : "memory");
-        else if (in && !lo && hi) asm volatile("st.shared.b16 [%0], %1;" ::"r"(a + 2), "h"((uint16_t)(w >> 16)) : "memory");
-        else if (in && lo) asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"((uint16_t)w) : "memory");
+        for (int h = 0; h < 4; ++h) w[h] = Word<T>::join(g + i0 * kU + h * kW);
+        if (cls(i0 * kU) < C)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + step(i0)), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                       "r"(w[3]) : "memory");
+        continue;
+      }
+      const bool all = whole(i0);
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) {
+        const uint32_t a = at + step(i0 + j), w = Word<T>::join(g + (i0 + j) * kU);
+        const int c = cls((i0 + j) * kU);
+        const bool lo = !(kU == 2 && i0 + j == 0) || c0 >= 0;   // else the half word is another row's
+        if (lo && (all || c + kU <= C)) asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(w) : "memory");
+        else if (!lo) asm volatile("st.shared.b16 [%0], %1;" ::"r"(a + 2), "h"((uint16_t)(w >> 16)) : "memory");
+        else if (kU == 2 && c < C) asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"((uint16_t)w) : "memory");
       }
     }
   }
+  // Values are worked on eight at a time, as far as the row reaches in any lane.
+  static constexpr int kPart = E < 8 ? E : 8;
+  __device__ __forceinline__ bool reaches(int e0) const { return e0 == 0 || off(e0) < C; }
   __device__ __forceinline__ float max() const {
     float m = v[0];
 #pragma unroll
-    for (int e = 1; e < E; ++e) m = fmaxf(m, v[e]);
+    for (int e0 = 0; e0 < E; e0 += kPart) {
+      if (!reaches(e0)) break;
+#pragma unroll
+      for (int e = e0; e < e0 + kPart; ++e) m = fmaxf(m, v[e]);
+    }
     return group_max<G>(m);
+  }
+  // v = f(v), two at a time.
+  template <typename F>
+  __device__ __forceinline__ void each2(F&& f) {
+#pragma unroll
+    for (int e0 = 0; e0 < E; e0 += kPart) {
+      if (!reaches(e0)) break;
+#pragma unroll
+      for (int e = e0; e < e0 + kPart; e += 2) {
+        const float2 g = f(make_float2(v[e], v[e + 1]));
+        v[e] = g.x;
+        v[e + 1] = g.y;
+      }
+    }
   }
 };
 template <typename T>
@@ -335,10 +387,11 @@ __device__ __forceinline__ void tile_flush(const Tile& t, const View& v, void* d
   }
 }
 
-// Walks the tiles of a persistent block: body(row index, shared address of
-// the row, in range) for each group of G lanes and row. All lanes of a warp
-// call body together; a group without a row of its own repeats the last one
-// and writes nothing.
+// Walks the tiles of a persistent block: body(first row of the tile, row
+// within it, shared address of the row, in range) for each group of G lanes
+// and row (in two parts: the first is the same for the block, so addresses
+// need no 64-bit arithmetic per row). All lanes of a warp call body together;
+// a group without a row of its own repeats the last one and writes nothing.
 template <typename T, int G, bool WRITES, typename Body>
 __device__ __forceinline__ void tile_walk(const Tile& t, const View& v, const void* z, const View& dv, void* dz,
                                           Body&& body) {
@@ -365,7 +418,7 @@ __device__ __forceinline__ void tile_walk(const Tile& t, const View& v, const vo
     const int nr = (int)(t.nrows - r0 < t.rows ? t.nrows - r0 : t.rows);
     for (int i = 0; i < nr; i += R) {
       const int q = i + sub, at = q < nr ? q : nr - 1;
-      body(r0 + at, base + st * t.stage_bytes + at * (t.stride * (int)sizeof(T)), q < nr);
+      body(r0, at, base + st * t.stage_bytes + at * (t.stride * (int)sizeof(T)), q < nr);
     }
     if (WRITES) {
       __syncthreads();
@@ -488,11 +541,6 @@ struct VecRow {
   __device__ __forceinline__ int cls(int v) const { return v * Vec<T>::kElems - off; }
 };
 
-// Running maximum and sums of exponentials, t_c = (z_c - m) k with
-// k = log2(e) / T: s = sum 2^t, u = sum 2^t t. m = -inf: nothing finite yet.
-struct Run {
-  float m, s, u;
-};
 __device__ __forceinline__ Run run_empty() { return {-INFINITY, 0.f, 0.f}; }
 __device__ __forceinline__ Run run_merge(const Run& a, const Run& b, float k) {
   const float m = fmaxf(a.m, b.m), mm = anchor(m);
@@ -531,6 +579,38 @@ __device__ __forceinline__ void run2_add(Run2& r, const float* x, float k) {
     if (ENT) r.u = __ffma2_rn(e, t, r.u);
   }
 }
+// A row in registers: v becomes the exponents t, and the group's run over it
+// comes back (places outside the row hold -inf and add nothing).
+template <typename Row>
+__device__ __forceinline__ Run tile_run(Row& x, float k) {
+  const float m = x.max(), mm = -anchor(m);
+  const float2 m2 = {mm, mm}, k2 = {k, k};
+  float2 s = {0.f, 0.f}, u = {0.f, 0.f};
+  x.each2([&](float2 z) {
+    float2 t = __fmul2_rn(__fadd2_rn(z, m2), k2);
+    t = make_float2(max_nan(t.x, kFloor), max_nan(t.y, kFloor));
+    const float2 e = {ex2(t.x), ex2(t.y)};
+    s = __fadd2_rn(s, e);
+    u = __ffma2_rn(e, t, u);
+    return t;
+  });
+  return {m, group_sum<Row::kG>(s.x + s.y), group_sum<Row::kG>(u.x + u.y)};
+}
+// The same without the entropy's sum: v becomes the exponentials themselves.
+template <typename Row>
+__device__ __forceinline__ Run tile_exp(Row& x, float k) {
+  const float m = x.max(), mm = -anchor(m);
+  const float2 m2 = {mm, mm}, k2 = {k, k};
+  float2 s = {0.f, 0.f};
+  x.each2([&](float2 z) {
+    const float2 t = __fmul2_rn(__fadd2_rn(z, m2), k2);
+    const float2 e = {ex2(t.x), ex2(t.y)};
+    s = __fadd2_rn(s, e);
+    return e;
+  });
+  return {m, group_sum<Row::kG>(s.x + s.y), 0.f};
+}
+
 // As run2_add<N, true>, with the exponents bounded only in a batch that turns
 // u into NaN: 0 * -inf, from a masked class (the sum s then needs no repair).
 template <int N, int U, typename Split>
