@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
   constexpr int VE = Vec<T>::kElems, U = kBatch;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ RunShared<NT> runs;
-  __shared__ Run mine;
+  __shared__ Run mine, joined;
   __shared__ float2 pair_sums[4];
   __shared__ int idx[R4C_TOPK_MAX];
   uint8_t* marks = dyn + VecRing<NT, U, kStages>::kBytes;
@@ -131,17 +131,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
         run2_one<false>(part, Elem<T>::to_f(x.row[e]), k);
     };
     if (f0 > v0 && tid < VE) edge(v0, tid);
-    if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) edge(f1, tid - 32);
+    if (f1 < v1 && f1 >= f0 && tid >= NT - VE) edge(f1, tid - (NT - VE));
     Run run = run_block<NT>(part.join(), k, runs);
     if (mark >= 0) reinterpret_cast<uint32_t*>(marks)[mark >> 5] = 0;
     if (cs > 1) {
       if (tid == 0) mine = run;
       cluster_sync();
-      if (cr == 0)
-        for (uint32_t q = 1; q < cs; ++q) run = run_merge(run, cluster_ld_run(&mine, q), k);
+      if (cr == 0) {
+        if (tid < 32) {
+          run = run_cluster(&mine, (int)cs, k);
+          if (tid == 0) joined = run;
+        }
+        __syncthreads();
+        run = joined;
+      }
     }
     if (cr == 0) {
-      __syncthreads();   // runs is free again
       Run l{first ? zc : -INFINITY, first && zc != -INFINITY ? 1.f : 0.f, 0.f};
       if (isnan(zc)) l = {0.f, zc, 0.f};
       if (a.rest) l = run_block<NT>(l, k, runs);
@@ -167,7 +172,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
       if (tid == 0) {
         float sum_q = 0.f;
         loss = 0.f;
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4 && i < NT / 32; ++i) {
           sum_q += pair_sums[i].x;
           loss += pair_sums[i].y;
         }
@@ -187,15 +192,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
 }
 
 // One block per piece of a row; the listed classes are written over at the end.
-template <typename T>
-__global__ void __launch_bounds__(kGradThreads) bwd_block_kernel(Args a) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) bwd_block_kernel(Args a) {
   __shared__ int idx[R4C_TOPK_MAX];
   __shared__ float qj[R4C_TOPK_MAX];
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x / a.segs;
   T* dz = static_cast<T*>(a.dz) + a.dv.base(r);
   extern __shared__ __align__(16) uint8_t ring[];
-  GradPiece<T> piece(static_cast<const T*>(a.z) + a.v.base(r), dz, a.C, blockIdx.x % a.segs, a.segs, ring);
+  GradPiece<T, NT> piece(static_cast<const T*>(a.z) + a.v.base(r), dz, a.C, blockIdx.x % a.segs, a.segs, ring);
   const Stats st = a.stats[r];
   if (st.w == 0.f) {
     piece.write([](float2) { return make_float2(0.f, 0.f); });
@@ -277,17 +282,21 @@ cudaError_t launch_fwd_block(const Args& a, int* blocks, cudaStream_t s) {
 template <typename T>
 cudaError_t launch_fwd(Args& a, int* blocks, cudaStream_t s) {
   if (a.C <= kTileClasses) return launch_tiles<T>(a, false, blocks, s);
-  if ((int64_t)a.C * sizeof(T) <= 16 << 10) return launch_fwd_block<T, 128>(a, blocks, s);
-  return launch_fwd_block<T, 256>(a, blocks, s);
+  if (row_threads(a.C, sizeof(T), a.K) == kWarpRow) return launch_fwd_block<T, kWarpRow>(a, blocks, s);
+  return launch_fwd_block<T, kLongRow>(a, blocks, s);
 }
 template <typename T>
 cudaError_t launch_bwd(Args& a, cudaStream_t s) {
   int blocks;
   if (a.C <= kTileClasses) return launch_tiles<T>(a, true, &blocks, s);
-  a.segs = grad_pieces(a.nrows, a.C, sizeof(T));
+  const int threads = row_threads(a.C, sizeof(T), a.K);
+  a.segs = grad_pieces(a.nrows, a.C, sizeof(T), threads);
   if (a.nrows * a.segs > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  return launch_cluster(bwd_block_kernel<T>, a.nrows * a.segs, kGradThreads, 1,
-                        VecRing<kGradThreads, kGradBatch, kGradStages>::kBytes, s, a);
+  if (threads == kWarpRow)
+    return launch_cluster(bwd_block_kernel<T, kWarpRow>, a.nrows, kWarpRow, 1,
+                          VecRing<kWarpRow, kGradBatch, kGradStages>::kBytes, s, a);
+  return launch_cluster(bwd_block_kernel<T, kLongRow>, a.nrows * a.segs, kLongRow, 1,
+                        VecRing<kLongRow, kGradBatch, kGradStages>::kBytes, s, a);
 }
 
 }  // namespace distill

@@ -29,7 +29,7 @@ struct Stats {           // per streamed row, written by the forward for the bac
   float w;               // the row's weight, 0: takes no part
 };
 
-constexpr int kParts = kSMs * 16;   // most blocks of a forward: each leaves one partial sum
+constexpr int kParts = kSMs * 32;   // most blocks of a forward: each leaves one partial sum
 
 struct Args {
   const void* z;

@@ -198,7 +198,10 @@ __global__ void __launch_bounds__(kTileThreads) bwd_tile_kernel(BwdArgs a) {
 // equal values, for one) it is raised by bisection over them first.
 constexpr int kQuarters = 4;
 // Candidate places; a cluster's first block also takes in the others' lists.
-__host__ __device__ inline int cand_places(int cs, int K) { return cs * K > 512 ? cs * K : 512; }
+__host__ __device__ inline int cand_places(int cs, int K, int threads) {
+  const int n = cs * K > 4 * K ? cs * K : 4 * K;
+  return n > 2 * threads ? n : 2 * threads;
+}
 struct TopShared {
   uint64_t* cand;     // `places` of them
   uint64_t* top;      // R4C_TOPK_MAX
@@ -208,7 +211,7 @@ struct TopShared {
   int places, n_active, n_cand;
 };
 inline size_t top_bytes(int cs, int K, int threads) {
-  return (cand_places(cs, K) + R4C_TOPK_MAX) * sizeof(uint64_t) + kQuarters * threads * 2 * sizeof(uint32_t);
+  return (cand_places(cs, K, threads) + R4C_TOPK_MAX) * sizeof(uint64_t) + kQuarters * threads * 2 * sizeof(uint32_t);
 }
 __device__ __forceinline__ uint32_t order_of(float v) { return (uint32_t)(rank_key(v, 0) >> 32); }
 
@@ -321,8 +324,8 @@ __device__ __noinline__ void select_top(const uint4* p, const T* row, int off, i
       const int c = v0 * VE - off + tid;
       if (c >= 0 && c < C) look(Elem<T>::to_f(row[c]), c);
     }
-    if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) {
-      const int c = f1 * VE - off + tid - 32;
+    if (f1 < v1 && f1 >= f0 && tid >= NT - VE) {
+      const int c = f1 * VE - off + tid - (NT - VE);
       if (c >= 0 && c < C) look(Elem<T>::to_f(row[c]), c);
     }
     if (!keep && count) atomicAdd(&sh.n_cand, count);
@@ -358,7 +361,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
   constexpr int VE = Vec<T>::kElems, U = kBatch;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ RunShared<NT> runs;
-  __shared__ Run mine;
+  __shared__ Run mine, joined;
   __shared__ TopShared top;
   const int tid = threadIdx.x;
   uint32_t cs = 1, cr = 0;
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
   if (cs > 1) cr = cluster_rank();
   if (TOP && tid == 0) {
     top.cand = reinterpret_cast<uint64_t*>(dyn + VecRing<NT, U, kStages>::kBytes);
-    top.places = cand_places((int)cs, a.K);
+    top.places = cand_places((int)cs, a.K, NT);
     top.top = top.cand + top.places;
     top.best = reinterpret_cast<uint32_t*>(top.top + R4C_TOPK_MAX);
     top.active = reinterpret_cast<int*>(top.best + kQuarters * NT);
@@ -418,20 +421,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
       if (c >= 0 && c < a.C) run2_one<true>(part, Elem<T>::to_f(x.row[c]), k);
     };
     if (f0 > v0 && tid < VE) edge(x.cls(v0) + tid);
-    if (f1 < v1 && f1 >= f0 && tid >= 32 && tid < 32 + VE) edge(x.cls(f1) + tid - 32);
+    if (f1 < v1 && f1 >= f0 && tid >= NT - VE) edge(x.cls(f1) + tid - (NT - VE));
     Run run = run_block<NT>(part.join(), k, runs);   // (and the quarters' values are in place)
     if (TOP) select_top<T, NT>(x.p, x.row, x.off, a.C, v0, v1, f0, f1, per, a.K, &top);
     if (cs > 1) {
       if (tid == 0) mine = run;
       cluster_sync();
       if (cr == 0) {
-        for (uint32_t q = 1; q < cs; ++q) run = run_merge(run, cluster_ld_run(&mine, q), k);
-        if (TOP) {
-          // the blocks' ordered lists, side by side: a key's place is the number of larger keys in each
+        if (TOP)   // the blocks' ordered lists, side by side: a key's place is the number of larger keys in each
           for (int i = tid; i < (int)cs * a.K; i += NT)
             top.cand[i] = cluster_ld_u64(cluster_map(top.top + i % a.K, i / a.K));
-          __syncthreads();
+        if (tid < 32) {
+          run = run_cluster(&mine, (int)cs, k);
+          if (tid == 0) joined = run;
         }
+        __syncthreads();
+        run = joined;
       }
     }
     if (cr == 0) {
@@ -483,12 +488,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
 }
 
 // One block per piece of a row.
-template <typename T>
-__global__ void __launch_bounds__(kGradThreads) bwd_block_kernel(BwdArgs a) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) bwd_block_kernel(BwdArgs a) {
   extern __shared__ __align__(16) uint8_t ring[];
   const int64_t r = blockIdx.x / a.segs;
   T* dz = static_cast<T*>(a.dz) + a.dv.base(r);
-  GradPiece<T> piece(static_cast<const T*>(a.z) + a.v.base(r), dz, a.C, blockIdx.x % a.segs, a.segs, ring);
+  GradPiece<T, NT> piece(static_cast<const T*>(a.z) + a.v.base(r), dz, a.C, blockIdx.x % a.segs, a.segs, ring);
   const int t = label_of(a.target, r, a.C, a.ignore, a.err);
   const float gl = a.g_logp && t >= 0 ? a.g_logp[r * a.gl_inc] : 0.f;
   const float gh = a.g_entropy ? a.g_entropy[r * a.gh_inc] : 0.f;
@@ -545,8 +550,8 @@ cudaError_t launch_fwd(FwdArgs& a, cudaStream_t s) {
       return launch_tile(fwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::VEC>, a.tile, s, a);
     });
   }
-  if ((int64_t)a.C * sizeof(T) <= 16 << 10) return launch_fwd_block<T, 128>(a, s);
-  return launch_fwd_block<T, 256>(a, s);
+  if (row_threads(a.C, sizeof(T), a.K) == kWarpRow) return launch_fwd_block<T, kWarpRow>(a, s);
+  return launch_fwd_block<T, kLongRow>(a, s);
 }
 
 template <typename T>
@@ -559,10 +564,14 @@ cudaError_t launch_bwd(BwdArgs& a, cudaStream_t s) {
       return launch_tile(bwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::VEC>, a.tile, s, a);
     });
   }
-  a.segs = grad_pieces(a.nrows, a.C, sizeof(T));
+  const int threads = row_threads(a.C, sizeof(T), 0);
+  a.segs = grad_pieces(a.nrows, a.C, sizeof(T), threads);
   if (a.nrows * a.segs > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  return launch_cluster(bwd_block_kernel<T>, a.nrows * a.segs, kGradThreads, 1,
-                        VecRing<kGradThreads, kGradBatch, kGradStages>::kBytes, s, a);
+  if (threads == kWarpRow)
+    return launch_cluster(bwd_block_kernel<T, kWarpRow>, a.nrows, kWarpRow, 1,
+                          VecRing<kWarpRow, kGradBatch, kGradStages>::kBytes, s, a);
+  return launch_cluster(bwd_block_kernel<T, kLongRow>, a.nrows * a.segs, kLongRow, 1,
+                        VecRing<kLongRow, kGradBatch, kGradStages>::kBytes, s, a);
 }
 
 }  // namespace logp

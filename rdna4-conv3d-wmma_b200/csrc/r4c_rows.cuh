@@ -35,6 +35,12 @@ constexpr float kRestNoise = 1e-6f;
 constexpr int kTileClasses = 1024;
 constexpr int kTileThreads = 256;
 constexpr int kSMs = 148;
+// Threads to a streamed row: one warp up to 16 KB (what a row costs beyond its
+// elements is paid per warp: 16384 rows of 1500 bf16 classes take half the
+// time of 128 threads), else 256. A thread holds at most one of the k pairs
+// or asks for at most a quarter of them to be found per vector it has.
+constexpr int kWarpRow = 32, kLongRow = 256;
+inline int row_threads(int C, int es, int k) { return (int64_t)C * es <= 16 << 10 && k <= kWarpRow ? kWarpRow : kLongRow; }
 
 struct View {
   int64_t inner, so, si, sc;   // inner 0: one stride walks all rows
@@ -721,17 +727,18 @@ struct VecRing {
 
 // A block's piece of a row's gradient: dz = pair(z) for every class of the
 // piece, two at a time.
-constexpr int kGradThreads = 256, kGradBatch = 4, kGradStages = 3;
+constexpr int kGradBatch = 4, kGradStages = 3;
 // Pieces of a row: about sixteen vectors a thread, fewer where the rows alone leave SMs idle.
-inline int grad_pieces(int64_t nrows, int C, int es) {
+inline int grad_pieces(int64_t nrows, int C, int es, int threads) {
   const int64_t nv = ((int64_t)C * es + 15) / 16 + 1;
-  int64_t most = (nv + kGradThreads * 2 - 1) / (kGradThreads * 2), p = (nv + kGradThreads * 16 - 1) / (kGradThreads * 16);
+  int64_t most = (nv + threads * 2 - 1) / (threads * 2), p = (nv + threads * 16 - 1) / (threads * 16);
+  if (threads == kWarpRow) return 1;
   while (p < most && nrows * p < 4 * kSMs) ++p;
   return (int)p;
 }
-template <typename T>
+template <typename T, int NT_>
 struct GradPiece {
-  static constexpr int VE = Vec<T>::kElems, U = kGradBatch, NT = kGradThreads;
+  static constexpr int VE = Vec<T>::kElems, U = kGradBatch, NT = NT_;
   VecRow<T> x, y;
   int v0, v1, f0, f1;
   VecRing<NT, U, kGradStages> ring;
@@ -784,7 +791,7 @@ struct GradPiece {
       if (c >= 0 && c < x.C) row[c] = Elem<T>::from_f(pair(make_float2(Elem<T>::to_f(x.row[c]), 0.f)).x);
     };
     if (f0 > v0 && threadIdx.x < VE) edge(x.cls(v0) + threadIdx.x);
-    if (f1 < v1 && f1 >= f0 && threadIdx.x >= 32 && threadIdx.x < 32 + VE) edge(x.cls(f1) + threadIdx.x - 32);
+    if (f1 < v1 && f1 >= f0 && threadIdx.x >= NT - VE) edge(x.cls(f1) + threadIdx.x - (NT - VE));
   }
 };
 
@@ -878,11 +885,22 @@ struct RowStream {
   }
 };
 
+// The runs of a cluster's blocks joined, in every lane of the calling warp.
+__device__ __forceinline__ Run run_cluster(const Run* mine, int cs, float k) {
+  const int lane = threadIdx.x & 31;
+  Run r = lane < cs ? cluster_ld_run(mine, lane) : run_empty();
+#pragma unroll
+  for (int o = 8; o; o >>= 1)
+    r = run_merge(r, Run{__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o),
+                         __shfl_xor_sync(0xffffffffu, r.u, o)}, k);
+  return {__shfl_sync(0xffffffffu, r.m, 0), __shfl_sync(0xffffffffu, r.s, 0), __shfl_sync(0xffffffffu, r.u, 0)};
+}
+
 // Blocks that share a row: as many as bring the rows to two blocks an SM, in
 // powers of two up to 16, while each keeps a few vectors a thread.
 inline int cluster_size(int64_t nrows, int C, int es, int threads) {
   int cs = 1;
-  while (cs < 16 && nrows * cs * 2 <= 2 * kSMs && (int64_t)C * es >= (int64_t)threads * 16 * 2 * (cs * 2)) cs *= 2;
+  while (cs < 8 && nrows * cs * 2 <= 2 * kSMs && (int64_t)C * es >= (int64_t)threads * 16 * 2 * (cs * 2)) cs *= 2;
   return cs;
 }
 
