@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
     if (cs > 1) cluster_sync();
     else __syncthreads();
   }
-  if (a.part) leave_part<NT>(sum_loss, sum_w, a.part);
+  if (a.part) leave_part<NT>(sum_loss, sum_w, a);
 }
 
 // One block per piece of a row; the listed classes are written over at the end.
@@ -359,6 +359,8 @@ extern "C" int r4c_distill_fwd(const r4c_rows_desc* d, const void* logits, int k
   if (!a.err) return R4C_ERR_NO_DEVICE;
   a.row_loss = row_loss;
   a.part = loss ? static_cast<double*>(state) : nullptr;
+  a.loss = loss;
+  a.total = reinterpret_cast<float*>(static_cast<char*>(state) + kTotalAt);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   int blocks = 0;
@@ -368,9 +370,8 @@ extern "C" int r4c_distill_fwd(const r4c_rows_desc* d, const void* logits, int k
     else e = distill::launch_fwd<float>(a, &blocks, s);
     note_launches(1);
   }
-  if (e == cudaSuccess && loss) {
-    distill::mean_kernel<<<1, distill::kMeanThreads, 0, s>>>(
-        a.part, blocks, loss, reinterpret_cast<float*>(static_cast<char*>(state) + kTotalAt));
+  if (e == cudaSuccess && loss && blocks != 1) {
+    distill::mean_kernel<<<1, distill::kMeanThreads, 0, s>>>(a.part, blocks, loss, a.total);
     e = cudaGetLastError();
     note_launches(1);
   }

@@ -45,6 +45,8 @@ struct Args {
   const float* weight;
   float* row_loss;       // forward: w L per row, or null
   double* part;          // forward: (sum w L, sum w) of each block, or null
+  float* loss;           // the mean and the sum of weights, written by a launch of one block itself
+  float* total;
   Stats* stats;
   const float* total_weight;
   const float* grad;
@@ -81,7 +83,7 @@ __device__ __forceinline__ float grad_scale(const Args& a, int64_t r) {
 }
 // A block's (sum of losses, sum of weights), in a fixed order.
 template <int NT>
-__device__ __forceinline__ void leave_part(double loss, double w, double* part) {
+__device__ __forceinline__ void leave_part(double loss, double w, const Args& a) {
   __shared__ double sh[2][NT / 32];
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -98,8 +100,13 @@ __device__ __forceinline__ void leave_part(double loss, double w, double* part) 
       loss += sh[0][i];
       w += sh[1][i];
     }
-    part[2 * blockIdx.x] = loss;
-    part[2 * blockIdx.x + 1] = w;
+    if (gridDim.x == 1) {
+      a.loss[0] = (float)(loss / w);   // no row takes part: NaN
+      a.total[0] = (float)w;
+    } else {
+      a.part[2 * blockIdx.x] = loss;
+      a.part[2 * blockIdx.x + 1] = w;
+    }
   }
 }
 

@@ -17,7 +17,7 @@ namespace distill {
 
 constexpr int kMostSlots = 4;   // pairs of a lane; kernels hold two or four
 
-template <typename T, int G, int E, bool VEC, bool BWD, int kSlots, bool PLAIN>
+template <typename T, int G, int E, int UB, bool BWD, int kSlots, bool PLAIN>
 __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
   constexpr int ES = (int)sizeof(T);
   const float k = a.inv_t * kLog2e;
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
         if (has(s) && in && pc[s] >= 0) sh_put<T>(row + pc[s] * ES, rest ? -INFINITY : pz[s]);
       if (G > 1) __syncwarp();
     }
-    TileRow<T, G, E, VEC> x;
+    TileRow<T, G, E, UB> x;
     x.load(row, a.C);
     if (BWD && G > 1) __syncwarp();   // read by all before any of it is written over
 
@@ -210,16 +210,17 @@ __global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
           sh_put<T>(row + pc[i] * ES, scale * (mass_s * prob((pz[i] - s.m) * a.inv_t) - q_of[i]));
     }
   });
-  if (!BWD && a.part) leave_part<kTileThreads>(sum_loss.value(), sum_w.value(), a.part);
+  if (!BWD && a.part) leave_part<kTileThreads>(sum_loss.value(), sum_w.value(), a);
 }
 
 // As for other tiles, with lanes enough for the pairs.
 inline TileKind pairs_kind(int C, int K, int es) {
   TileKind kind = tile_kind(C, es);
   if (K <= kind.g * kMostSlots) return kind;
-  if (C <= 64 && K <= 8 * kMostSlots) return {8, 8, kind.vec};
-  if (C <= 256) return {32, 8, kind.vec};
-  return {32, 32, kind.vec};
+  const int ub = kind.ub == 16 ? 16 : 4;
+  if (C <= 64 && K <= 8 * kMostSlots) return {8, 8, ub};
+  if (C <= 256) return {32, 8, ub};
+  return {32, 32, ub};
 }
 
 template <typename T>
@@ -232,18 +233,18 @@ cudaError_t launch_tiles(Args& a, bool bwd, int* blocks, cudaStream_t s) {
   const bool plain = a.t_dtype == R4C_F32 && !a.t_wide;
   auto launch = [&](auto c) {
     constexpr int G = decltype(c)::G, E = decltype(c)::E;
-    constexpr bool VEC = decltype(c)::VEC;
+    constexpr int UB = decltype(c)::UB;
     if (plain && a.K <= 2 * G) {
-      if (bwd) return launch_tile(tile_kernel<T, G, E, VEC, true, 2, true>, a.tile, s, a);
-      return launch_tile(tile_kernel<T, G, E, VEC, false, 2, true>, a.tile, s, a);
+      if (bwd) return launch_tile(tile_kernel<T, G, E, UB, true, 2, true>, a.tile, s, a);
+      return launch_tile(tile_kernel<T, G, E, UB, false, 2, true>, a.tile, s, a);
     }
-    if (plain && bwd) return launch_tile(tile_kernel<T, G, E, VEC, true, 4, true>, a.tile, s, a);
-    if (plain) return launch_tile(tile_kernel<T, G, E, VEC, false, 4, true>, a.tile, s, a);
-    if (bwd) return launch_tile(tile_kernel<T, G, E, VEC, true, 4, false>, a.tile, s, a);
-    return launch_tile(tile_kernel<T, G, E, VEC, false, 4, false>, a.tile, s, a);
+    if (plain && bwd) return launch_tile(tile_kernel<T, G, E, UB, true, 4, true>, a.tile, s, a);
+    if (plain) return launch_tile(tile_kernel<T, G, E, UB, false, 4, true>, a.tile, s, a);
+    if (bwd) return launch_tile(tile_kernel<T, G, E, UB, true, 4, false>, a.tile, s, a);
+    return launch_tile(tile_kernel<T, G, E, UB, false, 4, false>, a.tile, s, a);
   };
-  if (kind.g == 8 && kind.e == 8) return kind.vec ? launch(TileConst<8, 8, true>{}) : launch(TileConst<8, 8, false>{});
-  if (kind.g == 32 && kind.e == 8) return kind.vec ? launch(TileConst<32, 8, true>{}) : launch(TileConst<32, 8, false>{});
+  if (kind.g == 8 && kind.e == 8) return kind.ub == 16 ? launch(TileConst<8, 8, 16>{}) : launch(TileConst<8, 8, 4>{});
+  if (kind.g == 32 && kind.e == 8) return kind.ub == 16 ? launch(TileConst<32, 8, 16>{}) : launch(TileConst<32, 8, 4>{});
   return for_tile_kind<T>(kind, launch);
 }
 

@@ -22,7 +22,7 @@ struct FwdArgs {
   int64_t ignore, nrows;
   View v;
   Tile tile;
-  int C, K, pairs;   // pairs: K = 2 and the outputs 8-byte aligned
+  int C, ign, K, pairs;   // pairs: K = 2 and the outputs 8-byte aligned
   float inv_t;
   float *logp, *entropy, *lse, *top_logp;
   int32_t* top_index;
@@ -36,7 +36,7 @@ struct BwdArgs {
   int64_t ignore, nrows;
   View v, dv;
   Tile tile;
-  int C, segs;
+  int C, ign, segs;
   float inv_t;
   const float* entropy;
   const float2* stats;
@@ -46,16 +46,14 @@ struct BwdArgs {
   int* err;
 };
 
-// The row's label, -1 when it has none or takes no part.
-__device__ __forceinline__ int label_of(const int64_t* target, int64_t r, int C, int64_t ignore, int* err) {
+// The row's label, -1 when it has none or takes no part. (ign: ignore_index
+// where it is a class, else -1; most labels need one comparison in 64 bits.)
+__device__ __forceinline__ int label_of(const int64_t* target, int64_t r, int C, int64_t ignore, int ign, int* err) {
   if (!target) return -1;
   const int64_t t = target[r];
-  if (t == ignore) return -1;
-  if (t < 0 || t >= C) {
-    atomicExch(err, 6);
-    return -1;
-  }
-  return (int)t;
+  if ((uint64_t)t < (uint64_t)C) return (int)t == ign ? -1 : (int)t;
+  if (t != ignore) atomicExch(err, 6);
+  return -1;
 }
 
 // What a row's sums say; bad: NaN or +inf in the row, empty: no finite logit.
@@ -93,23 +91,60 @@ template <> struct TopKey<float> {
   static __device__ __forceinline__ float value(long long k) { return key_value((uint64_t)k ^ 0x8000000000000000ull); }
 };
 
-template <typename T, int G, int E, bool VEC>
+template <typename T, int G, int E, int UB>
 __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
   const float k = a.inv_t * kLog2e;
   tile_walk<T, G, false>(a.tile, a.v, a.z, a.v, nullptr, [&](int64_t r0, int r, uint32_t row, bool in) {
-    TileRow<T, G, E, VEC> x;
+    TileRow<T, G, E, UB> x;
     x.load(row, a.C);
+    // Two alternatives of a lane's own row: the two largest in one pass
+    // (a later class takes a place only by a larger value).
+    float b1 = x.v[0], b2 = -INFINITY;
+    int c1 = 0, c2 = 1;
+    if (G == 1 && a.pairs) {
+      const bool half = x.c0 < 0;   // the first value is no class
+      if (half) {
+        b1 = x.v[1];
+        c1 = 1;
+        c2 = 2;
+      } else {
+        const bool up = x.v[1] > b1;
+        b2 = up ? b1 : x.v[1];
+        b1 = up ? x.v[1] : b1;
+        c1 = up;
+        c2 = !up;
+      }
+#pragma unroll
+      for (int e = 2; e < E; ++e) {
+        const bool up = x.v[e] > b1, mid = x.v[e] > b2;
+        c2 = up ? c1 : mid ? e : c2;
+        b2 = up ? b1 : mid ? x.v[e] : b2;
+        c1 = up ? e : c1;
+        b1 = up ? x.v[e] : b1;
+      }
+      c1 -= half;
+      c2 -= half;
+    }
     const Run run = tile_run(x, k);
     const RowOut o(run, lg2(run.s), a.inv_t);
     if (in && x.lane == 0) {
       if (a.target) {
-        const int t = label_of(a.target + r0, r, a.C, a.ignore, a.err);
+        const int t = label_of(a.target + r0, r, a.C, a.ignore, a.ign, a.err);
         (a.logp + r0)[r] = t < 0 ? 0.f : o.logp(sh_get<T>(row + t * (int)sizeof(T)));
       }
       (a.entropy + r0)[r] = o.entropy(run);
       (a.lse + r0)[r] = o.lse();
     }
     if (a.K == 0) return;
+    float* tl = a.top_logp + r0 * a.K + r * a.K;
+    int32_t* ti = a.top_index + r0 * a.K + r * a.K;
+    if (G == 1 && a.pairs) {   // stored whole: half-written sectors cost twice
+      if (in) {                // (a bad row's sums are NaN and make its values NaN)
+        *reinterpret_cast<float2*>(tl) = make_float2(o.logp(b1), o.logp(b2));
+        *reinterpret_cast<int2*>(ti) = o.bad ? make_int2(-1, -1) : make_int2(c1, c2);
+      }
+      return;
+    }
     // the most probable classes, one after the other, from the row as it was
     x.load(row, a.C);
     using Key = TopKey<T>;
@@ -117,8 +152,6 @@ __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) key[e] = Key::make(x.v[e], x.cls(e));   // past the row: -inf, ranked after every class
     if (x.c0 < 0) key[0] = Key::kNone;                                  // the half word before it is no class
-    float* tl = a.top_logp + r0 * a.K + r * a.K;
-    int32_t* ti = a.top_index + r0 * a.K + r * a.K;
     auto next = [&](float* l, int* c) {
       typename Key::type b = key[0];
 #pragma unroll
@@ -133,17 +166,6 @@ __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
       *l = o.bad ? NAN : o.logp(Key::value(b));
       *c = o.bad ? -1 : Key::cls(b);
     };
-    if (G == 1 && a.pairs) {   // two alternatives are stored whole: half-written sectors cost twice
-      float2 l;
-      int2 c;
-      next(&l.x, &c.x);
-      next(&l.y, &c.y);
-      if (in) {
-        *reinterpret_cast<float2*>(tl) = l;
-        *reinterpret_cast<int2*>(ti) = c;
-      }
-      return;
-    }
     for (int j = 0; j < a.K; ++j) {
       float l;
       int c;
@@ -156,12 +178,12 @@ __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
   });
 }
 
-template <typename T, int G, int E, bool VEC>
+template <typename T, int G, int E, int UB>
 __global__ void __launch_bounds__(kTileThreads) bwd_tile_kernel(BwdArgs a) {
   const float k = a.inv_t * kLog2e;
   tile_walk<T, G, true>(a.tile, a.v, a.z, a.dv, a.dz, [&](int64_t r0, int r, uint32_t row, bool in) {
-    TileRow<T, G, E, VEC> x;
-    const int t = a.target ? label_of(a.target + r0, r, a.C, a.ignore, a.err) : -1;
+    TileRow<T, G, E, UB> x;
+    const int t = a.target ? label_of(a.target + r0, r, a.C, a.ignore, a.ign, a.err) : -1;
     const float gl = a.g_logp && t >= 0 ? (a.g_logp + r0 * a.gl_inc)[r * a.gl_inc] : 0.f;
     const float gh = a.g_entropy ? (a.g_entropy + r0 * a.gh_inc)[r * a.gh_inc] : 0.f;
     const float gs = a.g_lse ? (a.g_lse + r0 * a.gs_inc)[r * a.gs_inc] : 0.f;
@@ -443,7 +465,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
       const RowOut o(run, log2f(run.s), a.inv_t);
       if (tid == 0) {
         if (a.target) {
-          const int t = label_of(a.target, r, a.C, a.ignore, a.err);
+          const int t = label_of(a.target, r, a.C, a.ignore, a.ign, a.err);
           a.logp[r] = t < 0 ? 0.f : o.logp(Elem<T>::to_f(x.row[t]));
         }
         a.entropy[r] = o.entropy(run);
@@ -494,7 +516,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) bwd_block_kernel(BwdArgs a) {
   const int64_t r = blockIdx.x / a.segs;
   T* dz = static_cast<T*>(a.dz) + a.dv.base(r);
   GradPiece<T, NT> piece(static_cast<const T*>(a.z) + a.v.base(r), dz, a.C, blockIdx.x % a.segs, a.segs, ring);
-  const int t = label_of(a.target, r, a.C, a.ignore, a.err);
+  const int t = label_of(a.target, r, a.C, a.ignore, a.ign, a.err);
   const float gl = a.g_logp && t >= 0 ? a.g_logp[r * a.gl_inc] : 0.f;
   const float gh = a.g_entropy ? a.g_entropy[r * a.gh_inc] : 0.f;
   const float gs = a.g_lse ? a.g_lse[r * a.gs_inc] : 0.f;
@@ -547,7 +569,7 @@ cudaError_t launch_fwd(FwdArgs& a, cudaStream_t s) {
     const TileKind kind = tile_kind(a.C, sizeof(T));
     a.tile = make_tile(a.nrows, a.C, sizeof(T), kind.g, dense_rows(a.v, a.nrows, a.C, a.z));
     return for_tile_kind<T>(kind, [&](auto c) {
-      return launch_tile(fwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::VEC>, a.tile, s, a);
+      return launch_tile(fwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::UB>, a.tile, s, a);
     });
   }
   if (row_threads(a.C, sizeof(T), a.K) == kWarpRow) return launch_fwd_block<T, kWarpRow>(a, s);
@@ -561,7 +583,7 @@ cudaError_t launch_bwd(BwdArgs& a, cudaStream_t s) {
     a.tile = make_tile(a.nrows, a.C, sizeof(T), kind.g,
                        dense_rows(a.v, a.nrows, a.C, a.z) && dense_rows(a.dv, a.nrows, a.C, a.dz));
     return for_tile_kind<T>(kind, [&](auto c) {
-      return launch_tile(bwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::VEC>, a.tile, s, a);
+      return launch_tile(bwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::UB>, a.tile, s, a);
     });
   }
   const int threads = row_threads(a.C, sizeof(T), 0);
@@ -604,8 +626,9 @@ extern "C" int r4c_logp_fwd(const r4c_rows_desc* d, const void* logits, const in
   if (!logits || !entropy || !lse || (target && !logp) || (top_k > 0 && (!top_logp || !top_index))) return R4C_ERR_INVALID;
   int* err = tc::device_error_flag();
   if (!err) return R4C_ERR_NO_DEVICE;
+  const int ign = ignore_index >= 0 && ignore_index < d->classes ? (int)ignore_index : -1;
   const int pairs = top_k == 2 && !(((uintptr_t)top_logp | (uintptr_t)top_index) & 7);
-  logp::FwdArgs a{logits, target, ignore_index, d->rows, rows::make_view(d), {}, d->classes, top_k, pairs,
+  logp::FwdArgs a{logits, target, ignore_index, d->rows, rows::make_view(d), {}, d->classes, ign, top_k, pairs,
                   1.f / d->temperature, logp, entropy, lse, top_logp, top_index, static_cast<float2*>(stats), err};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
@@ -626,8 +649,9 @@ extern "C" int r4c_logp_bwd(const r4c_rows_desc* d, const void* logits, const in
   if (!logits || !dlogits || !entropy || (!stats && r4c_logp_stats_size(d)) || (g_logp && !target)) return R4C_ERR_INVALID;
   int* err = tc::device_error_flag();
   if (!err) return R4C_ERR_NO_DEVICE;
+  const int ign = ignore_index >= 0 && ignore_index < d->classes ? (int)ignore_index : -1;
   logp::BwdArgs a{logits, target, ignore_index, d->rows, rows::make_view(d), rows::make_grad_view(d), {}, d->classes,
-                  0, 1.f / d->temperature, entropy, static_cast<const float2*>(stats), g_logp, g_entropy, g_lse,
+                  ign, 0, 1.f / d->temperature, entropy, static_cast<const float2*>(stats), g_logp, g_entropy, g_lse,
                   g_logp_inc, g_entropy_inc, g_lse_inc, dlogits, err};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;

@@ -196,16 +196,17 @@ struct Tile {
 };
 constexpr int kTileStages = 3;
 
-// One lane's part of a row: E values in units of a 16-byte vector (VEC: rows
-// are 16-byte aligned) or a 32-bit word, taken cyclically by the lanes, so
-// value e is class c0 + off(e) and classes ascend with e. A row of 2-byte
+// One lane's part of a row: E values in units of UB = 16, 8 or 4 bytes (rows
+// are that aligned, or UB = 4), taken cyclically by the lanes, so value e is
+// class c0 + off(e) and classes ascend with e. With UB = 4 a row of 2-byte
 // elements may start in the middle of a word: c0 is then one lower (-1 in
 // lane 0: not a class).
-template <typename T, int G, int E, bool VEC>
+template <typename T, int G, int E, int UB>
 struct TileRow {
   static constexpr int kG = G, kW = Word<T>::kElems;
-  static constexpr int kU = VEC ? 16 / (int)sizeof(T) : kW;   // elements of a unit
-  static constexpr int kN = E / kU;                           // units of a lane
+  static constexpr int kU = UB / (int)sizeof(T);   // elements of a unit
+  static constexpr int kN = E / kU;                // units of a lane
+  static constexpr bool VEC = UB > 4, kHalf = UB == 4 && kW == 2;   // kHalf: rows may start in a word's middle
   float v[E];
   int lane, c0, C;
   uint32_t at;   // shared address of the lane's first unit
@@ -221,17 +222,23 @@ struct TileRow {
   __device__ __forceinline__ void load(uint32_t row, int classes) {
     C = classes;
     lane = (threadIdx.x & 31) & (G - 1);
-    c0 = kU * lane - (kU == 2 ? (row >> 1) & 1 : 0);
-    at = (kU == 2 ? row & ~3u : row) + lane * (kU * (int)sizeof(T));
+    c0 = kU * lane - (kHalf ? (row >> 1) & 1 : 0);
+    at = (kHalf ? row & ~3u : row) + lane * UB;
 #pragma unroll
     for (int i0 = 0; i0 < kN; i0 += kGroup) {
       if (VEC) {
-        uint32_t w[4] = {Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf};
-        if (cls(i0 * kU) < C)
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + step(i0)) : "memory");
+        uint32_t w[UB / 4];
 #pragma unroll
-        for (int h = 0; h < 4; ++h) Word<T>::split(w[h], v + i0 * kU + h * kW);
+        for (int h = 0; h < UB / 4; ++h) w[h] = Word<T>::kNegInf;
+        if (cls(i0 * kU) < C) {
+          if constexpr (UB == 16)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + step(i0)) : "memory");
+          else if constexpr (UB == 8)
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at + step(i0)) : "memory");
+        }
+#pragma unroll
+        for (int h = 0; h < UB / 4; ++h) Word<T>::split(w[h], v + i0 * kU + h * kW);
       } else {
         uint32_t w[kGroup];
         if (whole(i0)) {
@@ -244,26 +251,30 @@ struct TileRow {
             const int c = cls((i0 + j) * kU);
             w[j] = Word<T>::kNegInf;
             if (c < C) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[j]) : "r"(at + step(i0 + j)) : "memory");
-            if (kU == 2 && c + 1 >= C) w[j] = (w[j] & 0xffffu) | (Word<T>::kNegInf & 0xffff0000u);
+            if (kHalf && c + 1 >= C) w[j] = (w[j] & 0xffffu) | (Word<T>::kNegInf & 0xffff0000u);
           }
         }
 #pragma unroll
         for (int j = 0; j < kGroup; ++j) Word<T>::split(w[j], v + (i0 + j) * kU);
       }
     }
-    if (kU == 2 && c0 < 0) v[0] = -INFINITY;
+    if (kHalf && c0 < 0) v[0] = -INFINITY;
   }
   // Writes g over the row in shared memory.
   __device__ __forceinline__ void store(const float* g) const {
 #pragma unroll
     for (int i0 = 0; i0 < kN; i0 += kGroup) {
       if (VEC) {
-        uint32_t w[4];
+        uint32_t w[UB / 4];
 #pragma unroll
-        for (int h = 0; h < 4; ++h) w[h] = Word<T>::join(g + i0 * kU + h * kW);
-        if (cls(i0 * kU) < C)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + step(i0)), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                       "r"(w[3]) : "memory");
+        for (int h = 0; h < UB / 4; ++h) w[h] = Word<T>::join(g + i0 * kU + h * kW);
+        if (cls(i0 * kU) < C) {
+          if constexpr (UB == 16)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + step(i0)), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                         "r"(w[3]) : "memory");
+          else if constexpr (UB == 8)
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + step(i0)), "r"(w[0]), "r"(w[1]) : "memory");
+        }
         continue;
       }
       const bool all = whole(i0);
@@ -271,10 +282,10 @@ struct TileRow {
       for (int j = 0; j < kGroup; ++j) {
         const uint32_t a = at + step(i0 + j), w = Word<T>::join(g + (i0 + j) * kU);
         const int c = cls((i0 + j) * kU);
-        const bool lo = !(kU == 2 && i0 + j == 0) || c0 >= 0;   // else the half word is another row's
+        const bool lo = !(kHalf && i0 + j == 0) || c0 >= 0;   // else the half word is another row's
         if (lo && (all || c + kU <= C)) asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(w) : "memory");
         else if (!lo) asm volatile("st.shared.b16 [%0], %1;" ::"r"(a + 2), "h"((uint16_t)(w >> 16)) : "memory");
-        else if (kU == 2 && c < C) asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"((uint16_t)w) : "memory");
+        else if (kHalf && c < C) asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"((uint16_t)w) : "memory");
       }
     }
   }
@@ -441,45 +452,45 @@ inline bool dense_rows(const View& v, int64_t rows, int classes, const void* p) 
 // 32 registers of values allow, since what a row costs beyond its elements is
 // paid once per group of lanes.
 struct TileKind {
-  int g, e;
-  bool vec;
+  int g, e, ub;
 };
+inline int row_unit(int C, int es) { return C * es % 16 == 0 ? 16 : C * es % 8 == 0 ? 8 : 4; }
 inline TileKind tile_kind(int C, int es) {
-  const bool vec = C * es % 16 == 0;
-  if (C <= 32) return {1, C <= 4 ? 4 : C <= 8 ? 8 : C <= 16 ? 16 : 32, vec};
+  const int ub = row_unit(C, es);
+  if (C <= 32) return {1, C <= 4 ? 4 : C <= 8 ? 8 : C <= 16 ? 16 : 32, ub};
   int g = 2;
   while (C > g * 32) g *= 2;
-  return {g, 32, vec};
+  return {g, 32, ub == 16 ? 16 : 4};
 }
-// Calls f(G, E, VEC as constants) for a kind; vectors need as many values as they hold.
-template <int G_, int E_, bool VEC_>
+// Calls f(G, E, UB as constants) for a kind; a unit needs as many values as it holds.
+template <int G_, int E_, int UB_>
 struct TileConst {
-  static constexpr int G = G_, E = E_;
-  static constexpr bool VEC = VEC_;
+  static constexpr int G = G_, E = E_, UB = UB_;
 };
 template <typename T, typename F>
 inline cudaError_t for_tile_kind(const TileKind& k, F&& f) {
-#define R4C_TILE(G, E)                                                             \
-  if (k.g == G && k.e == E) {                                                      \
-    if constexpr (E * sizeof(T) >= 16) {                                           \
-      if (k.vec) return f(TileConst<G, E, true>{});                                \
-    }                                                                              \
-    return f(TileConst<G, E, false>{});                                            \
+#define R4C_TILE(G, E)                                            \
+  if (k.g == G && k.e == E) {                                     \
+    if constexpr (E * sizeof(T) >= 16)                            \
+      if (k.ub == 16) return f(TileConst<G, E, 16>{});            \
+    if constexpr (G == 1)                                         \
+      if (k.ub == 8) return f(TileConst<G, E, 8>{});              \
+    return f(TileConst<G, E, 4>{});                               \
   }
   R4C_TILE(1, 4) R4C_TILE(1, 8) R4C_TILE(1, 16) R4C_TILE(1, 32) R4C_TILE(2, 32) R4C_TILE(4, 32) R4C_TILE(8, 32)
   R4C_TILE(16, 32) R4C_TILE(32, 32)
 #undef R4C_TILE
   return cudaErrorInvalidValue;
 }
-// Tiles of up to 16 KB (at least one row for each group of lanes): three of
-// them in flight in each of the blocks of an SM keep the memory busy.
+// Tiles of up to 16 KB, 8 KB for the shortest rows (at least one row for each
+// group of lanes): three of them in flight in each of the blocks of an SM keep the memory busy.
 inline Tile make_tile(int64_t nrows, int C, int es, int g, bool dense) {
   Tile t{};
   t.nrows = nrows;
   t.C = C;
   t.mode = !dense ? kGather : C * es % 16 ? kCopy : kCopyPadded;
-  // rows that lie an even number of 16-byte chunks (or 4-byte words) apart would meet in the same banks
-  const int unit = C * es % 16 == 0 ? 16 : 4;
+  // rows that lie an even number of units apart would meet in the same banks
+  const int unit = row_unit(C, es);
   t.stride = t.mode == kCopy ? C : ((C * es + unit - 1) / unit | 1) * unit / es;
   t.chunks = C * es / 16;
   t.recip = t.chunks ? (uint32_t)(((1ull << 32) + t.chunks - 1) / t.chunks) : 0;

@@ -20,7 +20,7 @@ import torch
 
 from . import _native
 
-_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_FLOATS = frozenset((torch.bfloat16, torch.float16, torch.float32))
 
 
 class LogProbs(NamedTuple):
@@ -33,11 +33,12 @@ class LogProbs(NamedTuple):
 
 
 def check_logits(logits: torch.Tensor, temperature: float) -> None:
-    if logits.dim() < 2:
-        raise ValueError(f"logits must be (N, C, ...), got shape {tuple(logits.shape)}")
-    if logits.shape[1] == 0:
+    shape = logits.shape
+    if len(shape) < 2:
+        raise ValueError(f"logits must be (N, C, ...), got shape {tuple(shape)}")
+    if shape[1] == 0:
         raise ValueError("logits have no classes")
-    if not logits.is_floating_point() or (logits.is_cuda and logits.dtype not in _FLOATS):
+    if logits.dtype not in _FLOATS and (logits.is_cuda or not logits.is_floating_point()):
         raise TypeError(f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
     if not (math.isfinite(temperature) and temperature > 0):
         raise ValueError(f"temperature must be finite and positive, got {temperature}")
@@ -86,13 +87,14 @@ def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, *, to
     no distribution: its values are NaN and its top_index -1.
     """
     check_logits(logits, temperature)
-    shape = logits.shape[:1] + logits.shape[2:]
-    if not 0 <= top_k <= min(_native.TOPK_MAX, logits.shape[1]):
-        raise ValueError(f"top_k must be in [0, min({_native.TOPK_MAX}, C = {logits.shape[1]})], got {top_k}")
+    zs = logits.shape
+    if not 0 <= top_k <= _native.TOPK_MAX or top_k > zs[1]:
+        raise ValueError(f"top_k must be in [0, min({_native.TOPK_MAX}, C = {zs[1]})], got {top_k}")
     if target is not None:
-        if target.shape != shape:
-            raise ValueError(f"target must have shape {tuple(shape)}, got {tuple(target.shape)}")
-        if target.is_floating_point() or target.is_complex() or target.dtype == torch.bool:
+        ts = target.shape
+        if len(ts) != len(zs) - 1 or ts[0] != zs[0] or ts[1:] != zs[2:]:
+            raise ValueError(f"target must have shape {tuple(zs[:1] + zs[2:])}, got {tuple(target.shape)}")
+        if target.dtype != torch.int64 and target.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
             raise TypeError(f"target must hold integers, got {target.dtype}")
         if target.device != logits.device:
             raise ValueError(f"target is on {target.device}, logits on {logits.device}")

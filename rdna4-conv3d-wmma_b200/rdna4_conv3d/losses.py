@@ -95,24 +95,26 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
     (on a CUDA device it is unused and sets code 6 in ``_native.device_error()``).
     """
     check_logits(logits, temperature)
-    shape = logits.shape[:1] + logits.shape[2:]
-    if reduction not in ("mean", "none"):
+    mean = reduction == "mean"
+    if not mean and reduction != "none":
         raise ValueError(f"reduction must be 'mean' or 'none', got {reduction!r}")
-    if teacher_logp.shape != teacher_index.shape or teacher_logp.shape[:-1] != shape:
-        raise ValueError(f"teacher_logp and teacher_index must have shape {tuple(shape)} + (k,), got "
-                         f"{tuple(teacher_logp.shape)} and {tuple(teacher_index.shape)}")
-    k = teacher_logp.shape[-1]
-    if not 1 <= k <= _native.TOPK_MAX:
-        raise ValueError(f"the teacher's classes per row must be in [1, {_native.TOPK_MAX}], got {k}")
+    zs, ts, dev = logits.shape, teacher_logp.shape, logits.device
+    if teacher_index.shape != ts or len(ts) != len(zs) or ts[0] != zs[0] or ts[1:-1] != zs[2:]:
+        raise ValueError(f"teacher_logp and teacher_index must have shape {tuple(zs[:1] + zs[2:])} + (k,), got "
+                         f"{tuple(ts)} and {tuple(teacher_index.shape)}")
+    if not 1 <= ts[-1] <= _native.TOPK_MAX:
+        raise ValueError(f"the teacher's classes per row must be in [1, {_native.TOPK_MAX}], got {ts[-1]}")
     if not teacher_logp.is_floating_point():
         raise TypeError(f"teacher_logp must be a floating type, got {teacher_logp.dtype}")
     if teacher_index.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"teacher_index must be int32 or int64, got {teacher_index.dtype}")
-    if weight is not None and weight.shape != shape:
-        raise ValueError(f"weight must have shape {tuple(shape)}, got {tuple(weight.shape)}")
-    for name, t in (("teacher_logp", teacher_logp), ("teacher_index", teacher_index), ("weight", weight)):
-        if t is not None and t.device != logits.device:
-            raise ValueError(f"{name} is on {t.device}, logits on {logits.device}")
+    if teacher_logp.device != dev or teacher_index.device != dev:
+        raise ValueError(f"the teacher is on {teacher_logp.device} and {teacher_index.device}, logits on {dev}")
+    if weight is not None:
+        if weight.shape != zs[:1] + zs[2:]:
+            raise ValueError(f"weight must have shape {tuple(zs[:1] + zs[2:])}, got {tuple(weight.shape)}")
+        if weight.device != dev:
+            raise ValueError(f"weight is on {weight.device}, logits on {dev}")
     if not logits.is_cuda:
         return _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weight, reduction)
     if teacher_logp.requires_grad:
@@ -121,11 +123,11 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
         teacher_logp = teacher_logp.float()
     if weight is not None:
         weight = weight.detach().to(torch.float32).contiguous()
-    teacher_logp, teacher_index, mean = teacher_logp.contiguous(), teacher_index.contiguous(), reduction == "mean"
+    teacher_logp, teacher_index, rest = teacher_logp.contiguous(), teacher_index.contiguous(), bool(rest)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return DistillTopKFn.apply(logits, teacher_logp, teacher_index, temperature, bool(rest), weight, mean)
+        return DistillTopKFn.apply(logits, teacher_logp, teacher_index, temperature, rest, weight, mean)
     rows = _native.Rows(logits, temperature)
-    return _native.distill_forward(rows, teacher_logp, teacher_index, bool(rest), weight, mean)[0]
+    return _native.distill_forward(rows, teacher_logp, teacher_index, rest, weight, mean)[0]
 
 
 def _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weight, reduction):
