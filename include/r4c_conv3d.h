@@ -421,7 +421,7 @@ int r4c_logp_bwd(const r4c_rows_desc* desc, const void* logits, const int64_t* t
  * r4c_distill_bwd writes dlogits = grad[r * grad_inc] * w * dL/dz, divided by
  * sum(w) with mean = 1 (the forward had loss given).
  * Above 1024 classes the classes must be contiguous (class_stride 1), and
- * rest = 1 takes about ten million classes at most.
+ * rest = 1 takes about four million classes at most.
  */
 size_t r4c_distill_state_size(const r4c_rows_desc* desc);
 int r4c_distill_fwd(const r4c_rows_desc* desc, const void* logits, int k, const void* teacher_logp, int teacher_dtype,

@@ -270,11 +270,11 @@ constexpr size_t kMostMarks = 128 << 10;
 template <typename T, int NT>
 cudaError_t launch_fwd_block(const Args& a, int* blocks, cudaStream_t s) {
   int cs = cluster_size(a.nrows, a.C, sizeof(T), NT);
-  while (a.rest && cs < 16 && mark_bytes<T>(a.C, cs) > kMostMarks) cs *= 2;
+  while (a.rest && cs < 8 && mark_bytes<T>(a.C, cs) > kMostMarks) cs *= 2;
   const size_t smem = VecRing<NT, kBatch, kStages>::kBytes + (a.rest ? mark_bytes<T>(a.C, cs) : 0);
-  const int64_t most = (int64_t)kSMs * blocks_per_sm(NT, smem) / cs * cs;
+  const int64_t most = (int64_t)kSMs * blocks_per_sm(fwd_block_kernel<T, NT>, NT, smem) / cs * cs;
   int64_t grid = a.nrows * cs;
-  if (grid > most) grid = most;
+  if (grid > most) grid = most;   // (0: launch_cluster gives the error)
   *blocks = (int)grid;
   return launch_cluster(fwd_block_kernel<T, NT>, grid, NT, cs, smem, s, a);
 }
@@ -311,8 +311,8 @@ int check(const r4c_rows_desc* d, int k, const void* t_logp, int t_dtype, const 
   if (!rows::valid_dtype(d->dtype) || !rows::valid_dtype(t_dtype)) return R4C_ERR_UNSUPPORTED;
   if (d->classes > rows::kTileClasses && (d->class_stride != 1 || d->grad_class_stride != 1)) return R4C_ERR_UNSUPPORTED;
   if (k > R4C_TOPK_MAX) return R4C_ERR_TOO_LARGE;
-  // the marks of the listed classes, spread over a cluster of 16 blocks
-  if (rest && distill::mark_bytes<float>(d->classes, 16) > distill::kMostMarks) return R4C_ERR_TOO_LARGE;
+  // the marks of the listed classes, spread over a cluster of 8 blocks
+  if (rest && distill::mark_bytes<float>(d->classes, 8) > distill::kMostMarks) return R4C_ERR_TOO_LARGE;
   return R4C_OK;
 }
 // The state: the blocks' partial sums, the sum of weights, the rows' statistics.

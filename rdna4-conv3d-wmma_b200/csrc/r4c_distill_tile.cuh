@@ -229,19 +229,18 @@ cudaError_t launch_tiles(Args& a, bool bwd, int* blocks, cudaStream_t s) {
   a.tile = make_tile(a.nrows, a.C, sizeof(T), kind.g,
                      dense_rows(a.v, a.nrows, a.C, a.z) && (!bwd || dense_rows(a.dv, a.nrows, a.C, a.dz)));
   a.even = a.K % 2 == 0 && !(((uintptr_t)a.t_logp | (uintptr_t)a.t_index) & 7);
-  *blocks = tile_grid(a.tile);
   const bool plain = a.t_dtype == R4C_F32 && !a.t_wide;
   auto launch = [&](auto c) {
     constexpr int G = decltype(c)::G, E = decltype(c)::E;
     constexpr int UB = decltype(c)::UB;
     if (plain && a.K <= 2 * G) {
-      if (bwd) return launch_tile(tile_kernel<T, G, E, UB, true, 2, true>, a.tile, s, a);
-      return launch_tile(tile_kernel<T, G, E, UB, false, 2, true>, a.tile, s, a);
+      if (bwd) return launch_tile(tile_kernel<T, G, E, UB, true, 2, true>, a.tile, blocks, s, a);
+      return launch_tile(tile_kernel<T, G, E, UB, false, 2, true>, a.tile, blocks, s, a);
     }
-    if (plain && bwd) return launch_tile(tile_kernel<T, G, E, UB, true, 4, true>, a.tile, s, a);
-    if (plain) return launch_tile(tile_kernel<T, G, E, UB, false, 4, true>, a.tile, s, a);
-    if (bwd) return launch_tile(tile_kernel<T, G, E, UB, true, 4, false>, a.tile, s, a);
-    return launch_tile(tile_kernel<T, G, E, UB, false, 4, false>, a.tile, s, a);
+    if (plain && bwd) return launch_tile(tile_kernel<T, G, E, UB, true, 4, true>, a.tile, blocks, s, a);
+    if (plain) return launch_tile(tile_kernel<T, G, E, UB, false, 4, true>, a.tile, blocks, s, a);
+    if (bwd) return launch_tile(tile_kernel<T, G, E, UB, true, 4, false>, a.tile, blocks, s, a);
+    return launch_tile(tile_kernel<T, G, E, UB, false, 4, false>, a.tile, blocks, s, a);
   };
   if (kind.g == 8 && kind.e == 8) return kind.ub == 16 ? launch(TileConst<8, 8, 16>{}) : launch(TileConst<8, 8, 4>{});
   if (kind.g == 32 && kind.e == 8) return kind.ub == 16 ? launch(TileConst<32, 8, 16>{}) : launch(TileConst<32, 8, 4>{});

@@ -556,20 +556,21 @@ cudaError_t launch_fwd_block(const FwdArgs& a, cudaStream_t s) {
   const int cs = cluster_size(a.nrows, a.C, sizeof(T), NT);
   const size_t smem = VecRing<NT, kBatch, kStages>::kBytes +
                       (a.K > 0 ? top_bytes(cs, a.K, NT) : 0);
-  const int64_t most = (int64_t)kSMs * blocks_per_sm(NT, smem);
+  auto* kernel = a.K > 0 ? fwd_block_kernel<T, NT, true> : fwd_block_kernel<T, NT, false>;
+  const int64_t most = (int64_t)kSMs * blocks_per_sm(kernel, NT, smem);
   int64_t grid = a.nrows * cs;
   if (cs == 1 && grid > most) grid = most;
-  if (a.K > 0) return launch_cluster(fwd_block_kernel<T, NT, true>, grid, NT, cs, smem, s, a);
-  return launch_cluster(fwd_block_kernel<T, NT, false>, grid, NT, cs, smem, s, a);
+  return launch_cluster(kernel, grid, NT, cs, smem, s, a);
 }
 
 template <typename T>
 cudaError_t launch_fwd(FwdArgs& a, cudaStream_t s) {
   if (a.C <= kTileClasses) {
+    int blocks;
     const TileKind kind = tile_kind(a.C, sizeof(T));
     a.tile = make_tile(a.nrows, a.C, sizeof(T), kind.g, dense_rows(a.v, a.nrows, a.C, a.z));
     return for_tile_kind<T>(kind, [&](auto c) {
-      return launch_tile(fwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::UB>, a.tile, s, a);
+      return launch_tile(fwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::UB>, a.tile, &blocks, s, a);
     });
   }
   if (row_threads(a.C, sizeof(T), a.K) == kWarpRow) return launch_fwd_block<T, kWarpRow>(a, s);
@@ -579,11 +580,12 @@ cudaError_t launch_fwd(FwdArgs& a, cudaStream_t s) {
 template <typename T>
 cudaError_t launch_bwd(BwdArgs& a, cudaStream_t s) {
   if (a.C <= kTileClasses) {
+    int blocks;
     const TileKind kind = tile_kind(a.C, sizeof(T));
     a.tile = make_tile(a.nrows, a.C, sizeof(T), kind.g,
                        dense_rows(a.v, a.nrows, a.C, a.z) && dense_rows(a.dv, a.nrows, a.C, a.dz));
     return for_tile_kind<T>(kind, [&](auto c) {
-      return launch_tile(bwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::UB>, a.tile, s, a);
+      return launch_tile(bwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::UB>, a.tile, &blocks, s, a);
     });
   }
   const int threads = row_threads(a.C, sizeof(T), 0);

@@ -35,10 +35,11 @@ constexpr float kRestNoise = 1e-6f;
 constexpr int kTileClasses = 1024;
 constexpr int kTileThreads = 256;
 constexpr int kSMs = 148;
-// Threads to a streamed row: one warp up to 16 KB (what a row costs beyond its
-// elements is paid per warp: 16384 rows of 1500 bf16 classes take half the
-// time of 128 threads), else 256. A thread holds at most one of the k pairs
-// or asks for at most a quarter of them to be found per vector it has.
+// Threads to a streamed row: one warp up to 16 KB, else 256. What a row costs
+// beyond its elements is paid per warp: 16384 rows of 1500 bf16 classes took
+// 63 us forward and 87 us backward with 128 and 256 threads, 29 and 29 us with
+// 32. More than 32 pairs or alternatives take 256, so that each pair has a
+// thread and there are maxima enough to choose from.
 constexpr int kWarpRow = 32, kLongRow = 256;
 inline int row_threads(int C, int es, int k) { return (int64_t)C * es <= 16 << 10 && k <= kWarpRow ? kWarpRow : kLongRow; }
 
@@ -504,21 +505,42 @@ inline Tile make_tile(int64_t nrows, int C, int es, int g, bool dense) {
   t.stage_bytes = (t.rows * t.stride * es + 31) / 16 * 16;
   return t;
 }
-// Blocks of a persistent tile launch: what shared memory and threads let an SM hold.
 inline size_t tile_smem(const Tile& t) { return (size_t)(t.mode == kGather ? 1 : kTileStages) * t.stage_bytes; }
-inline int tile_grid(const Tile& t) {
-  int per_sm = (int)((216 << 10) / (tile_smem(t) + 1024));
-  per_sm = per_sm < 1 ? 1 : per_sm > 8 ? 8 : per_sm;
-  return (int)(t.ntiles < kSMs * per_sm ? t.ntiles : kSMs * per_sm);
+
+// Blocks of a kernel that an SM holds, remembered per host thread (asking
+// takes longer than a launch): a persistent grid of more would leave some of
+// them to run alone after the others. Also allows the kernel its shared
+// memory where that is above the default (44 KB, with the kernels' static
+// shared memory).
+template <typename K>
+inline int blocks_per_sm(K* kernel, int threads, size_t smem) {
+  struct Known {
+    const void* kernel;
+    size_t smem;
+    int dev, blocks;
+  };
+  static thread_local Known known[256];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const void* f = reinterpret_cast<const void*>(kernel);
+  Known& k = known[((reinterpret_cast<uintptr_t>(f) >> 4) * 2654435761u + smem / 16 * 40503u + dev) % 256];
+  if (k.kernel == f && k.smem == smem && k.dev == dev) return k.blocks;
+  if (smem > 44 << 10 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return 0;
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) return 0;
+  k = {f, smem, dev, n};
+  return n;
 }
+// *blocks: the size of the grid.
 template <typename K, typename A>
-inline cudaError_t launch_tile(K* kernel, const Tile& t, cudaStream_t st, const A& a) {
+inline cudaError_t launch_tile(K* kernel, const Tile& t, int* blocks, cudaStream_t st, const A& a) {
   const size_t smem = tile_smem(t);
-  if (smem > 48 << 10) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
-  kernel<<<tile_grid(t), kTileThreads, smem, st>>>(a);
+  const int per_sm = blocks_per_sm(kernel, kTileThreads, smem);
+  if (per_sm < 1) return cudaErrorInvalidConfiguration;
+  *blocks = (int)(t.ntiles < kSMs * per_sm ? t.ntiles : kSMs * per_sm);
+  kernel<<<*blocks, kTileThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -908,27 +930,17 @@ __device__ __forceinline__ Run run_cluster(const Run* mine, int cs, float k) {
 }
 
 // Blocks that share a row: as many as bring the rows to two blocks an SM, in
-// powers of two up to 16, while each keeps a few vectors a thread.
+// powers of two up to 8 (16 were slower: one row of 131072 took 25 us, not 16),
+// while each keeps a few vectors a thread.
 inline int cluster_size(int64_t nrows, int C, int es, int threads) {
   int cs = 1;
   while (cs < 8 && nrows * cs * 2 <= 2 * kSMs && (int64_t)C * es >= (int64_t)threads * 16 * 2 * (cs * 2)) cs *= 2;
   return cs;
 }
 
-// Blocks of `threads` that an SM holds with this much dynamic shared memory
-// (the kernels keep to 64 registers a thread): a persistent grid of more
-// would leave some of them to run alone after the others.
-inline int blocks_per_sm(int threads, size_t smem) {
-  const int by_smem = (int)((227 << 10) / (smem + 4096)), by_threads = 1024 / threads;
-  return by_smem < by_threads ? by_smem : by_threads;
-}
-
 template <typename K, typename A>
 inline cudaError_t launch_cluster(K* kernel, int64_t grid, int threads, int cs, size_t smem, cudaStream_t st, const A& a) {
-  if (smem > 44 << 10) {   // with the kernels' static shared memory, above the default
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
+  if (blocks_per_sm(kernel, threads, smem) < 1) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[1];
   cfg.gridDim = dim3((unsigned)grid);
@@ -936,10 +948,6 @@ inline cudaError_t launch_cluster(K* kernel, int64_t grid, int threads, int cs, 
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   if (cs > 1) {
-    if (cs > 8) {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return e;
-    }
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = cs;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
