@@ -18,7 +18,7 @@ namespace distill {
 constexpr int kMostSlots = 4;   // pairs of a lane; kernels hold two or four
 
 template <typename T, int G, int E, int UB, bool BWD, int kSlots, bool PLAIN>
-__global__ void __launch_bounds__(kTileThreads) tile_kernel(Args a) {
+__global__ void __launch_bounds__(kTileThreads, kSlots == 2 ? 4 : 3) tile_kernel(Args a) {
   constexpr int ES = (int)sizeof(T);
   const float k = a.inv_t * kLog2e;
   const bool rest = a.rest;
