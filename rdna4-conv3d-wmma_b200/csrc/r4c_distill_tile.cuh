@@ -17,8 +17,14 @@ namespace distill {
 
 constexpr int kMostSlots = 4;   // pairs of a lane; kernels hold two or four
 
+// Blocks an SM should hold: issue-bound kernels gain from more warps as long
+// as nothing spills.
+constexpr int tile_blocks(int g, int e, int slots, bool bwd) {
+  return g == 1 && e <= 8 && slots == 2 ? (bwd ? 6 : 8) : slots == 2 ? 4 : 3;
+}
+
 template <typename T, int G, int E, int UB, bool BWD, int kSlots, bool PLAIN>
-__global__ void __launch_bounds__(kTileThreads, kSlots == 2 ? 4 : 3) tile_kernel(Args a) {
+__global__ void __launch_bounds__(kTileThreads, tile_blocks(G, E, kSlots, BWD)) tile_kernel(Args a) {
   constexpr int ES = (int)sizeof(T);
   const float k = a.inv_t * kLog2e;
   const bool rest = a.rest;

@@ -418,12 +418,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
       uint4 w[U];
       float vm[U];
       stream.take(w);
+      if (left < U * NT) {   // the last batch: nothing past the row
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (left < U * NT && tid + i * NT >= left)
-          w[i] = make_uint4(Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf);
-        vm[i] = Vec<T>::top(w[i]);
+        for (int i = 0; i < U; ++i)
+          if (tid + i * NT >= left)
+            w[i] = make_uint4(Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf, Word<T>::kNegInf);
       }
+#pragma unroll
+      for (int i = 0; i < U; ++i) vm[i] = Vec<T>::top(w[i]);
       const float bm = fmaxf(fmaxf(vm[0], vm[1]), fmaxf(vm[2], vm[3]));
       run2_raise<true>(part, bm, k);
       run2_batch<VE, U>(part, k, [&](int i, float* y) { Vec<T>::split(i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3], y); });

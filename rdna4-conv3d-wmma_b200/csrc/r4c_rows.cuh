@@ -740,9 +740,14 @@ struct VecRing {
   // Vectors p[i * NT] for i * NT < left (left counts from this thread's first); any left: the batch is counted.
   __device__ __forceinline__ void issue(const uint4* p, int left) {
     const uint32_t d = base + in * (U * NT * 16);
+    if ((U - 1) * NT < left) {
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (i * NT < left) sm100::cp_async_16(d + i * (NT * 16), p + i * NT, 16);
+      for (int i = 0; i < U; ++i) sm100::cp_async_16(d + i * (NT * 16), p + i * NT, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < U - 1; ++i)
+        if (i * NT < left) sm100::cp_async_16(d + i * (NT * 16), p + i * NT, 16);
+    }
     sm100::cp_async_commit();
     in = in == S - 1 ? 0 : in + 1;
   }
