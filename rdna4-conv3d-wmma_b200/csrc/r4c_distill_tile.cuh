@@ -8,6 +8,13 @@
 // places set to -inf) before it is loaded, so that the loops over classes know
 // nothing of the list; in the backward the pairs' lanes write the listed
 // classes' gradients over the row at the end.
+//
+// Issue slots bound both directions (0.70 to 0.78 of them used). B200, kernel
+// alone: 4.2M rows of 4 bf16 classes, two pairs and a rest, 57 us forward and
+// 61 us backward (0.27 and 0.34 of a copy's rate; 310 and 370 instructions a
+// row, of which reading the pairs is 15, the loss 20); 369k rows of 105
+// classes with eight pairs 50 and 68 us. Tests of the list per class instead
+// took 171 and 203 us there.
 #pragma once
 
 #include "r4c_distill.cuh"

@@ -7,8 +7,9 @@
 //
 // The difference z_c - max z is taken before it is scaled, so rows of the
 // type's lowest value stay a uniform distribution instead of overflowing.
-// Both directions read each logit once and are bound by memory; the kernels
-// for short and long rows are described in r4c_rows.cuh.
+// Both directions read each logit once; how short and long rows are read is
+// described in r4c_rows.cuh. Figures below: B200, kernel alone, L2 flushed;
+// "of copy" is against a copy's 6.55 TB/s.
 #include "r4c_rows.cuh"
 
 namespace r4c {
@@ -91,6 +92,15 @@ template <> struct TopKey<float> {
   static __device__ __forceinline__ float value(long long k) { return key_value((uint64_t)k ^ 0x8000000000000000ull); }
 };
 
+// Short rows, forward. With the whole row in the registers of G lanes the
+// maximum is known before the first exponential, so there is no rescaling;
+// the entropy comes from sum 2^t t in the same pass, and the alternatives
+// from rounds of a maximum over unique keys (two of them, of a lane's own
+// row, from one pass that keeps the two largest). What it does beyond the
+// exponentials bounds it: 4.2M rows of 4 bf16 classes with labels and two
+// alternatives take 41 us, 0.69 of copy, at 210 instructions a row, of which
+// the alternatives are 70, the label 30 and the sums 27; 369k rows of 105
+// fp16 classes 38 us, 0.34 of copy, at 0.75 of the issue slots.
 template <typename T, int G, int E, int UB>
 __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
   const float k = a.inv_t * kLog2e;
@@ -178,6 +188,10 @@ __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
   });
 }
 
+// Short rows, backward: dz_c = 2^t (c0 - cb t) with the row's constants, then
+// the label's own term. The sums are computed again: reading them back would
+// be 8 bytes a row, as much as four bf16 logits. 369k rows of 105 fp16
+// classes take 61 us (0.40 of copy, 0.73 of the issue slots).
 template <typename T, int G, int E, int UB>
 __global__ void __launch_bounds__(kTileThreads) bwd_tile_kernel(BwdArgs a) {
   const float k = a.inv_t * kLog2e;
@@ -377,6 +391,16 @@ __device__ __noinline__ void select_top(const uint4* p, const T* row, int off, i
   __syncthreads();
 }
 
+// Long rows, forward: one pass with a running maximum and sums, in batches of
+// four vectors a thread that are copied ahead, across the rows' ends too. The
+// exponential unit bounds it for 16-bit logits (16 a clock and SM, 0.6 to 0.7
+// of it busy), the memory for fp32: 4096 rows of 131072 bf16 classes 199 us
+// (0.82 of copy), 4096 of 65536 fp32 178 us (0.92); with one alternative
+// 237 us, with twenty 250 us: noting the quarters' maxima costs 18 us, finding
+// the classes 20 to 35 us, more where the rows under way (592 of 256 KB) pass
+// L2. A third batch in flight changed nothing (two: 129 us, three: 137 us for
+// 2048 rows with four alternatives). One row of 131072 takes 16 us with
+// twenty alternatives, 10 us without, on eight blocks.
 constexpr int kBatch = 4, kStages = 2;
 template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
@@ -511,7 +535,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
   }
 }
 
-// One block per piece of a row.
+// Long rows, backward: elementwise from two saved numbers a row, one block per
+// piece of a row; memory bounds it. 4095 rows of 32771 bf16 classes, with the
+// entropy's gradient, 100 us (0.82 of copy; the rows' odd ends and the clamp
+// of masked classes cost what is missing). Pieces of 4 vectors a thread
+// instead of 16 took 120 us: what a block reads before it starts is the same.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) bwd_block_kernel(BwdArgs a) {
   extern __shared__ __align__(16) uint8_t ring[];

@@ -603,7 +603,11 @@ def ce_backward(logits_cl: torch.Tensor, target: torch.Tensor, ignore_index: int
 # Rows of logits: log-probabilities (r4c_logp_*), distillation (r4c_distill_*)
 # ---------------------------------------------------------------------------
 TOPK_MAX = 128
-_TILE_CLASSES = 32    # rows up to this many classes are read with any class stride
+# Rows up to this many classes are read with any class stride; wider ones are
+# copied class-last first (105 bf16 classes laid out class first: 193 + 62 us
+# forward + backward with the copy, 102 + 187 us gathered; 300 classes: 647 +
+# 206 against 858 + 1650 us).
+_TILE_CLASSES = 32
 
 
 def _row_strides(t: torch.Tensor):
