@@ -379,7 +379,7 @@ extern "C" int r4c_distill_fwd(const r4c_rows_desc* d, const void* logits, int k
     e = cudaGetLastError();
     note_launches(1);
   }
-  return e == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
+  return rows::status(e);
 }
 
 extern "C" int r4c_distill_bwd(const r4c_rows_desc* d, const void* logits, int k, const void* teacher_logp,
@@ -404,5 +404,5 @@ extern "C" int r4c_distill_bwd(const r4c_rows_desc* d, const void* logits, int k
   else if (d->dtype == R4C_F16) e = distill::launch_bwd<__half>(a, s);
   else e = distill::launch_bwd<float>(a, s);
   note_launches(1);
-  return e == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
+  return rows::status(e);
 }

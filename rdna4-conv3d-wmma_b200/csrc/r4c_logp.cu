@@ -668,7 +668,7 @@ extern "C" int r4c_logp_fwd(const r4c_rows_desc* d, const void* logits, const in
   else if (d->dtype == R4C_F16) e = logp::launch_fwd<__half>(a, s);
   else e = logp::launch_fwd<float>(a, s);
   note_launches(1);
-  return e == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
+  return rows::status(e);
 }
 
 extern "C" int r4c_logp_bwd(const r4c_rows_desc* d, const void* logits, const int64_t* target, int64_t ignore_index,
@@ -691,5 +691,5 @@ extern "C" int r4c_logp_bwd(const r4c_rows_desc* d, const void* logits, const in
   else if (d->dtype == R4C_F16) e = logp::launch_bwd<__half>(a, s);
   else e = logp::launch_bwd<float>(a, s);
   note_launches(1);
-  return e == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
+  return rows::status(e);
 }

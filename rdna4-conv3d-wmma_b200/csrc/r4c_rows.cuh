@@ -53,6 +53,12 @@ struct View {
 inline bool valid_desc(const r4c_rows_desc* d) {
   return d && d->rows >= 0 && d->inner > 0 && d->classes > 0 && std::isfinite(d->temperature) && d->temperature > 0.f;
 }
+// The entry's status; a failed launch leaves no error behind for the next call to find.
+inline int status(cudaError_t e) {
+  if (e == cudaSuccess) return R4C_OK;
+  cudaGetLastError();
+  return R4C_ERR_CUDA;
+}
 inline bool valid_dtype(int dt) { return dt == R4C_BF16 || dt == R4C_F16 || dt == R4C_F32; }
 inline View make_view(const r4c_rows_desc* d) {
   return {d->inner >= d->rows ? 0 : d->inner, d->outer_stride, d->inner_stride, d->class_stride};
@@ -512,6 +518,7 @@ inline size_t tile_smem(const Tile& t) { return (size_t)(t.mode == kGather ? 1 :
 // them to run alone after the others. Also allows the kernel its shared
 // memory where that is above the default (44 KB, with the kernels' static
 // shared memory).
+constexpr int kMostShared = 200 << 10;
 template <typename K>
 inline int blocks_per_sm(K* kernel, int threads, size_t smem) {
   struct Known {
@@ -525,8 +532,10 @@ inline int blocks_per_sm(K* kernel, int threads, size_t smem) {
   const void* f = reinterpret_cast<const void*>(kernel);
   Known& k = known[((reinterpret_cast<uintptr_t>(f) >> 4) * 2654435761u + smem / 16 * 40503u + dev) % 256];
   if (k.kernel == f && k.smem == smem && k.dev == dev) return k.blocks;
+  // the allowance is the kernel's for good, so it is one for all sizes: a later, smaller one would take it back
+  if (smem > kMostShared) return 0;
   if (smem > 44 << 10 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess)
     return 0;
   int n = 0;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) return 0;

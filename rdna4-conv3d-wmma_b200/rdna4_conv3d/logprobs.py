@@ -122,12 +122,12 @@ def _log_probs_torch(logits, target, top_k, temperature, ignore_index) -> LogPro
     m = s.detach().amax(-1, keepdim=True)
     m = torch.where(empty | bad, torch.zeros_like(m), m)
     d = s - m
-    # masked classes leave the graph: their gradient is 0, not 0 * inf
+    # masked classes leave the sums: their share of the gradient is 0, not 0 * inf
     dead = (d == -inf) | bad
     e = torch.where(dead, torch.zeros_like(d), torch.exp(torch.where(dead, torch.zeros_like(d), d)))
     total = e.sum(-1, keepdim=True)
     ln_s = torch.log(torch.where(empty | bad, torch.ones_like(total), total))
-    ln_p = torch.where(d == -inf, torch.full_like(d, -inf), d - ln_s)
+    ln_p = torch.where(empty, torch.full_like(d, -inf), d - ln_s)
     p = e / torch.where(empty | bad, torch.ones_like(total), total)
     entropy = -(p * torch.where(dead, torch.zeros_like(d), ln_p)).sum(-1)
     lse = (m + ln_s).squeeze(-1)

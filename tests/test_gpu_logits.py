@@ -187,6 +187,22 @@ def test_log_probs_differences(cuda_ready, c):
     assert abs(float(diff) - float((dz.double() * u.double()).sum())) <= 1.5e-3
 
 
+def test_sizes_in_any_order(cuda_ready):
+    """One kernel with growing and shrinking tiles: what a launch allows it must not be taken back by another."""
+    from rdna4_conv3d.logprobs import log_probs
+    from rdna4_conv3d.losses import distill_topk
+    for lo, hi in ((33, 63), (66, 127), (129, 255), (260, 511), (520, 1023), (1100, 50021)):
+        for n in (1, 40, 900 if hi < 2000 else 20):
+            for c in (hi, lo, hi, lo + 1, hi - 2, lo, hi):
+                z = torch.zeros(n, c, device="cuda", requires_grad=True)
+                v, idx = torch.zeros(n, 3, device="cuda"), torch.arange(3, device="cuda").expand(n, 3)
+                o = log_probs(z, top_k=2)
+                loss = distill_topk(z, v, idx) + o.entropy.sum()
+                dz, = torch.autograd.grad(loss, z)
+                assert o.top_index[-1].tolist() == [0, 1]
+                assert abs(float(o.lse.detach()[0]) - float(torch.tensor(float(c)).log())) < 1e-4
+
+
 def test_second_derivatives_are_refused(cuda_ready):
     from rdna4_conv3d.logprobs import log_probs
     from rdna4_conv3d.losses import distill_topk

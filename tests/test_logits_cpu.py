@@ -68,6 +68,9 @@ def test_log_probs_special_rows():
         assert_values(getattr(out, name), ref[name], name, 1e-12, 1e-12)
     assert_values(out.top_logp, ref["top_logp"], "top_logp", 1e-12, 1e-12)
     assert torch.equal(out.top_index.long(), ref["top_index"])
+    dz, = torch.autograd.grad((out.logp, out.entropy, out.lse), z, (torch.ones(9, dtype=torch.float64),) * 3)
+    fine = [0, 1, 2, 3, 4, 5, 8]                         # a masked label (row 2) still gets its own term
+    assert torch.allclose(dz[fine], ref["dz"][fine], atol=1e-12)
     assert out.top_index[6].tolist() == [-1] * 6 and out.top_index[1].tolist() == [0, 1, 2, 3, 4, 5]
 
 
