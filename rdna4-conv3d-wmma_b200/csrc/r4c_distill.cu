@@ -293,14 +293,14 @@ template <typename T>
 cudaError_t launch_bwd(Args& a, cudaStream_t s) {
   int blocks;
   if (a.C <= kTileClasses) return launch_tiles<T>(a, true, &blocks, s);
-  const int threads = row_threads(a.C, sizeof(T), a.K);
+  const int threads = row_threads(a.C, sizeof(T), a.K) == kWarpRow ? kWarpRow : kGradRow;
   a.segs = grad_pieces(a.nrows, a.C, sizeof(T), threads);
   if (a.nrows * a.segs > 0x7fffffff) return cudaErrorInvalidConfiguration;
   if (threads == kWarpRow)
     return launch_cluster(bwd_block_kernel<T, kWarpRow>, a.nrows, kWarpRow, 1,
                           VecRing<kWarpRow, kGradBatch, kGradStages>::kBytes, s, a);
-  return launch_cluster(bwd_block_kernel<T, kLongRow>, a.nrows * a.segs, kLongRow, 1,
-                        VecRing<kLongRow, kGradBatch, kGradStages>::kBytes, s, a);
+  return launch_cluster(bwd_block_kernel<T, kGradRow>, a.nrows * a.segs, kGradRow, 1,
+                        VecRing<kGradRow, kGradBatch, kGradStages>::kBytes, s, a);
 }
 
 }  // namespace distill

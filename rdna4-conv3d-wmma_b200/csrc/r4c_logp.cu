@@ -396,10 +396,8 @@ __device__ __noinline__ void select_top(const uint4* p, const T* row, int off, i
 // exponential unit bounds it for 16-bit logits (16 a clock and SM, 0.6 to 0.7
 // of it busy), the memory for fp32: 4096 rows of 131072 bf16 classes 199 us
 // (0.82 of copy), 4096 of 65536 fp32 178 us (0.92); with one alternative
-// 237 us, with twenty 250 us: noting the quarters' maxima costs 18 us, finding
-// the classes 20 to 35 us, more where the rows under way (592 of 256 KB) pass
-// L2. A third batch in flight changed nothing (two: 129 us, three: 137 us for
-// 2048 rows with four alternatives). One row of 131072 takes 16 us with
+// 201 us, with twenty 236 us (128 threads a row; 234 and 250 us with 256). A
+// third batch in flight changed nothing. One row of 131072 takes 16 us with
 // twenty alternatives, 10 us without, on eight blocks.
 constexpr int kBatch = 4, kStages = 2;
 template <typename T, int NT, bool TOP>
@@ -537,9 +535,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
 
 // Long rows, backward: elementwise from two saved numbers a row, one block per
 // piece of a row; memory bounds it. 4095 rows of 32771 bf16 classes, with the
-// entropy's gradient, 100 us (0.82 of copy; the rows' odd ends and the clamp
-// of masked classes cost what is missing). Pieces of 4 vectors a thread
-// instead of 16 took 120 us: what a block reads before it starts is the same.
+// entropy's gradient, 90 us (0.91 of copy; 101 us with 256 threads). Pieces
+// of 4 vectors a thread instead of 16 took 120 us: what a block reads before it
+// starts is the same.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) bwd_block_kernel(BwdArgs a) {
   extern __shared__ __align__(16) uint8_t ring[];
@@ -604,6 +602,7 @@ cudaError_t launch_fwd(FwdArgs& a, cudaStream_t s) {
     });
   }
   if (row_threads(a.C, sizeof(T), a.K) == kWarpRow) return launch_fwd_block<T, kWarpRow>(a, s);
+  if (a.K > 0 && a.nrows >= 4 * kSMs) return launch_fwd_block<T, kManyRows>(a, s);
   return launch_fwd_block<T, kLongRow>(a, s);
 }
 
@@ -618,14 +617,14 @@ cudaError_t launch_bwd(BwdArgs& a, cudaStream_t s) {
       return launch_tile(bwd_tile_kernel<T, decltype(c)::G, decltype(c)::E, decltype(c)::UB>, a.tile, &blocks, s, a);
     });
   }
-  const int threads = row_threads(a.C, sizeof(T), 0);
+  const int threads = row_threads(a.C, sizeof(T), 0) == kWarpRow ? kWarpRow : kGradRow;
   a.segs = grad_pieces(a.nrows, a.C, sizeof(T), threads);
   if (a.nrows * a.segs > 0x7fffffff) return cudaErrorInvalidConfiguration;
   if (threads == kWarpRow)
     return launch_cluster(bwd_block_kernel<T, kWarpRow>, a.nrows, kWarpRow, 1,
                           VecRing<kWarpRow, kGradBatch, kGradStages>::kBytes, s, a);
-  return launch_cluster(bwd_block_kernel<T, kLongRow>, a.nrows * a.segs, kLongRow, 1,
-                        VecRing<kLongRow, kGradBatch, kGradStages>::kBytes, s, a);
+  return launch_cluster(bwd_block_kernel<T, kGradRow>, a.nrows * a.segs, kGradRow, 1,
+                        VecRing<kGradRow, kGradBatch, kGradStages>::kBytes, s, a);
 }
 
 }  // namespace logp

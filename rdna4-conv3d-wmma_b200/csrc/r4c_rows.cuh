@@ -40,7 +40,11 @@ constexpr int kSMs = 148;
 // 63 us forward and 87 us backward with 128 and 256 threads, 29 and 29 us with
 // 32. More than 32 pairs or alternatives take 256, so that each pair has a
 // thread and there are maxima enough to choose from.
-constexpr int kWarpRow = 32, kLongRow = 256;
+// (Where they are many, 128 threads do better for alternatives, whose search
+// fewer warps then wait for: 4096 rows of 131072 with one take 201 us, not 234;
+// without alternatives 218, not 196. Gradients take 128 as well: 4095 rows of
+// 32771 with the entropy's 90 us, not 101.)
+constexpr int kWarpRow = 32, kLongRow = 256, kManyRows = 128, kGradRow = 128;
 inline int row_threads(int C, int es, int k) { return (int64_t)C * es <= 16 << 10 && k <= kWarpRow ? kWarpRow : kLongRow; }
 
 struct View {
