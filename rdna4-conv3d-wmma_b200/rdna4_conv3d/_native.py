@@ -664,6 +664,48 @@ class Rows:
         self.desc = RowsDesc(n, inner or 1, so, si, sc, so, si, sc, c, dtype_code(z.dtype), temperature)
 
 
+class SavedRows:
+    """What a backward knows of its forward's rows beside the tensors it saved.
+    A saved tensor may come back as another one with the same values (hooks
+    that offload or pack what autograd keeps): other strides get a descriptor
+    of their own, another shape, type or device never reaches a kernel."""
+    __slots__ = ("desc", "shape", "_z")
+
+    def __init__(self, rows: Rows):
+        z = rows.z
+        self.desc, self.shape, self._z = rows.desc, rows.shape, (z.shape, z.stride(), z.dtype, z.device)
+
+    def logits(self, z: torch.Tensor):
+        """(logits as the kernels read them, their descriptor)."""
+        shape, stride, dtype, device = self._z
+        _as_saved(z, shape, dtype, device)
+        if z.stride() == stride:
+            return z, self.desc
+        rows = Rows(z, self.desc.temperature)
+        return rows.z, rows.desc
+
+    def dense(self, t: Optional[torch.Tensor], dtype: torch.dtype, *more: int) -> Optional[torch.Tensor]:
+        """A per-row tensor (N, ..., *more) as the kernels read it."""
+        if t is None:
+            return None
+        _as_saved(t, (*self.shape, *more) if more else self.shape, dtype, self._z[3])
+        return t.contiguous()
+
+    def buffer(self, t: Optional[torch.Tensor], nbytes: int) -> Optional[torch.Tensor]:
+        """A forward's own bytes for its backward, 16-byte aligned."""
+        if t is None:
+            return None
+        _as_saved(t, (nbytes,), torch.uint8, self._z[3])
+        t = t.contiguous()
+        return t.clone() if t.data_ptr() & 15 else t
+
+
+def _as_saved(t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> None:
+    if t.dtype != dtype or t.shape != shape or t.device != device:
+        raise RuntimeError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, "
+                           f"saved was {dtype} {tuple(shape)} on {device}")
+
+
 def rows_grad(z: torch.Tensor, desc: RowsDesc) -> torch.Tensor:
     """A new tensor for the gradient of rows that lie as ``z``; sets the descriptor's gradient strides."""
     dz = torch.empty_like(z)

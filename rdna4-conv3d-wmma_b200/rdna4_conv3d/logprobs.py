@@ -57,7 +57,8 @@ class LogProbsFn(torch.autograd.Function):
         logp, entropy, lse, top_logp, top_index, stats = _native.logp_forward(rows, target, ignore_index, top_k, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(rows.z, target, entropy, stats)
-        ctx.desc, ctx.ignore_index = rows.desc, ignore_index
+        ctx.rows, ctx.ignore_index = _native.SavedRows(rows), ignore_index
+        ctx.stats_bytes = 0 if stats is None else stats.numel()
         if top_k:
             ctx.mark_non_differentiable(top_logp, top_index)
         return logp, entropy, lse, top_logp, top_index
@@ -66,7 +67,11 @@ class LogProbsFn(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy, g_lse, _top_logp, _top_index):
         refuse_twice()
         z, target, entropy, stats = ctx.saved_tensors
-        dz = _native.logp_backward(z, ctx.desc, target, ctx.ignore_index, entropy, stats, g_logp, g_entropy, g_lse)
+        rows = ctx.rows
+        z, desc = rows.logits(z)
+        target, entropy = rows.dense(target, torch.int64), rows.dense(entropy, torch.float32)
+        stats = rows.buffer(stats, ctx.stats_bytes)
+        dz = _native.logp_backward(z, desc, target, ctx.ignore_index, entropy, stats, g_logp, g_entropy, g_lse)
         return dz, None, None, None, None
 
 

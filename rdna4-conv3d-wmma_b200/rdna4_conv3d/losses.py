@@ -62,14 +62,19 @@ class DistillTopKFn(torch.autograd.Function):
         rows = _native.Rows(logits, temperature)
         loss, state = _native.distill_forward(rows, teacher_logp, teacher_index, rest, weight, mean)
         ctx.save_for_backward(rows.z, teacher_logp, teacher_index, weight, state)
-        ctx.desc, ctx.rest, ctx.mean = rows.desc, rest, mean
+        ctx.rows, ctx.rest, ctx.mean = _native.SavedRows(rows), rest, mean
+        ctx.teacher = teacher_logp.dtype, teacher_index.dtype, teacher_logp.shape[-1], state.numel()
         return loss
 
     @staticmethod
     def backward(ctx, grad):
         refuse_twice()
         z, teacher_logp, teacher_index, weight, state = ctx.saved_tensors
-        dz = _native.distill_backward(z, ctx.desc, teacher_logp, teacher_index, ctx.rest, weight, ctx.mean, state, grad)
+        rows, (logp_dtype, index_dtype, k, nbytes) = ctx.rows, ctx.teacher
+        z, desc = rows.logits(z)
+        teacher_logp, teacher_index = rows.dense(teacher_logp, logp_dtype, k), rows.dense(teacher_index, index_dtype, k)
+        weight, state = rows.dense(weight, torch.float32), rows.buffer(state, nbytes)
+        dz = _native.distill_backward(z, desc, teacher_logp, teacher_index, ctx.rest, weight, ctx.mean, state, grad)
         return dz, None, None, None, None, None, None
 
 

@@ -1,0 +1,58 @@
+"""log_probs and distill_topk on a B200 where rows, layouts or callers are unusual.
+
+Each test compares with the 64-bit definitions, or with another call of the
+same operator that the definitions say is the same.
+"""
+from contextlib import nullcontext
+
+import pytest
+import torch
+
+from logit_refs import assert_grad, rows_of
+from test_gpu_logits import BF, _gen, _logits, _teacher
+
+pytestmark = pytest.mark.gpu
+
+
+def _transposed_copy(t):
+    """The same values in the opposite memory order."""
+    back = tuple(reversed(range(t.dim())))
+    return t.clone().permute(back).contiguous().permute(back)
+
+
+@pytest.mark.parametrize("hooks", ["cpu", "pinned", "transposed"])
+@pytest.mark.parametrize("c", [4, 105, 1030])
+@pytest.mark.parametrize("view", ["slice", "last", "first", "wide"])
+def test_gradients_under_saved_tensor_hooks(cuda_ready, view, c, hooks):
+    """Saved tensors that come back with other strides: each row's gradient is that of the same call without hooks.
+    Other places of a row's classes in the kernels' lanes add its sums in another order, hence the derived bounds."""
+    from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
+    from rdna4_conv3d.logprobs import log_probs
+    from rdna4_conv3d.losses import distill_topk
+    if view == "slice":
+        z = _logits((5, c + 14), BF)[:, 3:c + 3]
+    elif view == "last":
+        z = _logits((2, c, 3, 4, 5), BF).contiguous(memory_format=torch.channels_last_3d)
+    elif view == "first":
+        z = _logits((2, c, 3, 4, 5), BF)
+    else:
+        z = _logits((2, c + 3, 3, 4, 5), BF).contiguous(memory_format=torch.channels_last_3d)[:, 1:c + 1]
+    z.requires_grad_(True)
+    rows = z.shape[:1] + z.shape[2:]
+    t = torch.randint(0, c, rows, device="cuda", generator=_gen(2))
+    v, idx = _teacher(rows.numel(), c, 3)
+    v, idx = v.view(*rows, 3), idx.view(*rows, 3)
+    wt = torch.rand(rows, device="cuda", generator=_gen(3))
+
+    def grads(hook):
+        with hook():
+            o = log_probs(z, t, temperature=2.0)
+            loss = distill_topk(z, v, idx, temperature=2.0, rest=c > 4, weight=wt, reduction="none")
+        a, = torch.autograd.grad(o.logp.sum() - o.entropy.sum(), z)
+        b, = torch.autograd.grad(loss.sum(), z)
+        return rows_of(a), rows_of(b)
+
+    hook = {"cpu": save_on_cpu, "pinned": lambda: save_on_cpu(pin_memory=True),
+            "transposed": lambda: saved_tensors_hooks(_transposed_copy, lambda x: x)}[hooks]
+    for got, want in zip(grads(hook), grads(nullcontext)):
+        assert_grad(got, want, BF)
