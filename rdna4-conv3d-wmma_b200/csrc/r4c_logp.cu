@@ -214,6 +214,10 @@ __global__ void __launch_bounds__(kTileThreads) bwd_tile_kernel(BwdArgs a) {
     float zt = 0.f;
     if (t >= 0) zt = sh_get<T>(row + t * (int)sizeof(T));
     x.each2([&](float2 q) { return __fmul2_rn(make_float2(ex2(q.x), ex2(q.y)), __ffma2_rn(b2, q, c2)); });
+    if (none) {   // not 0 * NaN
+#pragma unroll
+      for (int e = 0; e < E; ++e) x.v[e] = 0.f;
+    }
     if (G > 1) __syncwarp();   // every lane has read the row (and the label's logit)
     if (in) x.store(x.v);
     if (G > 1) __syncwarp();

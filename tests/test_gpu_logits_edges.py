@@ -8,8 +8,8 @@ from contextlib import nullcontext
 import pytest
 import torch
 
-from logit_refs import assert_grad, rows_of
-from test_gpu_logits import BF, _gen, _logits, _teacher
+from logit_refs import NEG, assert_grad, log_probs_ref, rows_of
+from test_gpu_logits import BF, DTYPES, _gen, _logits, _teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,31 @@ def test_gradients_under_saved_tensor_hooks(cuda_ready, view, c, hooks):
             "transposed": lambda: saved_tensors_hooks(_transposed_copy, lambda x: x)}[hooks]
     for got, want in zip(grads(hook), grads(nullcontext)):
         assert_grad(got, want, BF)
+
+
+@DTYPES
+@pytest.mark.parametrize("c", [4, 7, 105, 1000, 3000])
+def test_a_bad_row_without_upstream_gradient_has_none(cuda_ready, c, dtype):
+    """0 times NaN is not a gradient: rows that hold a NaN or +inf and are ignored (or whose upstream values are all
+    zero) leave the weights alone; with an upstream gradient they are NaN; so it is in the 64-bit definition."""
+    from rdna4_conv3d.logprobs import log_probs
+    z = _logits((8, c), dtype)
+    z[1, c // 2] = float("nan")
+    z[2, c - 1] = float("inf")
+    z[3] = float("nan")
+    z[4, 0] = float("nan")
+    z[5] = NEG
+    z.requires_grad_(True)
+    t = torch.arange(8, device="cuda") % c
+    t[1:4] = -100
+    ones, zeros = torch.ones(8).double(), torch.zeros(8).double()
+    out = log_probs(z, t)
+    dz, = torch.autograd.grad(out.logp.sum(), z)
+    ref = log_probs_ref(rows_of(z), t.cpu(), 0, 1.0, -100, ones)
+    assert not ref["dz"][1:4].any() and bool(ref["dz"][4].isnan().all())
+    assert_grad(rows_of(dz), ref["dz"], dtype)
+    out = log_probs(z, t)
+    gh = ones.clone()
+    gh[[1, 3, 4]] = 0.0
+    dz, = torch.autograd.grad((out.logp, out.entropy), z, (zeros.float().cuda(), gh.float().cuda()))
+    assert_grad(rows_of(dz), log_probs_ref(rows_of(z), t.cpu(), 0, 1.0, -100, zeros, gh)["dz"], dtype)
