@@ -151,7 +151,9 @@ def _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weigh
     part = valid.any(-1) & ~(z == -inf).all(-1) & (w != 0)
     w = torch.where(part, w, zero)
     z = torch.where(part.unsqueeze(-1), z, zero)
-    s = z / temperature
+    # differences from a maximum, taken before they are scaled: far from zero, lse would swallow ln S
+    m = z.detach().amax(-1, keepdim=True)
+    s = (z - m) / temperature
     lse = torch.logsumexp(s, -1, keepdim=True)
     v = torch.where(valid, v, zero - inf)
     if not rest:
@@ -164,11 +166,15 @@ def _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weigh
         qr = 1.0 - q.sum(-1)
         qr = torch.where(qr >= 1e-6, qr, zero)
         seen = torch.zeros(z.shape, dtype=torch.int64, device=z.device).scatter_add(-1, i, valid.long()) > 0
-        alive = ~seen & (s != -inf)
+        alive = ~seen & (z != -inf)
         any_alive = alive.any(-1)
-        lse_r = torch.logsumexp(torch.where(alive | ~any_alive.unsqueeze(-1), s, zero - inf), -1)
-        lse_r = torch.where(any_alive, lse_r, zero - inf)
-        rest_term = qr * (torch.log(torch.where(qr > 0, qr, zero + 1.0)) - lse_r + lse.squeeze(-1))
+        # the unlisted classes from a maximum of their own, which may lie far below the row's
+        mr = torch.where(alive, z.detach(), zero - inf).amax(-1, keepdim=True)
+        mr = torch.where(any_alive.unsqueeze(-1), mr, m)
+        sr = torch.where(alive, (z - mr) / temperature, zero - inf)
+        ln_r = torch.logsumexp(torch.where(any_alive.unsqueeze(-1), sr, zero), -1) + ((mr - m) / temperature).squeeze(-1)
+        ln_r = torch.where(any_alive, ln_r, zero - inf)
+        rest_term = qr * (torch.log(torch.where(qr > 0, qr, zero + 1.0)) - ln_r + lse.squeeze(-1))
         row = row + torch.where(qr > 0, rest_term, zero)
     out = torch.float32 if acc == torch.float32 else acc
     row = torch.where(part, temperature * temperature * w * row, zero)

@@ -1,0 +1,51 @@
+"""log_probs and distill_topk on the CPU where rows, types or callers are unusual."""
+import pytest
+import torch
+
+from logit_refs import NEG, assert_grad, assert_values, distill_ref, log_probs_ref, rows_of
+from rdna4_conv3d.losses import distill_topk
+from rdna4_conv3d.logprobs import log_probs
+
+DTYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "fp16", "fp32"])
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _teacher(rows, c, k, seed=3):
+    idx = torch.argsort(torch.rand((rows, c), generator=_gen(seed)), 1)[:, :k]
+    v = torch.randn((rows, k + 1), generator=_gen(seed + 1))
+    return (v - torch.logsumexp(v, 1, keepdim=True))[:, :k], idx
+
+
+@DTYPES
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+@pytest.mark.parametrize("rest", [False, True], ids=["renorm", "rest"])
+def test_distill_of_large_logits(dtype, rest, temperature):
+    """Rows far from zero, where a log-sum-exp of the logits themselves swallows ln S; fp32 arithmetic, so the
+    bounds of the kernels: 3e-5 T^2 absolute and 5e-6 relative for a loss."""
+    top, low = torch.finfo(dtype).max, torch.finfo(dtype).min
+    c = 8
+    z = 3 * torch.randn((9, c), generator=_gen(0))
+    z[0] = min(1e9, top)
+    z[1] = low
+    z[2] += 3e4
+    z[3] -= 3e4
+    z[4] = top
+    z = z.to(dtype)
+    v, idx = _teacher(9, c, 3)
+    z[5] = low                                           # the unlisted classes far below the listed ones
+    z[5, idx[5]] = torch.tensor([0.0, 1.0, 2.0]).to(dtype)
+    z[6] = 1.0
+    z[6, idx[6]] = low / 2                               # ... and far above them
+    z[7] = NEG
+    z[7, :4] = low
+    z[8, idx[8]] = NEG
+    z.requires_grad_(True)
+    loss = distill_topk(z, v, idx, temperature=temperature, rest=rest, reduction="none")
+    dz, = torch.autograd.grad(loss, z, torch.ones(9))
+    want, _, dwant = distill_ref(rows_of(z), v.double(), idx, temperature, rest)
+    want = torch.where(want > torch.finfo(torch.float32).max, torch.full_like(want, float("inf")), want)
+    assert_values(loss, want, "loss", 3e-5 * temperature ** 2, 5e-6)
+    assert_grad(rows_of(dz), dwant, dtype)
