@@ -614,6 +614,8 @@ def _row_strides(t: torch.Tensor):
     """(inner, outer stride, inner stride, class stride) of (N, C, ...) logits
     whose dims after the class walk one stride; None when they do not."""
     n, c = int(t.shape[0]), int(t.shape[1])
+    if t.numel() == 0:                   # no rows: nothing to walk
+        return 1, 0, c, 1
     st = t.stride()
     inner, si = 1, 0
     for size, stride in zip(reversed(t.shape[2:]), reversed(st[2:])):

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from logit_refs import NEG, assert_grad, assert_values, distill_ref, log_probs_ref, rows_of
+from rdna4_conv3d import _native
 from rdna4_conv3d.losses import distill_topk
 from rdna4_conv3d.logprobs import log_probs
 
@@ -49,3 +50,23 @@ def test_distill_of_large_logits(dtype, rest, temperature):
     want = torch.where(want > torch.finfo(torch.float32).max, torch.full_like(want, float("inf")), want)
     assert_values(loss, want, "loss", 3e-5 * temperature ** 2, 5e-6)
     assert_grad(rows_of(dz), dwant, dtype)
+
+
+EMPTY = [(0, 4), (0, 4, 2, 2, 2), (2, 4, 0, 3, 3), (2, 4, 3, 0, 3), (2, 4, 3, 3, 0), (2, 4, 0), (2, 40, 3, 0, 0), (2, 1030, 2, 0),
+         (1, 1, 0)]
+
+
+@pytest.mark.parametrize("layout", ["first", "last", "cut"])
+@pytest.mark.parametrize("shape", EMPTY, ids=str)
+def test_empty_maps_have_a_descriptor(shape, layout):
+    z = torch.zeros(shape)
+    if layout == "last":
+        z = z.movedim(1, -1).contiguous().movedim(-1, 1)
+    elif layout == "cut":
+        z = torch.zeros([s + 1 for s in shape])[tuple(slice(0, s) for s in shape)]
+    rows = _native.Rows(z, 1.0)
+    assert rows.desc.rows == 0 and rows.desc.classes == shape[1] and rows.desc.inner > 0
+    assert rows.shape == z.shape[:1] + z.shape[2:] and rows.z.shape == z.shape
+    assert shape[1] <= 1024 or rows.desc.class_stride == 1
+    assert _native.rows_grad(rows.z, rows.desc).shape == z.shape
+    assert shape[1] <= 1024 or rows.desc.grad_class_stride == 1
