@@ -355,6 +355,7 @@ extern "C" int r4c_distill_fwd(const r4c_rows_desc* d, const void* logits, int k
                                r4c_stream_t stream) {
   const int rc = check(d, k, teacher_logp, teacher_dtype, teacher_index, index_bits, rest);
   if (rc != R4C_OK) return rc;
+  if (d->rows == 0 && !loss) return R4C_OK;
   if ((!row_loss && !loss) || (d->rows > 0 && !logits)) return R4C_ERR_INVALID;
   if (!state || state_bytes < r4c_distill_state_size(d)) return R4C_ERR_WORKSPACE;
   if ((uintptr_t)state & 15) return R4C_ERR_ALIGN;

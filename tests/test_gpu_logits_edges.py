@@ -84,3 +84,21 @@ def test_a_bad_row_without_upstream_gradient_has_none(cuda_ready, c, dtype):
     gh[[1, 3, 4]] = 0.0
     dz, = torch.autograd.grad((out.logp, out.entropy), z, (zeros.float().cuda(), gh.float().cuda()))
     assert_grad(rows_of(dz), log_probs_ref(rows_of(z), t.cpu(), 0, 1.0, -100, zeros, gh)["dz"], dtype)
+
+
+@pytest.mark.parametrize("shape", [(0, 4), (2, 4, 0, 3, 3), (2, 4, 3, 0, 3), (2, 4, 3, 3, 0), (2, 40, 3, 0, 0), (2, 1030, 2, 0)],
+                         ids=str)
+def test_empty_maps(cuda_ready, shape):
+    from rdna4_conv3d.logprobs import log_probs
+    from rdna4_conv3d.losses import distill_topk
+    z = torch.zeros(shape, dtype=BF, device="cuda", requires_grad=True)
+    rows = z.shape[:1] + z.shape[2:]
+    out = log_probs(z, torch.zeros(rows, dtype=torch.long, device="cuda"), top_k=2)
+    assert out.logp.shape == rows and out.top_index.shape == (*rows, 2)
+    assert torch.autograd.grad(out.entropy.sum(), z)[0].shape == z.shape
+    v, idx = torch.zeros((*rows, 3), device="cuda"), torch.zeros((*rows, 3), dtype=torch.int32, device="cuda")
+    for rest in (False, True):
+        none = distill_topk(z, v, idx, rest=rest, reduction="none")
+        assert none.shape == rows and torch.autograd.grad(none.sum(), z)[0].shape == z.shape
+        mean = distill_topk(z, v, idx, rest=rest)
+        assert torch.isnan(mean) and torch.autograd.grad(mean, z)[0].shape == z.shape

@@ -70,3 +70,16 @@ def test_empty_maps_have_a_descriptor(shape, layout):
     assert shape[1] <= 1024 or rows.desc.class_stride == 1
     assert _native.rows_grad(rows.z, rows.desc).shape == z.shape
     assert shape[1] <= 1024 or rows.desc.grad_class_stride == 1
+
+
+def test_the_c_entry_of_distill_takes_no_rows():
+    """An empty tensor has a null address: the rows' losses of no rows are nothing to write."""
+    L = _native.lib()
+    d = _native.RowsDesc(0, 1, 0, 8, 1, 0, 8, 1, 8, _native.R4C_BF16, 1.0)
+    nothing = [None] * 2
+    assert L.r4c_distill_fwd(d, None, 2, None, _native.R4C_F32, None, 32, 0, None, *nothing, None, 0, None) == 0
+    assert L.r4c_distill_fwd(d, None, 0, None, _native.R4C_F32, None, 32, 0, None, *nothing, None, 0, None) == -1
+    d.rows, d.inner = 4, 4                               # rows, and no place for their losses
+    one = torch.zeros(16)
+    at = one.data_ptr()
+    assert L.r4c_distill_fwd(d, at, 2, at, _native.R4C_F32, at, 32, 0, None, *nothing, None, 0, None) == -1
