@@ -136,8 +136,9 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
 
 
 def _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weight, reduction):
-    """The same loss in torch operations, at least in fp32."""
-    acc = torch.promote_types(logits.dtype, torch.float32)
+    """The same loss in torch operations, in 64 bits: the gradient is a difference of probabilities, and torch's
+    own roundings of each would be what is left of it where the student agrees with the teacher."""
+    acc = torch.float64
     inf = float("inf")
     z = logits.movedim(1, -1).to(acc)
     v, i = teacher_logp.detach().to(acc), teacher_index.to(torch.int64)
@@ -176,7 +177,7 @@ def _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weigh
         ln_r = torch.where(any_alive, ln_r, zero - inf)
         rest_term = qr * (torch.log(torch.where(qr > 0, qr, zero + 1.0)) - ln_r + lse.squeeze(-1))
         row = row + torch.where(qr > 0, rest_term, zero)
-    out = torch.float32 if acc == torch.float32 else acc
+    out = torch.promote_types(logits.dtype, torch.float32)
     row = torch.where(part, temperature * temperature * w * row, zero)
     if reduction == "none":
         return row.to(out)

@@ -83,3 +83,17 @@ def test_the_c_entry_of_distill_takes_no_rows():
     one = torch.zeros(16)
     at = one.data_ptr()
     assert L.r4c_distill_fwd(d, at, 2, at, _native.R4C_F32, at, 32, 0, None, *nothing, None, 0, None) == -1
+
+
+@pytest.mark.parametrize("rest", [False, True], ids=["renorm", "rest"])
+@pytest.mark.parametrize("gap", [0.1, 1e-3, 1e-6])
+def test_distill_gradient_where_the_student_agrees(gap, rest):
+    """p - q of fp32 logits close to the teacher's own: rounded once, not left to the roundings of p and q."""
+    want_p = torch.log_softmax(3 * torch.randn((300, 2), generator=_gen(0), dtype=torch.float64), 1).float()
+    z = (want_p + gap * torch.randn((300, 2), generator=_gen(1))).requires_grad_(True)
+    idx = torch.tensor([1, 0]).expand(300, 2)
+    v = want_p[:, [1, 0]]
+    loss = distill_topk(z, v, idx, rest=rest, reduction="none")
+    dz, = torch.autograd.grad(loss.sum(), z)
+    _, _, want = distill_ref(rows_of(z), v.double(), idx, 1.0, rest)
+    assert_grad(dz, want, torch.float32)
