@@ -409,10 +409,11 @@ int r4c_logp_bwd(const r4c_rows_desc* desc, const void* logits, const int64_t* t
  * A pair with a negative class or log-probability -inf is void; a class >= C
  * is void and sets code 6 in the device error flag; a class listed twice
  * counts with both its q. q_r below 1e-6 is the rounding of the sum and counts
- * as 0. A row takes no part (weight 0, gradient 0) when all its pairs are
- * void, its weight is 0 or it has no finite logit. teacher_logp is bf16, fp16
- * or fp32, teacher_index 32- or 64-bit integers (index_bits), weight (fp32,
- * >= 0) may be null: 1 for every row.
+ * as 0; so does, where every unlisted class is -inf or none is left, what the
+ * rounding of 16-bit log-probabilities explains. A row takes no part (weight
+ * 0, gradient 0) when all its pairs are void, its weight is 0 or it has no
+ * finite logit. teacher_logp is bf16, fp16 or fp32, teacher_index 32- or
+ * 64-bit integers (index_bits), weight (fp32, >= 0) may be null: 1 for every row.
  * r4c_distill_fwd writes row_loss[r] = w[r] L[r] (may be null) or, with loss
  * given, loss[0] = sum(w L) / sum(w) (device memory; summed in a fixed order
  * in double; NaN when no row takes part). `state` of

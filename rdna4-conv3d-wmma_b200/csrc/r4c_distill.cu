@@ -27,14 +27,17 @@ __device__ __forceinline__ uint4 mask_vec(uint4 w, uint32_t bits) {
 // the K pairs. The exponential unit bounds it for 16-bit logits (0.65 of it
 // busy): 4096 rows of 131072 bf16 classes with 64 pairs 215 us, 0.76 of a
 // copy's rate, 203 us without a rest and one pair; fp32 0.89.
+// ROUNDED: a rest with 16-bit log-probabilities. Their noise takes registers
+// that the others cannot spare (220 -> 234 us for the 64 pairs above).
 constexpr int kBatch = 4, kStages = 2;
-template <typename T, int NT>
+template <typename T, int NT, bool ROUNDED>
 __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
   constexpr int VE = Vec<T>::kElems, U = kBatch;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ RunShared<NT> runs;
   __shared__ Run mine, joined;
   __shared__ float2 pair_sums[4];
+  __shared__ float pair_noises[4];
   __shared__ int idx[R4C_TOPK_MAX];
   uint8_t* marks = dyn + VecRing<NT, U, kStages>::kBytes;
   const int tid = threadIdx.x;
@@ -167,6 +170,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
       }
       __syncthreads();
       // (the sums of K <= 128 numbers: the first four warps hold them)
+      if (ROUNDED) {
+        const float noise = group_sum<32>(pair_noise(q, v, a.t_round));
+        if ((tid & 31) == 0 && tid < 128) pair_noises[tid >> 5] = noise;
+      }
       q = group_sum<32>(q);
       loss = group_sum<32>(loss);
       if ((tid & 31) == 0 && tid < 128) pair_sums[tid >> 5] = make_float2(q, loss);
@@ -178,7 +185,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
           sum_q += pair_sums[i].x;
           loss += pair_sums[i].y;
         }
-        const float qr = a.rest ? rest_mass(sum_q) : 0.f;
+        float noise = 0.f;
+        if (ROUNDED && s.sr == 0.f)
+          for (int i = 0; i < 4 && i < NT / 32; ++i) noise += pair_noises[i];
+        const float qr = a.rest ? rest_mass(sum_q, noise) : 0.f;
         if (s.empty) w = 0.f;
         loss = w == 0.f ? 0.f : w * a.temp * a.temp * (loss + rest_loss(qr, s, a.inv_t));
         if (a.row_loss) a.row_loss[r] = loss;
@@ -271,16 +281,20 @@ size_t mark_bytes(int C, int cs) {
 }
 constexpr size_t kMostMarks = 128 << 10;
 
-template <typename T, int NT>
-cudaError_t launch_fwd_block(const Args& a, int* blocks, cudaStream_t s) {
+template <typename T, int NT, bool ROUNDED>
+cudaError_t launch_fwd_rows(const Args& a, int* blocks, cudaStream_t s) {
   int cs = cluster_size(a.nrows, a.C, sizeof(T), NT);
   while (a.rest && cs < 8 && mark_bytes<T>(a.C, cs) > kMostMarks) cs *= 2;
   const size_t smem = VecRing<NT, kBatch, kStages>::kBytes + (a.rest ? mark_bytes<T>(a.C, cs) : 0);
-  const int64_t most = (int64_t)kSMs * blocks_per_sm(fwd_block_kernel<T, NT>, NT, smem) / cs * cs;
+  const int64_t most = (int64_t)kSMs * blocks_per_sm(fwd_block_kernel<T, NT, ROUNDED>, NT, smem) / cs * cs;
   int64_t grid = a.nrows * cs;
   if (grid > most) grid = most;   // (0: launch_cluster gives the error)
   *blocks = (int)grid;
-  return launch_cluster(fwd_block_kernel<T, NT>, grid, NT, cs, smem, s, a);
+  return launch_cluster(fwd_block_kernel<T, NT, ROUNDED>, grid, NT, cs, smem, s, a);
+}
+template <typename T, int NT>
+cudaError_t launch_fwd_block(const Args& a, int* blocks, cudaStream_t s) {
+  return a.rest && a.t_round > 0.f ? launch_fwd_rows<T, NT, true>(a, blocks, s) : launch_fwd_rows<T, NT, false>(a, blocks, s);
 }
 
 template <typename T>
@@ -338,6 +352,7 @@ distill::Args make_args(const r4c_rows_desc* d, const void* logits, int k, const
   a.t_index = t_index;
   a.t_dtype = t_dtype;
   a.t_wide = index_bits == 64;
+  a.t_round = t_dtype == R4C_BF16 ? 0x1p-8f : t_dtype == R4C_F16 ? 0x1p-11f : 0.f;
   a.weight = weight;
   a.stats = reinterpret_cast<distill::Stats*>(static_cast<char*>(state) + kStatsAt);
   return a;

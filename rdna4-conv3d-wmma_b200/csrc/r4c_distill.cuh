@@ -42,6 +42,7 @@ struct Args {
   const void* t_logp;
   const void* t_index;
   int t_dtype, t_wide;
+  float t_round;         // the largest relative rounding of 16-bit log-probabilities, 0 for fp32
   const float* weight;
   float* row_loss;       // forward: w L per row, or null
   double* part;          // forward: (sum w L, sum w) of each block, or null
@@ -126,10 +127,18 @@ struct RowSums {
     empty = s == 0.f;
   }
 };
-// q_r from the sum of the listed q.
-__device__ __forceinline__ float rest_mass(float sum_q) {
+// What rounding v = ln q to 16 bits takes from q at most: q (e^x - 1), x = round |v|.
+__device__ __forceinline__ float pair_noise(float q, float v, float round) {
+  const float x = round * fabsf(v);
+  return q > 0.f ? q * fmaf(x, x, x) : 0.f;
+}
+// q_r from the sum of the listed q. `noise` is what the stored pairs' rounding
+// explains, given only where the student has no unlisted class: mass on none
+// is infinitely far off, and there it would be so for a teacher that lists
+// all there is. With unlisted classes 1 - sum q is the best that is known.
+__device__ __forceinline__ float rest_mass(float sum_q, float noise) {
   const float qr = 1.f - sum_q;
-  return qr >= kRestNoise ? qr : 0.f;
+  return qr >= kRestNoise + noise ? qr : 0.f;
 }
 // q_r (ln q_r - ln p_r)
 __device__ __forceinline__ float rest_loss(float qr, const RowSums& s, float inv_t) {

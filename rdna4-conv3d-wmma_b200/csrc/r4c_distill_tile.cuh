@@ -163,7 +163,14 @@ __global__ void __launch_bounds__(kTileThreads, tile_blocks(G, E, kSlots, BWD)) 
     }
     sum_q = group_sum<G>(sum_q);
     // (exact divisions where p - q may cancel)
-    const float qi = rest ? 1.f : 1.f / sum_q, qr = rest ? rest_mass(sum_q) : 0.f;
+    float noise = 0.f;
+    if (!PLAIN && rest && a.t_round > 0.f) {
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) noise += pair_noise(pq[i], pv[i], a.t_round);
+      noise = group_sum<G>(noise);
+      if (s.sr != 0.f) noise = 0.f;
+    }
+    const float qi = rest ? 1.f : 1.f / sum_q, qr = rest ? rest_mass(sum_q, noise) : 0.f;
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) pq[i] *= qi;
 

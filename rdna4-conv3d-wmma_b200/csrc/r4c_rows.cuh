@@ -30,7 +30,8 @@ namespace rows {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// A rest mass 1 - sum(q) below this is the rounding of the teacher's own sum.
+// A rest mass 1 - sum(q) below this is the rounding of the teacher's own sum
+// (of fp32 log-probabilities; r4c_distill.cuh has that of 16-bit ones).
 constexpr float kRestNoise = 1e-6f;
 constexpr int kTileClasses = 1024;
 constexpr int kTileThreads = 256;

@@ -90,7 +90,9 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
         is listed twice counts with both its probabilities.
     rest: False -- the k probabilities are renormalised (so the teacher's
         logits / temperature serve as well); True -- they are taken as they
-        are, and what is missing to 1 stands for all other classes together.
+        are, and what is missing to 1 stands for all other classes together
+        (less than 1e-6 is rounding and counts as nothing; so does, where the
+        student has no other class, what rounding to bf16 or fp16 explains).
     weight: (N, ...), >= 0: the weight of each voxel or token (0: masked).
     reduction: 'mean' -- sum(w L) / sum(w), NaN when no row takes part; 'none' -- w L, (N, ...).
 
@@ -165,10 +167,15 @@ def _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weigh
     row = torch.where(some, q * (torch.where(some, v, zero) - torch.where(some, ln_p, zero)), zero).sum(-1)
     if rest:
         qr = 1.0 - q.sum(-1)
-        qr = torch.where(qr >= 1e-6, qr, zero)
         seen = torch.zeros(z.shape, dtype=torch.int64, device=z.device).scatter_add(-1, i, valid.long()) > 0
         alive = ~seen & (z != -inf)
         any_alive = alive.any(-1)
+        # what the sum's rounding explains is no rest, nor is what that of 16-bit pairs explains against no class
+        noise = torch.zeros_like(qr)
+        if teacher_logp.dtype in (torch.bfloat16, torch.float16):
+            x = (torch.where(q > 0, v, zero) * (0.5 * torch.finfo(teacher_logp.dtype).eps)).abs()
+            noise = torch.where(any_alive, noise, (q * (x + x * x)).sum(-1))
+        qr = torch.where(qr >= 1e-6 + noise, qr, zero)
         # the unlisted classes from a maximum of their own, which may lie far below the row's
         mr = torch.where(alive, z.detach(), zero - inf).amax(-1, keepdim=True)
         mr = torch.where(any_alive.unsqueeze(-1), mr, m)

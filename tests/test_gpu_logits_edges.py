@@ -8,8 +8,9 @@ from contextlib import nullcontext
 import pytest
 import torch
 
-from logit_refs import NEG, assert_grad, log_probs_ref, rows_of
-from test_gpu_logits import BF, DTYPES, _gen, _logits, _teacher
+from logit_edge_refs import no_rest_ref, stored, student
+from logit_refs import NEG, assert_grad, assert_values, log_probs_ref, rows_of
+from test_gpu_logits import BF, DTYPES, FP, HF, _check_distill, _gen, _logits, _teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +103,38 @@ def test_empty_maps(cuda_ready, shape):
         assert none.shape == rows and torch.autograd.grad(none.sum(), z)[0].shape == z.shape
         mean = distill_topk(z, v, idx, rest=rest)
         assert torch.isnan(mean) and torch.autograd.grad(mean, z)[0].shape == z.shape
+
+
+TEACHERS = pytest.mark.parametrize("stored_as", [BF, HF, FP], ids=["bf16", "fp16", "fp32"])
+
+
+@TEACHERS
+@pytest.mark.parametrize("wide", [False, True], ids=["int32", "int64"])
+@pytest.mark.parametrize("c,k", [(2, 2), (4, 4), (5, 5), (20, 20), (128, 128), (40, 7), (300, 128), (1030, 20), (9001, 128)])
+def test_a_stored_teacher_that_lists_all_there_is(cuda_ready, c, k, wide, stored_as):
+    """As on the CPU: no class is left, so the stored values' rounding is no mass of a rest."""
+    from rdna4_conv3d.losses import distill_topk
+    v, idx = stored(c, k, 40, stored_as)
+    z = student(c, k, idx).cuda().requires_grad_(True)
+    loss = distill_topk(z, v.cuda(), (idx if wide else idx.int()).cuda(), temperature=2.0, rest=True, reduction="none")
+    want, dwant = no_rest_ref(z.detach().cpu().double(), v.double(), idx, 2.0)
+    assert_values(loss, want, "loss", 1.2e-4, 5e-6)
+    dz, = torch.autograd.grad(loss.sum(), z)
+    assert_grad(dz, dwant, FP)
+
+
+@TEACHERS
+@pytest.mark.parametrize("wide", [False, True], ids=["int32", "int64"])
+@pytest.mark.parametrize("c", [12, 200, 3000])
+def test_a_stored_teacher_that_does_not(cuda_ready, c, wide, stored_as):
+    from rdna4_conv3d.losses import distill_topk
+    v, idx = stored(c, 6, 50, stored_as)
+    v = (v.double() + torch.log(torch.tensor(0.8).double())).to(stored_as)
+    ti = (idx if wide else idx.int()).cuda()
+    _check_distill(_logits((50, c), FP), v.float().cuda(), ti, 1.0, True, None, "none")
+    z = _logits((50, c), FP).requires_grad_(True)
+    loss = distill_topk(z, v.cuda(), ti, rest=True, reduction="none")
+    same = distill_topk(z, v.float().cuda(), ti, rest=True, reduction="none")
+    assert_values(loss, same.detach().cpu().double(), "loss", 3e-5, 5e-6)
+    out = distill_topk(student(c, 6, idx).cuda(), v.cuda(), ti, rest=True, reduction="none")
+    assert bool(torch.isinf(out).all())

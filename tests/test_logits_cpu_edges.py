@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from logit_edge_refs import no_rest_ref, stored, student
 from logit_refs import NEG, assert_grad, assert_values, distill_ref, log_probs_ref, rows_of
 from rdna4_conv3d import _native
 from rdna4_conv3d.losses import distill_topk
@@ -97,3 +98,31 @@ def test_distill_gradient_where_the_student_agrees(gap, rest):
     dz, = torch.autograd.grad(loss.sum(), z)
     _, _, want = distill_ref(rows_of(z), v.double(), idx, 1.0, rest)
     assert_grad(dz, want, torch.float32)
+
+
+TEACHERS = pytest.mark.parametrize("stored_as", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "fp16", "fp32"])
+
+
+@TEACHERS
+@pytest.mark.parametrize("c,k", [(2, 2), (5, 5), (20, 20), (128, 128), (40, 7)])
+def test_a_stored_teacher_that_lists_all_there_is(c, k, stored_as):
+    """What its rounding leaves of 1 is not mass on classes that the student does not have; fp32 arithmetic,
+    the kernels' bounds."""
+    v, idx = stored(c, k, 400, stored_as)
+    z = student(c, k, idx).requires_grad_(True)
+    loss = distill_topk(z, v, idx, temperature=2.0, rest=True, reduction="none")
+    want, dwant = no_rest_ref(z.detach().double(), v.double(), idx, 2.0)
+    assert_values(loss, want, "loss", 1.2e-4, 5e-6)
+    dz, = torch.autograd.grad(loss.sum(), z)
+    assert_grad(dz, dwant, torch.float32)
+
+
+@TEACHERS
+def test_a_stored_teacher_that_does_not(stored_as):
+    """Missing mass beyond the rounding still counts: against live classes as it is, against none as infinite."""
+    v, idx = stored(12, 6, 50, stored_as)
+    v = (v.double() + torch.log(torch.tensor(0.8).double())).to(stored_as)
+    z = 3 * torch.randn((50, 12), generator=_gen(2))
+    loss = distill_topk(z, v, idx, rest=True, reduction="none")
+    assert_values(loss, distill_ref(z.double(), v.double(), idx, 1.0, True)[0], "loss", 3e-5, 5e-6)
+    assert torch.isinf(distill_topk(student(12, 6, idx), v, idx, rest=True, reduction="none")).all()
