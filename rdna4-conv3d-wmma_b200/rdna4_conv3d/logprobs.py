@@ -17,6 +17,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _native
 
@@ -48,6 +49,12 @@ def refuse_twice() -> None:
     """In a backward: the native gradients have no graph of their own."""
     if torch.is_grad_enabled():
         raise RuntimeError("the native gradient of this operator cannot be differentiated again (create_graph)")
+
+
+def refuse_forward_mode(logits: torch.Tensor) -> None:
+    """Before a launch: the kernels would drop a tangent."""
+    if unpack_dual(logits).tangent is not None:
+        raise RuntimeError("this operator has no forward-mode derivative on a CUDA device")
 
 
 class LogProbsFn(torch.autograd.Function):
@@ -86,10 +93,11 @@ def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, *, to
         ``_native.device_error()``).
     top_k: how many of the most probable classes to return, at most 128.
 
-    ``logp``, ``entropy`` and ``lse`` carry gradients to the logits;
-    ``top_logp`` does not. A row without a finite logit has lse, logp and
-    top_logp -inf, entropy 0 and no gradient; one that holds a NaN or +inf has
-    no distribution: its values are NaN and its top_index -1.
+    ``logp``, ``entropy`` and ``lse`` carry gradients to the logits (reverse
+    mode, once; on the CPU as torch has them); ``top_logp`` does not. A row
+    without a finite logit has lse, logp and top_logp -inf, entropy 0 and no
+    gradient; one that holds a NaN or +inf has no distribution: its values are
+    NaN and its top_index -1.
     """
     check_logits(logits, temperature)
     zs = logits.shape
@@ -105,6 +113,7 @@ def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, *, to
             raise ValueError(f"target is on {target.device}, logits on {logits.device}")
     if not logits.is_cuda:
         return _log_probs_torch(logits, target, top_k, temperature, ignore_index)
+    refuse_forward_mode(logits)
     if target is not None:
         if target.dtype != torch.int64:
             target = target.to(torch.int64)

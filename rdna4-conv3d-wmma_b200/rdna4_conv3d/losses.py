@@ -22,7 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _native
-from .logprobs import check_logits, refuse_twice
+from .logprobs import check_logits, refuse_forward_mode, refuse_twice
 
 
 class CrossEntropyNDHWCFn(torch.autograd.Function):
@@ -98,8 +98,9 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
 
     Rows whose places are all unused, whose weight is 0 or whose logits are
     all -inf take no part: loss 0, no share of the mean, no gradient. The
-    gradient reaches the logits only. An index beyond the classes is an error
-    (on a CUDA device it is unused and sets code 6 in ``_native.device_error()``).
+    gradient reaches the logits only (reverse mode, once; on the CPU as torch
+    has it). An index beyond the classes is an error (on a CUDA device it is
+    unused and sets code 6 in ``_native.device_error()``).
     """
     check_logits(logits, temperature)
     mean = reduction == "mean"
@@ -124,6 +125,7 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
             raise ValueError(f"weight is on {weight.device}, logits on {dev}")
     if not logits.is_cuda:
         return _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weight, reduction)
+    refuse_forward_mode(logits)
     if teacher_logp.requires_grad:
         teacher_logp = teacher_logp.detach()
     if teacher_logp.dtype == torch.float64:

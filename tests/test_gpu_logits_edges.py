@@ -138,3 +138,23 @@ def test_a_stored_teacher_that_does_not(cuda_ready, c, wide, stored_as):
     assert_values(loss, same.detach().cpu().double(), "loss", 3e-5, 5e-6)
     out = distill_topk(student(c, 6, idx).cuda(), v.cuda(), ti, rest=True, reduction="none")
     assert bool(torch.isinf(out).all())
+
+
+@pytest.mark.parametrize("c", [5, 2000])
+def test_forward_mode_is_refused(cuda_ready, c):
+    import torch.autograd.forward_ad as fwAD
+    from rdna4_conv3d.logprobs import log_probs
+    from rdna4_conv3d.losses import distill_topk
+    z = _logits((3, c), FP)
+    v, idx = _teacher(3, c, 2)
+    for call in (lambda x: log_probs(x).entropy, lambda x: distill_topk(x, v, idx)):
+        with fwAD.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(fwAD.make_dual(z, torch.ones_like(z)))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(call, (z,), (torch.ones_like(z),))
+        # nor does any other transform see through the kernels: none goes by in silence
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(z[None])
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda x: call(x).sum())(z)

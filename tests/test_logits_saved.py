@@ -1,6 +1,6 @@
-"""What the backwards of log_probs and distill_topk make of saved tensors that come back changed.
+"""What autograd may ask of log_probs and distill_topk beyond a plain backward.
 
-Hooks on saved tensors (``torch.autograd.graph``: offloading, packing) give
+Forward-mode derivatives, which the kernels do not have, are refused. Hooks on saved tensors (``torch.autograd.graph``: offloading, packing) give
 the same values back, but with any strides. The kernels read through addresses
 and a descriptor, so here, on the CPU and in place of the launch, the
 descriptor is walked over the tensors that the launch would get: every place
@@ -8,11 +8,12 @@ must lie inside them and hold the row's own value.
 """
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd.graph import saved_tensors_hooks
 
 from rdna4_conv3d import _native
-from rdna4_conv3d.logprobs import LogProbsFn
-from rdna4_conv3d.losses import DistillTopKFn
+from rdna4_conv3d.logprobs import LogProbsFn, log_probs
+from rdna4_conv3d.losses import DistillTopKFn, distill_topk
 
 
 def _walk(t, desc, outer, inner, cls):
@@ -137,3 +138,38 @@ def test_tensors_that_are_not_the_saved_ones_are_refused(launches, which, spoil)
         with pytest.raises(RuntimeError, match="saved"):
             torch.autograd.grad(y, z)
     assert not launches
+
+
+class _OnDevice(torch.Tensor):
+    """A CPU tensor that calls itself one of a CUDA device: the native path up to its launches."""
+    is_cuda = True
+
+
+@pytest.mark.parametrize("wants_grad", [False, True])
+@pytest.mark.parametrize("c", [5, 1030])
+def test_forward_mode_is_refused(launches, c, wants_grad):
+    """The kernels carry no tangent; outputs without one would read as a derivative of zero."""
+    z = torch.randn(3, c).as_subclass(_OnDevice)
+    v, i = torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int32)
+    calls = (lambda x: log_probs(x).entropy, lambda x: distill_topk(x, v, i))
+    with fwAD.dual_level():
+        x = fwAD.make_dual(z.requires_grad_(wants_grad), torch.ones(3, c))
+        assert x.is_cuda and x.requires_grad == wants_grad
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(x)
+            call(z.detach())                             # within a level, without a tangent
+    for call in calls:
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(call, (z.detach(),), (torch.ones(3, c),))
+
+
+def test_forward_mode_on_the_cpu():
+    """The torch path has tangents: they agree with the gradient."""
+    z, u = torch.randn(3, 7, dtype=torch.float64), torch.randn(3, 7, dtype=torch.float64)
+    v, i = torch.log(torch.full((3, 2), 0.3)), torch.tensor([[0, 1]] * 3)
+    for call in (lambda x: log_probs(x).entropy.sum(), lambda x: distill_topk(x, v, i, rest=True)):
+        tangent = torch.func.jvp(call, (z,), (u,))[1]
+        x = z.clone().requires_grad_(True)
+        dz, = torch.autograd.grad(call(x), x)
+        assert abs(float(tangent) - float((dz * u).sum())) < 1e-12
