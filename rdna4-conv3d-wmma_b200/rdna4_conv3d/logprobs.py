@@ -123,6 +123,35 @@ def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, *, to
     return LogProbs(*_native.logp_forward(_native.Rows(logits, temperature), target, ignore_index, top_k, False)[:5])
 
 
+class _BadRowsFn(torch.autograd.Function):
+    """Values of rows that may be bad (a NaN or +inf logit), as they are; a bad row's logits get a gradient of NaN
+    where any of its values has one that is not 0."""
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(z, bad, *values):
+        return tuple(v.clone() for v in values)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(inputs[0], inputs[1])
+        ctx.save_for_forward(inputs[1])
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        z, bad = ctx.saved_tensors
+        hit = torch.zeros_like(bad)
+        for g in grads:
+            if g is not None:
+                hit = hit | (g != 0).unsqueeze(-1)
+        return torch.where(hit & bad, float("nan"), torch.zeros_like(z)), None, *grads
+
+    @staticmethod
+    def jvp(ctx, _z, _bad, *tangents):
+        return tangents
+
+
 def _log_probs_torch(logits, target, top_k, temperature, ignore_index) -> LogProbs:
     """The same values in torch operations, at least in fp32."""
     acc = torch.promote_types(logits.dtype, torch.float32)
@@ -150,13 +179,16 @@ def _log_probs_torch(logits, target, top_k, temperature, ignore_index) -> LogPro
     b = bad.squeeze(-1)
     entropy, lse = torch.where(b, nan, entropy), torch.where(b, nan, lse)
     logp = None
-    if target is not None:
+    if target is None:
+        entropy, lse = _BadRowsFn.apply(z, bad, entropy, lse)
+    else:
         t = target.to(torch.int64)
         counted = t != ignore_index
         if bool((((t < 0) | (t >= c)) & counted).any()):
             raise IndexError(f"target out of range [0, {c})")
         at = torch.where(counted, t, torch.zeros_like(t)).unsqueeze(-1)
         logp = torch.where(b, nan, ln_p.gather(-1, at).squeeze(-1))
+        logp, entropy, lse = _BadRowsFn.apply(z, bad, logp, entropy, lse)
         logp = torch.where(counted, logp, torch.zeros_like(logp)).to(out)
     top_logp = top_index = None
     if top_k:

@@ -126,3 +126,36 @@ def test_a_stored_teacher_that_does_not(stored_as):
     loss = distill_topk(z, v, idx, rest=True, reduction="none")
     assert_values(loss, distill_ref(z.double(), v.double(), idx, 1.0, True)[0], "loss", 3e-5, 5e-6)
     assert torch.isinf(distill_topk(student(12, 6, idx), v, idx, rest=True, reduction="none")).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64], ids=["fp32", "fp64"])
+def test_gradients_of_bad_rows(dtype):
+    """NaN for a row of NaN or +inf logits that has an upstream gradient, as on a CUDA device; 0 for one that has none."""
+    z = 3 * torch.randn((9, 6), generator=_gen(4), dtype=torch.float64)
+    z[1, 2] = z[4, 0] = z[6, 5] = float("nan")
+    z[2, 5] = z[7, 1] = float("inf")
+    z[3] = float("nan")
+    z[5] = NEG
+    z = z.to(dtype).requires_grad_(True)
+    t = torch.arange(9) % 6
+    t[1:4] = -100
+    ones = torch.ones(9, dtype=torch.float64)
+    some = ones.clone()
+    some[[4, 7]] = 0.0
+    for gl, gh, gs in ((ones, None, None), (None, some, None), (None, None, some), (some, some, None), (ones, ones, ones),
+                       (some, 0 * ones, some)):
+        out = log_probs(z, t)
+        ups = [(o, g) for o, g in zip(out[:3], (gl, gh, gs)) if g is not None]
+        dz, = torch.autograd.grad([o for o, _ in ups], z, [g.to(o.dtype) for o, g in ups])
+        assert_grad(dz, log_probs_ref(rows_of(z), t, 0, 1.0, -100, gl, gh, gs)["dz"], torch.float32)
+
+
+def test_log_probs_in_transforms():
+    """On the CPU the operator stays a composition that torch can transform."""
+    z, u = torch.randn(2, 3, 7, dtype=torch.float64), torch.randn(2, 3, 7, dtype=torch.float64)
+    f = lambda x: (lambda o: o.entropy.sum() + o.lse.sum())(log_probs(x))  # noqa: E731
+    each = torch.stack([f(x) for x in z])
+    assert torch.allclose(torch.func.vmap(f)(z), each)
+    dz = torch.func.vmap(torch.func.grad(f))(z)
+    assert torch.allclose(torch.func.jvp(torch.func.vmap(f), (z,), (u,))[1], (dz * u).sum((1, 2)))
+    assert torch.autograd.gradgradcheck(f, (z[0].clone().requires_grad_(True),))
