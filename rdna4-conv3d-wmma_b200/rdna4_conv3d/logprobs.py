@@ -57,6 +57,18 @@ def refuse_forward_mode(logits: torch.Tensor) -> None:
         raise RuntimeError("this operator has no forward-mode derivative on a CUDA device")
 
 
+def through_autograd(logits: torch.Tensor) -> bool:
+    """Whether a call goes through its autograd Function: where a gradient may follow, and under torch.jit.trace,
+    which records a Function, but of bare launches only the empty tensors that they fill."""
+    return torch.is_grad_enabled() and logits.requires_grad or torch._C._is_tracing()
+
+
+def refuse_proxies() -> None:
+    """Before a launch: make_fx would keep this call's outputs as constants of its graph."""
+    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("this operator cannot be traced into a graph of proxies (make_fx) on a CUDA device")
+
+
 class LogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target, top_k, temperature, ignore_index):
@@ -114,11 +126,12 @@ def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, *, to
     if not logits.is_cuda:
         return _log_probs_torch(logits, target, top_k, temperature, ignore_index)
     refuse_forward_mode(logits)
+    refuse_proxies()
     if target is not None:
         if target.dtype != torch.int64:
             target = target.to(torch.int64)
         target = target.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if through_autograd(logits):
         return LogProbs(*LogProbsFn.apply(logits, target, top_k, temperature, ignore_index))
     return LogProbs(*_native.logp_forward(_native.Rows(logits, temperature), target, ignore_index, top_k, False)[:5])
 

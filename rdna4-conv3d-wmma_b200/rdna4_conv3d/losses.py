@@ -22,7 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _native
-from .logprobs import check_logits, refuse_forward_mode, refuse_twice
+from .logprobs import check_logits, refuse_forward_mode, refuse_proxies, refuse_twice, through_autograd
 
 
 class CrossEntropyNDHWCFn(torch.autograd.Function):
@@ -126,6 +126,7 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
     if not logits.is_cuda:
         return _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weight, reduction)
     refuse_forward_mode(logits)
+    refuse_proxies()
     if teacher_logp.requires_grad:
         teacher_logp = teacher_logp.detach()
     if teacher_logp.dtype == torch.float64:
@@ -133,7 +134,7 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
     if weight is not None:
         weight = weight.detach().to(torch.float32).contiguous()
     teacher_logp, teacher_index, rest = teacher_logp.contiguous(), teacher_index.contiguous(), bool(rest)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if through_autograd(logits):
         return DistillTopKFn.apply(logits, teacher_logp, teacher_index, temperature, rest, weight, mean)
     rows = _native.Rows(logits, temperature)
     return _native.distill_forward(rows, teacher_logp, teacher_index, rest, weight, mean)[0]

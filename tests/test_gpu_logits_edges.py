@@ -158,3 +158,22 @@ def test_forward_mode_is_refused(cuda_ready, c):
             torch.func.vmap(call)(z[None])
         with pytest.raises(RuntimeError):
             torch.func.grad(lambda x: call(x).sum())(z)
+
+
+@pytest.mark.parametrize("wants_grad", [False, True])
+@pytest.mark.parametrize("c", [6, 2000])
+def test_traces_run_the_operators_again(cuda_ready, c, wants_grad):
+    """A trace computes from the inputs that it is given, or there is none."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from rdna4_conv3d.logprobs import log_probs
+    from rdna4_conv3d.losses import distill_topk
+    z, more = _logits((4, c), BF).requires_grad_(wants_grad), _logits((4, c), BF, seed=8).requires_grad_(wants_grad)
+    v, idx = _teacher(4, c, 2)
+    for f in (lambda x: log_probs(x, top_k=2).entropy * 2, lambda x: log_probs(x, top_k=2).top_logp * 2,
+              lambda x: distill_topk(x, v, idx) * 2):
+        want = f(more)
+        assert torch.equal(torch.jit.trace(f, (z,), check_trace=False)(more), want)
+        torch._dynamo.reset()
+        assert torch.equal(torch.compile(f, backend="eager")(more), want)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(f)(z)
