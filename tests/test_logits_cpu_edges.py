@@ -159,3 +159,19 @@ def test_log_probs_in_transforms():
     dz = torch.func.vmap(torch.func.grad(f))(z)
     assert torch.allclose(torch.func.jvp(torch.func.vmap(f), (z,), (u,))[1], (dz * u).sum((1, 2)))
     assert torch.autograd.gradgradcheck(f, (z[0].clone().requires_grad_(True),))
+
+
+def test_a_rest_over_too_many_classes_is_refused():
+    """The marks of the listed classes of one row fill the shared memory of a cluster at about four million classes."""
+    L = _native.lib()
+    one = torch.zeros(16)
+    at, state = one.data_ptr(), torch.zeros(1 << 17, dtype=torch.uint8)
+    sp = (state.data_ptr() + 15) // 16 * 16
+
+    def call(c, rest):
+        d = _native.RowsDesc(0, 1, 0, c, 1, 0, c, 1, c, _native.R4C_BF16, 1.0)
+        return L.r4c_distill_fwd(d, at, 2, at, _native.R4C_F32, at, 32, rest, None, at, None, sp, 1 << 16, None)
+
+    too_large = -7
+    assert [call(c, 1) for c in (1 << 20, 4000000, 5000000)] == [0, 0, too_large] and call(5000000, 0) == 0
+    assert "four million" in distill_topk.__doc__
