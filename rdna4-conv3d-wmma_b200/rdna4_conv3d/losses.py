@@ -22,6 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _native
+from .conv3d_wmma import _as_ndhwc
 from .logprobs import check_logits, refuse_forward_mode, refuse_proxies, refuse_twice, through_autograd
 
 
@@ -38,6 +39,8 @@ class CrossEntropyNDHWCFn(torch.autograd.Function):
         logits, target, loss_count = ctx.saved_tensors
         dz = None
         if ctx.needs_input_grad[0]:
+            # (hooks on saved tensors may give them back in other strides)
+            logits, target, loss_count = _as_ndhwc(logits), target.contiguous(), loss_count.contiguous()
             dz = _native.ce_backward(logits, target, ctx.ignore_index, loss_count, grad)
         return dz, None, None
 
