@@ -22,8 +22,16 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _native
+from .conv3d_wmma import _as_ndhwc
 
 _HALF = (torch.float16, torch.bfloat16)
+
+
+def _as_read(x, *more):
+    """Saved tensors in the layouts that the kernels read: hooks may give them back in other strides, or off the
+    16 bytes that a vector load needs."""
+    more = (t.contiguous() for t in more)
+    return (_as_ndhwc(x), *(t.clone() if t.data_ptr() & 15 else t for t in more))
 
 
 class BNReLUFn(torch.autograd.Function):
@@ -41,7 +49,7 @@ class BNReLUFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy):
-        x, mi, ss = ctx.saved_tensors
+        x, mi, ss = _as_read(*ctx.saved_tensors)
         gy = gy.contiguous(memory_format=torch.channels_last_3d)
         if gy.dtype != x.dtype:
             gy = gy.to(x.dtype)
@@ -70,7 +78,7 @@ class BNReLUPoolFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gbuf, gp):
-        x, mi, af, am = ctx.saved_tensors
+        x, mi, af, am = _as_read(*ctx.saved_tensors)
         cl = torch.channels_last_3d
         if gbuf is None:
             gbuf = torch.zeros((x.shape[0], ctx.lead + x.shape[1]) + tuple(x.shape[2:]), dtype=x.dtype,

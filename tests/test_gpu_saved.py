@@ -54,3 +54,39 @@ def test_cross_entropy(cuda_ready, dtype, hook):
     assert _native.launch_count() > n0
     got, = _grads(lambda: cross_entropy(z, t), (z,), HOOKS[hook])
     assert torch.equal(got, want)
+
+
+@hooks
+@pytest.mark.parametrize("pool", [False, True])
+def test_bn_relu(cuda_ready, pool, hook):
+    from rdna4_conv3d import _native
+    from rdna4_conv3d.bn_relu import BNReLUFn, BNReLUPoolFn
+    x = torch.randn(2, 24, 6, 8, 10, device="cuda", generator=_gen(1)).bfloat16().contiguous(memory_format=CL).requires_grad_(True)
+    w = (1 + 0.1 * torch.randn(24, device="cuda", generator=_gen(2))).requires_grad_(True)
+    b = (0.1 * torch.randn(24, device="cuda", generator=_gen(4))).requires_grad_(True)
+
+    def forward():
+        if pool:
+            buf, p = BNReLUPoolFn.apply(x, w, b, None, None, 0.1, 1e-5, 24)
+            return torch.cat([buf[:, 24:].reshape(-1), p.reshape(-1)])
+        return BNReLUFn.apply(x, w, b, None, None, 0.1, 1e-5, True, None)
+
+    n0 = _native.launch_count()
+    want = _grads(forward, (x, w, b), nullcontext)
+    assert _native.launch_count() > n0
+    for a, e in zip(_grads(forward, (x, w, b), HOOKS[hook]), want):
+        assert torch.equal(a, e)
+
+
+@hooks
+@pytest.mark.parametrize("transposed", [False, True])
+def test_convolutions(cuda_ready, transposed, hook):
+    """(These already read what they are given.)"""
+    from rdna4_conv3d.conv3d_wmma import Conv3dWmma, ConvTranspose3dWmma
+    x = torch.randn(1, 24, 6, 8, 10, device="cuda", generator=_gen(1)).bfloat16().contiguous(memory_format=CL).requires_grad_(True)
+    torch.manual_seed(0)
+    m = (ConvTranspose3dWmma(24, 16, 2, stride=2) if transposed else Conv3dWmma(24, 32, 3, padding=1)).cuda().bfloat16()
+    inputs = (x, *m.parameters())
+    want = _grads(lambda: m(x), inputs, nullcontext)
+    for a, e in zip(_grads(lambda: m(x), inputs, HOOKS[hook]), want):
+        assert torch.equal(a, e)
