@@ -671,41 +671,39 @@ class SavedRows:
     A saved tensor may come back as another one with the same values (hooks
     that offload or pack what autograd keeps): other strides get a descriptor
     of their own, another shape, type or device never reaches a kernel."""
-    __slots__ = ("desc", "shape", "_z")
+    __slots__ = ("desc", "shape", "stride", "dtype", "device")
 
     def __init__(self, rows: Rows):
         z = rows.z
-        self.desc, self.shape, self._z = rows.desc, rows.shape, (z.shape, z.stride(), z.dtype, z.device)
+        self.desc, self.shape, self.stride, self.dtype, self.device = rows.desc, z.shape, z.stride(), z.dtype, z.device
 
     def logits(self, z: torch.Tensor):
         """(logits as the kernels read them, their descriptor)."""
-        shape, stride, dtype, device = self._z
-        _as_saved(z, shape, dtype, device)
-        if z.stride() == stride:
+        if z.shape != self.shape or z.dtype is not self.dtype or z.device != self.device:
+            _not_as_saved(z, self.shape, self.dtype, self.device)
+        if z.stride() == self.stride:
             return z, self.desc
         rows = Rows(z, self.desc.temperature)
         return rows.z, rows.desc
 
-    def dense(self, t: Optional[torch.Tensor], dtype: torch.dtype, *more: int) -> Optional[torch.Tensor]:
-        """A per-row tensor (N, ..., *more) as the kernels read it."""
-        if t is None:
-            return None
-        _as_saved(t, (*self.shape, *more) if more else self.shape, dtype, self._z[3])
-        return t.contiguous()
+    def dense(self, t: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tensor:
+        """A per-row tensor of this shape as the kernels read it."""
+        if t.shape != shape or t.dtype is not dtype or t.device != self.device:
+            _not_as_saved(t, shape, dtype, self.device)
+        return t if t.is_contiguous() else t.contiguous()
 
-    def buffer(self, t: Optional[torch.Tensor], nbytes: int) -> Optional[torch.Tensor]:
+    def buffer(self, t: torch.Tensor, nbytes: int) -> torch.Tensor:
         """A forward's own bytes for its backward, 16-byte aligned."""
-        if t is None:
-            return None
-        _as_saved(t, (nbytes,), torch.uint8, self._z[3])
-        t = t.contiguous()
-        return t.clone() if t.data_ptr() & 15 else t
+        if t.numel() != nbytes or t.dtype is not torch.uint8 or t.device != self.device:
+            _not_as_saved(t, (nbytes,), torch.uint8, self.device)
+        if not t.is_contiguous() or t.data_ptr() & 15:
+            t = t.clone(memory_format=torch.contiguous_format)
+        return t
 
 
-def _as_saved(t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> None:
-    if t.dtype != dtype or t.shape != shape or t.device != device:
-        raise RuntimeError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, "
-                           f"saved was {dtype} {tuple(shape)} on {device}")
+def _not_as_saved(t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> None:
+    raise RuntimeError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, "
+                       f"saved was {dtype} {tuple(shape)} on {device}")
 
 
 def rows_grad(z: torch.Tensor, desc: RowsDesc) -> torch.Tensor:

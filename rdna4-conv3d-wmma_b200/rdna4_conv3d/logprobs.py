@@ -17,11 +17,12 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 from . import _native
 
 _FLOATS = frozenset((torch.bfloat16, torch.float16, torch.float32))
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
 
 
 class LogProbs(NamedTuple):
@@ -51,21 +52,12 @@ def refuse_twice() -> None:
         raise RuntimeError("the native gradient of this operator cannot be differentiated again (create_graph)")
 
 
-def refuse_forward_mode(logits: torch.Tensor) -> None:
-    """Before a launch: the kernels would drop a tangent."""
-    if unpack_dual(logits).tangent is not None:
+def refuse_blind(logits: torch.Tensor) -> None:
+    """Before a launch: what would go by it in silence. The kernels drop a forward-mode tangent, and make_fx keeps
+    the outputs of this call as constants of its graph."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(logits).tangent is not None:
         raise RuntimeError("this operator has no forward-mode derivative on a CUDA device")
-
-
-def through_autograd(logits: torch.Tensor) -> bool:
-    """Whether a call goes through its autograd Function: where a gradient may follow, and under torch.jit.trace,
-    which records a Function, but of bare launches only the empty tensors that they fill."""
-    return torch.is_grad_enabled() and logits.requires_grad or torch._C._is_tracing()
-
-
-def refuse_proxies() -> None:
-    """Before a launch: make_fx would keep this call's outputs as constants of its graph."""
-    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+    if torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(_PROXY) is not None:
         raise RuntimeError("this operator cannot be traced into a graph of proxies (make_fx) on a CUDA device")
 
 
@@ -76,8 +68,9 @@ class LogProbsFn(torch.autograd.Function):
         logp, entropy, lse, top_logp, top_index, stats = _native.logp_forward(rows, target, ignore_index, top_k, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(rows.z, target, entropy, stats)
-        ctx.rows, ctx.ignore_index = _native.SavedRows(rows), ignore_index
-        ctx.stats_bytes = 0 if stats is None else stats.numel()
+        ctx.rows, ctx.row_shape, ctx.ignore_index = _native.SavedRows(rows), rows.shape, ignore_index
+        if stats is not None:
+            ctx.stats_bytes = stats.numel()
         if top_k:
             ctx.mark_non_differentiable(top_logp, top_index)
         return logp, entropy, lse, top_logp, top_index
@@ -88,8 +81,11 @@ class LogProbsFn(torch.autograd.Function):
         z, target, entropy, stats = ctx.saved_tensors
         rows = ctx.rows
         z, desc = rows.logits(z)
-        target, entropy = rows.dense(target, torch.int64), rows.dense(entropy, torch.float32)
-        stats = rows.buffer(stats, ctx.stats_bytes)
+        if target is not None:
+            target = rows.dense(target, ctx.row_shape, torch.int64)
+        entropy = rows.dense(entropy, ctx.row_shape, torch.float32)
+        if stats is not None:
+            stats = rows.buffer(stats, ctx.stats_bytes)
         dz = _native.logp_backward(z, desc, target, ctx.ignore_index, entropy, stats, g_logp, g_entropy, g_lse)
         return dz, None, None, None, None
 
@@ -125,13 +121,13 @@ def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, *, to
             raise ValueError(f"target is on {target.device}, logits on {logits.device}")
     if not logits.is_cuda:
         return _log_probs_torch(logits, target, top_k, temperature, ignore_index)
-    refuse_forward_mode(logits)
-    refuse_proxies()
+    refuse_blind(logits)
     if target is not None:
         if target.dtype != torch.int64:
             target = target.to(torch.int64)
         target = target.contiguous()
-    if through_autograd(logits):
+    # (torch.jit.trace records a Function, but of bare launches only the empty tensors that they fill)
+    if torch.is_grad_enabled() and logits.requires_grad or torch._C._is_tracing():
         return LogProbs(*LogProbsFn.apply(logits, target, top_k, temperature, ignore_index))
     return LogProbs(*_native.logp_forward(_native.Rows(logits, temperature), target, ignore_index, top_k, False)[:5])
 

@@ -23,7 +23,7 @@ import torch.nn.functional as F
 
 from . import _native
 from .conv3d_wmma import _as_ndhwc
-from .logprobs import check_logits, refuse_forward_mode, refuse_proxies, refuse_twice, through_autograd
+from .logprobs import check_logits, refuse_blind, refuse_twice
 
 
 class CrossEntropyNDHWCFn(torch.autograd.Function):
@@ -66,17 +66,20 @@ class DistillTopKFn(torch.autograd.Function):
         loss, state = _native.distill_forward(rows, teacher_logp, teacher_index, rest, weight, mean)
         ctx.save_for_backward(rows.z, teacher_logp, teacher_index, weight, state)
         ctx.rows, ctx.rest, ctx.mean = _native.SavedRows(rows), rest, mean
-        ctx.teacher = teacher_logp.dtype, teacher_index.dtype, teacher_logp.shape[-1], state.numel()
+        ctx.teacher = teacher_logp.shape, teacher_logp.dtype, teacher_index.dtype, state.numel()
         return loss
 
     @staticmethod
     def backward(ctx, grad):
         refuse_twice()
         z, teacher_logp, teacher_index, weight, state = ctx.saved_tensors
-        rows, (logp_dtype, index_dtype, k, nbytes) = ctx.rows, ctx.teacher
+        rows, (shape, logp_dtype, index_dtype, nbytes) = ctx.rows, ctx.teacher
         z, desc = rows.logits(z)
-        teacher_logp, teacher_index = rows.dense(teacher_logp, logp_dtype, k), rows.dense(teacher_index, index_dtype, k)
-        weight, state = rows.dense(weight, torch.float32), rows.buffer(state, nbytes)
+        teacher_logp = rows.dense(teacher_logp, shape, logp_dtype)
+        teacher_index = rows.dense(teacher_index, shape, index_dtype)
+        if weight is not None:
+            weight = rows.dense(weight, shape[:-1], torch.float32)
+        state = rows.buffer(state, nbytes)
         dz = _native.distill_backward(z, desc, teacher_logp, teacher_index, ctx.rest, weight, ctx.mean, state, grad)
         return dz, None, None, None, None, None, None
 
@@ -129,8 +132,7 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
             raise ValueError(f"weight is on {weight.device}, logits on {dev}")
     if not logits.is_cuda:
         return _distill_torch(logits, teacher_logp, teacher_index, temperature, rest, weight, reduction)
-    refuse_forward_mode(logits)
-    refuse_proxies()
+    refuse_blind(logits)
     if teacher_logp.requires_grad:
         teacher_logp = teacher_logp.detach()
     if teacher_logp.dtype == torch.float64:
@@ -138,7 +140,7 @@ def distill_topk(logits: torch.Tensor, teacher_logp: torch.Tensor, teacher_index
     if weight is not None:
         weight = weight.detach().to(torch.float32).contiguous()
     teacher_logp, teacher_index, rest = teacher_logp.contiguous(), teacher_index.contiguous(), bool(rest)
-    if through_autograd(logits):
+    if torch.is_grad_enabled() and logits.requires_grad or torch._C._is_tracing():
         return DistillTopKFn.apply(logits, teacher_logp, teacher_index, temperature, rest, weight, mean)
     rows = _native.Rows(logits, temperature)
     return _native.distill_forward(rows, teacher_logp, teacher_index, rest, weight, mean)[0]
