@@ -24,9 +24,10 @@ __device__ __forceinline__ uint4 mask_vec(uint4 w, uint32_t bits) {
 // One block (or cluster) per row. The listed classes are marked by a bit each
 // (a byte per vector) in shared memory, so that the streaming loop leaves
 // them out at the price of one byte load per vector; their own sum comes from
-// the K pairs. The exponential unit bounds it for 16-bit logits (0.65 of it
-// busy): 4096 rows of 131072 bf16 classes with 64 pairs 215 us, 0.76 of a
-// copy's rate, 203 us without a rest and one pair; fp32 0.89.
+// the K pairs. For 16-bit logits the exponential unit, the issue slots and
+// DRAM are at 0.65 each, and the rows' ends are between them: 4096 rows of
+// 131072 bf16 classes with 64 pairs 219 us, 0.75 of a copy's rate, 204 us
+// without a rest and one pair; 4096 of 65536 fp32 185 us (0.89).
 // ROUNDED: a rest with 16-bit log-probabilities. Their noise takes registers
 // that the others cannot spare (220 -> 234 us for the 64 pairs above).
 constexpr int kBatch = 4, kStages = 2;
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(Args a) {
 
 // Elementwise from the row's saved sums, one block per piece of a row; the
 // listed classes are written over at the end. Memory bounds it: 4096 rows of
-// 131072 bf16 classes 325 us, a copy's rate.
+// 131072 bf16 classes 326 us, a copy's rate.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) bwd_block_kernel(Args a) {
   __shared__ int idx[R4C_TOPK_MAX];

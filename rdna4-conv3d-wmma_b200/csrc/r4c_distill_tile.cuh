@@ -2,19 +2,22 @@
 //
 // Both directions read the row once into registers; the backward computes the
 // row's sums again rather than loading saved ones, which for the four classes
-// of a segmentation would be more bytes than the logits. The teacher's pairs
+// of a segmentation would be more bytes than the logits (for a hundred classes
+// they would be few; that form is not built). The teacher's pairs
 // stay in registers as well, lane l of a row's group taking pairs l, l + G, ...
 // With a rest bucket the listed classes are taken out of the staged row (their
 // places set to -inf) before it is loaded, so that the loops over classes know
 // nothing of the list; in the backward the pairs' lanes write the listed
 // classes' gradients over the row at the end.
 //
-// Issue slots bound both directions (0.70 to 0.78 of them used). B200, kernel
-// alone: 4.2M rows of 4 bf16 classes, two pairs and a rest, 57 us forward and
-// 61 us backward (0.27 and 0.34 of a copy's rate; 310 and 370 instructions a
-// row, of which reading the pairs is 15, the loss 20); 369k rows of 105
-// classes with eight pairs 50 and 68 us. Tests of the list per class instead
-// took 171 and 203 us there.
+// Both directions run out of issue slots first (0.70 to 0.78 of them used,
+// DRAM 0.21 to 0.31). B200, kernel alone: 4.2M rows of 4 bf16 classes, two pairs
+// and a rest, 60 us forward and 65 us backward (0.25 and 0.31 of a copy's rate;
+// 310 and 370 instructions a row, of which reading the pairs is 15, the loss
+// 20); one pair 56 and 59 us, three (four places for them) 85 and 96 us. 369k
+// rows of 105 classes with eight pairs and weights 50 and 70 us, with nine and
+// a rest 67 and 82 us, with twenty (32 lanes a row) 222 and 262 us. Tests of
+// the list per class instead took 171 and 203 us with eight.
 #pragma once
 
 #include "r4c_distill.cuh"

@@ -97,10 +97,14 @@ template <> struct TopKey<float> {
 // the entropy comes from sum 2^t t in the same pass, and the alternatives
 // from rounds of a maximum over unique keys (two of them, of a lane's own
 // row, from one pass that keeps the two largest). What it does beyond the
-// exponentials bounds it: 4.2M rows of 4 bf16 classes with labels and two
-// alternatives take 41 us, 0.69 of copy, at 210 instructions a row, of which
-// the alternatives are 70, the label 30 and the sums 27; 369k rows of 105
-// fp16 classes 38 us, 0.34 of copy, at 0.75 of the issue slots.
+// exponentials fills its issue slots (0.70 to 0.75 of them) before the memory
+// is busy: 4.2M rows of 4 bf16 classes with labels and two alternatives take
+// 41 us, 0.69 of copy, at 210 instructions a row, of which the alternatives
+// are 70, the label 30 and the sums 27; 369k rows of 105 fp16 classes 39 us,
+// 0.33 of copy. The rounds go over all of a lane's keys, so they cost far more
+// than a pass: with 0, 1, 5 and 20 alternatives 369k rows of 105 bf16 classes
+// take 39, 64, 98 and 225 us, fp32 (keys of 64 bits) 57, 98, 190 and 539 us;
+// 4.2M rows of 4 with 1, 2 and 3 take 47, 41 and 65 us.
 template <typename T, int G, int E, int UB>
 __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
   const float k = a.inv_t * kLog2e;
@@ -190,8 +194,9 @@ __global__ void __launch_bounds__(kTileThreads) fwd_tile_kernel(FwdArgs a) {
 
 // Short rows, backward: dz_c = 2^t (c0 - cb t) with the row's constants, then
 // the label's own term. The sums are computed again: reading them back would
-// be 8 bytes a row, as much as four bf16 logits. 369k rows of 105 fp16
-// classes take 61 us (0.40 of copy, 0.73 of the issue slots).
+// be 8 bytes a row, as much as four bf16 logits (little beside a hundred, but
+// that form is not built). 369k rows of 105 fp16 classes take 61 us (0.40 of
+// copy, 0.73 of the issue slots).
 template <typename T, int G, int E, int UB>
 __global__ void __launch_bounds__(kTileThreads) bwd_tile_kernel(BwdArgs a) {
   const float k = a.inv_t * kLog2e;
@@ -397,11 +402,12 @@ __device__ __noinline__ void select_top(const uint4* p, const T* row, int off, i
 
 // Long rows, forward: one pass with a running maximum and sums, in batches of
 // four vectors a thread that are copied ahead, across the rows' ends too. The
-// exponential unit bounds it for 16-bit logits (16 a clock and SM, 0.6 to 0.7
-// of it busy), the memory for fp32: 4096 rows of 131072 bf16 classes 199 us
-// (0.82 of copy), 4096 of 65536 fp32 178 us (0.92); with one alternative
-// 201 us, with twenty 236 us (128 threads a row; 234 and 250 us with 256). A
-// third batch in flight changed nothing. One row of 131072 takes 16 us with
+// memory bounds it for fp32. For 16-bit logits nothing is full (issue slots
+// 0.65, the exponential unit 0.57, DRAM 0.53 at 32771 classes), and the largest
+// stall is the block's barriers at the rows' ends. 4096 rows of 131072 bf16
+// classes take 195 us (0.84 of copy), 4096 of 65536 fp32 174 us (0.94), 4095 of
+// 32771 bf16 70 us (0.59); the first with one alternative 201 us, with twenty
+// 236 us (128 threads a row; 231 and 248 us with 256). A third batch in flight changed nothing. One row of 131072 takes 16 us with
 // twenty alternatives, 10 us without, on eight blocks.
 constexpr int kBatch = 4, kStages = 2;
 template <typename T, int NT, bool TOP>
@@ -539,7 +545,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) fwd_block_kernel(FwdArgs a) {
 
 // Long rows, backward: elementwise from two saved numbers a row, one block per
 // piece of a row; memory bounds it. 4095 rows of 32771 bf16 classes, with the
-// entropy's gradient, 90 us (0.91 of copy; 101 us with 256 threads). Pieces
+// entropy's gradient, 90 us (0.91 of copy; 100 us with 256 threads). Pieces
 // of 4 vectors a thread instead of 16 took 120 us: what a block reads before it
 // starts is the same.
 template <typename T, int NT>

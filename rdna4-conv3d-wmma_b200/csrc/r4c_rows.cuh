@@ -14,9 +14,9 @@
 // * Above ("block"): a block, or a cluster of blocks when there are few rows,
 //   streams over the row in 16-byte loads and keeps a running maximum and sum.
 //
-// These kernels are bound by instruction issue before they are bound by
-// memory: at 6.5 TB/s an SM has about 11 instructions for each 16-bit logit.
-// So the arithmetic is packed (two fp32 a instruction), maxima are taken on
+// At 6.5 TB/s an SM has about 11 instructions for each 16-bit logit, and what
+// these kernels do for a row as a whole comes on top: most spend their issue
+// slots before the memory's time. So the arithmetic is packed (two fp32 a instruction), maxima are taken on
 // packed words, and checks are made per vector or per row, not per element.
 #pragma once
 
@@ -37,14 +37,14 @@ constexpr int kTileClasses = 1024;
 constexpr int kTileThreads = 256;
 constexpr int kSMs = 148;
 // Threads to a streamed row: one warp up to 16 KB, else 256. What a row costs
-// beyond its elements is paid per warp: 16384 rows of 1500 bf16 classes took
-// 63 us forward and 87 us backward with 128 and 256 threads, 29 and 29 us with
-// 32. More than 32 pairs or alternatives take 256, so that each pair has a
+// beyond its elements is paid per warp: 16384 rows of 1500 bf16 classes take
+// 125 us forward with 256 threads (119 with an alternative) and 52 us backward
+// with 128, 29 (47) and 31 us with 32. More than 32 pairs or alternatives take 256, so that each pair has a
 // thread and there are maxima enough to choose from.
 // (Where they are many, 128 threads do better for alternatives, whose search
-// fewer warps then wait for: 4096 rows of 131072 with one take 201 us, not 234;
-// without alternatives 218, not 196. Gradients take 128 as well: 4095 rows of
-// 32771 with the entropy's 90 us, not 101.)
+// fewer warps then wait for: 4096 rows of 131072 with one take 201 us, not 231;
+// without alternatives 217, not 195. Gradients take 128 as well: 4095 rows of
+// 32771 with the entropy's 90 us, not 100.)
 constexpr int kWarpRow = 32, kLongRow = 256, kManyRows = 128, kGradRow = 128;
 inline int row_threads(int C, int es, int k) { return (int64_t)C * es <= 16 << 10 && k <= kWarpRow ? kWarpRow : kLongRow; }
 
