@@ -382,8 +382,9 @@ typedef struct r4c_rows_desc {
  *   top_logp, top_index [rows][top_k]: largest first, equal logits by lowest class (0 <= top_k <= R4C_TOPK_MAX, <= classes)
  * Rows without a finite logit (all -inf): lse, logp and top_logp -inf, entropy
  * 0, no gradient. Rows that hold a NaN or +inf have no distribution: every
- * float is NaN and top_index -1. A class outside [0, C) that is not
- * ignore_index counts as ignored and sets code 6 in the device error flag.
+ * float is NaN (logp 0 where ignored), top_index -1, the gradient NaN or, where
+ * the row has no upstream gradient other than 0, 0. A class outside [0, C) that
+ * is not ignore_index counts as ignored and sets code 6 in the device error flag.
  * Above 1024 classes the classes must be contiguous (class_stride 1).
  * `stats` (r4c_logp_stats_size(desc) bytes, null allowed when that is 0 or
  * when no backward follows) carries the rows' maxima and sums to r4c_logp_bwd,

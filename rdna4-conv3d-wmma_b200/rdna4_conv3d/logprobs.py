@@ -105,7 +105,8 @@ def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, *, to
     mode, once; on the CPU as torch has them); ``top_logp`` does not. A row
     without a finite logit has lse, logp and top_logp -inf, entropy 0 and no
     gradient; one that holds a NaN or +inf has no distribution: its values are
-    NaN and its top_index -1.
+    NaN (logp 0 where ignored), its top_index -1, and its gradient NaN, or 0
+    where it has no upstream gradient other than 0.
     """
     check_logits(logits, temperature)
     zs = logits.shape
