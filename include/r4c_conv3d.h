@@ -434,6 +434,62 @@ int r4c_distill_bwd(const r4c_rows_desc* desc, const void* logits, int k, const 
                     const float* grad, int grad_inc, const void* state, void* dlogits, r4c_stream_t stream);
 
 /*
+ * Activations in 8 bits, to be kept until a backward pass. Every 32 elements
+ * in memory order share one power of two, 2^e with the least e >= -127 that
+ * brings their largest finite magnitude to at most 127 (R4C_Q8_INT8) or 448
+ * (R4C_Q8_E4M3); a code is x 2^-e rounded to the nearest, ties to even: a
+ * signed byte, or an 8-bit floating-point number of 4 exponent and 3 mantissa
+ * bits. NaN and infinities are held as NaN (-128 and 0x7f). r4c_unpack8 writes
+ * code * 2^e in the given type, at most its largest finite number. `count`
+ * elements of bf16, fp16 or fp32; codes: count bytes, 16-byte aligned;
+ * exponents: (count + 31) / 32 bytes that hold e + 127. No reference
+ * counterpart (its autograd keeps activations whole).
+ */
+enum { R4C_Q8_INT8 = 0, R4C_Q8_E4M3 = 1 };
+int r4c_pack8(const void* x, int64_t count, int dtype, int format, void* codes, void* exponents, r4c_stream_t stream);
+int r4c_unpack8(const void* codes, const void* exponents, int64_t count, int dtype, int format, void* x,
+                r4c_stream_t stream);
+
+/*
+ * Group normalisation with an activation on channels-last activations:
+ * `samples` x `inner` voxels x `channels`, channels innermost and dense, in
+ * `groups` equal groups of neighbouring channels.
+ *   mean, rstd of a (sample, group): biased variance, rstd = (var + eps)^-1/2
+ *   y = act((x - mean) * (rstd * gamma) + beta)
+ * gamma, beta (channels each, both param_dtype) may be null: 1 and 0. x, y,
+ * dy, dx bf16, fp16 or fp32 (dtype), 16-byte aligned; arithmetic in fp32,
+ * sums across threads in fp64 and in a fixed order. mean_rstd: (mean, rstd)
+ * per sample and group, 2 * samples * groups floats, written by the forward
+ * and read by the backward.
+ * With codes and exponents given (both or neither) the forward also writes x
+ * as r4c_pack8 does. The backward takes those (x = codes, `exponents`,
+ * `format`) or, with exponents null, x itself:
+ *   xh = (x - mean) * rstd,  dz = dy * act'(z)
+ *   dgamma = sum dz * xh,  dbeta = sum dz              (fp32; each may be null)
+ *   dx = rstd * (dz * gamma - mean_g(dz * gamma) - xh * mean_g(dz * gamma * xh))   (may be null)
+ * where the 8 bits stand for the values that they hold, and mean and rstd are
+ * those of x itself. relu and leaky_relu have slope 0 and `slope` at z <= 0.
+ * gelu is z * Phi(z) with the normal distribution function. `ws`:
+ * r4c_gn_workspace_size(desc, backward) bytes, 16-byte aligned.
+ * No reference counterpart (its blocks normalise over the batch,
+ * benches/unet_e2e.py:13-20).
+ */
+enum { R4C_ACT_NONE = 0, R4C_ACT_RELU = 1, R4C_ACT_LEAKY_RELU = 2, R4C_ACT_SILU = 3, R4C_ACT_GELU = 4 };
+typedef struct r4c_gn_desc {
+  int64_t samples, inner;
+  int32_t channels, groups;
+  int32_t dtype, param_dtype;
+  int32_t activation;
+  float eps, slope;
+} r4c_gn_desc;
+size_t r4c_gn_workspace_size(const r4c_gn_desc* desc, int backward);
+int r4c_gn_fwd(const r4c_gn_desc* desc, const void* x, const void* gamma, const void* beta, void* y, float* mean_rstd,
+               int format, void* codes, void* exponents, void* ws, size_t ws_bytes, r4c_stream_t stream);
+int r4c_gn_bwd(const r4c_gn_desc* desc, const void* dy, const void* x, int format, const void* exponents,
+               const float* mean_rstd, const void* gamma, const void* beta, void* dx, float* dgamma, float* dbeta,
+               void* ws, size_t ws_bytes, r4c_stream_t stream);
+
+/*
  * Conv3d weight and bias gradient without any allocation. No counterpart in
  * the reference: it exists for callers that cannot allocate device memory,
  * e.g. a plugin or custom op running inside another framework that owns the

@@ -1,0 +1,147 @@
+// r4c_gn.cu — group normalisation with an activation: plans and entry points (r4c_gn_*).
+#include <algorithm>
+#include <numeric>
+
+#include "r4c_gn.cuh"
+
+namespace r4c {
+namespace gn {
+namespace {
+
+struct Plan {
+  Geo g;
+  int V, threads;
+};
+
+bool ok_desc(const r4c_gn_desc* d) {
+  return d && d->samples >= 0 && d->inner >= 0 && d->channels > 0 && d->groups > 0 && d->channels % d->groups == 0 &&
+         (d->dtype == R4C_BF16 || d->dtype == R4C_F16 || d->dtype == R4C_F32) &&
+         (d->param_dtype == R4C_BF16 || d->param_dtype == R4C_F16 || d->param_dtype == R4C_F32) &&
+         d->activation >= R4C_ACT_NONE && d->activation <= R4C_ACT_GELU && d->eps >= 0.f;
+}
+
+// How the blocks share the data; false where a count passes a launch's limits.
+bool make_plan(const r4c_gn_desc* d, Plan* pl) {
+  Geo& g = pl->g;
+  const int64_t C = d->channels;
+  if (d->inner > INT64_MAX / 8 / C || (d->samples && d->inner * C > INT64_MAX / 8 / d->samples)) return false;
+  g.sample = d->inner * C;
+  g.C = d->channels;
+  g.G = d->groups;
+  g.Cg = g.C / g.G;
+  g.inv_m = 1.0 / ((double)g.Cg * (double)std::max<int64_t>(1, d->inner));
+  g.eps = d->eps;
+  g.slope = d->slope;
+  g.act = d->activation;
+  g.pdtype = d->param_dtype;
+  g.format = 0;
+  // the widest vector whose rows of lcm(C, V) elements divide a sample; several voxels in a row only while such a
+  // row fits a block's threads
+  int V = 16 / (int)dtype_bytes(d->dtype);
+  for (; V > 1; V /= 2) {
+    const int64_t L = std::lcm(C, (int64_t)V);
+    if (g.sample % L == 0 && (L == C || L <= kThreads * V)) break;
+  }
+  pl->V = V;
+  g.L = (int)std::lcm(C, (int64_t)V);
+  g.rows = g.sample / g.L;
+  const int lanes = g.L / V;
+  g.tiles = cdiv(lanes, kThreads);
+  g.lanes = cdiv(lanes, g.tiles);
+  g.R = std::max(1, kThreads / g.lanes);
+  pl->threads = cdiv(g.R * g.lanes, 32) * 32;
+  // about four blocks an SM in one wave, none with less than four rows for each thread
+  const int64_t want = std::max<int64_t>(1, 148 * 4 / std::max<int64_t>(1, d->samples * g.tiles));
+  g.nb = (int)std::max<int64_t>(1, std::min<int64_t>(want, (g.rows + 4 * g.R - 1) / (4 * g.R)));
+  g.chunk = ((g.rows + g.nb - 1) / g.nb + g.R - 1) / g.R * g.R;
+  if (g.chunk > 0) g.nb = (int)std::max<int64_t>(1, (g.rows + g.chunk - 1) / g.chunk);
+  g.blocks = d->samples * g.nb;
+  return g.blocks <= INT32_MAX && g.tiles <= 65535;
+}
+
+size_t fwd_bytes(const Geo& g) { return align_up((size_t)g.blocks * g.tiles * g.G * sizeof(double2), 256); }
+size_t cpart_bytes(const Geo& g) { return align_up((size_t)g.blocks * g.C * sizeof(float2), 256); }
+size_t gpart_bytes(const Geo& g) { return align_up((size_t)g.blocks * g.tiles * g.G * sizeof(float2), 256); }
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int status(cudaError_t e) { return e == cudaSuccess ? R4C_OK : R4C_ERR_CUDA; }
+
+}  // namespace
+}  // namespace gn
+}  // namespace r4c
+
+using namespace r4c::gn;
+
+extern "C" {
+
+size_t r4c_gn_workspace_size(const r4c_gn_desc* desc, int backward) {
+  Plan pl;
+  if (!ok_desc(desc) || !make_plan(desc, &pl)) return 0;
+  return backward ? cpart_bytes(pl.g) + gpart_bytes(pl.g) : fwd_bytes(pl.g);
+}
+
+int r4c_gn_fwd(const r4c_gn_desc* desc, const void* x, const void* gamma, const void* beta, void* y, float* mean_rstd,
+               int format, void* codes, void* exponents, void* ws, size_t ws_bytes, r4c_stream_t stream) {
+  if (!ok_desc(desc)) return R4C_ERR_INVALID;
+  if (desc->samples == 0 || desc->inner == 0) return R4C_OK;
+  Plan pl;
+  if (!make_plan(desc, &pl)) return R4C_ERR_TOO_LARGE;
+  if (!x || !y || !mean_rstd || (codes == nullptr) != (exponents == nullptr)) return R4C_ERR_INVALID;
+  if (codes && format != R4C_Q8_INT8 && format != R4C_Q8_E4M3) return R4C_ERR_INVALID;
+  if (!aligned(x) || !aligned(y) || !aligned(codes) || !aligned(ws)) return R4C_ERR_ALIGN;
+  if (!ws || ws_bytes < fwd_bytes(pl.g)) return R4C_ERR_WORKSPACE;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  FwdArgs a;
+  a.x = x;
+  a.gamma = gamma;
+  a.beta = beta;
+  a.y = y;
+  a.mean_rstd = reinterpret_cast<float2*>(mean_rstd);
+  a.part = static_cast<double2*>(ws);
+  cudaError_t e;
+  if (desc->dtype == R4C_BF16) e = launch_fwd<__nv_bfloat16>(a, pl.g, pl.V, pl.threads, s);
+  else if (desc->dtype == R4C_F16) e = launch_fwd<__half>(a, pl.g, pl.V, pl.threads, s);
+  else e = launch_fwd<float>(a, pl.g, pl.V, pl.threads, s);
+  if (e != cudaSuccess) return status(e);
+  if (codes) return r4c_pack8(x, desc->samples * pl.g.sample, desc->dtype, format, codes, exponents, stream);
+  return R4C_OK;
+}
+
+int r4c_gn_bwd(const r4c_gn_desc* desc, const void* dy, const void* x, int format, const void* exponents,
+               const float* mean_rstd, const void* gamma, const void* beta, void* dx, float* dgamma, float* dbeta,
+               void* ws, size_t ws_bytes, r4c_stream_t stream) {
+  if (!ok_desc(desc)) return R4C_ERR_INVALID;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (desc->samples == 0 || desc->inner == 0) {
+    const size_t bytes = sizeof(float) * (size_t)desc->channels;
+    if (dgamma && cudaMemsetAsync(dgamma, 0, bytes, s) != cudaSuccess) return R4C_ERR_CUDA;
+    if (dbeta && cudaMemsetAsync(dbeta, 0, bytes, s) != cudaSuccess) return R4C_ERR_CUDA;
+    return R4C_OK;
+  }
+  Plan pl;
+  if (!make_plan(desc, &pl)) return R4C_ERR_TOO_LARGE;
+  if (!dy || !x || !mean_rstd) return R4C_ERR_INVALID;
+  if (exponents && format != R4C_Q8_INT8 && format != R4C_Q8_E4M3) return R4C_ERR_INVALID;
+  if (!aligned(dy) || !aligned(x) || !aligned(dx) || !aligned(ws)) return R4C_ERR_ALIGN;
+  if (!ws || ws_bytes < cpart_bytes(pl.g) + gpart_bytes(pl.g)) return R4C_ERR_WORKSPACE;
+  if (!dx && !dgamma && !dbeta) return R4C_OK;
+  BwdArgs a;
+  a.dy = dy;
+  a.x = x;
+  a.gamma = gamma;
+  a.beta = beta;
+  a.exps = static_cast<const uint8_t*>(exponents);
+  a.mean_rstd = reinterpret_cast<const float2*>(mean_rstd);
+  a.dx = dx;
+  a.dgamma = dgamma;
+  a.dbeta = dbeta;
+  a.cpart = static_cast<float2*>(ws);
+  a.gpart = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) + cpart_bytes(pl.g));
+  pl.g.format = format;
+  if (desc->dtype == R4C_BF16) return status(launch_bwd<__nv_bfloat16>(a, pl.g, pl.V, pl.threads, s));
+  if (desc->dtype == R4C_F16) return status(launch_bwd<__half>(a, pl.g, pl.V, pl.threads, s));
+  return status(launch_bwd<float>(a, pl.g, pl.V, pl.threads, s));
+}
+
+}  // extern "C"

@@ -1,0 +1,182 @@
+// r4c_q8.cu — activations into 8 bits and back (r4c_pack8, r4c_unpack8).
+//
+// Element-wise passes over memory order, bound by HBM: pack reads b bytes and writes 1.03, unpack the reverse
+// (b = 2 or 4). A thread holds 8 elements (16 bytes of bf16 / fp16, 32 of fp32), four threads a block of 32, whose
+// maximum takes two shuffles; four such pieces a thread and step keep enough loads in flight.
+#include <algorithm>
+
+#include "r4c_internal.h"
+#include "r4c_q8.cuh"
+
+namespace r4c {
+namespace q8 {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;
+
+// 8 elements as 16-byte words: one of 16-bit types, two of fp32.
+template <typename T>
+struct Oct {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+  }
+  __device__ __forceinline__ void to_f(float (&f)[8]) const {
+    const T* p = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = Elem<T>::to_f(p[k]);
+  }
+  __device__ __forceinline__ void from_f(const float (&f)[8]) {
+    T* p = reinterpret_cast<T*>(w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) p[k] = Elem<T>::from_f(f[k]);
+  }
+};
+
+// `vec`: x lies on 16 bytes (codes always do). The last, incomplete eight elements go one by one.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) pack_kernel(const T* __restrict__ x, int64_t count, int vec, int format,
+                                                        uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
+  const int64_t octs = (count + 7) / 8, full = vec ? count / 8 : 0;
+  const int64_t step = (int64_t)gridDim.x * kThreads;
+  // whole warps walk together: the bound is rounded up to a warp's 32 threads
+  const int64_t bound = (octs + 31) / 32 * 32;
+  for (int64_t base = (int64_t)blockIdx.x * kThreads + threadIdx.x; base < bound; base += step * kUnroll) {
+    Oct<T> a[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = base + u * step;
+#pragma unroll
+      for (int k = 0; k < (int)sizeof(T) / 2; ++k) a[u].w[k] = make_uint4(0, 0, 0, 0);
+      if (i < full) {
+        a[u].load(x + i * 8);
+      } else if (i < octs) {
+        T* p = reinterpret_cast<T*>(a[u].w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i * 8 + k < count) p[k] = x[i * 8 + k];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = base + u * step;
+      if (i >= bound) break;                       // the same for a whole warp
+      float f[8];
+      a[u].to_f(f);
+      const int byte = exponent_byte(block_amax<8>(f, 0xffffffffu), format);
+      const Codes<8> c = encode<8>(f, byte, format);
+      if (i >= octs) continue;
+      if ((i + 1) * 8 <= count) {
+        store_codes<8>(codes + i * 8, c);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i * 8 + k < count) codes[i * 8 + k] = (uint8_t)(c.w[k / 4] >> (8 * (k % 4)));
+      }
+      if ((i & 3) == 0) exps[i >> 2] = (uint8_t)byte;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) unpack_kernel(const uint8_t* __restrict__ codes,
+                                                          const uint8_t* __restrict__ exps, int64_t count, int vec,
+                                                          int format, T* __restrict__ x) {
+  const int64_t octs = (count + 7) / 8, full = count / 8;
+  const int64_t step = (int64_t)gridDim.x * kThreads;
+  for (int64_t base = (int64_t)blockIdx.x * kThreads + threadIdx.x; base < octs; base += step * kUnroll) {
+    Codes<8> c[kUnroll];
+    int byte[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = base + u * step;
+      c[u].w[0] = c[u].w[1] = 0;
+      byte[u] = 0;
+      if (i < full) {
+        c[u] = load_codes<8>(codes + i * 8);
+      } else if (i < octs) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i * 8 + k < count) c[u].w[k / 4] |= (uint32_t)codes[i * 8 + k] << (8 * (k % 4));
+      }
+      if (i < octs) byte[u] = exps[i >> 2];
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = base + u * step;
+      if (i >= octs) break;
+      float f[8];
+      decode<T, 8>(c[u], byte[u], format, f);
+      if (vec && i < full) {
+        Oct<T> o;
+        o.from_f(f);
+        o.store(x + i * 8);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i * 8 + k < count) x[i * 8 + k] = Elem<T>::from_f(f[k]);
+      }
+    }
+  }
+}
+
+static int grid_for(int64_t count) {
+  const int64_t octs = (count + 7) / 8;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((octs + kThreads - 1) / kThreads, 148 * 8));
+}
+
+static bool ok_args(const void* x, const void* codes, const void* exps, int64_t count, int dtype, int format) {
+  return x && codes && exps && count >= 0 && (dtype == R4C_BF16 || dtype == R4C_F16 || dtype == R4C_F32) &&
+         (format == R4C_Q8_INT8 || format == R4C_Q8_E4M3) && (reinterpret_cast<uintptr_t>(codes) & 15) == 0 &&
+         (reinterpret_cast<uintptr_t>(x) & (dtype_bytes(dtype) - 1)) == 0;
+}
+
+}  // namespace q8
+}  // namespace r4c
+
+using namespace r4c::q8;
+
+extern "C" {
+
+int r4c_pack8(const void* x, int64_t count, int dtype, int format, void* codes, void* exponents,
+              r4c_stream_t stream) {
+  if (count == 0) return R4C_OK;
+  if (!ok_args(x, codes, exponents, count, dtype, format)) return R4C_ERR_INVALID;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int grid = grid_for(count), vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  uint8_t* c = static_cast<uint8_t*>(codes);
+  uint8_t* e = static_cast<uint8_t*>(exponents);
+  if (dtype == R4C_BF16)
+    pack_kernel<<<grid, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(x), count, vec, format, c, e);
+  else if (dtype == R4C_F16)
+    pack_kernel<<<grid, kThreads, 0, s>>>(static_cast<const __half*>(x), count, vec, format, c, e);
+  else
+    pack_kernel<<<grid, kThreads, 0, s>>>(static_cast<const float*>(x), count, vec, format, c, e);
+  r4c::note_launches(1);
+  return cudaGetLastError() == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
+}
+
+int r4c_unpack8(const void* codes, const void* exponents, int64_t count, int dtype, int format, void* x,
+                r4c_stream_t stream) {
+  if (count == 0) return R4C_OK;
+  if (!ok_args(x, codes, exponents, count, dtype, format)) return R4C_ERR_INVALID;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int grid = grid_for(count), vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  const uint8_t* c = static_cast<const uint8_t*>(codes);
+  const uint8_t* e = static_cast<const uint8_t*>(exponents);
+  if (dtype == R4C_BF16)
+    unpack_kernel<<<grid, kThreads, 0, s>>>(c, e, count, vec, format, static_cast<__nv_bfloat16*>(x));
+  else if (dtype == R4C_F16)
+    unpack_kernel<<<grid, kThreads, 0, s>>>(c, e, count, vec, format, static_cast<__half*>(x));
+  else
+    unpack_kernel<<<grid, kThreads, 0, s>>>(c, e, count, vec, format, static_cast<float*>(x));
+  r4c::note_launches(1);
+  return cudaGetLastError() == cudaSuccess ? R4C_OK : R4C_ERR_CUDA;
+}
+
+}  // extern "C"

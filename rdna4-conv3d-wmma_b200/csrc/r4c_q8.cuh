@@ -1,0 +1,171 @@
+// r4c_q8.cuh — an activation in 8 bits: codes with one power of two for every 32 elements in memory order.
+//
+// Block of 32: a = largest finite magnitude, e = the least integer >= -127 with a <= M 2^e, M = 127 (whole numbers
+// with a sign) or 448 (8-bit floating point, 4 exponent and 3 mantissa bits). code = x 2^-e rounded to the nearest,
+// ties to even; NaN and infinities get the code of NaN (-128, or 0x7f). The stored byte is e + 127. Powers of two
+// keep every product exact, so the codes are the same wherever they are computed, and 8 bits for 32 elements cost
+// 3 % where an fp32 scale would cost 12 %. Rounding: half a unit of 2^e, that is at most a / 127 (int8), or 2^-4 of
+// the value down to a / 57344 (e4m3).
+// Read back: code 2^e in the activation's type, rounded to nearest (only fp16 numbers below 2^-14 can need it), at
+// most the type's largest finite number (a code may round up past it).
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "r4c_common.cuh"
+
+namespace r4c {
+namespace q8 {
+
+constexpr int kBlock = 32;
+
+// Stored exponent byte of a block whose largest finite magnitude has these fp32 bits.
+__device__ __forceinline__ int exponent_byte(uint32_t amax_bits, int format) {
+  const int e = (int)(amax_bits >> 23);
+  const uint32_t m = amax_bits & 0x7fffffu;
+  // 127 = 1.984375 * 2^6, 448 = 1.75 * 2^8: one power more when the mantissa is above the limit's
+  const int b = format == R4C_Q8_INT8 ? e - 6 + (m > 0x7e0000u ? 1 : 0) : e - 8 + (m > 0x600000u ? 1 : 0);
+  return b < 0 ? 0 : b;
+}
+__device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
+__device__ __forceinline__ float scale(int byte) {
+  return __uint_as_float(byte ? (uint32_t)byte << 23 : 0x00400000u);
+}
+
+// V codes (V = 1, 2, 4 or 8) in the low bytes of the words.
+template <int V>
+struct Codes {
+  uint32_t w[V > 4 ? 2 : 1];
+};
+
+template <int V>
+__device__ __forceinline__ Codes<V> load_codes(const uint8_t* p) {
+  Codes<V> c;
+  if constexpr (V == 8) {
+    const uint2 r = *reinterpret_cast<const uint2*>(p);
+    c.w[0] = r.x;
+    c.w[1] = r.y;
+  } else if constexpr (V == 4) {
+    c.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (V == 2) {
+    c.w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else {
+    c.w[0] = *p;
+  }
+  return c;
+}
+template <int V>
+__device__ __forceinline__ void store_codes(uint8_t* p, const Codes<V>& c) {
+  if constexpr (V == 8)
+    *reinterpret_cast<uint2*>(p) = make_uint2(c.w[0], c.w[1]);
+  else if constexpr (V == 4)
+    *reinterpret_cast<uint32_t*>(p) = c.w[0];
+  else if constexpr (V == 2)
+    *reinterpret_cast<uint16_t*>(p) = (uint16_t)c.w[0];
+  else
+    *p = (uint8_t)c.w[0];
+}
+
+template <int V>
+__device__ __forceinline__ Codes<V> encode(const float (&f)[V], int byte, int format) {
+  Codes<V> c;
+  c.w[0] = 0;
+  if constexpr (V > 4) c.w[1] = 0;
+  const float inv = inverse_scale(byte);
+  if (format == R4C_Q8_INT8) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int q = fabsf(f[k]) < INFINITY ? __float2int_rn(f[k] * inv) : -128;
+      c.w[k / 4] |= (uint32_t)(q & 0xff) << (8 * (k % 4));
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const uint32_t q = fabsf(f[k]) < INFINITY ? __nv_cvt_float_to_fp8(f[k] * inv, __NV_SATFINITE, __NV_E4M3) : 0x7fu;
+      c.w[k / 4] |= q << (8 * (k % 4));
+    }
+  }
+  return c;
+}
+
+// Bytes below / above which a value may need T's rounding / T's largest number.
+template <typename T> struct Limits;
+template <> struct Limits<__half> {
+  static constexpr int low = 103, high_int8 = 136, high_e4m3 = 134;
+  static __device__ __forceinline__ float most() { return 65504.f; }
+};
+template <> struct Limits<__nv_bfloat16> {
+  static constexpr int low = -1, high_int8 = 248, high_e4m3 = 246;
+  static __device__ __forceinline__ float most() { return __uint_as_float(0x7f7f0000u); }
+};
+template <> struct Limits<float> {
+  static constexpr int low = -1, high_int8 = 248, high_e4m3 = 246;
+  static __device__ __forceinline__ float most() { return __uint_as_float(0x7f7fffffu); }
+};
+
+// The values of T that the codes stand for.
+template <typename T, int V>
+__device__ __forceinline__ void decode(const Codes<V>& c, int byte, int format, float (&f)[V]) {
+  const float s = scale(byte);
+  if (format == R4C_Q8_INT8) {
+    // 0x4b0000uu is 2^23 + u exactly: the signed code is that minus 2^23 + 128 (no integer-to-float conversions,
+    // which share a slow pipe)
+    uint32_t nan = 0;
+#pragma unroll
+    for (int i = 0; i < (V > 4 ? 2 : 1); ++i) {
+      const uint32_t u = c.w[i] ^ 0x80808080u;
+      uint32_t zero = (u - 0x01010101u) & ~u & 0x80808080u;   // a byte of u is 0: some code is -128
+      if (V < 4) zero &= (1u << (8 * V)) - 1;
+      nan |= zero;
+#pragma unroll
+      for (int k = 4 * i; k < V && k < 4 * i + 4; ++k)
+        f[k] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + (k & 3))) - 8388736.f) * s;
+    }
+    if (nan) {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (((c.w[k / 4] >> (8 * (k % 4))) & 0xffu) == 0x80u) f[k] = __uint_as_float(0x7fc00000u);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const __nv_fp8_storage_t b = (__nv_fp8_storage_t)((c.w[k / 4] >> (8 * (k % 4))) & 0xffu);
+      f[k] = __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3))) * s;
+    }
+  }
+  const int high = format == R4C_Q8_INT8 ? Limits<T>::high_int8 : Limits<T>::high_e4m3;
+  if (byte > high || byte < Limits<T>::low) {
+    const float most = Limits<T>::most();
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      f[k] = f[k] > most ? most : (f[k] < -most ? -most : f[k]);
+      f[k] = Elem<T>::to_f(Elem<T>::from_f(f[k]));
+    }
+  }
+}
+
+// Largest finite magnitude (fp32 bits) of a block that 32 / V neighbouring lanes hold, V elements each; every lane of
+// `mask` takes part.
+template <int V>
+__device__ __forceinline__ uint32_t block_amax(const float (&f)[V], uint32_t mask) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < V; ++k) m = max(m, __float_as_uint(f[k]) & 0x7fffffffu);
+  const uint32_t own = m;
+#pragma unroll
+  for (int o = 1; o < kBlock / V; o <<= 1) m = max(m, __shfl_xor_sync(mask, m, o));
+  if (__any_sync(mask, own >= 0x7f800000u)) {   // NaN or infinities somewhere: the finite ones alone
+    m = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const uint32_t b = __float_as_uint(f[k]) & 0x7fffffffu;
+      m = max(m, b < 0x7f800000u ? b : 0u);
+    }
+#pragma unroll
+    for (int o = 1; o < kBlock / V; o <<= 1) m = max(m, __shfl_xor_sync(mask, m, o));
+  }
+  return m;
+}
+
+}  // namespace q8
+}  // namespace r4c

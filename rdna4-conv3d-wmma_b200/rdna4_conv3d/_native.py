@@ -56,6 +56,14 @@ class RowsDesc(ctypes.Structure):
                 ("classes", ctypes.c_int32), ("dtype", ctypes.c_int32), ("temperature", ctypes.c_float)]
 
 
+class GnDesc(ctypes.Structure):
+    """r4c_gn_desc: channels-last activations in groups (include/r4c_conv3d.h)."""
+    _fields_ = [("samples", ctypes.c_int64), ("inner", ctypes.c_int64),
+                ("channels", ctypes.c_int32), ("groups", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("param_dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("slope", ctypes.c_float)]
+
+
 class NativeError(RuntimeError):
     """A C-ABI entry point returned a non-zero status."""
 
@@ -69,6 +77,7 @@ def _bind(lib) -> None:
     D = ctypes.POINTER(ConvDesc)
     X = ctypes.POINTER(ConvexDesc)
     R = ctypes.POINTER(RowsDesc)
+    N = ctypes.POINTER(GnDesc)
     sz = ctypes.c_size_t
     i = ctypes.c_int
     i64 = ctypes.c_int64
@@ -113,6 +122,11 @@ def _bind(lib) -> None:
         "r4c_distill_state_size": ([R], sz),
         "r4c_distill_fwd": ([R, P, i, P, i, P, i, i, P, P, P, P, sz, P], i),
         "r4c_distill_bwd": ([R, P, i, P, i, P, i, i, P, i, P, i, P, P, P], i),
+        "r4c_pack8": ([P, i64, i, i, P, P, P], i),
+        "r4c_unpack8": ([P, P, i64, i, i, P, P], i),
+        "r4c_gn_workspace_size": ([N, i], sz),
+        "r4c_gn_fwd": ([N, P, P, P, P, P, i, P, P, P, sz, P], i),
+        "r4c_gn_bwd": ([N, P, P, i, P, P, P, P, P, P, P, P, sz, P], i),
         "r4c_convex_plan": ([X], i),
         "r4c_convex_workspace_size": ([X, i], sz),
         "r4c_convex_fwd": ([X, P, P, P, P, P, sz, P], i),
@@ -802,3 +816,75 @@ def distill_backward(z: torch.Tensor, desc: RowsDesc, teacher_logp: torch.Tensor
             8 * teacher_index.element_size(), rest, None if weight is None else weight.data_ptr(), mean,
             g.data_ptr(), 0 if mean else inc, state.data_ptr(), dz.data_ptr())
     return dz
+
+
+# ---------------------------------------------------------------------------
+# Activations in 8 bits (r4c_pack8, r4c_unpack8); group normalisation (r4c_gn_*)
+# ---------------------------------------------------------------------------
+Q8_BLOCK = 32
+Q8_FORMATS = {"int8": 0, "e4m3": 1}
+ACTIVATIONS = {"none": 0, "relu": 1, "leaky_relu": 2, "silu": 3, "gelu": 4}
+
+
+def q8_buffers(x: torch.Tensor):
+    """Empty codes and exponents for x's elements."""
+    count = x.numel()
+    return (x.new_empty(count, dtype=torch.uint8),
+            x.new_empty((count + Q8_BLOCK - 1) // Q8_BLOCK, dtype=torch.uint8))
+
+
+def pack8(x: torch.Tensor, fmt: int):
+    """(codes, exponents) of a dense tensor's elements in memory order."""
+    codes, exps = q8_buffers(x)
+    _launch("r4c_pack8", lib().r4c_pack8, x.device, x.data_ptr(), x.numel(), dtype_code(x.dtype), fmt,
+            codes.data_ptr(), exps.data_ptr())
+    return codes, exps
+
+
+def unpack8(codes: torch.Tensor, exps: torch.Tensor, fmt: int, out: torch.Tensor) -> torch.Tensor:
+    """Writes the values of the codes into a dense tensor, in its memory order."""
+    _launch("r4c_unpack8", lib().r4c_unpack8, out.device, codes.data_ptr(), exps.data_ptr(), out.numel(),
+            dtype_code(out.dtype), fmt, out.data_ptr())
+    return out
+
+
+def gn_desc(x: torch.Tensor, groups: int, params_dtype: torch.dtype, eps: float, activation: int,
+            slope: float) -> GnDesc:
+    shape = x.shape
+    return GnDesc(shape[0], shape[2:].numel(), shape[1], groups, dtype_code(x.dtype), dtype_code(params_dtype),
+                  activation, eps, slope)
+
+
+def _addr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def gn_forward(x: torch.Tensor, desc: GnDesc, weight, bias, fmt: Optional[int]):
+    """(y, mean_rstd, codes or None, exponents or None) of a channels-last dense x."""
+    L = lib()
+    y = class_last_empty(x)
+    mean_rstd = x.new_empty((2 * desc.samples * desc.groups,), dtype=torch.float32)
+    codes = exps = None
+    if fmt is not None:
+        codes, exps = q8_buffers(x)
+    nb = L.r4c_gn_workspace_size(desc, 0)
+    ws = x.new_empty(nb, dtype=torch.uint8)
+    _launch("r4c_gn_fwd", L.r4c_gn_fwd, x.device, desc, x.data_ptr(), _addr(weight), _addr(bias), y.data_ptr(),
+            mean_rstd.data_ptr(), fmt or 0, _addr(codes), _addr(exps), ws.data_ptr(), nb)
+    return y, mean_rstd, codes, exps
+
+
+def gn_backward(dy: torch.Tensor, desc: GnDesc, x, fmt: int, exps, mean_rstd, weight, bias, need_dx: bool,
+                need_params: bool):
+    """(dx, dweight, dbias); fp32 parameter gradients; x the activation, or its codes with ``exps``."""
+    L = lib()
+    dx = class_last_empty(dy) if need_dx else None
+    dw = db = None
+    if need_params:
+        dw = dy.new_empty((desc.channels,), dtype=torch.float32)
+        db = torch.empty_like(dw)
+    nb = L.r4c_gn_workspace_size(desc, 1)
+    ws = dy.new_empty(nb, dtype=torch.uint8)
+    _launch("r4c_gn_bwd", L.r4c_gn_bwd, dy.device, desc, dy.data_ptr(), x.data_ptr(), fmt, _addr(exps),
+            mean_rstd.data_ptr(), _addr(weight), _addr(bias), _addr(dx), _addr(dw), _addr(db), ws.data_ptr(), nb)
+    return dx, dw, db

@@ -343,51 +343,86 @@ class Conv3dWmmaFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_out):
         x, weight = ctx.saved_tensors
-        stride, padding, dilation, ks = ctx.stride, ctx.padding, ctx.dilation, ctx.kernel_size
-        cin, cout = int(x.shape[1]), int(weight.shape[0])
-        go = grad_out if grad_out.dtype in _HALF else grad_out.to(torch.float16)
-        x_c = x if x.dtype in _HALF else x.to(torch.float16)
-        if go.dtype != x_c.dtype:
-            go = go.to(x_c.dtype)
-        if x.is_cuda and wmma_ok_dw(cin, cout, ks, stride, dilation, 1):
-            go = _as_ndhwc(go)        # one dense NDHWC copy for both kernel legs
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        want_db = ctx.has_bias and need_b
-        dx_leg = need_x and wmma_ok_dx(cin, cout, ks, stride, dilation, 1)
-        dw_leg = need_w and wmma_ok_dw(cin, cout, ks, stride, dilation, 1)
+        return (*_conv3d_backward(ctx, x.shape, x.dtype, lambda: x, weight, grad_out), None, None, None)
 
-        # dW and db first, so a data-parallel reduction overlaps the dX kernel.
-        dw = db = None
-        if need_w:
-            if dw_leg:
-                dw, db = _launch_wgrad(x_c, go, weight.shape, padding, want_db)
-            else:
-                w_c = weight if weight.dtype in _HALF else weight.to(x_c.dtype)
-                dw = torch.nn.grad.conv3d_weight(x_c, weight.shape, go.contiguous(), stride, padding,
-                                                 dilation, 1).float()
-                del w_c
-        if want_db and db is None:
-            db = go.float().sum(dim=(0, 2, 3, 4))
-        handle = _reduce_async([dw, db])
 
-        gx = None
-        if need_x:
-            if dx_leg:
-                gx = _launch_dgrad(go, weight, x.shape, padding)
-            else:
-                w_c = weight.to(go.dtype)
-                gx = torch.nn.grad.conv3d_input(x.shape, w_c, go.contiguous(), stride, padding, dilation, 1)
-            if gx.dtype != x.dtype:
-                gx = gx.to(x.dtype)
-            if ctx.x_layout == torch.contiguous_format:
-                gx = gx.contiguous()
-        if handle is not None:
-            handle.wait()
-        if dw is not None and dw.dtype != weight.dtype:
-            dw = dw.to(weight.dtype)
-        if db is not None and ctx.bias_dtype is not None and db.dtype != ctx.bias_dtype:
-            db = db.to(ctx.bias_dtype)
-        return gx, dw, db, None, None, None
+def _conv3d_backward(ctx, x_shape, x_dtype, x_of, weight, grad_out):
+    """(dX, dW, db) of a conv on the B200 kernels; ``x_of()`` gives its input (asked for dW alone)."""
+    stride, padding, dilation, ks = ctx.stride, ctx.padding, ctx.dilation, ctx.kernel_size
+    cin, cout = int(x_shape[1]), int(weight.shape[0])
+    go = grad_out if grad_out.dtype in _HALF else grad_out.to(torch.float16)
+    c_dtype = x_dtype if x_dtype in _HALF else torch.float16
+    if go.dtype != c_dtype:
+        go = go.to(c_dtype)
+    if grad_out.is_cuda and wmma_ok_dw(cin, cout, ks, stride, dilation, 1):
+        go = _as_ndhwc(go)        # one dense NDHWC copy for both kernel legs
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    want_db = ctx.has_bias and need_b
+    dx_leg = need_x and wmma_ok_dx(cin, cout, ks, stride, dilation, 1)
+    dw_leg = need_w and wmma_ok_dw(cin, cout, ks, stride, dilation, 1)
+
+    # dW and db first, so a data-parallel reduction overlaps the dX kernel.
+    dw = db = None
+    if need_w:
+        x = x_of()
+        x_c = x if x_dtype in _HALF else x.to(torch.float16)
+        if dw_leg:
+            dw, db = _launch_wgrad(x_c, go, weight.shape, padding, want_db)
+        else:
+            dw = torch.nn.grad.conv3d_weight(x_c, weight.shape, go.contiguous(), stride, padding,
+                                             dilation, 1).float()
+        del x, x_c
+    if want_db and db is None:
+        db = go.float().sum(dim=(0, 2, 3, 4))
+    handle = _reduce_async([dw, db])
+
+    gx = None
+    if need_x:
+        if dx_leg:
+            gx = _launch_dgrad(go, weight, x_shape, padding)
+        else:
+            w_c = weight.to(go.dtype)
+            gx = torch.nn.grad.conv3d_input(x_shape, w_c, go.contiguous(), stride, padding, dilation, 1)
+        if gx.dtype != x_dtype:
+            gx = gx.to(x_dtype)
+        if ctx.x_layout == torch.contiguous_format:
+            gx = gx.contiguous()
+    if handle is not None:
+        handle.wait()
+    if dw is not None and dw.dtype != weight.dtype:
+        dw = dw.to(weight.dtype)
+    if db is not None and ctx.bias_dtype is not None and db.dtype != ctx.bias_dtype:
+        db = db.to(ctx.bias_dtype)
+    return gx, dw, db
+
+
+class Conv3dKept8Fn(torch.autograd.Function):
+    """Conv3dWmmaFn whose input is kept for the weight gradient in 8 bits
+    (``checkpoint8.pack8``); y and dX are the same, dW is that of the values
+    that the 8 bits hold."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, stride, padding, dilation, fmt):
+        from .checkpoint8 import pack8
+        y = Conv3dWmmaFn.forward(x, weight, bias, stride, padding, dilation)
+        packed = pack8(x, fmt) if ctx.needs_input_grad[1] else (None, None)
+        ctx.save_for_backward(packed[0], packed[1], weight)
+        ctx.packed = packed[2:]
+        ctx.was = x.shape, x.dtype
+        ctx.has_bias = bias is not None
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.stride, ctx.padding, ctx.dilation = stride, padding, dilation
+        ctx.kernel_size = tuple(int(s) for s in weight.shape[2:])
+        ctx.x_layout = (torch.channels_last_3d if x.is_contiguous(memory_format=torch.channels_last_3d)
+                        else torch.contiguous_format)
+        return y
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        from .checkpoint8 import Packed8, unpack8
+        codes, exps, weight = ctx.saved_tensors
+        return (*_conv3d_backward(ctx, *ctx.was, lambda: unpack8(Packed8(codes, exps, *ctx.packed)), weight, grad_out),
+                None, None, None, None)
 
 
 def _autocast_dtype():
@@ -426,8 +461,15 @@ def _autocast_args(x, weight, bias):
     return (x if x.dtype == dt else x.to(dt)), weight, bias
 
 
-def conv3d_wmma(x, weight, bias=None, stride=1, padding=0, dilation=1, groups=1):
-    """Functional Conv3d; same arguments as F.conv3d (integer/tuple padding)."""
+def conv3d_wmma(x, weight, bias=None, stride=1, padding=0, dilation=1, groups=1, *, checkpoint=None):
+    """Functional Conv3d; same arguments as F.conv3d (integer/tuple padding).
+
+    ``checkpoint`` ('int8' or 'e4m3'): the input is kept for the weight
+    gradient in 8 bits (``checkpoint8.pack8``) where a bf16, fp16 or fp32 one
+    runs on the k=1 and k=3 stride-1 kernels; other convs keep it whole."""
+    if checkpoint is not None:
+        from .checkpoint8 import check_format
+        check_format(checkpoint, "checkpoint")
     if x.is_cuda and _wmma_hw() and not isinstance(padding, str):
         cin, cout = int(x.shape[1]), int(weight.shape[0])
         if _k2s2_ok(x, cin, cout, weight.shape[2:], stride, padding, dilation, groups) or (
@@ -436,7 +478,12 @@ def conv3d_wmma(x, weight, bias=None, stride=1, padding=0, dilation=1, groups=1)
     if groups != 1:
         return F.conv3d(x, weight, bias, stride, padding, dilation, groups)
     x, weight, bias = _autocast_args(x, weight, bias)
-    return Conv3dWmmaFn.apply(x, weight, bias, _t3(stride), _t3(padding), _t3(dilation))
+    args = x, weight, bias, _t3(stride), _t3(padding), _t3(dilation)
+    if (checkpoint is not None and torch.is_grad_enabled() and weight.requires_grad and x.is_cuda
+            and (x.dtype in _HALF or x.dtype == torch.float32)
+            and wmma_ok_dw(int(x.shape[1]), int(weight.shape[0]), tuple(weight.shape[2:]), args[3], args[5], 1)):
+        return Conv3dKept8Fn.apply(*args, checkpoint)
+    return Conv3dWmmaFn.apply(*args)
 
 
 def _check_isolated(weight, stride, dilation):
@@ -598,7 +645,12 @@ def swap_conv3d(module: nn.Module) -> int:
 
 
 class Conv3dWmma(nn.Conv3d):
-    """Drop-in ``nn.Conv3d``: B200 kernels for in-scope geometry on CUDA tensors."""
+    """Drop-in ``nn.Conv3d``: B200 kernels for in-scope geometry on CUDA tensors.
+
+    ``checkpoint`` (None, 'int8' or 'e4m3'; an attribute, None at first): how
+    the input is kept for the weight gradient, see ``conv3d_wmma``."""
+
+    checkpoint = None
 
     def forward(self, x):
         if not x.is_cuda or self.padding_mode != "zeros" or isinstance(self.padding, str):
@@ -613,7 +665,8 @@ class Conv3dWmma(nn.Conv3d):
         plan = conv3d_plan(cin, cout, self.kernel_size, self.stride, self.dilation, self.groups)
         if all(v == "miopen" for v in plan.values()):
             return super().forward(x)
-        return conv3d_wmma(x, self.weight, self.bias, self.stride, self.padding, self.dilation, 1)
+        return conv3d_wmma(x, self.weight, self.bias, self.stride, self.padding, self.dilation, 1,
+                           checkpoint=self.checkpoint)
 
 
 # ---------------------------------------------------------------------------

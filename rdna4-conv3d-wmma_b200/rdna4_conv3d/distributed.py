@@ -22,6 +22,7 @@ import torch
 import torch.distributed as dist
 
 from .bn_relu import BatchNormReLU3d
+from .group_norm import GroupNormAct3d, _act_torch, _normalised
 
 
 def _cw():
@@ -577,6 +578,71 @@ class DepthShardedBatchNormReLU3d(BatchNormReLU3d):
         return self.running_mean.detach().float().contiguous()
 
 
+class _ShardedGroupNormFn(torch.autograd.Function):
+    """GroupNormAct3d whose statistics span every rank of ``group``, in torch operations (fp32, or fp64 for fp64)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, activation, slope, group):
+        n, c = x.shape[:2]
+        xg = x.double().reshape(n, groups, -1)
+        s = torch.stack([xg.sum(-1), (xg * xg).sum(-1), torch.full_like(xg[..., 0], xg.shape[-1])])
+        dist.all_reduce(s, group=group)
+        total = s[2, 0, 0]
+        acc = torch.promote_types(x.dtype, torch.float32)
+        mean = s[0] / total
+        rstd = (((s[1] / total - mean * mean).clamp(min=0) + eps) ** -0.5).to(acc).unsqueeze(-1)
+        mean = mean.to(acc).unsqueeze(-1)
+        ctx.save_for_backward(x, mean, rstd, total, weight, bias)
+        ctx.args = groups, activation, slope, group
+        z, _ = _ShardedGroupNormFn._z(x, mean, rstd, weight, bias, groups)
+        return _act_torch(z, activation, slope).to(x.dtype)
+
+    @staticmethod
+    def _z(x, mean, rstd, weight, bias, groups):
+        xh = _normalised(x.to(mean.dtype), groups, mean, rstd)
+        each = (1, x.shape[1]) + (1,) * (x.dim() - 2)
+        z = xh if weight is None else xh * weight.to(xh.dtype).reshape(each)
+        return (z if bias is None else z + bias.to(xh.dtype).reshape(each)), xh
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, mean, rstd, total, weight, bias = ctx.saved_tensors
+        groups, activation, slope, group = ctx.args
+        n, c = x.shape[:2]
+        z, xh = _ShardedGroupNormFn._z(x, mean, rstd, weight, bias, groups)
+        with torch.enable_grad():
+            z = z.requires_grad_(True)
+            dz, = torch.autograd.grad(_act_torch(z, activation, slope), z, gy.to(z.dtype))
+        # whole-volume sums per sample and channel: they give dgamma and dbeta, and the groups' means
+        dims = tuple(range(2, x.dim()))
+        s = torch.stack([dz.double().sum(dims), (dz.double() * xh).sum(dims)])
+        dist.all_reduce(s, group=group)
+        w = torch.ones(c, dtype=z.dtype, device=x.device) if weight is None else weight.to(z.dtype)
+        a, b = ((s * w).reshape(2, n, groups, -1).sum(-1, keepdim=True) / total).to(z.dtype)
+        g = (dz * w.reshape((1, c) + (1,) * len(dims))).reshape(n, groups, -1)
+        dx = ((g - a - xh.reshape(n, groups, -1) * b) * rstd).reshape(x.shape)
+        dw = s[1].sum(0).to(weight.dtype) if weight is not None else None
+        db = s[0].sum(0).to(bias.dtype) if bias is not None else None
+        return dx.to(x.dtype), dw, db, None, None, None, None, None
+
+
+class DepthShardedGroupNormAct3d(GroupNormAct3d):
+    """GroupNormAct3d over a D-sharded volume: each rank holds one D slab of
+    the same samples, statistics and gradient sums are all-reduced over
+    ``group`` (torch operations; the input is kept whole). Weight and bias
+    gradients come out as whole-volume sums."""
+
+    def __init__(self, *args, group=None, **kw):
+        super().__init__(*args, **kw)
+        self.group = group
+
+    def forward(self, x):
+        if not (dist.is_available() and dist.is_initialized()):
+            return super().forward(x)
+        return _ShardedGroupNormFn.apply(x, self.weight, self.bias, self.num_groups, self.eps, self.activation,
+                                         self.negative_slope, self.group)
+
+
 class DepthShardedConv3d(torch.nn.Conv3d):
     """Conv3d (k=3, pad=1) over a D-sharded volume; other geometries run
     locally (k=1 convs need no halo)."""
@@ -598,8 +664,10 @@ class DepthShardedConv3d(torch.nn.Conv3d):
 def depth_shard_model(model: torch.nn.Module, group=None) -> List[torch.nn.Parameter]:
     """Convert a model in place for depth sharding over ``group``: every k3
     pad-1 Conv3d becomes a DepthShardedConv3d (halo exchange), every
-    BatchNorm3d a DepthShardedBatchNorm3d and every fused BatchNormReLU3d a
-    DepthShardedBatchNormReLU3d (statistics over the whole volume).
+    BatchNorm3d a DepthShardedBatchNorm3d, every fused BatchNormReLU3d a
+    DepthShardedBatchNormReLU3d and every GroupNormAct3d a
+    DepthShardedGroupNormAct3d (statistics over the whole volume; activations
+    are kept whole, whatever ``checkpoint`` says).
     Pooling, k2s2 transpose convs, concatenation and k1 convs need no
     exchange. Returns the parameters whose gradients are still per-slab
     partial sums (the transpose convs and k1 convs): reduce them with
@@ -633,6 +701,14 @@ def depth_shard_model(model: torch.nn.Module, group=None) -> List[torch.nn.Param
                                               child.track_running_stats, group=group,
                                               device=None if ref is None else ref.device,
                                               dtype=None if ref is None else ref.dtype)
+                new.load_state_dict(child.state_dict())
+                setattr(mod, name, new)
+            elif isinstance(child, GroupNormAct3d) and not isinstance(child, DepthShardedGroupNormAct3d):
+                ref = child.weight
+                new = DepthShardedGroupNormAct3d(child.num_groups, child.num_channels, child.eps, child.affine,
+                                                 child.activation, child.negative_slope, group=group,
+                                                 device=None if ref is None else ref.device,
+                                                 dtype=None if ref is None else ref.dtype)
                 new.load_state_dict(child.state_dict())
                 setattr(mod, name, new)
             elif isinstance(child, (torch.nn.Conv3d, torch.nn.ConvTranspose3d)) \

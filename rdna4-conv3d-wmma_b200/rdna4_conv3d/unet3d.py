@@ -24,25 +24,40 @@ import torch.nn as nn
 from .conv3d_wmma import Conv3dWmma, ConvTranspose3dWmma
 
 
-def conv_block(cin: int, cout: int, conv=nn.Conv3d) -> nn.Sequential:
-    """Two (k3 pad1 conv + BatchNorm3d + ReLU) layers."""
+_ACTIVATIONS = {"relu": lambda: nn.ReLU(inplace=True), "leaky_relu": lambda: nn.LeakyReLU(inplace=True),
+                "silu": lambda: nn.SiLU(inplace=True), "gelu": nn.GELU}
+
+
+def conv_block(cin: int, cout: int, conv=nn.Conv3d, norm: str = "batch", groups: int = 8,
+               activation: str = "relu") -> nn.Sequential:
+    """Two (k3 pad1 conv + normalisation + activation) layers: BatchNorm3d
+    (``norm='batch'``) or GroupNorm of ``groups`` groups (``'group'``), ReLU
+    unless ``activation`` names another."""
+    if norm not in ("batch", "group"):
+        raise ValueError(f"norm must be 'batch' or 'group', got {norm!r}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(map(repr, _ACTIVATIONS))}, got {activation!r}")
+    norm_of = (lambda: nn.BatchNorm3d(cout)) if norm == "batch" else (lambda: nn.GroupNorm(groups, cout))
+    act_of = _ACTIVATIONS[activation]
     return nn.Sequential(
-        conv(cin, cout, 3, padding=1), nn.BatchNorm3d(cout), nn.ReLU(inplace=True),
-        conv(cout, cout, 3, padding=1), nn.BatchNorm3d(cout), nn.ReLU(inplace=True),
+        conv(cin, cout, 3, padding=1), norm_of(), act_of(),
+        conv(cout, cout, 3, padding=1), norm_of(), act_of(),
     )
 
 
 class UNet3D(nn.Module):
     def __init__(self, in_channels: int = 1, n_classes: int = 4, base: int = 24, levels: int = 4,
-                 conv=nn.Conv3d, tconv=nn.ConvTranspose3d):
+                 conv=nn.Conv3d, tconv=nn.ConvTranspose3d, norm: str = "batch", groups: int = 8,
+                 activation: str = "relu"):
         super().__init__()
+        more = (conv, norm, groups, activation)
         ch = [base * 2 ** i for i in range(levels)]
         self.channels = ch
         self.enc = nn.ModuleList(
-            [conv_block(in_channels if i == 0 else ch[i - 1], ch[i], conv) for i in range(levels)])
+            [conv_block(in_channels if i == 0 else ch[i - 1], ch[i], *more) for i in range(levels)])
         self.pool = nn.MaxPool3d(2)
         self.up = nn.ModuleList([tconv(ch[i + 1], ch[i], 2, stride=2) for i in reversed(range(levels - 1))])
-        self.dec = nn.ModuleList([conv_block(2 * ch[i], ch[i], conv) for i in reversed(range(levels - 1))])
+        self.dec = nn.ModuleList([conv_block(2 * ch[i], ch[i], *more) for i in reversed(range(levels - 1))])
         self.head = conv(ch[0], n_classes, 1)
 
     def _fused_skips(self) -> bool:
@@ -87,16 +102,28 @@ class UNet3D(nn.Module):
 
 
 def unet3d(base: int = 24, levels: int = 4, in_channels: int = 1, n_classes: int = 4, wmma: bool = True,
-           device=None, fuse_bn: bool = None) -> UNet3D:
+           device=None, fuse_bn: bool = None, norm: str = "batch", groups: int = 8, activation: str = "relu",
+           checkpoint: str = None) -> UNet3D:
     """The UNet3D on this package's kernels (``wmma=True``) or on stock PyTorch,
     channels_last_3d parameters on ``device``. ``fuse_bn`` (default: same as
-    ``wmma``) runs each BatchNorm3d + ReLU pair on the fused kernels; the
-    state_dict keys are those of the stock model either way."""
+    ``wmma``) runs each normalisation + activation pair on the fused kernels
+    (BatchNorm3d with ReLU, GroupNorm with any activation); the state_dict keys
+    are those of the stock model either way. ``norm``, ``groups`` and
+    ``activation``: see ``conv_block``. ``checkpoint`` ('int8' or 'e4m3'): the
+    convolutions and group norms keep their inputs for the backward pass in 8
+    bits (``checkpoint8.checkpoint_activations``)."""
     conv, tconv = (Conv3dWmma, ConvTranspose3dWmma) if wmma else (nn.Conv3d, nn.ConvTranspose3d)
-    net = UNet3D(in_channels, n_classes, base, levels, conv, tconv)
+    if checkpoint is not None and not wmma:
+        raise ValueError("checkpoint needs this package's layers (wmma=True)")
+    net = UNet3D(in_channels, n_classes, base, levels, conv, tconv, norm, groups, activation)
     if wmma if fuse_bn is None else fuse_bn:
         from .bn_relu import fuse_bn_relu
+        from .group_norm import fuse_group_norm
         fuse_bn_relu(net)
+        fuse_group_norm(net)
+    if checkpoint is not None:
+        from .checkpoint8 import checkpoint_activations
+        checkpoint_activations(net, checkpoint)
     if device is not None:
         net = net.to(device)
     net = net.to(memory_format=torch.channels_last_3d)

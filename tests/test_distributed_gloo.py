@@ -221,3 +221,49 @@ def test_depth_sharded_unet_matches_full_volume():
         for n, b in net.named_buffers():
             if b.dtype.is_floating_point:
                 torch.testing.assert_close(r["bufs"][n], b, rtol=1e-9, atol=1e-9, msg=n)
+
+
+def _small_group_unet():
+    from rdna4_conv3d.group_norm import fuse_group_norm
+    from rdna4_conv3d.unet3d import UNet3D
+    torch.manual_seed(3)
+    net = UNet3D(in_channels=1, n_classes=2, base=4, levels=3, norm="group", groups=2, activation="silu").double()
+    assert fuse_group_norm(net) == 10
+    for p in net.parameters():
+        torch.nn.init.normal_(p, std=0.3)
+    return net
+
+
+def _worker_depth_group_unet(rank, port, outdir):
+    import rdna4_conv3d  # noqa: F401
+    from rdna4_conv3d.distributed import DepthShardedGroupNormAct3d, GradSync, depth_shard_model
+    _init(rank, port)
+    try:
+        net = _small_group_unet()
+        partial = depth_shard_model(net)
+        assert sum(isinstance(m, DepthShardedGroupNormAct3d) for m in net.modules()) == 10
+        GradSync(partial, average=False)
+        g = torch.Generator().manual_seed(9)
+        x = torch.randn(2, 1, 16, 8, 8, generator=g, dtype=torch.float64)
+        gy = torch.randn(2, 2, 16, 8, 8, generator=g, dtype=torch.float64)
+        y = net(_slab(x, rank))
+        (y * _slab(gy, rank)).sum().backward()
+        torch.save({"y": y.detach(), "grads": {n: p.grad.clone() for n, p in net.named_parameters()}},
+                   os.path.join(outdir, f"r{rank}.pt"))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_depth_sharded_group_norm_unet_matches_full_volume():
+    """The same UNet on group norms: statistics of each sample over both slabs, fp64."""
+    res = _run(_worker_depth_group_unet)
+    net = _small_group_unet()
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(2, 1, 16, 8, 8, generator=g, dtype=torch.float64)
+    gy = torch.randn(2, 2, 16, 8, 8, generator=g, dtype=torch.float64)
+    y = net(x)
+    (y * gy).sum().backward()
+    torch.testing.assert_close(torch.cat([r["y"] for r in res], dim=2), y.detach(), rtol=1e-9, atol=1e-9)
+    for r in res:
+        for n, p in net.named_parameters():
+            torch.testing.assert_close(r["grads"][n], p.grad, rtol=1e-8, atol=1e-9, msg=n)
