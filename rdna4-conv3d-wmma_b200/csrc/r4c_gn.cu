@@ -21,7 +21,7 @@ bool ok_desc(const r4c_gn_desc* d) {
 }
 
 // How the blocks share the data; false where a count passes a launch's limits.
-bool make_plan(const r4c_gn_desc* d, Plan* pl) {
+bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
   Geo& g = pl->g;
   const int64_t C = d->channels;
   if (d->inner > INT64_MAX / 8 / C || (d->samples && d->inner * C > INT64_MAX / 8 / d->samples)) return false;
@@ -34,7 +34,7 @@ bool make_plan(const r4c_gn_desc* d, Plan* pl) {
   g.slope = d->slope;
   g.act = d->activation;
   g.pdtype = d->param_dtype;
-  g.format = 0;
+  g.format = g.pack = 0;
   // the widest vector whose rows of lcm(C, V) elements divide a sample; several voxels in a row only while such a
   // row fits a block's threads
   int V = 16 / (int)dtype_bytes(d->dtype);
@@ -49,14 +49,25 @@ bool make_plan(const r4c_gn_desc* d, Plan* pl) {
   g.tiles = cdiv(lanes, kThreads);
   g.lanes = cdiv(lanes, g.tiles);
   g.R = std::max(1, kThreads / g.lanes);
+  if (g.R > 4) g.R = g.R / 4 * 4;       // a tile of rows starts at a block of 32 elements (fused packing)
   pl->threads = cdiv(g.R * g.lanes, 32) * 32;
-  // about four blocks an SM in one wave, none with less than four rows for each thread
-  const int64_t want = std::max<int64_t>(1, 148 * 4 / std::max<int64_t>(1, d->samples * g.tiles));
+  // one wave of the blocks that fit the SMs (the kernels' __launch_bounds__), none with less than four rows for each
+  // thread
+  const int64_t fit = 148 * (backward ? 2 : 3);
+  const int64_t want = std::max<int64_t>(1, fit / std::max<int64_t>(1, d->samples * g.tiles));
   g.nb = (int)std::max<int64_t>(1, std::min<int64_t>(want, (g.rows + 4 * g.R - 1) / (4 * g.R)));
   g.chunk = ((g.rows + g.nb - 1) / g.nb + g.R - 1) / g.R * g.R;
   if (g.chunk > 0) g.nb = (int)std::max<int64_t>(1, (g.rows + g.chunk - 1) / g.chunk);
   g.blocks = d->samples * g.nb;
-  return g.blocks <= INT32_MAX && g.tiles <= 65535;
+  return g.blocks + g.C <= INT32_MAX && g.tiles <= 65535 && g.chunk / g.R < INT32_MAX;
+}
+
+// Whether a block of 32 elements is 32 / V neighbouring threads' in every tile of rows, so that the forward can write
+// the 8 bits in its own pass over x.
+bool fused_pack(const Plan& pl, size_t elem) {
+  const Geo& g = pl.g;
+  return pl.V * elem == 16 && g.tiles == 1 && g.sample % r4c::q8::kBlock == 0 &&
+         (int64_t)g.R * g.L % r4c::q8::kBlock == 0;
 }
 
 size_t fwd_bytes(const Geo& g) { return align_up((size_t)g.blocks * g.tiles * g.G * sizeof(double2), 256); }
@@ -77,7 +88,7 @@ extern "C" {
 
 size_t r4c_gn_workspace_size(const r4c_gn_desc* desc, int backward) {
   Plan pl;
-  if (!ok_desc(desc) || !make_plan(desc, &pl)) return 0;
+  if (!ok_desc(desc) || !make_plan(desc, backward != 0, &pl)) return 0;
   return backward ? cpart_bytes(pl.g) + gpart_bytes(pl.g) : fwd_bytes(pl.g);
 }
 
@@ -86,7 +97,7 @@ int r4c_gn_fwd(const r4c_gn_desc* desc, const void* x, const void* gamma, const 
   if (!ok_desc(desc)) return R4C_ERR_INVALID;
   if (desc->samples == 0 || desc->inner == 0) return R4C_OK;
   Plan pl;
-  if (!make_plan(desc, &pl)) return R4C_ERR_TOO_LARGE;
+  if (!make_plan(desc, false, &pl)) return R4C_ERR_TOO_LARGE;
   if (!x || !y || !mean_rstd || (codes == nullptr) != (exponents == nullptr)) return R4C_ERR_INVALID;
   if (codes && format != R4C_Q8_INT8 && format != R4C_Q8_E4M3) return R4C_ERR_INVALID;
   if (!aligned(x) || !aligned(y) || !aligned(codes) || !aligned(ws)) return R4C_ERR_ALIGN;
@@ -99,12 +110,16 @@ int r4c_gn_fwd(const r4c_gn_desc* desc, const void* x, const void* gamma, const 
   a.y = y;
   a.mean_rstd = reinterpret_cast<float2*>(mean_rstd);
   a.part = static_cast<double2*>(ws);
+  a.codes = static_cast<uint8_t*>(codes);
+  a.exps = static_cast<uint8_t*>(exponents);
+  pl.g.format = format;
+  pl.g.pack = codes && fused_pack(pl, r4c::dtype_bytes(desc->dtype));
   cudaError_t e;
   if (desc->dtype == R4C_BF16) e = launch_fwd<__nv_bfloat16>(a, pl.g, pl.V, pl.threads, s);
   else if (desc->dtype == R4C_F16) e = launch_fwd<__half>(a, pl.g, pl.V, pl.threads, s);
   else e = launch_fwd<float>(a, pl.g, pl.V, pl.threads, s);
   if (e != cudaSuccess) return status(e);
-  if (codes) return r4c_pack8(x, desc->samples * pl.g.sample, desc->dtype, format, codes, exponents, stream);
+  if (codes && !pl.g.pack) return r4c_pack8(x, desc->samples * pl.g.sample, desc->dtype, format, codes, exponents, stream);
   return R4C_OK;
 }
 
@@ -120,7 +135,7 @@ int r4c_gn_bwd(const r4c_gn_desc* desc, const void* dy, const void* x, int forma
     return R4C_OK;
   }
   Plan pl;
-  if (!make_plan(desc, &pl)) return R4C_ERR_TOO_LARGE;
+  if (!make_plan(desc, true, &pl)) return R4C_ERR_TOO_LARGE;
   if (!dy || !x || !mean_rstd) return R4C_ERR_INVALID;
   if (exponents && format != R4C_Q8_INT8 && format != R4C_Q8_E4M3) return R4C_ERR_INVALID;
   if (!aligned(dy) || !aligned(x) || !aligned(dx) || !aligned(ws)) return R4C_ERR_ALIGN;

@@ -40,31 +40,78 @@ struct Geo {
   int lanes;         // vectors of a row in a channel tile (L / V when there is one tile)
   int tiles;
   int R;             // rows that a block's threads cover at a time
-  int nb;            // blocks of a sample and channel tile
+  int nb;            // blocks of a sample and channel tile (the cluster's, where one keeps a sample)
+  int pack;          // the forward writes x in 8 bits too
 };
 
-// V elements of T, moved as one word.
-template <int B> struct Word;
-template <> struct Word<16> { using type = uint4; };
-template <> struct Word<8> { using type = uint2; };
-template <> struct Word<4> { using type = uint32_t; };
-template <> struct Word<2> { using type = uint16_t; };
+// V elements of T, moved as one word; in fp32 as pairs, for the packed arithmetic (two fp32 an instruction: half the
+// issue slots, which bound these kernels before the memory does).
+template <int V> constexpr int kPairs = (V + 1) / 2;
 
 template <typename T, int V>
 struct Vec {
-  using W = typename Word<V * sizeof(T)>::type;
-  W raw;
-  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const W*>(p); }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<W*>(p) = raw; }
-  __device__ __forceinline__ void to_f(float (&f)[V]) const {
-    const T* p = reinterpret_cast<const T*>(&raw);
+  static constexpr int B = V * (int)sizeof(T);
+  uint32_t w[B >= 4 ? B / 4 : 1];
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = Elem<T>::to_f(p[i]);
+    for (int i = 0; i < (B >= 4 ? B / 4 : 1); ++i) w[i] = 0;
   }
-  __device__ __forceinline__ void from_f(const float (&f)[V]) {
-    T* p = reinterpret_cast<T*>(&raw);
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (B == 16) {
+      const uint4 r = *reinterpret_cast<const uint4*>(p);
+      w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
+    } else if constexpr (B == 8) {
+      const uint2 r = *reinterpret_cast<const uint2*>(p);
+      w[0] = r.x, w[1] = r.y;
+    } else if constexpr (B == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (B == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (B == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (B == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+  }
+  __device__ __forceinline__ void to_f(float2 (&f)[kPairs<V>]) const {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) p[i] = Elem<T>::from_f(f[i]);
+      for (int k = 0; k < V; ++k) (k & 1 ? f[k / 2].y : f[k / 2].x) = __uint_as_float(w[k]);
+      if constexpr (V == 1) f[0].y = 0.f;
+    } else if constexpr (V == 1) {
+      const uint16_t h = (uint16_t)w[0];
+      f[0] = make_float2(Elem<T>::to_f(*reinterpret_cast<const T*>(&h)), 0.f);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) {
+        if constexpr (__is_same(T, __nv_bfloat16))
+          f[k] = make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+        else
+          f[k] = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+      }
+    }
+  }
+  __device__ __forceinline__ void from_f(const float2 (&f)[kPairs<V>]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) w[k] = __float_as_uint(k & 1 ? f[k / 2].y : f[k / 2].x);
+    } else if constexpr (V == 1) {
+      const T h = Elem<T>::from_f(f[0].x);
+      w[0] = *reinterpret_cast<const uint16_t*>(&h);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) {
+        if constexpr (__is_same(T, __nv_bfloat16)) {
+          const __nv_bfloat162 h = __float22bfloat162_rn(f[k]);
+          w[k] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __half2 h = __float22half2_rn(f[k]);
+          w[k] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+    }
   }
 };
 
@@ -74,18 +121,29 @@ struct Source;
 template <typename T, int V>
 struct Source<T, V, false> {
   Vec<T, V> v;
+  __device__ __forceinline__ void zero() { v.zero(); }
   __device__ __forceinline__ void load(const void* x, const uint8_t*, int64_t at) { v.load(static_cast<const T*>(x) + at); }
-  __device__ __forceinline__ void to_f(int, float (&f)[V]) const { v.to_f(f); }
+  __device__ __forceinline__ void to_f(int, float2 (&f)[kPairs<V>]) const { v.to_f(f); }
 };
 template <typename T, int V>
 struct Source<T, V, true> {
   q8::Codes<V> c;
   int byte;
+  __device__ __forceinline__ void zero() {
+    c.w[0] = 0;
+    if constexpr (V > 4) c.w[1] = 0;
+    byte = 0;
+  }
   __device__ __forceinline__ void load(const void* x, const uint8_t* exps, int64_t at) {
     c = q8::load_codes<V>(static_cast<const uint8_t*>(x) + at);
     byte = exps[at / q8::kBlock];
   }
-  __device__ __forceinline__ void to_f(int format, float (&f)[V]) const { q8::decode<T, V>(c, byte, format, f); }
+  __device__ __forceinline__ void to_f(int format, float2 (&f)[kPairs<V>]) const {
+    float e[V];
+    q8::decode<T, V>(c, byte, format, e);
+#pragma unroll
+    for (int k = 0; k < kPairs<V>; ++k) f[k] = make_float2(e[2 * k], V > 1 ? e[V > 1 ? 2 * k + 1 : 0] : 0.f);
+  }
 };
 
 __device__ __forceinline__ float param(const void* p, int dtype, int c, float none) {
@@ -95,48 +153,135 @@ __device__ __forceinline__ float param(const void* p, int dtype, int c, float no
   return __half2float(static_cast<const __half*>(p)[c]);
 }
 
+__device__ __forceinline__ float2 two(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // 1 / (1 + e^-z): for 16-bit results the hardware's exponential and reciprocal (relative error about 2^-21, the
 // result's own half step is 2^-9 or 2^-12), the library's in full precision for fp32.
 template <typename T>
-__device__ __forceinline__ float sigmoid(float z) {
-  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-z));
-  return __fdividef(1.f, 1.f + __expf(-z));
-}
-
-template <typename T>
-__device__ __forceinline__ float act_value(float z, int act, float slope) {
-  switch (act) {
-    case R4C_ACT_RELU: return z <= 0.f ? 0.f : z;              // NaN stays
-    case R4C_ACT_LEAKY_RELU: return z <= 0.f ? z * slope : z;
-    case R4C_ACT_SILU: return z * sigmoid<T>(z);
-    case R4C_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678f));
-    default: return z;
-  }
-}
-template <typename T>
-__device__ __forceinline__ float act_slope(float z, int act, float slope) {
-  switch (act) {
-    case R4C_ACT_RELU: return z <= 0.f ? 0.f : 1.f;
-    case R4C_ACT_LEAKY_RELU: return z <= 0.f ? slope : 1.f;
-    case R4C_ACT_SILU: {
-      const float s = sigmoid<T>(z);
-      return s * fmaf(z, 1.f - s, 1.f);
-    }
-    case R4C_ACT_GELU: {
-      const float e = sizeof(T) == 4 ? expf(-0.5f * z * z) : __expf(-0.5f * z * z);
-      return fmaf(z, e * 0.39894228f, 0.5f * (1.f + erff(z * 0.70710678f)));
-    }
-    default: return 1.f;
+__device__ __forceinline__ float2 sigmoid(float2 z) {
+  if constexpr (sizeof(T) == 4) {
+    return make_float2(1.f / (1.f + expf(-z.x)), 1.f / (1.f + expf(-z.y)));
+  } else {
+    const float2 t = __fmul2_rn(z, two(-1.44269504f));
+    const float2 e = __fadd2_rn(make_float2(ex2(t.x), ex2(t.y)), two(1.f));
+    return make_float2(rcp(e.x), rcp(e.y));
   }
 }
 
-// Where a block's threads stand: sample n, part b of it, channel tile, and a thread's lane and row.
+// Phi(z) and e^(-z^2/2). 16-bit results: the rational approximation 7.1.26 of Abramowitz and Stegun's Handbook,
+// erfc(u) = (a1 t + .. + a5 t^5) e^(-u^2), t = 1 / (1 + 0.3275911 u), off by at most 1.5e-7; fp32 results: erff.
+template <typename T>
+__device__ __forceinline__ void normal(float2 z, float2& phi, float2& e) {
+  if constexpr (sizeof(T) == 4) {
+    e = make_float2(expf(-0.5f * z.x * z.x), expf(-0.5f * z.y * z.y));
+    phi = make_float2(0.5f * (1.f + erff(z.x * 0.70710678f)), 0.5f * (1.f + erff(z.y * 0.70710678f)));
+  } else {
+    const float2 q = __fmul2_rn(__fmul2_rn(z, z), two(-0.72134752f));
+    e = make_float2(ex2(q.x), ex2(q.y));
+    const float2 d = __ffma2_rn(make_float2(fabsf(z.x), fabsf(z.y)), two(0.23164190f), two(1.f));
+    const float2 t = make_float2(rcp(d.x), rcp(d.y));
+    // halves of a5 .. a1: half of erfc
+    float2 p = __ffma2_rn(t, two(0.530702715f), two(-0.726576014f));
+    p = __ffma2_rn(p, t, two(0.710706871f));
+    p = __ffma2_rn(p, t, two(-0.142248368f));
+    p = __ffma2_rn(p, t, two(0.127414796f));
+    p = __fmul2_rn(__fmul2_rn(p, t), e);
+    const float2 c = __ffma2_rn(p, two(-1.f), two(1.f));
+    phi = make_float2(z.x < 0.f ? p.x : c.x, z.y < 0.f ? p.y : c.y);
+    if (!(fabsf(z.x) < INFINITY)) phi.x = z.x - z.x;           // NaN and infinities: as z * NaN
+    if (!(fabsf(z.y) < INFINITY)) phi.y = z.y - z.y;
+  }
+}
+
+// ACT: the activation, or -1: read from the descriptor (narrow vectors, which are rare: one kernel for all).
+template <typename T, int ACT>
+__device__ __forceinline__ float2 act_value(float2 z, float slope) {
+  if constexpr (ACT == R4C_ACT_RELU) return make_float2(z.x <= 0.f ? 0.f : z.x, z.y <= 0.f ? 0.f : z.y);   // NaN stays
+  if constexpr (ACT == R4C_ACT_LEAKY_RELU) {
+    const float2 s = __fmul2_rn(z, two(slope));
+    return make_float2(z.x <= 0.f ? s.x : z.x, z.y <= 0.f ? s.y : z.y);
+  }
+  if constexpr (ACT == R4C_ACT_SILU) return __fmul2_rn(z, sigmoid<T>(z));
+  if constexpr (ACT == R4C_ACT_GELU) {
+    float2 phi, e;
+    normal<T>(z, phi, e);
+    return __fmul2_rn(z, phi);
+  }
+  return z;
+}
+// dy * act'(z)
+template <typename T, int ACT>
+__device__ __forceinline__ float2 act_grad(float2 dy, float2 z, float slope) {
+  if constexpr (ACT == R4C_ACT_RELU) return make_float2(z.x <= 0.f ? 0.f : dy.x, z.y <= 0.f ? 0.f : dy.y);
+  if constexpr (ACT == R4C_ACT_LEAKY_RELU) {
+    const float2 s = __fmul2_rn(dy, two(slope));
+    return make_float2(z.x <= 0.f ? s.x : dy.x, z.y <= 0.f ? s.y : dy.y);
+  }
+  if constexpr (ACT == R4C_ACT_SILU) {
+    const float2 s = sigmoid<T>(z);
+    // s (1 + z (1 - s))
+    return __fmul2_rn(__fmul2_rn(dy, s), __ffma2_rn(z, __ffma2_rn(s, two(-1.f), two(1.f)), two(1.f)));
+  }
+  if constexpr (ACT == R4C_ACT_GELU) {
+    float2 phi, e;
+    normal<T>(z, phi, e);
+    return __fmul2_rn(dy, __ffma2_rn(__fmul2_rn(z, e), two(0.39894228f), phi));
+  }
+  return dy;
+}
+template <typename T, int ACT, int P>
+__device__ __forceinline__ void act_values(float2 (&z)[P], int act, float slope) {
+  if constexpr (ACT >= 0) {
+#pragma unroll
+    for (int k = 0; k < P; ++k) z[k] = act_value<T, ACT>(z[k], slope);
+  } else {
+    switch (act) {
+      case R4C_ACT_RELU: act_values<T, R4C_ACT_RELU>(z, act, slope); break;
+      case R4C_ACT_LEAKY_RELU: act_values<T, R4C_ACT_LEAKY_RELU>(z, act, slope); break;
+      case R4C_ACT_SILU: act_values<T, R4C_ACT_SILU>(z, act, slope); break;
+      case R4C_ACT_GELU: act_values<T, R4C_ACT_GELU>(z, act, slope); break;
+    }
+  }
+}
+// dy becomes dy * act'(z)
+template <typename T, int ACT, int P>
+__device__ __forceinline__ void act_grads(float2 (&dy)[P], const float2 (&z)[P], int act, float slope) {
+  if constexpr (ACT >= 0) {
+#pragma unroll
+    for (int k = 0; k < P; ++k) dy[k] = act_grad<T, ACT>(dy[k], z[k], slope);
+  } else {
+    switch (act) {
+      case R4C_ACT_RELU: act_grads<T, R4C_ACT_RELU>(dy, z, act, slope); break;
+      case R4C_ACT_LEAKY_RELU: act_grads<T, R4C_ACT_LEAKY_RELU>(dy, z, act, slope); break;
+      case R4C_ACT_SILU: act_grads<T, R4C_ACT_SILU>(dy, z, act, slope); break;
+      case R4C_ACT_GELU: act_grads<T, R4C_ACT_GELU>(dy, z, act, slope); break;
+    }
+  }
+}
+
+// Where a block's threads stand: sample n, part b of it, channel tile, and a thread's lane and row; its rows are
+// row, row + R, .. of the block's `count` tiles of R rows from r0 on.
 struct Place {
-  int64_t n;
+  int64_t n, r0, left;  // left: rows of the block
+  int64_t at;           // the thread's first element
+  int64_t step;         // elements from one tile to the next
+  int tiles;            // of R rows
   int b, tile, lane, row;
-  int j0, j1;         // the tile's elements of a row
-  int ga, gb;         // the tile's groups
+  int j0, j1;           // the channel tile's elements of a row
+  int ga, gb;           // its groups
   bool active;
+  // whether tile t holds a row for this thread
+  __device__ __forceinline__ bool in(int t, int R) const { return active && (int64_t)t * R + row < left; }
 };
 template <int V>
 __device__ __forceinline__ Place place(const Geo& g) {
@@ -151,6 +296,11 @@ __device__ __forceinline__ Place place(const Geo& g) {
   p.ga = g.tiles == 1 ? 0 : p.j0 / g.Cg;
   p.gb = g.tiles == 1 ? g.G : (p.j1 - 1) / g.Cg + 1;
   p.active = p.row < g.R && p.j0 + p.lane * V < p.j1;
+  p.r0 = p.b * g.chunk;
+  p.left = min(g.chunk, g.rows - p.r0);
+  p.tiles = p.left > 0 ? (int)((p.left + g.R - 1) / g.R) : 0;
+  p.at = p.n * g.sample + (p.r0 + p.row) * g.L + p.j0 + p.lane * V;
+  p.step = (int64_t)g.R * g.L;
   return p;
 }
 
@@ -160,161 +310,229 @@ __device__ __forceinline__ int threads_per(int items, int threads) {
   while (t > 1 && t * items > threads) t >>= 1;
   return t;
 }
+template <typename S>
+__device__ __forceinline__ void join(S& a, S& b, int width) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (o < width) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+  }
+}
+
+// f(item, a, c) -> adds item's terms of thread `sub` of `tp`; g(item, a, c) gets the sums. Every thread of the block
+// calls it (the shuffles need whole warps; blocks are multiples of 32 threads).
+template <typename S, typename F, typename Out>
+__device__ __forceinline__ void each_sum(int items, F f, Out out) {
+  const int tp = threads_per(items, blockDim.x), sub = threadIdx.x % tp, per = blockDim.x / tp;
+  for (int base = 0; base < items; base += per) {
+    const int i = base + threadIdx.x / tp;
+    S a = 0, c = 0;
+    if (i < items) f(i, sub, tp, a, c);
+    join(a, c, tp);
+    if (i < items && sub == 0) out(i, a, c);
+  }
+}
+
+// Launched while the kernel before it may still run: what that one wrote may be read from here on.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// The thread's mean (negated), rstd * w and b.
+template <int V>
+struct Affine {
+  float2 nmu[kPairs<V>], a[kPairs<V>], b[kPairs<V>];
+  template <typename Stat>
+  __device__ __forceinline__ void load(const Geo& g, const Place& p, const void* gamma, const void* beta, Stat stat) {
+#pragma unroll
+    for (int k = 0; k < 2 * kPairs<V>; ++k) {
+      float m = 0.f, s = 0.f, t = 0.f;
+      if (k < V) {
+        const int c = (p.j0 + p.lane * V + k) % g.C;
+        const float2 q = stat(c / g.Cg);
+        m = -q.x;
+        s = q.y * param(gamma, g.pdtype, c, 1.f);
+        t = param(beta, g.pdtype, c, 0.f);
+      }
+      (k & 1 ? nmu[k / 2].y : nmu[k / 2].x) = m;
+      (k & 1 ? a[k / 2].y : a[k / 2].x) = s;
+      (k & 1 ? b[k / 2].y : b[k / 2].x) = t;
+    }
+  }
+};
 
 // ---------------------------------------------------------------------------
-// Forward: sums
+// Forward
 // ---------------------------------------------------------------------------
+// A thread's sums around its first value.
+template <typename T, int V>
+struct Moments {
+  float2 np[kPairs<V>], s1[kPairs<V>], s2[kPairs<V>];
+  int count;
+  __device__ __forceinline__ void zero() {
+    count = 0;
+#pragma unroll
+    for (int k = 0; k < kPairs<V>; ++k) np[k] = s1[k] = s2[k] = two(0.f);
+  }
+  __device__ __forceinline__ void pivot(const Vec<T, V>& v) {
+    v.to_f(np);
+#pragma unroll
+    for (int k = 0; k < kPairs<V>; ++k) np[k] = __fmul2_rn(np[k], two(-1.f));
+  }
+  __device__ __forceinline__ void add(const Vec<T, V>& v) {
+    float2 f[kPairs<V>];
+    v.to_f(f);
+    ++count;
+#pragma unroll
+    for (int k = 0; k < kPairs<V>; ++k) {
+      const float2 d = __fadd2_rn(f[k], np[k]);
+      s1[k] = __fadd2_rn(s1[k], d);
+      s2[k] = __ffma2_rn(d, d, s2[k]);
+    }
+  }
+  // (sum x, sum x^2) of column k in fp64
+  __device__ __forceinline__ double2 sums(int k) const {
+    const double q = -(double)(k & 1 ? np[k / 2].y : np[k / 2].x), a = k & 1 ? s1[k / 2].y : s1[k / 2].x;
+    const double s = k & 1 ? s2[k / 2].y : s2[k / 2].x, c = count;
+    return make_double2(c * q + a, s + 2.0 * q * a + c * q * q);
+  }
+};
+
+// The block's sums of each of its groups: out(group, sum x, sum x^2).
+template <typename T, int V, typename Out>
+__device__ __forceinline__ void block_moments(const Geo& g, const Place& p, const Moments<T, V>& m,
+                                              double2* __restrict__ red, Out out) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) red[k * kThreads + threadIdx.x] = m.sums(k);
+  __syncthreads();
+  const int reps = g.L / g.C;
+  each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
+    const int gi = p.ga + i;
+    const int lo = max(gi * g.Cg, g.tiles == 1 ? 0 : p.j0), hi = min((gi + 1) * g.Cg, g.tiles == 1 ? g.C : p.j1);
+    const int w = hi - lo, total = reps * w * g.R;
+    for (int e = sub; e < total; e += tp) {
+      const int row = e % g.R, q = e / g.R;
+      const int j = (q / w) * g.C + lo + q % w - p.j0;
+      const double2 v = red[(j % V) * kThreads + row * g.lanes + j / V];
+      a += v.x;
+      c += v.y;
+    }
+  }, [&](int i, double a, double c) { out(p.ga + i, a, c); });
+}
+
+__device__ __forceinline__ float2 mean_rstd_of(const Geo& g, double a, double c) {
+  const double mean = a * g.inv_m;
+  double var = c * g.inv_m - mean * mean;
+  if (var < 0.0) var = 0.0;
+  return make_float2((float)mean, (float)(1.0 / sqrt(var + (double)g.eps)));
+}
+
 // part[((n * nb + b) * tiles + tile) * G + g] = (sum x, sum x^2) of the block's share of group g.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) stats_kernel(const T* __restrict__ x, const Geo g,
-                                                         double2* __restrict__ part) {
+__global__ void __launch_bounds__(kThreads, 4) stats_kernel(const T* __restrict__ x, const __grid_constant__ Geo g,
+                                                            double2* __restrict__ part) {
   constexpr int U = 4;
   __shared__ double2 red[V * kThreads];
+  let_next_start();
   const Place p = place<V>(g);
-  const int64_t r0 = p.b * g.chunk, r1 = min(r0 + g.chunk, g.rows);
-  float s1[V], s2[V], pv[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) s1[k] = s2[k] = pv[k] = 0.f;
-  int cnt = 0;
-  if (p.active && r0 + p.row < r1) {
-    const T* src = x + p.n * g.sample + p.j0 + p.lane * V;
+  Moments<T, V> m;
+  m.zero();
+  if (p.in(0, g.R)) {
+    const T* src = x + p.at;
     {
       Vec<T, V> a;
-      a.load(src + (r0 + p.row) * g.L);
-      a.to_f(pv);
+      a.load(src);
+      m.pivot(a);
     }
-    for (int64_t r = r0 + p.row; r < r1; r += U * g.R) {
+    int t = 0;
+    for (; t + U < p.tiles; t += U, src += U * p.step) {      // whole tiles: the last one comes below
       Vec<T, V> a[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (r + u * g.R < r1) a[u].load(src + (r + u * g.R) * g.L);
+      for (int u = 0; u < U; ++u) a[u].load(src + u * p.step);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (r + u * g.R >= r1) break;
-        float f[V];
-        a[u].to_f(f);
-        ++cnt;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float d = f[k] - pv[k];
-          s1[k] += d;
-          s2[k] = fmaf(d, d, s2[k]);
-        }
-      }
+      for (int u = 0; u < U; ++u) m.add(a[u]);
     }
+    for (; t < p.tiles; ++t, src += p.step)
+      if (p.in(t, g.R)) {
+        Vec<T, V> a;
+        a.load(src);
+        m.add(a);
+      }
   }
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const double q = pv[k], a = s1[k], c = cnt;
-    red[k * kThreads + threadIdx.x] = make_double2(c * q + a, (double)s2[k] + 2.0 * q * a + c * q * q);
-  }
-  __syncthreads();
-  const int groups = p.gb - p.ga, tp = threads_per(groups, blockDim.x);
-  const int sub = threadIdx.x % tp;
   double2* out = part + ((int64_t)blockIdx.x * g.tiles + p.tile) * g.G;
   if (g.tiles > 1)
     for (int i = threadIdx.x; i < g.G; i += blockDim.x)
       if (i < p.ga || i >= p.gb) out[i] = make_double2(0.0, 0.0);
-  const int reps = g.L / g.C;
-  // the loop bound is the same for every thread of a warp: the shuffles below need all lanes
-  for (int base = 0; base < groups; base += blockDim.x / tp) {
-    const int gi = p.ga + base + threadIdx.x / tp;
-    double a = 0.0, c = 0.0;
-    if (gi < p.gb && threadIdx.x / tp < blockDim.x / tp) {
-      const int lo = max(gi * g.Cg, g.tiles == 1 ? 0 : p.j0), hi = min((gi + 1) * g.Cg, g.tiles == 1 ? g.C : p.j1);
-      const int w = hi - lo, total = reps * w * g.R;
-      for (int e = sub; e < total; e += tp) {
-        const int row = e % g.R, q = e / g.R;
-        const int j = (q / w) * g.C + lo + q % w - p.j0;
-        const double2 v = red[(j % V) * kThreads + row * g.lanes + j / V];
-        a += v.x;
-        c += v.y;
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      if (o < tp) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        c += __shfl_xor_sync(0xffffffffu, c, o);
-      }
-    }
-    if (sub == 0 && gi < p.gb && threadIdx.x / tp < blockDim.x / tp) out[gi] = make_double2(a, c);
-  }
+  block_moments<T, V>(g, p, m, red, [&](int gi, double a, double c) { out[gi] = make_double2(a, c); });
 }
 
-// ---------------------------------------------------------------------------
-// Forward: y
-// ---------------------------------------------------------------------------
-// Mean and rstd of the tile's groups from the blocks' partial sums, into shared memory.
-__device__ __forceinline__ void finish_stats(const Geo& g, const Place& p, const double2* __restrict__ part,
-                                             float2* stat) {
-  const int groups = p.gb - p.ga, tp = threads_per(groups, blockDim.x), sub = threadIdx.x % tp;
-  const int np = g.nb * g.tiles;
-  const double2* src = part + p.n * np * g.G;
-  for (int base = 0; base < groups; base += blockDim.x / tp) {
-    const int gi = p.ga + base + threadIdx.x / tp;
-    const bool own = gi < p.gb && threadIdx.x / tp < blockDim.x / tp;
-    double a = 0.0, c = 0.0;
-    if (own)
-      for (int i = sub; i < np; i += tp) {
-        const double2 v = src[(int64_t)i * g.G + gi];
-        a += v.x;
-        c += v.y;
-      }
+// y of one vector, and its 8 bits (PACK: a block of 32 elements lies in 32 / V neighbouring threads, all with or all
+// without a row here; every thread of the warp calls it).
+template <typename T, int V, int ACT, bool PACK>
+__device__ __forceinline__ void apply_one(const Vec<T, V>& v, const Affine<V>& k, const Geo& g, bool in, int64_t at,
+                                          T* __restrict__ y, uint8_t* __restrict__ codes,
+                                          uint8_t* __restrict__ exps) {
+  float2 f[kPairs<V>];
+  v.to_f(f);
+  if constexpr (PACK) {
+    float e[V];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      if (o < tp) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        c += __shfl_xor_sync(0xffffffffu, c, o);
-      }
-    }
-    if (own && sub == 0) {
-      const double mean = a * g.inv_m;
-      double var = c * g.inv_m - mean * mean;
-      if (var < 0.0) var = 0.0;
-      stat[gi - p.ga] = make_float2((float)mean, (float)(1.0 / sqrt(var + (double)g.eps)));
+    for (int i = 0; i < V; ++i) e[i] = i & 1 ? f[i / 2].y : f[i / 2].x;
+    bool finite;
+    const int byte = q8::exponent_byte(q8::block_amax<V>(e, 0xffffffffu, &finite), g.format);
+    const q8::Codes<V> c = q8::encode<V>(e, byte, g.format, finite);
+    if (in) {
+      q8::store_codes<V>(codes + at, c);
+      if (at % q8::kBlock == 0) exps[at / q8::kBlock] = (uint8_t)byte;
     }
   }
-  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) f[i] = __ffma2_rn(__fadd2_rn(f[i], k.nmu[i]), k.a[i], k.b[i]);
+  act_values<T, ACT>(f, g.act, g.slope);
+  Vec<T, V> r;
+  r.from_f(f);
+  if (in) r.store(y + at);
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) apply_kernel(const T* __restrict__ x, const void* __restrict__ gamma,
-                                                         const void* __restrict__ beta, const Geo g,
-                                                         const double2* __restrict__ part,
-                                                         float2* __restrict__ mean_rstd, T* __restrict__ y) {
+// From the last row to the first: what the sums read last is what the L2 cache still has.
+template <typename T, int V, int ACT, bool PACK>
+__global__ void __launch_bounds__(kThreads, 3) apply_kernel(const T* __restrict__ x, const void* __restrict__ gamma,
+                                                            const void* __restrict__ beta,
+                                                            const __grid_constant__ Geo g,
+                                                            const double2* __restrict__ part,
+                                                            float2* __restrict__ mean_rstd, T* __restrict__ y,
+                                                            uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
   constexpr int U = 4;
   extern __shared__ float2 stat[];
   const Place p = place<V>(g);
-  finish_stats(g, p, part, stat);
+  wait_for_previous();
+  const int np = g.nb * g.tiles;
+  const double2* src = part + p.n * np * g.G + p.ga;
+  each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
+#pragma unroll 4
+    for (int e = sub; e < np; e += tp) {
+      const double2 v = src[(int64_t)e * g.G + i];
+      a += v.x;
+      c += v.y;
+    }
+  }, [&](int i, double a, double c) { stat[i] = mean_rstd_of(g, a, c); });
+  __syncthreads();
   if (p.b == 0)
     for (int i = threadIdx.x; i < p.gb - p.ga; i += blockDim.x) mean_rstd[p.n * g.G + p.ga + i] = stat[i];
-  if (!p.active) return;
-  float mu[V], a[V], b[V];
-  const int j = p.j0 + p.lane * V;
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int c = (j + k) % g.C;
-    const float2 s = stat[c / g.Cg - p.ga];
-    mu[k] = s.x;
-    a[k] = s.y * param(gamma, g.pdtype, c, 1.f);
-    b[k] = param(beta, g.pdtype, c, 0.f);
-  }
-  const int64_t r0 = p.b * g.chunk, r1 = min(r0 + g.chunk, g.rows), at = p.n * g.sample + j;
-  for (int64_t r = r0 + p.row; r < r1; r += U * g.R) {
+  Affine<V> k;
+  if (p.active) k.load(g, p, gamma, beta, [&](int gi) { return stat[gi - p.ga]; });
+  for (int t = p.tiles - 1; t >= 0; t -= U) {
     Vec<T, V> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (r + u * g.R < r1) v[u].load(x + at + (r + u * g.R) * g.L);
+    for (int u = 0; u < U; ++u) {
+      v[u].zero();
+      if (t - u >= 0 && p.in(t - u, g.R)) v[u].load(x + p.at + (t - u) * p.step);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (r + u * g.R >= r1) break;
-      float f[V];
-      v[u].to_f(f);
-#pragma unroll
-      for (int k = 0; k < V; ++k) f[k] = act_value<T>(fmaf(f[k] - mu[k], a[k], b[k]), g.act, g.slope);
-      v[u].from_f(f);
-      v[u].store(y + at + (r + u * g.R) * g.L);
+      if (t - u < 0) break;
+      apply_one<T, V, ACT, PACK>(v[u], k, g, p.in(t - u, g.R), p.at + (t - u) * p.step, y, codes, exps);
     }
   }
 }
@@ -322,217 +540,220 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const T* __restrict__ x
 // ---------------------------------------------------------------------------
 // Backward: sums
 // ---------------------------------------------------------------------------
+// dz and x - mean of one vector.
+template <typename T, int V, int ACT, bool Q>
+__device__ __forceinline__ void grad_one(const Source<T, V, Q>& v, const Vec<T, V>& d, const Affine<V>& k, const Geo& g,
+                                         float2 (&xm)[kPairs<V>], float2 (&dz)[kPairs<V>]) {
+  v.to_f(g.format, xm);
+  d.to_f(dz);
+  float2 z[kPairs<V>];
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) {
+    xm[i] = __fadd2_rn(xm[i], k.nmu[i]);
+    z[i] = __ffma2_rn(xm[i], k.a[i], k.b[i]);
+  }
+  act_grads<T, ACT>(dz, z, g.act, g.slope);
+}
+
+// The block's (sum dz, sum dz * (x - mean)) of a thread's columns: cpart gets them per channel (the second times rstd),
+// out(group, ..) the same times w, summed over the tile's channels of the group.
+template <int V, typename Stat, typename Out>
+__device__ __forceinline__ void block_grads(const Geo& g, const Place& p, const float2 (&s1)[kPairs<V>],
+                                            const float2 (&s2)[kPairs<V>], const void* gamma, float2* __restrict__ red,
+                                            float2* __restrict__ cols, float2* __restrict__ cpart, Stat stat, Out out) {
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+    red[k * kThreads + threadIdx.x] = k & 1 ? make_float2(s1[k / 2].y, s2[k / 2].y) : make_float2(s1[k / 2].x, s2[k / 2].x);
+  __syncthreads();
+  const int ncol = p.j1 - p.j0, reps = g.L / g.C, nch = g.tiles == 1 ? g.C : ncol;
+  each_sum<float>(nch, [&](int i, int sub, int tp, float& a, float& c) {
+    for (int e = sub; e < reps * g.R; e += tp) {
+      const int j = (e / g.R) * g.C + i;
+      const float2 v = red[(j % V) * kThreads + (e % g.R) * g.lanes + j / V];
+      a += v.x;
+      c += v.y;
+    }
+  }, [&](int i, float a, float c) {
+    const int ch = p.j0 + i;
+    const float2 s = make_float2(a, c * stat(ch / g.Cg).y);
+    cols[i] = s;
+    cpart[(int64_t)blockIdx.x * g.C + ch] = s;
+  });
+  __syncthreads();
+  each_sum<float>(p.gb - p.ga, [&](int i, int sub, int tp, float& a, float& c) {
+    const int lo = max((p.ga + i) * g.Cg, p.j0), hi = min((p.ga + i + 1) * g.Cg, p.j0 + nch);
+    for (int ch = lo + sub; ch < hi; ch += tp) {
+      const float w = param(gamma, g.pdtype, ch, 1.f);
+      a = fmaf(w, cols[ch - p.j0].x, a);
+      c = fmaf(w, cols[ch - p.j0].y, c);
+    }
+  }, [&](int i, float a, float c) { out(p.ga + i, a, c); });
+}
+
 // cpart[(n * nb + b) * C + c] = (sum dz, sum dz * xh) of the block's rows, and
 // gpart[((n * nb + b) * tiles + tile) * G + g] = the same times w, summed over the tile's channels of the group.
-template <typename T, int V, bool Q>
-__global__ void __launch_bounds__(kThreads) bwd_sums_kernel(const T* __restrict__ dy, const void* __restrict__ x,
-                                                            const uint8_t* __restrict__ exps,
-                                                            const float2* __restrict__ mean_rstd,
-                                                            const void* __restrict__ gamma,
-                                                            const void* __restrict__ beta, const Geo g,
-                                                            float2* __restrict__ cpart, float2* __restrict__ gpart) {
+template <typename T, int V, int ACT, bool Q>
+__global__ void __launch_bounds__(kThreads, 2) bwd_sums_kernel(const T* __restrict__ dy, const void* __restrict__ x,
+                                                               const uint8_t* __restrict__ exps,
+                                                               const float2* __restrict__ mean_rstd,
+                                                               const void* __restrict__ gamma,
+                                                               const void* __restrict__ beta,
+                                                               const __grid_constant__ Geo g,
+                                                               float2* __restrict__ cpart, float2* __restrict__ gpart) {
   constexpr int U = 4;
   __shared__ float2 red[V * kThreads];
-  __shared__ float2 cols[V * kThreads];     // per column of the tile, (j1 - j0) <= V * kThreads
+  __shared__ float2 cols[V * kThreads];     // per channel of the tile
+  let_next_start();
   const Place p = place<V>(g);
-  const int64_t r0 = p.b * g.chunk, r1 = min(r0 + g.chunk, g.rows);
-  float s1[V], s2[V];
+  const float2* stats = mean_rstd + p.n * g.G;
+  float2 s1[kPairs<V>], s2[kPairs<V>];
 #pragma unroll
-  for (int k = 0; k < V; ++k) s1[k] = s2[k] = 0.f;
-  if (p.active) {
-    float mu[V], a[V], b[V], rs[V];
-    const int j = p.j0 + p.lane * V;
+  for (int k = 0; k < kPairs<V>; ++k) s1[k] = s2[k] = two(0.f);
+  if (p.in(0, g.R)) {
+    Affine<V> k;
+    k.load(g, p, gamma, beta, [&](int gi) { return stats[gi]; });
+    auto add = [&](const Source<T, V, Q>& v, const Vec<T, V>& d) {
+      float2 xm[kPairs<V>], dz[kPairs<V>];
+      grad_one<T, V, ACT, Q>(v, d, k, g, xm, dz);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = (j + k) % g.C;
-      const float2 s = mean_rstd[p.n * g.G + c / g.Cg];
-      mu[k] = s.x;
-      rs[k] = s.y;
-      a[k] = s.y * param(gamma, g.pdtype, c, 1.f);
-      b[k] = param(beta, g.pdtype, c, 0.f);
-    }
-    const int64_t at = p.n * g.sample + j;
-    for (int64_t r = r0 + p.row; r < r1; r += U * g.R) {
+      for (int i = 0; i < kPairs<V>; ++i) {
+        s1[i] = __fadd2_rn(s1[i], dz[i]);
+        s2[i] = __ffma2_rn(dz[i], xm[i], s2[i]);
+      }
+    };
+    int t = 0;
+    int64_t at = p.at;
+    for (; t + U < p.tiles; t += U, at += U * p.step) {        // whole tiles: the last one comes below
       Source<T, V, Q> v[U];
       Vec<T, V> d[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (r + u * g.R < r1) {
-          v[u].load(x, exps, at + (r + u * g.R) * g.L);
-          d[u].load(dy + at + (r + u * g.R) * g.L);
-        }
-#pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (r + u * g.R >= r1) break;
-        float f[V], h[V];
-        v[u].to_f(g.format, f);
-        d[u].to_f(h);
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float xm = f[k] - mu[k];
-          const float dz = h[k] * act_slope<T>(fmaf(xm, a[k], b[k]), g.act, g.slope);
-          s1[k] += dz;
-          s2[k] = fmaf(dz, xm, s2[k]);
-        }
+        v[u].load(x, exps, at + u * p.step);
+        d[u].load(dy + at + u * p.step);
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(v[u], d[u]);
     }
-#pragma unroll
-    for (int k = 0; k < V; ++k) s2[k] *= rs[k];
-  }
-#pragma unroll
-  for (int k = 0; k < V; ++k) red[k * kThreads + threadIdx.x] = make_float2(s1[k], s2[k]);
-  __syncthreads();
-  const int ncol = p.j1 - p.j0;
-  {
-    const int tp = threads_per(ncol, blockDim.x), sub = threadIdx.x % tp;
-    for (int base = 0; base < ncol; base += blockDim.x / tp) {
-      const int j = base + threadIdx.x / tp;
-      const bool own = j < ncol && threadIdx.x / tp < blockDim.x / tp;
-      float u = 0.f, v = 0.f;
-      if (own)
-        for (int r = sub; r < g.R; r += tp) {
-          const float2 e = red[(j % V) * kThreads + r * g.lanes + j / V];
-          u += e.x;
-          v += e.y;
-        }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        if (o < tp) {
-          u += __shfl_xor_sync(0xffffffffu, u, o);
-          v += __shfl_xor_sync(0xffffffffu, v, o);
-        }
+    for (; t < p.tiles; ++t, at += p.step)
+      if (p.in(t, g.R)) {
+        Source<T, V, Q> v;
+        Vec<T, V> d;
+        v.load(x, exps, at);
+        d.load(dy + at);
+        add(v, d);
       }
-      if (own && sub == 0) cols[j] = make_float2(u, v);
-    }
   }
-  __syncthreads();
-  const int reps = g.L / g.C, nch = g.tiles == 1 ? g.C : ncol;
-  for (int i = threadIdx.x; i < nch; i += blockDim.x) {
-    float2 s = cols[i];
-    for (int q = 1; q < reps; ++q) {
-      const float2 e = cols[q * g.C + i];
-      s.x += e.x;
-      s.y += e.y;
-    }
-    cols[i] = s;                            // columns of one channel are this thread's alone
-    cpart[(int64_t)blockIdx.x * g.C + p.j0 + i] = s;
-  }
-  __syncthreads();
   float2* out = gpart + ((int64_t)blockIdx.x * g.tiles + p.tile) * g.G;
-  for (int i = threadIdx.x; i < g.G; i += blockDim.x) {
-    float u = 0.f, v = 0.f;
-    const int lo = max(i * g.Cg, p.j0), hi = min((i + 1) * g.Cg, p.j0 + nch);
-    for (int c = lo; c < hi; ++c) {
-      const float w = param(gamma, g.pdtype, c, 1.f);
-      u = fmaf(w, cols[c - p.j0].x, u);
-      v = fmaf(w, cols[c - p.j0].y, v);
-    }
-    out[i] = make_float2(u, v);
-  }
+  if (g.tiles > 1)
+    for (int i = threadIdx.x; i < g.G; i += blockDim.x)
+      if (i < p.ga || i >= p.gb) out[i] = make_float2(0.f, 0.f);
+  block_grads<V>(g, p, s1, s2, gamma, red, cols, cpart, [&](int gi) { return stats[gi]; },
+                 [&](int gi, float a, float c) { out[gi] = make_float2(a, c); });
 }
 
 // ---------------------------------------------------------------------------
 // Backward: dx, and the gradients of weight and bias
 // ---------------------------------------------------------------------------
-template <typename T, int V, bool Q>
-__global__ void __launch_bounds__(kThreads) bwd_dx_kernel(const T* __restrict__ dy, const void* __restrict__ x,
-                                                          const uint8_t* __restrict__ exps,
-                                                          const float2* __restrict__ mean_rstd,
-                                                          const void* __restrict__ gamma,
-                                                          const void* __restrict__ beta, const Geo g,
-                                                          const float2* __restrict__ gpart, T* __restrict__ dx) {
-  constexpr int U = 4;
-  extern __shared__ float2 coef[];          // per group of the tile: rstd * A, rstd^2 * B
-  const Place p = place<V>(g);
-  {
-    const int groups = p.gb - p.ga, tp = threads_per(groups, blockDim.x), sub = threadIdx.x % tp;
-    const int np = g.nb * g.tiles;
-    const float2* src = gpart + p.n * np * g.G;
-    for (int base = 0; base < groups; base += blockDim.x / tp) {
-      const int gi = p.ga + base + threadIdx.x / tp;
-      const bool own = gi < p.gb && threadIdx.x / tp < blockDim.x / tp;
-      double u = 0.0, v = 0.0;
-      if (own)
-        for (int i = sub; i < np; i += tp) {
-          const float2 e = src[(int64_t)i * g.G + gi];
-          u += e.x;
-          v += e.y;
-        }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        if (o < tp) {
-          u += __shfl_xor_sync(0xffffffffu, u, o);
-          v += __shfl_xor_sync(0xffffffffu, v, o);
-        }
-      }
-      if (own && sub == 0) {
-        const double r = mean_rstd[p.n * g.G + gi].y;
-        coef[gi - p.ga] = make_float2((float)(r * u * g.inv_m), (float)(r * r * v * g.inv_m));
-      }
-    }
-    __syncthreads();
-  }
-  if (!p.active) return;
-  float mu[V], a[V], b[V], k1[V], k2[V];
-  const int j = p.j0 + p.lane * V;
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int c = (j + k) % g.C;
-    const float2 s = mean_rstd[p.n * g.G + c / g.Cg];
-    const float2 q = coef[c / g.Cg - p.ga];
-    mu[k] = s.x;
-    a[k] = s.y * param(gamma, g.pdtype, c, 1.f);
-    b[k] = param(beta, g.pdtype, c, 0.f);
-    k1[k] = q.x;
-    k2[k] = q.y;
-  }
-  const int64_t r0 = p.b * g.chunk, r1 = min(r0 + g.chunk, g.rows), at = p.n * g.sample + j;
-  for (int64_t r = r0 + p.row; r < r1; r += U * g.R) {
-    Source<T, V, Q> v[U];
-    Vec<T, V> d[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (r + u * g.R < r1) {
-        v[u].load(x, exps, at + (r + u * g.R) * g.L);
-        d[u].load(dy + at + (r + u * g.R) * g.L);
-      }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (r + u * g.R >= r1) break;
-      float f[V], h[V];
-      v[u].to_f(g.format, f);
-      d[u].to_f(h);
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float xm = f[k] - mu[k];
-        const float dz = h[k] * act_slope<T>(fmaf(xm, a[k], b[k]), g.act, g.slope);
-        h[k] = fmaf(dz, a[k], -fmaf(xm, k2[k], k1[k]));
-      }
-      d[u].from_f(h);
-      d[u].store(dx + at + (r + u * g.R) * g.L);
-    }
-  }
-}
-
 // dw, db: a warp a channel over the (sample, block) sums, in a fixed order.
-inline __global__ void __launch_bounds__(kThreads) params_kernel(const float2* __restrict__ cpart, int64_t parts, int C,
-                                                                 float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  const int c = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, lane = threadIdx.x & 31;
-  if (c >= C) return;
+__device__ __forceinline__ void param_grads(const float2* __restrict__ cpart, int64_t parts, int C, int c,
+                                            float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  const int lane = threadIdx.x & 31;
   double u = 0.0, v = 0.0;
+#pragma unroll 8
   for (int64_t i = lane; i < parts; i += 32) {
     const float2 e = cpart[i * C + c];
     u += e.x;
     v += e.y;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    u += __shfl_xor_sync(0xffffffffu, u, o);
-    v += __shfl_xor_sync(0xffffffffu, v, o);
-  }
+  join(u, v, 32);
   if (lane == 0) {
     if (dbeta) dbeta[c] = (float)u;
     if (dgamma) dgamma[c] = (float)v;
+  }
+}
+inline __global__ void __launch_bounds__(kThreads) params_kernel(const float2* __restrict__ cpart, int64_t parts, int C,
+                                                                 float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  wait_for_previous();
+  const int c = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+  if (c < C) param_grads(cpart, parts, C, c, dgamma, dbeta);
+}
+
+// dx of one vector; k1, k2: rstd * A, rstd^2 * B.
+template <typename T, int V, int ACT, bool Q>
+__device__ __forceinline__ Vec<T, V> dx_one(const Source<T, V, Q>& v, const Vec<T, V>& d, const Affine<V>& k,
+                                            const float2 (&k1)[kPairs<V>], const float2 (&k2)[kPairs<V>], const Geo& g) {
+  float2 xm[kPairs<V>], dz[kPairs<V>];
+  grad_one<T, V, ACT, Q>(v, d, k, g, xm, dz);
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i)
+    dz[i] = __ffma2_rn(dz[i], k.a[i], __fmul2_rn(__ffma2_rn(xm[i], k2[i], k1[i]), two(-1.f)));
+  Vec<T, V> r;
+  r.from_f(dz);
+  return r;
+}
+
+// Blocks from g.blocks on sum the parameters' gradients, beside the others.
+template <typename T, int V, int ACT, bool Q>
+__global__ void __launch_bounds__(kThreads, 2) bwd_dx_kernel(const T* __restrict__ dy, const void* __restrict__ x,
+                                                             const uint8_t* __restrict__ exps,
+                                                             const float2* __restrict__ mean_rstd,
+                                                             const void* __restrict__ gamma,
+                                                             const void* __restrict__ beta,
+                                                             const __grid_constant__ Geo g,
+                                                             const float2* __restrict__ cpart,
+                                                             const float2* __restrict__ gpart, T* __restrict__ dx,
+                                                             float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  constexpr int U = 4;
+  extern __shared__ float2 coef[];          // per group of the tile: rstd * A, rstd^2 * B
+  if (blockIdx.x >= g.blocks) {
+    wait_for_previous();
+    const int warps = blockDim.x / 32;
+    const int64_t c = ((blockIdx.x - g.blocks) * gridDim.y + blockIdx.y) * warps + threadIdx.x / 32;
+    if (c < g.C) param_grads(cpart, g.blocks, g.C, (int)c, dgamma, dbeta);
+    return;
+  }
+  const Place p = place<V>(g);
+  const float2* stats = mean_rstd + p.n * g.G;
+  Affine<V> k;
+  if (p.active) k.load(g, p, gamma, beta, [&](int gi) { return stats[gi]; });
+  wait_for_previous();
+  const int np = g.nb * g.tiles;
+  const float2* src = gpart + p.n * np * g.G + p.ga;
+  each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
+#pragma unroll 4
+    for (int e = sub; e < np; e += tp) {
+      const float2 v = src[(int64_t)e * g.G + i];
+      a += v.x;
+      c += v.y;
+    }
+  }, [&](int i, double a, double c) {
+    const double r = stats[p.ga + i].y;
+    coef[i] = make_float2((float)(r * a * g.inv_m), (float)(r * r * c * g.inv_m));
+  });
+  __syncthreads();
+  if (!p.active) return;
+  float2 k1[kPairs<V>], k2[kPairs<V>];
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) {
+    const int j = p.j0 + p.lane * V + 2 * i;
+    const float2 q = coef[j % g.C / g.Cg - p.ga];
+    const float2 h = V > 1 ? coef[(j + 1) % g.C / g.Cg - p.ga] : q;
+    k1[i] = make_float2(q.x, h.x);
+    k2[i] = make_float2(q.y, h.y);
+  }
+  for (int t = p.tiles - 1; t >= 0; t -= U) {
+    Source<T, V, Q> v[U];
+    Vec<T, V> d[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t - u >= 0 && p.in(t - u, g.R)) {
+        v[u].load(x, exps, p.at + (t - u) * p.step);
+        d[u].load(dy + p.at + (t - u) * p.step);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t - u >= 0 && p.in(t - u, g.R))
+        dx_one<T, V, ACT, Q>(v[u], d[u], k, k1, k2, g).store(dx + p.at + (t - u) * p.step);
   }
 }
 
@@ -544,6 +765,7 @@ struct FwdArgs {
   void* y;
   float2* mean_rstd;
   double2* part;
+  uint8_t *codes, *exps;    // null: not wanted
 };
 struct BwdArgs {
   const void *dy, *x, *gamma, *beta;

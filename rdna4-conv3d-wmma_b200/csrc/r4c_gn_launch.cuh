@@ -6,52 +6,103 @@
 namespace r4c {
 namespace gn {
 
-template <typename T, int V>
+// A launch that may start while the one before it in the stream still runs (it waits itself before it reads).
+template <typename... P, typename... A>
+cudaError_t launch_next(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+template <typename T, int V, int ACT>
 cudaError_t fwd_v(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   const dim3 grid((unsigned)g.blocks, g.tiles);
   const T* x = static_cast<const T*>(a.x);
   const size_t smem = sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
   stats_kernel<T, V><<<grid, threads, 0, s>>>(x, g, a.part);
-  apply_kernel<T, V><<<grid, threads, smem, s>>>(x, a.gamma, a.beta, g, a.part, a.mean_rstd, static_cast<T*>(a.y));
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  auto apply = apply_kernel<T, V, ACT, false>;
+  if constexpr (V * sizeof(T) == 16)
+    if (g.pack) apply = apply_kernel<T, V, ACT, true>;
+  e = launch_next(apply, grid, threads, smem, s, x, a.gamma, a.beta, g, a.part, a.mean_rstd, static_cast<T*>(a.y),
+                  a.codes, a.exps);
   note_launches(2);
-  return cudaGetLastError();
+  return e;
 }
 
-template <typename T, int V, bool Q>
+template <typename T, int V, int ACT, bool Q>
 cudaError_t bwd_v(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
-  const dim3 grid((unsigned)g.blocks, g.tiles);
+  dim3 grid((unsigned)g.blocks, g.tiles);
   const T* dy = static_cast<const T*>(a.dy);
   const size_t smem = sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
-  bwd_sums_kernel<T, V, Q><<<grid, threads, 0, s>>>(dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.cpart, a.gpart);
-  note_launches(1);
-  if (a.dx) {
-    bwd_dx_kernel<T, V, Q><<<grid, threads, smem, s>>>(dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.gpart,
-                                                      static_cast<T*>(a.dx));
-    note_launches(1);
+  bwd_sums_kernel<T, V, ACT, Q><<<grid, threads, 0, s>>>(dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.cpart, a.gpart);
+  note_launches(2);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const bool params = a.dgamma || a.dbeta;
+  if (!a.dx)
+    return launch_next(params_kernel, dim3(cdiv(g.C, kThreads / 32)), kThreads, 0, s, a.cpart, g.blocks, g.C, a.dgamma, a.dbeta);
+  if (params) grid.x += cdiv(g.C, (int64_t)g.tiles * (threads / 32));
+  return launch_next(bwd_dx_kernel<T, V, ACT, Q>, grid, threads, smem, s, dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta,
+                     g, a.cpart, a.gpart, static_cast<T*>(a.dx), a.dgamma, a.dbeta);
+}
+
+// The widest vectors have a kernel for each activation; narrower ones (channels that are no multiple of a vector in
+// volumes of odd sizes) one for all.
+template <typename T, int V>
+cudaError_t fwd_act(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
+  if constexpr (V * sizeof(T) == 16) {
+    switch (g.act) {
+      case R4C_ACT_NONE: return fwd_v<T, V, R4C_ACT_NONE>(a, g, threads, s);
+      case R4C_ACT_RELU: return fwd_v<T, V, R4C_ACT_RELU>(a, g, threads, s);
+      case R4C_ACT_LEAKY_RELU: return fwd_v<T, V, R4C_ACT_LEAKY_RELU>(a, g, threads, s);
+      case R4C_ACT_SILU: return fwd_v<T, V, R4C_ACT_SILU>(a, g, threads, s);
+      default: return fwd_v<T, V, R4C_ACT_GELU>(a, g, threads, s);
+    }
+  } else {
+    return fwd_v<T, V, -1>(a, g, threads, s);
   }
-  if (a.dgamma || a.dbeta) {
-    params_kernel<<<cdiv(g.C, kThreads / 32), kThreads, 0, s>>>(a.cpart, g.blocks, g.C, a.dgamma, a.dbeta);
-    note_launches(1);
+}
+template <typename T, int V, bool Q>
+cudaError_t bwd_act(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
+  if constexpr (V * sizeof(T) == 16) {
+    switch (g.act) {
+      case R4C_ACT_NONE: return bwd_v<T, V, R4C_ACT_NONE, Q>(a, g, threads, s);
+      case R4C_ACT_RELU: return bwd_v<T, V, R4C_ACT_RELU, Q>(a, g, threads, s);
+      case R4C_ACT_LEAKY_RELU: return bwd_v<T, V, R4C_ACT_LEAKY_RELU, Q>(a, g, threads, s);
+      case R4C_ACT_SILU: return bwd_v<T, V, R4C_ACT_SILU, Q>(a, g, threads, s);
+      default: return bwd_v<T, V, R4C_ACT_GELU, Q>(a, g, threads, s);
+    }
+  } else {
+    return bwd_v<T, V, -1, Q>(a, g, threads, s);
   }
-  return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t launch_fwd(const FwdArgs& a, const Geo& g, int V, int threads, cudaStream_t s) {
   if constexpr (sizeof(T) == 2)
-    if (V == 8) return fwd_v<T, 8>(a, g, threads, s);
-  if (V == 4) return fwd_v<T, 4>(a, g, threads, s);
-  if (V == 2) return fwd_v<T, 2>(a, g, threads, s);
-  return fwd_v<T, 1>(a, g, threads, s);
+    if (V == 8) return fwd_act<T, 8>(a, g, threads, s);
+  if (V == 4) return fwd_act<T, 4>(a, g, threads, s);
+  if (V == 2) return fwd_act<T, 2>(a, g, threads, s);
+  return fwd_act<T, 1>(a, g, threads, s);
 }
 
 template <typename T, bool Q>
 cudaError_t bwd_q(const BwdArgs& a, const Geo& g, int V, int threads, cudaStream_t s) {
   if constexpr (sizeof(T) == 2)
-    if (V == 8) return bwd_v<T, 8, Q>(a, g, threads, s);
-  if (V == 4) return bwd_v<T, 4, Q>(a, g, threads, s);
-  if (V == 2) return bwd_v<T, 2, Q>(a, g, threads, s);
-  return bwd_v<T, 1, Q>(a, g, threads, s);
+    if (V == 8) return bwd_act<T, 8, Q>(a, g, threads, s);
+  if (V == 4) return bwd_act<T, 4, Q>(a, g, threads, s);
+  if (V == 2) return bwd_act<T, 2, Q>(a, g, threads, s);
+  return bwd_act<T, 1, Q>(a, g, threads, s);
 }
 template <typename T>
 cudaError_t launch_bwd(const BwdArgs& a, const Geo& g, int V, int threads, cudaStream_t s) {

@@ -40,7 +40,7 @@ struct Oct {
 
 // `vec`: x lies on 16 bytes (codes always do). The last, incomplete eight elements go one by one.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) pack_kernel(const T* __restrict__ x, int64_t count, int vec, int format,
+__global__ void __launch_bounds__(kThreads, 4) pack_kernel(const T* __restrict__ x, int64_t count, int vec, int format,
                                                         uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
   const int64_t octs = (count + 7) / 8, full = vec ? count / 8 : 0;
   const int64_t step = (int64_t)gridDim.x * kThreads;
@@ -68,8 +68,9 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const T* __restrict__ x,
       if (i >= bound) break;                       // the same for a whole warp
       float f[8];
       a[u].to_f(f);
-      const int byte = exponent_byte(block_amax<8>(f, 0xffffffffu), format);
-      const Codes<8> c = encode<8>(f, byte, format);
+      bool finite;
+      const int byte = exponent_byte(block_amax<8>(f, 0xffffffffu, &finite), format);
+      const Codes<8> c = encode<8>(f, byte, format, finite);
       if (i >= octs) continue;
       if ((i + 1) * 8 <= count) {
         store_codes<8>(codes + i * 8, c);
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const T* __restrict__ x,
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) unpack_kernel(const uint8_t* __restrict__ codes,
+__global__ void __launch_bounds__(kThreads, 6) unpack_kernel(const uint8_t* __restrict__ codes,
                                                           const uint8_t* __restrict__ exps, int64_t count, int vec,
                                                           int format, T* __restrict__ x) {
   const int64_t octs = (count + 7) / 8, full = count / 8;
@@ -125,9 +126,10 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const uint8_t* __restr
   }
 }
 
-static int grid_for(int64_t count) {
+// One wave of `fit` blocks an SM.
+static int grid_for(int64_t count, int fit) {
   const int64_t octs = (count + 7) / 8;
-  return (int)std::max<int64_t>(1, std::min<int64_t>((octs + kThreads - 1) / kThreads, 148 * 8));
+  return (int)std::max<int64_t>(1, std::min<int64_t>((octs + kThreads - 1) / kThreads, 148 * fit));
 }
 
 static bool ok_args(const void* x, const void* codes, const void* exps, int64_t count, int dtype, int format) {
@@ -148,7 +150,7 @@ int r4c_pack8(const void* x, int64_t count, int dtype, int format, void* codes, 
   if (count == 0) return R4C_OK;
   if (!ok_args(x, codes, exponents, count, dtype, format)) return R4C_ERR_INVALID;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int grid = grid_for(count), vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  const int grid = grid_for(count, 4), vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   uint8_t* c = static_cast<uint8_t*>(codes);
   uint8_t* e = static_cast<uint8_t*>(exponents);
   if (dtype == R4C_BF16)
@@ -166,7 +168,7 @@ int r4c_unpack8(const void* codes, const void* exponents, int64_t count, int dty
   if (count == 0) return R4C_OK;
   if (!ok_args(x, codes, exponents, count, dtype, format)) return R4C_ERR_INVALID;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int grid = grid_for(count), vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  const int grid = grid_for(count, 6), vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const uint8_t* e = static_cast<const uint8_t*>(exponents);
   if (dtype == R4C_BF16)

@@ -66,24 +66,34 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const Codes<V>& c) {
     *p = (uint8_t)c.w[0];
 }
 
+// `finite`: no NaN or infinity among them.
 template <int V>
-__device__ __forceinline__ Codes<V> encode(const float (&f)[V], int byte, int format) {
+__device__ __forceinline__ Codes<V> encode(const float (&f)[V], int byte, int format, bool finite) {
+  static_assert(V % 4 == 0, "whole words of codes");
   Codes<V> c;
-  c.w[0] = 0;
-  if constexpr (V > 4) c.w[1] = 0;
   const float inv = inverse_scale(byte);
-  if (format == R4C_Q8_INT8) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int q = fabsf(f[k]) < INFINITY ? __float2int_rn(f[k] * inv) : -128;
-      c.w[k / 4] |= (uint32_t)(q & 0xff) << (8 * (k % 4));
+  for (int i = 0; i < V / 4; ++i) {
+    const float2 lo = __fmul2_rn(make_float2(f[4 * i], f[4 * i + 1]), make_float2(inv, inv));
+    const float2 hi = __fmul2_rn(make_float2(f[4 * i + 2], f[4 * i + 3]), make_float2(inv, inv));
+    if (format == R4C_Q8_INT8) {
+      // 1.5 * 2^23 + q rounds q to the nearest whole number, ties to even, and leaves it in the low byte
+      const float2 m = make_float2(12582912.f, 12582912.f);
+      const float2 a = __fadd2_rn(lo, m), b = __fadd2_rn(hi, m);
+      const uint32_t ab = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040);
+      const uint32_t cd = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
+      c.w[i] = __byte_perm(ab, cd, 0x5410);
+    } else {
+      const uint32_t ab = __nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3);
+      const uint32_t cd = __nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3);
+      c.w[i] = ab | cd << 16;
     }
-  } else {
+  }
+  if (!finite) {
+    const uint32_t nan = format == R4C_Q8_INT8 ? 0x80u : 0x7fu;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const uint32_t q = fabsf(f[k]) < INFINITY ? __nv_cvt_float_to_fp8(f[k] * inv, __NV_SATFINITE, __NV_E4M3) : 0x7fu;
-      c.w[k / 4] |= q << (8 * (k % 4));
-    }
+    for (int k = 0; k < V; ++k)
+      if (!(fabsf(f[k]) < INFINITY)) c.w[k / 4] = (c.w[k / 4] & ~(0xffu << (8 * (k % 4)))) | nan << (8 * (k % 4));
   }
   return c;
 }
@@ -119,18 +129,34 @@ __device__ __forceinline__ void decode(const Codes<V>& c, int byte, int format, 
       nan |= zero;
 #pragma unroll
       for (int k = 4 * i; k < V && k < 4 * i + 4; ++k)
-        f[k] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + (k & 3))) - 8388736.f) * s;
+        f[k] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + (k & 3)));
+    }
+    if constexpr (V == 1) {
+      f[0] = (f[0] - 8388736.f) * s;
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; k += 2) {
+        const float2 d = __fmul2_rn(__fadd2_rn(make_float2(f[k], f[k + 1]), make_float2(-8388736.f, -8388736.f)),
+                                    make_float2(s, s));
+        f[k] = d.x;
+        f[k + 1] = d.y;
+      }
     }
     if (nan) {
 #pragma unroll
       for (int k = 0; k < V; ++k)
         if (((c.w[k / 4] >> (8 * (k % 4))) & 0xffu) == 0x80u) f[k] = __uint_as_float(0x7fc00000u);
     }
+  } else if constexpr (V == 1) {
+    f[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(c.w[0] & 0xffu), __NV_E4M3))) * s;
   } else {
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const __nv_fp8_storage_t b = (__nv_fp8_storage_t)((c.w[k / 4] >> (8 * (k % 4))) & 0xffu);
-      f[k] = __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3))) * s;
+    for (int k = 0; k < V; k += 2) {
+      const __nv_fp8x2_storage_t b = (__nv_fp8x2_storage_t)(c.w[k / 4] >> (8 * (k % 4)));
+      const float2 h = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(b, __NV_E4M3)));
+      const float2 d = __fmul2_rn(h, make_float2(s, s));
+      f[k] = d.x;
+      f[k + 1] = d.y;
     }
   }
   const int high = format == R4C_Q8_INT8 ? Limits<T>::high_int8 : Limits<T>::high_e4m3;
@@ -145,25 +171,24 @@ __device__ __forceinline__ void decode(const Codes<V>& c, int byte, int format, 
 }
 
 // Largest finite magnitude (fp32 bits) of a block that 32 / V neighbouring lanes hold, V elements each; every lane of
-// `mask` takes part.
+// `mask` takes part. `finite`: this lane's elements all are.
 template <int V>
-__device__ __forceinline__ uint32_t block_amax(const float (&f)[V], uint32_t mask) {
+__device__ __forceinline__ uint32_t block_amax(const float (&f)[V], uint32_t mask, bool* finite) {
   uint32_t m = 0;
 #pragma unroll
   for (int k = 0; k < V; ++k) m = max(m, __float_as_uint(f[k]) & 0x7fffffffu);
-  const uint32_t own = m;
-#pragma unroll
-  for (int o = 1; o < kBlock / V; o <<= 1) m = max(m, __shfl_xor_sync(mask, m, o));
-  if (__any_sync(mask, own >= 0x7f800000u)) {   // NaN or infinities somewhere: the finite ones alone
+  const bool bad = m >= 0x7f800000u;
+  *finite = !bad;
+  if (__any_sync(mask, bad)) {                  // NaN or infinities somewhere: the finite ones alone
     m = 0;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const uint32_t b = __float_as_uint(f[k]) & 0x7fffffffu;
       m = max(m, b < 0x7f800000u ? b : 0u);
     }
-#pragma unroll
-    for (int o = 1; o < kBlock / V; o <<= 1) m = max(m, __shfl_xor_sync(mask, m, o));
   }
+#pragma unroll
+  for (int o = 1; o < kBlock / V; o <<= 1) m = max(m, __shfl_xor_sync(mask, m, o));
   return m;
 }
 
