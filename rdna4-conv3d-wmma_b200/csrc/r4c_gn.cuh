@@ -8,7 +8,8 @@
 //   A = mean over the group of dz * w,  B = mean over the group of dz * w * xh
 //   dx = rstd * (dz * w - A - xh * B)
 // Two passes over the data each way: sums, then the element-wise result (the statistics of a group need all of it).
-// Both are bound by memory: forward 3, backward 5 activations read or written.
+// Both are bound by memory: forward 3, backward 5 activations read or written. Samples that fit the registers of a
+// cluster take one.
 //
 // A thread owns a vector of V neighbouring elements in every R-th row of its block's range, so its channels and with
 // them the parameters stay in registers. A row is a voxel's channels, or L / C voxels together where C is no multiple
@@ -27,6 +28,9 @@ namespace r4c {
 namespace gn {
 
 constexpr int kThreads = 256;   // at most, per block
+// Samples that a cluster keeps in registers: vectors of a thread at most (forward; backward, which keeps dy too),
+// groups of a channel tile at most (shared memory).
+constexpr int kSmallFwd = 16, kSmallBwd = 8, kSmallGroups = 256;
 
 struct Geo {
   int64_t sample;    // elements of a sample, S * C
@@ -42,6 +46,7 @@ struct Geo {
   int R;             // rows that a block's threads cover at a time
   int nb;            // blocks of a sample and channel tile (the cluster's, where one keeps a sample)
   int pack;          // the forward writes x in 8 bits too
+  int small;         // vectors that a thread keeps in registers (small samples), or 0: two passes
 };
 
 // V elements of T, moved as one word; in fp32 as pairs, for the packed arithmetic (two fp32 an instruction: half the
@@ -339,25 +344,29 @@ __device__ __forceinline__ void each_sum(int items, F f, Out out) {
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// The thread's mean (negated), rstd * w and b.
+// The thread's mean (negated), rstd * w and b; w and b do not wait for the statistics.
 template <int V>
 struct Affine {
   float2 nmu[kPairs<V>], a[kPairs<V>], b[kPairs<V>];
-  template <typename Stat>
-  __device__ __forceinline__ void load(const Geo& g, const Place& p, const void* gamma, const void* beta, Stat stat) {
+  __device__ __forceinline__ void params(const Geo& g, const Place& p, const void* gamma, const void* beta) {
 #pragma unroll
-    for (int k = 0; k < 2 * kPairs<V>; ++k) {
-      float m = 0.f, s = 0.f, t = 0.f;
-      if (k < V) {
-        const int c = (p.j0 + p.lane * V + k) % g.C;
-        const float2 q = stat(c / g.Cg);
-        m = -q.x;
-        s = q.y * param(gamma, g.pdtype, c, 1.f);
-        t = param(beta, g.pdtype, c, 0.f);
-      }
-      (k & 1 ? nmu[k / 2].y : nmu[k / 2].x) = m;
-      (k & 1 ? a[k / 2].y : a[k / 2].x) = s;
-      (k & 1 ? b[k / 2].y : b[k / 2].x) = t;
+    for (int k = 0; k < kPairs<V>; ++k) {
+      nmu[k] = a[k] = b[k] = two(0.f);
+      if (!p.active) continue;
+      const int c0 = (p.j0 + p.lane * V + 2 * k) % g.C, c1 = V > 1 ? (p.j0 + p.lane * V + 2 * k + 1) % g.C : c0;
+      a[k] = make_float2(param(gamma, g.pdtype, c0, 1.f), param(gamma, g.pdtype, c1, 1.f));
+      b[k] = make_float2(param(beta, g.pdtype, c0, 0.f), param(beta, g.pdtype, c1, 0.f));
+    }
+  }
+  template <typename Stat>
+  __device__ __forceinline__ void stats(const Geo& g, const Place& p, Stat stat) {
+    if (!p.active) return;
+#pragma unroll
+    for (int k = 0; k < kPairs<V>; ++k) {
+      const int c0 = (p.j0 + p.lane * V + 2 * k) % g.C, c1 = V > 1 ? (p.j0 + p.lane * V + 2 * k + 1) % g.C : c0;
+      const float2 q = stat(c0 / g.Cg), r = stat(c1 / g.Cg);
+      nmu[k] = make_float2(-q.x, -r.x);
+      a[k] = __fmul2_rn(a[k], make_float2(q.y, r.y));
     }
   }
 };
@@ -506,6 +515,8 @@ __global__ void __launch_bounds__(kThreads, 3) apply_kernel(const T* __restrict_
   constexpr int U = 4;
   extern __shared__ float2 stat[];
   const Place p = place<V>(g);
+  Affine<V> k;
+  k.params(g, p, gamma, beta);
   wait_for_previous();
   const int np = g.nb * g.tiles;
   const double2* src = part + p.n * np * g.G + p.ga;
@@ -520,8 +531,7 @@ __global__ void __launch_bounds__(kThreads, 3) apply_kernel(const T* __restrict_
   __syncthreads();
   if (p.b == 0)
     for (int i = threadIdx.x; i < p.gb - p.ga; i += blockDim.x) mean_rstd[p.n * g.G + p.ga + i] = stat[i];
-  Affine<V> k;
-  if (p.active) k.load(g, p, gamma, beta, [&](int gi) { return stat[gi - p.ga]; });
+  k.stats(g, p, [&](int gi) { return stat[gi - p.ga]; });
   for (int t = p.tiles - 1; t >= 0; t -= U) {
     Vec<T, V> v[U];
 #pragma unroll
@@ -611,7 +621,8 @@ __global__ void __launch_bounds__(kThreads, 2) bwd_sums_kernel(const T* __restri
   for (int k = 0; k < kPairs<V>; ++k) s1[k] = s2[k] = two(0.f);
   if (p.in(0, g.R)) {
     Affine<V> k;
-    k.load(g, p, gamma, beta, [&](int gi) { return stats[gi]; });
+    k.params(g, p, gamma, beta);
+    k.stats(g, p, [&](int gi) { return stats[gi]; });
     auto add = [&](const Source<T, V, Q>& v, const Vec<T, V>& d) {
       float2 xm[kPairs<V>], dz[kPairs<V>];
       grad_one<T, V, ACT, Q>(v, d, k, g, xm, dz);
@@ -654,7 +665,8 @@ __global__ void __launch_bounds__(kThreads, 2) bwd_sums_kernel(const T* __restri
 // ---------------------------------------------------------------------------
 // Backward: dx, and the gradients of weight and bias
 // ---------------------------------------------------------------------------
-// dw, db: a warp a channel over the (sample, block) sums, in a fixed order.
+// dw, db: a warp, or a block, sums a channel over the (sample, block) parts, in a fixed order.
+constexpr int64_t kWideParts = 2048;      // from here on a block a channel (70,000 parts of 16 channels: 160 -> 21 us)
 __device__ __forceinline__ void param_grads(const float2* __restrict__ cpart, int64_t parts, int C, int c,
                                             float* __restrict__ dgamma, float* __restrict__ dbeta) {
   const int lane = threadIdx.x & 31;
@@ -673,9 +685,33 @@ __device__ __forceinline__ void param_grads(const float2* __restrict__ cpart, in
 }
 inline __global__ void __launch_bounds__(kThreads) params_kernel(const float2* __restrict__ cpart, int64_t parts, int C,
                                                                  float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  __shared__ double2 warps[kThreads / 32];
   wait_for_previous();
-  const int c = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-  if (c < C) param_grads(cpart, parts, C, c, dgamma, dbeta);
+  if (parts < kWideParts) {
+    const int c = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+    if (c < C) param_grads(cpart, parts, C, c, dgamma, dbeta);
+    return;
+  }
+  const int c = blockIdx.x;
+  double u = 0.0, v = 0.0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < parts; i += kThreads) {
+    const float2 e = cpart[i * C + c];
+    u += e.x;
+    v += e.y;
+  }
+  join(u, v, 32);
+  if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = make_double2(u, v);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    u = v = 0.0;
+    for (int i = 0; i < kThreads / 32; ++i) {
+      u += warps[i].x;
+      v += warps[i].y;
+    }
+    if (dbeta) dbeta[c] = (float)u;
+    if (dgamma) dgamma[c] = (float)v;
+  }
 }
 
 // dx of one vector; k1, k2: rstd * A, rstd^2 * B.
@@ -690,6 +726,23 @@ __device__ __forceinline__ Vec<T, V> dx_one(const Source<T, V, Q>& v, const Vec<
   Vec<T, V> r;
   r.from_f(dz);
   return r;
+}
+
+// The thread's rstd * A and rstd^2 * B from its groups'.
+template <int V>
+__device__ __forceinline__ void thread_coef(const Geo& g, const Place& p, const float2* coef, float2 (&k1)[kPairs<V>],
+                                            float2 (&k2)[kPairs<V>]) {
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) {
+    const int j = p.j0 + p.lane * V + 2 * i;
+    const float2 q = coef[j % g.C / g.Cg - p.ga];
+    const float2 h = V > 1 ? coef[(j + 1) % g.C / g.Cg - p.ga] : q;
+    k1[i] = make_float2(q.x, h.x);
+    k2[i] = make_float2(q.y, h.y);
+  }
+}
+__device__ __forceinline__ float2 coef_of(const Geo& g, double rstd, double a, double c) {
+  return make_float2((float)(rstd * a * g.inv_m), (float)(rstd * rstd * c * g.inv_m));
 }
 
 // Blocks from g.blocks on sum the parameters' gradients, beside the others.
@@ -715,7 +768,8 @@ __global__ void __launch_bounds__(kThreads, 2) bwd_dx_kernel(const T* __restrict
   const Place p = place<V>(g);
   const float2* stats = mean_rstd + p.n * g.G;
   Affine<V> k;
-  if (p.active) k.load(g, p, gamma, beta, [&](int gi) { return stats[gi]; });
+  k.params(g, p, gamma, beta);
+  k.stats(g, p, [&](int gi) { return stats[gi]; });
   wait_for_previous();
   const int np = g.nb * g.tiles;
   const float2* src = gpart + p.n * np * g.G + p.ga;
@@ -726,21 +780,11 @@ __global__ void __launch_bounds__(kThreads, 2) bwd_dx_kernel(const T* __restrict
       a += v.x;
       c += v.y;
     }
-  }, [&](int i, double a, double c) {
-    const double r = stats[p.ga + i].y;
-    coef[i] = make_float2((float)(r * a * g.inv_m), (float)(r * r * c * g.inv_m));
-  });
+  }, [&](int i, double a, double c) { coef[i] = coef_of(g, stats[p.ga + i].y, a, c); });
   __syncthreads();
   if (!p.active) return;
   float2 k1[kPairs<V>], k2[kPairs<V>];
-#pragma unroll
-  for (int i = 0; i < kPairs<V>; ++i) {
-    const int j = p.j0 + p.lane * V + 2 * i;
-    const float2 q = coef[j % g.C / g.Cg - p.ga];
-    const float2 h = V > 1 ? coef[(j + 1) % g.C / g.Cg - p.ga] : q;
-    k1[i] = make_float2(q.x, h.x);
-    k2[i] = make_float2(q.y, h.y);
-  }
+  thread_coef<V>(g, p, coef, k1, k2);
   for (int t = p.tiles - 1; t >= 0; t -= U) {
     Source<T, V, Q> v[U];
     Vec<T, V> d[U];
@@ -755,6 +799,140 @@ __global__ void __launch_bounds__(kThreads, 2) bwd_dx_kernel(const T* __restrict
       if (t - u >= 0 && p.in(t - u, g.R))
         dx_one<T, V, ACT, Q>(v[u], d[u], k, k1, k2, g).store(dx + p.at + (t - u) * p.step);
   }
+}
+
+// ---------------------------------------------------------------------------
+// Small samples: one launch, data in registers
+// ---------------------------------------------------------------------------
+// A cluster of g.nb blocks keeps a sample's groups (all, or a channel tile of whole groups) in registers, NV vectors a
+// thread, between the sums and the result: every element is read once, nothing goes through memory in between, and one
+// launch does what two did. The blocks' sums are exchanged through shared memory.
+__device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ double2 remote(const double2* p, uint32_t rank) {
+  double2 v;
+  asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];"
+               : "=d"(v.x), "=d"(v.y) : "r"(in_block(shared_at(p), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Sums over the cluster's blocks of what each has in `mine` per group: out(group of the tile, sum, sum). Returns with
+// an arrival on the cluster's barrier that the caller waits for before it exits (others may still read `mine`).
+template <typename Out>
+__device__ __forceinline__ void cluster_sums(const Geo& g, int groups, const double2* mine, Out out) {
+  if (g.nb > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  each_sum<double>(groups, [&](int i, int sub, int tp, double& a, double& c) {
+    for (int r = sub; r < g.nb; r += tp) {
+      const double2 v = g.nb > 1 ? remote(mine + i, r) : mine[i];
+      a += v.x;
+      c += v.y;
+    }
+  }, out);
+  __syncthreads();
+  if (g.nb > 1) cluster_arrive();
+}
+
+template <typename T, int V, int ACT, bool PACK, int NV>
+__global__ void __launch_bounds__(kThreads, 2) fwd_small_kernel(const T* __restrict__ x, const void* __restrict__ gamma,
+                                                                const void* __restrict__ beta,
+                                                                const __grid_constant__ Geo g,
+                                                                float2* __restrict__ mean_rstd, T* __restrict__ y,
+                                                                uint8_t* __restrict__ codes,
+                                                                uint8_t* __restrict__ exps) {
+  __shared__ double2 red[V * kThreads];
+  extern __shared__ double2 mine[];
+  const Place p = place<V>(g);
+  const int groups = p.gb - p.ga;
+  float2* stat = reinterpret_cast<float2*>(mine + groups);
+  Vec<T, V> v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    v[i].zero();
+    if (p.in(i, g.R)) v[i].load(x + p.at + i * p.step);
+  }
+  Affine<V> k;
+  k.params(g, p, gamma, beta);
+  Moments<T, V> m;
+  m.zero();
+  m.pivot(v[0]);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (p.in(i, g.R)) m.add(v[i]);
+  block_moments<T, V>(g, p, m, red, [&](int gi, double a, double c) { mine[gi - p.ga] = make_double2(a, c); });
+  cluster_sums(g, groups, mine, [&](int i, double a, double c) { stat[i] = mean_rstd_of(g, a, c); });
+  if (p.b == 0)
+    for (int i = threadIdx.x; i < groups; i += blockDim.x) mean_rstd[p.n * g.G + p.ga + i] = stat[i];
+  k.stats(g, p, [&](int gi) { return stat[gi - p.ga]; });
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i < p.tiles) apply_one<T, V, ACT, PACK>(v[i], k, g, p.in(i, g.R), p.at + i * p.step, y, codes, exps);
+  if (g.nb > 1) cluster_wait();
+}
+
+template <typename T, int V, int ACT, bool Q, int NV>
+__global__ void __launch_bounds__(kThreads, NV > 4 ? 1 : 2)
+    bwd_small_kernel(const T* __restrict__ dy, const void* __restrict__ x, const uint8_t* __restrict__ exps,
+                     const float2* __restrict__ mean_rstd, const void* __restrict__ gamma,
+                     const void* __restrict__ beta, const __grid_constant__ Geo g, float2* __restrict__ cpart,
+                     T* __restrict__ dx) {
+  __shared__ float2 red[V * kThreads];
+  __shared__ float2 cols[V * kThreads];
+  extern __shared__ double2 mine[];
+  let_next_start();
+  const Place p = place<V>(g);
+  const int groups = p.gb - p.ga;
+  float2* coef = reinterpret_cast<float2*>(mine + groups);
+  const float2* stats = mean_rstd + p.n * g.G;
+  Source<T, V, Q> v[NV];
+  Vec<T, V> d[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    v[i].zero();
+    d[i].zero();
+    if (p.in(i, g.R)) {
+      v[i].load(x, exps, p.at + i * p.step);
+      d[i].load(dy + p.at + i * p.step);
+    }
+  }
+  Affine<V> k;
+  k.params(g, p, gamma, beta);
+  k.stats(g, p, [&](int gi) { return stats[gi]; });
+  float2 s1[kPairs<V>], s2[kPairs<V>];
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) s1[i] = s2[i] = two(0.f);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (p.in(i, g.R)) {
+      float2 xm[kPairs<V>], dz[kPairs<V>];
+      grad_one<T, V, ACT, Q>(v[i], d[i], k, g, xm, dz);
+#pragma unroll
+      for (int j = 0; j < kPairs<V>; ++j) {
+        s1[j] = __fadd2_rn(s1[j], dz[j]);
+        s2[j] = __ffma2_rn(dz[j], xm[j], s2[j]);
+      }
+    }
+  block_grads<V>(g, p, s1, s2, gamma, red, cols, cpart, [&](int gi) { return stats[gi]; },
+                 [&](int gi, float a, float c) { mine[gi - p.ga] = make_double2(a, c); });
+  cluster_sums(g, groups, mine, [&](int i, double a, double c) { coef[i] = coef_of(g, stats[p.ga + i].y, a, c); });
+  if (p.active) {
+    float2 k1[kPairs<V>], k2[kPairs<V>];
+    thread_coef<V>(g, p, coef, k1, k2);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (p.in(i, g.R)) dx_one<T, V, ACT, Q>(v[i], d[i], k, k1, k2, g).store(dx + p.at + i * p.step);
+  }
+  if (g.nb > 1) cluster_wait();
 }
 
 // ---------------------------------------------------------------------------

@@ -6,12 +6,9 @@
 namespace r4c {
 namespace gn {
 
-// A launch that may start while the one before it in the stream still runs (it waits itself before it reads).
 template <typename... P, typename... A>
-cudaError_t launch_next(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
+cudaError_t launch_with(cudaLaunchAttribute at, void (*kernel)(P...), dim3 grid, int threads, size_t smem,
+                        cudaStream_t s, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -21,11 +18,41 @@ cudaError_t launch_next(void (*kernel)(P...), dim3 grid, int threads, size_t sme
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
+// A launch that may start while the one before it in the stream still runs (it waits itself before it reads).
+template <typename... P, typename... A>
+cudaError_t launch_next(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  return launch_with(at, kernel, grid, threads, smem, s, args...);
+}
+template <typename... P, typename... A>
+cudaError_t launch_cluster(int blocks, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s,
+                           A... args) {
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = blocks;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  return launch_with(at, kernel, grid, threads, smem, s, args...);
+}
+
+template <typename T, int V, int ACT, bool PACK>
+auto fwd_small_of(const Geo& g) {
+  return g.small <= 4 ? fwd_small_kernel<T, V, ACT, PACK, 4> : fwd_small_kernel<T, V, ACT, PACK, kSmallFwd>;
+}
 
 template <typename T, int V, int ACT>
 cudaError_t fwd_v(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   const dim3 grid((unsigned)g.blocks, g.tiles);
   const T* x = static_cast<const T*>(a.x);
+  if (g.small) {
+    auto kernel = fwd_small_of<T, V, ACT, false>(g);
+    if constexpr (V * sizeof(T) == 16)
+      if (g.pack) kernel = fwd_small_of<T, V, ACT, true>(g);
+    note_launches(1);
+    return launch_cluster(g.nb, kernel, grid, threads, kSmallGroups * (sizeof(double2) + sizeof(float2)), s, x, a.gamma,
+                          a.beta, g, a.mean_rstd, static_cast<T*>(a.y), a.codes, a.exps);
+  }
   const size_t smem = sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
   stats_kernel<T, V><<<grid, threads, 0, s>>>(x, g, a.part);
   cudaError_t e = cudaGetLastError();
@@ -43,17 +70,31 @@ template <typename T, int V, int ACT, bool Q>
 cudaError_t bwd_v(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   dim3 grid((unsigned)g.blocks, g.tiles);
   const T* dy = static_cast<const T*>(a.dy);
+  const bool params = a.dgamma || a.dbeta;
+  auto params_next = [&] {
+    note_launches(1);
+    return launch_next(params_kernel, dim3(g.blocks < kWideParts ? cdiv(g.C, kThreads / 32) : g.C), kThreads, 0, s,
+                       a.cpart, g.blocks, g.C, a.dgamma, a.dbeta);
+  };
+  if (g.small && a.dx) {
+    auto kernel = g.small <= 4 ? bwd_small_kernel<T, V, ACT, Q, 4> : bwd_small_kernel<T, V, ACT, Q, kSmallBwd>;
+    note_launches(1);
+    const cudaError_t e = launch_cluster(g.nb, kernel, grid, threads, kSmallGroups * (sizeof(double2) + sizeof(float2)), s,
+                                         dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.cpart, static_cast<T*>(a.dx));
+    return e != cudaSuccess || !params ? e : params_next();
+  }
   const size_t smem = sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
   bwd_sums_kernel<T, V, ACT, Q><<<grid, threads, 0, s>>>(dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.cpart, a.gpart);
-  note_launches(2);
+  note_launches(1);
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  const bool params = a.dgamma || a.dbeta;
-  if (!a.dx)
-    return launch_next(params_kernel, dim3(cdiv(g.C, kThreads / 32)), kThreads, 0, s, a.cpart, g.blocks, g.C, a.dgamma, a.dbeta);
-  if (params) grid.x += cdiv(g.C, (int64_t)g.tiles * (threads / 32));
-  return launch_next(bwd_dx_kernel<T, V, ACT, Q>, grid, threads, smem, s, dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta,
-                     g, a.cpart, a.gpart, static_cast<T*>(a.dx), a.dgamma, a.dbeta);
+  if (e != cudaSuccess || !a.dx) return e != cudaSuccess ? e : params_next();
+  const bool beside = params && g.blocks < kWideParts;
+  if (beside) grid.x += cdiv(g.C, (int64_t)g.tiles * (threads / 32));
+  note_launches(1);
+  e = launch_next(bwd_dx_kernel<T, V, ACT, Q>, grid, threads, smem, s, dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta,
+                  g, a.cpart, a.gpart, static_cast<T*>(a.dx), a.dgamma, a.dbeta);
+  if (e != cudaSuccess || !params || beside) return e;
+  return params_next();
 }
 
 // The widest vectors have a kernel for each activation; narrower ones (channels that are no multiple of a vector in

@@ -855,22 +855,21 @@ def gn_desc(x: torch.Tensor, groups: int, params_dtype: torch.dtype, eps: float,
                   activation, eps, slope)
 
 
-def _addr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
 def gn_forward(x: torch.Tensor, desc: GnDesc, weight, bias, fmt: Optional[int]):
     """(y, mean_rstd, codes or None, exponents or None) of a channels-last dense x."""
     L = lib()
-    y = class_last_empty(x)
+    y = torch.empty_like(x)
     mean_rstd = x.new_empty((2 * desc.samples * desc.groups,), dtype=torch.float32)
-    codes = exps = None
+    codes = exps = ws = None
     if fmt is not None:
         codes, exps = q8_buffers(x)
     nb = L.r4c_gn_workspace_size(desc, 0)
-    ws = x.new_empty(nb, dtype=torch.uint8)
-    _launch("r4c_gn_fwd", L.r4c_gn_fwd, x.device, desc, x.data_ptr(), _addr(weight), _addr(bias), y.data_ptr(),
-            mean_rstd.data_ptr(), fmt or 0, _addr(codes), _addr(exps), ws.data_ptr(), nb)
+    if nb:
+        ws = x.new_empty(nb, dtype=torch.uint8)
+    _launch("r4c_gn_fwd", L.r4c_gn_fwd, x.device, desc, x.data_ptr(), None if weight is None else weight.data_ptr(),
+            None if bias is None else bias.data_ptr(), y.data_ptr(), mean_rstd.data_ptr(), fmt or 0,
+            None if codes is None else codes.data_ptr(), None if codes is None else exps.data_ptr(),
+            None if ws is None else ws.data_ptr(), nb)
     return y, mean_rstd, codes, exps
 
 
@@ -878,13 +877,16 @@ def gn_backward(dy: torch.Tensor, desc: GnDesc, x, fmt: int, exps, mean_rstd, we
                 need_params: bool):
     """(dx, dweight, dbias); fp32 parameter gradients; x the activation, or its codes with ``exps``."""
     L = lib()
-    dx = class_last_empty(dy) if need_dx else None
+    dx = torch.empty_like(dy) if need_dx else None
     dw = db = None
     if need_params:
         dw = dy.new_empty((desc.channels,), dtype=torch.float32)
         db = torch.empty_like(dw)
     nb = L.r4c_gn_workspace_size(desc, 1)
     ws = dy.new_empty(nb, dtype=torch.uint8)
-    _launch("r4c_gn_bwd", L.r4c_gn_bwd, dy.device, desc, dy.data_ptr(), x.data_ptr(), fmt, _addr(exps),
-            mean_rstd.data_ptr(), _addr(weight), _addr(bias), _addr(dx), _addr(dw), _addr(db), ws.data_ptr(), nb)
+    _launch("r4c_gn_bwd", L.r4c_gn_bwd, dy.device, desc, dy.data_ptr(), x.data_ptr(), fmt,
+            None if exps is None else exps.data_ptr(), mean_rstd.data_ptr(),
+            None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
+            None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+            None if db is None else db.data_ptr(), ws.data_ptr(), nb)
     return dx, dw, db

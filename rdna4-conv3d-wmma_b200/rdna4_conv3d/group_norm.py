@@ -51,10 +51,13 @@ def _channels_last(t: torch.Tensor) -> torch.Tensor:
 
 def _params(weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]):
     """(weight, bias, their type) as the kernels read them."""
-    dtypes = {t.dtype for t in (weight, bias) if t is not None}
-    dtype = dtypes.pop() if len(dtypes) == 1 else torch.float32
-    if dtype not in _FLOATS:
-        dtype = torch.float32
+    if weight is not None and bias is not None and weight.dtype is bias.dtype and weight.dtype in _FLOATS:
+        if weight.is_contiguous() and bias.is_contiguous():
+            return weight, bias, weight.dtype
+        dtype = weight.dtype
+    else:
+        given = weight if bias is None else bias if weight is None else None
+        dtype = torch.float32 if given is None or given.dtype not in _FLOATS else given.dtype
     return tuple(None if t is None else t.detach().to(dtype).contiguous() for t in (weight, bias)) + (dtype,)
 
 

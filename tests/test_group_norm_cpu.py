@@ -236,6 +236,9 @@ def test_entries_refuse():
         if need:
             assert (bwd if back else fwd)(_d(), nb=need - 1) == -3
     assert fwd(_d(samples=0)) == 0 and fwd(_d(inner=0)) == 0
+    for back in (0, 1):                                  # sizes of nothing, and of one voxel
+        for change in (dict(samples=0), dict(inner=0), dict(inner=1), dict(inner=1, channels=1, groups=1)):
+            assert lib.r4c_gn_workspace_size(_d(**change), back) >= 0
     for fn in (lib.r4c_pack8, ):
         assert fn(p, 8, 5, 0, p, p, None) == -1 and fn(p, 8, 0, 2, p, p, None) == -1 and fn(p, -1, 0, 0, p, p, None) == -1
         assert fn(None, 8, 0, 0, p, p, None) == -1 and fn(p, 8, 0, 0, odd, p, None) == -1
