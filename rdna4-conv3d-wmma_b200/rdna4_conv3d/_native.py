@@ -13,6 +13,7 @@ Reference counterpart: the JIT loader of the HIP extension
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 from typing import Optional, Tuple
@@ -848,43 +849,52 @@ def unpack8(codes: torch.Tensor, exps: torch.Tensor, fmt: int, out: torch.Tensor
     return out
 
 
-def gn_desc(x: torch.Tensor, groups: int, params_dtype: torch.dtype, eps: float, activation: int,
-            slope: float) -> GnDesc:
-    shape = x.shape
-    return GnDesc(shape[0], shape[2:].numel(), shape[1], groups, dtype_code(x.dtype), dtype_code(params_dtype),
-                  activation, eps, slope)
+class GnPlan:
+    """A descriptor with the workspace that each direction takes."""
+    __slots__ = ("desc", "fwd_bytes", "bwd_bytes", "stats")
+
+    def __init__(self, desc: GnDesc):
+        L = lib()
+        self.desc, self.stats = desc, 2 * desc.samples * desc.groups
+        self.fwd_bytes, self.bwd_bytes = L.r4c_gn_workspace_size(desc, 0), L.r4c_gn_workspace_size(desc, 1)
 
 
-def gn_forward(x: torch.Tensor, desc: GnDesc, weight, bias, fmt: Optional[int]):
+@functools.lru_cache(maxsize=512)
+def gn_plan(shape: torch.Size, groups: int, dtype: torch.dtype, params_dtype: torch.dtype, eps: float, activation: int,
+            slope: float) -> GnPlan:
+    """The plan of a call's sizes and types (its kernels are chosen by those alone)."""
+    return GnPlan(GnDesc(shape[0], shape[2:].numel(), shape[1], groups, dtype_code(dtype), dtype_code(params_dtype),
+                         activation, eps, slope))
+
+
+def gn_forward(x: torch.Tensor, plan: GnPlan, weight, bias, fmt: Optional[int]):
     """(y, mean_rstd, codes or None, exponents or None) of a channels-last dense x."""
-    L = lib()
     y = torch.empty_like(x)
-    mean_rstd = x.new_empty((2 * desc.samples * desc.groups,), dtype=torch.float32)
+    mean_rstd = x.new_empty((plan.stats,), dtype=torch.float32)
     codes = exps = ws = None
     if fmt is not None:
         codes, exps = q8_buffers(x)
-    nb = L.r4c_gn_workspace_size(desc, 0)
+    nb = plan.fwd_bytes
     if nb:
         ws = x.new_empty(nb, dtype=torch.uint8)
-    _launch("r4c_gn_fwd", L.r4c_gn_fwd, x.device, desc, x.data_ptr(), None if weight is None else weight.data_ptr(),
+    _launch("r4c_gn_fwd", _lib.r4c_gn_fwd, x.device, plan.desc, x.data_ptr(), None if weight is None else weight.data_ptr(),
             None if bias is None else bias.data_ptr(), y.data_ptr(), mean_rstd.data_ptr(), fmt or 0,
             None if codes is None else codes.data_ptr(), None if codes is None else exps.data_ptr(),
             None if ws is None else ws.data_ptr(), nb)
     return y, mean_rstd, codes, exps
 
 
-def gn_backward(dy: torch.Tensor, desc: GnDesc, x, fmt: int, exps, mean_rstd, weight, bias, need_dx: bool,
+def gn_backward(dy: torch.Tensor, plan: GnPlan, x, fmt: int, exps, mean_rstd, weight, bias, need_dx: bool,
                 need_params: bool):
     """(dx, dweight, dbias); fp32 parameter gradients; x the activation, or its codes with ``exps``."""
-    L = lib()
     dx = torch.empty_like(dy) if need_dx else None
     dw = db = None
     if need_params:
-        dw = dy.new_empty((desc.channels,), dtype=torch.float32)
+        dw = dy.new_empty((plan.desc.channels,), dtype=torch.float32)
         db = torch.empty_like(dw)
-    nb = L.r4c_gn_workspace_size(desc, 1)
+    nb = plan.bwd_bytes
     ws = dy.new_empty(nb, dtype=torch.uint8)
-    _launch("r4c_gn_bwd", L.r4c_gn_bwd, dy.device, desc, dy.data_ptr(), x.data_ptr(), fmt,
+    _launch("r4c_gn_bwd", _lib.r4c_gn_bwd, dy.device, plan.desc, dy.data_ptr(), x.data_ptr(), fmt,
             None if exps is None else exps.data_ptr(), mean_rstd.data_ptr(),
             None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
             None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),

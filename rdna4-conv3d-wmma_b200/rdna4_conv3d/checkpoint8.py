@@ -87,7 +87,7 @@ def unpack8(packed: Packed8) -> torch.Tensor:
     codes, exps, shape, stride, dtype, fmt = packed
     check_format(fmt)
     count = shape.numel()
-    if codes.numel() != count or exps.numel() != -(-count // _native.Q8_BLOCK):
+    if codes.numel() != count or exps.numel() != (count + 31) // _native.Q8_BLOCK:
         raise ValueError(f"{count} elements need as many codes and {-(-count // _native.Q8_BLOCK)} exponents, got "
                          f"{codes.numel()} and {exps.numel()}")
     if codes.dtype != torch.uint8 or exps.dtype != torch.uint8 or codes.device != exps.device:

@@ -61,11 +61,11 @@ def _params(weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]):
     return tuple(None if t is None else t.detach().to(dtype).contiguous() for t in (weight, bias)) + (dtype,)
 
 
-def _as_saved(t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """A saved tensor (hooks may give back another one with the same values), dense and on 16 bytes."""
-    if t.shape != shape or t.dtype is not dtype or t.device != device:
-        _native._not_as_saved(t, shape, dtype, device)
-    if not t.is_contiguous() or t.data_ptr() & 15:
+def _as_saved(t: torch.Tensor, count: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A saved vector (hooks may give back another one with the same values), dense and on 16 bytes."""
+    if t.shape != (count,) or t.dtype is not dtype or t.device != device:
+        _native._not_as_saved(t, (count,), dtype, device)
+    if t.data_ptr() & 15 or not t.is_contiguous():
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -74,37 +74,47 @@ class GroupNormActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, activation, slope, fmt):
         w, b, pdtype = _params(weight, bias)
-        desc = _native.gn_desc(x, groups, pdtype, eps, activation, slope)
-        y, mean_rstd, codes, exps = _native.gn_forward(x, desc, w, b, fmt)
+        args = x.shape, groups, x.dtype, pdtype, eps, activation, slope
+        y, mean_rstd, codes, exps = _native.gn_forward(x, _native.gn_plan(*args), w, b, fmt)
         ctx.save_for_backward(x if fmt is None else codes, exps, mean_rstd, weight, bias)
-        ctx.desc, ctx.fmt = desc, fmt
-        ctx.was = x.shape, x.dtype, x.device
+        ctx.args, ctx.fmt, ctx.device = args, fmt, x.device
         return y
 
     @staticmethod
     def backward(ctx, gy):
         refuse_twice()
         x, exps, mean_rstd, weight, bias = ctx.saved_tensors
-        desc, fmt, (shape, dtype, device) = ctx.desc, ctx.fmt, ctx.was
+        args, fmt, device = ctx.args, ctx.fmt, ctx.device
+        shape, dtype = args[0], args[2]
         if fmt is None:
             if x.shape != shape or x.dtype is not dtype or x.device != device:
                 _native._not_as_saved(x, shape, dtype, device)
             x = _channels_last(x)
         else:
             count = shape.numel()
-            x = _as_saved(x, (count,), torch.uint8, device)
-            exps = _as_saved(exps, (-(-count // _native.Q8_BLOCK),), torch.uint8, device)
-        mean_rstd = _as_saved(mean_rstd, (2 * desc.samples * desc.groups,), torch.float32, device)
-        for t in (weight, bias):
-            if t is not None and (t.shape != (desc.channels,) or t.device != device):
-                _native._not_as_saved(t, (desc.channels,), t.dtype, device)
+            x = _as_saved(x, count, torch.uint8, device)
+            exps = _as_saved(exps, -(-count // _native.Q8_BLOCK), torch.uint8, device)
         w, b, pdtype = _params(weight, bias)
-        desc.param_dtype = _native.dtype_code(pdtype)
-        gy = _channels_last(gy if gy.dtype is dtype else gy.to(dtype))
+        for t in (w, b):
+            if t is not None and (t.shape[0] != shape[1] or t.device != device):
+                _native._not_as_saved(t, (shape[1],), pdtype, device)
+        if pdtype is not args[3]:
+            args = (*args[:3], pdtype, *args[4:])
+        plan = _native.gn_plan(*args)
+        mean_rstd = _as_saved(mean_rstd, plan.stats, torch.float32, device)
+        if gy.dtype is not dtype:
+            gy = gy.to(dtype)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx, dw, db = _native.gn_backward(gy, desc, x, fmt or 0, exps, mean_rstd, w, b, need_x, need_w or need_b)
-        dw = dw.to(weight.dtype) if need_w else None
-        db = db.to(bias.dtype) if need_b else None
+        dx, dw, db = _native.gn_backward(_channels_last(gy), plan, x, fmt or 0, exps, mean_rstd, w, b, need_x,
+                                         need_w or need_b)
+        if not need_w:
+            dw = None
+        elif weight.dtype is not torch.float32:
+            dw = dw.to(weight.dtype)
+        if not need_b:
+            db = None
+        elif bias.dtype is not torch.float32:
+            db = db.to(bias.dtype)
         return dx, dw, db, None, None, None, None, None
 
 
@@ -165,7 +175,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
         fmt = None if checkpoint is None else _native.Q8_FORMATS[checkpoint]
         return GroupNormActFn.apply(x, weight, bias, num_groups, eps, code, negative_slope, fmt)
     w, b, pdtype = _params(weight, bias)
-    return _native.gn_forward(x, _native.gn_desc(x, num_groups, pdtype, eps, code, negative_slope), w, b, None)[0]
+    return _native.gn_forward(x, _native.gn_plan(x.shape, num_groups, x.dtype, pdtype, eps, code, negative_slope), w, b,
+                              None)[0]
 
 
 def _act_torch(z, activation, slope):
