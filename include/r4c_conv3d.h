@@ -457,7 +457,8 @@ int r4c_unpack8(const void* codes, const void* exponents, int64_t count, int dty
  *   mean, rstd of a (sample, group): biased variance, rstd = (var + eps)^-1/2
  *   y = act((x - mean) * (rstd * gamma) + beta)
  * gamma, beta (channels each, both param_dtype) may be null: 1 and 0. x, y,
- * dy, dx bf16, fp16 or fp32 (dtype), 16-byte aligned; arithmetic in fp32,
+ * dy, dx bf16, fp16 or fp32 (dtype), 16-byte aligned, as are codes and the
+ * exponents that the backward takes; arithmetic in fp32,
  * sums across threads in fp64 and in a fixed order. mean_rstd: (mean, rstd)
  * per sample and group, 2 * samples * groups floats, written by the forward
  * and read by the backward.

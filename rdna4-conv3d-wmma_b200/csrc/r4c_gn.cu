@@ -12,6 +12,7 @@ namespace {
 struct Plan {
   Geo g;
   int V, threads;
+  int stats_nb;
 };
 
 bool ok_desc(const r4c_gn_desc* d) {
@@ -60,12 +61,19 @@ void plan_small(const r4c_gn_desc* d, bool backward, int V, Geo& g, int* threads
   }
 }
 
+// Blocks a sample so that all fill the SMs once, `fit` on each, and a thread has four rows or more.
+int blocks_for(const Geo& g, int64_t samples, int fit) {
+  const int64_t want = std::max<int64_t>(1, 148 * fit / std::max<int64_t>(1, samples * g.tiles));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (g.rows + 4 * g.R - 1) / (4 * g.R)));
+}
+
 // How the blocks share the data; false where a count passes a launch's limits.
 bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
   Geo& g = pl->g;
   const int64_t C = d->channels;
   if (d->inner > INT64_MAX / 8 / C || (d->samples && d->inner * C > INT64_MAX / 8 / d->samples)) return false;
   g.sample = d->inner * C;
+  g.samples = d->samples;
   g.C = d->channels;
   g.G = d->groups;
   g.Cg = g.C / g.G;
@@ -74,7 +82,8 @@ bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
   g.slope = d->slope;
   g.act = d->activation;
   g.pdtype = d->param_dtype;
-  g.format = g.pack = 0;
+  g.format = g.pack = g.wide_params = 0;
+  pl->stats_nb = 1;
   // the widest vector whose rows of lcm(C, V) elements divide a sample; several voxels in a row only while such a
   // row fits a block's threads
   int V = 16 / (int)dtype_bytes(d->dtype);
@@ -89,6 +98,8 @@ bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
   if (g.rows > 0) plan_small(d, backward, V, g, &pl->threads);
   if (g.small) {
     g.blocks = d->samples * g.nb;
+    g.chunk_tiles = g.small;
+    g.np = g.nb * g.tiles;
     return g.blocks + g.C <= INT32_MAX;
   }
   const int lanes = g.L / V;
@@ -97,15 +108,14 @@ bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
   g.R = std::max(1, kThreads / g.lanes);
   if (g.R > 4) g.R = g.R / 4 * 4;       // a tile of rows starts at a block of 32 elements (fused packing)
   pl->threads = cdiv(g.R * g.lanes, 32) * 32;
-  // one wave of the blocks that fit the SMs (the kernels' __launch_bounds__), none with less than four rows for each
-  // thread
-  const int64_t fit = 148 * (backward ? 2 : 3);
-  const int64_t want = std::max<int64_t>(1, fit / std::max<int64_t>(1, d->samples * g.tiles));
-  g.nb = (int)std::max<int64_t>(1, std::min<int64_t>(want, (g.rows + 4 * g.R - 1) / (4 * g.R)));
-  g.chunk = ((g.rows + g.nb - 1) / g.nb + g.R - 1) / g.R * g.R;
-  if (g.chunk > 0) g.nb = (int)std::max<int64_t>(1, (g.rows + g.chunk - 1) / g.chunk);
-  g.blocks = d->samples * g.nb;
-  return g.blocks + g.C <= INT32_MAX && g.tiles <= 65535 && g.chunk / g.R < INT32_MAX;
+  // one wave of the blocks that fit the SMs, none with less than four rows for each thread
+  pl->stats_nb = blocks_for(g, d->samples, kStatsBlocks);
+  g = split(g, blocks_for(g, d->samples, backward ? kBwdBlocks : kApplyBlocks));
+  const Geo sums = split(g, pl->stats_nb);
+  pl->stats_nb = sums.nb;
+  g.np = (backward ? g.nb : sums.nb) * g.tiles;
+  const int64_t most = std::max(g.blocks, sums.blocks);
+  return most + g.C <= INT32_MAX && g.tiles <= 65535 && g.rows / g.R < INT32_MAX;
 }
 
 // Whether a block of 32 elements is 32 / V neighbouring threads' in every tile of rows, so that the forward can write
@@ -117,9 +127,16 @@ bool fused_pack(const Plan& pl, size_t elem) {
   return g.C % r4c::q8::kBlock == 0 && g.lanes * pl.V % r4c::q8::kBlock == 0;
 }
 
-size_t fwd_bytes(const Geo& g) { return align_up((size_t)g.blocks * g.tiles * g.G * sizeof(double2), 256); }
+size_t fwd_bytes(const Plan& pl) {
+  return align_up((size_t)(pl.g.blocks / pl.g.nb) * pl.stats_nb * pl.g.tiles * pl.g.G * sizeof(double2), 256);
+}
 size_t cpart_bytes(const Geo& g) { return align_up((size_t)g.blocks * g.C * sizeof(float2), 256); }
 size_t gpart_bytes(const Geo& g) { return align_up((size_t)g.blocks * g.tiles * g.G * sizeof(float2), 256); }
+
+// Parameters as fp32 words of four: a thread's channels follow each other where a row is one voxel.
+int wide_params(const Geo& g, const void* gamma, const void* beta) {
+  return g.pdtype == R4C_F32 && g.L == g.C && ((reinterpret_cast<uintptr_t>(gamma) | reinterpret_cast<uintptr_t>(beta)) & 15) == 0;
+}
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -137,7 +154,7 @@ size_t r4c_gn_workspace_size(const r4c_gn_desc* desc, int backward) {
   Plan pl;
   if (!ok_desc(desc) || !make_plan(desc, backward != 0, &pl)) return 0;
   if (backward) return cpart_bytes(pl.g) + gpart_bytes(pl.g);
-  return pl.g.small ? 0 : fwd_bytes(pl.g);
+  return pl.g.small ? 0 : fwd_bytes(pl);
 }
 
 int r4c_gn_fwd(const r4c_gn_desc* desc, const void* x, const void* gamma, const void* beta, void* y, float* mean_rstd,
@@ -149,7 +166,7 @@ int r4c_gn_fwd(const r4c_gn_desc* desc, const void* x, const void* gamma, const 
   if (!x || !y || !mean_rstd || (codes == nullptr) != (exponents == nullptr)) return R4C_ERR_INVALID;
   if (codes && format != R4C_Q8_INT8 && format != R4C_Q8_E4M3) return R4C_ERR_INVALID;
   if (!aligned(x) || !aligned(y) || !aligned(codes) || !aligned(ws)) return R4C_ERR_ALIGN;
-  if (!pl.g.small && (!ws || ws_bytes < fwd_bytes(pl.g))) return R4C_ERR_WORKSPACE;
+  if (!pl.g.small && (!ws || ws_bytes < fwd_bytes(pl))) return R4C_ERR_WORKSPACE;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   FwdArgs a;
   a.x = x;
@@ -158,6 +175,8 @@ int r4c_gn_fwd(const r4c_gn_desc* desc, const void* x, const void* gamma, const 
   a.y = y;
   a.mean_rstd = reinterpret_cast<float2*>(mean_rstd);
   a.part = static_cast<double2*>(ws);
+  a.stats_nb = pl.stats_nb;
+  pl.g.wide_params = wide_params(pl.g, gamma, beta);
   a.codes = static_cast<uint8_t*>(codes);
   a.exps = static_cast<uint8_t*>(exponents);
   pl.g.format = format;
@@ -186,7 +205,7 @@ int r4c_gn_bwd(const r4c_gn_desc* desc, const void* dy, const void* x, int forma
   if (!make_plan(desc, true, &pl)) return R4C_ERR_TOO_LARGE;
   if (!dy || !x || !mean_rstd) return R4C_ERR_INVALID;
   if (exponents && format != R4C_Q8_INT8 && format != R4C_Q8_E4M3) return R4C_ERR_INVALID;
-  if (!aligned(dy) || !aligned(x) || !aligned(dx) || !aligned(ws)) return R4C_ERR_ALIGN;
+  if (!aligned(dy) || !aligned(x) || !aligned(exponents) || !aligned(dx) || !aligned(ws)) return R4C_ERR_ALIGN;
   if (!ws || ws_bytes < cpart_bytes(pl.g) + gpart_bytes(pl.g)) return R4C_ERR_WORKSPACE;
   if (!dx && !dgamma && !dbeta) return R4C_OK;
   BwdArgs a;
@@ -202,6 +221,7 @@ int r4c_gn_bwd(const r4c_gn_desc* desc, const void* dy, const void* x, int forma
   a.cpart = static_cast<float2*>(ws);
   a.gpart = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) + cpart_bytes(pl.g));
   pl.g.format = format;
+  pl.g.wide_params = wide_params(pl.g, gamma, beta);
   if (desc->dtype == R4C_BF16) return status(launch_bwd<__nv_bfloat16>(a, pl.g, pl.V, pl.threads, s));
   if (desc->dtype == R4C_F16) return status(launch_bwd<__half>(a, pl.g, pl.V, pl.threads, s));
   return status(launch_bwd<float>(a, pl.g, pl.V, pl.threads, s));

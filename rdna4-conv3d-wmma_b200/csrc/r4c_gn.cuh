@@ -21,6 +21,8 @@
 // fp64 about zero, in a fixed order: same bits on every run.
 #pragma once
 
+#include <algorithm>
+
 #include "r4c_internal.h"
 #include "r4c_q8.cuh"
 
@@ -30,13 +32,17 @@ namespace gn {
 constexpr int kThreads = 256;   // at most, per block
 // Samples that a cluster keeps in registers: vectors of a thread at most (forward; backward, which keeps dy too),
 // groups of a channel tile at most (shared memory).
+// Blocks that fit an SM beside each other (the registers that each kernel may take follow from it).
+constexpr int kStatsBlocks = 4, kApplyBlocks = 4, kBwdBlocks = 3;
+// Vectors of a thread on their way at a time, plus one.
+constexpr int kFwdAhead = 8, kBwdAhead = 4;
 constexpr int kSmallFwd = 16, kSmallBwd = 8, kSmallGroups = 256;
 
 struct Geo {
   int64_t sample;    // elements of a sample, S * C
   int64_t rows;      // rows of L elements of a sample
   int64_t chunk;     // rows of a block, a multiple of R
-  int64_t blocks;    // samples * nb: blocks of one channel tile
+  int64_t samples, blocks;   // blocks of one channel tile: samples * nb
   double inv_m;      // 1 / (Cg * S)
   float eps, slope;
   int act, pdtype, format;
@@ -44,10 +50,22 @@ struct Geo {
   int lanes;         // vectors of a row in a channel tile (L / V when there is one tile)
   int tiles;
   int R;             // rows that a block's threads cover at a time
+  int chunk_tiles;   // chunk / R
   int nb;            // blocks of a sample and channel tile (the cluster's, where one keeps a sample)
+  int np;            // parts of a sample's sums that the second pass reads: blocks of the first times channel tiles
+  int wide_params;   // w and b are fp32 on 16 bytes, and a thread's channels follow each other
   int pack;          // the forward writes x in 8 bits too
   int small;         // vectors that a thread keeps in registers (small samples), or 0: two passes
 };
+
+// The same data in another number of blocks a sample.
+inline Geo split(Geo g, int nb) {
+  g.chunk = std::max<int64_t>(1, ((g.rows + nb - 1) / nb + g.R - 1) / g.R) * g.R;
+  g.chunk_tiles = (int)(g.chunk / g.R);
+  g.nb = (int)std::max<int64_t>(1, (g.rows + g.chunk - 1) / g.chunk);
+  g.blocks = g.samples * g.nb;
+  return g;
+}
 
 // V elements of T, moved as one word; in fp32 as pairs, for the packed arithmetic (two fp32 an instruction: half the
 // issue slots, which bound these kernels before the memory does).
@@ -148,6 +166,82 @@ struct Source<T, V, true> {
     q8::decode<T, V>(c, byte, format, e);
 #pragma unroll
     for (int k = 0; k < kPairs<V>; ++k) f[k] = make_float2(e[2 * k], V > 1 ? e[V > 1 ? 2 * k + 1 : 0] : 0.f);
+  }
+};
+
+__device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// A copy of BYTES bytes into shared memory that runs beside the thread (two bytes, which the hardware has no such copy
+// for, are moved at once).
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+  if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  } else if constexpr (BYTES >= 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+  } else if constexpr (BYTES == 2) {
+    const uint16_t v = *static_cast<const uint16_t*>(from);
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
+  } else {
+    const uint32_t v = *static_cast<const uint8_t*>(from);
+    asm volatile("st.shared.u8 [%0], %1;" ::"r"(to), "r"(v) : "memory");
+  }
+}
+
+// A thread's next vectors of x (and dy), D of them on their way in its own slots of shared memory: what the memory's
+// latency needs in flight (some 100 KB an SM) costs no registers, and no thread waits for another.
+template <typename T, int V, bool Q, bool DY, int D>
+struct Ring {
+  static constexpr int XB = V * (Q ? 1 : (int)sizeof(T)), YB = V * (int)sizeof(T);
+  static constexpr int kDy = D * kThreads * XB, kExp = kDy + (DY ? D * kThreads * YB : 0);
+  static constexpr int kBytes = kExp + (Q ? D * kThreads * 4 : 0);
+  const char *x, *dy;             // this thread's first vector
+  const uint8_t* exps;
+  int64_t at, count;              // its index, and the elements of x (for the exponents' end)
+  int64_t step;
+  uint32_t slot;
+
+  __device__ __forceinline__ Ring(void* smem, const void* x_, const T* dy_, const uint8_t* exps_, int64_t at_,
+                                  int64_t step_, int64_t count_) {
+    at = at_;
+    step = step_;
+    x = static_cast<const char*>(x_) + at * (Q ? 1 : (int)sizeof(T));
+    dy = DY ? reinterpret_cast<const char*>(dy_ + at) : nullptr;
+    exps = exps_;
+    count = count_;
+    slot = shared_at(smem);
+  }
+  // starts vector t, if the thread has it
+  __device__ __forceinline__ void start(int t, bool has) {
+    if (has) {
+      const int i = t & (D - 1);
+      copy_async<XB>(slot + (i * kThreads + threadIdx.x) * XB, x + t * step * (Q ? 1 : (int)sizeof(T)));
+      if constexpr (DY) copy_async<YB>(slot + kDy + (i * kThreads + threadIdx.x) * YB, dy + t * step * (int)sizeof(T));
+      if constexpr (Q) {
+        // the word that holds the block's exponent, as far as the array goes
+        const int64_t e = (at + t * step) / q8::kBlock & ~(int64_t)3;
+        const int64_t left = (count + q8::kBlock - 1) / q8::kBlock - e;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(slot + kExp + (i * kThreads + threadIdx.x) * 4),
+                     "l"(exps + e), "r"(left < 4 ? (int)left : 4) : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // the oldest has landed (D - 1 were started after it was the newest)
+  __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory"); }
+  __device__ __forceinline__ void drain() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+  __device__ __forceinline__ void get(int t, Source<T, V, Q>& v, char* smem) const {
+    const int i = (t & (D - 1)) * kThreads + threadIdx.x;
+    if constexpr (Q) {
+      v.c = q8::load_codes<V>(reinterpret_cast<const uint8_t*>(smem) + i * XB);
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + kExp + i * 4);
+      v.byte = (w >> (8 * (int)((at + t * step) / q8::kBlock & 3))) & 0xff;
+    } else {
+      v.v.load(reinterpret_cast<const T*>(smem + i * XB));
+    }
+  }
+  __device__ __forceinline__ void get_dy(int t, Vec<T, V>& d, char* smem) const {
+    d.load(reinterpret_cast<const T*>(smem + kDy + ((t & (D - 1)) * kThreads + threadIdx.x) * YB));
   }
 };
 
@@ -274,40 +368,75 @@ __device__ __forceinline__ void act_grads(float2 (&dy)[P], const float2 (&z)[P],
   }
 }
 
-// Where a block's threads stand: sample n, part b of it, channel tile, and a thread's lane and row; its rows are
-// row, row + R, .. of the block's `count` tiles of R rows from r0 on.
+// Where a block's threads stand: sample n, part b of it, channel tile, and a thread's lane and row. A thread's rows are
+// row, row + R, .. of the block's rows: one in each of the first `mine` of its `tiles` tiles of R rows. Divisions by
+// run-time sizes cost tens of instructions, which a short kernel feels: each thread makes two, the rest is counted up.
 struct Place {
-  int64_t n, r0, left;  // left: rows of the block
+  int64_t n;
   int64_t at;           // the thread's first element
-  int64_t step;         // elements from one tile to the next
-  int tiles;            // of R rows
+  int64_t step;         // elements from one tile of rows to the next
+  int tiles, mine;
   int b, tile, lane, row;
   int j0, j1;           // the channel tile's elements of a row
-  int ga, gb;           // its groups
+  int c, gi, in_group;  // the thread's first channel, its group and its place there
+  int ga, gb;           // the channel tile's groups
   bool active;
-  // whether tile t holds a row for this thread
-  __device__ __forceinline__ bool in(int t, int R) const { return active && (int64_t)t * R + row < left; }
 };
 template <int V>
 __device__ __forceinline__ Place place(const Geo& g) {
   Place p;
-  p.n = blockIdx.x / g.nb;
-  p.b = (int)(blockIdx.x - p.n * g.nb);
+  if (g.nb == 1) {
+    p.n = blockIdx.x;
+    p.b = 0;
+  } else {
+    const unsigned n = blockIdx.x / (unsigned)g.nb;
+    p.n = n;
+    p.b = (int)(blockIdx.x - n * g.nb);
+  }
   p.tile = blockIdx.y;
-  p.lane = threadIdx.x % g.lanes;
-  p.row = threadIdx.x / g.lanes;
+  p.row = (int)(threadIdx.x / (unsigned)g.lanes);
+  p.lane = (int)threadIdx.x - p.row * g.lanes;
   p.j0 = p.tile * g.lanes * V;
   p.j1 = min(p.j0 + g.lanes * V, g.L);
-  p.ga = g.tiles == 1 ? 0 : p.j0 / g.Cg;
-  p.gb = g.tiles == 1 ? g.G : (p.j1 - 1) / g.Cg + 1;
-  p.active = p.row < g.R && p.j0 + p.lane * V < p.j1;
-  p.r0 = p.b * g.chunk;
-  p.left = min(g.chunk, g.rows - p.r0);
-  p.tiles = p.left > 0 ? (int)((p.left + g.R - 1) / g.R) : 0;
-  p.at = p.n * g.sample + (p.r0 + p.row) * g.L + p.j0 + p.lane * V;
+  const int j = p.j0 + p.lane * V;
+  p.active = p.row < g.R && j < p.j1;
+  p.c = g.L == g.C ? j : (int)((unsigned)j % (unsigned)g.C);
+  p.gi = (int)((unsigned)p.c / (unsigned)g.Cg);
+  p.in_group = p.c - p.gi * g.Cg;
+  if (g.tiles == 1) {
+    p.ga = 0;
+    p.gb = g.G;
+  } else {
+    p.ga = (int)((unsigned)p.j0 / (unsigned)g.Cg);
+    p.gb = (int)((unsigned)(p.j1 - 1) / (unsigned)g.Cg) + 1;
+  }
+  const int64_t r0 = p.b * g.chunk;
+  const int64_t left = min(g.chunk, g.rows - r0);
+  p.tiles = left == g.chunk ? g.chunk_tiles : left > 0 ? (int)((left + g.R - 1) / g.R) : 0;
+  const int64_t last = left - (int64_t)(p.tiles - 1) * g.R;    // rows of the last tile
+  p.mine = p.active ? p.tiles - (p.row < last ? 0 : 1) : 0;
+  if (p.mine < 0) p.mine = 0;
+  p.at = p.n * g.sample + (r0 + p.row) * g.L + j;
   p.step = (int64_t)g.R * g.L;
   return p;
 }
+
+// f(column k of the thread, its channel, its group) for its V columns, in order.
+template <int V, typename F>
+__device__ __forceinline__ void each_column(const Geo& g, const Place& p, F f) {
+  int c = p.c, gi = p.gi, in = p.in_group;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    f(k, c, gi);
+    ++c;
+    if (++in == g.Cg) {
+      in = 0;
+      ++gi;
+    }
+    if (c == g.C) c = gi = in = 0;
+  }
+}
+__device__ __forceinline__ void put(float2* f, int k, float v) { (k & 1 ? f[k / 2].y : f[k / 2].x) = v; }
 
 // Neighbouring threads for each of `items` sums: the largest power of two that the block has, at most a warp.
 __device__ __forceinline__ int threads_per(int items, int threads) {
@@ -326,18 +455,25 @@ __device__ __forceinline__ void join(S& a, S& b, int width) {
   }
 }
 
-// f(item, a, c) -> adds item's terms of thread `sub` of `tp`; g(item, a, c) gets the sums. Every thread of the block
-// calls it (the shuffles need whole warps; blocks are multiples of 32 threads).
+// f(item, sub, tp, a, c) adds the terms of item that are thread `sub`'s of `tp`; out(item, a, c) gets the sums. Every
+// thread of the block calls it (the shuffles need whole warps; blocks are multiples of 32 threads).
 template <typename S, typename F, typename Out>
 __device__ __forceinline__ void each_sum(int items, F f, Out out) {
-  const int tp = threads_per(items, blockDim.x), sub = threadIdx.x % tp, per = blockDim.x / tp;
+  const int tp = threads_per(items, blockDim.x), sub = threadIdx.x & (tp - 1);
+  const int first = threadIdx.x / tp, per = blockDim.x / tp;    // (tp is a power of two)
   for (int base = 0; base < items; base += per) {
-    const int i = base + threadIdx.x / tp;
+    const int i = base + first;
     S a = 0, c = 0;
     if (i < items) f(i, sub, tp, a, c);
     join(a, c, tp);
     if (i < items && sub == 0) out(i, a, c);
   }
+}
+// each_sum's threads of an item shared out over columns and rows of a table: the rows' share.
+__device__ __forceinline__ int row_threads(int tp, int rows) {
+  int t = 1;
+  while (2 * t <= tp && 2 * t <= rows) t *= 2;
+  return t;
 }
 
 // Launched while the kernel before it may still run: what that one wrote may be read from here on.
@@ -351,23 +487,46 @@ struct Affine {
   __device__ __forceinline__ void params(const Geo& g, const Place& p, const void* gamma, const void* beta) {
 #pragma unroll
     for (int k = 0; k < kPairs<V>; ++k) {
-      nmu[k] = a[k] = b[k] = two(0.f);
-      if (!p.active) continue;
-      const int c0 = (p.j0 + p.lane * V + 2 * k) % g.C, c1 = V > 1 ? (p.j0 + p.lane * V + 2 * k + 1) % g.C : c0;
-      a[k] = make_float2(param(gamma, g.pdtype, c0, 1.f), param(gamma, g.pdtype, c1, 1.f));
-      b[k] = make_float2(param(beta, g.pdtype, c0, 0.f), param(beta, g.pdtype, c1, 0.f));
+      nmu[k] = b[k] = two(0.f);
+      a[k] = two(1.f);
+    }
+    if (!p.active) return;
+    if (V % 4 == 0 && g.wide_params) {          // fp32, on 16 bytes, channels without a wrap
+#pragma unroll
+      for (int k = 0; k < V / 4; ++k) {
+        if (gamma) {
+          const float4 v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(gamma) + p.c) + k);
+          a[2 * k] = make_float2(v.x, v.y);
+          a[2 * k + 1] = make_float2(v.z, v.w);
+        }
+        if (beta) {
+          const float4 v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(beta) + p.c) + k);
+          b[2 * k] = make_float2(v.x, v.y);
+          b[2 * k + 1] = make_float2(v.z, v.w);
+        }
+      }
+    } else {
+      each_column<V>(g, p, [&](int k, int c, int) {
+        put(a, k, param(gamma, g.pdtype, c, 1.f));
+        put(b, k, param(beta, g.pdtype, c, 0.f));
+      });
     }
   }
   template <typename Stat>
   __device__ __forceinline__ void stats(const Geo& g, const Place& p, Stat stat) {
     if (!p.active) return;
+    float2 r[kPairs<V>];
+    if constexpr (V == 1) r[0] = two(0.f);
+    float2 q = make_float2(0.f, 0.f);
+    int have = -1;
+    each_column<V>(g, p, [&](int k, int, int gi) {
+      if (gi != have) q = stat(gi);
+      have = gi;
+      put(nmu, k, -q.x);
+      put(r, k, q.y);
+    });
 #pragma unroll
-    for (int k = 0; k < kPairs<V>; ++k) {
-      const int c0 = (p.j0 + p.lane * V + 2 * k) % g.C, c1 = V > 1 ? (p.j0 + p.lane * V + 2 * k + 1) % g.C : c0;
-      const float2 q = stat(c0 / g.Cg), r = stat(c1 / g.Cg);
-      nmu[k] = make_float2(-q.x, -r.x);
-      a[k] = __fmul2_rn(a[k], make_float2(q.y, r.y));
-    }
+    for (int k = 0; k < kPairs<V>; ++k) a[k] = __fmul2_rn(a[k], r[k]);
   }
 };
 
@@ -412,68 +571,91 @@ struct Moments {
 template <typename T, int V, typename Out>
 __device__ __forceinline__ void block_moments(const Geo& g, const Place& p, const Moments<T, V>& m,
                                               double2* __restrict__ red, Out out) {
+  // a thread whose columns all belong to one group adds them first
+  const bool merged = V > 1 && g.L == g.C && (g.Cg & (V - 1)) == 0;
+  if (merged) {
+    double2 t = m.sums(0);
 #pragma unroll
-  for (int k = 0; k < V; ++k) red[k * kThreads + threadIdx.x] = m.sums(k);
+    for (int k = 1; k < V; ++k) {
+      const double2 v = m.sums(k);
+      t.x += v.x;
+      t.y += v.y;
+    }
+    red[threadIdx.x] = t;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) red[k * kThreads + threadIdx.x] = m.sums(k);
+  }
   __syncthreads();
-  const int reps = g.L / g.C;
-  each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
-    const int gi = p.ga + i;
-    const int lo = max(gi * g.Cg, g.tiles == 1 ? 0 : p.j0), hi = min((gi + 1) * g.Cg, g.tiles == 1 ? g.C : p.j1);
-    const int w = hi - lo, total = reps * w * g.R;
-    for (int e = sub; e < total; e += tp) {
-      const int row = e % g.R, q = e / g.R;
-      const int j = (q / w) * g.C + lo + q % w - p.j0;
-      const double2 v = red[(j % V) * kThreads + row * g.lanes + j / V];
-      a += v.x;
-      c += v.y;
+  const int tp = threads_per(p.gb - p.ga, blockDim.x), tr = row_threads(tp, g.R), tc = tp / tr;
+  each_sum<double>(p.gb - p.ga, [&](int i, int sub, int, double& a, double& c) {
+    const int gi = p.ga + i, sr = sub & (tr - 1), sc = sub / tr;
+    int lo = gi * g.Cg, hi = lo + g.Cg;
+    if (g.tiles > 1) {
+      lo = max(lo, p.j0) - p.j0;
+      hi = min(hi, p.j1) - p.j0;
+    }
+    if (merged) {
+      for (int l = lo / V + sc; l < hi / V; l += tc)
+        for (int r = sr; r < g.R; r += tr) {
+          const double2 v = red[r * g.lanes + l];
+          a += v.x;
+          c += v.y;
+        }
+    } else {
+      for (int base = 0; base < g.L; base += g.C)         // once, unless a row holds several voxels
+        for (int j = base + lo + sc; j < base + hi; j += tc)
+          for (int r = sr; r < g.R; r += tr) {
+            const double2 v = red[(j % V) * kThreads + r * g.lanes + j / V];
+            a += v.x;
+            c += v.y;
+          }
     }
   }, [&](int i, double a, double c) { out(p.ga + i, a, c); });
 }
 
+// (var + eps)^-1/2 from the fp32 reciprocal root and one step of Newton's method in fp64 (2^-22 becomes 2^-43; an fp64
+// root and division would be a hundred instructions in a row).
 __device__ __forceinline__ float2 mean_rstd_of(const Geo& g, double a, double c) {
   const double mean = a * g.inv_m;
   double var = c * g.inv_m - mean * mean;
   if (var < 0.0) var = 0.0;
-  return make_float2((float)mean, (float)(1.0 / sqrt(var + (double)g.eps)));
+  const double v = var + (double)g.eps;
+  const float f = (float)v, r0 = rsqrtf(f);
+  if (!(f >= 1e-30f && f <= 1e30f)) return make_float2((float)mean, (float)(1.0 / sqrt(v)));
+  const double r = r0;
+  return make_float2((float)mean, (float)(r * (1.5 - 0.5 * v * r * r)));
 }
 
 // part[((n * nb + b) * tiles + tile) * G + g] = (sum x, sum x^2) of the block's share of group g.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, 4) stats_kernel(const T* __restrict__ x, const __grid_constant__ Geo g,
-                                                            double2* __restrict__ part) {
-  constexpr int U = 4;
-  __shared__ double2 red[V * kThreads];
+__global__ void __launch_bounds__(kThreads, kStatsBlocks) stats_kernel(const T* __restrict__ x,
+                                                                       const __grid_constant__ Geo g,
+                                                                       double2* __restrict__ part) {
+  using R = Ring<T, V, false, false, kFwdAhead>;
+  __shared__ __align__(16) char smem[R::kBytes > V * kThreads * 16 ? R::kBytes : V * kThreads * 16];
   let_next_start();
   const Place p = place<V>(g);
+  R ring(smem, x, nullptr, nullptr, p.at, p.step, 0);
+#pragma unroll
+  for (int t = 0; t < kFwdAhead - 1; ++t) ring.start(t, t < p.mine);
   Moments<T, V> m;
   m.zero();
-  if (p.in(0, g.R)) {
-    const T* src = x + p.at;
-    {
-      Vec<T, V> a;
-      a.load(src);
-      m.pivot(a);
-    }
-    int t = 0;
-    for (; t + U < p.tiles; t += U, src += U * p.step) {      // whole tiles: the last one comes below
-      Vec<T, V> a[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) a[u].load(src + u * p.step);
-#pragma unroll
-      for (int u = 0; u < U; ++u) m.add(a[u]);
-    }
-    for (; t < p.tiles; ++t, src += p.step)
-      if (p.in(t, g.R)) {
-        Vec<T, V> a;
-        a.load(src);
-        m.add(a);
-      }
+  for (int t = 0; t < p.mine; ++t) {
+    Source<T, V, false> a;
+    ring.wait();
+    ring.get(t, a, smem);
+    ring.start(t + kFwdAhead - 1, t + kFwdAhead - 1 < p.mine);
+    if (t == 0) m.pivot(a.v);
+    m.add(a.v);
   }
+  ring.drain();
+  __syncthreads();
   double2* out = part + ((int64_t)blockIdx.x * g.tiles + p.tile) * g.G;
   if (g.tiles > 1)
     for (int i = threadIdx.x; i < g.G; i += blockDim.x)
       if (i < p.ga || i >= p.gb) out[i] = make_double2(0.0, 0.0);
-  block_moments<T, V>(g, p, m, red, [&](int gi, double a, double c) { out[gi] = make_double2(a, c); });
+  block_moments<T, V>(g, p, m, reinterpret_cast<double2*>(smem), [&](int gi, double a, double c) { out[gi] = make_double2(a, c); });
 }
 
 // y of one vector, and its 8 bits (PACK: a block of 32 elements lies in 32 / V neighbouring threads, all with or all
@@ -506,23 +688,26 @@ __device__ __forceinline__ void apply_one(const Vec<T, V>& v, const Affine<V>& k
 
 // From the last row to the first: what the sums read last is what the L2 cache still has.
 template <typename T, int V, int ACT, bool PACK>
-__global__ void __launch_bounds__(kThreads, 3) apply_kernel(const T* __restrict__ x, const void* __restrict__ gamma,
-                                                            const void* __restrict__ beta,
-                                                            const __grid_constant__ Geo g,
-                                                            const double2* __restrict__ part,
-                                                            float2* __restrict__ mean_rstd, T* __restrict__ y,
-                                                            uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
-  constexpr int U = 4;
-  extern __shared__ float2 stat[];
+__global__ void __launch_bounds__(kThreads, kApplyBlocks) apply_kernel(
+    const T* __restrict__ x, const void* __restrict__ gamma, const void* __restrict__ beta,
+    const __grid_constant__ Geo g, const double2* __restrict__ part, float2* __restrict__ mean_rstd,
+    T* __restrict__ y, uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
+  using R = Ring<T, V, false, false, kFwdAhead>;
+  extern __shared__ __align__(16) char smem[];
+  float2* stat = reinterpret_cast<float2*>(smem + R::kBytes);
   const Place p = place<V>(g);
+  // (x is older than the kernel before this one)
+  const int end = p.tiles - 1;
+  R ring(smem, x, nullptr, nullptr, p.at + end * p.step, -p.step, 0);
+#pragma unroll
+  for (int t = 0; t < kFwdAhead - 1; ++t) ring.start(t, t <= end && end - t < p.mine);
   Affine<V> k;
   k.params(g, p, gamma, beta);
   wait_for_previous();
-  const int np = g.nb * g.tiles;
-  const double2* src = part + p.n * np * g.G + p.ga;
+  const double2* src = part + p.n * g.np * g.G + p.ga;
   each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
 #pragma unroll 4
-    for (int e = sub; e < np; e += tp) {
+    for (int e = sub; e < g.np; e += tp) {
       const double2 v = src[(int64_t)e * g.G + i];
       a += v.x;
       c += v.y;
@@ -532,18 +717,15 @@ __global__ void __launch_bounds__(kThreads, 3) apply_kernel(const T* __restrict_
   if (p.b == 0)
     for (int i = threadIdx.x; i < p.gb - p.ga; i += blockDim.x) mean_rstd[p.n * g.G + p.ga + i] = stat[i];
   k.stats(g, p, [&](int gi) { return stat[gi - p.ga]; });
-  for (int t = p.tiles - 1; t >= 0; t -= U) {
-    Vec<T, V> v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      v[u].zero();
-      if (t - u >= 0 && p.in(t - u, g.R)) v[u].load(x + p.at + (t - u) * p.step);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (t - u < 0) break;
-      apply_one<T, V, ACT, PACK>(v[u], k, g, p.in(t - u, g.R), p.at + (t - u) * p.step, y, codes, exps);
-    }
+  for (int t = 0; t < p.tiles; ++t) {
+    const int next = t + kFwdAhead - 1;
+    const bool in = end - t < p.mine;
+    Source<T, V, false> v;
+    ring.wait();
+    v.zero();
+    if (in) ring.get(t, v, smem);
+    ring.start(next, next <= end && end - next < p.mine);
+    apply_one<T, V, ACT, PACK>(v.v, k, g, in, p.at + (end - t) * p.step, y, codes, exps);
   }
 }
 
@@ -575,17 +757,17 @@ __device__ __forceinline__ void block_grads(const Geo& g, const Place& p, const 
   for (int k = 0; k < V; ++k)
     red[k * kThreads + threadIdx.x] = k & 1 ? make_float2(s1[k / 2].y, s2[k / 2].y) : make_float2(s1[k / 2].x, s2[k / 2].x);
   __syncthreads();
-  const int ncol = p.j1 - p.j0, reps = g.L / g.C, nch = g.tiles == 1 ? g.C : ncol;
+  const int nch = g.tiles == 1 ? g.C : p.j1 - p.j0;
   each_sum<float>(nch, [&](int i, int sub, int tp, float& a, float& c) {
-    for (int e = sub; e < reps * g.R; e += tp) {
-      const int j = (e / g.R) * g.C + i;
-      const float2 v = red[(j % V) * kThreads + (e % g.R) * g.lanes + j / V];
-      a += v.x;
-      c += v.y;
-    }
+    for (int j = i; j < (g.tiles == 1 ? g.L : nch); j += g.C)
+      for (int r = sub; r < g.R; r += tp) {
+        const float2 v = red[(j % V) * kThreads + r * g.lanes + j / V];
+        a += v.x;
+        c += v.y;
+      }
   }, [&](int i, float a, float c) {
     const int ch = p.j0 + i;
-    const float2 s = make_float2(a, c * stat(ch / g.Cg).y);
+    const float2 s = make_float2(a, c * stat((int)((unsigned)ch / (unsigned)g.Cg)).y);
     cols[i] = s;
     cpart[(int64_t)blockIdx.x * g.C + ch] = s;
   });
@@ -603,63 +785,48 @@ __device__ __forceinline__ void block_grads(const Geo& g, const Place& p, const 
 // cpart[(n * nb + b) * C + c] = (sum dz, sum dz * xh) of the block's rows, and
 // gpart[((n * nb + b) * tiles + tile) * G + g] = the same times w, summed over the tile's channels of the group.
 template <typename T, int V, int ACT, bool Q>
-__global__ void __launch_bounds__(kThreads, 2) bwd_sums_kernel(const T* __restrict__ dy, const void* __restrict__ x,
-                                                               const uint8_t* __restrict__ exps,
-                                                               const float2* __restrict__ mean_rstd,
-                                                               const void* __restrict__ gamma,
-                                                               const void* __restrict__ beta,
-                                                               const __grid_constant__ Geo g,
-                                                               float2* __restrict__ cpart, float2* __restrict__ gpart) {
-  constexpr int U = 4;
-  __shared__ float2 red[V * kThreads];
-  __shared__ float2 cols[V * kThreads];     // per channel of the tile
+__global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_sums_kernel(
+    const T* __restrict__ dy, const void* __restrict__ x, const uint8_t* __restrict__ exps,
+    const float2* __restrict__ mean_rstd, const void* __restrict__ gamma, const void* __restrict__ beta,
+    const __grid_constant__ Geo g, float2* __restrict__ cpart, float2* __restrict__ gpart) {
+  using R = Ring<T, V, Q, true, kBwdAhead>;
+  constexpr int kTable = V * kThreads * (int)sizeof(float2);
+  __shared__ __align__(16) char smem[R::kBytes > 2 * kTable ? R::kBytes : 2 * kTable];
   let_next_start();
   const Place p = place<V>(g);
+  R ring(smem, x, dy, exps, p.at, p.step, g.sample * g.samples);
+#pragma unroll
+  for (int t = 0; t < kBwdAhead - 1; ++t) ring.start(t, t < p.mine);
   const float2* stats = mean_rstd + p.n * g.G;
-  float2 s1[kPairs<V>], s2[kPairs<V>];
+  Affine<V> k;
+  k.params(g, p, gamma, beta);
+  k.stats(g, p, [&](int gi) { return stats[gi]; });
+  float2 a1[kPairs<V>], a2[kPairs<V>];
 #pragma unroll
-  for (int k = 0; k < kPairs<V>; ++k) s1[k] = s2[k] = two(0.f);
-  if (p.in(0, g.R)) {
-    Affine<V> k;
-    k.params(g, p, gamma, beta);
-    k.stats(g, p, [&](int gi) { return stats[gi]; });
-    auto add = [&](const Source<T, V, Q>& v, const Vec<T, V>& d) {
-      float2 xm[kPairs<V>], dz[kPairs<V>];
-      grad_one<T, V, ACT, Q>(v, d, k, g, xm, dz);
+  for (int i = 0; i < kPairs<V>; ++i) a1[i] = a2[i] = two(0.f);
+  for (int t = 0; t < p.mine; ++t) {
+    Source<T, V, Q> v;
+    Vec<T, V> d;
+    ring.wait();
+    ring.get(t, v, smem);
+    ring.get_dy(t, d, smem);
+    ring.start(t + kBwdAhead - 1, t + kBwdAhead - 1 < p.mine);
+    float2 xm[kPairs<V>], dz[kPairs<V>];
+    grad_one<T, V, ACT, Q>(v, d, k, g, xm, dz);
 #pragma unroll
-      for (int i = 0; i < kPairs<V>; ++i) {
-        s1[i] = __fadd2_rn(s1[i], dz[i]);
-        s2[i] = __ffma2_rn(dz[i], xm[i], s2[i]);
-      }
-    };
-    int t = 0;
-    int64_t at = p.at;
-    for (; t + U < p.tiles; t += U, at += U * p.step) {        // whole tiles: the last one comes below
-      Source<T, V, Q> v[U];
-      Vec<T, V> d[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        v[u].load(x, exps, at + u * p.step);
-        d[u].load(dy + at + u * p.step);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) add(v[u], d[u]);
+    for (int i = 0; i < kPairs<V>; ++i) {
+      a1[i] = __fadd2_rn(a1[i], dz[i]);
+      a2[i] = __ffma2_rn(dz[i], xm[i], a2[i]);
     }
-    for (; t < p.tiles; ++t, at += p.step)
-      if (p.in(t, g.R)) {
-        Source<T, V, Q> v;
-        Vec<T, V> d;
-        v.load(x, exps, at);
-        d.load(dy + at);
-        add(v, d);
-      }
   }
+  ring.drain();
+  __syncthreads();
   float2* out = gpart + ((int64_t)blockIdx.x * g.tiles + p.tile) * g.G;
   if (g.tiles > 1)
     for (int i = threadIdx.x; i < g.G; i += blockDim.x)
       if (i < p.ga || i >= p.gb) out[i] = make_float2(0.f, 0.f);
-  block_grads<V>(g, p, s1, s2, gamma, red, cols, cpart, [&](int gi) { return stats[gi]; },
-                 [&](int gi, float a, float c) { out[gi] = make_float2(a, c); });
+  block_grads<V>(g, p, a1, a2, gamma, reinterpret_cast<float2*>(smem), reinterpret_cast<float2*>(smem + kTable), cpart,
+                 [&](int gi) { return stats[gi]; }, [&](int gi, float a, float c) { out[gi] = make_float2(a, c); });
 }
 
 // ---------------------------------------------------------------------------
@@ -732,14 +899,12 @@ __device__ __forceinline__ Vec<T, V> dx_one(const Source<T, V, Q>& v, const Vec<
 template <int V>
 __device__ __forceinline__ void thread_coef(const Geo& g, const Place& p, const float2* coef, float2 (&k1)[kPairs<V>],
                                             float2 (&k2)[kPairs<V>]) {
-#pragma unroll
-  for (int i = 0; i < kPairs<V>; ++i) {
-    const int j = p.j0 + p.lane * V + 2 * i;
-    const float2 q = coef[j % g.C / g.Cg - p.ga];
-    const float2 h = V > 1 ? coef[(j + 1) % g.C / g.Cg - p.ga] : q;
-    k1[i] = make_float2(q.x, h.x);
-    k2[i] = make_float2(q.y, h.y);
-  }
+  if constexpr (V == 1) k1[0] = k2[0] = two(0.f);
+  each_column<V>(g, p, [&](int k, int, int gi) {
+    const float2 q = coef[gi - p.ga];
+    put(k1, k, q.x);
+    put(k2, k, q.y);
+  });
 }
 __device__ __forceinline__ float2 coef_of(const Geo& g, double rstd, double a, double c) {
   return make_float2((float)(rstd * a * g.inv_m), (float)(rstd * rstd * c * g.inv_m));
@@ -747,17 +912,14 @@ __device__ __forceinline__ float2 coef_of(const Geo& g, double rstd, double a, d
 
 // Blocks from g.blocks on sum the parameters' gradients, beside the others.
 template <typename T, int V, int ACT, bool Q>
-__global__ void __launch_bounds__(kThreads, 2) bwd_dx_kernel(const T* __restrict__ dy, const void* __restrict__ x,
-                                                             const uint8_t* __restrict__ exps,
-                                                             const float2* __restrict__ mean_rstd,
-                                                             const void* __restrict__ gamma,
-                                                             const void* __restrict__ beta,
-                                                             const __grid_constant__ Geo g,
-                                                             const float2* __restrict__ cpart,
-                                                             const float2* __restrict__ gpart, T* __restrict__ dx,
-                                                             float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  constexpr int U = 4;
-  extern __shared__ float2 coef[];          // per group of the tile: rstd * A, rstd^2 * B
+__global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
+    const T* __restrict__ dy, const void* __restrict__ x, const uint8_t* __restrict__ exps,
+    const float2* __restrict__ mean_rstd, const void* __restrict__ gamma, const void* __restrict__ beta,
+    const __grid_constant__ Geo g, const float2* __restrict__ cpart, const float2* __restrict__ gpart,
+    T* __restrict__ dx, float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  using R = Ring<T, V, Q, true, kBwdAhead>;
+  extern __shared__ __align__(16) char smem[];
+  float2* coef = reinterpret_cast<float2*>(smem + R::kBytes);   // per group of the tile: rstd * A, rstd^2 * B
   if (blockIdx.x >= g.blocks) {
     wait_for_previous();
     const int warps = blockDim.x / 32;
@@ -767,38 +929,44 @@ __global__ void __launch_bounds__(kThreads, 2) bwd_dx_kernel(const T* __restrict
   }
   const Place p = place<V>(g);
   const float2* stats = mean_rstd + p.n * g.G;
+  // (what it reads is older than the kernel before this one)
+  const int end = p.tiles - 1, skip = p.tiles - p.mine;          // skip: 1 for a thread without a row in the last tile
+  R ring(smem, x, dy, exps, p.at + end * p.step, -p.step, g.sample * g.samples);
+#pragma unroll
+  for (int t = 0; t < kBwdAhead - 1; ++t) ring.start(t, t >= skip && t <= end);
   Affine<V> k;
   k.params(g, p, gamma, beta);
   k.stats(g, p, [&](int gi) { return stats[gi]; });
   wait_for_previous();
-  const int np = g.nb * g.tiles;
-  const float2* src = gpart + p.n * np * g.G + p.ga;
+  const float2* src = gpart + p.n * g.np * g.G + p.ga;
   each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
 #pragma unroll 4
-    for (int e = sub; e < np; e += tp) {
+    for (int e = sub; e < g.np; e += tp) {
       const float2 v = src[(int64_t)e * g.G + i];
       a += v.x;
       c += v.y;
     }
   }, [&](int i, double a, double c) { coef[i] = coef_of(g, stats[p.ga + i].y, a, c); });
   __syncthreads();
-  if (!p.active) return;
-  float2 k1[kPairs<V>], k2[kPairs<V>];
-  thread_coef<V>(g, p, coef, k1, k2);
-  for (int t = p.tiles - 1; t >= 0; t -= U) {
-    Source<T, V, Q> v[U];
-    Vec<T, V> d[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (t - u >= 0 && p.in(t - u, g.R)) {
-        v[u].load(x, exps, p.at + (t - u) * p.step);
-        d[u].load(dy + p.at + (t - u) * p.step);
+  if (p.mine > 0) {
+    float2 k1[kPairs<V>], k2[kPairs<V>];
+    thread_coef<V>(g, p, coef, k1, k2);
+    for (int t = 0; t <= end; ++t) {
+      const int next = t + kBwdAhead - 1;
+      ring.wait();
+      if (t >= skip) {
+        Source<T, V, Q> v;
+        Vec<T, V> d;
+        ring.get(t, v, smem);
+        ring.get_dy(t, d, smem);
+        ring.start(next, next <= end);
+        dx_one<T, V, ACT, Q>(v, d, k, k1, k2, g).store(dx + p.at + (end - t) * p.step);
+      } else {
+        ring.start(next, next <= end);
       }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (t - u >= 0 && p.in(t - u, g.R))
-        dx_one<T, V, ACT, Q>(v[u], d[u], k, k1, k2, g).store(dx + p.at + (t - u) * p.step);
+    }
   }
+  ring.drain();
 }
 
 // ---------------------------------------------------------------------------
@@ -807,7 +975,6 @@ __global__ void __launch_bounds__(kThreads, 2) bwd_dx_kernel(const T* __restrict
 // A cluster of g.nb blocks keeps a sample's groups (all, or a channel tile of whole groups) in registers, NV vectors a
 // thread, between the sums and the result: every element is read once, nothing goes through memory in between, and one
 // launch does what two did. The blocks' sums are exchanged through shared memory.
-__device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
@@ -859,7 +1026,7 @@ __global__ void __launch_bounds__(kThreads, 2) fwd_small_kernel(const T* __restr
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     v[i].zero();
-    if (p.in(i, g.R)) v[i].load(x + p.at + i * p.step);
+    if (i < p.mine) v[i].load(x + p.at + i * p.step);
   }
   Affine<V> k;
   k.params(g, p, gamma, beta);
@@ -868,7 +1035,7 @@ __global__ void __launch_bounds__(kThreads, 2) fwd_small_kernel(const T* __restr
   m.pivot(v[0]);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if (p.in(i, g.R)) m.add(v[i]);
+    if (i < p.mine) m.add(v[i]);
   block_moments<T, V>(g, p, m, red, [&](int gi, double a, double c) { mine[gi - p.ga] = make_double2(a, c); });
   cluster_sums(g, groups, mine, [&](int i, double a, double c) { stat[i] = mean_rstd_of(g, a, c); });
   if (p.b == 0)
@@ -876,7 +1043,7 @@ __global__ void __launch_bounds__(kThreads, 2) fwd_small_kernel(const T* __restr
   k.stats(g, p, [&](int gi) { return stat[gi - p.ga]; });
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if (i < p.tiles) apply_one<T, V, ACT, PACK>(v[i], k, g, p.in(i, g.R), p.at + i * p.step, y, codes, exps);
+    if (i < p.tiles) apply_one<T, V, ACT, PACK>(v[i], k, g, i < p.mine, p.at + i * p.step, y, codes, exps);
   if (g.nb > 1) cluster_wait();
 }
 
@@ -900,7 +1067,7 @@ __global__ void __launch_bounds__(kThreads, NV > 4 ? 1 : 2)
   for (int i = 0; i < NV; ++i) {
     v[i].zero();
     d[i].zero();
-    if (p.in(i, g.R)) {
+    if (i < p.mine) {
       v[i].load(x, exps, p.at + i * p.step);
       d[i].load(dy + p.at + i * p.step);
     }
@@ -913,7 +1080,7 @@ __global__ void __launch_bounds__(kThreads, NV > 4 ? 1 : 2)
   for (int i = 0; i < kPairs<V>; ++i) s1[i] = s2[i] = two(0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if (p.in(i, g.R)) {
+    if (i < p.mine) {
       float2 xm[kPairs<V>], dz[kPairs<V>];
       grad_one<T, V, ACT, Q>(v[i], d[i], k, g, xm, dz);
 #pragma unroll
@@ -930,7 +1097,7 @@ __global__ void __launch_bounds__(kThreads, NV > 4 ? 1 : 2)
     thread_coef<V>(g, p, coef, k1, k2);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (p.in(i, g.R)) dx_one<T, V, ACT, Q>(v[i], d[i], k, k1, k2, g).store(dx + p.at + i * p.step);
+      if (i < p.mine) dx_one<T, V, ACT, Q>(v[i], d[i], k, k1, k2, g).store(dx + p.at + i * p.step);
   }
   if (g.nb > 1) cluster_wait();
 }
@@ -944,6 +1111,7 @@ struct FwdArgs {
   float2* mean_rstd;
   double2* part;
   uint8_t *codes, *exps;    // null: not wanted
+  int stats_nb;             // blocks a sample of the sums
 };
 struct BwdArgs {
   const void *dy, *x, *gamma, *beta;

@@ -53,8 +53,10 @@ cudaError_t fwd_v(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
     return launch_cluster(g.nb, kernel, grid, threads, kSmallGroups * (sizeof(double2) + sizeof(float2)), s, x, a.gamma,
                           a.beta, g, a.mean_rstd, static_cast<T*>(a.y), a.codes, a.exps);
   }
-  const size_t smem = sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
-  stats_kernel<T, V><<<grid, threads, 0, s>>>(x, g, a.part);
+  const size_t smem = Ring<T, V, false, false, kFwdAhead>::kBytes + sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
+  // the sums' blocks are smaller than the second pass's: more of them fit an SM
+  const Geo sums = split(g, a.stats_nb);
+  stats_kernel<T, V><<<dim3((unsigned)sums.blocks, g.tiles), threads, 0, s>>>(x, sums, a.part);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   auto apply = apply_kernel<T, V, ACT, false>;
@@ -83,7 +85,7 @@ cudaError_t bwd_v(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
                                          dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.cpart, static_cast<T*>(a.dx));
     return e != cudaSuccess || !params ? e : params_next();
   }
-  const size_t smem = sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
+  const size_t smem = Ring<T, V, Q, true, kBwdAhead>::kBytes + sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
   bwd_sums_kernel<T, V, ACT, Q><<<grid, threads, 0, s>>>(dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.cpart, a.gpart);
   note_launches(1);
   cudaError_t e = cudaGetLastError();
