@@ -22,29 +22,31 @@ bool ok_desc(const r4c_gn_desc* d) {
          d->activation >= R4C_ACT_NONE && d->activation <= R4C_ACT_GELU && d->eps >= 0.f;
 }
 
-// A cluster for each sample and channel tile of whole groups, if one can keep its share in registers. Narrower tiles
-// and larger clusters bring more SMs to few samples; tiles below 64 bytes a voxel would read sectors twice. Of the ways
-// that fit, the least modelled time: waves of (1 us + 0.08 us for each vector of a thread), and 0.7 us for an exchange
-// between blocks.
+// A cluster for each sample and channel tile of whole groups, if one can keep its share on chip and is expected to be
+// faster than two passes. Narrower tiles and larger clusters bring more SMs to few samples; tiles below 48 bytes a
+// voxel would read sectors twice. The modelled times (us) follow these measurements, forward / backward without the
+// parameters' sums: [1,192,4,8,8] bf16 silu, 1 block of 6 vectors a thread 5.9, 8 blocks of 1 vector 4.4, two passes
+// 5.9; [64,96,6,6,6] 96 groups, 6 vectors 5.5 / 6.6, two passes 9.7 / 10.5; [4,192,8,16,16] 6 vectors in clusters of 4
+// 7.5 / 10.6, two passes 7.7 / 11.9; 512 blocks in clusters of 4 for the second of these 11.4 / 14.9.
 void plan_small(const r4c_gn_desc* d, bool backward, int V, Geo& g, int* threads) {
   const int most = backward ? kSmallBwd : kSmallFwd, elem = (int)dtype_bytes(d->dtype);
-  double best = 1e30;
+  const double each = backward ? 0.5 : 0.35, mb = (double)d->samples * (double)g.sample * elem * 1e-6;
+  double best = (backward ? 9.0 : 5.6) + 0.65 * mb + (double)d->samples / 300.0;
   for (int k = g.G;; k = (k + 1) / 2) {
     const bool whole = k == g.G;
     const int64_t width = whole ? g.L : (int64_t)k * g.Cg;
-    const bool ok = whole || (g.L == g.C && width % V == 0 && width * elem >= 64);
+    const bool ok = whole || (g.L == g.C && width % V == 0 && width * elem >= 48);
     if (ok && width / V <= kThreads && k <= kSmallGroups) {
       const int lanes = (int)(width / V), tiles = whole ? 1 : cdiv(g.G, k);
       for (int cl = 1; cl <= 8; cl *= 2) {
-        const int64_t per = (g.rows + cl - 1) / cl;
+        const int64_t per = std::max<int64_t>(1, (g.rows + cl - 1) / cl);
         int R = (int)std::min<int64_t>(std::max(1, kThreads / lanes), per);
         if (R > 4) R = R / 4 * 4;
         const int64_t nv = (per + R - 1) / R;
         if (nv > most || (cl > 1 && per < 4)) continue;
         const double blocks = (double)d->samples * tiles * cl;
-        const double fit = 148.0 * (backward && nv > 4 ? 1 : 2);
-        const double sectors = whole || width * elem % 32 == 0 ? 1.0 : 1.0 + 16.0 / (double)(width * elem);
-        const double cost = std::ceil(blocks / fit) * (1.0 + 0.08 * nv * sectors) + (cl > 1 ? 0.7 : 0.0);
+        const double waves = std::ceil(blocks / (148.0 * 2));
+        const double cost = 3.5 + each * nv + (cl > 1 ? 0.2 + 0.004 * blocks : 0.0) + (waves - 1.0) * (1.5 + each * nv);
         if (cost < best - 1e-9) {
           best = cost;
           g.small = (int)nv;
@@ -84,18 +86,16 @@ bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
   g.pdtype = d->param_dtype;
   g.format = g.pack = g.wide_params = 0;
   pl->stats_nb = 1;
-  // the widest vector whose rows of lcm(C, V) elements divide a sample; several voxels in a row only while such a
-  // row fits a block's threads
+  // the widest vector that parts a voxel's channels, or whose rows of lcm(C, V) elements (several voxels) fit a block's
+  // threads
   int V = 16 / (int)dtype_bytes(d->dtype);
-  for (; V > 1; V /= 2) {
-    const int64_t L = std::lcm(C, (int64_t)V);
-    if (g.sample % L == 0 && (L == C || L <= kThreads * V)) break;
-  }
+  while (C % V != 0 && std::lcm(C, (int64_t)V) > kThreads * V) V /= 2;
   pl->V = V;
   g.L = (int)std::lcm(C, (int64_t)V);
   g.rows = g.sample / g.L;
+  g.edges = g.sample % g.L != 0;
   g.small = 0;
-  if (g.rows > 0) plan_small(d, backward, V, g, &pl->threads);
+  if (g.rows > 0 || g.edges) plan_small(d, backward, V, g, &pl->threads);
   if (g.small) {
     g.blocks = d->samples * g.nb;
     g.chunk_tiles = g.small;
@@ -122,7 +122,7 @@ bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
 // the 8 bits in its own pass over x.
 bool fused_pack(const Plan& pl, size_t elem) {
   const Geo& g = pl.g;
-  if (pl.V * elem != 16 || g.sample % r4c::q8::kBlock) return false;
+  if (pl.V * elem != 16 || g.edges || g.sample % r4c::q8::kBlock) return false;
   if (g.tiles == 1) return (int64_t)g.R * g.L % r4c::q8::kBlock == 0;
   return g.C % r4c::q8::kBlock == 0 && g.lanes * pl.V % r4c::q8::kBlock == 0;
 }

@@ -8,13 +8,14 @@
 //   A = mean over the group of dz * w,  B = mean over the group of dz * w * xh
 //   dx = rstd * (dz * w - A - xh * B)
 // Two passes over the data each way: sums, then the element-wise result (the statistics of a group need all of it).
-// Both are bound by memory: forward 3, backward 5 activations read or written. Samples that fit the registers of a
-// cluster take one.
+// Both are bound by memory: forward 3, backward 5 activations read or written. Samples that fit the shared memory
+// of a cluster take one.
 //
 // A thread owns a vector of V neighbouring elements in every R-th row of its block's range, so its channels and with
 // them the parameters stay in registers. A row is a voxel's channels, or L / C voxels together where C is no multiple
-// of V (L = lcm(C, V)), so that odd channel counts still move 16 bytes at a time. Rows wider than a block's threads
-// are cut into channel tiles.
+// of V (L = lcm(C, V)), so that odd channel counts still move 16 bytes at a time; what is left of a sample before its
+// first whole vector and behind its last whole row (its edges) goes element by element. Rows wider than a block's
+// threads are cut into channel tiles.
 //
 // Sums: a thread keeps sum (x - p) and sum (x - p)^2 in fp32 around its own first value p, so nothing cancels where
 // |mean| >> std, and an outlier as p spoils one thread's few elements at most; threads, blocks and samples add in
@@ -30,17 +31,17 @@ namespace r4c {
 namespace gn {
 
 constexpr int kThreads = 256;   // at most, per block
-// Samples that a cluster keeps in registers: vectors of a thread at most (forward; backward, which keeps dy too),
-// groups of a channel tile at most (shared memory).
 // Blocks that fit an SM beside each other (the registers that each kernel may take follow from it).
 constexpr int kStatsBlocks = 4, kApplyBlocks = 4, kBwdBlocks = 3;
 // Vectors of a thread on their way at a time, plus one.
 constexpr int kFwdAhead = 8, kBwdAhead = 4;
+// Samples that a cluster keeps on chip: vectors of a thread at most (forward; backward, which keeps dy too), groups of
+// a channel tile at most.
 constexpr int kSmallFwd = 16, kSmallBwd = 8, kSmallGroups = 256;
 
 struct Geo {
   int64_t sample;    // elements of a sample, S * C
-  int64_t rows;      // rows of L elements of a sample
+  int64_t rows;      // rows of L elements of a sample (with edges: of the longest)
   int64_t chunk;     // rows of a block, a multiple of R
   int64_t samples, blocks;   // blocks of one channel tile: samples * nb
   double inv_m;      // 1 / (Cg * S)
@@ -52,10 +53,11 @@ struct Geo {
   int R;             // rows that a block's threads cover at a time
   int chunk_tiles;   // chunk / R
   int nb;            // blocks of a sample and channel tile (the cluster's, where one keeps a sample)
+  int edges;         // samples do not part into whole rows that start on a vector
   int np;            // parts of a sample's sums that the second pass reads: blocks of the first times channel tiles
   int wide_params;   // w and b are fp32 on 16 bytes, and a thread's channels follow each other
   int pack;          // the forward writes x in 8 bits too
-  int small;         // vectors that a thread keeps in registers (small samples), or 0: two passes
+  int small;         // vectors that a thread keeps in shared memory (small samples), or 0: two passes
 };
 
 // The same data in another number of blocks a sample.
@@ -379,6 +381,7 @@ struct Place {
   int b, tile, lane, row;
   int j0, j1;           // the channel tile's elements of a row
   int c, gi, in_group;  // the thread's first channel, its group and its place there
+  int shift;            // the channel of a row's first element
   int ga, gb;           // the channel tile's groups
   bool active;
 };
@@ -400,7 +403,15 @@ __device__ __forceinline__ Place place(const Geo& g) {
   p.j1 = min(p.j0 + g.lanes * V, g.L);
   const int j = p.j0 + p.lane * V;
   p.active = p.row < g.R && j < p.j1;
-  p.c = g.L == g.C ? j : (int)((unsigned)j % (unsigned)g.C);
+  int64_t first = p.n * g.sample, rows = g.rows;
+  p.shift = 0;
+  if (g.edges) {
+    const int head = (int)(-first & (V - 1));
+    p.shift = head < g.C ? head : head % g.C;
+    first += head;
+    if (g.sample - head < rows * g.L) --rows;
+  }
+  p.c = g.L == g.C ? j : (int)((unsigned)(j + p.shift) % (unsigned)g.C);
   p.gi = (int)((unsigned)p.c / (unsigned)g.Cg);
   p.in_group = p.c - p.gi * g.Cg;
   if (g.tiles == 1) {
@@ -411,15 +422,49 @@ __device__ __forceinline__ Place place(const Geo& g) {
     p.gb = (int)((unsigned)(p.j1 - 1) / (unsigned)g.Cg) + 1;
   }
   const int64_t r0 = p.b * g.chunk;
-  const int64_t left = min(g.chunk, g.rows - r0);
+  const int64_t left = min(g.chunk, rows - r0);
   p.tiles = left == g.chunk ? g.chunk_tiles : left > 0 ? (int)((left + g.R - 1) / g.R) : 0;
   const int64_t last = left - (int64_t)(p.tiles - 1) * g.R;    // rows of the last tile
   p.mine = p.active ? p.tiles - (p.row < last ? 0 : 1) : 0;
   if (p.mine < 0) p.mine = 0;
-  p.at = p.n * g.sample + (r0 + p.row) * g.L + j;
+  p.at = first + (r0 + p.row) * g.L + j;
   p.step = (int64_t)g.R * g.L;
   return p;
 }
+
+// A sample's edges, which its first block works on: elements [first, first + head) and [tail_at, tail_at + tail).
+struct Edges {
+  int64_t first, tail_at;
+  int head, tail, tail_c;   // tail_c: the tail's first channel
+  template <int V>
+  static __device__ __forceinline__ Edges of(const Geo& g, const Place& p) {
+    Edges e;
+    e.first = p.n * g.sample;
+    e.head = (int)(-e.first & (V - 1));
+    if (e.head > g.sample) e.head = (int)g.sample;
+    int64_t rows = g.rows;
+    if (g.sample - e.head < rows * g.L) --rows;
+    const int64_t inside = e.head + (rows > 0 ? rows * g.L : 0);
+    e.tail_at = e.first + inside;
+    e.tail = (int)(g.sample - inside);
+    e.tail_c = (int)(inside % g.C);
+    return e;
+  }
+  // f(element) for those of channel c
+  template <typename F>
+  __device__ __forceinline__ void each_of(const Geo& g, int c, F f) const {
+    for (int i = c; i < head; i += g.C) f(first + i);
+    for (int i = c >= tail_c ? c - tail_c : c - tail_c + g.C; i < tail; i += g.C) f(tail_at + i);
+  }
+  // f(element, channel) for this thread's share of all
+  template <typename F>
+  __device__ __forceinline__ void each(const Geo& g, F f) const {
+    for (int i = threadIdx.x; i < head + tail; i += blockDim.x) {
+      if (i < head) f(first + i, i % g.C);
+      else f(tail_at + (i - head), (tail_c + (i - head)) % g.C);
+    }
+  }
+};
 
 // f(column k of the thread, its channel, its group) for its V columns, in order.
 template <int V, typename F>
@@ -570,7 +615,7 @@ struct Moments {
 // The block's sums of each of its groups: out(group, sum x, sum x^2).
 template <typename T, int V, typename Out>
 __device__ __forceinline__ void block_moments(const Geo& g, const Place& p, const Moments<T, V>& m,
-                                              double2* __restrict__ red, Out out) {
+                                              const T* __restrict__ x, double2* __restrict__ red, Out out) {
   // a thread whose columns all belong to one group adds them first
   const bool merged = V > 1 && g.L == g.C && (g.Cg & (V - 1)) == 0;
   if (merged) {
@@ -604,12 +649,23 @@ __device__ __forceinline__ void block_moments(const Geo& g, const Place& p, cons
         }
     } else {
       for (int base = 0; base < g.L; base += g.C)         // once, unless a row holds several voxels
-        for (int j = base + lo + sc; j < base + hi; j += tc)
+        for (int ch = lo + sc; ch < hi; ch += tc) {
+          const int j = base + (ch >= p.shift ? ch - p.shift : ch - p.shift + g.C);
           for (int r = sr; r < g.R; r += tr) {
             const double2 v = red[(j % V) * kThreads + r * g.lanes + j / V];
             a += v.x;
             c += v.y;
           }
+        }
+    }
+    if (g.edges && p.b == 0) {
+      const Edges e = Edges::of<V>(g, p);
+      for (int ch = lo + sub; ch < hi; ch += tp)
+        e.each_of(g, ch, [&](int64_t at) {
+          const double v = Elem<T>::to_f(x[at]);
+          a += v;
+          c += v * v;
+        });
     }
   }, [&](int i, double a, double c) { out(p.ga + i, a, c); });
 }
@@ -655,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, kStatsBlocks) stats_kernel(const T* 
   if (g.tiles > 1)
     for (int i = threadIdx.x; i < g.G; i += blockDim.x)
       if (i < p.ga || i >= p.gb) out[i] = make_double2(0.0, 0.0);
-  block_moments<T, V>(g, p, m, reinterpret_cast<double2*>(smem), [&](int gi, double a, double c) { out[gi] = make_double2(a, c); });
+  block_moments<T, V>(g, p, m, x, reinterpret_cast<double2*>(smem), [&](int gi, double a, double c) { out[gi] = make_double2(a, c); });
 }
 
 // y of one vector, and its 8 bits (PACK: a block of 32 elements lies in 32 / V neighbouring threads, all with or all
@@ -671,7 +727,7 @@ __device__ __forceinline__ void apply_one(const Vec<T, V>& v, const Affine<V>& k
 #pragma unroll
     for (int i = 0; i < V; ++i) e[i] = i & 1 ? f[i / 2].y : f[i / 2].x;
     bool finite;
-    const int byte = q8::exponent_byte(q8::block_amax<V>(e, 0xffffffffu, &finite), g.format);
+    const int byte = q8::exponent_byte(q8::block_amax<T>(v.w, 0xffffffffu, &finite), g.format);
     const q8::Codes<V> c = q8::encode<V>(e, byte, g.format, finite);
     if (in) {
       q8::store_codes<V>(codes + at, c);
@@ -684,6 +740,19 @@ __device__ __forceinline__ void apply_one(const Vec<T, V>& v, const Affine<V>& k
   Vec<T, V> r;
   r.from_f(f);
   if (in) r.store(y + at);
+}
+
+// y of a sample's edges.
+template <typename T, int V, int ACT, typename Stat>
+__device__ __forceinline__ void apply_edges(const Geo& g, const Place& p, const T* __restrict__ x, const void* gamma,
+                                            const void* beta, T* __restrict__ y, Stat stat) {
+  Edges::of<V>(g, p).each(g, [&](int64_t at, int c) {
+    const float2 s = stat((int)((unsigned)c / (unsigned)g.Cg));
+    float2 z[1] = {two(fmaf(Elem<T>::to_f(x[at]) - s.x, s.y * param(gamma, g.pdtype, c, 1.f),
+                            param(beta, g.pdtype, c, 0.f)))};
+    act_values<T, ACT>(z, g.act, g.slope);
+    y[at] = Elem<T>::from_f(z[0].x);
+  });
 }
 
 // From the last row to the first: what the sums read last is what the L2 cache still has.
@@ -727,6 +796,7 @@ __global__ void __launch_bounds__(kThreads, kApplyBlocks) apply_kernel(
     ring.start(next, next <= end && end - next < p.mine);
     apply_one<T, V, ACT, PACK>(v.v, k, g, in, p.at + (end - t) * p.step, y, codes, exps);
   }
+  if (g.edges && p.b == 0) apply_edges<T, V, ACT>(g, p, x, gamma, beta, y, [&](int gi) { return stat[gi - p.ga]; });
 }
 
 // ---------------------------------------------------------------------------
@@ -747,24 +817,50 @@ __device__ __forceinline__ void grad_one(const Source<T, V, Q>& v, const Vec<T, 
   act_grads<T, ACT>(dz, z, g.act, g.slope);
 }
 
+// dz and x - mean of one element of channel c.
+template <typename T, int ACT, bool Q>
+__device__ __forceinline__ float2 grad_edge(const Geo& g, const T* __restrict__ dy, const void* __restrict__ x,
+                                            const uint8_t* __restrict__ exps, const void* gamma, const void* beta,
+                                            int64_t at, int c, float2 stat) {
+  Source<T, 1, Q> v;
+  float2 xm[1], dz[1] = {make_float2(Elem<T>::to_f(dy[at]), 0.f)};
+  v.load(x, exps, at);
+  v.to_f(g.format, xm);
+  xm[0].x -= stat.x;
+  const float2 z[1] = {make_float2(
+      fmaf(xm[0].x, stat.y * param(gamma, g.pdtype, c, 1.f), param(beta, g.pdtype, c, 0.f)), 0.f)};
+  act_grads<T, ACT>(dz, z, g.act, g.slope);
+  return make_float2(dz[0].x, xm[0].x);
+}
+
 // The block's (sum dz, sum dz * (x - mean)) of a thread's columns: cpart gets them per channel (the second times rstd),
-// out(group, ..) the same times w, summed over the tile's channels of the group.
-template <int V, typename Stat, typename Out>
+// out(group, ..) the same times w, summed over the tile's channels of the group. edge(element, channel, stat): an
+// edge's dz and x - mean.
+template <int V, typename Stat, typename Edge, typename Out>
 __device__ __forceinline__ void block_grads(const Geo& g, const Place& p, const float2 (&s1)[kPairs<V>],
                                             const float2 (&s2)[kPairs<V>], const void* gamma, float2* __restrict__ red,
-                                            float2* __restrict__ cols, float2* __restrict__ cpart, Stat stat, Out out) {
+                                            float2* __restrict__ cols, float2* __restrict__ cpart, Stat stat, Edge edge,
+                                            Out out) {
 #pragma unroll
   for (int k = 0; k < V; ++k)
     red[k * kThreads + threadIdx.x] = k & 1 ? make_float2(s1[k / 2].y, s2[k / 2].y) : make_float2(s1[k / 2].x, s2[k / 2].x);
   __syncthreads();
   const int nch = g.tiles == 1 ? g.C : p.j1 - p.j0;
   each_sum<float>(nch, [&](int i, int sub, int tp, float& a, float& c) {
-    for (int j = i; j < (g.tiles == 1 ? g.L : nch); j += g.C)
+    for (int j = i >= p.shift ? i - p.shift : i - p.shift + g.C; j < (g.tiles == 1 ? g.L : nch); j += g.C)
       for (int r = sub; r < g.R; r += tp) {
         const float2 v = red[(j % V) * kThreads + r * g.lanes + j / V];
         a += v.x;
         c += v.y;
       }
+    if (g.edges && p.b == 0 && sub == 0) {
+      const float2 s = stat((int)((unsigned)i / (unsigned)g.Cg));
+      Edges::of<V>(g, p).each_of(g, i, [&](int64_t at) {
+        const float2 e = edge(at, i, s);
+        a += e.x;
+        c = fmaf(e.x, e.y, c);
+      });
+    }
   }, [&](int i, float a, float c) {
     const int ch = p.j0 + i;
     const float2 s = make_float2(a, c * stat((int)((unsigned)ch / (unsigned)g.Cg)).y);
@@ -826,7 +922,9 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_sums_kernel(
     for (int i = threadIdx.x; i < g.G; i += blockDim.x)
       if (i < p.ga || i >= p.gb) out[i] = make_float2(0.f, 0.f);
   block_grads<V>(g, p, a1, a2, gamma, reinterpret_cast<float2*>(smem), reinterpret_cast<float2*>(smem + kTable), cpart,
-                 [&](int gi) { return stats[gi]; }, [&](int gi, float a, float c) { out[gi] = make_float2(a, c); });
+                 [&](int gi) { return stats[gi]; },
+                 [&](int64_t at, int c, float2 s) { return grad_edge<T, ACT, Q>(g, dy, x, exps, gamma, beta, at, c, s); },
+                 [&](int gi, float a, float c) { out[gi] = make_float2(a, c); });
 }
 
 // ---------------------------------------------------------------------------
@@ -910,6 +1008,20 @@ __device__ __forceinline__ float2 coef_of(const Geo& g, double rstd, double a, d
   return make_float2((float)(rstd * a * g.inv_m), (float)(rstd * rstd * c * g.inv_m));
 }
 
+// dx of a sample's edges.
+template <typename T, int V, int ACT, bool Q>
+__device__ __forceinline__ void dx_edges(const Geo& g, const Place& p, const T* __restrict__ dy,
+                                         const void* __restrict__ x, const uint8_t* __restrict__ exps, const void* gamma,
+                                         const void* beta, const float2* __restrict__ stats, const float2* coef,
+                                         T* __restrict__ dx) {
+  Edges::of<V>(g, p).each(g, [&](int64_t at, int c) {
+    const int gi = (int)((unsigned)c / (unsigned)g.Cg);
+    const float2 s = stats[gi], q = coef[gi - p.ga];
+    const float2 e = grad_edge<T, ACT, Q>(g, dy, x, exps, gamma, beta, at, c, s);
+    dx[at] = Elem<T>::from_f(fmaf(e.x, s.y * param(gamma, g.pdtype, c, 1.f), -fmaf(e.y, q.y, q.x)));
+  });
+}
+
 // Blocks from g.blocks on sum the parameters' gradients, beside the others.
 template <typename T, int V, int ACT, bool Q>
 __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
@@ -966,15 +1078,18 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
       }
     }
   }
+  if (g.edges && p.b == 0) dx_edges<T, V, ACT, Q>(g, p, dy, x, exps, gamma, beta, stats, coef, dx);
   ring.drain();
 }
 
 // ---------------------------------------------------------------------------
-// Small samples: one launch, data in registers
+// Small samples: one launch, data in shared memory
 // ---------------------------------------------------------------------------
-// A cluster of g.nb blocks keeps a sample's groups (all, or a channel tile of whole groups) in registers, NV vectors a
-// thread, between the sums and the result: every element is read once, nothing goes through memory in between, and one
-// launch does what two did. The blocks' sums are exchanged through shared memory.
+// A cluster of g.nb blocks keeps a sample's groups (all, or a channel tile of whole groups) in its shared memory, up to
+// g.small vectors a thread, between the sums and the result: every element is read once, nothing goes through memory
+// in between, and one launch does what two did. The blocks' sums are exchanged through shared memory. The loops stay
+// rolled: code that runs once is paced by its own fetches (vectors in registers, unrolled: 8.5 us for [4,192,8,16,16]
+// where two passes took 7.7).
 __device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
@@ -1010,95 +1125,130 @@ __device__ __forceinline__ void cluster_sums(const Geo& g, int groups, const dou
   if (g.nb > 1) cluster_arrive();
 }
 
-template <typename T, int V, int ACT, bool PACK, int NV>
-__global__ void __launch_bounds__(kThreads, 2) fwd_small_kernel(const T* __restrict__ x, const void* __restrict__ gamma,
-                                                                const void* __restrict__ beta,
-                                                                const __grid_constant__ Geo g,
-                                                                float2* __restrict__ mean_rstd, T* __restrict__ y,
-                                                                uint8_t* __restrict__ codes,
-                                                                uint8_t* __restrict__ exps) {
-  __shared__ double2 red[V * kThreads];
-  extern __shared__ double2 mine[];
+// Bytes of a small kernel's shared memory: its vectors, then the blocks' tables, then each group's two results.
+template <typename T, int V>
+constexpr int small_fwd_bytes(int vectors) {
+  return vectors * kThreads * V * (int)sizeof(T) + V * kThreads * (int)sizeof(double2) +
+         kSmallGroups * (int)(sizeof(double2) + sizeof(float2));
+}
+template <typename T, int V, bool Q>
+constexpr int small_bwd_bytes(int vectors) {
+  return vectors * kThreads * V * ((Q ? 1 : (int)sizeof(T)) + (int)sizeof(T)) + 2 * V * kThreads * (int)sizeof(float2) +
+         kSmallGroups * (int)(sizeof(double2) + sizeof(float2));
+}
+
+template <typename T, int V, int ACT, bool PACK>
+__global__ void __launch_bounds__(kThreads) fwd_small_kernel(const T* __restrict__ x, const void* __restrict__ gamma,
+                                                             const void* __restrict__ beta,
+                                                             const __grid_constant__ Geo g,
+                                                             float2* __restrict__ mean_rstd, T* __restrict__ y,
+                                                             uint8_t* __restrict__ codes,
+                                                             uint8_t* __restrict__ exps) {
+  constexpr int B = V * (int)sizeof(T);
+  extern __shared__ __align__(16) char smem[];
+  double2* red = reinterpret_cast<double2*>(smem + g.small * kThreads * B);
+  double2* mine = red + V * kThreads;
+  float2* stat = reinterpret_cast<float2*>(mine + kSmallGroups);
   const Place p = place<V>(g);
   const int groups = p.gb - p.ga;
-  float2* stat = reinterpret_cast<float2*>(mine + groups);
-  Vec<T, V> v[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    v[i].zero();
-    if (i < p.mine) v[i].load(x + p.at + i * p.step);
-  }
+  const char* own = smem + threadIdx.x * B;
+  for (int t = 0; t < p.mine; ++t) copy_async<B>(shared_at(own) + t * kThreads * B, x + p.at + t * p.step);
   Affine<V> k;
   k.params(g, p, gamma, beta);
+  asm volatile("cp.async.wait_all;" ::: "memory");
   Moments<T, V> m;
   m.zero();
-  m.pivot(v[0]);
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i < p.mine) m.add(v[i]);
-  block_moments<T, V>(g, p, m, red, [&](int gi, double a, double c) { mine[gi - p.ga] = make_double2(a, c); });
+#pragma unroll 2
+  for (int t = 0; t < p.mine; ++t) {
+    Vec<T, V> v;
+    v.load(reinterpret_cast<const T*>(own + t * kThreads * B));
+    if (t == 0) m.pivot(v);
+    m.add(v);
+  }
+  block_moments<T, V>(g, p, m, x, red, [&](int gi, double a, double c) { mine[gi - p.ga] = make_double2(a, c); });
   cluster_sums(g, groups, mine, [&](int i, double a, double c) { stat[i] = mean_rstd_of(g, a, c); });
   if (p.b == 0)
     for (int i = threadIdx.x; i < groups; i += blockDim.x) mean_rstd[p.n * g.G + p.ga + i] = stat[i];
   k.stats(g, p, [&](int gi) { return stat[gi - p.ga]; });
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i < p.tiles) apply_one<T, V, ACT, PACK>(v[i], k, g, i < p.mine, p.at + i * p.step, y, codes, exps);
+#pragma unroll 2
+  for (int t = 0; t < p.tiles; ++t) {
+    Vec<T, V> v;
+    v.zero();
+    if (t < p.mine) v.load(reinterpret_cast<const T*>(own + t * kThreads * B));
+    apply_one<T, V, ACT, PACK>(v, k, g, t < p.mine, p.at + t * p.step, y, codes, exps);
+  }
+  if (g.edges && p.b == 0) apply_edges<T, V, ACT>(g, p, x, gamma, beta, y, [&](int gi) { return stat[gi - p.ga]; });
   if (g.nb > 1) cluster_wait();
 }
 
-template <typename T, int V, int ACT, bool Q, int NV>
-__global__ void __launch_bounds__(kThreads, NV > 4 ? 1 : 2)
+template <typename T, int V, int ACT, bool Q>
+__global__ void __launch_bounds__(kThreads)
     bwd_small_kernel(const T* __restrict__ dy, const void* __restrict__ x, const uint8_t* __restrict__ exps,
                      const float2* __restrict__ mean_rstd, const void* __restrict__ gamma,
                      const void* __restrict__ beta, const __grid_constant__ Geo g, float2* __restrict__ cpart,
                      T* __restrict__ dx) {
-  __shared__ float2 red[V * kThreads];
-  __shared__ float2 cols[V * kThreads];
-  extern __shared__ double2 mine[];
+  constexpr int XB = V * (Q ? 1 : (int)sizeof(T)), YB = V * (int)sizeof(T);
+  extern __shared__ __align__(16) char smem[];
+  char* dys = smem + g.small * kThreads * XB;
+  float2* red = reinterpret_cast<float2*>(dys + g.small * kThreads * YB);
+  float2* cols = red + V * kThreads;
+  double2* mine = reinterpret_cast<double2*>(cols + V * kThreads);
+  float2* coef = reinterpret_cast<float2*>(mine + kSmallGroups);
   let_next_start();
   const Place p = place<V>(g);
   const int groups = p.gb - p.ga;
-  float2* coef = reinterpret_cast<float2*>(mine + groups);
-  const float2* stats = mean_rstd + p.n * g.G;
-  Source<T, V, Q> v[NV];
-  Vec<T, V> d[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    v[i].zero();
-    d[i].zero();
-    if (i < p.mine) {
-      v[i].load(x, exps, p.at + i * p.step);
-      d[i].load(dy + p.at + i * p.step);
-    }
+  const char *own = smem + threadIdx.x * XB, *own_dy = dys + threadIdx.x * YB;
+  for (int t = 0; t < p.mine; ++t) {
+    copy_async<XB>(shared_at(own) + t * kThreads * XB,
+                   static_cast<const char*>(x) + (p.at + t * p.step) * (Q ? 1 : (int)sizeof(T)));
+    copy_async<YB>(shared_at(own_dy) + t * kThreads * YB, dy + p.at + t * p.step);
   }
+  const float2* stats = mean_rstd + p.n * g.G;
   Affine<V> k;
   k.params(g, p, gamma, beta);
   k.stats(g, p, [&](int gi) { return stats[gi]; });
+  auto get = [&](int t, Source<T, V, Q>& v, Vec<T, V>& d) {
+    if constexpr (Q) {
+      v.c = q8::load_codes<V>(reinterpret_cast<const uint8_t*>(own + t * kThreads * XB));
+      v.byte = exps[(p.at + t * p.step) / q8::kBlock];
+    } else {
+      v.v.load(reinterpret_cast<const T*>(own + t * kThreads * XB));
+    }
+    d.load(reinterpret_cast<const T*>(own_dy + t * kThreads * YB));
+  };
   float2 s1[kPairs<V>], s2[kPairs<V>];
 #pragma unroll
   for (int i = 0; i < kPairs<V>; ++i) s1[i] = s2[i] = two(0.f);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 2
+  for (int t = 0; t < p.mine; ++t) {
+    Source<T, V, Q> v;
+    Vec<T, V> d;
+    get(t, v, d);
+    float2 xm[kPairs<V>], dz[kPairs<V>];
+    grad_one<T, V, ACT, Q>(v, d, k, g, xm, dz);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i < p.mine) {
-      float2 xm[kPairs<V>], dz[kPairs<V>];
-      grad_one<T, V, ACT, Q>(v[i], d[i], k, g, xm, dz);
-#pragma unroll
-      for (int j = 0; j < kPairs<V>; ++j) {
-        s1[j] = __fadd2_rn(s1[j], dz[j]);
-        s2[j] = __ffma2_rn(dz[j], xm[j], s2[j]);
-      }
+    for (int j = 0; j < kPairs<V>; ++j) {
+      s1[j] = __fadd2_rn(s1[j], dz[j]);
+      s2[j] = __ffma2_rn(dz[j], xm[j], s2[j]);
     }
+  }
   block_grads<V>(g, p, s1, s2, gamma, red, cols, cpart, [&](int gi) { return stats[gi]; },
+                 [&](int64_t at, int c, float2 s) { return grad_edge<T, ACT, Q>(g, dy, x, exps, gamma, beta, at, c, s); },
                  [&](int gi, float a, float c) { mine[gi - p.ga] = make_double2(a, c); });
   cluster_sums(g, groups, mine, [&](int i, double a, double c) { coef[i] = coef_of(g, stats[p.ga + i].y, a, c); });
-  if (p.active) {
+  if (p.mine > 0) {
     float2 k1[kPairs<V>], k2[kPairs<V>];
     thread_coef<V>(g, p, coef, k1, k2);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i < p.mine) dx_one<T, V, ACT, Q>(v[i], d[i], k, k1, k2, g).store(dx + p.at + i * p.step);
+#pragma unroll 2
+    for (int t = 0; t < p.mine; ++t) {
+      Source<T, V, Q> v;
+      Vec<T, V> d;
+      get(t, v, d);
+      dx_one<T, V, ACT, Q>(v, d, k, k1, k2, g).store(dx + p.at + t * p.step);
+    }
   }
+  if (g.edges && p.b == 0) dx_edges<T, V, ACT, Q>(g, p, dy, x, exps, gamma, beta, stats, coef, dx);
   if (g.nb > 1) cluster_wait();
 }
 

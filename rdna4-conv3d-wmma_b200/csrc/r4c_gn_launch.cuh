@@ -1,6 +1,8 @@
 // r4c_gn_launch.cuh — the launches of r4c_gn.cuh for one element type.
 #pragma once
 
+#include <atomic>
+
 #include "r4c_gn.cuh"
 
 namespace r4c {
@@ -36,9 +38,41 @@ cudaError_t launch_cluster(int blocks, void (*kernel)(P...), dim3 grid, int thre
   return launch_with(at, kernel, grid, threads, smem, s, args...);
 }
 
+// Allows a kernel its shared memory above 48 KB, once a device.
+template <typename K>
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<uint64_t>& devices) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (devices.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) devices.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <typename T, int V, int ACT, bool PACK>
-auto fwd_small_of(const Geo& g) {
-  return g.small <= 4 ? fwd_small_kernel<T, V, ACT, PACK, 4> : fwd_small_kernel<T, V, ACT, PACK, kSmallFwd>;
+cudaError_t fwd_small(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
+  static std::atomic<uint64_t> allowed{0};
+  auto kernel = fwd_small_kernel<T, V, ACT, PACK>;
+  const cudaError_t e = allow_shared(kernel, small_fwd_bytes<T, V>(kSmallFwd), allowed);
+  if (e != cudaSuccess) return e;
+  note_launches(1);
+  return launch_cluster(g.nb, kernel, dim3((unsigned)g.blocks, g.tiles), threads, small_fwd_bytes<T, V>(g.small), s,
+                        static_cast<const T*>(a.x), a.gamma, a.beta, g, a.mean_rstd, static_cast<T*>(a.y), a.codes,
+                        a.exps);
+}
+template <typename T, int V, int ACT, bool Q>
+cudaError_t bwd_small(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
+  static std::atomic<uint64_t> allowed{0};
+  auto kernel = bwd_small_kernel<T, V, ACT, Q>;
+  const cudaError_t e = allow_shared(kernel, small_bwd_bytes<T, V, Q>(kSmallBwd), allowed);
+  if (e != cudaSuccess) return e;
+  note_launches(1);
+  return launch_cluster(g.nb, kernel, dim3((unsigned)g.blocks, g.tiles), threads, small_bwd_bytes<T, V, Q>(g.small), s,
+                        static_cast<const T*>(a.dy), a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.cpart,
+                        static_cast<T*>(a.dx));
 }
 
 template <typename T, int V, int ACT>
@@ -46,12 +80,9 @@ cudaError_t fwd_v(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   const dim3 grid((unsigned)g.blocks, g.tiles);
   const T* x = static_cast<const T*>(a.x);
   if (g.small) {
-    auto kernel = fwd_small_of<T, V, ACT, false>(g);
     if constexpr (V * sizeof(T) == 16)
-      if (g.pack) kernel = fwd_small_of<T, V, ACT, true>(g);
-    note_launches(1);
-    return launch_cluster(g.nb, kernel, grid, threads, kSmallGroups * (sizeof(double2) + sizeof(float2)), s, x, a.gamma,
-                          a.beta, g, a.mean_rstd, static_cast<T*>(a.y), a.codes, a.exps);
+      if (g.pack) return fwd_small<T, V, ACT, true>(a, g, threads, s);
+    return fwd_small<T, V, ACT, false>(a, g, threads, s);
   }
   const size_t smem = Ring<T, V, false, false, kFwdAhead>::kBytes + sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
   // the sums' blocks are smaller than the second pass's: more of them fit an SM
@@ -79,10 +110,7 @@ cudaError_t bwd_v(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
                        a.cpart, g.blocks, g.C, a.dgamma, a.dbeta);
   };
   if (g.small && a.dx) {
-    auto kernel = g.small <= 4 ? bwd_small_kernel<T, V, ACT, Q, 4> : bwd_small_kernel<T, V, ACT, Q, kSmallBwd>;
-    note_launches(1);
-    const cudaError_t e = launch_cluster(g.nb, kernel, grid, threads, kSmallGroups * (sizeof(double2) + sizeof(float2)), s,
-                                         dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.cpart, static_cast<T*>(a.dx));
+    const cudaError_t e = bwd_small<T, V, ACT, Q>(a, g, threads, s);
     return e != cudaSuccess || !params ? e : params_next();
   }
   const size_t smem = Ring<T, V, Q, true, kBwdAhead>::kBytes + sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);

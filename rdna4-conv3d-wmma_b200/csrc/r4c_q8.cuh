@@ -125,7 +125,7 @@ __device__ __forceinline__ void decode(const Codes<V>& c, int byte, int format, 
     for (int i = 0; i < (V > 4 ? 2 : 1); ++i) {
       const uint32_t u = c.w[i] ^ 0x80808080u;
       uint32_t zero = (u - 0x01010101u) & ~u & 0x80808080u;   // a byte of u is 0: some code is -128
-      if (V < 4) zero &= (1u << (8 * V)) - 1;
+      if (V < 4) zero &= 0xffffffffu >> (32 - 8 * (V < 4 ? V : 4));
       nan |= zero;
 #pragma unroll
       for (int k = 4 * i; k < V && k < 4 * i + 4; ++k)
@@ -170,26 +170,48 @@ __device__ __forceinline__ void decode(const Codes<V>& c, int byte, int format, 
   }
 }
 
-// Largest finite magnitude (fp32 bits) of a block that 32 / V neighbouring lanes hold, V elements each; every lane of
-// `mask` takes part. `finite`: this lane's elements all are.
-template <int V>
-__device__ __forceinline__ uint32_t block_amax(const float (&f)[V], uint32_t mask, bool* finite) {
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Largest finite magnitude (fp32 bits) of a block that lies in neighbouring lanes, each with NW words of T; every lane of
+// `mask` takes part. `finite`: this lane's elements all are. Magnitudes of one type order as their bits do, so 16-bit
+// types are compared two at a time as they lie.
+template <typename T, int NW>
+__device__ __forceinline__ uint32_t block_amax(const uint32_t (&w)[NW], uint32_t mask, bool* finite) {
+  constexpr bool kWide = sizeof(T) == 4;
+  constexpr uint32_t kSign = kWide ? 0x7fffffffu : 0x7fff7fffu;
+  // infinity's bits: everything from there on is not finite
+  constexpr uint32_t kInf = kWide ? 0x7f800000u : (__is_same(T, __half) ? 0x7c00u : 0x7f80u);
+  auto larger = [](uint32_t a, uint32_t b) { return kWide ? max(a, b) : max_u16x2(a, b); };
+  auto halves = [&](uint32_t m) { return kWide ? m : max(m & 0xffffu, m >> 16); };
   uint32_t m = 0;
 #pragma unroll
-  for (int k = 0; k < V; ++k) m = max(m, __float_as_uint(f[k]) & 0x7fffffffu);
-  const bool bad = m >= 0x7f800000u;
+  for (int k = 0; k < NW; ++k) m = larger(m, w[k] & kSign);
+  m = halves(m);
+  const bool bad = m >= kInf;
   *finite = !bad;
   if (__any_sync(mask, bad)) {                  // NaN or infinities somewhere: the finite ones alone
     m = 0;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const uint32_t b = __float_as_uint(f[k]) & 0x7fffffffu;
-      m = max(m, b < 0x7f800000u ? b : 0u);
+    for (int k = 0; k < NW; ++k) {
+      const uint32_t v = w[k] & kSign;
+      if constexpr (kWide) {
+        m = max(m, v < kInf ? v : 0u);
+      } else {
+        m = max(m, (v & 0xffffu) < kInf ? v & 0xffffu : 0u);
+        m = max(m, (v >> 16) < kInf ? v >> 16 : 0u);
+      }
     }
   }
+  constexpr int kLanes = kBlock * (int)sizeof(T) / 4 / NW;
 #pragma unroll
-  for (int o = 1; o < kBlock / V; o <<= 1) m = max(m, __shfl_xor_sync(mask, m, o));
-  return m;
+  for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(mask, m, o));
+  if constexpr (kWide) return m;
+  else if constexpr (__is_same(T, __half)) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+  else return m << 16;
 }
 
 }  // namespace q8

@@ -80,7 +80,11 @@ def check(got, want, names=None):
     for k, (v, bound) in want.items():
         if names is not None and k not in names:
             continue
-        d = (got[k].detach().double() - v).abs()
+        t = got[k].detach().double()
+        d = (t - v).abs()
+        # beyond its type's range a value rounds to infinity (a group of one element has rstd = eps^-1/2 = 316, and with
+        # x in 8 bits xh = 316 (x8 - x): dx = -rstd g xh^2 passes 65504)
+        d = torch.where(t.isinf() & (t.sign() == v.sign()) & (v.abs() + bound >= torch.finfo(got[k].dtype).max), 0.0, d)
         worst = (d - bound).max().item() if d.numel() else 0.0
         assert d.numel() == 0 or bool((d <= bound).all()), f"{k}: {worst:.3e} beyond its bound"
 

@@ -497,3 +497,19 @@ def test_compiled_between_graphs(cuda_ready):
     torch.autograd.grad(y, (x, w, b), dy)
 
 
+
+
+# samples that begin and end inside a vector or a row of several voxels: nothing but edges, one whole row, many
+EDGES = [((3, 1, 1, 1, 3), 1), ((3, 3, 1, 1, 1), 3), ((7, 5, 1, 1, 7), 5), ((5, 12, 1, 3, 3), 4), ((3, 20, 3, 3, 3), 5),
+         ((3, 30, 7, 11, 13), 6), ((2, 30, 37, 41, 53), 6), ((3, 199, 3, 5, 7), 199), ((2, 255, 3, 3, 3), 17),
+         ((3, 257, 3, 3, 3), 257), ((2, 300, 5, 5, 5), 3), ((3, 1028, 3, 3, 1), 4), ((9, 36, 1, 1, 5), 1), ((5, 13, 21, 23, 25), 1)]
+
+
+@pytest.mark.parametrize("fmt", [None, "int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("shape,groups", EDGES, ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else f"g{v}")
+def test_edges_of_samples(cuda_ready, shape, groups, dtype, fmt):
+    _verify(*_args(shape, groups, dtype), act="gelu" if dtype is FP else "silu", fmt=fmt)
+    x, _, w, b, dy = _args(shape, groups, dtype, seed=5)
+    y = group_norm_act(x.detach(), groups, w.detach(), b.detach(), activation="relu")
+    R.check(dict(y=y), R.ref(x, groups, w, b, 1e-5, "relu", SLOPE))
