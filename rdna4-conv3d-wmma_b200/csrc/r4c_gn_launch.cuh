@@ -80,7 +80,7 @@ cudaError_t fwd_v(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   const dim3 grid((unsigned)g.blocks, g.tiles);
   const T* x = static_cast<const T*>(a.x);
   if (g.small) {
-    if constexpr (V * sizeof(T) == 16)
+    if constexpr (V * sizeof(T) == 16 && ACT >= 0)
       if (g.pack) return fwd_small<T, V, ACT, true>(a, g, threads, s);
     return fwd_small<T, V, ACT, false>(a, g, threads, s);
   }
@@ -91,7 +91,7 @@ cudaError_t fwd_v(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   auto apply = apply_kernel<T, V, ACT, false>;
-  if constexpr (V * sizeof(T) == 16)
+  if constexpr (V * sizeof(T) == 16 && ACT >= 0)             // (samples with edges are packed on their own)
     if (g.pack) apply = apply_kernel<T, V, ACT, true>;
   e = launch_next(apply, grid, threads, smem, s, x, a.gamma, a.beta, g, a.part, a.mean_rstd, static_cast<T*>(a.y),
                   a.codes, a.exps);
@@ -127,11 +127,11 @@ cudaError_t bwd_v(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   return params_next();
 }
 
-// The widest vectors have a kernel for each activation; narrower ones (channels that are no multiple of a vector in
-// volumes of odd sizes) one for all.
+// The widest vectors have a kernel for each activation; narrower ones and samples with edges one for all.
 template <typename T, int V>
 cudaError_t fwd_act(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   if constexpr (V * sizeof(T) == 16) {
+    if (g.edges) return fwd_v<T, V, -1>(a, g, threads, s);
     switch (g.act) {
       case R4C_ACT_NONE: return fwd_v<T, V, R4C_ACT_NONE>(a, g, threads, s);
       case R4C_ACT_RELU: return fwd_v<T, V, R4C_ACT_RELU>(a, g, threads, s);
@@ -146,6 +146,7 @@ cudaError_t fwd_act(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s)
 template <typename T, int V, bool Q>
 cudaError_t bwd_act(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   if constexpr (V * sizeof(T) == 16) {
+    if (g.edges) return bwd_v<T, V, -1, Q>(a, g, threads, s);
     switch (g.act) {
       case R4C_ACT_NONE: return bwd_v<T, V, R4C_ACT_NONE, Q>(a, g, threads, s);
       case R4C_ACT_RELU: return bwd_v<T, V, R4C_ACT_RELU, Q>(a, g, threads, s);
