@@ -464,7 +464,9 @@ int r4c_unpack8(const void* codes, const void* exponents, int64_t count, int dty
  * and read by the backward.
  * With codes and exponents given (both or neither) the forward also writes x
  * as r4c_pack8 does. The backward takes those (x = codes, `exponents`,
- * `format`) or, with exponents null, x itself:
+ * `format`; it reads exponents in words, (elements + 127) / 128 of 4 bytes, of
+ * which the last may hold anything behind the exponents) or, with exponents
+ * null, x itself:
  *   xh = (x - mean) * rstd,  dz = dy * act'(z)
  *   dgamma = sum dz * xh,  dbeta = sum dz              (fp32; each may be null)
  *   dx = rstd * (dz * gamma - mean_g(dz * gamma) - xh * mean_g(dz * gamma * xh))   (may be null)

@@ -190,60 +190,63 @@ __device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
   }
 }
 
-// A thread's next vectors of x (and dy), D of them on their way in its own slots of shared memory: what the memory's
-// latency needs in flight (some 100 KB an SM) costs no registers, and no thread waits for another.
+// A thread's next vectors of x (and dy), D - 1 of them on their way in its own slots of shared memory: what the memory's
+// latency needs in flight (some 100 KB an SM) costs no registers, and no thread waits for another. Slots are constants
+// in loops unrolled by D, addresses are counted up: these kernels issue instructions two cycles out of three.
 template <typename T, int V, bool Q, bool DY, int D>
 struct Ring {
-  static constexpr int XB = V * (Q ? 1 : (int)sizeof(T)), YB = V * (int)sizeof(T);
+  static constexpr int XS = Q ? 1 : (int)sizeof(T), XB = V * XS, YB = V * (int)sizeof(T);
   static constexpr int kDy = D * kThreads * XB, kExp = kDy + (DY ? D * kThreads * YB : 0);
   static constexpr int kBytes = kExp + (Q ? D * kThreads * 4 : 0);
-  const char *x, *dy;             // this thread's first vector
+  const char *x, *dy;             // the next vector to start
   const uint8_t* exps;
-  int64_t at, count;              // its index, and the elements of x (for the exponents' end)
-  int64_t step;
-  uint32_t slot;
+  int64_t at, step;               // its element, and the elements from one to the next
+  uint32_t got;                   // the element of the next vector to take, its low bits
+  uint32_t slot;                  // this thread's first slots
+  const char* mem;
 
-  __device__ __forceinline__ Ring(void* smem, const void* x_, const T* dy_, const uint8_t* exps_, int64_t at_,
-                                  int64_t step_, int64_t count_) {
+  __device__ __forceinline__ Ring(char* smem, const void* x_, const T* dy_, const uint8_t* exps_, int64_t at_,
+                                  int64_t step_) {
     at = at_;
     step = step_;
-    x = static_cast<const char*>(x_) + at * (Q ? 1 : (int)sizeof(T));
+    x = static_cast<const char*>(x_) + at * XS;
     dy = DY ? reinterpret_cast<const char*>(dy_ + at) : nullptr;
     exps = exps_;
-    count = count_;
+    got = (uint32_t)at;
     slot = shared_at(smem);
+    mem = smem;
   }
-  // starts vector t, if the thread has it
-  __device__ __forceinline__ void start(int t, bool has) {
+  // starts the next vector into slot i, if the thread has it
+  __device__ __forceinline__ void start(int i, bool has) {
     if (has) {
-      const int i = t & (D - 1);
-      copy_async<XB>(slot + (i * kThreads + threadIdx.x) * XB, x + t * step * (Q ? 1 : (int)sizeof(T)));
-      if constexpr (DY) copy_async<YB>(slot + kDy + (i * kThreads + threadIdx.x) * YB, dy + t * step * (int)sizeof(T));
-      if constexpr (Q) {
-        // the word that holds the block's exponent, as far as the array goes
-        const int64_t e = (at + t * step) / q8::kBlock & ~(int64_t)3;
-        const int64_t left = (count + q8::kBlock - 1) / q8::kBlock - e;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(slot + kExp + (i * kThreads + threadIdx.x) * 4),
-                     "l"(exps + e), "r"(left < 4 ? (int)left : 4) : "memory");
-      }
+      copy_async<XB>(slot + (i * kThreads + threadIdx.x) * XB, x);
+      if constexpr (DY) copy_async<YB>(slot + kDy + (i * kThreads + threadIdx.x) * YB, dy);
+      if constexpr (Q)            // the word that holds the block's exponent
+        copy_async<4>(slot + kExp + (i * kThreads + threadIdx.x) * 4, exps + (at / q8::kBlock & ~(int64_t)3));
     }
+    x += step * XS;
+    if constexpr (DY) dy += step * (int)sizeof(T);
+    if constexpr (Q) at += step;
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // the oldest has landed (D - 1 were started after it was the newest)
+  // the oldest has landed (D - 2 were started after it)
   __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory"); }
   __device__ __forceinline__ void drain() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
-  __device__ __forceinline__ void get(int t, Source<T, V, Q>& v, char* smem) const {
-    const int i = (t & (D - 1)) * kThreads + threadIdx.x;
+  __device__ __forceinline__ void get(int i, Source<T, V, Q>& v) const {
+    const char* p = mem + (i * kThreads + threadIdx.x) * XB;
     if constexpr (Q) {
-      v.c = q8::load_codes<V>(reinterpret_cast<const uint8_t*>(smem) + i * XB);
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + kExp + i * 4);
-      v.byte = (w >> (8 * (int)((at + t * step) / q8::kBlock & 3))) & 0xff;
+      v.c = q8::load_codes<V>(reinterpret_cast<const uint8_t*>(p));
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(mem + kExp + (i * kThreads + threadIdx.x) * 4);
+      v.byte = (int)__byte_perm(w, 0, 0x4440 | (got / q8::kBlock & 3));
     } else {
-      v.v.load(reinterpret_cast<const T*>(smem + i * XB));
+      v.v.load(reinterpret_cast<const T*>(p));
     }
   }
-  __device__ __forceinline__ void get_dy(int t, Vec<T, V>& d, char* smem) const {
-    d.load(reinterpret_cast<const T*>(smem + kDy + ((t & (D - 1)) * kThreads + threadIdx.x) * YB));
+  __device__ __forceinline__ void get_dy(int i, Vec<T, V>& d) const {
+    d.load(reinterpret_cast<const T*>(mem + kDy + (i * kThreads + threadIdx.x) * YB));
+  }
+  __device__ __forceinline__ void next() {
+    if constexpr (Q) got += (uint32_t)step;
   }
 };
 
@@ -267,7 +270,8 @@ __device__ __forceinline__ float rcp(float x) {
 }
 
 // 1 / (1 + e^-z): for 16-bit results the hardware's exponential and reciprocal (relative error about 2^-21, the
-// result's own half step is 2^-9 or 2^-12), the library's in full precision for fp32.
+// result's own half step is 2^-9 or 2^-12), the library's in full precision for fp32. (One reciprocal for two elements
+// would let a neighbour's NaN, perhaps another group's, change the last bit.)
 template <typename T>
 __device__ __forceinline__ float2 sigmoid(float2 z) {
   if constexpr (sizeof(T) == 4) {
@@ -527,8 +531,10 @@ __device__ __forceinline__ int row_threads(int tp, int rows) {
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// The thread's mean (negated), rstd * w and b; w and b do not wait for the statistics.
-template <int V>
+// The thread's parameters: z = (x - mean) * a + b with a = rstd * w. For 16-bit x the mean goes into b (z = x * a + b'):
+// its rounding is 2^-24 of |mean| a, where x's own step is 2^-8 or 2^-11 of |x|. w and b do not wait for the statistics.
+template <typename T> constexpr bool kCentred = sizeof(T) == 4;
+template <typename T, int V>
 struct Affine {
   float2 nmu[kPairs<V>], a[kPairs<V>], b[kPairs<V>];
   __device__ __forceinline__ void params(const Geo& g, const Place& p, const void* gamma, const void* beta) {
@@ -573,7 +579,15 @@ struct Affine {
       put(r, k, q.y);
     });
 #pragma unroll
-    for (int k = 0; k < kPairs<V>; ++k) a[k] = __fmul2_rn(a[k], r[k]);
+    for (int k = 0; k < kPairs<V>; ++k) {
+      a[k] = __fmul2_rn(a[k], r[k]);
+      if constexpr (!kCentred<T>) b[k] = __ffma2_rn(nmu[k], a[k], b[k]);
+    }
+  }
+  // x becomes x - mean (or stays: 16-bit types); z of it
+  __device__ __forceinline__ float2 z(int k, float2& x) const {
+    if constexpr (kCentred<T>) x = __fadd2_rn(x, nmu[k]);
+    return __ffma2_rn(x, a[k], b[k]);
   }
 };
 
@@ -694,18 +708,27 @@ __global__ void __launch_bounds__(kThreads, kStatsBlocks) stats_kernel(const T* 
   __shared__ __align__(16) char smem[R::kBytes > V * kThreads * 16 ? R::kBytes : V * kThreads * 16];
   let_next_start();
   const Place p = place<V>(g);
-  R ring(smem, x, nullptr, nullptr, p.at, p.step, 0);
+  R ring(smem, x, nullptr, nullptr, p.at, p.step);
 #pragma unroll
-  for (int t = 0; t < kFwdAhead - 1; ++t) ring.start(t, t < p.mine);
+  for (int i = 0; i < kFwdAhead - 1; ++i) ring.start(i, i < p.mine);
   Moments<T, V> m;
   m.zero();
-  for (int t = 0; t < p.mine; ++t) {
-    Source<T, V, false> a;
-    ring.wait();
-    ring.get(t, a, smem);
-    ring.start(t + kFwdAhead - 1, t + kFwdAhead - 1 < p.mine);
-    if (t == 0) m.pivot(a.v);
-    m.add(a.v);
+  if (p.mine > 0) {
+    Vec<T, V> a;
+    a.load(x + p.at);
+    m.pivot(a);
+  }
+#pragma unroll 1
+  for (int t = 0; t < p.mine; t += kFwdAhead) {
+#pragma unroll
+    for (int i = 0; i < kFwdAhead; ++i) {
+      if (t + i >= p.mine) break;
+      Source<T, V, false> a;
+      ring.wait();
+      ring.get(i, a);
+      ring.start((i + kFwdAhead - 1) % kFwdAhead, t + i + kFwdAhead - 1 < p.mine);
+      m.add(a.v);
+    }
   }
   ring.drain();
   __syncthreads();
@@ -716,11 +739,11 @@ __global__ void __launch_bounds__(kThreads, kStatsBlocks) stats_kernel(const T* 
   block_moments<T, V>(g, p, m, x, reinterpret_cast<double2*>(smem), [&](int gi, double a, double c) { out[gi] = make_double2(a, c); });
 }
 
-// y of one vector, and its 8 bits (PACK: a block of 32 elements lies in 32 / V neighbouring threads, all with or all
+// y of one vector at element `at`, into `to`, and its 8 bits (PACK: a block of 32 elements lies in 32 / V neighbouring threads, all with or all
 // without a row here; every thread of the warp calls it).
 template <typename T, int V, int ACT, bool PACK>
-__device__ __forceinline__ void apply_one(const Vec<T, V>& v, const Affine<V>& k, const Geo& g, bool in, int64_t at,
-                                          T* __restrict__ y, uint8_t* __restrict__ codes,
+__device__ __forceinline__ void apply_one(const Vec<T, V>& v, const Affine<T, V>& k, const Geo& g, bool in, int64_t at,
+                                          T* __restrict__ to, uint8_t* __restrict__ codes,
                                           uint8_t* __restrict__ exps) {
   float2 f[kPairs<V>];
   v.to_f(f);
@@ -733,15 +756,15 @@ __device__ __forceinline__ void apply_one(const Vec<T, V>& v, const Affine<V>& k
     const q8::Codes<V> c = q8::encode<V>(e, byte, g.format, finite);
     if (in) {
       q8::store_codes<V>(codes + at, c);
-      if (at % q8::kBlock == 0) exps[at / q8::kBlock] = (uint8_t)byte;
+      if (((uint32_t)at & (q8::kBlock - 1)) == 0) exps[at / q8::kBlock] = (uint8_t)byte;
     }
   }
 #pragma unroll
-  for (int i = 0; i < kPairs<V>; ++i) f[i] = __ffma2_rn(__fadd2_rn(f[i], k.nmu[i]), k.a[i], k.b[i]);
+  for (int i = 0; i < kPairs<V>; ++i) f[i] = k.z(i, f[i]);
   act_values<T, ACT>(f, g.act, g.slope);
   Vec<T, V> r;
   r.from_f(f);
-  if (in) r.store(y + at);
+  if (in) r.store(to);
 }
 
 // y of a sample's edges.
@@ -768,11 +791,13 @@ __global__ void __launch_bounds__(kThreads, kApplyBlocks) apply_kernel(
   float2* stat = reinterpret_cast<float2*>(smem + R::kBytes);
   const Place p = place<V>(g);
   // (x is older than the kernel before this one)
-  const int end = p.tiles - 1;
-  R ring(smem, x, nullptr, nullptr, p.at + end * p.step, -p.step, 0);
+  const int skip = p.tiles - p.mine;       // 1 for a thread without a row in the last tile
+  int64_t at = p.at + (p.tiles - 1) * p.step;
+  T* to = y + at;
+  R ring(smem, x, nullptr, nullptr, at, -p.step);
 #pragma unroll
-  for (int t = 0; t < kFwdAhead - 1; ++t) ring.start(t, t <= end && end - t < p.mine);
-  Affine<V> k;
+  for (int i = 0; i < kFwdAhead - 1; ++i) ring.start(i, i >= skip && i < p.tiles);
+  Affine<T, V> k;
   k.params(g, p, gamma, beta);
   wait_for_previous();
   const double2* src = part + p.n * g.np * g.G + p.ga;
@@ -788,15 +813,22 @@ __global__ void __launch_bounds__(kThreads, kApplyBlocks) apply_kernel(
   if (p.b == 0)
     for (int i = threadIdx.x; i < p.gb - p.ga; i += blockDim.x) mean_rstd[p.n * g.G + p.ga + i] = stat[i];
   k.stats(g, p, [&](int gi) { return stat[gi - p.ga]; });
-  for (int t = 0; t < p.tiles; ++t) {
-    const int next = t + kFwdAhead - 1;
-    const bool in = end - t < p.mine;
-    Source<T, V, false> v;
-    ring.wait();
-    v.zero();
-    if (in) ring.get(t, v, smem);
-    ring.start(next, next <= end && end - next < p.mine);
-    apply_one<T, V, ACT, PACK>(v.v, k, g, in, p.at + (end - t) * p.step, y, codes, exps);
+#pragma unroll 1
+  for (int t = 0; t < p.tiles; t += kFwdAhead) {
+#pragma unroll
+    for (int i = 0; i < kFwdAhead; ++i) {
+      if (t + i >= p.tiles) break;
+      const bool in = t + i >= skip;
+      Source<T, V, false> v;
+      ring.wait();
+      if (PACK) v.zero();
+      if (in) ring.get(i, v);
+      const int next = t + i + kFwdAhead - 1;
+      ring.start((i + kFwdAhead - 1) % kFwdAhead, next >= skip && next < p.tiles);
+      if (PACK || in) apply_one<T, V, ACT, PACK>(v.v, k, g, in, at, to, codes, exps);
+      at -= p.step;
+      to -= p.step;
+    }
   }
   if (ACT < 0 && g.edges && p.b == 0) apply_edges<T, V, ACT>(g, p, x, gamma, beta, y, [&](int gi) { return stat[gi - p.ga]; });
 }
@@ -804,22 +836,19 @@ __global__ void __launch_bounds__(kThreads, kApplyBlocks) apply_kernel(
 // ---------------------------------------------------------------------------
 // Backward: sums
 // ---------------------------------------------------------------------------
-// dz and x - mean of one vector.
+// dz and x - mean (16-bit types: x) of one vector.
 template <typename T, int V, int ACT, bool Q>
-__device__ __forceinline__ void grad_one(const Source<T, V, Q>& v, const Vec<T, V>& d, const Affine<V>& k, const Geo& g,
+__device__ __forceinline__ void grad_one(const Source<T, V, Q>& v, const Vec<T, V>& d, const Affine<T, V>& k, const Geo& g,
                                          float2 (&xm)[kPairs<V>], float2 (&dz)[kPairs<V>]) {
   v.to_f(g.format, xm);
   d.to_f(dz);
   float2 z[kPairs<V>];
 #pragma unroll
-  for (int i = 0; i < kPairs<V>; ++i) {
-    xm[i] = __fadd2_rn(xm[i], k.nmu[i]);
-    z[i] = __ffma2_rn(xm[i], k.a[i], k.b[i]);
-  }
+  for (int i = 0; i < kPairs<V>; ++i) z[i] = k.z(i, xm[i]);
   act_grads<T, ACT>(dz, z, g.act, g.slope);
 }
 
-// dz and x - mean of one element of channel c.
+// dz and x - mean (16-bit types: x) of one element of channel c.
 template <typename T, int ACT, bool Q>
 __device__ __forceinline__ float2 grad_edge(const Geo& g, const T* __restrict__ dy, const void* __restrict__ x,
                                             const uint8_t* __restrict__ exps, const void* gamma, const void* beta,
@@ -828,17 +857,17 @@ __device__ __forceinline__ float2 grad_edge(const Geo& g, const T* __restrict__ 
   float2 xm[1], dz[1] = {make_float2(Elem<T>::to_f(dy[at]), 0.f)};
   v.load(x, exps, at);
   v.to_f(g.format, xm);
-  xm[0].x -= stat.x;
-  const float2 z[1] = {make_float2(
-      fmaf(xm[0].x, stat.y * param(gamma, g.pdtype, c, 1.f), param(beta, g.pdtype, c, 0.f)), 0.f)};
+  const float a = stat.y * param(gamma, g.pdtype, c, 1.f), b = param(beta, g.pdtype, c, 0.f);
+  if (kCentred<T>) xm[0].x -= stat.x;
+  const float2 z[1] = {make_float2(fmaf(xm[0].x, a, kCentred<T> ? b : fmaf(-stat.x, a, b)), 0.f)};
   act_grads<T, ACT>(dz, z, g.act, g.slope);
   return make_float2(dz[0].x, xm[0].x);
 }
 
-// The block's (sum dz, sum dz * (x - mean)) of a thread's columns: cpart gets them per channel (the second times rstd),
-// out(group, ..) the same times w, summed over the tile's channels of the group. edge(element, channel, stat): an
-// edge's dz and x - mean.
-template <int V, bool EDGES, typename Stat, typename Edge, typename Out>
+// The block's (sum dz, sum dz * (x - mean)) of a thread's columns (16-bit types: sum dz * x): cpart gets them per channel
+// (the second times rstd), out(group, ..) the same times w, summed over the tile's channels of the group.
+// edge(element, channel, stat): an edge's dz and x - mean, or x.
+template <typename T, int V, bool EDGES, typename Stat, typename Edge, typename Out>
 __device__ __forceinline__ void block_grads(const Geo& g, const Place& p, const float2 (&s1)[kPairs<V>],
                                             const float2 (&s2)[kPairs<V>], const void* gamma, float2* __restrict__ red,
                                             float2* __restrict__ cols, float2* __restrict__ cpart, Stat stat, Edge edge,
@@ -865,7 +894,8 @@ __device__ __forceinline__ void block_grads(const Geo& g, const Place& p, const 
     }
   }, [&](int i, float a, float c) {
     const int ch = p.j0 + i;
-    const float2 s = make_float2(a, c * stat((int)((unsigned)ch / (unsigned)g.Cg)).y);
+    const float2 m = stat((int)((unsigned)ch / (unsigned)g.Cg));
+    const float2 s = make_float2(a, (kCentred<T> ? c : fmaf(-m.x, a, c)) * m.y);
     cols[i] = s;
     cpart[(int64_t)blockIdx.x * g.C + ch] = s;
   });
@@ -892,29 +922,35 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_sums_kernel(
   __shared__ __align__(16) char smem[R::kBytes > 2 * kTable ? R::kBytes : 2 * kTable];
   let_next_start();
   const Place p = place<V>(g);
-  R ring(smem, x, dy, exps, p.at, p.step, g.sample * g.samples);
+  R ring(smem, x, dy, exps, p.at, p.step);
 #pragma unroll
-  for (int t = 0; t < kBwdAhead - 1; ++t) ring.start(t, t < p.mine);
+  for (int i = 0; i < kBwdAhead - 1; ++i) ring.start(i, i < p.mine);
   const float2* stats = mean_rstd + p.n * g.G;
-  Affine<V> k;
+  Affine<T, V> k;
   k.params(g, p, gamma, beta);
   k.stats(g, p, [&](int gi) { return stats[gi]; });
   float2 a1[kPairs<V>], a2[kPairs<V>];
 #pragma unroll
   for (int i = 0; i < kPairs<V>; ++i) a1[i] = a2[i] = two(0.f);
-  for (int t = 0; t < p.mine; ++t) {
-    Source<T, V, Q> v;
-    Vec<T, V> d;
-    ring.wait();
-    ring.get(t, v, smem);
-    ring.get_dy(t, d, smem);
-    ring.start(t + kBwdAhead - 1, t + kBwdAhead - 1 < p.mine);
-    float2 xm[kPairs<V>], dz[kPairs<V>];
-    grad_one<T, V, ACT, Q>(v, d, k, g, xm, dz);
+#pragma unroll 1
+  for (int t = 0; t < p.mine; t += kBwdAhead) {
 #pragma unroll
-    for (int i = 0; i < kPairs<V>; ++i) {
-      a1[i] = __fadd2_rn(a1[i], dz[i]);
-      a2[i] = __ffma2_rn(dz[i], xm[i], a2[i]);
+    for (int i = 0; i < kBwdAhead; ++i) {
+      if (t + i >= p.mine) break;
+      Source<T, V, Q> v;
+      Vec<T, V> d;
+      ring.wait();
+      ring.get(i, v);
+      ring.get_dy(i, d);
+      ring.next();
+      ring.start((i + kBwdAhead - 1) % kBwdAhead, t + i + kBwdAhead - 1 < p.mine);
+      float2 xm[kPairs<V>], dz[kPairs<V>];
+      grad_one<T, V, ACT, Q>(v, d, k, g, xm, dz);
+#pragma unroll
+      for (int j = 0; j < kPairs<V>; ++j) {
+        a1[j] = __fadd2_rn(a1[j], dz[j]);
+        a2[j] = __ffma2_rn(dz[j], xm[j], a2[j]);
+      }
     }
   }
   ring.drain();
@@ -923,7 +959,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_sums_kernel(
   if (g.tiles > 1)
     for (int i = threadIdx.x; i < g.G; i += blockDim.x)
       if (i < p.ga || i >= p.gb) out[i] = make_float2(0.f, 0.f);
-  block_grads<V, (ACT < 0)>(g, p, a1, a2, gamma, reinterpret_cast<float2*>(smem), reinterpret_cast<float2*>(smem + kTable), cpart,
+  block_grads<T, V, (ACT < 0)>(g, p, a1, a2, gamma, reinterpret_cast<float2*>(smem), reinterpret_cast<float2*>(smem + kTable), cpart,
                  [&](int gi) { return stats[gi]; },
                  [&](int64_t at, int c, float2 s) { return grad_edge<T, ACT, Q>(g, dy, x, exps, gamma, beta, at, c, s); },
                  [&](int gi, float a, float c) { out[gi] = make_float2(a, c); });
@@ -983,7 +1019,7 @@ inline __global__ void __launch_bounds__(kThreads) params_kernel(const float2* _
 
 // dx of one vector; k1, k2: rstd * A, rstd^2 * B.
 template <typename T, int V, int ACT, bool Q>
-__device__ __forceinline__ Vec<T, V> dx_one(const Source<T, V, Q>& v, const Vec<T, V>& d, const Affine<V>& k,
+__device__ __forceinline__ Vec<T, V> dx_one(const Source<T, V, Q>& v, const Vec<T, V>& d, const Affine<T, V>& k,
                                             const float2 (&k1)[kPairs<V>], const float2 (&k2)[kPairs<V>], const Geo& g) {
   float2 xm[kPairs<V>], dz[kPairs<V>];
   grad_one<T, V, ACT, Q>(v, d, k, g, xm, dz);
@@ -1006,8 +1042,11 @@ __device__ __forceinline__ void thread_coef(const Geo& g, const Place& p, const 
     put(k2, k, q.y);
   });
 }
-__device__ __forceinline__ float2 coef_of(const Geo& g, double rstd, double a, double c) {
-  return make_float2((float)(rstd * a * g.inv_m), (float)(rstd * rstd * c * g.inv_m));
+// dx = dz * rstd * w - (first + second * (x - mean)); for 16-bit types of x itself.
+template <typename T>
+__device__ __forceinline__ float2 coef_of(const Geo& g, float2 stat, double a, double c) {
+  const double rstd = stat.y, first = rstd * a * g.inv_m, second = rstd * rstd * c * g.inv_m;
+  return make_float2((float)(kCentred<T> ? first : first - stat.x * second), (float)second);
 }
 
 // dx of a sample's edges.
@@ -1044,11 +1083,13 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
   const Place p = place<V>(g);
   const float2* stats = mean_rstd + p.n * g.G;
   // (what it reads is older than the kernel before this one)
-  const int end = p.tiles - 1, skip = p.tiles - p.mine;          // skip: 1 for a thread without a row in the last tile
-  R ring(smem, x, dy, exps, p.at + end * p.step, -p.step, g.sample * g.samples);
+  const int skip = p.tiles - p.mine;       // 1 for a thread without a row in the last tile
+  const int64_t at = p.at + (p.tiles - 1) * p.step;
+  T* to = dx + at;
+  R ring(smem, x, dy, exps, at, -p.step);
 #pragma unroll
-  for (int t = 0; t < kBwdAhead - 1; ++t) ring.start(t, t >= skip && t <= end);
-  Affine<V> k;
+  for (int i = 0; i < kBwdAhead - 1; ++i) ring.start(i, i >= skip && i < p.tiles);
+  Affine<T, V> k;
   k.params(g, p, gamma, beta);
   k.stats(g, p, [&](int gi) { return stats[gi]; });
   wait_for_previous();
@@ -1060,23 +1101,29 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
       a += v.x;
       c += v.y;
     }
-  }, [&](int i, double a, double c) { coef[i] = coef_of(g, stats[p.ga + i].y, a, c); });
+  }, [&](int i, double a, double c) { coef[i] = coef_of<T>(g, stats[p.ga + i], a, c); });
   __syncthreads();
   if (p.mine > 0) {
     float2 k1[kPairs<V>], k2[kPairs<V>];
     thread_coef<V>(g, p, coef, k1, k2);
-    for (int t = 0; t <= end; ++t) {
-      const int next = t + kBwdAhead - 1;
-      ring.wait();
-      if (t >= skip) {
+#pragma unroll 1
+    for (int t = 0; t < p.tiles; t += kBwdAhead) {
+#pragma unroll
+      for (int i = 0; i < kBwdAhead; ++i) {
+        if (t + i >= p.tiles) break;
+        const bool in = t + i >= skip;
         Source<T, V, Q> v;
         Vec<T, V> d;
-        ring.get(t, v, smem);
-        ring.get_dy(t, d, smem);
-        ring.start(next, next <= end);
-        dx_one<T, V, ACT, Q>(v, d, k, k1, k2, g).store(dx + p.at + (end - t) * p.step);
-      } else {
-        ring.start(next, next <= end);
+        ring.wait();
+        if (in) {
+          ring.get(i, v);
+          ring.get_dy(i, d);
+        }
+        ring.next();
+        const int next = t + i + kBwdAhead - 1;
+        ring.start((i + kBwdAhead - 1) % kBwdAhead, next >= skip && next < p.tiles);
+        if (in) dx_one<T, V, ACT, Q>(v, d, k, k1, k2, g).store(to);
+        to -= p.step;
       }
     }
   }
@@ -1155,7 +1202,7 @@ __global__ void __launch_bounds__(kThreads) fwd_small_kernel(const T* __restrict
   const int groups = p.gb - p.ga;
   const char* own = smem + threadIdx.x * B;
   for (int t = 0; t < p.mine; ++t) copy_async<B>(shared_at(own) + t * kThreads * B, x + p.at + t * p.step);
-  Affine<V> k;
+  Affine<T, V> k;
   k.params(g, p, gamma, beta);
   asm volatile("cp.async.wait_all;" ::: "memory");
   Moments<T, V> m;
@@ -1177,7 +1224,7 @@ __global__ void __launch_bounds__(kThreads) fwd_small_kernel(const T* __restrict
     Vec<T, V> v;
     v.zero();
     if (t < p.mine) v.load(reinterpret_cast<const T*>(own + t * kThreads * B));
-    apply_one<T, V, ACT, PACK>(v, k, g, t < p.mine, p.at + t * p.step, y, codes, exps);
+    apply_one<T, V, ACT, PACK>(v, k, g, t < p.mine, p.at + t * p.step, y + p.at + t * p.step, codes, exps);
   }
   if (ACT < 0 && g.edges && p.b == 0) apply_edges<T, V, ACT>(g, p, x, gamma, beta, y, [&](int gi) { return stat[gi - p.ga]; });
   if (g.nb > 1) cluster_wait();
@@ -1206,7 +1253,7 @@ __global__ void __launch_bounds__(kThreads)
     copy_async<YB>(shared_at(own_dy) + t * kThreads * YB, dy + p.at + t * p.step);
   }
   const float2* stats = mean_rstd + p.n * g.G;
-  Affine<V> k;
+  Affine<T, V> k;
   k.params(g, p, gamma, beta);
   k.stats(g, p, [&](int gi) { return stats[gi]; });
   auto get = [&](int t, Source<T, V, Q>& v, Vec<T, V>& d) {
@@ -1235,10 +1282,10 @@ __global__ void __launch_bounds__(kThreads)
       s2[j] = __ffma2_rn(dz[j], xm[j], s2[j]);
     }
   }
-  block_grads<V, (ACT < 0)>(g, p, s1, s2, gamma, red, cols, cpart, [&](int gi) { return stats[gi]; },
+  block_grads<T, V, (ACT < 0)>(g, p, s1, s2, gamma, red, cols, cpart, [&](int gi) { return stats[gi]; },
                  [&](int64_t at, int c, float2 s) { return grad_edge<T, ACT, Q>(g, dy, x, exps, gamma, beta, at, c, s); },
                  [&](int gi, float a, float c) { mine[gi - p.ga] = make_double2(a, c); });
-  cluster_sums(g, groups, mine, [&](int i, double a, double c) { coef[i] = coef_of(g, stats[p.ga + i].y, a, c); });
+  cluster_sums(g, groups, mine, [&](int i, double a, double c) { coef[i] = coef_of<T>(g, stats[p.ga + i], a, c); });
   if (p.mine > 0) {
     float2 k1[kPairs<V>], k2[kPairs<V>];
     thread_coef<V>(g, p, coef, k1, k2);

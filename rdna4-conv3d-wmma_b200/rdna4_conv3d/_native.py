@@ -827,11 +827,15 @@ Q8_FORMATS = {"int8": 0, "e4m3": 1}
 ACTIVATIONS = {"none": 0, "relu": 1, "leaky_relu": 2, "silu": 3, "gelu": 4}
 
 
-def q8_buffers(x: torch.Tensor):
+def q8_exponents(count: int, words: bool = False) -> int:
+    """Exponents of count elements; ``words``: as whole words, which the group norm's backward reads."""
+    return (count + 127) // 128 * 4 if words else (count + Q8_BLOCK - 1) // Q8_BLOCK
+
+
+def q8_buffers(x: torch.Tensor, words: bool = False):
     """Empty codes and exponents for x's elements."""
     count = x.numel()
-    return (x.new_empty(count, dtype=torch.uint8),
-            x.new_empty((count + Q8_BLOCK - 1) // Q8_BLOCK, dtype=torch.uint8))
+    return x.new_empty(count, dtype=torch.uint8), x.new_empty(q8_exponents(count, words), dtype=torch.uint8)
 
 
 def pack8(x: torch.Tensor, fmt: int):
@@ -873,7 +877,7 @@ def gn_forward(x: torch.Tensor, plan: GnPlan, weight, bias, fmt: Optional[int]):
     mean_rstd = x.new_empty((plan.stats,), dtype=torch.float32)
     codes = exps = ws = None
     if fmt is not None:
-        codes, exps = q8_buffers(x)
+        codes, exps = q8_buffers(x, True)
     nb = plan.fwd_bytes
     if nb:
         ws = x.new_empty(nb, dtype=torch.uint8)

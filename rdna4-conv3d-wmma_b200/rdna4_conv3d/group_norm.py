@@ -93,7 +93,7 @@ class GroupNormActFn(torch.autograd.Function):
         else:
             count = shape.numel()
             x = _as_saved(x, count, torch.uint8, device)
-            exps = _as_saved(exps, -(-count // _native.Q8_BLOCK), torch.uint8, device)
+            exps = _as_saved(exps, _native.q8_exponents(count, True), torch.uint8, device)
         w, b, pdtype = _params(weight, bias)
         for t in (w, b):
             if t is not None and (t.shape[0] != shape[1] or t.device != device):
