@@ -19,12 +19,10 @@ namespace q8 {
 
 constexpr int kBlock = 32;
 
-// Stored exponent byte of a block whose largest finite magnitude has these fp32 bits.
+// Stored exponent byte of a block whose largest finite magnitude has these fp32 bits. 127 = 1.984375 * 2^6 and
+// 448 = 1.75 * 2^8: what is added to the mantissa carries into the exponent when it is above theirs (0x7e0000, 0x600000).
 __device__ __forceinline__ int exponent_byte(uint32_t amax_bits, int format) {
-  const int e = (int)(amax_bits >> 23);
-  const uint32_t m = amax_bits & 0x7fffffu;
-  // 127 = 1.984375 * 2^6, 448 = 1.75 * 2^8: one power more when the mantissa is above the limit's
-  const int b = format == R4C_Q8_INT8 ? e - 6 + (m > 0x7e0000u ? 1 : 0) : e - 8 + (m > 0x600000u ? 1 : 0);
+  const int b = format == R4C_Q8_INT8 ? (int)((amax_bits + 0x1ffffu) >> 23) - 6 : (int)((amax_bits + 0x1fffffu) >> 23) - 8;
   return b < 0 ? 0 : b;
 }
 __device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
@@ -170,27 +168,30 @@ __device__ __forceinline__ void decode(const Codes<V>& c, int byte, int format, 
   }
 }
 
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+// The larger magnitudes of two pairs of 16-bit numbers; NaN stays.
+template <typename T>
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  if constexpr (__is_same(T, __half)) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
 // Largest finite magnitude (fp32 bits) of a block that lies in neighbouring lanes, each with NW words of T; every lane of
-// `mask` takes part. `finite`: this lane's elements all are. Magnitudes of one type order as their bits do, so 16-bit
-// types are compared two at a time as they lie.
+// `mask` takes part. `finite`: this lane's elements all are. 16-bit types are compared two at a time as they lie.
 template <typename T, int NW>
 __device__ __forceinline__ uint32_t block_amax(const uint32_t (&w)[NW], uint32_t mask, bool* finite) {
   constexpr bool kWide = sizeof(T) == 4;
   constexpr uint32_t kSign = kWide ? 0x7fffffffu : 0x7fff7fffu;
   // infinity's bits: everything from there on is not finite
   constexpr uint32_t kInf = kWide ? 0x7f800000u : (__is_same(T, __half) ? 0x7c00u : 0x7f80u);
-  auto larger = [](uint32_t a, uint32_t b) { return kWide ? max(a, b) : max_u16x2(a, b); };
-  auto halves = [&](uint32_t m) { return kWide ? m : max(m & 0xffffu, m >> 16); };
-  uint32_t m = 0;
+  uint32_t m = w[0] & kSign;
 #pragma unroll
-  for (int k = 0; k < NW; ++k) m = larger(m, w[k] & kSign);
-  m = halves(m);
+  for (int k = 1; k < NW; ++k) {
+    if constexpr (kWide) m = max(m, w[k] & kSign);
+    else m = larger2<T>(m, w[k] & kSign);
+  }
+  if constexpr (!kWide) m = max(m & 0xffffu, m >> 16);
   const bool bad = m >= kInf;
   *finite = !bad;
   if (__any_sync(mask, bad)) {                  // NaN or infinities somewhere: the finite ones alone

@@ -841,7 +841,7 @@ def q8_buffers(x: torch.Tensor, words: bool = False):
 def pack8(x: torch.Tensor, fmt: int):
     """(codes, exponents) of a dense tensor's elements in memory order."""
     codes, exps = q8_buffers(x)
-    _launch("r4c_pack8", lib().r4c_pack8, x.device, x.data_ptr(), x.numel(), dtype_code(x.dtype), fmt,
+    _launch("r4c_pack8", lib().r4c_pack8, x.device, x.data_ptr(), codes.shape[0], dtype_code(x.dtype), fmt,
             codes.data_ptr(), exps.data_ptr())
     return codes, exps
 

@@ -67,25 +67,29 @@ def pack8(x: torch.Tensor, format: str = "int8") -> Packed8:
     and infinities come back as NaN. A tensor with gaps or overlaps is copied
     first; autograd does not see this call.
     """
-    check_format(format)
-    if x.dtype not in _FLOATS:
-        raise TypeError(f"pack8 takes bf16, fp16 or fp32, got {x.dtype}")
+    dtype = x.dtype
+    code = _native.Q8_FORMATS.get(format)
+    if code is None:
+        check_format(format)
+    if dtype not in _FLOATS:
+        raise TypeError(f"pack8 takes bf16, fp16 or fp32, got {dtype}")
     refuse_blind(x)
-    xd = x.detach()
-    if not _is_dense(xd):
-        xd = xd.contiguous()
+    if not _is_dense(x):
+        x = x.detach().contiguous()
     if not x.is_cuda:
-        codes, exps = _pack_torch(xd, format)
+        codes, exps = _pack_torch(x.detach(), format)
     else:
-        codes, exps = _native.pack8(xd, _native.Q8_FORMATS[format])
-    return Packed8(codes, exps, xd.shape, xd.stride(), xd.dtype, format)
+        codes, exps = _native.pack8(x, code)
+    return Packed8(codes, exps, x.shape, x.stride(), dtype, format)
 
 
 def unpack8(packed: Packed8) -> torch.Tensor:
     """The values that the 8 bits hold, in the packed tensor's type, shape and strides: code * 2^e, at most the
     type's largest finite number."""
     codes, exps, shape, stride, dtype, fmt = packed
-    check_format(fmt)
+    code = _native.Q8_FORMATS.get(fmt)
+    if code is None:
+        check_format(fmt)
     count = shape.numel()
     if codes.numel() != count or exps.numel() != (count + 31) // _native.Q8_BLOCK:
         raise ValueError(f"{count} elements need as many codes and {-(-count // _native.Q8_BLOCK)} exponents, got "
@@ -97,12 +101,13 @@ def unpack8(packed: Packed8) -> torch.Tensor:
     out = torch.empty_strided(shape, stride, dtype=dtype, device=codes.device)
     if not _is_dense(out):
         raise ValueError(f"strides {tuple(stride)} of shape {tuple(shape)} leave gaps or overlap")
-    if not codes.is_contiguous() or codes.data_ptr() & 15:
+    if codes.data_ptr() & 15 or not codes.is_contiguous():
         codes = codes.clone(memory_format=torch.contiguous_format)
-    exps = exps.contiguous()
+    if not exps.is_contiguous():
+        exps = exps.contiguous()
     if not codes.is_cuda:
         return _unpack_torch(codes, exps, fmt, out)
-    return _native.unpack8(codes, exps, _native.Q8_FORMATS[fmt], out)
+    return _native.unpack8(codes, exps, code, out)
 
 
 def _memory_order(x: torch.Tensor) -> torch.Tensor:
