@@ -12,7 +12,7 @@ namespace {
 struct Plan {
   Geo g;
   int V, threads;
-  int stats_nb;
+  int sums_nb;       // blocks a sample of the sums
 };
 
 bool ok_desc(const r4c_gn_desc* d) {
@@ -24,10 +24,10 @@ bool ok_desc(const r4c_gn_desc* d) {
 
 // A cluster for each sample and channel tile of whole groups, if one can keep its share on chip and is expected to be
 // faster than two passes. Narrower tiles and larger clusters bring more SMs to few samples; tiles below 48 bytes a
-// voxel would read sectors twice. The modelled times (us) follow these measurements, forward / backward without the
-// parameters' sums: [1,192,4,8,8] bf16 silu, 1 block of 6 vectors a thread 5.9, 8 blocks of 1 vector 4.4, two passes
-// 5.9; [64,96,6,6,6] 96 groups, 6 vectors 5.5 / 6.6, two passes 9.7 / 10.5; [4,192,8,16,16] 6 vectors in clusters of 4
-// 7.5 / 10.6, two passes 7.7 / 11.9; 512 blocks in clusters of 4 for the second of these 11.4 / 14.9.
+// voxel would read sectors twice. The modelled times (us) follow these measurements, forward / backward: [1,192,4,8,8]
+// bf16 silu, 1 block of 6 vectors a thread 5.9, 8 blocks of 1 vector 4.4, two passes 5.7; [64,96,6,6,6] 96 groups, 6
+// vectors 5.5 / 8.4, two passes 9.7 / 10.5, 512 blocks in clusters of 4 11.4 / 17.4; [4,192,8,16,16] 6 vectors in 128
+// blocks in clusters of 4 7.5 / 12.8, two passes 7.9 / 11.6. (The small backward's parameters take a launch of their own.)
 void plan_small(const r4c_gn_desc* d, bool backward, int V, Geo& g, int* threads) {
   const int most = backward ? kSmallBwd : kSmallFwd, elem = (int)dtype_bytes(d->dtype);
   const double each = backward ? 0.5 : 0.35, mb = (double)d->samples * (double)g.sample * elem * 1e-6;
@@ -46,7 +46,8 @@ void plan_small(const r4c_gn_desc* d, bool backward, int V, Geo& g, int* threads
         if (nv > most || (cl > 1 && per < 4)) continue;
         const double blocks = (double)d->samples * tiles * cl;
         const double waves = std::ceil(blocks / (148.0 * 2));
-        const double cost = 3.5 + each * nv + (cl > 1 ? 0.2 + 0.004 * blocks : 0.0) + (waves - 1.0) * (1.5 + each * nv);
+        const double cost = (backward ? 5.5 : 3.5) + each * nv + (cl > 1 ? 0.2 + (backward ? 0.025 : 0.015) * blocks : 0.0) +
+                            (waves - 1.0) * (1.5 + each * nv);
         if (cost < best - 1e-9) {
           best = cost;
           g.small = (int)nv;
@@ -85,7 +86,7 @@ bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
   g.act = d->activation;
   g.pdtype = d->param_dtype;
   g.format = g.pack = g.wide_params = 0;
-  pl->stats_nb = 1;
+  pl->sums_nb = 1;
   // the widest vector that parts a voxel's channels, or whose rows of lcm(C, V) elements (several voxels) fit a block's
   // threads
   int V = 16 / (int)dtype_bytes(d->dtype);
@@ -100,6 +101,7 @@ bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
     g.blocks = d->samples * g.nb;
     g.chunk_tiles = g.small;
     g.np = g.nb * g.tiles;
+    pl->sums_nb = g.nb;
     return g.blocks + g.C <= INT32_MAX;
   }
   const int lanes = g.L / V;
@@ -108,12 +110,12 @@ bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
   g.R = std::max(1, kThreads / g.lanes);
   if (g.R > 4) g.R = g.R / 4 * 4;       // a tile of rows starts at a block of 32 elements (fused packing)
   pl->threads = cdiv(g.R * g.lanes, 32) * 32;
-  // one wave of the blocks that fit the SMs, none with less than four rows for each thread
-  pl->stats_nb = blocks_for(g, d->samples, kStatsBlocks);
+  // one wave of blocks, none with less than four rows for each thread; the sums' wave leaves room for blocks of the
+  // second pass, which start under it
+  const Geo sums = split(g, blocks_for(g, d->samples, backward ? kBwdSumsFit : kStatsFit));
+  pl->sums_nb = sums.nb;
   g = split(g, blocks_for(g, d->samples, backward ? kBwdBlocks : kApplyBlocks));
-  const Geo sums = split(g, pl->stats_nb);
-  pl->stats_nb = sums.nb;
-  g.np = (backward ? g.nb : sums.nb) * g.tiles;
+  g.np = sums.nb * g.tiles;
   const int64_t most = std::max(g.blocks, sums.blocks);
   return most + g.C <= INT32_MAX && g.tiles <= 65535 && g.rows / g.R < INT32_MAX;
 }
@@ -128,10 +130,12 @@ bool fused_pack(const Plan& pl, size_t elem) {
 }
 
 size_t fwd_bytes(const Plan& pl) {
-  return align_up((size_t)(pl.g.blocks / pl.g.nb) * pl.stats_nb * pl.g.tiles * pl.g.G * sizeof(double2), 256);
+  return align_up((size_t)pl.g.samples * pl.sums_nb * pl.g.tiles * pl.g.G * sizeof(double2), 256);
 }
-size_t cpart_bytes(const Geo& g) { return align_up((size_t)g.blocks * g.C * sizeof(float2), 256); }
-size_t gpart_bytes(const Geo& g) { return align_up((size_t)g.blocks * g.tiles * g.G * sizeof(float2), 256); }
+size_t cpart_bytes(const Plan& pl) { return align_up((size_t)pl.g.samples * pl.sums_nb * pl.g.C * sizeof(float2), 256); }
+size_t bwd_bytes(const Plan& pl) {
+  return cpart_bytes(pl) + align_up((size_t)pl.g.samples * pl.sums_nb * pl.g.tiles * pl.g.G * sizeof(float2), 256);
+}
 
 // Parameters as fp32 words of four: a thread's channels follow each other where a row is one voxel.
 int wide_params(const Geo& g, const void* gamma, const void* beta) {
@@ -153,7 +157,7 @@ extern "C" {
 size_t r4c_gn_workspace_size(const r4c_gn_desc* desc, int backward) {
   Plan pl;
   if (!ok_desc(desc) || !make_plan(desc, backward != 0, &pl)) return 0;
-  if (backward) return cpart_bytes(pl.g) + gpart_bytes(pl.g);
+  if (backward) return bwd_bytes(pl);
   return pl.g.small ? 0 : fwd_bytes(pl);
 }
 
@@ -175,7 +179,7 @@ int r4c_gn_fwd(const r4c_gn_desc* desc, const void* x, const void* gamma, const 
   a.y = y;
   a.mean_rstd = reinterpret_cast<float2*>(mean_rstd);
   a.part = static_cast<double2*>(ws);
-  a.stats_nb = pl.stats_nb;
+  a.sums_nb = pl.sums_nb;
   pl.g.wide_params = wide_params(pl.g, gamma, beta);
   a.codes = static_cast<uint8_t*>(codes);
   a.exps = static_cast<uint8_t*>(exponents);
@@ -206,7 +210,7 @@ int r4c_gn_bwd(const r4c_gn_desc* desc, const void* dy, const void* x, int forma
   if (!dy || !x || !mean_rstd) return R4C_ERR_INVALID;
   if (exponents && format != R4C_Q8_INT8 && format != R4C_Q8_E4M3) return R4C_ERR_INVALID;
   if (!aligned(dy) || !aligned(x) || !aligned(exponents) || !aligned(dx) || !aligned(ws)) return R4C_ERR_ALIGN;
-  if (!ws || ws_bytes < cpart_bytes(pl.g) + gpart_bytes(pl.g)) return R4C_ERR_WORKSPACE;
+  if (!ws || ws_bytes < bwd_bytes(pl)) return R4C_ERR_WORKSPACE;
   if (!dx && !dgamma && !dbeta) return R4C_OK;
   BwdArgs a;
   a.dy = dy;
@@ -219,7 +223,8 @@ int r4c_gn_bwd(const r4c_gn_desc* desc, const void* dy, const void* x, int forma
   a.dgamma = dgamma;
   a.dbeta = dbeta;
   a.cpart = static_cast<float2*>(ws);
-  a.gpart = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) + cpart_bytes(pl.g));
+  a.gpart = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) + cpart_bytes(pl));
+  a.sums_nb = pl.sums_nb;
   pl.g.format = format;
   pl.g.wide_params = wide_params(pl.g, gamma, beta);
   if (desc->dtype == R4C_BF16) return status(launch_bwd<__nv_bfloat16>(a, pl.g, pl.V, pl.threads, s));

@@ -33,6 +33,9 @@ namespace gn {
 constexpr int kThreads = 256;   // at most, per block
 // Blocks that fit an SM beside each other (the registers that each kernel may take follow from it).
 constexpr int kStatsBlocks = 4, kApplyBlocks = 4, kBwdBlocks = 3;
+// Blocks an SM that the sums run in: with two of them, blocks of the second pass fit beside them and have started when
+// the sums end (forward of [4,48,32,64,64] 26.7 -> 24.1 us, [2,30,37,41,53] 18.8 -> 16.4, [4,24,64,128,128] the same).
+constexpr int kStatsFit = 2, kBwdSumsFit = 3;
 // Vectors of a thread on their way at a time, plus one.
 constexpr int kFwdAhead = 8, kBwdAhead = 4;
 // Samples that a cluster keeps on chip: vectors of a thread at most (forward; backward, which keeps dy too), groups of
@@ -1068,7 +1071,7 @@ template <typename T, int V, int ACT, bool Q>
 __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
     const T* __restrict__ dy, const void* __restrict__ x, const uint8_t* __restrict__ exps,
     const float2* __restrict__ mean_rstd, const void* __restrict__ gamma, const void* __restrict__ beta,
-    const __grid_constant__ Geo g, const float2* __restrict__ cpart, const float2* __restrict__ gpart,
+    const __grid_constant__ Geo g, int64_t parts, const float2* __restrict__ cpart, const float2* __restrict__ gpart,
     T* __restrict__ dx, float* __restrict__ dgamma, float* __restrict__ dbeta) {
   using R = Ring<T, V, Q, true, kBwdAhead>;
   extern __shared__ __align__(16) char smem[];
@@ -1077,7 +1080,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
     wait_for_previous();
     const int warps = blockDim.x / 32;
     const int64_t c = ((blockIdx.x - g.blocks) * gridDim.y + blockIdx.y) * warps + threadIdx.x / 32;
-    if (c < g.C) param_grads(cpart, g.blocks, g.C, (int)c, dgamma, dbeta);
+    if (c < g.C) param_grads(cpart, parts, g.C, (int)c, dgamma, dbeta);
     return;
   }
   const Place p = place<V>(g);
@@ -1310,7 +1313,7 @@ struct FwdArgs {
   float2* mean_rstd;
   double2* part;
   uint8_t *codes, *exps;    // null: not wanted
-  int stats_nb;             // blocks a sample of the sums
+  int sums_nb;              // blocks a sample of the sums
 };
 struct BwdArgs {
   const void *dy, *x, *gamma, *beta;
@@ -1319,6 +1322,7 @@ struct BwdArgs {
   void* dx;                 // null: not wanted
   float *dgamma, *dbeta;    // null: not wanted
   float2 *cpart, *gpart;
+  int sums_nb;              // blocks a sample of the sums
 };
 
 template <typename T> cudaError_t launch_fwd(const FwdArgs& a, const Geo& g, int V, int threads, cudaStream_t s);

@@ -85,8 +85,7 @@ cudaError_t fwd_v(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
     return fwd_small<T, V, ACT, false>(a, g, threads, s);
   }
   const size_t smem = Ring<T, V, false, false, kFwdAhead>::kBytes + sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
-  // the sums' blocks are smaller than the second pass's: more of them fit an SM
-  const Geo sums = split(g, a.stats_nb);
+  const Geo sums = split(g, a.sums_nb);
   stats_kernel<T, V><<<dim3((unsigned)sums.blocks, g.tiles), threads, 0, s>>>(x, sums, a.part);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
@@ -104,25 +103,27 @@ cudaError_t bwd_v(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   dim3 grid((unsigned)g.blocks, g.tiles);
   const T* dy = static_cast<const T*>(a.dy);
   const bool params = a.dgamma || a.dbeta;
+  const Geo sums = g.small ? g : split(g, a.sums_nb);
   auto params_next = [&] {
     note_launches(1);
-    return launch_next(params_kernel, dim3(g.blocks < kWideParts ? cdiv(g.C, kThreads / 32) : g.C), kThreads, 0, s,
-                       a.cpart, g.blocks, g.C, a.dgamma, a.dbeta);
+    return launch_next(params_kernel, dim3(sums.blocks < kWideParts ? cdiv(g.C, kThreads / 32) : g.C), kThreads, 0, s,
+                       a.cpart, sums.blocks, g.C, a.dgamma, a.dbeta);
   };
   if (g.small && a.dx) {
     const cudaError_t e = bwd_small<T, V, ACT, Q>(a, g, threads, s);
     return e != cudaSuccess || !params ? e : params_next();
   }
   const size_t smem = Ring<T, V, Q, true, kBwdAhead>::kBytes + sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
-  bwd_sums_kernel<T, V, ACT, Q><<<grid, threads, 0, s>>>(dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.cpart, a.gpart);
+  bwd_sums_kernel<T, V, ACT, Q><<<dim3((unsigned)sums.blocks, g.tiles), threads, 0, s>>>(
+      dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, sums, a.cpart, a.gpart);
   note_launches(1);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !a.dx) return e != cudaSuccess ? e : params_next();
-  const bool beside = params && g.blocks < kWideParts;
+  const bool beside = params && sums.blocks < kWideParts;
   if (beside) grid.x += cdiv(g.C, (int64_t)g.tiles * (threads / 32));
   note_launches(1);
   e = launch_next(bwd_dx_kernel<T, V, ACT, Q>, grid, threads, smem, s, dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta,
-                  g, a.cpart, a.gpart, static_cast<T*>(a.dx), a.dgamma, a.dbeta);
+                  g, sums.blocks, a.cpart, a.gpart, static_cast<T*>(a.dx), a.dgamma, a.dbeta);
   if (e != cudaSuccess || !params || beside) return e;
   return params_next();
 }
