@@ -420,6 +420,8 @@ class Conv3dKept8Fn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_out):
         from .checkpoint8 import Packed8, unpack8
+        from .logprobs import refuse_twice
+        refuse_twice()
         codes, exps, weight = ctx.saved_tensors
         return (*_conv3d_backward(ctx, *ctx.was, lambda: unpack8(Packed8(codes, exps, *ctx.packed)), weight, grad_out),
                 None, None, None, None)

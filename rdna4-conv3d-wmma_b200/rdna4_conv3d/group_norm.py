@@ -200,8 +200,11 @@ def _normalised(x, groups, mean, rstd):
 def _group_norm_torch(x, groups, weight, bias, eps, activation, slope, checkpoint):
     """The same in torch operations, at least in fp32."""
     if x.numel() == 0:
-        y = x if weight is None else x * weight.reshape(1, -1, *(1,) * (x.dim() - 2)).to(x.dtype)
-        return y.clone()
+        y, each = x.clone(), (1, -1) + (1,) * (x.dim() - 2)
+        for t in (weight, bias):                         # (they get gradients of 0)
+            if t is not None:
+                y = y + t.reshape(each).to(x.dtype)
+        return y
     if checkpoint is not None and torch.is_grad_enabled():
         return _KeptTorchFn.apply(x, weight, bias, groups, eps, activation, slope, checkpoint)
     acc = torch.promote_types(x.dtype, torch.float32)

@@ -513,3 +513,75 @@ def test_edges_of_samples(cuda_ready, shape, groups, dtype, fmt):
     x, _, w, b, dy = _args(shape, groups, dtype, seed=5)
     y = group_norm_act(x.detach(), groups, w.detach(), b.detach(), activation="relu")
     R.check(dict(y=y), R.ref(x, groups, w, b, 1e-5, "relu", SLOPE))
+
+
+def test_one_sample_past_32_bits(cuda_ready):
+    """A single sample of 2.2 G elements: offsets inside it pass 32 bits."""
+    x = torch.empty((1, 720, 320, 400, 24), device="cuda", dtype=BF).normal_(generator=_gen(1)).movedim(-1, 1)
+    assert x.numel() > 2 ** 31
+    w = torch.linspace(0.5, 1.5, 24, device="cuda")
+    s1 = torch.zeros(8, dtype=torch.float64, device="cuda")
+    s2 = torch.zeros_like(s1)
+    for part in x[0].split(40, 1):
+        v = part.movedim(0, -1).reshape(-1, 8, 3).float()
+        s1 += v.sum((0, 2), dtype=torch.float64)
+        s2 += (v * v).sum((0, 2), dtype=torch.float64)
+        del v
+    m = x.numel() / 8
+    mean = (s1 / m).repeat_interleave(3).reshape(24, 1, 1)
+    rstd = ((s2 / m - (s1 / m) ** 2 + 1e-5) ** -0.5).repeat_interleave(3).reshape(24, 1, 1)
+    y = group_norm_act(x, 8, w)
+    for d in (0, 359, 719):
+        want = (x[0, :, d].double() - mean) * rstd * w.double().reshape(24, 1, 1)
+        # half a step, and the sums of squares taken here in fp32 products (2^-24 each, unbiased) far below it
+        assert bool(((y[0, :, d].double() - want).abs() <= R.half_step(want, BF) + R.K * (1 + want.abs())).all())
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    y = group_norm_act(x, 8, w, checkpoint="e4m3")
+    dy = torch.zeros_like(y)
+    dy[0, :, 719] = 1.0                                   # dz = w there: dw = the sum of xh over the last plane
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    xh = (R.held(x.detach()[:, :, 719:], "e4m3")[0, :, 0].double() - mean) * rstd
+    # (blocks of 32 elements are the same: a plane is a whole number of them)
+    torch.testing.assert_close(dw.double(), xh.sum((1, 2)), rtol=1e-4, atol=128000 * R.K)
+    assert bool(dx[0, :, 719].abs().amax() > 0.1) and bool(dx[0, :, 0].abs().amax() < 1e-2)
+
+
+def test_refuses_a_second_differentiation_of_kept_convs(cuda_ready):
+    from rdna4_conv3d import conv3d_wmma
+    x = torch.randn(1, 8, 4, 8, 8, device="cuda", dtype=BF).contiguous(memory_format=CL).requires_grad_(True)
+    w = torch.randn(8, 8, 3, 3, 3, device="cuda", requires_grad=True)
+    y = conv3d_wmma(x, w, None, 1, 1, checkpoint="int8")
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(y.float().sum(), w, create_graph=True)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_hooks_on_kept_convs(cuda_ready, fmt):
+    from rdna4_conv3d import conv3d_wmma
+    x = torch.randn(2, 24, 6, 8, 10, device="cuda", dtype=BF, generator=_gen(1)).contiguous(memory_format=CL).requires_grad_(True)
+    w = torch.randn(24, 24, 3, 3, 3, device="cuda", generator=_gen(2), requires_grad=True)
+    want = torch.autograd.grad(conv3d_wmma(x, w, None, 1, 1, checkpoint=fmt).float().sum(), (x, w))
+    for hook in HOOKS.values():
+        with hook():
+            y = conv3d_wmma(x, w, None, 1, 1, checkpoint=fmt)
+        for a, b in zip(torch.autograd.grad(y.float().sum(), (x, w)), want):
+            assert torch.equal(a, b)
+    with saved_tensors_hooks(lambda t: t[:3].clone(), lambda t: t):
+        y = conv3d_wmma(x, w, None, 1, 1, checkpoint=fmt)
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.autograd.grad(y.float().sum(), w)
+
+
+def test_inference_and_frozen_parts(cuda_ready):
+    x, w, b, dy = _inputs((2, 24, 5, 6, 7), BF)
+    want = R.ref(x, 8, w, b, 1e-5, "gelu", SLOPE)
+    with torch.inference_mode():
+        R.check(dict(y=group_norm_act(x, 8, w, b, activation="gelu", checkpoint="int8")), want)
+    m = GroupNormAct3d(8, 24, activation="gelu", checkpoint="int8").cuda().requires_grad_(False)
+    y = m(x.detach())
+    assert not y.requires_grad
+    y = m(x)
+    assert torch.equal(y, m(x.detach()))
+    y.backward(dy)
+    assert x.grad is not None and m.weight.grad is None

@@ -106,6 +106,12 @@ def test_empty_and_degenerate():
     torch.testing.assert_close(group_norm_act(x, 5, w, b), b.expand(2, 5))
 
 
+def test_empty_bias():
+    x, b = torch.zeros(2, 6, 0), torch.ones(6, requires_grad=True)
+    group_norm_act(x, 3, None, b).sum().backward()
+    assert bool((b.grad == 0).all())
+
+
 # --- 8 bits ------------------------------------------------------------------
 def special(dtype, seed=2):
     """Blocks that a format can go wrong at: nothing, one value, border values, subnormals, huge and non-finite ones."""
