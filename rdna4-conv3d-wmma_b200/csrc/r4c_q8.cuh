@@ -26,9 +26,7 @@ __device__ __forceinline__ int exponent_byte(uint32_t amax_bits, int format) {
   return b < 0 ? 0 : b;
 }
 __device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
-__device__ __forceinline__ float scale(int byte) {
-  return __uint_as_float(byte ? (uint32_t)byte << 23 : 0x00400000u);
-}
+__device__ __forceinline__ float scale(int byte) { return __uint_as_float(max((uint32_t)byte << 23, 0x00400000u)); }
 
 // V codes (V = 1, 2, 4 or 8) in the low bytes of the words.
 template <int V>
@@ -115,56 +113,58 @@ template <> struct Limits<float> {
 template <typename T, int V>
 __device__ __forceinline__ void decode(const Codes<V>& c, int byte, int format, float (&f)[V]) {
   const float s = scale(byte);
+  bool rare = byte < Limits<T>::low;                          // T's rounding, its largest number, NaN
   if (format == R4C_Q8_INT8) {
     // 0x4b0000uu is 2^23 + u exactly: the signed code is that minus 2^23 + 128 (no integer-to-float conversions,
-    // which share a slow pipe)
-    uint32_t nan = 0;
+    // which share a slow pipe). Times 2^e it is exact either way round: one multiply-add a value, while
+    // 2^e (2^23 + 128) is a number (e <= 103).
+    constexpr int kHigh = Limits<T>::high_int8 < 230 ? Limits<T>::high_int8 : 230;
+    uint32_t u[V > 4 ? 2 : 1], zero = 0;
 #pragma unroll
     for (int i = 0; i < (V > 4 ? 2 : 1); ++i) {
-      const uint32_t u = c.w[i] ^ 0x80808080u;
-      uint32_t zero = (u - 0x01010101u) & ~u & 0x80808080u;   // a byte of u is 0: some code is -128
-      if (V < 4) zero &= 0xffffffffu >> (32 - 8 * (V < 4 ? V : 4));
-      nan |= zero;
-#pragma unroll
-      for (int k = 4 * i; k < V && k < 4 * i + 4; ++k)
-        f[k] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + (k & 3)));
+      u[i] = c.w[i] ^ 0x80808080u;
+      zero |= (u[i] - 0x01010101u) & ~u[i];                   // a byte of u is 0: some code is -128
     }
+    zero &= V < 4 ? 0x80808080u >> (32 - 8 * (V < 4 ? V : 4)) : 0x80808080u;
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = __uint_as_float(__byte_perm(u[k / 4], 0x4b000000u, 0x7440 + (k & 3)));
+    rare |= byte > kHigh || zero != 0;
+    if (!rare) {
+      const float m = -8388736.f * s;
+      if constexpr (V == 1) f[0] = fmaf(f[0], s, m);
+#pragma unroll
+      for (int k = 0; k + 1 < V; k += 2) {
+        const float2 d = __ffma2_rn(make_float2(f[k], f[k + 1]), make_float2(s, s), make_float2(m, m));
+        f[k] = d.x;
+        f[k + 1] = d.y;
+      }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float q = f[k] - 8388736.f;
+      f[k] = q == -128.f ? __uint_as_float(0x7fc00000u) : q * s;
+    }
+  } else {
+    rare |= byte > Limits<T>::high_e4m3;
     if constexpr (V == 1) {
-      f[0] = (f[0] - 8388736.f) * s;
+      f[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(c.w[0] & 0xffu), __NV_E4M3))) * s;
     } else {
 #pragma unroll
       for (int k = 0; k < V; k += 2) {
-        const float2 d = __fmul2_rn(__fadd2_rn(make_float2(f[k], f[k + 1]), make_float2(-8388736.f, -8388736.f)),
-                                    make_float2(s, s));
+        const __nv_fp8x2_storage_t b = (__nv_fp8x2_storage_t)(c.w[k / 4] >> (8 * (k % 4)));
+        const float2 d = __fmul2_rn(__half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(b, __NV_E4M3))), make_float2(s, s));
         f[k] = d.x;
         f[k + 1] = d.y;
       }
     }
-    if (nan) {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (((c.w[k / 4] >> (8 * (k % 4))) & 0xffu) == 0x80u) f[k] = __uint_as_float(0x7fc00000u);
-    }
-  } else if constexpr (V == 1) {
-    f[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(c.w[0] & 0xffu), __NV_E4M3))) * s;
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; k += 2) {
-      const __nv_fp8x2_storage_t b = (__nv_fp8x2_storage_t)(c.w[k / 4] >> (8 * (k % 4)));
-      const float2 h = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(b, __NV_E4M3)));
-      const float2 d = __fmul2_rn(h, make_float2(s, s));
-      f[k] = d.x;
-      f[k + 1] = d.y;
-    }
+    if (!rare) return;
   }
-  const int high = format == R4C_Q8_INT8 ? Limits<T>::high_int8 : Limits<T>::high_e4m3;
-  if (byte > high || byte < Limits<T>::low) {
-    const float most = Limits<T>::most();
+  const float most = Limits<T>::most();
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      f[k] = f[k] > most ? most : (f[k] < -most ? -most : f[k]);
-      f[k] = Elem<T>::to_f(Elem<T>::from_f(f[k]));
-    }
+  for (int k = 0; k < V; ++k) {
+    f[k] = f[k] > most ? most : (f[k] < -most ? -most : f[k]);
+    f[k] = Elem<T>::to_f(Elem<T>::from_f(f[k]));
   }
 }
 
