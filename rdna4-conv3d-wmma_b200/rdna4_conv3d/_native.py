@@ -888,7 +888,7 @@ def gn_forward(x: torch.Tensor, plan: GnPlan, weight, bias, fmt: Optional[int]):
     return y, mean_rstd, codes, exps
 
 
-def gn_backward(dy: torch.Tensor, plan: GnPlan, x, fmt: int, exps, mean_rstd, weight, bias, need_dx: bool,
+def gn_backward(dy: torch.Tensor, plan: GnPlan, x, fmt: Optional[int], exps, mean_rstd, weight, bias, need_dx: bool,
                 need_params: bool):
     """(dx, dweight, dbias); fp32 parameter gradients; x the activation, or its codes with ``exps``."""
     dx = torch.empty_like(dy) if need_dx else None
@@ -898,7 +898,7 @@ def gn_backward(dy: torch.Tensor, plan: GnPlan, x, fmt: int, exps, mean_rstd, we
         db = torch.empty_like(dw)
     nb = plan.bwd_bytes
     ws = dy.new_empty(nb, dtype=torch.uint8)
-    _launch("r4c_gn_bwd", _lib.r4c_gn_bwd, dy.device, plan.desc, dy.data_ptr(), x.data_ptr(), fmt,
+    _launch("r4c_gn_bwd", _lib.r4c_gn_bwd, dy.device, plan.desc, dy.data_ptr(), x.data_ptr(), fmt or 0,
             None if exps is None else exps.data_ptr(), mean_rstd.data_ptr(),
             None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
             None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),

@@ -71,21 +71,25 @@ def _as_saved(t: torch.Tensor, count: int, dtype: torch.dtype, device: torch.dev
 
 
 class GroupNormActFn(torch.autograd.Function):
+    """``args``: (groups, eps, activation, slope, format or None)."""
+
     @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, activation, slope, fmt):
+    def forward(ctx, x, weight, bias, args):
+        groups, eps, activation, slope, fmt = args
         w, b, pdtype = _params(weight, bias)
-        args = x.shape, groups, x.dtype, pdtype, eps, activation, slope
-        y, mean_rstd, codes, exps = _native.gn_forward(x, _native.gn_plan(*args), w, b, fmt)
+        key = x.shape, groups, x.dtype, pdtype, eps, activation, slope
+        plan = _native.gn_plan(*key)
+        y, mean_rstd, codes, exps = _native.gn_forward(x, plan, w, b, fmt)
         ctx.save_for_backward(x if fmt is None else codes, exps, mean_rstd, weight, bias)
-        ctx.args, ctx.fmt, ctx.device = args, fmt, x.device
+        ctx.key, ctx.plan, ctx.fmt, ctx.device = key, plan, fmt, x.device
         return y
 
     @staticmethod
     def backward(ctx, gy):
         refuse_twice()
         x, exps, mean_rstd, weight, bias = ctx.saved_tensors
-        args, fmt, device = ctx.args, ctx.fmt, ctx.device
-        shape, dtype = args[0], args[2]
+        key, plan, fmt, device = ctx.key, ctx.plan, ctx.fmt, ctx.device
+        shape, dtype = key[0], key[2]
         if fmt is None:
             if x.shape != shape or x.dtype is not dtype or x.device != device:
                 _native._not_as_saved(x, shape, dtype, device)
@@ -94,19 +98,18 @@ class GroupNormActFn(torch.autograd.Function):
             count = shape.numel()
             x = _as_saved(x, count, torch.uint8, device)
             exps = _as_saved(exps, _native.q8_exponents(count, True), torch.uint8, device)
-        w, b, pdtype = _params(weight, bias)
-        for t in (w, b):
-            if t is not None and (t.shape[0] != shape[1] or t.device != device):
-                _native._not_as_saved(t, (shape[1],), pdtype, device)
-        if pdtype is not args[3]:
-            args = (*args[:3], pdtype, *args[4:])
-        plan = _native.gn_plan(*args)
         mean_rstd = _as_saved(mean_rstd, plan.stats, torch.float32, device)
+        w, b, pdtype = _params(weight, bias)
+        if w is not None and (w.shape != (shape[1],) or w.device != device):
+            _native._not_as_saved(w, (shape[1],), pdtype, device)
+        if b is not None and (b.shape != (shape[1],) or b.device != device):
+            _native._not_as_saved(b, (shape[1],), pdtype, device)
+        if pdtype is not key[3]:
+            plan = _native.gn_plan(*key[:3], pdtype, *key[4:])
         if gy.dtype is not dtype:
             gy = gy.to(dtype)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx, dw, db = _native.gn_backward(_channels_last(gy), plan, x, fmt or 0, exps, mean_rstd, w, b, need_x,
-                                         need_w or need_b)
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dx, dw, db = _native.gn_backward(_channels_last(gy), plan, x, fmt, exps, mean_rstd, w, b, need_x, need_w or need_b)
         if not need_w:
             dw = None
         elif weight.dtype is not torch.float32:
@@ -115,7 +118,7 @@ class GroupNormActFn(torch.autograd.Function):
             db = None
         elif bias.dtype is not torch.float32:
             db = db.to(bias.dtype)
-        return dx, dw, db, None, None, None, None, None
+        return dx, dw, db, None
 
 
 def _check(x, num_groups, weight, bias, eps, activation, negative_slope, checkpoint) -> None:
@@ -173,7 +176,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     needs = x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad
     if torch.is_grad_enabled() and needs or torch._C._is_tracing():
         fmt = None if checkpoint is None else _native.Q8_FORMATS[checkpoint]
-        return GroupNormActFn.apply(x, weight, bias, num_groups, eps, code, negative_slope, fmt)
+        return GroupNormActFn.apply(x, weight, bias, (num_groups, eps, code, negative_slope, fmt))
     w, b, pdtype = _params(weight, bias)
     return _native.gn_forward(x, _native.gn_plan(x.shape, num_groups, x.dtype, pdtype, eps, code, negative_slope), w, b,
                               None)[0]
