@@ -827,15 +827,10 @@ Q8_FORMATS = {"int8": 0, "e4m3": 1}
 ACTIVATIONS = {"none": 0, "relu": 1, "leaky_relu": 2, "silu": 3, "gelu": 4}
 
 
-def q8_exponents(count: int, words: bool = False) -> int:
-    """Exponents of count elements; ``words``: as whole words, which the group norm's backward reads."""
-    return (count + 127) // 128 * 4 if words else (count + Q8_BLOCK - 1) // Q8_BLOCK
-
-
-def q8_buffers(x: torch.Tensor, words: bool = False):
+def q8_buffers(x: torch.Tensor):
     """Empty codes and exponents for x's elements."""
     count = x.numel()
-    return x.new_empty(count, dtype=torch.uint8), x.new_empty(q8_exponents(count, words), dtype=torch.uint8)
+    return x.new_empty(count, dtype=torch.uint8), x.new_empty((count + Q8_BLOCK - 1) // Q8_BLOCK, dtype=torch.uint8)
 
 
 def pack8(x: torch.Tensor, fmt: int):
@@ -853,14 +848,26 @@ def unpack8(codes: torch.Tensor, exps: torch.Tensor, fmt: int, out: torch.Tensor
     return out
 
 
+def _up(n: int, unit: int) -> int:
+    return (n + unit - 1) // unit * unit
+
+
 class GnPlan:
-    """A descriptor with the workspace that each direction takes."""
-    __slots__ = ("desc", "fwd_bytes", "bwd_bytes", "stats")
+    """A descriptor with the sizes of what goes with it: ``stats`` floats that the forward writes for the backward, in
+    one allocation with the forward's own workspace (``kept`` floats in all); of the 8 bits the codes' end and the
+    whole (``q8_at``, ``q8_bytes``); the backward's workspace."""
+    __slots__ = ("desc", "stats", "kept", "ws_at", "fwd_bytes", "bwd_bytes", "q8_at", "q8_bytes")
 
     def __init__(self, desc: GnDesc):
         L = lib()
+        count = desc.samples * desc.inner * desc.channels
         self.desc, self.stats = desc, 2 * desc.samples * desc.groups
         self.fwd_bytes, self.bwd_bytes = L.r4c_gn_workspace_size(desc, 0), L.r4c_gn_workspace_size(desc, 1)
+        self.ws_at = _up(4 * self.stats, 256)
+        self.kept = (self.ws_at + self.fwd_bytes) // 4 if self.fwd_bytes else self.stats
+        self.q8_at = _up(count, 256)
+        # (the backward reads exponents in words)
+        self.q8_bytes = self.q8_at + _up((count + Q8_BLOCK - 1) // Q8_BLOCK, 4)
 
 
 @functools.lru_cache(maxsize=512)
@@ -872,34 +879,33 @@ def gn_plan(shape: torch.Size, groups: int, dtype: torch.dtype, params_dtype: to
 
 
 def gn_forward(x: torch.Tensor, plan: GnPlan, weight, bias, fmt: Optional[int]):
-    """(y, mean_rstd, codes or None, exponents or None) of a channels-last dense x."""
+    """(y, stats, x's 8 bits or None) of a channels-last dense x. Few allocations: each is some microseconds of a call."""
     y = torch.empty_like(x)
-    mean_rstd = x.new_empty((plan.stats,), dtype=torch.float32)
-    codes = exps = ws = None
+    stats = x.new_empty(plan.kept, dtype=torch.float32)
+    q8, codes, exps = None, None, None
     if fmt is not None:
-        codes, exps = q8_buffers(x, True)
-    nb = plan.fwd_bytes
-    if nb:
-        ws = x.new_empty(nb, dtype=torch.uint8)
+        q8 = x.new_empty(plan.q8_bytes, dtype=torch.uint8)
+        codes = q8.data_ptr()
+        exps = codes + plan.q8_at
+    nb, at = plan.fwd_bytes, stats.data_ptr()
     _launch("r4c_gn_fwd", _lib.r4c_gn_fwd, x.device, plan.desc, x.data_ptr(), None if weight is None else weight.data_ptr(),
-            None if bias is None else bias.data_ptr(), y.data_ptr(), mean_rstd.data_ptr(), fmt or 0,
-            None if codes is None else codes.data_ptr(), None if codes is None else exps.data_ptr(),
-            None if ws is None else ws.data_ptr(), nb)
-    return y, mean_rstd, codes, exps
+            None if bias is None else bias.data_ptr(), y.data_ptr(), at, fmt or 0, codes, exps,
+            at + plan.ws_at if nb else None, nb)
+    return y, stats, q8
 
 
-def gn_backward(dy: torch.Tensor, plan: GnPlan, x, fmt: Optional[int], exps, mean_rstd, weight, bias, need_dx: bool,
+def gn_backward(dy: torch.Tensor, plan: GnPlan, x, fmt: Optional[int], stats, weight, bias, need_dx: bool,
                 need_params: bool):
-    """(dx, dweight, dbias); fp32 parameter gradients; x the activation, or its codes with ``exps``."""
+    """(dx, dweight, dbias); fp32 parameter gradients; x the activation, or with ``fmt`` its 8 bits."""
     dx = torch.empty_like(dy) if need_dx else None
     dw = db = None
     if need_params:
         dw = dy.new_empty((plan.desc.channels,), dtype=torch.float32)
         db = torch.empty_like(dw)
-    nb = plan.bwd_bytes
+    nb, at = plan.bwd_bytes, x.data_ptr()
     ws = dy.new_empty(nb, dtype=torch.uint8)
-    _launch("r4c_gn_bwd", _lib.r4c_gn_bwd, dy.device, plan.desc, dy.data_ptr(), x.data_ptr(), fmt or 0,
-            None if exps is None else exps.data_ptr(), mean_rstd.data_ptr(),
+    _launch("r4c_gn_bwd", _lib.r4c_gn_bwd, dy.device, plan.desc, dy.data_ptr(), at, fmt or 0,
+            None if fmt is None else at + plan.q8_at, stats.data_ptr(),
             None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
             None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
             None if db is None else db.data_ptr(), ws.data_ptr(), nb)

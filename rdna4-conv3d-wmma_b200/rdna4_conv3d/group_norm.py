@@ -79,15 +79,15 @@ class GroupNormActFn(torch.autograd.Function):
         w, b, pdtype = _params(weight, bias)
         key = x.shape, groups, x.dtype, pdtype, eps, activation, slope
         plan = _native.gn_plan(*key)
-        y, mean_rstd, codes, exps = _native.gn_forward(x, plan, w, b, fmt)
-        ctx.save_for_backward(x if fmt is None else codes, exps, mean_rstd, weight, bias)
+        y, stats, q8 = _native.gn_forward(x, plan, w, b, fmt)
+        ctx.save_for_backward(x if fmt is None else q8, stats, weight, bias)
         ctx.key, ctx.plan, ctx.fmt, ctx.device = key, plan, fmt, x.device
         return y
 
     @staticmethod
     def backward(ctx, gy):
         refuse_twice()
-        x, exps, mean_rstd, weight, bias = ctx.saved_tensors
+        x, stats, weight, bias = ctx.saved_tensors
         key, plan, fmt, device = ctx.key, ctx.plan, ctx.fmt, ctx.device
         shape, dtype = key[0], key[2]
         if fmt is None:
@@ -95,10 +95,8 @@ class GroupNormActFn(torch.autograd.Function):
                 _native._not_as_saved(x, shape, dtype, device)
             x = _channels_last(x)
         else:
-            count = shape.numel()
-            x = _as_saved(x, count, torch.uint8, device)
-            exps = _as_saved(exps, _native.q8_exponents(count, True), torch.uint8, device)
-        mean_rstd = _as_saved(mean_rstd, plan.stats, torch.float32, device)
+            x = _as_saved(x, plan.q8_bytes, torch.uint8, device)
+        stats = _as_saved(stats, plan.kept, torch.float32, device)
         w, b, pdtype = _params(weight, bias)
         if w is not None and (w.shape != (shape[1],) or w.device != device):
             _native._not_as_saved(w, (shape[1],), pdtype, device)
@@ -109,7 +107,7 @@ class GroupNormActFn(torch.autograd.Function):
         if gy.dtype is not dtype:
             gy = gy.to(dtype)
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dx, dw, db = _native.gn_backward(_channels_last(gy), plan, x, fmt, exps, mean_rstd, w, b, need_x, need_w or need_b)
+        dx, dw, db = _native.gn_backward(_channels_last(gy), plan, x, fmt, stats, w, b, need_x, need_w or need_b)
         if not need_w:
             dw = None
         elif weight.dtype is not torch.float32:
