@@ -74,6 +74,12 @@ def pack8(x: torch.Tensor, format: str = "int8") -> Packed8:
     if dtype not in _FLOATS:
         raise TypeError(f"pack8 takes bf16, fp16 or fp32, got {dtype}")
     refuse_blind(x)
+    _refuse_trace(x)
+    return _pack8(x, format, code)
+
+
+def _pack8(x: torch.Tensor, format: str, code: int) -> Packed8:
+    dtype = x.dtype
     if not _is_dense(x):
         x = x.detach().contiguous()
     if not x.is_cuda:
@@ -83,6 +89,12 @@ def pack8(x: torch.Tensor, format: str = "int8") -> Packed8:
     return Packed8(codes, exps, x.shape, x.stride(), dtype, format)
 
 
+def _refuse_trace(t: torch.Tensor) -> None:
+    """torch.jit.trace would record the empty tensors that bare launches fill."""
+    if t.is_cuda and torch._C._is_tracing():
+        raise RuntimeError("pack8 and unpack8 cannot be traced by torch.jit.trace on a CUDA device")
+
+
 def unpack8(packed: Packed8) -> torch.Tensor:
     """The values that the 8 bits hold, in the packed tensor's type, shape and strides: code * 2^e, at most the
     type's largest finite number."""
@@ -90,6 +102,7 @@ def unpack8(packed: Packed8) -> torch.Tensor:
     code = _native.Q8_FORMATS.get(fmt)
     if code is None:
         check_format(fmt)
+    _refuse_trace(codes)
     count = shape.numel()
     if codes.numel() != count or exps.numel() != (count + 31) // _native.Q8_BLOCK:
         raise ValueError(f"{count} elements need as many codes and {-(-count // _native.Q8_BLOCK)} exponents, got "

@@ -403,9 +403,9 @@ class Conv3dKept8Fn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, stride, padding, dilation, fmt):
-        from .checkpoint8 import pack8
+        from .checkpoint8 import _pack8
         y = Conv3dWmmaFn.forward(x, weight, bias, stride, padding, dilation)
-        packed = pack8(x, fmt) if ctx.needs_input_grad[1] else (None, None)
+        packed = _pack8(x, fmt, _native.Q8_FORMATS[fmt]) if ctx.needs_input_grad[1] else (None, None)
         ctx.save_for_backward(packed[0], packed[1], weight)
         ctx.packed = packed[2:]
         ctx.was = x.shape, x.dtype

@@ -585,3 +585,43 @@ def test_inference_and_frozen_parts(cuda_ready):
     assert torch.equal(y, m(x.detach()))
     y.backward(dy)
     assert x.grad is not None and m.weight.grad is None
+
+
+@pytest.mark.parametrize("wants_grad", [False, True])
+@pytest.mark.parametrize("fmt", [None, "int8"])
+@pytest.mark.parametrize("shape", [(2, 24, 5, 6, 7), (2, 24, 32, 64, 64)])
+def test_traces_run_the_operator_again(cuda_ready, shape, fmt, wants_grad):
+    """A trace computes from the inputs that it is given, or there is none."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, b, _ = _inputs(shape, BF)
+    more = _inputs(shape, BF, seed=8)[0]
+    x, more = (t.detach().requires_grad_(wants_grad) for t in (x, more))
+    w, b = (t.detach().requires_grad_(wants_grad) for t in (w, b))
+    # (parameters as inputs: torch.jit.trace takes no constants that require gradients)
+    f = lambda t, w, b: group_norm_act(t, 8, w, b, activation="silu", checkpoint=fmt) * 2  # noqa: E731
+    want = f(more, w, b)
+    assert torch.equal(torch.jit.trace(f, (x, w, b), check_trace=False)(more, w, b), want)
+    torch._dynamo.reset()
+    assert torch.equal(torch.compile(f, backend="eager")(more, w, b), want)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(f)(x, w, b)
+
+
+def test_packing_is_not_traced(cuda_ready):
+    x = torch.randn(1000, device="cuda")
+    p = pack8(x)
+    for f in (lambda t: pack8(t).codes, lambda t: unpack8(p._replace(codes=t.to(torch.uint8)[:1000])) * 1):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, (x,), check_trace=False)
+    torch._dynamo.reset()
+    f = lambda t: unpack8(pack8(t * 2, "e4m3")) + 1  # noqa: E731
+    assert torch.equal(torch.compile(f, backend="eager")(x), f(x))
+
+
+def test_kept_convs_in_traces(cuda_ready):
+    from rdna4_conv3d import conv3d_wmma
+    x, more = (torch.randn(1, 8, 4, 8, 8, device="cuda", dtype=BF, generator=_gen(s)).contiguous(memory_format=CL) for s in (1, 2))
+    w = torch.randn(8, 8, 3, 3, 3, device="cuda", generator=_gen(3), requires_grad=True)
+    f = lambda t, w: conv3d_wmma(t, w, None, 1, 1, checkpoint="int8") * 2  # noqa: E731
+    want = f(more, w)
+    assert torch.equal(torch.jit.trace(f, (x, w), check_trace=False)(more, w), want)
