@@ -110,11 +110,12 @@ bool make_plan(const r4c_gn_desc* d, bool backward, Plan* pl) {
   g.R = std::max(1, kThreads / g.lanes);
   if (g.R > 4) g.R = g.R / 4 * 4;       // a tile of rows starts at a block of 32 elements (fused packing)
   pl->threads = cdiv(g.R * g.lanes, 32) * 32;
-  // one wave of blocks, none with less than four rows for each thread; the sums' wave leaves room for blocks of the
-  // second pass, which start under it
-  const Geo sums = split(g, blocks_for(g, d->samples, backward ? kBwdSumsFit : kStatsFit));
+  // one wave of blocks, none with less than four rows for each thread
+  const double each_sm = (double)d->samples * g.tiles * (double)((g.rows + g.R - 1) / g.R) / 148.0;
+  const int sums_fit = each_sm < kShortSums ? 1 : backward ? kBwdSumsFit : kStatsFit;
+  const Geo sums = split(g, blocks_for(g, d->samples, sums_fit));
   pl->sums_nb = sums.nb;
-  g = split(g, blocks_for(g, d->samples, backward ? kBwdBlocks : kApplyBlocks));
+  g = split(g, blocks_for(g, d->samples, backward ? kBwdFit : kApplyFit));
   g.np = sums.nb * g.tiles;
   const int64_t most = std::max(g.blocks, sums.blocks);
   return most + g.C <= INT32_MAX && g.tiles <= 65535 && g.rows / g.R < INT32_MAX;

@@ -34,9 +34,13 @@ namespace gn {
 constexpr int kThreads = 256;   // at most, per block
 // Blocks that fit an SM beside each other (the registers that each kernel may take follow from it).
 constexpr int kStatsBlocks = 4, kApplyBlocks = 4, kBwdBlocks = 3;
-// Blocks an SM that the sums run in: with two of them, blocks of the second pass fit beside them and have started when
-// the sums end (forward of [4,48,32,64,64] 26.7 -> 24.1 us, [2,30,37,41,53] 18.8 -> 16.4, [4,24,64,128,128] the same).
-constexpr int kStatsFit = 2, kBwdSumsFit = 3;
+// Blocks an SM that each pass runs in. The forward's two and two fit beside each other, so the second pass has started
+// when the sums end; short sums take one block an SM (fewer parts to join). Measured, sums 4 + y 4 / 2 + 4 / 2 + 2 / 1 + 2
+// (us): [4,24,64,128,128] - / 104 / 101 / 110, [4,48,32,64,64] 26.7 / 24.0 / 23.2 / 24.3, [2,32,33,47,50] fp32 17.1 /
+// 15.2 / 14.6 / 13.9, [2,30,37,41,53] 18.8 / 15.9 / 16.3 / 14.9. Backward, sums 3 / 2 / 1 with dx 3: [4,24,64,128,128] 170
+// / 173 / 198, [4,48,32,64,64] 40 / 42 / 47, [2,32,33,47,50] 23.8 / 23.1 / 22.8, [3,40,21,35,45] kept 16.7 / 15.2 / 14.3.
+constexpr int kStatsFit = 2, kApplyFit = 2, kBwdSumsFit = 3, kBwdFit = 3;
+constexpr int64_t kShortSums = 48;   // tiles of rows an SM, below which sums are short
 // Vectors of a thread on their way at a time, plus one.
 constexpr int kFwdAhead = 8, kBwdAhead = 4;
 // Samples that a cluster keeps on chip: vectors of a thread at most (forward; backward, which keeps dy too), groups of

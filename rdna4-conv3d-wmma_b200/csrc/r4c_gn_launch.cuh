@@ -75,6 +75,17 @@ cudaError_t bwd_small(const BwdArgs& a, const Geo& g, int threads, cudaStream_t 
                         static_cast<T*>(a.dx));
 }
 
+// Both passes with the SM's memory divided alike (all of it shared): blocks of the second may start beside the first's.
+template <typename K>
+void all_shared(K kernel, std::atomic<uint64_t>& devices) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return;
+  const uint64_t bit = 1ull << dev;
+  if (devices.load(std::memory_order_relaxed) & bit) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) == cudaSuccess)
+    devices.fetch_or(bit, std::memory_order_relaxed);
+}
+
 template <typename T, int V, int ACT>
 cudaError_t fwd_v(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   const dim3 grid((unsigned)g.blocks, g.tiles);
@@ -86,12 +97,15 @@ cudaError_t fwd_v(const FwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   }
   const size_t smem = Ring<T, V, false, false, kFwdAhead>::kBytes + sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
   const Geo sums = split(g, a.sums_nb);
+  static std::atomic<uint64_t> shared_s{0}, shared_a[2] = {{0}, {0}};
+  all_shared(stats_kernel<T, V>, shared_s);
   stats_kernel<T, V><<<dim3((unsigned)sums.blocks, g.tiles), threads, 0, s>>>(x, sums, a.part);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   auto apply = apply_kernel<T, V, ACT, false>;
   if constexpr (V * sizeof(T) == 16 && ACT >= 0)             // (samples with edges are packed on their own)
     if (g.pack) apply = apply_kernel<T, V, ACT, true>;
+  all_shared(apply, shared_a[g.pack != 0]);
   e = launch_next(apply, grid, threads, smem, s, x, a.gamma, a.beta, g, a.part, a.mean_rstd, static_cast<T*>(a.y),
                   a.codes, a.exps);
   note_launches(2);
@@ -114,6 +128,9 @@ cudaError_t bwd_v(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
     return e != cudaSuccess || !params ? e : params_next();
   }
   const size_t smem = Ring<T, V, Q, true, kBwdAhead>::kBytes + sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
+  static std::atomic<uint64_t> shared_s{0}, shared_d{0};
+  all_shared(bwd_sums_kernel<T, V, ACT, Q>, shared_s);
+  all_shared(bwd_dx_kernel<T, V, ACT, Q>, shared_d);
   bwd_sums_kernel<T, V, ACT, Q><<<dim3((unsigned)sums.blocks, g.tiles), threads, 0, s>>>(
       dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, sums, a.cpart, a.gpart);
   note_launches(1);
