@@ -38,6 +38,7 @@ void plan_small(const r4c_gn_desc* d, bool backward, int V, Geo& g, int* threads
     const bool ok = whole || (g.L == g.C && width % V == 0 && width * elem >= 48);
     if (ok && width / V <= kThreads && k <= kSmallGroups) {
       const int lanes = (int)(width / V), tiles = whole ? 1 : cdiv(g.G, k);
+      if (tiles > 65535) break;
       for (int cl = 1; cl <= 8; cl *= 2) {
         const int64_t per = std::max<int64_t>(1, (g.rows + cl - 1) / cl);
         int R = (int)std::min<int64_t>(std::max(1, kThreads / lanes), per);
@@ -145,7 +146,11 @@ int wide_params(const Geo& g, const void* gamma, const void* beta) {
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-int status(cudaError_t e) { return e == cudaSuccess ? R4C_OK : R4C_ERR_CUDA; }
+int status(cudaError_t e) {
+  if (e == cudaSuccess) return R4C_OK;
+  (void)cudaGetLastError();             // a failed launch leaves no error behind for the next call
+  return R4C_ERR_CUDA;
+}
 
 }  // namespace
 }  // namespace gn

@@ -84,6 +84,8 @@ void all_shared(K kernel, std::atomic<uint64_t>& devices) {
   if (devices.load(std::memory_order_relaxed) & bit) return;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) == cudaSuccess)
     devices.fetch_or(bit, std::memory_order_relaxed);
+  else
+    (void)cudaGetLastError();           // (a preference)
 }
 
 template <typename T, int V, int ACT>
