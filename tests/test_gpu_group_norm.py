@@ -625,3 +625,30 @@ def test_kept_convs_in_traces(cuda_ready):
     f = lambda t, w: conv3d_wmma(t, w, None, 1, 1, checkpoint="int8") * 2  # noqa: E731
     want = f(more, w)
     assert torch.equal(torch.jit.trace(f, (x, w), check_trace=False)(more, w), want)
+
+
+@pytest.mark.parametrize("fmt", [None, "int8"])
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("act", ACTIVATIONS)
+def test_steep(cuda_ready, act, dtype, fmt):
+    """Weights of some hundred, either sign: the activations' flat ends, exponentials out of range."""
+    for shape in ((2, 24, 9, 10, 11), (2, 24, 32, 48, 48)):
+        x, w, b, dy = _inputs(shape, dtype)
+        with torch.no_grad():
+            w.mul_(torch.linspace(-400, 400, 24, device="cuda"))
+            b.mul_(200)
+        got = _verify(x, 8, w, b, dy, act, fmt)
+        assert all(bool(v.isfinite().all()) for v in got.values())
+
+
+@pytest.mark.parametrize("fmt", [None, "e4m3"])
+@pytest.mark.parametrize("shape", [(3, 24), (2, 24, 50), (2, 24, 9, 11), (2, 24, 3, 4, 5, 6), (2, 1, 7, 8, 9)])
+def test_dimensions(cuda_ready, shape, fmt):
+    """Tokens, sequences, images, volumes and more, channels last or first."""
+    groups = 4 if shape[1] > 1 else 1
+    args = _args(shape, groups, HF)
+    want = _verify(*args, act="gelu", fmt=fmt)
+    x, _, w, b, dy = args
+    first = x.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True)
+    for k, v in _run(first, groups, w, b, dy.contiguous(), "gelu", fmt).items():
+        assert torch.equal(v, want[k]), k
