@@ -9,8 +9,8 @@
 //   dx = rstd * (dz * w - A - xh * B)
 // Two passes over the data each way: sums, then the element-wise result (the statistics of a group need all of it).
 // Both are bound by memory: forward 3, backward 5 activations read or written. Samples that fit the shared memory
-// of a cluster take one. [4,24,64,128,128] bf16 with silu (201 MB): forward 37 + 66 us (5.9 TB/s), backward 72 + 98 us
-// (5.9 TB/s); with x in 8 bits 37 + 96 and 82 + 90 us, where instructions (150 to 190 a warp and vector) are the bound.
+// of a cluster take one. [4,24,64,128,128] bf16 with silu (201 MB): forward 107 us (5.6 TB/s), backward 171 us (5.9
+// TB/s), with relu 100 us forward (6.1 TB/s); with x in 8 bits too 133 and 174 us, where instructions (150 to 190 a warp and vector) are the bound.
 //
 // A thread owns a vector of V neighbouring elements in every R-th row of its block's range, so its channels and with
 // them the parameters stay in registers. A row is a voxel's channels, or L / C voxels together where C is no multiple
