@@ -292,14 +292,14 @@ class GroupNormAct3d(nn.GroupNorm):
 
 
 def _activation_of(m: nn.Module):
-    """(name, slope) of an activation module that the kernels have, else None."""
-    if isinstance(m, nn.ReLU):
+    """(name, slope) of an activation module that the kernels have, else None (a subclass may have its own forward)."""
+    if type(m) is nn.ReLU:
         return "relu", 0.0
-    if isinstance(m, nn.LeakyReLU):
+    if type(m) is nn.LeakyReLU:
         return "leaky_relu", m.negative_slope
-    if isinstance(m, nn.SiLU):
+    if type(m) is nn.SiLU:
         return "silu", 0.0
-    if isinstance(m, nn.GELU) and m.approximate == "none":
+    if type(m) is nn.GELU and m.approximate == "none":
         return "gelu", 0.0
     return None
 
