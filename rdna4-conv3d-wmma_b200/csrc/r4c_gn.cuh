@@ -538,6 +538,38 @@ __device__ __forceinline__ int row_threads(int tp, int rows) {
 // Launched while the kernel before it may still run: what that one wrote may be read from here on.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// What the kernel before this one wrote, while this one may already have run: the pointers are not __restrict__ (which
+// would promise that nothing changes it) and the loads are volatile, so that none goes ahead of the wait, which makes all
+// that was written visible. (Loads past the L1, ld.relaxed.gpu, take the parameters' sums 4 us longer at [4,48,32,64,64]:
+// neighbouring channels share sectors.)
+__device__ __forceinline__ double2 from_previous(const double2* p) {
+  double2 v;
+  asm volatile("ld.global.v2.f64 {%0, %1}, [%2];" : "=d"(v.x), "=d"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 from_previous(const float2* p) {
+  float2 v;
+  asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+  return v;
+}
+// Adds p[i * stride] for i = first, first + step, .. below end, in that order, U loads on their way at a time.
+template <int U, typename P>
+__device__ __forceinline__ void add_previous(const P* p, int64_t first, int64_t step, int64_t end, int64_t stride, double& a,
+                                             double& c) {
+  for (int64_t i = first; i < end; i += U * step) {
+    P v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u].x = v[u].y = 0;
+      if (i + u * step < end) v[u] = from_previous(p + (i + u * step) * stride);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      a += v[u].x;
+      c += v[u].y;
+    }
+  }
+}
 
 // The thread's parameters: z = (x - mean) * a + b with a = rstd * w. For 16-bit x the mean goes into b (z = x * a + b'):
 // its rounding is 2^-24 of |mean| a, where x's own step is 2^-8 or 2^-11 of |x|; likewise sum dz * x and the sums'
@@ -793,7 +825,7 @@ __device__ __forceinline__ void apply_edges(const Geo& g, const Place& p, const 
 template <typename T, int V, int ACT, bool PACK>
 __global__ void __launch_bounds__(kThreads, kApplyBlocks) apply_kernel(
     const T* __restrict__ x, const void* __restrict__ gamma, const void* __restrict__ beta,
-    const __grid_constant__ Geo g, const double2* __restrict__ part, float2* __restrict__ mean_rstd,
+    const __grid_constant__ Geo g, const double2* part, float2* __restrict__ mean_rstd,
     T* __restrict__ y, uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
   using R = Ring<T, V, false, false, kFwdAhead>;
   extern __shared__ __align__(16) char smem[];
@@ -811,12 +843,7 @@ __global__ void __launch_bounds__(kThreads, kApplyBlocks) apply_kernel(
   wait_for_previous();
   const double2* src = part + p.n * g.np * g.G + p.ga;
   each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
-#pragma unroll 4
-    for (int e = sub; e < g.np; e += tp) {
-      const double2 v = src[(int64_t)e * g.G + i];
-      a += v.x;
-      c += v.y;
-    }
+    add_previous<4>(src + i, sub, tp, g.np, g.G, a, c);
   }, [&](int i, double a, double c) { stat[i] = mean_rstd_of(g, a, c); });
   __syncthreads();
   if (p.b == 0)
@@ -979,23 +1006,18 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_sums_kernel(
 // ---------------------------------------------------------------------------
 // dw, db: a warp, or a block, sums a channel over the (sample, block) parts, in a fixed order.
 constexpr int64_t kWideParts = 2048;      // from here on a block a channel (70,000 parts of 16 channels: 160 -> 21 us)
-__device__ __forceinline__ void param_grads(const float2* __restrict__ cpart, int64_t parts, int C, int c,
+__device__ __forceinline__ void param_grads(const float2* cpart, int64_t parts, int C, int c,
                                             float* __restrict__ dgamma, float* __restrict__ dbeta) {
   const int lane = threadIdx.x & 31;
   double u = 0.0, v = 0.0;
-#pragma unroll 8
-  for (int64_t i = lane; i < parts; i += 32) {
-    const float2 e = cpart[i * C + c];
-    u += e.x;
-    v += e.y;
-  }
+  add_previous<8>(cpart + c, lane, 32, parts, C, u, v);
   join(u, v, 32);
   if (lane == 0) {
     if (dbeta) dbeta[c] = (float)u;
     if (dgamma) dgamma[c] = (float)v;
   }
 }
-inline __global__ void __launch_bounds__(kThreads) params_kernel(const float2* __restrict__ cpart, int64_t parts, int C,
+inline __global__ void __launch_bounds__(kThreads) params_kernel(const float2* cpart, int64_t parts, int C,
                                                                  float* __restrict__ dgamma, float* __restrict__ dbeta) {
   __shared__ double2 warps[kThreads / 32];
   wait_for_previous();
@@ -1006,12 +1028,7 @@ inline __global__ void __launch_bounds__(kThreads) params_kernel(const float2* _
   }
   const int c = blockIdx.x;
   double u = 0.0, v = 0.0;
-#pragma unroll 8
-  for (int64_t i = threadIdx.x; i < parts; i += kThreads) {
-    const float2 e = cpart[i * C + c];
-    u += e.x;
-    v += e.y;
-  }
+  add_previous<8>(cpart + c, threadIdx.x, kThreads, parts, C, u, v);
   join(u, v, 32);
   if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = make_double2(u, v);
   __syncthreads();
@@ -1077,7 +1094,7 @@ template <typename T, int V, int ACT, bool Q>
 __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
     const T* __restrict__ dy, const void* __restrict__ x, const uint8_t* __restrict__ exps,
     const float2* __restrict__ mean_rstd, const void* __restrict__ gamma, const void* __restrict__ beta,
-    const __grid_constant__ Geo g, int64_t parts, const float2* __restrict__ cpart, const float2* __restrict__ gpart,
+    const __grid_constant__ Geo g, int64_t parts, const float2* cpart, const float2* gpart,
     T* __restrict__ dx, float* __restrict__ dgamma, float* __restrict__ dbeta) {
   using R = Ring<T, V, Q, true, kBwdAhead>;
   extern __shared__ __align__(16) char smem[];
@@ -1104,12 +1121,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
   wait_for_previous();
   const float2* src = gpart + p.n * g.np * g.G + p.ga;
   each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
-#pragma unroll 4
-    for (int e = sub; e < g.np; e += tp) {
-      const float2 v = src[(int64_t)e * g.G + i];
-      a += v.x;
-      c += v.y;
-    }
+    add_previous<4>(src + i, sub, tp, g.np, g.G, a, c);
   }, [&](int i, double a, double c) { coef[i] = coef_of<T>(g, stats[p.ga + i], a, c); });
   __syncthreads();
   if (p.mine > 0) {
