@@ -306,8 +306,8 @@ def _activation_of(m: nn.Module):
 
 def fuse_group_norm(model: nn.Module) -> int:
     """Replace each (GroupNorm, ReLU / LeakyReLU / SiLU / GELU) pair inside an
-    nn.Sequential with (GroupNormAct3d, Identity), copying the GroupNorm's
-    state. Returns the number of pairs fused."""
+    nn.Sequential with (GroupNormAct3d, Identity). The parameters are the
+    GroupNorm's own, not copies. Returns the number of pairs fused."""
     count = 0
     for child in model.children():
         count += fuse_group_norm(child)
@@ -316,13 +316,10 @@ def fuse_group_norm(model: nn.Module) -> int:
         for a, b in zip(names, names[1:]):
             norm, act = model._modules[a], _activation_of(model._modules[b])
             if type(norm) is nn.GroupNorm and act is not None:
-                ref = norm.weight
                 new = GroupNormAct3d(norm.num_groups, norm.num_channels, norm.eps, norm.affine, act[0], act[1],
-                                     device=None if ref is None else ref.device,
-                                     dtype=None if ref is None else ref.dtype)
-                new.load_state_dict(norm.state_dict())
-                new.train(norm.training)
-                model._modules[a] = new
+                                     device="meta")
+                new.weight, new.bias = norm.weight, norm.bias
+                model._modules[a] = new.train(norm.training)
                 model._modules[b] = nn.Identity()
                 count += 1
     return count

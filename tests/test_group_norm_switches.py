@@ -34,3 +34,35 @@ def test_activations_of_another_class_stay(act):
     want = seq(_x())
     assert fuse_group_norm(seq) == 0 and type(seq[0]) is nn.GroupNorm and seq[1] is act
     assert torch.equal(seq(_x()), want)
+
+
+def test_parameters_are_the_models_own():
+    """Frozen ones stay frozen, an optimizer's stay its own, tied ones stay tied."""
+    seq = nn.Sequential(nn.GroupNorm(2, 8), nn.ReLU(), nn.GroupNorm(2, 8), nn.SiLU())
+    seq[2].weight = seq[0].weight
+    seq[0].requires_grad_(False)
+    before = dict(seq.named_parameters(remove_duplicate=False))
+    assert fuse_group_norm(seq) == 2
+    after = dict(seq.named_parameters(remove_duplicate=False))
+    assert list(after) == list(before) and all(after[k] is before[k] for k in before)
+    assert not seq[0].weight.requires_grad and not seq[2].weight.requires_grad and seq[2].bias.requires_grad
+
+
+def test_a_norm_used_twice_stays_one():
+    norm = nn.GroupNorm(2, 8)
+    seq = nn.Sequential(norm, nn.ReLU(), nn.Sequential(norm, nn.SiLU()), norm)
+    want = seq(_x())
+    assert fuse_group_norm(seq) == 2
+    torch.testing.assert_close(seq(_x()), want, rtol=1e-4, atol=1e-4)
+    assert len(list(seq.parameters())) == 2 and seq[0].weight is seq[2][0].weight is norm.weight
+
+
+def test_without_parameters_and_without_a_bias():
+    plain, biased = nn.GroupNorm(2, 8, affine=False), nn.GroupNorm(2, 8)
+    biased.bias = None
+    nn.init.normal_(biased.weight)
+    seq = nn.Sequential(plain, nn.ReLU(), biased, nn.LeakyReLU(0.1))
+    want = seq(_x())
+    keys = list(seq.state_dict())
+    assert fuse_group_norm(seq) == 2 and list(seq.state_dict()) == keys
+    torch.testing.assert_close(seq(_x()), want, rtol=1e-4, atol=1e-4)
