@@ -304,10 +304,15 @@ def _activation_of(m: nn.Module):
     return None
 
 
+def _has_hooks(m: nn.Module) -> bool:
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
 def fuse_group_norm(model: nn.Module) -> int:
     """Replace each (GroupNorm, ReLU / LeakyReLU / SiLU / GELU) pair inside an
     nn.Sequential with (GroupNormAct3d, Identity). The parameters are the
-    GroupNorm's own, not copies. Returns the number of pairs fused."""
+    GroupNorm's own, not copies. Pairs with hooks on either module stay as they
+    are (what the hooks see would be gone). Returns the number of pairs fused."""
     count = 0
     for child in model.children():
         count += fuse_group_norm(child)
@@ -315,7 +320,7 @@ def fuse_group_norm(model: nn.Module) -> int:
         names = list(model._modules.keys())
         for a, b in zip(names, names[1:]):
             norm, act = model._modules[a], _activation_of(model._modules[b])
-            if type(norm) is nn.GroupNorm and act is not None:
+            if type(norm) is nn.GroupNorm and act is not None and not (_has_hooks(norm) or _has_hooks(model._modules[b])):
                 new = GroupNormAct3d(norm.num_groups, norm.num_channels, norm.eps, norm.affine, act[0], act[1],
                                      device="meta")
                 new.weight, new.bias = norm.weight, norm.bias

@@ -66,3 +66,21 @@ def test_without_parameters_and_without_a_bias():
     keys = list(seq.state_dict())
     assert fuse_group_norm(seq) == 2 and list(seq.state_dict()) == keys
     torch.testing.assert_close(seq(_x()), want, rtol=1e-4, atol=1e-4)
+
+
+HOOKS = {"forward": lambda m, seen: m.register_forward_hook(lambda *a: seen.append(1)),
+         "forward_pre": lambda m, seen: m.register_forward_pre_hook(lambda *a: seen.append(1)),
+         "backward": lambda m, seen: m.register_full_backward_hook(lambda *a: seen.append(1)),
+         "backward_pre": lambda m, seen: m.register_full_backward_pre_hook(lambda *a: seen.append(1))}
+
+
+@pytest.mark.parametrize("kind", sorted(HOOKS))
+@pytest.mark.parametrize("which", [0, 1])
+def test_modules_with_hooks_stay(kind, which):
+    """A hook sees the norm's output before the activation, which a fused pair does not have."""
+    seq = nn.Sequential(nn.GroupNorm(2, 8), nn.SiLU(), nn.GroupNorm(2, 8), nn.SiLU())
+    seen = []
+    HOOKS[kind](seq[which], seen)
+    assert fuse_group_norm(seq) == 1 and type(seq[0]) is nn.GroupNorm and isinstance(seq[2], GroupNormAct3d)
+    seq(_x().requires_grad_(True)).sum().backward()
+    assert seen == [1]
