@@ -186,7 +186,7 @@ def fuse_bn_relu(model: nn.Module) -> int:
         names = list(model._modules.keys())
         for a, b in zip(names, names[1:]):
             bn, act = model._modules[a], model._modules[b]
-            if type(bn) is nn.BatchNorm3d and isinstance(act, nn.ReLU):
+            if type(bn) is nn.BatchNorm3d and type(act) is nn.ReLU:
                 ref = bn.weight if bn.affine else bn.running_mean
                 new = BatchNormReLU3d(bn.num_features, bn.eps, bn.momentum, bn.affine, bn.track_running_stats,
                                       device=None if ref is None else ref.device,
