@@ -177,8 +177,8 @@ class BatchNormReLU3d(nn.BatchNorm3d):
 
 def fuse_bn_relu(model: nn.Module) -> int:
     """Replace each (BatchNorm3d, ReLU) pair inside an nn.Sequential with
-    (BatchNormReLU3d, Identity), copying the BatchNorm's state. Returns the
-    number of pairs fused."""
+    (BatchNormReLU3d, Identity). Parameters and statistics are the BatchNorm's
+    own, not copies. Returns the number of pairs fused."""
     count = 0
     for child in model.children():
         count += fuse_bn_relu(child)
@@ -187,13 +187,11 @@ def fuse_bn_relu(model: nn.Module) -> int:
         for a, b in zip(names, names[1:]):
             bn, act = model._modules[a], model._modules[b]
             if type(bn) is nn.BatchNorm3d and type(act) is nn.ReLU:
-                ref = bn.weight if bn.affine else bn.running_mean
                 new = BatchNormReLU3d(bn.num_features, bn.eps, bn.momentum, bn.affine, bn.track_running_stats,
-                                      device=None if ref is None else ref.device,
-                                      dtype=None if ref is None else ref.dtype)
-                new.load_state_dict(bn.state_dict())
-                new.train(bn.training)
-                model._modules[a] = new
+                                      device="meta")
+                for name in ("weight", "bias", "running_mean", "running_var", "num_batches_tracked"):
+                    setattr(new, name, getattr(bn, name))
+                model._modules[a] = new.train(bn.training)
                 model._modules[b] = nn.Identity()
                 count += 1
     return count
