@@ -175,10 +175,15 @@ class BatchNormReLU3d(nn.BatchNorm3d):
                                   float(self.eps), int(lead), self._sums_hook(), self._pivot())
 
 
+def has_hooks(m: nn.Module) -> bool:
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
 def fuse_bn_relu(model: nn.Module) -> int:
     """Replace each (BatchNorm3d, ReLU) pair inside an nn.Sequential with
     (BatchNormReLU3d, Identity). Parameters and statistics are the BatchNorm's
-    own, not copies. Returns the number of pairs fused."""
+    own, not copies. Pairs with hooks on either module stay as they are (what
+    the hooks see would be gone). Returns the number of pairs fused."""
     count = 0
     for child in model.children():
         count += fuse_bn_relu(child)
@@ -186,7 +191,7 @@ def fuse_bn_relu(model: nn.Module) -> int:
         names = list(model._modules.keys())
         for a, b in zip(names, names[1:]):
             bn, act = model._modules[a], model._modules[b]
-            if type(bn) is nn.BatchNorm3d and type(act) is nn.ReLU:
+            if type(bn) is nn.BatchNorm3d and type(act) is nn.ReLU and not (has_hooks(bn) or has_hooks(act)):
                 new = BatchNormReLU3d(bn.num_features, bn.eps, bn.momentum, bn.affine, bn.track_running_stats,
                                       device="meta")
                 for name in ("weight", "bias", "running_mean", "running_var", "num_batches_tracked"):

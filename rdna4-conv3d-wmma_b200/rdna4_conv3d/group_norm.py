@@ -28,6 +28,7 @@ import torch
 import torch.nn as nn
 
 from . import _native
+from .bn_relu import has_hooks
 from .checkpoint8 import _pack_torch, _unpack_torch, check_format
 from .logprobs import refuse_blind, refuse_twice
 
@@ -304,10 +305,6 @@ def _activation_of(m: nn.Module):
     return None
 
 
-def _has_hooks(m: nn.Module) -> bool:
-    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
-
-
 def fuse_group_norm(model: nn.Module) -> int:
     """Replace each (GroupNorm, ReLU / LeakyReLU / SiLU / GELU) pair inside an
     nn.Sequential with (GroupNormAct3d, Identity). The parameters are the
@@ -320,7 +317,7 @@ def fuse_group_norm(model: nn.Module) -> int:
         names = list(model._modules.keys())
         for a, b in zip(names, names[1:]):
             norm, act = model._modules[a], _activation_of(model._modules[b])
-            if type(norm) is nn.GroupNorm and act is not None and not (_has_hooks(norm) or _has_hooks(model._modules[b])):
+            if type(norm) is nn.GroupNorm and act is not None and not (has_hooks(norm) or has_hooks(model._modules[b])):
                 new = GroupNormAct3d(norm.num_groups, norm.num_channels, norm.eps, norm.affine, act[0], act[1],
                                      device="meta")
                 new.weight, new.bias = norm.weight, norm.bias

@@ -37,3 +37,14 @@ def test_parameters_and_statistics_are_the_models_own():
     assert not seq[0].weight.requires_grad and seq[2].weight is seq[4].weight
     seq(_x())
     assert int(seq[2].num_batches_tracked) == 2 and int(twin[2].num_batches_tracked) == 2
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_modules_with_hooks_stay(which):
+    """A hook sees the norm's output before the activation, which a fused pair does not have."""
+    seq = nn.Sequential(nn.BatchNorm3d(8), nn.ReLU(), nn.BatchNorm3d(8), nn.ReLU())
+    seen = []
+    seq[which].register_forward_hook(lambda *a: seen.append(1))
+    assert fuse_bn_relu(seq) == 1 and type(seq[0]) is nn.BatchNorm3d and isinstance(seq[2], BatchNormReLU3d)
+    seq(_x())
+    assert seen == [1]
