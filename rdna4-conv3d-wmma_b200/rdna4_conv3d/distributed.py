@@ -665,14 +665,19 @@ def depth_shard_model(model: torch.nn.Module, group=None) -> List[torch.nn.Param
     """Convert a model in place for depth sharding over ``group``: every k3
     pad-1 Conv3d becomes a DepthShardedConv3d (halo exchange), every
     BatchNorm3d a DepthShardedBatchNorm3d, every fused BatchNormReLU3d a
-    DepthShardedBatchNormReLU3d and every GroupNormAct3d a
+    DepthShardedBatchNormReLU3d and every GroupNorm and GroupNormAct3d a
     DepthShardedGroupNormAct3d (statistics over the whole volume; activations
-    are kept whole, whatever ``checkpoint`` says).
+    are kept whole, whatever ``checkpoint`` says). Group norms of other classes
+    are refused: their forward is not known.
     Pooling, k2s2 transpose convs, concatenation and k1 convs need no
     exchange. Returns the parameters whose gradients are still per-slab
     partial sums (the transpose convs and k1 convs): reduce them with
     ``GradSync(params, average=False)``."""
     partial: List[torch.nn.Parameter] = []
+    for name, mod in model.named_modules():
+        if isinstance(mod, torch.nn.GroupNorm) and \
+                type(mod) not in (torch.nn.GroupNorm, GroupNormAct3d, DepthShardedGroupNormAct3d):
+            raise TypeError(f"{name or 'the model'}: a {type(mod).__name__} cannot be sharded by depth")
 
     def convert(mod):
         for name, child in list(mod.named_children()):
@@ -703,10 +708,11 @@ def depth_shard_model(model: torch.nn.Module, group=None) -> List[torch.nn.Param
                                               dtype=None if ref is None else ref.dtype)
                 new.load_state_dict(child.state_dict())
                 setattr(mod, name, new)
-            elif isinstance(child, GroupNormAct3d) and not isinstance(child, DepthShardedGroupNormAct3d):
+            elif isinstance(child, torch.nn.GroupNorm) and not isinstance(child, DepthShardedGroupNormAct3d):
                 ref = child.weight
-                new = DepthShardedGroupNormAct3d(child.num_groups, child.num_channels, child.eps, child.affine,
-                                                 child.activation, child.negative_slope, group=group,
+                act = (child.activation, child.negative_slope) if isinstance(child, GroupNormAct3d) else ("none", 0.0)
+                new = DepthShardedGroupNormAct3d(child.num_groups, child.num_channels, child.eps, child.affine, *act,
+                                                 group=group,
                                                  device=None if ref is None else ref.device,
                                                  dtype=None if ref is None else ref.dtype)
                 new.load_state_dict(child.state_dict())

@@ -1,0 +1,75 @@
+"""Group norms of a depth-sharded model on CPU (gloo, two ranks), and what sharding a model keeps of it."""
+import os
+
+import pytest
+import torch
+import torch.distributed as dist
+import torch.nn as nn
+
+from test_distributed_gloo import _init, _run, _slab
+
+
+def _unfused_unet(**kw):
+    from rdna4_conv3d.unet3d import unet3d
+    torch.manual_seed(3)
+    net = unet3d(4, levels=2, n_classes=2, norm="group", groups=2, wmma=False, **kw).double()
+    for p in net.parameters():
+        nn.init.normal_(p, std=0.3)
+    return net
+
+
+def _data():
+    g = torch.Generator().manual_seed(9)
+    kw = dict(generator=g, dtype=torch.float64)
+    return torch.randn(2, 1, 16, 8, 8, **kw), torch.randn(2, 2, 16, 8, 8, **kw)
+
+
+def _worker_unfused(rank, port, outdir):
+    from rdna4_conv3d.distributed import DepthShardedGroupNormAct3d, GradSync, depth_shard_model
+    _init(rank, port)
+    try:
+        net = _unfused_unet()
+        partial = depth_shard_model(net)
+        assert sum(isinstance(m, DepthShardedGroupNormAct3d) for m in net.modules()) == 6
+        GradSync(partial, average=False)
+        x, gy = _data()
+        y = net(_slab(x, rank))
+        (y * _slab(gy, rank)).sum().backward()
+        torch.save({"y": y.detach(), "grads": {n: p.grad.clone() for n, p in net.named_parameters()}},
+                   os.path.join(outdir, f"r{rank}.pt"))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_plain_group_norms_take_the_whole_volume():
+    """nn.GroupNorm that no fusing replaced: fp64, against the unsharded model."""
+    res = _run(_worker_unfused)
+    net = _unfused_unet()
+    assert sum(type(m) is nn.GroupNorm for m in net.modules()) == 6
+    x, gy = _data()
+    y = net(x)
+    (y * gy).sum().backward()
+    torch.testing.assert_close(torch.cat([r["y"] for r in res], dim=2), y.detach(), rtol=1e-9, atol=1e-9)
+    for r in res:
+        for n, p in net.named_parameters():
+            torch.testing.assert_close(r["grads"][n], p.grad, rtol=1e-8, atol=1e-9, msg=n)
+
+
+class _OwnNorm(nn.GroupNorm):
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+def test_norms_of_another_class_are_refused():
+    """Their forward is not known, so neither is what it would need of the other slabs; nothing is converted."""
+    from rdna4_conv3d.distributed import depth_shard_model
+    from rdna4_conv3d.group_norm import GroupNormAct3d
+
+    class OwnAct(GroupNormAct3d):
+        pass
+
+    for norm in (_OwnNorm(2, 8), OwnAct(2, 8)):
+        net = nn.Sequential(nn.Conv3d(8, 8, 3, padding=1), norm)
+        with pytest.raises(TypeError, match="cannot be sharded"):
+            depth_shard_model(net)
+        assert type(net[0]) is nn.Conv3d and net[1] is norm
