@@ -661,6 +661,23 @@ class DepthShardedConv3d(torch.nn.Conv3d):
         return super().forward(x)
 
 
+_HOOKS = ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always_called", "_forward_pre_hooks",
+          "_forward_pre_hooks_with_kwargs", "_backward_hooks", "_backward_pre_hooks", "_is_full_backward_hook")
+
+
+def _keep(new: torch.nn.Module, old: torch.nn.Module) -> torch.nn.Module:
+    """``new`` with the parameters, buffers, mode and hooks of ``old`` (a reparametrised module's values are copied by
+    the caller: its hooks go with parameters that ``new`` does not have)."""
+    for mine, its in ((new._parameters, old._parameters), (new._buffers, old._buffers)):
+        for name in mine:
+            if name in its:
+                mine[name] = its[name]
+    if set(old._parameters) <= set(new._parameters):
+        for name in _HOOKS:
+            setattr(new, name, getattr(old, name))
+    return new.train(old.training)
+
+
 def depth_shard_model(model: torch.nn.Module, group=None) -> List[torch.nn.Parameter]:
     """Convert a model in place for depth sharding over ``group``: every k3
     pad-1 Conv3d becomes a DepthShardedConv3d (halo exchange), every
@@ -670,7 +687,8 @@ def depth_shard_model(model: torch.nn.Module, group=None) -> List[torch.nn.Param
     are kept whole, whatever ``checkpoint`` says). Group norms of other classes
     are refused: their forward is not known.
     Pooling, k2s2 transpose convs, concatenation and k1 convs need no
-    exchange. Returns the parameters whose gradients are still per-slab
+    exchange. Converted layers keep the model's own parameters, statistics,
+    mode and hooks. Returns the parameters whose gradients are still per-slab
     partial sums (the transpose convs and k1 convs): reduce them with
     ``GradSync(params, average=False)``."""
     partial: List[torch.nn.Parameter] = []
@@ -679,49 +697,46 @@ def depth_shard_model(model: torch.nn.Module, group=None) -> List[torch.nn.Param
                 type(mod) not in (torch.nn.GroupNorm, GroupNormAct3d, DepthShardedGroupNormAct3d):
             raise TypeError(f"{name or 'the model'}: a {type(mod).__name__} cannot be sharded by depth")
 
+    made = {}                                            # a module used twice stays one
+
+    def sharded(child):
+        """The sharded form of a layer; None for what has none."""
+        ref = next((t for t in (*child._parameters.values(), *child._buffers.values()) if t is not None), None)
+        kw = dict(group=group, device=None if ref is None else ref.device, dtype=None if ref is None else ref.dtype)
+        if isinstance(child, torch.nn.Conv3d) and child.kernel_size == (3, 3, 3) and child.padding == (1, 1, 1):
+            new = DepthShardedConv3d(child.in_channels, child.out_channels, 3, padding=1, bias=child.bias is not None, **kw)
+            with torch.no_grad():
+                new.weight.copy_(child.weight)
+                if child.bias is not None:
+                    new.bias.copy_(child.bias)
+        elif isinstance(child, BatchNormReLU3d):
+            new = DepthShardedBatchNormReLU3d(child.num_features, child.eps, child.momentum, child.affine,
+                                              child.track_running_stats, relu=child.relu, **kw)
+        elif isinstance(child, torch.nn.BatchNorm3d):
+            new = DepthShardedBatchNorm3d(child.num_features, child.eps, child.momentum, child.affine,
+                                          child.track_running_stats, **kw)
+        elif isinstance(child, torch.nn.GroupNorm):
+            act = (child.activation, child.negative_slope) if isinstance(child, GroupNormAct3d) else ("none", 0.0)
+            new = DepthShardedGroupNormAct3d(child.num_groups, child.num_channels, child.eps, child.affine, *act, **kw)
+        else:
+            return None
+        return _keep(new, child)
+
+    done = (DepthShardedConv3d, DepthShardedBatchNorm3d, DepthShardedBatchNormReLU3d, DepthShardedGroupNormAct3d)
+
     def convert(mod):
-        for name, child in list(mod.named_children()):
-            if isinstance(child, torch.nn.Conv3d) and not isinstance(child, DepthShardedConv3d) \
-                    and child.kernel_size == (3, 3, 3) and child.padding == (1, 1, 1):
-                new = DepthShardedConv3d(child.in_channels, child.out_channels, 3, padding=1,
-                                         bias=child.bias is not None, group=group,
-                                         device=child.weight.device, dtype=child.weight.dtype)
-                with torch.no_grad():
-                    new.weight.copy_(child.weight)
-                    if child.bias is not None:
-                        new.bias.copy_(child.bias)
-                setattr(mod, name, new)
-            elif isinstance(child, BatchNormReLU3d) and not isinstance(child, DepthShardedBatchNormReLU3d):
-                ref = child.weight if child.affine else child.running_mean
-                new = DepthShardedBatchNormReLU3d(child.num_features, child.eps, child.momentum, child.affine,
-                                                  child.track_running_stats, relu=child.relu, group=group,
-                                                  device=None if ref is None else ref.device,
-                                                  dtype=None if ref is None else ref.dtype)
-                new.load_state_dict(child.state_dict())
-                setattr(mod, name, new)
-            elif isinstance(child, torch.nn.BatchNorm3d) and not isinstance(child, DepthShardedBatchNorm3d) \
-                    and not isinstance(child, BatchNormReLU3d):
-                ref = child.weight if child.affine else child.running_mean
-                new = DepthShardedBatchNorm3d(child.num_features, child.eps, child.momentum, child.affine,
-                                              child.track_running_stats, group=group,
-                                              device=None if ref is None else ref.device,
-                                              dtype=None if ref is None else ref.dtype)
-                new.load_state_dict(child.state_dict())
-                setattr(mod, name, new)
-            elif isinstance(child, torch.nn.GroupNorm) and not isinstance(child, DepthShardedGroupNormAct3d):
-                ref = child.weight
-                act = (child.activation, child.negative_slope) if isinstance(child, GroupNormAct3d) else ("none", 0.0)
-                new = DepthShardedGroupNormAct3d(child.num_groups, child.num_channels, child.eps, child.affine, *act,
-                                                 group=group,
-                                                 device=None if ref is None else ref.device,
-                                                 dtype=None if ref is None else ref.dtype)
-                new.load_state_dict(child.state_dict())
-                setattr(mod, name, new)
-            elif isinstance(child, (torch.nn.Conv3d, torch.nn.ConvTranspose3d)) \
-                    and not isinstance(child, DepthShardedConv3d):
+        for name, child in list(mod._modules.items()):
+            if child is None or isinstance(child, done):
+                continue
+            if id(child) not in made:
+                made[id(child)] = sharded(child)
+            new = made[id(child)]
+            if new is not None:
+                mod._modules[name] = new
+            elif isinstance(child, (torch.nn.Conv3d, torch.nn.ConvTranspose3d)):
                 partial.extend(p for p in child.parameters(recurse=False) if p.requires_grad)
             else:
                 convert(child)
 
     convert(model)
-    return partial
+    return list({id(p): p for p in partial}.values())

@@ -73,3 +73,42 @@ def test_norms_of_another_class_are_refused():
         with pytest.raises(TypeError, match="cannot be sharded"):
             depth_shard_model(net)
         assert type(net[0]) is nn.Conv3d and net[1] is norm
+
+
+def _every_kind():
+    from rdna4_conv3d.bn_relu import BatchNormReLU3d
+    from rdna4_conv3d.group_norm import GroupNormAct3d
+    return nn.Sequential(nn.Conv3d(8, 8, 3, padding=1), nn.BatchNorm3d(8), BatchNormReLU3d(8), nn.GroupNorm(2, 8),
+                         GroupNormAct3d(4, 8, activation="silu"), nn.Conv3d(8, 8, 1))
+
+
+def test_sharding_keeps_parameters_statistics_mode_and_hooks():
+    """Frozen ones stay frozen, an optimizer's stay its own, eval stays eval; not-frozen convs alone are returned."""
+    from rdna4_conv3d.distributed import depth_shard_model
+    net = _every_kind().eval()
+    net[3].requires_grad_(False)
+    net[1].train()
+    was = dict(net.named_parameters()), dict(net.named_buffers())
+    seen = []
+    for i, m in enumerate(net):
+        m.register_forward_hook(lambda m, a, y, i=i: seen.append(i))
+    partial = depth_shard_model(net)
+    now = dict(net.named_parameters()), dict(net.named_buffers())
+    for a, b in zip(was, now):
+        assert list(a) == list(b) and all(a[k] is b[k] for k in a)
+    assert [type(m).__name__[:12] for m in net] == ["DepthSharded"] * 5 + ["Conv3d"]
+    assert [m.training for m in net] == [False, True, False, False, False, False]
+    assert len(partial) == 2 and partial[0] is net[5].weight and partial[1] is net[5].bias
+    # (without a process group the modules take their own slab as the volume; the conv asks for one)
+    net[1:](torch.randn(1, 8, 2, 3, 4))
+    assert seen == [1, 2, 3, 4, 5]
+
+
+def test_a_module_used_twice_is_sharded_twice():
+    from rdna4_conv3d.distributed import DepthShardedGroupNormAct3d, depth_shard_model
+    norm, conv = nn.GroupNorm(2, 8), nn.Conv3d(8, 8, 1)
+    net = nn.Sequential(norm, conv, norm, nn.Sequential(norm, conv))
+    partial = depth_shard_model(net)
+    assert all(isinstance(m, DepthShardedGroupNormAct3d) for m in (net[0], net[2], net[3][0]))
+    assert net[0] is net[2] and net[0] is net[3][0]
+    assert len(partial) == 2
