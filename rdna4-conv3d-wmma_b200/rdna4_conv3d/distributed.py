@@ -692,6 +692,8 @@ def depth_shard_model(model: torch.nn.Module, group=None) -> List[torch.nn.Param
     partial sums (the transpose convs and k1 convs): reduce them with
     ``GradSync(params, average=False)``."""
     partial: List[torch.nn.Parameter] = []
+    if isinstance(model, (torch.nn.Conv3d, torch.nn.ConvTranspose3d, torch.nn.BatchNorm3d, torch.nn.GroupNorm)):
+        raise TypeError("depth_shard_model replaces layers inside a model: put a single layer into an nn.Sequential")
     for name, mod in model.named_modules():
         if isinstance(mod, torch.nn.GroupNorm) and \
                 type(mod) not in (torch.nn.GroupNorm, GroupNormAct3d, DepthShardedGroupNormAct3d):

@@ -112,3 +112,11 @@ def test_a_module_used_twice_is_sharded_twice():
     assert all(isinstance(m, DepthShardedGroupNormAct3d) for m in (net[0], net[2], net[3][0]))
     assert net[0] is net[2] and net[0] is net[3][0]
     assert len(partial) == 2
+
+
+@pytest.mark.parametrize("root", [0, 1, 2, 3, 4])
+def test_a_single_layer_is_refused(root):
+    """It cannot be replaced inside itself, and would run unsharded without a word."""
+    from rdna4_conv3d.distributed import depth_shard_model
+    with pytest.raises(TypeError, match="inside"):
+        depth_shard_model(_every_kind()[root])
