@@ -120,3 +120,24 @@ def test_a_single_layer_is_refused(root):
     from rdna4_conv3d.distributed import depth_shard_model
     with pytest.raises(TypeError, match="inside"):
         depth_shard_model(_every_kind()[root])
+
+
+@pytest.fixture
+def alone():
+    """A process group of this process alone."""
+    import datetime
+
+    from test_distributed_gloo import _free_port
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{_free_port()}", rank=0, world_size=1,
+                            timeout=datetime.timedelta(seconds=60))
+    yield
+    dist.destroy_process_group()
+
+
+def test_a_second_differentiation_is_refused(alone):
+    """It would pass by the sums over the ranks."""
+    from rdna4_conv3d.distributed import DepthShardedGroupNormAct3d
+    x = torch.randn(1, 8, 2, 3, 4, requires_grad=True)
+    y = DepthShardedGroupNormAct3d(2, 8, activation="silu")(x)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
