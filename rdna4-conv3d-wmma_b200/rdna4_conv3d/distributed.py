@@ -586,13 +586,19 @@ class _ShardedGroupNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, groups, eps, activation, slope, group):
         n, c = x.shape[:2]
         xg = x.double().reshape(n, groups, -1)
-        s = torch.stack([xg.sum(-1), (xg * xg).sum(-1), torch.full_like(xg[..., 0], xg.shape[-1])])
-        dist.all_reduce(s, group=group)
-        total = s[2, 0, 0]
+        # every rank's (count, mean, sum of squares about it), joined by Chan's rule: sums of x^2 would cancel where
+        # |mean| >> spread
+        mean = xg.mean(-1)
+        own = torch.stack([torch.full_like(mean, xg.shape[-1]), mean, ((xg - mean.unsqueeze(-1)) ** 2).sum(-1)])
+        parts = [torch.empty_like(own) for _ in range(dist.get_world_size(group))]
+        dist.all_gather(parts, own, group=group)
+        count, mean, m2 = torch.stack(parts).unbind(1)
+        total, shift = count.sum(0), mean[0]
+        joint = shift + (count * (mean - shift)).sum(0) / total
+        var = (m2 + count * (mean - joint) ** 2).sum(0) / total
         acc = torch.promote_types(x.dtype, torch.float32)
-        mean = s[0] / total
-        rstd = (((s[1] / total - mean * mean).clamp(min=0) + eps) ** -0.5).to(acc).unsqueeze(-1)
-        mean = mean.to(acc).unsqueeze(-1)
+        rstd = ((var + eps) ** -0.5).to(acc).unsqueeze(-1)
+        mean, total = joint.to(acc).unsqueeze(-1), total[0, 0]
         ctx.save_for_backward(x, mean, rstd, total, weight, bias)
         ctx.args = groups, activation, slope, group
         z, _ = _ShardedGroupNormFn._z(x, mean, rstd, weight, bias, groups)
@@ -630,7 +636,7 @@ class _ShardedGroupNormFn(torch.autograd.Function):
 
 class DepthShardedGroupNormAct3d(GroupNormAct3d):
     """GroupNormAct3d over a D-sharded volume: each rank holds one D slab of
-    the same samples, statistics and gradient sums are all-reduced over
+    the same samples, statistics and gradient sums are those of all ranks of
     ``group`` (torch operations; the input is kept whole). Weight and bias
     gradients come out as whole-volume sums."""
 

@@ -141,3 +141,50 @@ def test_a_second_differentiation_is_refused(alone):
     y = DepthShardedGroupNormAct3d(2, 8, activation="silu")(x)
     with pytest.raises(RuntimeError, match="differentiated again"):
         torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def _far(value, dtype):
+    x = torch.full((1, 8, 4, 3, 5), value, dtype=dtype)
+    x[0, 0, 1, 2, 3] += 0.25                             # one group with a spread
+    return x, torch.randn(x.shape, generator=torch.Generator().manual_seed(4)).to(dtype)
+
+
+def _check_far(value, dtype, y, dx, ulps):
+    """(ulps: of the norm's own type; the mean's rounding moves x - mean by half a one of it)"""
+    x, dy = _far(value, dtype)
+    u = torch.finfo(torch.promote_types(dtype, torch.float32)).eps / 2
+    xd, g = (t.double().reshape(1, 4, -1) for t in (x, dy))
+    mean = xd.mean(-1, keepdim=True)
+    rstd = (((xd - mean) ** 2).mean(-1, keepdim=True) + 1e-5) ** -0.5
+    xh = (xd - mean) * rstd
+    c = (g * xh).mean(-1, keepdim=True)
+    want = rstd * (g - g.mean(-1, keepdim=True) - xh * c)
+    e = u * (abs(value) * rstd + ulps * xh.abs())
+    assert bool(((y.double().reshape(xh.shape) - xh).abs() <= e).all())
+    bound = rstd * (e * c.abs() + xh.abs() * (e * g.abs()).mean(-1, keepdim=True)
+                    + ulps * u * (g.abs() + g.abs().mean(-1, keepdim=True) + xh.abs() * (g * xh).abs().mean(-1, keepdim=True)))
+    assert bool(((dx.double().reshape(want.shape) - want).abs() <= bound).all())
+
+
+def _worker_far(rank, port, outdir):
+    from rdna4_conv3d.distributed import DepthShardedGroupNormAct3d
+    _init(rank, port)
+    try:
+        out = []
+        for value, dtype in ((30000.0, torch.float32), (1e6, torch.float32), (-1e9, torch.float64)):
+            x, dy = (_slab(t, rank) for t in _far(value, dtype))
+            x.requires_grad_(True)
+            y = DepthShardedGroupNormAct3d(4, 8, affine=False)(x)
+            out.append((y.detach(), torch.autograd.grad(y, x, dy)[0]))
+        torch.save(out, os.path.join(outdir, f"r{rank}.pt"))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_statistics_far_from_zero():
+    """A slab of one large value: nothing may cancel in the variance over the ranks."""
+    res = _run(_worker_far)
+    for i, (value, dtype) in enumerate(((30000.0, torch.float32), (1e6, torch.float32), (-1e9, torch.float64))):
+        y, dx = (torch.cat([r[i][k] for r in res], dim=2) for k in (0, 1))
+        # 16: a few products, and torch's blocked sums of 15 to 30 elements
+        _check_far(value, dtype, y, dx, 16)
