@@ -199,6 +199,15 @@ def _normalised(x, groups, mean, rstd):
     return ((x.reshape(n, groups, -1) - mean) * rstd).reshape(x.shape)
 
 
+def _centred(xg):
+    """(x - mean, mean) over the last dimension; the mean of what is left makes up for the first mean's rounding, which
+    is not small against a spread far below |mean|."""
+    mean = xg.mean(-1, keepdim=True)
+    d = xg - mean
+    rest = d.mean(-1, keepdim=True)
+    return d - rest, mean + rest
+
+
 def _group_norm_torch(x, groups, weight, bias, eps, activation, slope, checkpoint):
     """The same in torch operations, at least in fp32."""
     if x.numel() == 0:
@@ -211,10 +220,8 @@ def _group_norm_torch(x, groups, weight, bias, eps, activation, slope, checkpoin
         return _KeptTorchFn.apply(x, weight, bias, groups, eps, activation, slope, checkpoint)
     acc = torch.promote_types(x.dtype, torch.float32)
     n, c = x.shape[:2]
-    xg = x.to(acc).reshape(n, groups, -1)
-    mean = xg.mean(-1, keepdim=True)
-    var = ((xg - mean) ** 2).mean(-1, keepdim=True)
-    z = _normalised(x.to(acc), groups, mean, (var + eps) ** -0.5)
+    d, _ = _centred(x.to(acc).reshape(n, groups, -1))
+    z = (d * ((d ** 2).mean(-1, keepdim=True) + eps) ** -0.5).reshape(x.shape)
     each = (1, c) + (1,) * (x.dim() - 2)
     if weight is not None:
         z = z * weight.to(acc).reshape(each)
@@ -230,9 +237,8 @@ class _KeptTorchFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, activation, slope, checkpoint):
         n = x.shape[0]
-        xg = x.float().reshape(n, groups, -1)
-        mean = xg.mean(-1, keepdim=True)
-        rstd = (((xg - mean) ** 2).mean(-1, keepdim=True) + eps) ** -0.5
+        d, mean = _centred(x.float().reshape(n, groups, -1))
+        rstd = ((d ** 2).mean(-1, keepdim=True) + eps) ** -0.5
         codes, exps = _pack_torch(x.movedim(1, -1).contiguous(), checkpoint)
         ctx.save_for_backward(codes, exps, mean, rstd, weight, bias)
         ctx.args = x.shape, x.dtype, groups, activation, slope, checkpoint
