@@ -571,17 +571,22 @@ __device__ __forceinline__ void add_previous(const P* p, int64_t first, int64_t 
   }
 }
 
-// The thread's parameters: z = (x - mean) * a + b with a = rstd * w. For 16-bit x the mean goes into b (z = x * a + b'):
-// its rounding is 2^-24 of |mean| a, where x's own step is 2^-8 or 2^-11 of |x|; likewise sum dz * x and the sums'
-// difference stand for sum dz * (x - mean)). w and b do not wait for the statistics.
-template <typename T> constexpr bool kCentred = sizeof(T) == 4;
-template <typename T, int V>
+// The thread's parameters: z = (x - mean) * a + b with a = rstd * w. The mean is not taken into b, in 16-bit types neither:
+// 2^-24 of |mean| a is not small against xh where a group has next to no spread, and sums of dz * x would cancel against
+// mean * sum dz. w and b do not wait for the statistics.
+// SHARED: the means' negatives lie in shared memory, per column, and are read for each vector (for the gradients of
+// vectors of 8, whose registers would spill: [4,24,64,128,128] bf16 silu 175 us in registers, 170 so, kept in 8 bits 232
+// and 193).
+template <int V> constexpr bool kSharedMeans = V == 8;
+template <typename T, int V, bool SHARED = false>
 struct Affine {
-  float2 nmu[kPairs<V>], a[kPairs<V>], b[kPairs<V>];
+  float2 nmu[SHARED ? 1 : kPairs<V>], a[kPairs<V>], b[kPairs<V>];
+  float4* means;         // SHARED: the thread's columns'; threads of row 0 write them
   __device__ __forceinline__ void params(const Geo& g, const Place& p, const void* gamma, const void* beta) {
 #pragma unroll
     for (int k = 0; k < kPairs<V>; ++k) {
-      nmu[k] = b[k] = two(0.f);
+      if constexpr (!SHARED) nmu[k] = two(0.f);
+      b[k] = two(0.f);
       a[k] = two(1.f);
     }
     if (!p.active) return;
@@ -616,18 +621,21 @@ struct Affine {
     each_column<V>(g, p, [&](int k, int, int gi) {
       if (gi != have) q = stat(gi);
       have = gi;
-      put(nmu, k, -q.x);
+      if constexpr (!SHARED) put(nmu, k, -q.x);
+      else if (p.row == 0) reinterpret_cast<float*>(means)[k] = -q.x;
       put(r, k, q.y);
     });
 #pragma unroll
-    for (int k = 0; k < kPairs<V>; ++k) {
-      a[k] = __fmul2_rn(a[k], r[k]);
-      if constexpr (!kCentred<T>) b[k] = __ffma2_rn(nmu[k], a[k], b[k]);
-    }
+    for (int k = 0; k < kPairs<V>; ++k) a[k] = __fmul2_rn(a[k], r[k]);
   }
-  // x becomes x - mean (or stays: 16-bit types); z of it
+  // x becomes x - mean; z of it
   __device__ __forceinline__ float2 z(int k, float2& x) const {
-    if constexpr (kCentred<T>) x = __fadd2_rn(x, nmu[k]);
+    if constexpr (SHARED) {
+      const float4 m = means[k / 2];
+      x = __fadd2_rn(x, k & 1 ? make_float2(m.z, m.w) : make_float2(m.x, m.y));
+    } else {
+      x = __fadd2_rn(x, nmu[k]);
+    }
     return __ffma2_rn(x, a[k], b[k]);
   }
 };
@@ -872,9 +880,10 @@ __global__ void __launch_bounds__(kThreads, kApplyBlocks) apply_kernel(
 // ---------------------------------------------------------------------------
 // Backward: sums
 // ---------------------------------------------------------------------------
-// dz and x - mean (16-bit types: x) of one vector.
-template <typename T, int V, int ACT, bool Q>
-__device__ __forceinline__ void grad_one(const Source<T, V, Q>& v, const Vec<T, V>& d, const Affine<T, V>& k, const Geo& g,
+// dz and x - mean of one vector.
+template <typename T, int V, int ACT, bool Q, bool SHARED>
+__device__ __forceinline__ void grad_one(const Source<T, V, Q>& v, const Vec<T, V>& d, const Affine<T, V, SHARED>& k,
+                                         const Geo& g,
                                          float2 (&xm)[kPairs<V>], float2 (&dz)[kPairs<V>]) {
   v.to_f(g.format, xm);
   d.to_f(dz);
@@ -884,7 +893,7 @@ __device__ __forceinline__ void grad_one(const Source<T, V, Q>& v, const Vec<T, 
   act_grads<T, ACT>(dz, z, g.act, g.slope);
 }
 
-// dz and x - mean (16-bit types: x) of one element of channel c.
+// dz and x - mean of one element of channel c.
 template <typename T, int ACT, bool Q>
 __device__ __forceinline__ float2 grad_edge(const Geo& g, const T* __restrict__ dy, const void* __restrict__ x,
                                             const uint8_t* __restrict__ exps, const void* gamma, const void* beta,
@@ -894,16 +903,16 @@ __device__ __forceinline__ float2 grad_edge(const Geo& g, const T* __restrict__ 
   v.load(x, exps, at);
   v.to_f(g.format, xm);
   const float a = stat.y * param(gamma, g.pdtype, c, 1.f), b = param(beta, g.pdtype, c, 0.f);
-  if (kCentred<T>) xm[0].x -= stat.x;
-  const float2 z[1] = {make_float2(fmaf(xm[0].x, a, kCentred<T> ? b : fmaf(-stat.x, a, b)), 0.f)};
+  xm[0].x -= stat.x;
+  const float2 z[1] = {make_float2(fmaf(xm[0].x, a, b), 0.f)};
   act_grads<T, ACT>(dz, z, g.act, g.slope);
   return make_float2(dz[0].x, xm[0].x);
 }
 
-// The block's (sum dz, sum dz * (x - mean)) of a thread's columns (16-bit types: sum dz * x): cpart gets them per channel
-// (the second times rstd), out(group, ..) the same times w, summed over the tile's channels of the group.
-// edge(element, channel, stat): an edge's dz and x - mean, or x.
-template <typename T, int V, bool EDGES, typename Stat, typename Edge, typename Out>
+// The block's (sum dz, sum dz * (x - mean)) of a thread's columns: cpart gets them per channel (the second times rstd),
+// out(group, ..) the same times w, summed over the tile's channels of the group.
+// edge(element, channel, stat): an edge's dz and x - mean.
+template <int V, bool EDGES, typename Stat, typename Edge, typename Out>
 __device__ __forceinline__ void block_grads(const Geo& g, const Place& p, const float2 (&s1)[kPairs<V>],
                                             const float2 (&s2)[kPairs<V>], const void* gamma, float2* __restrict__ red,
                                             float2* __restrict__ cols, float2* __restrict__ cpart, Stat stat, Edge edge,
@@ -931,7 +940,7 @@ __device__ __forceinline__ void block_grads(const Geo& g, const Place& p, const 
   }, [&](int i, float a, float c) {
     const int ch = p.j0 + i;
     const float2 m = stat((int)((unsigned)ch / (unsigned)g.Cg));
-    const float2 s = make_float2(a, (kCentred<T> ? c : fmaf(-m.x, a, c)) * m.y);
+    const float2 s = make_float2(a, c * m.y);
     cols[i] = s;
     cpart[(int64_t)blockIdx.x * g.C + ch] = s;
   });
@@ -955,16 +964,19 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_sums_kernel(
     const __grid_constant__ Geo g, float2* __restrict__ cpart, float2* __restrict__ gpart) {
   using R = Ring<T, V, Q, true, kBwdAhead>;
   constexpr int kTable = V * kThreads * (int)sizeof(float2);
-  __shared__ __align__(16) char smem[R::kBytes > 2 * kTable ? R::kBytes : 2 * kTable];
+  constexpr int kLoop = R::kBytes + (kSharedMeans<V> ? V * kThreads * (int)sizeof(float) : 0);
+  __shared__ __align__(16) char smem[kLoop > 2 * kTable ? kLoop : 2 * kTable];
   let_next_start();
   const Place p = place<V>(g);
   R ring(smem, x, dy, exps, p.at, p.step);
 #pragma unroll
   for (int i = 0; i < kBwdAhead - 1; ++i) ring.start(i, i < p.mine);
   const float2* stats = mean_rstd + p.n * g.G;
-  Affine<T, V> k;
+  Affine<T, V, kSharedMeans<V>> k;
+  k.means = reinterpret_cast<float4*>(smem + R::kBytes) + p.lane * (V / 4);
   k.params(g, p, gamma, beta);
   k.stats(g, p, [&](int gi) { return stats[gi]; });
+  if constexpr (kSharedMeans<V>) __syncthreads();
   float2 a1[kPairs<V>], a2[kPairs<V>];
 #pragma unroll
   for (int i = 0; i < kPairs<V>; ++i) a1[i] = a2[i] = two(0.f);
@@ -995,7 +1007,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_sums_kernel(
   if (g.tiles > 1)
     for (int i = threadIdx.x; i < g.G; i += blockDim.x)
       if (i < p.ga || i >= p.gb) out[i] = make_float2(0.f, 0.f);
-  block_grads<T, V, (ACT < 0)>(g, p, a1, a2, gamma, reinterpret_cast<float2*>(smem), reinterpret_cast<float2*>(smem + kTable), cpart,
+  block_grads<V, (ACT < 0)>(g, p, a1, a2, gamma, reinterpret_cast<float2*>(smem), reinterpret_cast<float2*>(smem + kTable), cpart,
                  [&](int gi) { return stats[gi]; },
                  [&](int64_t at, int c, float2 s) { return grad_edge<T, ACT, Q>(g, dy, x, exps, gamma, beta, at, c, s); },
                  [&](int gi, float a, float c) { out[gi] = make_float2(a, c); });
@@ -1044,8 +1056,8 @@ inline __global__ void __launch_bounds__(kThreads) params_kernel(const float2* c
 }
 
 // dx of one vector; k1, k2: rstd * A, rstd^2 * B.
-template <typename T, int V, int ACT, bool Q>
-__device__ __forceinline__ Vec<T, V> dx_one(const Source<T, V, Q>& v, const Vec<T, V>& d, const Affine<T, V>& k,
+template <typename T, int V, int ACT, bool Q, bool SHARED>
+__device__ __forceinline__ Vec<T, V> dx_one(const Source<T, V, Q>& v, const Vec<T, V>& d, const Affine<T, V, SHARED>& k,
                                             const float2 (&k1)[kPairs<V>], const float2 (&k2)[kPairs<V>], const Geo& g) {
   float2 xm[kPairs<V>], dz[kPairs<V>];
   grad_one<T, V, ACT, Q>(v, d, k, g, xm, dz);
@@ -1068,11 +1080,10 @@ __device__ __forceinline__ void thread_coef(const Geo& g, const Place& p, const 
     put(k2, k, q.y);
   });
 }
-// dx = dz * rstd * w - (first + second * (x - mean)); for 16-bit types of x itself.
-template <typename T>
+// dx = dz * rstd * w - (first + second * (x - mean)).
 __device__ __forceinline__ float2 coef_of(const Geo& g, float2 stat, double a, double c) {
   const double rstd = stat.y, first = rstd * a * g.inv_m, second = rstd * rstd * c * g.inv_m;
-  return make_float2((float)(kCentred<T> ? first : first - stat.x * second), (float)second);
+  return make_float2((float)first, (float)second);
 }
 
 // dx of a sample's edges.
@@ -1115,14 +1126,15 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
   R ring(smem, x, dy, exps, at, -p.step);
 #pragma unroll
   for (int i = 0; i < kBwdAhead - 1; ++i) ring.start(i, i >= skip && i < p.tiles);
-  Affine<T, V> k;
+  Affine<T, V, kSharedMeans<V>> k;
+  k.means = reinterpret_cast<float4*>(coef + g.lanes * V) + p.lane * (V / 4);
   k.params(g, p, gamma, beta);
   k.stats(g, p, [&](int gi) { return stats[gi]; });
   wait_for_previous();
   const float2* src = gpart + p.n * g.np * g.G + p.ga;
   each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
     add_previous<4>(src + i, sub, tp, g.np, g.G, a, c);
-  }, [&](int i, double a, double c) { coef[i] = coef_of<T>(g, stats[p.ga + i], a, c); });
+  }, [&](int i, double a, double c) { coef[i] = coef_of(g, stats[p.ga + i], a, c); });
   __syncthreads();
   if (p.mine > 0) {
     float2 k1[kPairs<V>], k2[kPairs<V>];
@@ -1303,10 +1315,10 @@ __global__ void __launch_bounds__(kThreads)
       s2[j] = __ffma2_rn(dz[j], xm[j], s2[j]);
     }
   }
-  block_grads<T, V, (ACT < 0)>(g, p, s1, s2, gamma, red, cols, cpart, [&](int gi) { return stats[gi]; },
+  block_grads<V, (ACT < 0)>(g, p, s1, s2, gamma, red, cols, cpart, [&](int gi) { return stats[gi]; },
                  [&](int64_t at, int c, float2 s) { return grad_edge<T, ACT, Q>(g, dy, x, exps, gamma, beta, at, c, s); },
                  [&](int gi, float a, float c) { mine[gi - p.ga] = make_double2(a, c); });
-  cluster_sums(g, groups, mine, [&](int i, double a, double c) { coef[i] = coef_of<T>(g, stats[p.ga + i], a, c); });
+  cluster_sums(g, groups, mine, [&](int i, double a, double c) { coef[i] = coef_of(g, stats[p.ga + i], a, c); });
   if (p.mine > 0) {
     float2 k1[kPairs<V>], k2[kPairs<V>];
     thread_coef<V>(g, p, coef, k1, k2);

@@ -129,14 +129,19 @@ cudaError_t bwd_v(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
     const cudaError_t e = bwd_small<T, V, ACT, Q>(a, g, threads, s);
     return e != cudaSuccess || !params ? e : params_next();
   }
-  const size_t smem = Ring<T, V, Q, true, kBwdAhead>::kBytes + sizeof(float2) * (g.tiles == 1 ? g.G : g.lanes * V);
-  static std::atomic<uint64_t> shared_s{0}, shared_d{0};
+  using R = Ring<T, V, Q, true, kBwdAhead>;
+  // each group's coefficients, then the columns' means
+  constexpr size_t column = sizeof(float2) + (kSharedMeans<V> ? sizeof(float) : 0);
+  const size_t smem = R::kBytes + column * g.lanes * V;
+  static std::atomic<uint64_t> shared_s{0}, shared_d{0}, allowed{0};
+  cudaError_t e = allow_shared(bwd_dx_kernel<T, V, ACT, Q>, R::kBytes + (int)column * kThreads * V, allowed);
+  if (e != cudaSuccess) return e;
   all_shared(bwd_sums_kernel<T, V, ACT, Q>, shared_s);
   all_shared(bwd_dx_kernel<T, V, ACT, Q>, shared_d);
   bwd_sums_kernel<T, V, ACT, Q><<<dim3((unsigned)sums.blocks, g.tiles), threads, 0, s>>>(
       dy, a.x, a.exps, a.mean_rstd, a.gamma, a.beta, sums, a.cpart, a.gpart);
   note_launches(1);
-  cudaError_t e = cudaGetLastError();
+  e = cudaGetLastError();
   if (e != cudaSuccess || !a.dx) return e != cudaSuccess ? e : params_next();
   const bool beside = params && sums.blocks < kWideParts;
   if (beside) grid.x += cdiv(g.C, (int64_t)g.tiles * (threads / 32));

@@ -1,0 +1,84 @@
+"""Group norm where sums cancel: activations far from zero, groups without a spread, gradients that nearly vanish.
+
+u = 2^-24 is half a step of fp32. What the kernels may be off by: the mean (one rounding: u |mean|), rstd (u), a
+product or sum each (u), and fp32 sums of one thread, at most 64 terms at these sizes, each addition off by at most u of
+the sum of magnitudes. Beyond a thread sums are taken in 64 bits, which loses nothing that would show here.
+"""
+import pytest
+import torch
+
+import gn_refs as R
+from rdna4_conv3d.group_norm import group_norm_act
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+U = 2.0 ** -24
+CHAIN = 64 * U
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _last(t):
+    return t.movedim(1, -1).contiguous().movedim(-1, 1)
+
+
+def _over(t, groups):
+    n = t.shape[0]
+    m = t.reshape(n, groups, -1).mean(-1, keepdim=True)
+    return m.expand(n, groups, t.numel() // (n * groups)).reshape(t.shape)
+
+
+def _affine_check(x, groups, w, b, dy, fmt=None, eps=1e-5):
+    """y, dx, dw, db of act 'none' against 64 bits, with bounds of arithmetic on x - mean."""
+    x, w, b = (t.detach().requires_grad_(True) for t in (x, w, b))
+    y = group_norm_act(x, groups, w, b, eps, checkpoint=fmt)
+    got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(y, (x, w, b), dy)), y=y)
+    each = (1, x.shape[1]) + (1,) * (x.dim() - 2)
+    dims = (0, *range(2, x.dim()))
+    xd, g = x.detach().double(), dy.double()
+    wd, bd = w.detach().double().reshape(each), b.detach().double().reshape(each)
+    mean = _over(xd, groups)
+    rstd = (_over((xd - mean) ** 2, groups) + eps) ** -0.5
+    shift = U * (mean * rstd).abs()                      # of every xh: the mean's rounding
+    xh = (xd - mean) * rstd
+    want = {"y": (xh * wd + bd, R.half_step(xh * wd + bd, x.dtype) + (shift + 4 * U * xh.abs()) * wd.abs() + 2 * U * bd.abs())}
+    kept = xd if fmt is None else R.held(x, fmt).double()
+    xh = (kept - mean) * rstd
+    xh_e = shift + 4 * U * xh.abs()
+    gw = g * wd
+    a, c = _over(gw, groups), _over(gw * xh, groups)
+    # sums of a thread and of a channel's parts times w (one rounding each)
+    a_e = _over(gw.abs(), groups) * (CHAIN + 4 * U)
+    c_e = _over(gw.abs() * xh_e + (CHAIN + 4 * U) * (gw * xh).abs(), groups)
+    dx = rstd * (gw - a - xh * c)
+    dx_e = rstd * (a_e + xh.abs() * c_e + xh_e * c.abs() + 8 * U * (gw.abs() + a.abs() + (xh * c).abs()))
+    want["dx"] = dx, R.half_step(dx, x.dtype) + dx_e
+    dw = (g * xh).sum(dims)
+    want["dw"] = dw, ((CHAIN + 4 * U) * (g * xh).abs() + g.abs() * xh_e).sum(dims) + R.half_step(dw, w.dtype)
+    db = g.sum(dims)
+    want["db"] = db, CHAIN * g.abs().sum(dims) + R.half_step(db, b.dtype)
+    R.check(got, want)
+
+
+@pytest.mark.parametrize("shape", [(2, 24, 5, 6, 7), (1, 24, 24, 60, 40), (2, 25, 9, 20, 21), (2, 24, 64, 128, 128)])
+@pytest.mark.parametrize("fmt", [None, "int8"])
+@pytest.mark.parametrize("dtype,centre,spread", [(HF, 1000.0, 2.0), (BF, 500.0, 4.0), (HF, -300.0, 0.25), (FP, 1000.0, 0.25)])
+def test_far_from_zero_gradients(cuda_ready, shape, fmt, dtype, centre, spread):
+    """|mean| hundreds of spreads, gradients of one sign: sum dz x and mean sum dz nearly cancel."""
+    c, kw = shape[1], dict(device="cuda", generator=_gen(11))
+    x = _last((centre + spread * torch.randn(shape, **kw)).to(dtype))
+    dy = _last((0.3 + 0.05 * torch.randn(shape, **kw)).to(dtype))
+    w, b = 1 + 0.2 * torch.randn(c, **kw), 0.2 * torch.randn(c, **kw)
+    _affine_check(x, c if c == 25 else 8, w, b, dy, fmt)
+
+
+@pytest.mark.parametrize("shape,groups", [((1, 2048, 7001), 2048), ((1, 2040, 6000), 255), ((1, 4104, 3000), 8)])
+@pytest.mark.parametrize("fmt", [None, "int8"])
+def test_widest_rows(cuda_ready, shape, groups, fmt):
+    """As many channels as a block has threads for, in two passes: the largest tables in shared memory."""
+    c, kw = shape[1], dict(device="cuda", generator=_gen(15))
+    x, dy = (_last(torch.randn(shape, **kw).to(BF)) for _ in range(2))
+    _affine_check(x, groups, 1 + 0.2 * torch.randn(c, **kw), 0.2 * torch.randn(c, **kw), dy, fmt)
