@@ -134,9 +134,9 @@ bool fused_pack(const Plan& pl, size_t elem) {
 size_t fwd_bytes(const Plan& pl) {
   return align_up((size_t)pl.g.samples * pl.sums_nb * pl.g.tiles * pl.g.G * sizeof(double2), 256);
 }
-size_t cpart_bytes(const Plan& pl) { return align_up((size_t)pl.g.samples * pl.sums_nb * pl.g.C * sizeof(float2), 256); }
+size_t cpart_bytes(const Plan& pl) { return align_up((size_t)pl.g.samples * pl.sums_nb * pl.g.C * sizeof(double2), 256); }
 size_t bwd_bytes(const Plan& pl) {
-  return cpart_bytes(pl) + align_up((size_t)pl.g.samples * pl.sums_nb * pl.g.tiles * pl.g.G * sizeof(float2), 256);
+  return cpart_bytes(pl) + align_up((size_t)pl.g.samples * pl.sums_nb * pl.g.tiles * pl.g.G * sizeof(double2), 256);
 }
 
 // Parameters as fp32 words of four: a thread's channels follow each other where a row is one voxel.
@@ -228,8 +228,8 @@ int r4c_gn_bwd(const r4c_gn_desc* desc, const void* dy, const void* x, int forma
   a.dx = dx;
   a.dgamma = dgamma;
   a.dbeta = dbeta;
-  a.cpart = static_cast<float2*>(ws);
-  a.gpart = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) + cpart_bytes(pl));
+  a.cpart = static_cast<double2*>(ws);
+  a.gpart = reinterpret_cast<double2*>(static_cast<uint8_t*>(ws) + cpart_bytes(pl));
   a.sums_nb = pl.sums_nb;
   pl.g.format = format;
   pl.g.wide_params = wide_params(pl.g, gamma, beta);

@@ -19,8 +19,8 @@
 // threads are cut into channel tiles.
 //
 // Sums: a thread keeps sum (x - p) and sum (x - p)^2 in fp32 around its own first value p, so nothing cancels where
-// |mean| >> std, and an outlier as p spoils one thread's few elements at most; threads, blocks and samples add in
-// fp64 about zero, in a fixed order: same bits on every run.
+// |mean| >> std, and an outlier as p spoils one thread's few elements at most; backward sum dz and sum dz (x - mean).
+// Threads, blocks and samples add in fp64, in a fixed order: same bits on every run.
 #pragma once
 
 #include <algorithm>
@@ -547,20 +547,15 @@ __device__ __forceinline__ double2 from_previous(const double2* p) {
   asm volatile("ld.global.v2.f64 {%0, %1}, [%2];" : "=d"(v.x), "=d"(v.y) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ float2 from_previous(const float2* p) {
-  float2 v;
-  asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
-  return v;
-}
 // Adds p[i * stride] for i = first, first + step, .. below end, in that order, U loads on their way at a time.
-template <int U, typename P>
-__device__ __forceinline__ void add_previous(const P* p, int64_t first, int64_t step, int64_t end, int64_t stride, double& a,
+template <int U>
+__device__ __forceinline__ void add_previous(const double2* p, int64_t first, int64_t step, int64_t end, int64_t stride, double& a,
                                              double& c) {
   for (int64_t i = first; i < end; i += U * step) {
-    P v[U];
+    double2 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      v[u].x = v[u].y = 0;
+      v[u] = make_double2(0.0, 0.0);
       if (i + u * step < end) v[u] = from_previous(p + (i + u * step) * stride);
     }
 #pragma unroll
@@ -911,18 +906,19 @@ __device__ __forceinline__ float2 grad_edge(const Geo& g, const T* __restrict__ 
 
 // The block's (sum dz, sum dz * (x - mean)) of a thread's columns: cpart gets them per channel (the second times rstd),
 // out(group, ..) the same times w, summed over the tile's channels of the group.
-// edge(element, channel, stat): an edge's dz and x - mean.
+// edge(element, channel, stat): an edge's dz and x - mean. A thread's sums are fp32, everything from there on is fp64:
+// sums that nearly vanish would be left with the roundings of the parts.
 template <int V, bool EDGES, typename Stat, typename Edge, typename Out>
 __device__ __forceinline__ void block_grads(const Geo& g, const Place& p, const float2 (&s1)[kPairs<V>],
                                             const float2 (&s2)[kPairs<V>], const void* gamma, float2* __restrict__ red,
-                                            float2* __restrict__ cols, float2* __restrict__ cpart, Stat stat, Edge edge,
+                                            double2* __restrict__ cols, double2* __restrict__ cpart, Stat stat, Edge edge,
                                             Out out) {
 #pragma unroll
   for (int k = 0; k < V; ++k)
     red[k * kThreads + threadIdx.x] = k & 1 ? make_float2(s1[k / 2].y, s2[k / 2].y) : make_float2(s1[k / 2].x, s2[k / 2].x);
   __syncthreads();
   const int nch = g.tiles == 1 ? g.C : p.j1 - p.j0;
-  each_sum<float>(nch, [&](int i, int sub, int tp, float& a, float& c) {
+  each_sum<double>(nch, [&](int i, int sub, int tp, double& a, double& c) {
     for (int j = i >= p.shift ? i - p.shift : i - p.shift + g.C; j < (g.tiles == 1 ? g.L : nch); j += g.C)
       for (int r = sub; r < g.R; r += tp) {
         const float2 v = red[(j % V) * kThreads + r * g.lanes + j / V];
@@ -934,25 +930,25 @@ __device__ __forceinline__ void block_grads(const Geo& g, const Place& p, const 
       Edges::of<V>(g, p).each_of(g, i, [&](int64_t at) {
         const float2 e = edge(at, i, s);
         a += e.x;
-        c = fmaf(e.x, e.y, c);
+        c = fma((double)e.x, (double)e.y, c);
       });
     }
-  }, [&](int i, float a, float c) {
+  }, [&](int i, double a, double c) {
     const int ch = p.j0 + i;
     const float2 m = stat((int)((unsigned)ch / (unsigned)g.Cg));
-    const float2 s = make_float2(a, c * m.y);
+    const double2 s = make_double2(a, c * m.y);
     cols[i] = s;
     cpart[(int64_t)blockIdx.x * g.C + ch] = s;
   });
   __syncthreads();
-  each_sum<float>(p.gb - p.ga, [&](int i, int sub, int tp, float& a, float& c) {
+  each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
     const int lo = max((p.ga + i) * g.Cg, p.j0), hi = min((p.ga + i + 1) * g.Cg, p.j0 + nch);
     for (int ch = lo + sub; ch < hi; ch += tp) {
-      const float w = param(gamma, g.pdtype, ch, 1.f);
-      a = fmaf(w, cols[ch - p.j0].x, a);
-      c = fmaf(w, cols[ch - p.j0].y, c);
+      const double w = param(gamma, g.pdtype, ch, 1.f);
+      a = fma(w, cols[ch - p.j0].x, a);
+      c = fma(w, cols[ch - p.j0].y, c);
     }
-  }, [&](int i, float a, float c) { out(p.ga + i, a, c); });
+  }, [&](int i, double a, double c) { out(p.ga + i, a, c); });
 }
 
 // cpart[(n * nb + b) * C + c] = (sum dz, sum dz * xh) of the block's rows, and
@@ -961,11 +957,11 @@ template <typename T, int V, int ACT, bool Q>
 __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_sums_kernel(
     const T* __restrict__ dy, const void* __restrict__ x, const uint8_t* __restrict__ exps,
     const float2* __restrict__ mean_rstd, const void* __restrict__ gamma, const void* __restrict__ beta,
-    const __grid_constant__ Geo g, float2* __restrict__ cpart, float2* __restrict__ gpart) {
+    const __grid_constant__ Geo g, double2* __restrict__ cpart, double2* __restrict__ gpart) {
   using R = Ring<T, V, Q, true, kBwdAhead>;
   constexpr int kTable = V * kThreads * (int)sizeof(float2);
   constexpr int kLoop = R::kBytes + (kSharedMeans<V> ? V * kThreads * (int)sizeof(float) : 0);
-  __shared__ __align__(16) char smem[kLoop > 2 * kTable ? kLoop : 2 * kTable];
+  __shared__ __align__(16) char smem[kLoop > 3 * kTable ? kLoop : 3 * kTable];
   let_next_start();
   const Place p = place<V>(g);
   R ring(smem, x, dy, exps, p.at, p.step);
@@ -1003,14 +999,14 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_sums_kernel(
   }
   ring.drain();
   __syncthreads();
-  float2* out = gpart + ((int64_t)blockIdx.x * g.tiles + p.tile) * g.G;
+  double2* out = gpart + ((int64_t)blockIdx.x * g.tiles + p.tile) * g.G;
   if (g.tiles > 1)
     for (int i = threadIdx.x; i < g.G; i += blockDim.x)
-      if (i < p.ga || i >= p.gb) out[i] = make_float2(0.f, 0.f);
-  block_grads<V, (ACT < 0)>(g, p, a1, a2, gamma, reinterpret_cast<float2*>(smem), reinterpret_cast<float2*>(smem + kTable), cpart,
+      if (i < p.ga || i >= p.gb) out[i] = make_double2(0.0, 0.0);
+  block_grads<V, (ACT < 0)>(g, p, a1, a2, gamma, reinterpret_cast<float2*>(smem), reinterpret_cast<double2*>(smem + kTable), cpart,
                  [&](int gi) { return stats[gi]; },
                  [&](int64_t at, int c, float2 s) { return grad_edge<T, ACT, Q>(g, dy, x, exps, gamma, beta, at, c, s); },
-                 [&](int gi, float a, float c) { out[gi] = make_float2(a, c); });
+                 [&](int gi, double a, double c) { out[gi] = make_double2(a, c); });
 }
 
 // ---------------------------------------------------------------------------
@@ -1018,7 +1014,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_sums_kernel(
 // ---------------------------------------------------------------------------
 // dw, db: a warp, or a block, sums a channel over the (sample, block) parts, in a fixed order.
 constexpr int64_t kWideParts = 2048;      // from here on a block a channel (70,000 parts of 16 channels: 160 -> 21 us)
-__device__ __forceinline__ void param_grads(const float2* cpart, int64_t parts, int C, int c,
+__device__ __forceinline__ void param_grads(const double2* cpart, int64_t parts, int C, int c,
                                             float* __restrict__ dgamma, float* __restrict__ dbeta) {
   const int lane = threadIdx.x & 31;
   double u = 0.0, v = 0.0;
@@ -1029,7 +1025,7 @@ __device__ __forceinline__ void param_grads(const float2* cpart, int64_t parts, 
     if (dgamma) dgamma[c] = (float)v;
   }
 }
-inline __global__ void __launch_bounds__(kThreads) params_kernel(const float2* cpart, int64_t parts, int C,
+inline __global__ void __launch_bounds__(kThreads) params_kernel(const double2* cpart, int64_t parts, int C,
                                                                  float* __restrict__ dgamma, float* __restrict__ dbeta) {
   __shared__ double2 warps[kThreads / 32];
   wait_for_previous();
@@ -1105,7 +1101,7 @@ template <typename T, int V, int ACT, bool Q>
 __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
     const T* __restrict__ dy, const void* __restrict__ x, const uint8_t* __restrict__ exps,
     const float2* __restrict__ mean_rstd, const void* __restrict__ gamma, const void* __restrict__ beta,
-    const __grid_constant__ Geo g, int64_t parts, const float2* cpart, const float2* gpart,
+    const __grid_constant__ Geo g, int64_t parts, const double2* cpart, const double2* gpart,
     T* __restrict__ dx, float* __restrict__ dgamma, float* __restrict__ dbeta) {
   using R = Ring<T, V, Q, true, kBwdAhead>;
   extern __shared__ __align__(16) char smem[];
@@ -1131,7 +1127,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) bwd_dx_kernel(
   k.params(g, p, gamma, beta);
   k.stats(g, p, [&](int gi) { return stats[gi]; });
   wait_for_previous();
-  const float2* src = gpart + p.n * g.np * g.G + p.ga;
+  const double2* src = gpart + p.n * g.np * g.G + p.ga;
   each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
     add_previous<4>(src + i, sub, tp, g.np, g.G, a, c);
   }, [&](int i, double a, double c) { coef[i] = coef_of(g, stats[p.ga + i], a, c); });
@@ -1214,9 +1210,9 @@ constexpr int small_fwd_bytes(int vectors) {
          kSmallGroups * (int)(sizeof(double2) + sizeof(float2));
 }
 template <typename T, int V, bool Q>
-constexpr int small_bwd_bytes(int vectors) {
-  return vectors * kThreads * V * ((Q ? 1 : (int)sizeof(T)) + (int)sizeof(T)) + 2 * V * kThreads * (int)sizeof(float2) +
-         kSmallGroups * (int)(sizeof(double2) + sizeof(float2));
+constexpr int small_bwd_bytes(int vectors, int lanes) {
+  return vectors * kThreads * V * ((Q ? 1 : (int)sizeof(T)) + (int)sizeof(T)) + V * kThreads * (int)sizeof(float2) +
+         V * lanes * (int)sizeof(double2) + kSmallGroups * (int)(sizeof(double2) + sizeof(float2));
 }
 
 template <typename T, int V, int ACT, bool PACK>
@@ -1267,14 +1263,14 @@ template <typename T, int V, int ACT, bool Q>
 __global__ void __launch_bounds__(kThreads)
     bwd_small_kernel(const T* __restrict__ dy, const void* __restrict__ x, const uint8_t* __restrict__ exps,
                      const float2* __restrict__ mean_rstd, const void* __restrict__ gamma,
-                     const void* __restrict__ beta, const __grid_constant__ Geo g, float2* __restrict__ cpart,
+                     const void* __restrict__ beta, const __grid_constant__ Geo g, double2* __restrict__ cpart,
                      T* __restrict__ dx) {
   constexpr int XB = V * (Q ? 1 : (int)sizeof(T)), YB = V * (int)sizeof(T);
   extern __shared__ __align__(16) char smem[];
   char* dys = smem + g.small * kThreads * XB;
   float2* red = reinterpret_cast<float2*>(dys + g.small * kThreads * YB);
-  float2* cols = red + V * kThreads;
-  double2* mine = reinterpret_cast<double2*>(cols + V * kThreads);
+  double2* cols = reinterpret_cast<double2*>(red + V * kThreads);
+  double2* mine = cols + V * g.lanes;
   float2* coef = reinterpret_cast<float2*>(mine + kSmallGroups);
   let_next_start();
   const Place p = place<V>(g);
@@ -1317,7 +1313,7 @@ __global__ void __launch_bounds__(kThreads)
   }
   block_grads<V, (ACT < 0)>(g, p, s1, s2, gamma, red, cols, cpart, [&](int gi) { return stats[gi]; },
                  [&](int64_t at, int c, float2 s) { return grad_edge<T, ACT, Q>(g, dy, x, exps, gamma, beta, at, c, s); },
-                 [&](int gi, float a, float c) { mine[gi - p.ga] = make_double2(a, c); });
+                 [&](int gi, double a, double c) { mine[gi - p.ga] = make_double2(a, c); });
   cluster_sums(g, groups, mine, [&](int i, double a, double c) { coef[i] = coef_of(g, stats[p.ga + i], a, c); });
   if (p.mine > 0) {
     float2 k1[kPairs<V>], k2[kPairs<V>];
@@ -1351,7 +1347,7 @@ struct BwdArgs {
   const float2* mean_rstd;
   void* dx;                 // null: not wanted
   float *dgamma, *dbeta;    // null: not wanted
-  float2 *cpart, *gpart;
+  double2 *cpart, *gpart;
   int sums_nb;              // blocks a sample of the sums
 };
 

@@ -67,10 +67,10 @@ template <typename T, int V, int ACT, bool Q>
 cudaError_t bwd_small(const BwdArgs& a, const Geo& g, int threads, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
   auto kernel = bwd_small_kernel<T, V, ACT, Q>;
-  const cudaError_t e = allow_shared(kernel, small_bwd_bytes<T, V, Q>(kSmallBwd), allowed);
+  const cudaError_t e = allow_shared(kernel, small_bwd_bytes<T, V, Q>(kSmallBwd, kThreads), allowed);
   if (e != cudaSuccess) return e;
   note_launches(1);
-  return launch_cluster(g.nb, kernel, dim3((unsigned)g.blocks, g.tiles), threads, small_bwd_bytes<T, V, Q>(g.small), s,
+  return launch_cluster(g.nb, kernel, dim3((unsigned)g.blocks, g.tiles), threads, small_bwd_bytes<T, V, Q>(g.small, g.lanes), s,
                         static_cast<const T*>(a.dy), a.x, a.exps, a.mean_rstd, a.gamma, a.beta, g, a.cpart,
                         static_cast<T*>(a.dx));
 }

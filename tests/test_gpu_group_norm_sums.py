@@ -82,3 +82,27 @@ def test_widest_rows(cuda_ready, shape, groups, fmt):
     c, kw = shape[1], dict(device="cuda", generator=_gen(15))
     x, dy = (_last(torch.randn(shape, **kw).to(BF)) for _ in range(2))
     _affine_check(x, groups, 1 + 0.2 * torch.randn(c, **kw), 0.2 * torch.randn(c, **kw), dy, fmt)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("places", [(0, 1, 3), (0, 2, 3), (1, 2, 3), (0, 1, 2)])
+@pytest.mark.parametrize("voxels", [4, 20000])
+def test_sums_of_threads_in_64_bits(cuda_ready, dtype, places, voxels):
+    """db = 2^30 + 1 - 2^30, dw likewise, from voxels of different threads (the rest 0, and xh = 1 in them)."""
+    c = 8
+    x = torch.zeros(1, voxels, c, device="cuda")
+    x[:, ::2], x[:, 1::2] = 1.0, -1.0                    # mean 0, rstd 1 (eps 0)
+    x[:, :4] = torch.tensor([1.0, -1.0, 1.0, -1.0], device="cuda").reshape(4, 1)
+    at = [p * voxels // 4 for p in places]
+    dy = torch.zeros(1, voxels, c, device="cuda")
+    sign = x[0, :, 0].clone()
+    for i, v in zip(at, (2.0 ** 30, 1.0, -2.0 ** 30)):
+        dy[0, i] = v
+    x, dy = (t.to(dtype).movedim(-1, 1) for t in (x, dy))
+    w = torch.ones(c, device="cuda", requires_grad=True)
+    b = torch.zeros(c, device="cuda", requires_grad=True)
+    y = group_norm_act(x, 1, w, b, 0.0)
+    _, db = torch.autograd.grad(y, (w, b), dy, retain_graph=True)
+    assert bool((db == 1.0).all())
+    dw, _ = torch.autograd.grad(y, (w, b), dy * sign.to(dtype))
+    assert bool((dw == 1.0).all())
