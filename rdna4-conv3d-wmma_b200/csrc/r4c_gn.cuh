@@ -664,32 +664,42 @@ struct Moments {
       s2[k] = __ffma2_rn(d, d, s2[k]);
     }
   }
-  // (sum x, sum x^2) of column k in fp64
-  __device__ __forceinline__ double2 sums(int k) const {
-    const double q = -(double)(k & 1 ? np[k / 2].y : np[k / 2].x), a = k & 1 ? s1[k / 2].y : s1[k / 2].x;
+  // (sum x - o, sum (x - o)^2) of column k in fp64
+  __device__ __forceinline__ double2 sums(int k, double o) const {
+    const double q = -(double)(k & 1 ? np[k / 2].y : np[k / 2].x) - o, a = k & 1 ? s1[k / 2].y : s1[k / 2].x;
     const double s = k & 1 ? s2[k / 2].y : s2[k / 2].x, c = count;
     return make_double2(c * q + a, s + 2.0 * q * a + c * q * q);
   }
 };
 
-// The block's sums of each of its groups: out(group, sum x, sum x^2).
-template <typename T, int V, typename Out>
+// A group's origin in a sample: its first element. Sums are joined about it, so that fp64 keeps a variance far below
+// mean^2 (about zero, a group that is 30000 throughout had one of some 1e-7 instead of 0, against an eps of 1e-5).
+template <typename T>
+__device__ __forceinline__ float origin(const Geo& g, const Place& p, const T* __restrict__ x, int gi) {
+  return Elem<T>::to_f(x[p.n * g.sample + (int64_t)gi * g.Cg]);
+}
+
+// The block's sums of each of its groups: out(group, sum x - o, sum (x - o)^2), o = origin_of(group of the tile).
+template <typename T, int V, typename Origin, typename Out>
 __device__ __forceinline__ void block_moments(const Geo& g, const Place& p, const Moments<T, V>& m,
-                                              const T* __restrict__ x, double2* __restrict__ red, Out out) {
+                                              const T* __restrict__ x, double2* __restrict__ red, Origin origin_of,
+                                              Out out) {
   // a thread whose columns all belong to one group adds them first
   const bool merged = V > 1 && g.L == g.C && (g.Cg & (V - 1)) == 0;
-  if (merged) {
-    double2 t = m.sums(0);
+  if (p.active) {
+    if (merged) {
+      const double o = origin_of(p.gi - p.ga);
+      double2 t = m.sums(0, o);
 #pragma unroll
-    for (int k = 1; k < V; ++k) {
-      const double2 v = m.sums(k);
-      t.x += v.x;
-      t.y += v.y;
+      for (int k = 1; k < V; ++k) {
+        const double2 v = m.sums(k, o);
+        t.x += v.x;
+        t.y += v.y;
+      }
+      red[threadIdx.x] = t;
+    } else {
+      each_column<V>(g, p, [&](int k, int, int gi) { red[k * kThreads + threadIdx.x] = m.sums(k, origin_of(gi - p.ga)); });
     }
-    red[threadIdx.x] = t;
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k) red[k * kThreads + threadIdx.x] = m.sums(k);
   }
   __syncthreads();
   const int tp = threads_per(p.gb - p.ga, blockDim.x), tr = row_threads(tp, g.R), tc = tp / tr;
@@ -720,9 +730,10 @@ __device__ __forceinline__ void block_moments(const Geo& g, const Place& p, cons
     }
     if (g.edges && p.b == 0) {
       const Edges e = Edges::of<V>(g, p);
+      const double o = origin_of(i);
       for (int ch = lo + sub; ch < hi; ch += tp)
         e.each_of(g, ch, [&](int64_t at) {
-          const double v = Elem<T>::to_f(x[at]);
+          const double v = Elem<T>::to_f(x[at]) - o;
           a += v;
           c += v * v;
         });
@@ -730,11 +741,11 @@ __device__ __forceinline__ void block_moments(const Geo& g, const Place& p, cons
   }, [&](int i, double a, double c) { out(p.ga + i, a, c); });
 }
 
-// (var + eps)^-1/2 from the fp32 reciprocal root and one step of Newton's method in fp64 (2^-22 becomes 2^-43; an fp64
+// Mean and rstd from the sums about the group's origin; (var + eps)^-1/2 from the fp32 reciprocal root and one step of Newton's method in fp64 (2^-22 becomes 2^-43; an fp64
 // root and division would be a hundred instructions in a row).
-__device__ __forceinline__ float2 mean_rstd_of(const Geo& g, double a, double c) {
-  const double mean = a * g.inv_m;
-  double var = c * g.inv_m - mean * mean;
+__device__ __forceinline__ float2 mean_rstd_of(const Geo& g, double a, double c, double o) {
+  const double from_o = a * g.inv_m, mean = o + from_o;
+  double var = c * g.inv_m - from_o * from_o;
   if (var < 0.0) var = 0.0;
   const double v = var + (double)g.eps;
   const float f = (float)v, r0 = rsqrtf(f);
@@ -743,18 +754,20 @@ __device__ __forceinline__ float2 mean_rstd_of(const Geo& g, double a, double c)
   return make_float2((float)mean, (float)(r * (1.5 - 0.5 * v * r * r)));
 }
 
-// part[((n * nb + b) * tiles + tile) * G + g] = (sum x, sum x^2) of the block's share of group g.
+// part[((n * nb + b) * tiles + tile) * G + g] = (sum x - o, sum (x - o)^2) of the block's share of group g.
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, kStatsBlocks) stats_kernel(const T* __restrict__ x,
                                                                        const __grid_constant__ Geo g,
                                                                        double2* __restrict__ part) {
   using R = Ring<T, V, false, false, kFwdAhead>;
   __shared__ __align__(16) char smem[R::kBytes > V * kThreads * 16 ? R::kBytes : V * kThreads * 16];
+  __shared__ float origins[V * kThreads];     // of the tile's groups, no more than its columns
   let_next_start();
   const Place p = place<V>(g);
   R ring(smem, x, nullptr, nullptr, p.at, p.step);
 #pragma unroll
   for (int i = 0; i < kFwdAhead - 1; ++i) ring.start(i, i < p.mine);
+  for (int i = threadIdx.x; i < p.gb - p.ga; i += blockDim.x) origins[i] = origin(g, p, x, p.ga + i);
   Moments<T, V> m;
   m.zero();
   if (p.mine > 0) {
@@ -780,7 +793,8 @@ __global__ void __launch_bounds__(kThreads, kStatsBlocks) stats_kernel(const T* 
   if (g.tiles > 1)
     for (int i = threadIdx.x; i < g.G; i += blockDim.x)
       if (i < p.ga || i >= p.gb) out[i] = make_double2(0.0, 0.0);
-  block_moments<T, V>(g, p, m, x, reinterpret_cast<double2*>(smem), [&](int gi, double a, double c) { out[gi] = make_double2(a, c); });
+  block_moments<T, V>(g, p, m, x, reinterpret_cast<double2*>(smem), [&](int i) { return origins[i]; },
+                      [&](int gi, double a, double c) { out[gi] = make_double2(a, c); });
 }
 
 // y of one vector at element `at`, into `to`, and its 8 bits (PACK: a block of 32 elements lies in 32 / V neighbouring
@@ -843,11 +857,13 @@ __global__ void __launch_bounds__(kThreads, kApplyBlocks) apply_kernel(
   for (int i = 0; i < kFwdAhead - 1; ++i) ring.start(i, i >= skip && i < p.tiles);
   Affine<T, V> k;
   k.params(g, p, gamma, beta);
+  for (int i = threadIdx.x; i < p.gb - p.ga; i += blockDim.x) stat[i].x = origin(g, p, x, p.ga + i);
+  __syncthreads();
   wait_for_previous();
   const double2* src = part + p.n * g.np * g.G + p.ga;
   each_sum<double>(p.gb - p.ga, [&](int i, int sub, int tp, double& a, double& c) {
     add_previous<4>(src + i, sub, tp, g.np, g.G, a, c);
-  }, [&](int i, double a, double c) { stat[i] = mean_rstd_of(g, a, c); });
+  }, [&](int i, double a, double c) { stat[i] = mean_rstd_of(g, a, c, stat[i].x); });
   __syncthreads();
   if (p.b == 0)
     for (int i = threadIdx.x; i < p.gb - p.ga; i += blockDim.x) mean_rstd[p.n * g.G + p.ga + i] = stat[i];
@@ -1231,6 +1247,7 @@ __global__ void __launch_bounds__(kThreads) fwd_small_kernel(const T* __restrict
   const int groups = p.gb - p.ga;
   const char* own = smem + threadIdx.x * B;
   for (int t = 0; t < p.mine; ++t) copy_async<B>(shared_at(own) + t * kThreads * B, x + p.at + t * p.step);
+  for (int i = threadIdx.x; i < groups; i += blockDim.x) stat[i].x = origin(g, p, x, p.ga + i);
   Affine<T, V> k;
   k.params(g, p, gamma, beta);
   asm volatile("cp.async.wait_all;" ::: "memory");
@@ -1243,8 +1260,10 @@ __global__ void __launch_bounds__(kThreads) fwd_small_kernel(const T* __restrict
     if (t == 0) m.pivot(v);
     m.add(v);
   }
-  block_moments<T, V>(g, p, m, x, red, [&](int gi, double a, double c) { mine[gi - p.ga] = make_double2(a, c); });
-  cluster_sums(g, groups, mine, [&](int i, double a, double c) { stat[i] = mean_rstd_of(g, a, c); });
+  __syncthreads();
+  block_moments<T, V>(g, p, m, x, red, [&](int i) { return stat[i].x; },
+                      [&](int gi, double a, double c) { mine[gi - p.ga] = make_double2(a, c); });
+  cluster_sums(g, groups, mine, [&](int i, double a, double c) { stat[i] = mean_rstd_of(g, a, c, stat[i].x); });
   if (p.b == 0)
     for (int i = threadIdx.x; i < groups; i += blockDim.x) mean_rstd[p.n * g.G + p.ga + i] = stat[i];
   k.stats(g, p, [&](int gi) { return stat[gi - p.ga]; });

@@ -106,3 +106,50 @@ def test_sums_of_threads_in_64_bits(cuda_ready, dtype, places, voxels):
     assert bool((db == 1.0).all())
     dw, _ = torch.autograd.grad(y, (w, b), dy * sign.to(dtype))
     assert bool((dw == 1.0).all())
+
+
+@pytest.mark.parametrize("shape,groups", [((2, 24, 5, 6, 7), 8), ((1, 24, 24, 60, 40), 8), ((2, 25, 9, 20, 21), 5)])
+@pytest.mark.parametrize("dtype,value", [(BF, 100.0), (HF, 30000.0), (HF, 1000.0), (FP, 30000.0), (FP, 1e6), (FP, 0.1)])
+def test_constant_far_from_zero(cuda_ready, shape, groups, dtype, value):
+    """A background of one value: the variance is 0 however large the value, y is the bias, dx = (dz w - A) / sqrt(eps)."""
+    c, kw = shape[1], dict(device="cuda", generator=_gen(12))
+    x = _last(torch.full(shape, value, device="cuda").to(dtype))
+    dy = _last((torch.randn(shape, **kw) / 64).to(dtype))
+    w, b = 1 + 0.2 * torch.randn(c, **kw), 0.2 * torch.randn(c, **kw)
+    _affine_check(x, groups, w, b, dy)
+    y = group_norm_act(x, groups, w, b)
+    assert torch.equal(y, b.to(dtype).reshape(1, c, 1, 1, 1).expand(shape))
+
+
+@pytest.mark.parametrize("shape,groups", [((2, 24, 16, 32, 32), 8), ((2, 24, 64, 64, 64), 8)])
+@pytest.mark.parametrize("dtype,value,step", [(FP, 30000.0, 0.03125), (BF, 100.0, 0.5), (HF, 1000.0, 0.5)])
+def test_one_voxel_apart(cuda_ready, shape, groups, dtype, value, step):
+    """A group that is one value but for one voxel, and one whose first element is that voxel."""
+    c, kw = shape[1], dict(device="cuda", generator=_gen(13))
+    x = torch.full(shape, value, device="cuda")
+    x[0, ::3, 3, 4, 5] += step
+    x[1, ::3, 0, 0, 0] += step
+    dy = _last((torch.randn(shape, **kw) / 64).to(dtype))
+    w, b = 1 + 0.2 * torch.randn(c, **kw), 0.2 * torch.randn(c, **kw)
+    _affine_check(_last(x.to(dtype)), groups, w, b, dy)
+
+
+@pytest.mark.parametrize("shape", [(2, 24, 5, 6, 7), (2, 24, 40, 64, 64)])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_a_bad_first_element_stays_in_its_group(cuda_ready, shape, bad):
+    """What a group's sums are taken about."""
+    kw = dict(device="cuda", generator=_gen(16))
+    x, dy = (_last(torch.randn(shape, **kw).to(BF)) for _ in range(2))
+
+    def run(x):
+        x = x.detach().requires_grad_(True)
+        y = group_norm_act(x, 8, activation="silu")
+        return y.detach(), torch.autograd.grad(y, x, dy)[0]
+
+    clean = run(x)
+    x[1, 6, 0, 0, 0] = bad
+    for got, want in zip(run(x), clean):
+        got, want = got.unflatten(1, (8, 3)), want.unflatten(1, (8, 3))
+        assert bool(got[1, 2].isnan().all())
+        got[1, 2] = want[1, 2]
+        assert torch.equal(got, want)
