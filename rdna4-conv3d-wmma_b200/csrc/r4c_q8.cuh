@@ -94,18 +94,19 @@ __device__ __forceinline__ Codes<V> encode(const float (&f)[V], int byte, int fo
   return c;
 }
 
-// Bytes below / above which a value may need T's rounding / T's largest number.
+// Bytes below / above which a value may need T's rounding / T's largest number. (fp16's smallest step is 2^-24, a whole
+// number's 2^e, an e4m3 code's 2^(e-9). Codes of an fp16 tensor are multiples of its step all the same; others' may not be.)
 template <typename T> struct Limits;
 template <> struct Limits<__half> {
-  static constexpr int low = 103, high_int8 = 136, high_e4m3 = 134;
+  static constexpr int low_int8 = 103, low_e4m3 = 112, high_int8 = 136, high_e4m3 = 134;
   static __device__ __forceinline__ float most() { return 65504.f; }
 };
 template <> struct Limits<__nv_bfloat16> {
-  static constexpr int low = -1, high_int8 = 248, high_e4m3 = 246;
+  static constexpr int low_int8 = -1, low_e4m3 = -1, high_int8 = 248, high_e4m3 = 246;
   static __device__ __forceinline__ float most() { return __uint_as_float(0x7f7f0000u); }
 };
 template <> struct Limits<float> {
-  static constexpr int low = -1, high_int8 = 248, high_e4m3 = 246;
+  static constexpr int low_int8 = -1, low_e4m3 = -1, high_int8 = 248, high_e4m3 = 246;
   static __device__ __forceinline__ float most() { return __uint_as_float(0x7f7fffffu); }
 };
 
@@ -113,7 +114,7 @@ template <> struct Limits<float> {
 template <typename T, int V>
 __device__ __forceinline__ void decode(const Codes<V>& c, int byte, int format, float (&f)[V]) {
   const float s = scale(byte);
-  bool rare = byte < Limits<T>::low;                          // T's rounding, its largest number, NaN
+  bool rare = byte < (format == R4C_Q8_INT8 ? Limits<T>::low_int8 : Limits<T>::low_e4m3);   // T's rounding, its largest number, NaN
   if (format == R4C_Q8_INT8) {
     // 0x4b0000uu is 2^23 + u exactly: the signed code is that minus 2^23 + 128 (no integer-to-float conversions,
     // which share a slow pipe). Times 2^e it is exact either way round: one multiply-add a value, while

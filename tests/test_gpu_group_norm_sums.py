@@ -8,6 +8,8 @@ import pytest
 import torch
 
 import gn_refs as R
+from rdna4_conv3d import _native
+from rdna4_conv3d.checkpoint8 import Packed8, unpack8
 from rdna4_conv3d.group_norm import group_norm_act
 
 pytestmark = pytest.mark.gpu
@@ -153,3 +155,28 @@ def test_a_bad_first_element_stays_in_its_group(cuda_ready, shape, bad):
         assert bool(got[1, 2].isnan().all())
         got[1, 2] = want[1, 2]
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("shape", [(1, 16, 40), (1, 8, 3, 4, 5), (1, 16, 8, 64, 64), (1, 25, 9, 10)])
+def test_codes_are_read_in_the_activations_type(cuda_ready, shape):
+    """fp16 values below 2^-14 that have a fraction of its smallest step: the backward takes them rounded, as unpack8 does."""
+    c, count = shape[1], torch.Size(shape).numel()
+    kw = dict(device="cuda", generator=_gen(14))
+    plan = _native.gn_plan(torch.Size(shape), 1, HF, FP, 1e-5, 0, 0.0)
+    codes = torch.randint(0, 256, (count,), dtype=torch.uint8, **kw)
+    codes[(codes & 0x7f) == 0x7f] = 0x11                 # (no NaN)
+    exps = torch.randint(96, 120, (-(-count // 32),), dtype=torch.uint8, **kw)
+    q8 = torch.zeros(plan.q8_bytes, dtype=torch.uint8, device="cuda")
+    q8[:count] = codes
+    q8[plan.q8_at:plan.q8_at + exps.numel()] = exps
+    last = torch.Size((shape[0], *shape[2:], c))
+    x = unpack8(Packed8(codes, exps, last, torch.empty(last).stride(), HF, "e4m3")).movedim(-1, 1)
+    assert bool(x.isfinite().all())
+    dy = _last(torch.randn(shape, **kw).to(HF))
+    stats = torch.zeros(plan.kept, device="cuda")
+    stats[:2] = torch.tensor([0.0, 2.0 ** 16], device="cuda")
+    w, b = torch.ones(c, device="cuda"), torch.zeros(c, device="cuda")
+    want = _native.gn_backward(dy, plan, x, None, stats, w, b, True, True)
+    got = _native.gn_backward(dy, plan, q8, 1, stats, w, b, True, True)
+    for g, v in zip(got, want):
+        assert torch.equal(g, v)
