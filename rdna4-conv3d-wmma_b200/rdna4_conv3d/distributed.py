@@ -602,7 +602,8 @@ class _ShardedGroupNormFn(torch.autograd.Function):
         ctx.save_for_backward(x, mean, rstd, total, weight, bias)
         ctx.args = groups, activation, slope, group
         z, _ = _ShardedGroupNormFn._z(x, mean, rstd, weight, bias, groups)
-        return _act_torch(z, activation, slope).to(x.dtype)
+        # a tensor of its own, in x's layout: a view from in here could not be changed in place
+        return torch.empty_like(x).copy_(_act_torch(z, activation, slope))
 
     @staticmethod
     def _z(x, mean, rstd, weight, bias, groups):

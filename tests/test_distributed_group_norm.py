@@ -188,3 +188,22 @@ def test_statistics_far_from_zero():
         y, dx = (torch.cat([r[i][k] for r in res], dim=2) for k in (0, 1))
         # 16: a few products, and torch's blocked sums of 15 to 30 elements
         _check_far(value, dtype, y, dx, 16)
+
+
+@pytest.mark.parametrize("affine", [True, False])
+@pytest.mark.parametrize("last", [True, False])
+def test_an_in_place_activation_may_follow(alone, affine, last):
+    """As behind a stock norm; the result lies as the input does."""
+    from rdna4_conv3d.distributed import depth_shard_model
+    net = nn.Sequential(nn.GroupNorm(2, 8, affine=affine), nn.ReLU(inplace=True)).double()
+    x = torch.randn(2, 8, 2, 3, 4, dtype=torch.float64, generator=torch.Generator().manual_seed(1))
+    if last:
+        x = x.contiguous(memory_format=torch.channels_last_3d)
+    x.requires_grad_(True)
+    want = net(x)
+    gx, = torch.autograd.grad((want ** 2).sum(), x)
+    depth_shard_model(net)
+    y = net(x)
+    assert y.stride() == x.stride()
+    torch.testing.assert_close(y, want, rtol=1e-10, atol=1e-10)
+    torch.testing.assert_close(torch.autograd.grad((y ** 2).sum(), x)[0], gx, rtol=1e-10, atol=1e-10)
