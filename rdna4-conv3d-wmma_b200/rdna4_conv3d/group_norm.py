@@ -242,7 +242,9 @@ class _KeptTorchFn(torch.autograd.Function):
         codes, exps = _pack_torch(x.movedim(1, -1).contiguous(), checkpoint)
         ctx.save_for_backward(codes, exps, mean, rstd, weight, bias)
         ctx.args = x.shape, x.dtype, groups, activation, slope, checkpoint
-        return _group_norm_torch(x, groups, weight, bias, eps, activation, slope, None)
+        y = _group_norm_torch(x, groups, weight, bias, eps, activation, slope, None)
+        # (a tensor of its own: a view from in here could not be changed in place)
+        return torch.empty_strided(y.shape, y.stride(), dtype=y.dtype, device=y.device).copy_(y)
 
     @staticmethod
     def backward(ctx, gy):

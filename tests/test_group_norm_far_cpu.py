@@ -32,3 +32,16 @@ def test_one_value_far_from_zero(shape, groups, value, step, fmt):
         e = U * abs(value) * rstd
         bound = bound + rstd * 2 * e * (e * g.abs().mean(-1, keepdim=True))
         assert bool(((dx.double().reshape(want.shape) - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("fmt", [None, "int8", "e4m3"])
+@pytest.mark.parametrize("shape", [(2, 24, 3, 4, 5), (2, 24, 7), (2, 24)])
+def test_an_in_place_activation_may_follow(shape, fmt):
+    """As on a CUDA device: the result is no view of something inside."""
+    x = torch.randn(shape, generator=torch.Generator().manual_seed(5)).requires_grad_(True)
+    y = group_norm_act(x, 3, checkpoint=fmt)
+    want = torch.relu(y)
+    gx, = torch.autograd.grad((want ** 2).sum(), x)
+    y = torch.relu_(group_norm_act(x, 3, checkpoint=fmt))
+    assert torch.equal(y, want) and y.movedim(1, -1).is_contiguous()
+    assert torch.equal(torch.autograd.grad((y ** 2).sum(), x)[0], gx)
