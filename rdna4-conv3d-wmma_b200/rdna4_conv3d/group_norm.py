@@ -171,6 +171,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
         if t is not None:
             refuse_blind(t)
     code = _native.ACTIVATIONS[activation]
+    eps, negative_slope = float(eps), float(negative_slope)      # (plans are kept by them)
     x = _channels_last(x)
     needs = x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad
     if torch.is_grad_enabled() and needs or torch._C._is_tracing():
