@@ -9,8 +9,9 @@
 //   dx = rstd * (dz * w - A - xh * B)
 // Two passes over the data each way: sums, then the element-wise result (the statistics of a group need all of it).
 // Both are bound by memory: forward 3, backward 5 activations read or written. Samples that fit the shared memory
-// of a cluster take one. [4,24,64,128,128] bf16 with silu (201 MB): forward 107 us (5.6 TB/s), backward 171 us (5.9
-// TB/s), with relu 100 us forward (6.1 TB/s); with x in 8 bits too 133 and 174 us, where instructions (150 to 190 a warp and vector) are the bound.
+// of a cluster take one. [4,24,64,128,128] bf16 with silu (201 MB): forward 108 us (5.6 TB/s), backward 173 us (5.8
+// TB/s), with relu 100 us forward (6.0 TB/s); with x in 8 bits too 132 and 193 us, where neither the memory (3.3 to 4.0
+// TB/s) nor the issue slots (60 to 65 %, 160 to 190 instructions a warp and vector) are full.
 //
 // A thread owns a vector of V neighbouring elements in every R-th row of its block's range, so its channels and with
 // them the parameters stay in registers. A row is a voxel's channels, or L / C voxels together where C is no multiple
@@ -762,8 +763,8 @@ __device__ __forceinline__ void block_moments(const Geo& g, const Place& p, cons
   }, [&](int i, double a, double c) { out(p.ga + i, a, c); });
 }
 
-// Mean and rstd from the sums about the group's origin; (var + eps)^-1/2 from the fp32 reciprocal root and one step of Newton's method in fp64 (2^-22 becomes 2^-43; an fp64
-// root and division would be a hundred instructions in a row).
+// Mean and rstd from the sums about the group's origin; (var + eps)^-1/2 from the fp32 reciprocal root and one step of
+// Newton's method in fp64 (2^-22 becomes 2^-43; an fp64 root and division would be a hundred instructions in a row).
 __device__ __forceinline__ float2 mean_rstd_of(const Geo& g, double a, double c, double o) {
   const double from_o = a * g.inv_m, mean = o + from_o;
   double var = c * g.inv_m - from_o * from_o;

@@ -6,7 +6,8 @@ innermost, as every convolution of this package writes them: two native
 passes forward and two backward (r4c_gn_*; one launch each way for small
 activations), where stock PyTorch copies them to channels first, normalises,
 copies back and applies the activation on its own. bf16, fp16 or fp32 in and
-out, fp32 arithmetic, fp64 sums in a fixed order (same bits on every run).
+out, fp32 arithmetic on x - mean; a thread's sums in fp32, all others in fp64
+and in a fixed order (same bits on every run).
 
 ``checkpoint='int8'`` or ``'e4m3'`` keeps x for the backward pass in 8 bits
 (``checkpoint8``): the forward writes them beside y, the backward kernels read
