@@ -588,7 +588,7 @@ class _ShardedGroupNormFn(torch.autograd.Function):
         xg = x.double().reshape(n, groups, -1)
         # every rank's (count, mean, sum of squares about it), joined by Chan's rule: sums of x^2 would cancel where
         # |mean| >> spread
-        mean = xg.mean(-1)
+        mean = xg.sum(-1) / max(1, xg.shape[-1])          # (a slab may be empty)
         own = torch.stack([torch.full_like(mean, xg.shape[-1]), mean, ((xg - mean.unsqueeze(-1)) ** 2).sum(-1)])
         parts = [torch.empty_like(own) for _ in range(dist.get_world_size(group))]
         dist.all_gather(parts, own, group=group)

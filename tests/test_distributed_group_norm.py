@@ -207,3 +207,38 @@ def test_an_in_place_activation_may_follow(alone, affine, last):
     assert y.stride() == x.stride()
     torch.testing.assert_close(y, want, rtol=1e-10, atol=1e-10)
     torch.testing.assert_close(torch.autograd.grad((y ** 2).sum(), x)[0], gx, rtol=1e-10, atol=1e-10)
+
+
+def _worker_uneven(rank, port, outdir):
+    from rdna4_conv3d.distributed import DepthShardedGroupNormAct3d
+    _init(rank, port)
+    try:
+        out = []
+        for cut in (0, 1, 4):                            # planes of the first rank: none, one, all
+            x, dy = (t[:, :, :cut] if rank == 0 else t[:, :, cut:] for t in _far(3.0, torch.float64))
+            x = x.contiguous().requires_grad_(True)
+            norm = DepthShardedGroupNormAct3d(4, 8, activation="silu").double()
+            y = norm(x)
+            y.backward(dy)
+            out.append((y.detach(), x.grad, norm.weight.grad, norm.bias.grad))
+        torch.save(out, os.path.join(outdir, f"r{rank}.pt"))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_slabs_of_any_depth():
+    """A rank without a plane of its own takes part all the same."""
+    from rdna4_conv3d.group_norm import GroupNormAct3d
+    res = _run(_worker_uneven)
+    x, dy = _far(3.0, torch.float64)
+    norm = GroupNormAct3d(4, 8, activation="silu").double()
+    x.requires_grad_(True)
+    y = norm(x)
+    y.backward(dy)
+    kw = dict(rtol=1e-9, atol=1e-9)
+    for i in range(3):
+        torch.testing.assert_close(torch.cat([r[i][0] for r in res], dim=2), y.detach(), **kw)
+        torch.testing.assert_close(torch.cat([r[i][1] for r in res], dim=2), x.grad, **kw)
+        for r in res:
+            torch.testing.assert_close(r[i][2], norm.weight.grad, **kw)
+            torch.testing.assert_close(r[i][3], norm.bias.grad, **kw)
